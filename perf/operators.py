@@ -1,0 +1,560 @@
+"""The incremental operators as timed cases, each beside its plain form.
+
+  rotary    fused_rotary: rotary positions of q and k, forward or gradient
+  append    PagedCache.append: new tokens' k (rotated) and v into cache pages,
+            the rotated q beside them
+  attend    PagedCache.attention: a chunk of new tokens per sequence over the
+            pages of its whole context
+  branch    PagedCache.fork, reserve and free: continuations of a prefix
+            opened, grown by some tokens and dropped
+  compact   PagedCache.compact: live pages moved to the front of the pool
+
+Where `own` is false run() computes the operator in elementary torch operations
+in 32 bits (64 for angles); where it is true it makes the package's calls.
+exact() restates each from its definition in 64 bits, a sequence at a time.
+"""
+import importlib
+import math
+
+import numpy as np
+import torch
+
+own = False
+DEV = "cuda"
+BF16, F32 = torch.bfloat16, torch.float32
+TYPES = {"bf16": BF16, "f32": F32}
+THETA = 10000.0
+LAYERS = 14  # of the entropy model
+
+
+def listed():
+    return [
+        # q and k of a full [16, 8192] batch of the entropy model (12 heads of 64)
+        dict(name="rotary_batch", kind="rotary", batch=16, seq=8192, heads=12, kv_heads=12, dim=64,
+             rot=64, pairs="half", dtype="bf16", scaling="none", factor=1.0, start=0, back=False),
+        # the gradient at far positions: half the head, interleaved pairs, by-parts scaling
+        dict(name="rotary_grad_long", kind="rotary", batch=1, seq=5001, heads=32, kv_heads=8,
+             dim=128, rot=64, pairs="interleaved", dtype="f32", scaling="yarn", factor=16.0,
+             start=120000, back=True),
+        # one new byte in each of 64 running documents
+        dict(name="append_step", kind="append", seqs=64, chunk=1, ctx=4096, mix=1, heads=12,
+             kv_heads=12, dim=64, rot=64, pairs="half", page=16, dtype="bf16"),
+        # the first chunks of seven documents, ragged, grouped heads
+        dict(name="append_chunk", kind="append", seqs=7, chunk=2500, ctx=2500, mix=2, heads=32,
+             kv_heads=8, dim=128, rot=128, pairs="half", page=16, dtype="bf16"),
+        # one new byte of one document of about a thousand: latency
+        dict(name="attend_step", kind="attend", seqs=1, chunk=1, ctx=1000, mix=3, heads=12,
+             kv_heads=12, dim=64, window=0, page=16, dtype="bf16"),
+        # one new byte in each of 48 documents of up to 8192 bytes
+        dict(name="attend_step_batch", kind="attend", seqs=48, chunk=1, ctx=8192, mix=4, heads=12,
+             kv_heads=12, dim=64, window=0, page=16, dtype="bf16"),
+        # the same with grouped heads of 128 and long contexts
+        dict(name="attend_step_grouped", kind="attend", seqs=16, chunk=1, ctx=32768, mix=5,
+             heads=32, kv_heads=8, dim=128, window=0, page=32, dtype="bf16"),
+        # chunks of running documents under the model's sliding window
+        dict(name="attend_chunk_window", kind="attend", seqs=9, chunk=1025, ctx=8192, mix=6,
+             heads=12, kv_heads=12, dim=64, window=512, page=16, dtype="bf16"),
+        # long chunks over long contexts, grouped heads, full causal: the largest
+        dict(name="attend_chunk_grouped", kind="attend", seqs=2, chunk=2048, ctx=16384, mix=7,
+             heads=32, kv_heads=8, dim=128, window=0, page=64, dtype="bf16"),
+        # f32 throughout, short chunks
+        dict(name="attend_f32", kind="attend", seqs=3, chunk=100, ctx=1500, mix=8, heads=12,
+             kv_heads=12, dim=64, window=0, page=16, dtype="f32"),
+        # 24 continuations of running documents opened, grown and dropped, all layers
+        dict(name="pages_branch", kind="branch", seqs=24, live=32, grow=20, ctx=1500, mix=9,
+             layers=LAYERS, kv_heads=12, dim=64, page=16, dtype="bf16"),
+        # a pool with holes after half of its documents ended, all layers
+        dict(name="pages_compact", kind="compact", live=24, ended=24, ctx=1500, mix=10,
+             layers=LAYERS, kv_heads=12, dim=64, page=16, dtype="bf16"),
+    ]
+
+
+def _log(rng, lo, hi):
+    return max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+def draw(rng):
+    kind = rng.choice(["rotary", "append", "attend", "attend", "attend", "branch", "compact"])
+    mix = rng.randrange(1 << 20)
+    dtype = rng.choice(["bf16", "bf16", "bf16", "f32"])
+    heads, kv_heads, dim = rng.choice([(12, 12, 64), (12, 12, 64), (12, 4, 64), (32, 8, 128),
+                                       (8, 1, 128), (4, 2, 128)])
+    page = rng.choice([8, 16, 16, 32, 64, 128])
+    pairs = rng.choice(["half", "interleaved"])
+    rot = rng.choice([dim, dim, dim // 2, dim // 4])
+    if kind == "rotary":
+        batch, n = rng.choice([1, 1, 2, 7, 16]), _log(rng, 1, 65536)
+        n = min(n, 65536 * 24 * 64 // ((heads + kv_heads) * dim))
+        scaling = rng.choice(["none", "none", "linear", "ntk", "yarn"])
+        return dict(kind=kind, batch=batch, seq=max(1, n // batch), heads=heads,
+                    kv_heads=kv_heads, dim=dim, rot=rot, pairs=pairs, dtype=dtype,
+                    scaling=scaling, factor=1.0 if scaling == "none" else rng.choice([2.0, 8.0, 32.0]),
+                    start=rng.choice([0, 0, 1000, 100000, 1000000]), back=rng.random() < 0.4)
+    if kind == "append":
+        seqs, chunk = _log(rng, 1, 128), _log(rng, 1, 2048)
+        chunk = max(1, min(chunk, 16384 // seqs))
+        return dict(kind=kind, seqs=seqs, chunk=chunk, ctx=max(chunk, _log(rng, 1, 8192)), mix=mix,
+                    heads=heads, kv_heads=kv_heads, dim=dim, rot=rot, pairs=pairs, page=page,
+                    dtype=dtype)
+    if kind == "attend":
+        seqs = _log(rng, 1, 64)
+        chunk = 1 if rng.random() < 0.4 else _log(rng, 1, 2048)
+        ctx = max(chunk, _log(rng, 1, 32768))
+        window = rng.choice([0, 0, 512, 300])
+        # bounds on the new tokens, the cache (2 GB) and the scores (2^30 and, in f32, 2^27)
+        seqs = max(1, min(seqs, 4096 // chunk, (1 << 29) // (ctx * kv_heads * dim)))
+        most = (1 << 30) if dtype == "bf16" else (1 << 27)
+        chunk = max(1, min(chunk, most // (seqs * heads * ctx)))
+        return dict(kind=kind, seqs=seqs, chunk=chunk, ctx=ctx, mix=mix, heads=heads,
+                    kv_heads=kv_heads, dim=dim, window=window, page=page, dtype=dtype)
+    layers = rng.choice([1, 2, LAYERS])
+    live, ctx = _log(rng, 1, 48), _log(rng, 1, 1500)
+    # the pool: at most the listed one's bytes
+    live = max(1, min(live, 600000000 // (ctx * layers * kv_heads * dim * 2) // 2))
+    if kind == "branch":
+        return dict(kind=kind, seqs=_log(rng, 1, 32), live=live, grow=_log(rng, 1, 100), ctx=ctx,
+                    mix=mix, layers=layers, kv_heads=kv_heads, dim=dim, page=page, dtype=dtype)
+    return dict(kind=kind, live=live, ended=_log(rng, 1, live), ctx=ctx, mix=mix, layers=layers,
+                kv_heads=kv_heads, dim=dim, page=page, dtype=dtype)
+
+
+# ---- shapes of a case ------------------------------------------------------------
+
+def _ragged(case):
+    """(new tokens, context with them) of every sequence: the first has the full
+    sizes, the others anything up to them."""
+    r = np.random.RandomState(case["mix"])
+    n = 1 + (r.rand(case["seqs"]) * case["chunk"]).astype(np.int64)
+    n[0] = case["chunk"]
+    length = 1 + (r.rand(case["seqs"]) * case["ctx"]).astype(np.int64)
+    length[0] = case["ctx"]
+    return np.minimum(n, case["chunk"]), np.maximum(np.minimum(length, case["ctx"]), n)
+
+
+def _documents(case, count):
+    r = np.random.RandomState(case["mix"])
+    return 1 + (r.rand(count) * case["ctx"]).astype(np.int64)
+
+
+def _visible(n, length, window):
+    """Pairs of (new token, key) that a causal chunk sees."""
+    total = 0
+    for a, b in zip(n.tolist(), length.tolist()):
+        hi = np.arange(b - a, b) + 1
+        total += int((np.minimum(hi, window) if window else hi).sum())
+    return total
+
+
+def _keys_read(n, length, window):
+    return int((np.minimum(length, n + window - 1) if window else length).sum())
+
+
+def _forks(case):
+    """Which document each continuation comes from."""
+    r = np.random.RandomState(case["mix"] + 1)
+    return r.randint(0, case["live"], case["seqs"])
+
+
+def _inv_freq(rot, scaling, factor, original):
+    """Rotary frequencies in 64 bits and the factor on the rotated values."""
+    i = torch.arange(0, rot, 2, dtype=torch.float64, device=DEV) / rot
+    if scaling == "ntk":
+        return (THETA * factor ** (rot / (rot - 2))) ** -i, 1.0
+    f = THETA ** -i
+    if scaling == "linear":
+        return f / factor, 1.0
+    if scaling == "none":
+        return f, 1.0
+
+    def turn(beta):
+        return rot * math.log(original / (beta * 2 * math.pi)) / (2 * math.log(THETA))
+
+    lo, hi = max(math.floor(turn(32.0)), 0), min(math.ceil(turn(1.0)), rot - 1)
+    ramp = ((torch.arange(rot // 2, dtype=torch.float64, device=DEV) - lo)
+            / max(hi - lo, 0.001)).clamp(0, 1)
+    return f / factor * ramp + f * (1 - ramp), 0.1 * math.log(factor) + 1.0
+
+
+ORIGINAL = 8192  # positions before the scaling: the model's max_seqlen
+
+
+# ---- inputs ------------------------------------------------------------------------
+
+def _package(name):
+    return importlib.import_module("blt-burn_amd." + name)
+
+
+def _i32(x):
+    return torch.as_tensor(np.asarray(x, dtype=np.int32)).to(DEV)
+
+
+def _pages(lengths, page, spare, g):
+    """A shuffled pool: (table [seqs, columns] with -1 where no page is, refcounts)."""
+    need = -(-lengths // page)
+    pool = int(need.sum()) + spare
+    order = torch.randperm(pool, generator=g, device=DEV).cpu().numpy()
+    table = np.full((len(lengths), max(1, int(need.max()))), -1, np.int64)
+    at = 0
+    for s, k in enumerate(need.tolist()):
+        table[s, :k] = order[at:at + k]
+        at += k
+    used = np.zeros(pool, np.int64)
+    used[order[:at]] = 1
+    return table, used
+
+
+def _pool(shape, dtype, g):
+    out = torch.empty(shape, dtype=dtype, device=DEV)
+    for layer in out:  # a layer at a time: the 32-bit draw of one only
+        layer.copy_(torch.randn(layer.shape, generator=g, device=DEV))
+    return out
+
+
+def prepare(case, seed):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(seed)
+    c, t = case, TYPES[case["dtype"]]
+    if c["kind"] == "rotary":
+        # q and k as a projection leaves them: heads of one token side by side
+        H, K = c["heads"], c["kv_heads"]
+        x = torch.randn((c["batch"], c["seq"], H + K, c["dim"]), generator=g, device=DEV).to(t)
+        x = x.transpose(1, 2)
+        pos = torch.arange(c["start"], c["start"] + c["seq"], dtype=torch.int32, device=DEV)
+        st = dict(case=c, q=x[:, :H], k=x[:, H:], pos=pos)
+        if own:
+            F = _package("fused_ops")
+            st["plan"] = F.RotaryPlan(c["rot"], theta=THETA, pairs=c["pairs"],
+                                      scaling=c["scaling"], factor=c["factor"],
+                                      original_len=ORIGINAL, device=DEV)
+        return st
+    if c["kind"] in ("append", "attend"):
+        n, length = _ragged(c)
+        table, used = _pages(length, c["page"], 3, g)
+        shape = (1, len(used), c["kv_heads"], c["page"], c["dim"])
+        total = int(n.sum())
+        st = dict(case=c, k=_pool(shape, t, g), v=_pool(shape, t, g), table=_i32(table),
+                  lens=_i32(length), refs=_i32(used), total=total, most=int(n.max()),
+                  starts=_i32(np.concatenate([[0], np.cumsum(n)])))
+        st["q"] = torch.randn((total, c["heads"], c["dim"]), generator=g, device=DEV).to(t)
+        if c["kind"] == "append":
+            new = torch.randn((total, 2, c["kv_heads"], c["dim"]), generator=g, device=DEV).to(t)
+            st["k_new"], st["v_new"] = new[:, 0], new[:, 1]
+    else:
+        gone = c["seqs"] if c["kind"] == "branch" else c["ended"]
+        lens = _documents(c, c["live"] + (c["ended"] if c["kind"] == "compact" else 0))
+        if c["kind"] == "branch":
+            # room for every continuation's partial page and its growth
+            spare = gone * (2 + c["grow"] // c["page"]) + 5
+            table, used = _pages(lens, c["page"], spare, g)
+            cols = table.shape[1] + 1 + c["grow"] // c["page"]
+            wide = np.full((c["live"] + gone, cols), -1, np.int64)
+            wide[:c["live"], :table.shape[1]] = table
+            table, lens = wide, np.concatenate([lens, np.zeros(gone, np.int64)])
+        else:
+            table, used = _pages(lens, c["page"], 0, g)
+            used[table[c["live"]:][table[c["live"]:] >= 0]] = 0
+            table[c["live"]:] = -1
+            lens[c["live"]:] = 0
+        shape = (c["layers"], len(used), c["kv_heads"], c["page"], c["dim"])
+        st = dict(case=c, k=_pool(shape, t, g), v=_pool(shape, t, g), table=_i32(table),
+                  lens=_i32(lens), refs=_i32(used))
+        if c["kind"] == "branch":
+            st["src"], st["dst"] = _i32(_forks(c)), _i32(c["live"] + np.arange(gone))
+            st["grow"] = torch.full((gone,), c["grow"], dtype=torch.int32, device=DEV)
+        else:
+            st["table0"], st["refs0"] = st["table"].clone(), st["refs"].clone()
+    if own:
+        st["cache"] = _package("cache").PagedCache.wrap(st["k"], st["v"], st["table"], st["lens"],
+                                                        st["refs"])
+        if c["kind"] == "append":
+            st["plan"] = _package("fused_ops").RotaryPlan(c["rot"], theta=THETA, pairs=c["pairs"],
+                                                          device=DEV)
+    return st
+
+
+# ---- one pass ------------------------------------------------------------------------
+
+def run(state):
+    return {"rotary": _rotary, "append": _append, "attend": _attend, "branch": _branch,
+            "compact": _compact}[state["case"]["kind"]](state)
+
+
+def _turned(x, cos, sin, pairs):
+    """x [..., d] in 32 bits with its first 2 * cos.shape[-1] values rotated."""
+    half = cos.shape[-1]
+    rot, rest = x[..., :2 * half], x[..., 2 * half:]
+    if pairs == "half":
+        a, b = rot[..., :half], rot[..., half:]
+        return torch.cat([a * cos - b * sin, a * sin + b * cos, rest], -1)
+    a, b = rot[..., 0::2], rot[..., 1::2]
+    both = torch.stack([a * cos - b * sin, a * sin + b * cos], -1)
+    return torch.cat([both.flatten(-2), rest], -1)
+
+
+def _rotary(st):
+    c = st["case"]
+    if own:
+        return _package("fused_ops").fused_rotary(st["q"], st["k"], st["pos"], st["plan"],
+                                                  backward=c["back"])
+    f, mag = _inv_freq(c["rot"], c["scaling"], c["factor"], ORIGINAL)
+    angle = st["pos"].double()[:, None] * f
+    cos, sin = (angle.cos() * mag).float(), (angle.sin() * (-mag if c["back"] else mag)).float()
+    return tuple(_turned(x.float(), cos, sin, c["pairs"]).to(x.dtype) for x in (st["q"], st["k"]))
+
+
+def _rows(st):
+    """The sequence and the position of every new token."""
+    i = torch.arange(st["total"], device=DEV)
+    b = torch.searchsorted(st["starts"][1:].long(), i, right=True)
+    return b, st["lens"].long()[b] - st["starts"].long()[b + 1] + i
+
+
+def _append(st):
+    c = st["case"]
+    if own:
+        q = st["cache"].append(0, st["k_new"], st["v_new"], st["starts"], rotary=st["plan"],
+                               q=st["q"])
+        return q, st["k"], st["v"]
+    b, pos = _rows(st)
+    f, _ = _inv_freq(c["rot"], "none", 1.0, ORIGINAL)
+    angle = pos.double()[:, None] * f
+    cos, sin = angle.cos().float()[:, None], angle.sin().float()[:, None]
+    q = _turned(st["q"].float(), cos, sin, c["pairs"]).to(st["q"].dtype)
+    k = _turned(st["k_new"].float(), cos, sin, c["pairs"]).to(st["k"].dtype)
+    page, slot = st["table"].long()[b, pos // c["page"]], pos % c["page"]
+    st["k"][0][page, :, slot] = k
+    st["v"][0][page, :, slot] = st["v_new"]
+    return q, st["k"], st["v"]
+
+
+def _attend(st):
+    c = st["case"]
+    if own:
+        return st["cache"].attention(0, st["q"], st["starts"], window=c["window"])
+    H, K, d, B = c["heads"], c["kv_heads"], c["dim"], c["seqs"]
+    n, at = st["starts"][1:].long() - st["starts"][:-1].long(), st["starts"][:-1].long()
+    pages = st["table"].clamp(min=0).long()
+    k, v = (x[0][pages].transpose(1, 2).reshape(B, K, -1, d).float() for x in (st["k"], st["v"]))
+    row = torch.arange(st["most"], device=DEV)
+    take = (at[:, None] + row).clamp(max=st["total"] - 1)
+    q = st["q"][take].float().view(B, st["most"], K, H // K, d).permute(0, 2, 3, 1, 4)
+    q = q.reshape(B, K, -1, d) / math.sqrt(d)
+    s = torch.matmul(q, k.transpose(-1, -2)).view(B, K, H // K, st["most"], -1)
+    pos = (st["lens"].long() - n)[:, None] + row
+    key = torch.arange(k.shape[2], device=DEV)
+    seen = (key <= pos[..., None]) & (row < n[:, None])[..., None]
+    if c["window"]:
+        seen = seen & (key > pos[..., None] - c["window"])
+    s.masked_fill_(~seen[:, None, None], -math.inf)
+    s -= s.amax(-1, keepdim=True).clamp(min=-1e30)
+    p = s.exp_()
+    o = torch.matmul(p.view(B, K, -1, p.shape[-1]), v).view(B, K, H // K, st["most"], d)
+    o = o / p.sum(-1, keepdim=True).clamp(min=1e-30)
+    o = o.permute(0, 3, 1, 2, 4).reshape(B, st["most"], H, d)
+    b, _ = _rows(st)
+    return o[b, torch.arange(st["total"], device=DEV) - at[b]].to(st["q"].dtype)
+
+
+def _branch(st):
+    c, page = st["case"], st["case"]["page"]
+    if own:
+        cache = st["cache"]
+        cache.fork(st["src"], st["dst"])
+        cache.reserve(st["grow"], st["dst"])
+        cache.free(st["dst"])
+        return st["k"], st["v"], st["table"], st["lens"], st["refs"]
+    table, lens, refs = st["table"], st["lens"], st["refs"]
+    src, dst, cols = st["src"].long(), st["dst"].long(), torch.arange(table.shape[1], device=DEV)
+    # fork: full pages shared, a partial one copied into the lowest free page
+    n = lens[src].long()
+    full, part = n // page, n % page
+    has = part > 0
+    free = torch.argsort((refs != 0).to(torch.int32), stable=True)
+    rank = torch.where(has, has.cumsum(0) - 1, has.sum() + (~has).cumsum(0) - 1)
+    fresh = free[rank]
+    rows = table[src]
+    old = rows.gather(1, full.clamp(max=table.shape[1] - 1)[:, None])[:, 0].clamp(min=0).long()
+    shared = cols < full[:, None]
+    refs.scatter_add_(0, torch.where(shared, rows, 0).long().flatten(),
+                      shared.to(torch.int32).flatten())
+    refs[fresh] = has.to(torch.int32)
+    table[dst] = torch.where(shared, rows, torch.where(
+        (cols == full[:, None]) & has[:, None], fresh[:, None].to(torch.int32), table[dst]))
+    keep = (torch.arange(page, device=DEV) < part[:, None])[None, :, None, :, None]
+    for x in (st["k"], st["v"]):
+        x[:, fresh] = torch.where(keep, x[:, old], x[:, fresh])
+    lens[dst] = lens[src]
+    # reserve: the lowest free pages in the order of the sequences
+    have, want = -(-n // page), -(-(n + c["grow"]) // page)
+    first = (want - have).cumsum(0) - (want - have)
+    free = torch.argsort((refs != 0).to(torch.int32), stable=True)
+    more = (cols >= have[:, None]) & (cols < want[:, None])
+    ordinal = (first[:, None] + cols - have[:, None]).clamp(0, refs.numel() - 1)
+    table[dst] = torch.where(more, free[ordinal].to(torch.int32), table[dst])
+    refs.scatter_add_(0, torch.where(more, table[dst], 0).long().flatten(),
+                      more.to(torch.int32).flatten())
+    lens[dst] = (n + c["grow"]).to(torch.int32)
+    # free: a reference less for every page
+    mine = cols < want[:, None]
+    refs.scatter_add_(0, torch.where(mine, table[dst], 0).long().flatten(),
+                      -mine.to(torch.int32).flatten())
+    lens[dst] = 0
+    return st["k"], st["v"], table, lens, refs
+
+
+def _compact(st):
+    st["table"].copy_(st["table0"])  # the pool as it was: the moved pages' old places are intact
+    st["refs"].copy_(st["refs0"])
+    if own:
+        st["cache"].compact()
+        return st["k"], st["v"], st["table"], st["refs"]
+    refs, table = st["refs"], st["table"]
+    live = refs > 0
+    i = torch.arange(refs.numel(), device=DEV)
+    front = i < live.sum()
+    movers, holes = (live & ~front).nonzero()[:, 0], (~live & front).nonzero()[:, 0]
+    to = i.clone()
+    to[movers] = holes
+    for x in (st["k"], st["v"]):
+        x[:, holes] = x[:, movers]
+    refs[holes] = refs[movers]
+    refs[movers] = 0
+    own_page = torch.arange(table.shape[1], device=DEV) * st["case"]["page"] < st["lens"][:, None]
+    table.copy_(torch.where(own_page, to[table.clamp(min=0).long()].to(torch.int32), table))
+    return st["k"], st["v"], table, refs
+
+
+# ---- what a pass cannot do without ---------------------------------------------------
+
+def work(case):
+    c = case
+    e = 2 if c["dtype"] == "bf16" else 4
+    if c["kind"] == "rotary":
+        tokens, heads = c["batch"] * c["seq"], c["heads"] + c["kv_heads"]
+        return {"bytes": 2 * tokens * heads * c["dim"] * e + 4 * c["seq"],
+                "flops": 3 * tokens * heads * c["rot"]}
+    row = c["kv_heads"] * c["dim"] * e  # one token's k (or v) in one layer
+    if c["kind"] == "append":
+        tokens = int(_ragged(c)[0].sum())
+        return {"bytes": 2 * tokens * (2 * row + c["heads"] * c["dim"] * e),
+                "flops": 3 * tokens * (c["heads"] + c["kv_heads"]) * c["rot"]}
+    if c["kind"] == "attend":
+        n, length = _ragged(c)
+        return {"bytes": 2 * _keys_read(n, length, c["window"]) * row
+                         + 2 * int(n.sum()) * c["heads"] * c["dim"] * e,
+                "flops": 4 * c["dim"] * c["heads"] * _visible(n, length, c["window"])}
+    if c["kind"] == "branch":
+        lens = _documents(c, c["live"])[_forks(c)]
+        tables = 4 * int((2 * -(-lens // c["page"]) + 4).sum())
+        return {"bytes": 4 * int((lens % c["page"]).sum()) * row * c["layers"] + tables, "flops": 0}
+    lens = _documents(c, c["live"] + c["ended"])
+    need = -(-lens // c["page"])
+    live, pool = int(need[:c["live"]].sum()), int(need.sum())
+    moved = live * (pool - live) // max(1, pool)  # of a shuffled pool, on average
+    return {"bytes": 4 * moved * c["page"] * row * c["layers"] + 8 * pool + 8 * int(need.sum()),
+            "flops": 0}
+
+
+# ---- the definition, in 64 bits ------------------------------------------------------
+
+def _spin(x, pos, c):
+    """Rows of x [..., tokens, d] as complex pairs times exp(i * angle) in 64 bits."""
+    half = c["rot"] // 2
+    f = [THETA ** (-2.0 * i / c["rot"]) for i in range(half)]
+    mag, s, factor = 1.0, c.get("scaling", "none"), c.get("factor", 1.0)
+    if s == "linear":
+        f = [w / factor for w in f]
+    elif s == "ntk":
+        base = THETA * factor ** (c["rot"] / (c["rot"] - 2.0))
+        f = [base ** (-2.0 * i / c["rot"]) for i in range(half)]
+    elif s == "yarn":
+        mag = 1.0 + 0.1 * math.log(factor)
+        # the pair whose wave turns `beta` times over the original length
+        ends = [c["rot"] * math.log(ORIGINAL / (2 * math.pi * beta)) / (2 * math.log(THETA))
+                for beta in (32.0, 1.0)]
+        lo, hi = max(math.floor(ends[0]), 0), min(math.ceil(ends[1]), c["rot"] - 1)
+        for i in range(half):
+            share = min(1.0, max(0.0, (i - lo) / max(hi - lo, 0.001)))
+            f[i] = f[i] * (1.0 - share) + f[i] / factor * share
+    turn = torch.outer(pos.double(), torch.tensor(f, dtype=torch.float64, device=DEV))
+    wave = torch.polar(torch.full_like(turn, mag), -turn if c.get("back") else turn)
+    x = x.double()
+    head = x[..., :c["rot"]].contiguous()
+    if c["pairs"] == "half":
+        z = torch.complex(head[..., :half], head[..., half:]) * wave
+        return torch.cat([z.real, z.imag, x[..., c["rot"]:]], -1)
+    z = torch.view_as_complex(head.unflatten(-1, (half, 2))) * wave
+    return torch.cat([torch.view_as_real(z).flatten(-2), x[..., c["rot"]:]], -1)
+
+
+def exact(case, seed):
+    c, st = case, prepare(case, seed)
+    if c["kind"] == "rotary":
+        return _spin(st["q"], st["pos"], c), _spin(st["k"], st["pos"], c)
+    page, table = c["page"], st["table"].cpu().tolist()
+    if c["kind"] in ("append", "attend"):
+        n, length = (x.tolist() for x in _ragged(c))
+    if c["kind"] == "append":
+        q, k, v = st["q"].double(), st["k"].double(), st["v"].double()
+        at = 0
+        for b in range(c["seqs"]):
+            pos = torch.arange(length[b] - n[b], length[b], device=DEV)
+            rows = slice(at, at + n[b])
+            q[rows] = _spin(st["q"][rows].transpose(0, 1), pos, c).transpose(0, 1)
+            pages = torch.tensor(table[b], device=DEV)[pos // page]
+            k[0][pages, :, pos % page] = _spin(st["k_new"][rows].transpose(0, 1), pos,
+                                               c).transpose(0, 1)
+            v[0][pages, :, pos % page] = st["v_new"][rows].double()
+            at += n[b]
+        return q, k, v
+    if c["kind"] == "attend":
+        H, K, d = c["heads"], c["kv_heads"], c["dim"]
+        out = torch.empty((st["total"], H, d), dtype=torch.float64, device=DEV)
+        at = 0
+        for b in range(c["seqs"]):
+            pos = torch.arange(length[b] - n[b], length[b], device=DEV)
+            key = torch.arange(length[b], device=DEV)
+            hide = key[None] > pos[:, None]
+            if c["window"]:
+                hide |= key[None] <= pos[:, None] - c["window"]
+            pages = torch.tensor(table[b][:-(-length[b] // page)], device=DEV)
+            for h in range(H):
+                kh, vh = (x[0][pages, h // (H // K)].reshape(-1, d)[:length[b]].double()
+                          for x in (st["k"], st["v"]))
+                s = (st["q"][at:at + n[b], h].double() @ kh.t()) / math.sqrt(d)
+                out[at:at + n[b], h] = torch.softmax(s.masked_fill(hide, -math.inf), -1) @ vh
+            at += n[b]
+        return out
+    lens, refs = st["lens"].cpu().tolist(), st["refs"].cpu().tolist()
+    k, v = st["k"], st["v"]
+    if c["kind"] == "branch":
+        src, dst = st["src"].cpu().tolist(), st["dst"].cpu().tolist()
+        grabbed = []
+        for a in src:  # the forks take a page each where the last one is partial
+            fill = lens[a] % page
+            if fill:
+                new = refs.index(0)
+                refs[new] = 1
+                grabbed.append(new)
+                for x in (k, v):
+                    x[:, new, :, :fill] = x[:, table[a][lens[a] // page], :, :fill]
+        for b, a in zip(dst, src):
+            whole = lens[a] // page
+            table[b][:whole] = table[a][:whole]
+            if lens[a] % page:
+                table[b][whole] = grabbed.pop(0)
+        for b, a in zip(dst, src):
+            for col in range(-(-lens[a] // page), -(-(lens[a] + c["grow"]) // page)):
+                table[b][col] = refs.index(0)
+                refs[table[b][col]] = 1
+        refs = st["refs"].cpu().tolist()  # dropped again
+        return k, v, _i32(table), _i32(lens), _i32(refs)
+    live = sum(r > 0 for r in refs)
+    moved = dict(zip([p for p, r in enumerate(refs) if r and p >= live],
+                     [p for p, r in enumerate(refs) if not r and p < live]))
+    for p, to in moved.items():
+        refs[to], refs[p] = refs[p], 0
+        k[:, to], v[:, to] = k[:, p], v[:, p]
+    table = [[moved.get(p, p) if col * page < lens[s] else p for col, p in enumerate(row)]
+             for s, row in enumerate(table)]
+    return k, v, _i32(table), _i32(refs)
