@@ -19,6 +19,10 @@ EPS_AFTER_SQRT, EPS_INSIDE_SQRT = 0, 1
 PATCH_MONOTONIC, PATCH_GLOBAL = 0, 1
 EPI_BF16, EPI_F32, EPI_RESID_F32, EPI_QKV_ROPE, EPI_SILU_GATE = 0, 1, 2, 3, 4
 NUM_STAGES = 11
+DTYPE_F32, DTYPE_BF16 = 0, 1
+ROTARY_SCALING = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
+# blt_cache_status
+CACHE_FULL, CACHE_TOO_LONG, CACHE_BAD_INDEX, CACHE_BUSY, CACHE_NO_PAGE = 1, 2, 4, 8, 16
 
 EXPORTS = {
     # name: (restype, argtypes)
@@ -42,6 +46,21 @@ EXPORTS = {
     "blt_fused_attention_f32": (c_i32, [c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_i32,
                                         c_i32, c_vp]),
     "blt_rope_table_f32": (c_i32, [c_vp, c_i32, c_i32, c_f64, c_vp]),
+    "blt_rotary_frequencies": (c_i32, [c_i32, c_f64, c_i32, c_f64, c_f64, c_vp, c_vp]),
+    "blt_fused_rotary": (c_i32, [c_vp] * 4 + [c_i32] + [c_i64] * 4 + [c_i32] + [c_i64] * 12
+                         + [c_vp, c_i64, c_vp, c_i32, c_vp]),
+    "blt_cache_workspace_bytes": (c_i64, [c_vp, c_i64]),
+    "blt_cache_reserve": (c_i32, [c_vp, c_vp, c_vp, c_i64, c_vp]),
+    "blt_cache_trim": (c_i32, [c_vp, c_vp, c_vp, c_i64, c_vp, c_i64, c_vp]),
+    "blt_cache_fork": (c_i32, [c_vp, c_vp, c_vp, c_i64, c_vp, c_i64, c_vp]),
+    "blt_cache_compact": (c_i32, [c_vp, c_vp, c_i64, c_vp]),
+    "blt_cache_copy_pages": (c_i32, [c_vp, c_vp, c_vp, c_i64, c_vp]),
+    "blt_cache_append": (c_i32, [c_vp, c_i32] + [c_vp, c_i64, c_i64] * 4
+                         + [c_i64, c_vp, c_vp, c_i64, c_i64, c_vp, c_vp]),
+    "blt_paged_attention_workspace_bytes": (c_i64, [c_vp, c_i64, c_i64, c_i64]),
+    "blt_paged_attention": (c_i32, [c_vp, c_i32] + [c_vp, c_i64, c_i64] * 2
+                            + [c_i64, c_vp, c_vp, c_i64, c_i64, c_i32, c_i32, c_f32, c_vp, c_i64,
+                               c_vp]),
     "blt_patch_boundaries": (c_i32, [c_vp, c_i64, c_i64, c_f32, c_i32, c_vp, c_vp, c_vp, c_vp,
                                      c_vp]),
     "blt_patch_mask_starts": (c_i32, [c_vp, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp]),
@@ -120,6 +139,19 @@ class PatchRule(ctypes.Structure):
     """blt_patch_rule."""
     _fields_ = [("mode", c_i32), ("threshold", c_f32), ("mask", c_vp), ("starts", c_vp),
                 ("lengths", c_vp), ("count", c_vp)]
+
+
+class Rotary(ctypes.Structure):
+    """blt_rotary."""
+    _fields_ = [("freq", c_vp), ("rotary_dim", c_i32), ("interleaved", c_i32),
+                ("magnitude", c_f32)]
+
+
+class PagedCacheDesc(ctypes.Structure):
+    """blt_paged_cache."""
+    _fields_ = ([(n, c_vp) for n in ("k", "v", "page_table", "lens", "refcount", "status")]
+                + [(n, c_i32) for n in ("dtype", "n_layers", "num_pages", "n_kv_heads",
+                                        "page_size", "head_dim", "max_seqs", "max_pages")])
 
 
 class IngestStats(ctypes.Structure):

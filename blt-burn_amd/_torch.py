@@ -2,7 +2,7 @@
 handed to the C ABI (pointers, element counts, the current HIP stream)."""
 import torch
 
-from ._lib import BltError
+from ._lib import BltError, check
 
 
 # the raw current-stream handle without building a torch.cuda.Stream object
@@ -17,6 +17,16 @@ def stream_ptr(device=None):
         if device is None or isinstance(device, int):
             return _raw_stream(torch.cuda.current_device() if device is None else device)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def call_on(device, fn, what, *args):
+    """fn(*args, stream) on `device` (with an index) and its current stream: the
+    library launches on the current device, which may be another one."""
+    if torch.cuda.current_device() == device.index:
+        check(fn(*args, stream_ptr(device)), what)
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, stream_ptr(device)), what)
 
 
 def require_cuda(*tensors):

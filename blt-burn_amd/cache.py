@@ -1,0 +1,263 @@
+"""A paged key/value cache and attention over it: the incremental form of the
+entropy model's attention (the reference runs whole rows, model.rs:620-672).
+
+A step of a running batch is
+
+    cache.reserve(counts, seqs)                      # room for the new tokens
+    for each layer:
+        q = cache.append(layer, k, v, starts, seqs, rotary=plan, q=q)
+        o = cache.attention(layer, q, starts, seqs)
+
+and fork / trim / free / compact open, cut, drop and pack sequences.  All
+bookkeeping is on the device: no call synchronises, and all of them can be
+captured into a graph.  A call that the state does not allow (no free page, a
+sequence too long) sets a bit in the cache's status instead of raising; check()
+waits, raises BltError for it and clears it.  Calls on one cache must be
+stream-ordered.
+"""
+import ctypes
+
+import torch
+
+from . import _lib
+from ._lib import BltError
+from ._torch import call_on, require_cuda
+from .fused_ops import RotaryPlan
+
+__all__ = ["PagedCache"]
+
+_TYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
+_FAILURES = ((_lib.CACHE_FULL, "not enough free pages"),
+             (_lib.CACHE_TOO_LONG, "a sequence would pass its page table"),
+             (_lib.CACHE_BAD_INDEX, "an index out of range"),
+             (_lib.CACHE_BUSY, "a sequence twice in a call, or a fork onto one with tokens"),
+             (_lib.CACHE_NO_PAGE, "tokens appended where their sequence has no page"))
+
+
+class PagedCache:
+    """k, v [n_layers, num_pages, n_kv_heads, page_size, head_dim] (f32 or bf16) with
+    page_table [max_seqs, max_pages], lens [max_seqs] and refcount [num_pages], all
+    int32 tensors of the cache's device that may be read at any time (stream-ordered).
+    head_dim 64 or 128, page_size a power of two from 8 to 1024."""
+
+    def __init__(self, n_layers, n_kv_heads, head_dim, num_pages, max_seqs, max_len, page_size=16,
+                 dtype=torch.bfloat16, device=None):
+        if dtype not in _TYPES:
+            raise BltError("PagedCache: dtype must be float32 or bfloat16")
+        if min(n_layers, n_kv_heads, head_dim, num_pages, max_seqs, max_len, page_size) < 1:
+            raise BltError("PagedCache: sizes must be positive")
+        dev = torch.device("cuda" if device is None else device)
+        shape = (n_layers, num_pages, n_kv_heads, page_size, head_dim)
+        self._bind(torch.zeros(shape, dtype=dtype, device=dev),
+                   torch.zeros(shape, dtype=dtype, device=dev),
+                   torch.full((max_seqs, -(-max_len // page_size)), -1, dtype=torch.int32,
+                              device=dev),
+                   torch.zeros(max_seqs, dtype=torch.int32, device=dev),
+                   torch.zeros(num_pages, dtype=torch.int32, device=dev))
+
+    @classmethod
+    def wrap(cls, k, v, page_table, lens, refcount):
+        """A cache over tensors that the caller owns (shapes as above, contiguous), in
+        the state that they describe."""
+        self = cls.__new__(cls)
+        self._bind(k, v, page_table, lens, refcount)
+        return self
+
+    def _bind(self, k, v, page_table, lens, refcount):
+        require_cuda(k, v, page_table, lens, refcount)
+        if k.dim() != 5 or k.shape != v.shape or k.dtype != v.dtype or k.dtype not in _TYPES:
+            raise BltError("PagedCache: k and v must be f32 or bf16 [layers, pages, kv_heads, "
+                           "page_size, head_dim]")
+        if page_table.dim() != 2 or lens.dim() != 1 or refcount.dim() != 1 or \
+                page_table.shape[0] != lens.shape[0] or refcount.shape[0] != k.shape[1]:
+            raise BltError("PagedCache: page_table [seqs, columns], lens [seqs], refcount [pages]")
+        if any(t.dtype != torch.int32 for t in (page_table, lens, refcount)):
+            raise BltError("PagedCache: page_table, lens and refcount must be int32")
+        if any(t.device != k.device or not t.is_contiguous()
+               for t in (k, v, page_table, lens, refcount)):
+            raise BltError("PagedCache: tensors must be contiguous and on one device")
+        self.k, self.v = k, v
+        self.page_table, self.lens, self.refcount = page_table, lens, refcount
+        self.device, self.dtype = k.device, k.dtype
+        self.n_layers, self.num_pages, self.n_kv_heads, self.page_size, self.head_dim = k.shape
+        self.max_seqs, self.max_pages = page_table.shape
+        self._status = torch.zeros(1, dtype=torch.int32, device=k.device)
+        self._desc = _lib.PagedCacheDesc(
+            k.data_ptr(), v.data_ptr(), page_table.data_ptr(), lens.data_ptr(),
+            refcount.data_ptr(), self._status.data_ptr(), _TYPES[k.dtype], *k.shape[:3],
+            k.shape[3], k.shape[4], *page_table.shape)
+        self._ptr = ctypes.addressof(self._desc)
+        self._lib = _lib.lib()
+        self._heads = (self.n_kv_heads, self.head_dim)
+        if self._lib.blt_cache_workspace_bytes(self._ptr, 0) <= 0:
+            raise BltError("PagedCache: bad sizes")
+        # the library's own checks, once: an empty list does nothing else
+        call_on(self.device, self._lib.blt_cache_reserve, "PagedCache", self._ptr, None, None, 0)
+
+    # ---- status ---------------------------------------------------------------
+    def check(self):
+        """Wait for the calls so far; raise BltError if one of them failed, and clear it."""
+        bits = int(self._status.item())
+        if bits:
+            self._status.zero_()
+            raise BltError("paged cache: " + "; ".join(t for b, t in _FAILURES if bits & b))
+
+    # ---- lists of sequences ---------------------------------------------------
+    def _list(self, t, what, n=None):
+        require_cuda(t)
+        if t.dtype != torch.int32 or t.dim() != 1 or t.device != self.device or \
+                not t.is_contiguous() or (n is not None and t.shape[0] != n):
+            raise BltError("PagedCache: %s must be a contiguous int32 [%s] on %s"
+                           % (what, "n" if n is None else n, self.device))
+        return t.data_ptr()
+
+    def _workspace(self, nbytes):
+        return torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+
+    def reserve(self, counts, seqs=None):
+        """Grow sequence seqs[i] (None: i) by counts[i] tokens; missing pages are the free
+        ones with the lowest index.  All or, with a status bit, none."""
+        c = self._list(counts, "counts")
+        n = counts.shape[0]
+        s = None if seqs is None else self._list(seqs, "seqs", n)
+        call_on(self.device, self._lib.blt_cache_reserve, "cache_reserve", self._ptr, s, c, n)
+
+    def trim(self, lens, seqs=None):
+        """Cut sequence seqs[i] (None: i) to lens[i] tokens where it is longer."""
+        p = self._list(lens, "lens")
+        n = lens.shape[0]
+        s = None if seqs is None else self._list(seqs, "seqs", n)
+        size = self._lib.blt_cache_workspace_bytes(self._ptr, max(n, 1))
+        ws = self._workspace(size)
+        call_on(self.device, self._lib.blt_cache_trim, "cache_trim", self._ptr, s, p, n,
+                ws.data_ptr(), size)
+
+    def free(self, seqs):
+        """Drop sequences: their pages are free where no other sequence shares them."""
+        s = self._list(seqs, "seqs")
+        call_on(self.device, self._lib.blt_cache_trim, "cache_free", self._ptr, s, None,
+                seqs.shape[0], None, 0)
+
+    def fork(self, src, dst):
+        """Make every dst[i] (a sequence without tokens) a continuation of src[i]: full
+        pages are shared, a partly filled last page is copied."""
+        a = self._list(src, "src")
+        n = src.shape[0]
+        b = self._list(dst, "dst", n)
+        size = self._lib.blt_cache_workspace_bytes(self._ptr, max(n, 1))
+        ws = self._workspace(size)
+        call_on(self.device, self._lib.blt_cache_fork, "cache_fork", self._ptr, a, b, n,
+                ws.data_ptr(), size)
+
+    def compact(self):
+        """Move the used pages with the highest indices into the lowest free ones."""
+        size = self._lib.blt_cache_workspace_bytes(self._ptr, 0)
+        ws = self._workspace(size)
+        call_on(self.device, self._lib.blt_cache_compact, "cache_compact", self._ptr,
+                ws.data_ptr(), size)
+
+    def copy_pages(self, src, dst):
+        """Copy page src[i] to page dst[i] in every layer (no index twice in dst, none in
+        both)."""
+        a = self._list(src, "src")
+        b = self._list(dst, "dst", src.shape[0])
+        call_on(self.device, self._lib.blt_cache_copy_pages, "cache_copy_pages", self._ptr, a, b,
+                src.shape[0])
+
+    # ---- tokens ---------------------------------------------------------------
+    def _rows(self, starts, seqs):
+        p = self._list(starts, "starts")
+        B = starts.shape[0] - 1
+        if B < 0:
+            raise BltError("PagedCache: starts has one entry more than there are sequences")
+        return p, B, None if seqs is None else self._list(seqs, "seqs", B)
+
+    def _tokens(self, t, what, heads=None):
+        require_cuda(t)
+        if t.dim() != 3 or t.dtype != self.dtype or t.device != self.device or \
+                t.shape[2] != self.head_dim or (heads is not None and t.shape[1] != heads):
+            raise BltError("PagedCache: %s must be %s [tokens, %s, %d] on %s"
+                           % (what, self.dtype, "heads" if heads is None else heads,
+                              self.head_dim, self.device))
+
+    def append(self, layer, k, v, starts, seqs=None, rotary=None, q=None, out=None):
+        """Write the new tokens k, v [total, kv_heads, head_dim] into a layer: row b has
+        tokens starts[b] .. starts[b + 1] - 1 (int32 [rows + 1]) and they become the last
+        ones of sequence seqs[b] (None: b; none twice), whose length already counts them
+        (reserve).  rotary: a RotaryPlan that rotates k at its positions, and q [total, heads,
+        head_dim] if given, which is returned (into `out`, which may be q)."""
+        Hk, total = self.n_kv_heads, k.shape[0]
+        self._tokens(k, "k", Hk)
+        self._tokens(v, "v", Hk)
+        p, B, s = self._rows(starts, seqs)
+        if v.shape[0] != total:
+            raise BltError("PagedCache: k and v must have one number of tokens")
+        if k.stride(2) != 1:
+            k = k.contiguous()
+        if v.stride(2) != 1:
+            v = v.contiguous()
+        r = None
+        if rotary is not None:
+            if not isinstance(rotary, RotaryPlan):
+                raise TypeError("PagedCache.append expects a RotaryPlan")
+            if rotary.device != self.device:
+                raise BltError("PagedCache: the rotary plan is on another device")
+            r = rotary._ptr
+        qp, qs, op, os_, Hq = None, (0, 0), None, (0, 0), 0
+        if q is not None:
+            if rotary is None:
+                raise BltError("PagedCache.append: q is rotated only with a rotary plan")
+            self._tokens(q, "q")
+            if q.shape[0] != total:
+                raise BltError("PagedCache: q and k must have one number of tokens")
+            if q.stride(2) != 1:
+                q = q.contiguous()
+            Hq = q.shape[1]
+            if out is None:
+                out = torch.empty_like(q)
+            else:
+                self._tokens(out, "out", Hq)
+                if out.shape[0] != total or out.stride(2) != 1:
+                    raise BltError("PagedCache: out must match q, with a dense last dimension")
+            qp, qs, op, os_ = q.data_ptr(), q.stride(), out.data_ptr(), out.stride()
+        elif out is not None:
+            raise BltError("PagedCache.append: out without q")
+        ks, vs = k.stride(), v.stride()
+        call_on(self.device, self._lib.blt_cache_append, "cache_append", self._ptr, layer,
+                k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], qp, qs[0], qs[1], op,
+                os_[0], os_[1], Hq, p, s, B, total, r)
+        return out
+
+    def attention(self, layer, q, starts, seqs=None, causal=True, window=0, scale=None, out=None):
+        """Attention of new tokens q [total, heads, head_dim] over a layer of the cache,
+        whose lengths already count them (rows as in append; a sequence may appear twice):
+        the last of a row's n tokens sits at its sequence's last position.  Query head h
+        reads key head h // (heads / kv_heads).  causal: keys up to the token's own
+        position, with window > 0 only the last `window` of them; causal=False: every
+        key.  scale defaults to head_dim^-0.5.  Returns [total, heads, head_dim] (`out` if
+        given; tokens at starts[-1] and behind are left as they were there)."""
+        self._tokens(q, "q")
+        p, B, s = self._rows(starts, seqs)
+        total, H, d = q.shape
+        if H % self.n_kv_heads or H == 0:
+            raise BltError("PagedCache: q's heads must be a multiple of the cache's %d"
+                           % self.n_kv_heads)
+        es = 16 // q.element_size()
+        st = q.stride()
+        if st[2] != 1 or st[0] % es or st[1] % es or q.data_ptr() % 16:
+            q = q.clone(memory_format=torch.contiguous_format)
+            st = q.stride()
+        if out is None:
+            out = torch.empty((total, H, d), dtype=q.dtype, device=self.device)
+        else:
+            self._tokens(out, "out", H)
+            if out.shape[0] != total or out.stride(2) != 1:
+                raise BltError("PagedCache: out must match q, with a dense last dimension")
+        so = out.stride()
+        size = self._lib.blt_paged_attention_workspace_bytes(self._ptr, B, total, H)
+        ws = self._workspace(size) if size else None
+        call_on(self.device, self._lib.blt_paged_attention, "paged_attention", self._ptr, layer,
+                q.data_ptr(), st[0], st[1], out.data_ptr(), so[0], so[1], H, p, s, B, total,
+                1 if causal else 0, window, d ** -0.5 if scale is None else scale,
+                ws.data_ptr() if size else None, size)
+        return out

@@ -12,6 +12,7 @@
 #include <vector>
 
 #include "model.hpp"
+#include "paged.hpp"
 
 namespace blt {
 
@@ -303,6 +304,236 @@ int blt_rope_table_f32(float* out_device, int32_t head_dim, int32_t max_seqlen, 
                                STREAM(stream)));
   BLT_HIP_CHECK(hipStreamSynchronize(STREAM(stream)));
   return BLT_OK;
+}
+
+// ---- rotary positions --------------------------------------------------------
+int blt_rotary_frequencies(int32_t rotary_dim, double theta, int32_t scaling, double factor,
+                           double original_len, uint64_t* freq, float* magnitude) {
+  if (rotary_dim < 2 || rotary_dim % 2 || rotary_dim > 512)
+    return fail(BLT_ERR_SHAPE, "rotary_frequencies: rotary_dim must be even, 2 .. 512");
+  if (scaling < BLT_ROTARY_NONE || scaling > BLT_ROTARY_YARN)
+    return fail(BLT_ERR_INVALID, "rotary_frequencies: bad scaling");
+  if (!(theta > 1.0) || !(theta < 1e300))
+    return fail(BLT_ERR_SHAPE, "rotary_frequencies: theta must be above 1");
+  if (scaling != BLT_ROTARY_NONE && (!(factor >= 1.0) || !(factor < 1e9)))
+    return fail(BLT_ERR_SHAPE, "rotary_frequencies: factor must be 1 .. 1e9");
+  if (scaling == BLT_ROTARY_NTK && rotary_dim == 2)
+    return fail(BLT_ERR_SHAPE, "rotary_frequencies: NTK scaling needs rotary_dim > 2");
+  if (scaling == BLT_ROTARY_YARN && (!(original_len >= 1.0) || !(original_len < 1e12)))
+    return fail(BLT_ERR_SHAPE, "rotary_frequencies: original_len must be 1 .. 1e12");
+  if (!freq || !magnitude) return fail(BLT_ERR_INVALID, "rotary_frequencies: null pointer");
+  const long double two_pi = 6.283185307179586476925286766559006L;
+  const int half = rotary_dim / 2;
+  long double base = theta;
+  if (scaling == BLT_ROTARY_NTK)
+    base *= powl((long double)factor, (long double)rotary_dim / (rotary_dim - 2));
+  // the pair (a real index) whose wave turns `beta` times over original_len positions
+  auto pair_of = [&](double beta) {
+    return rotary_dim * log(original_len / (beta * (double)two_pi)) / (2.0 * log(theta));
+  };
+  double lo = 0.0, hi = 0.0;
+  if (scaling == BLT_ROTARY_YARN) {
+    lo = std::max(floor(pair_of(32.0)), 0.0);
+    hi = std::min(ceil(pair_of(1.0)), rotary_dim - 1.0);
+  }
+  for (int i = 0; i < half; ++i) {
+    long double f = powl(base, -2.0L * i / rotary_dim);
+    if (scaling == BLT_ROTARY_LINEAR) f /= factor;
+    if (scaling == BLT_ROTARY_YARN) {
+      const double ramp = std::min(1.0, std::max(0.0, (i - lo) / std::max(hi - lo, 0.001)));
+      f = f / factor * ramp + f * (1.0L - ramp);
+    }
+    // f <= 1 radian a position: below a sixth of a turn
+    freq[i] = (uint64_t)(f / two_pi * 18446744073709551616.0L + 0.5L);
+  }
+  *magnitude = scaling == BLT_ROTARY_YARN ? (float)(0.1 * log(factor) + 1.0) : 1.f;
+  return BLT_OK;
+}
+
+static int rotary_checks(const blt_rotary* r, int32_t d, const char* what) {
+  if (!r || !r->freq) return fail(BLT_ERR_INVALID, std::string(what) + ": null rotary table");
+  if (r->rotary_dim < 2 || r->rotary_dim % 2 || r->rotary_dim > d)
+    return fail(BLT_ERR_SHAPE, std::string(what) + ": rotary_dim must be even, 2 .. head_dim");
+  return 0;
+}
+
+int blt_fused_rotary(const void* q, const void* k, void* q_out, void* k_out, int32_t dtype,
+                     int64_t B, int64_t Hq, int64_t Hk, int64_t T, int32_t d, int64_t sb_q,
+                     int64_t sh_q, int64_t st_q, int64_t sb_k, int64_t sh_k, int64_t st_k,
+                     int64_t sb_qo, int64_t sh_qo, int64_t st_qo, int64_t sb_ko, int64_t sh_ko,
+                     int64_t st_ko, const int32_t* positions, int64_t sb_pos,
+                     const blt_rotary* rotary, int32_t backward, blt_stream_t stream) {
+  if (dtype != BLT_DTYPE_F32 && dtype != BLT_DTYPE_BF16)
+    return fail(BLT_ERR_INVALID, "fused_rotary: bad dtype");
+  if (B < 0 || T < 0 || Hq < 0 || Hk < 0 || Hq + Hk > 0xffff)
+    return fail(BLT_ERR_SHAPE, "fused_rotary: negative shape or more than 65535 heads");
+  if (d < 2 || d % 2 || d > 512)
+    return fail(BLT_ERR_SHAPE, "fused_rotary: head_dim must be even, 2 .. 512");
+  if (int rc = rotary_checks(rotary, d, "fused_rotary")) return rc;
+  if (B == 0 || T == 0 || Hq + Hk == 0) return BLT_OK;
+  if (T > 0x7fffffff || B > 0x7fffffff / T)
+    return fail(BLT_ERR_SHAPE, "fused_rotary: B * T must fit int32");
+  if ((Hq > 0 && (!q || !q_out)) || (Hk > 0 && (!k || !k_out)) || !positions)
+    return fail(BLT_ERR_INVALID, "fused_rotary: null pointer");
+  RotaryArgs a{};
+  a.q = RotarySet{q, q_out, (int)Hq, sb_q, sh_q, st_q, sb_qo, sh_qo, st_qo};
+  a.k = RotarySet{k, k_out, (int)Hk, sb_k, sh_k, st_k, sb_ko, sh_ko, st_ko};
+  a.B = B; a.T = T; a.d = d;
+  a.pos = positions; a.sb_pos = sb_pos;
+  a.r = *rotary;
+  a.r.interleaved = rotary->interleaved ? 1 : 0;
+  a.backward = backward ? 1 : 0;
+  return launch_rotary(a, dtype, STREAM(stream));
+}
+
+// ---- paged cache ---------------------------------------------------------------
+static int cache_checks(const blt_paged_cache* c, const char* what) {
+  const std::string w(what);
+  if (!c) return fail(BLT_ERR_INVALID, w + ": null cache");
+  if (c->dtype != BLT_DTYPE_F32 && c->dtype != BLT_DTYPE_BF16)
+    return fail(BLT_ERR_INVALID, w + ": bad cache dtype");
+  if (c->head_dim != 64 && c->head_dim != 128)
+    return fail(BLT_ERR_SHAPE, w + ": head_dim must be 64 or 128");
+  if (c->page_size < 8 || c->page_size > 1024 || (c->page_size & (c->page_size - 1)))
+    return fail(BLT_ERR_SHAPE, w + ": page_size must be a power of two, 8 .. 1024");
+  if (c->n_layers < 1 || c->n_layers > 4096 || c->num_pages < 1 || c->num_pages > (1 << 28) ||
+      c->n_kv_heads < 1 || c->n_kv_heads > 1024 || c->max_seqs < 1 || c->max_seqs > (1 << 20) ||
+      c->max_pages < 1 || c->max_pages > (1 << 20))
+    return fail(BLT_ERR_SHAPE, w + ": cache sizes out of range");
+  if (!c->k || !c->v || !c->page_table || !c->lens || !c->refcount || !c->status)
+    return fail(BLT_ERR_INVALID, w + ": null cache pointer");
+  if (((uintptr_t)c->k | (uintptr_t)c->v) & 15)
+    return fail(BLT_ERR_SHAPE, w + ": k and v must be 16-byte aligned");
+  return 0;
+}
+static int list_checks(const blt_paged_cache* c, int64_t n, const char* what) {
+  if (int rc = cache_checks(c, what)) return rc;
+  if (n < 0 || n > kPageListMax)
+    return fail(BLT_ERR_SHAPE, std::string(what) + ": at most 8192 entries a call");
+  return 0;
+}
+static int workspace_checks(const blt_paged_cache* c, int64_t n, const void* ws, int64_t bytes,
+                            const char* what) {
+  if (!ws || ((uintptr_t)ws & 15) || bytes < cache_workspace_bytes(*c, n))
+    return fail(BLT_ERR_INVALID, std::string(what) + ": workspace missing, misaligned or too small");
+  return 0;
+}
+
+int64_t blt_cache_workspace_bytes(const blt_paged_cache* cache, int64_t n) {
+  return !cache || n < 0 ? 0 : cache_workspace_bytes(*cache, n);
+}
+int blt_cache_reserve(const blt_paged_cache* cache, const int32_t* seqs, const int32_t* counts,
+                      int64_t n, blt_stream_t stream) {
+  if (int rc = list_checks(cache, n, "cache_reserve")) return rc;
+  if (n == 0) return BLT_OK;
+  if (!counts) return fail(BLT_ERR_INVALID, "cache_reserve: null counts");
+  if (!seqs && n > cache->max_seqs)
+    return fail(BLT_ERR_SHAPE, "cache_reserve: more counts than sequences");
+  return launch_cache_reserve(*cache, seqs, counts, n, STREAM(stream));
+}
+int blt_cache_trim(const blt_paged_cache* cache, const int32_t* seqs, const int32_t* new_lens,
+                   int64_t n, void* workspace, int64_t workspace_bytes, blt_stream_t stream) {
+  if (int rc = list_checks(cache, n, "cache_trim")) return rc;
+  if (n == 0) return BLT_OK;
+  if (!seqs && n > cache->max_seqs)
+    return fail(BLT_ERR_SHAPE, "cache_trim: more lengths than sequences");
+  if (new_lens)
+    if (int rc = workspace_checks(cache, n, workspace, workspace_bytes, "cache_trim")) return rc;
+  return launch_cache_trim(*cache, seqs, new_lens, n, workspace, STREAM(stream));
+}
+int blt_cache_fork(const blt_paged_cache* cache, const int32_t* src, const int32_t* dst, int64_t n,
+                   void* workspace, int64_t workspace_bytes, blt_stream_t stream) {
+  if (int rc = list_checks(cache, n, "cache_fork")) return rc;
+  if (n == 0) return BLT_OK;
+  if (!src || !dst) return fail(BLT_ERR_INVALID, "cache_fork: null list");
+  if (int rc = workspace_checks(cache, n, workspace, workspace_bytes, "cache_fork")) return rc;
+  return launch_cache_fork(*cache, src, dst, n, workspace, STREAM(stream));
+}
+int blt_cache_compact(const blt_paged_cache* cache, void* workspace, int64_t workspace_bytes,
+                      blt_stream_t stream) {
+  if (int rc = cache_checks(cache, "cache_compact")) return rc;
+  if (int rc = workspace_checks(cache, 0, workspace, workspace_bytes, "cache_compact")) return rc;
+  return launch_cache_compact(*cache, workspace, STREAM(stream));
+}
+int blt_cache_copy_pages(const blt_paged_cache* cache, const int32_t* src, const int32_t* dst,
+                         int64_t n, blt_stream_t stream) {
+  if (int rc = cache_checks(cache, "cache_copy_pages")) return rc;
+  if (n < 0 || n > 0x7fffffff) return fail(BLT_ERR_SHAPE, "cache_copy_pages: bad count");
+  if (n == 0) return BLT_OK;
+  if (!src || !dst) return fail(BLT_ERR_INVALID, "cache_copy_pages: null list");
+  return launch_cache_copy_pages(*cache, src, dst, n, STREAM(stream));
+}
+
+static int chunk_checks(const blt_paged_cache* c, int32_t layer, int64_t Hq, const int32_t* starts,
+                        int64_t B, int64_t total, const char* what) {
+  const std::string w(what);
+  if (layer < 0 || layer >= c->n_layers) return fail(BLT_ERR_SHAPE, w + ": no such layer");
+  if (B < 0 || B > 65536 || total < 0 || total > 0x7fffffff)
+    return fail(BLT_ERR_SHAPE, w + ": at most 65536 rows and 2^31 - 1 tokens");
+  if (Hq < 0 || Hq > 0xffff || (int64_t)Hq * total > 0x7fffffff)
+    return fail(BLT_ERR_SHAPE, w + ": heads * tokens must fit int32");
+  if (B > 0 && total > 0 && !starts) return fail(BLT_ERR_INVALID, w + ": null starts");
+  return 0;
+}
+
+int blt_cache_append(const blt_paged_cache* cache, int32_t layer, const void* k, int64_t st_k,
+                     int64_t sh_k, const void* v, int64_t st_v, int64_t sh_v, const void* q,
+                     int64_t st_q, int64_t sh_q, void* q_out, int64_t st_qo, int64_t sh_qo,
+                     int64_t Hq, const int32_t* starts, const int32_t* seqs, int64_t B,
+                     int64_t total, const blt_rotary* rotary, blt_stream_t stream) {
+  if (int rc = cache_checks(cache, "cache_append")) return rc;
+  if (int rc = chunk_checks(cache, layer, Hq, starts, B, total, "cache_append")) return rc;
+  if (rotary)
+    if (int rc = rotary_checks(rotary, cache->head_dim, "cache_append")) return rc;
+  if (!rotary && Hq) return fail(BLT_ERR_INVALID, "cache_append: q without rotary has nothing to do");
+  if (!seqs && B > cache->max_seqs)
+    return fail(BLT_ERR_SHAPE, "cache_append: more rows than sequences");
+  if (B == 0 || total == 0) return BLT_OK;
+  if (!k || !v || (Hq && (!q || !q_out))) return fail(BLT_ERR_INVALID, "cache_append: null pointer");
+  AppendArgs a{};
+  a.q = q; a.k = k; a.v = v; a.q_out = q_out; a.Hq = (int)Hq;
+  a.st_q = st_q; a.sh_q = sh_q; a.st_qo = st_qo; a.sh_qo = sh_qo;
+  a.st_k = st_k; a.sh_k = sh_k; a.st_v = st_v; a.sh_v = sh_v;
+  a.starts = starts; a.seqs = seqs; a.B = B; a.total = total; a.layer = layer;
+  if (rotary) {
+    a.r = *rotary;
+    a.r.interleaved = rotary->interleaved ? 1 : 0;
+  }
+  return launch_append(*cache, a, STREAM(stream));
+}
+
+int64_t blt_paged_attention_workspace_bytes(const blt_paged_cache* cache, int64_t B, int64_t total,
+                                            int64_t Hq) {
+  if (!cache || cache->n_kv_heads < 1 || Hq < 0 || B < 0 || total < 0) return 0;
+  return paged_attention_workspace_bytes(*cache, B, total, (int)Hq);
+}
+int blt_paged_attention(const blt_paged_cache* cache, int32_t layer, const void* q, int64_t st_q,
+                        int64_t sh_q, void* o, int64_t st_o, int64_t sh_o, int64_t Hq,
+                        const int32_t* starts, const int32_t* seqs, int64_t B, int64_t total,
+                        int32_t causal, int32_t window, float scale, void* workspace,
+                        int64_t workspace_bytes, blt_stream_t stream) {
+  if (int rc = cache_checks(cache, "paged_attention")) return rc;
+  if (int rc = chunk_checks(cache, layer, Hq, starts, B, total, "paged_attention")) return rc;
+  if (Hq < 1 || Hq % cache->n_kv_heads)
+    return fail(BLT_ERR_SHAPE, "paged_attention: heads must be a multiple of the cache's");
+  if (window < 0) return fail(BLT_ERR_SHAPE, "paged_attention: window must be >= 0");
+  if (!(scale > 0.f) || !(scale < 1e30f))
+    return fail(BLT_ERR_SHAPE, "paged_attention: scale must be positive and finite");
+  if (!seqs && B > cache->max_seqs)
+    return fail(BLT_ERR_SHAPE, "paged_attention: more rows than sequences");
+  if (B == 0 || total == 0) return BLT_OK;
+  if (!q || !o) return fail(BLT_ERR_INVALID, "paged_attention: null pointer");
+  const int64_t v = cache->dtype == BLT_DTYPE_BF16 ? 8 : 4;
+  if (((uintptr_t)q & 15) || ((uintptr_t)o & 15) || st_q % v || sh_q % v || st_o % v || sh_o % v)
+    return fail(BLT_ERR_SHAPE, "paged_attention: q and o need 16-byte aligned rows");
+  const int64_t need = paged_attention_workspace_bytes(*cache, B, total, (int)Hq);
+  if (need > 0 && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need))
+    return fail(BLT_ERR_INVALID, "paged_attention: workspace missing, misaligned or too small");
+  PagedAttnArgs a{};
+  a.q = q; a.o = o; a.st_q = st_q; a.sh_q = sh_q; a.st_o = st_o; a.sh_o = sh_o;
+  a.H = (int)Hq; a.starts = starts; a.seqs = seqs; a.B = B; a.total = total;
+  a.layer = layer; a.causal = causal ? 1 : 0; a.window = window; a.scale = scale;
+  return launch_paged_attention(*cache, a, workspace, STREAM(stream));
 }
 
 // ---- patcher -----------------------------------------------------------------

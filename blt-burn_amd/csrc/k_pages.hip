@@ -1,0 +1,480 @@
+// Page maintenance of the paged cache: reserve, trim, fork, compact, copy.
+//
+// All bookkeeping is on the device (page table, lengths, reference counts), so a
+// decode step can grow, branch and drop sequences without the host.  What has to
+// be decided in order (which free page goes to whom) is one block of 1024 threads
+// walking the reference counts with a block scan: latency-bound, a few us up to
+// some ten thousand pages.  What moves data (page contents of every layer, the shared
+// rows of the table) is a second kernel over many blocks that reads the first one's
+// list.  Free pages are always taken lowest index first, so results do not depend
+// on timing.
+//
+// Lengths hold a claim in their sign bit while a call runs: the first entry that sets
+// it owns the sequence, so a sequence listed twice is seen, not raced on.
+#include "paged.hpp"
+
+namespace blt {
+
+namespace {
+
+constexpr int NT = 1024;     // threads of a bookkeeping block
+constexpr int PER = 4;       // reference counts a thread reads per step
+constexpr int CLAIM = (int)0x80000000;
+
+// Workspace words: [0] number of copies; then three lists of `cap` words (source page,
+// destination page, tokens to copy) and, for compact, the page map.
+struct Lists {
+  int32_t* count;
+  int32_t *src, *dst, *fill, *map;
+};
+inline int64_t list_cap(const blt_paged_cache& c, int64_t n) {
+  return n > 0 ? n : (int64_t)c.num_pages / 2 + 1;
+}
+inline Lists lists_of(const blt_paged_cache& c, int64_t n, void* ws) {
+  int32_t* w = reinterpret_cast<int32_t*>(ws);
+  const int64_t cap = list_cap(c, n);
+  return Lists{w, w + 16, w + 16 + cap, w + 16 + 2 * cap, w + 16 + 3 * cap};
+}
+
+// Exclusive sum over the block's threads; `total` is the block's.  `part`: NT / 64 + 1
+// words of LDS.  Two barriers.
+__device__ inline int block_excl(int v, int* part, int& total) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int inc = wave_incl_scan(v);
+  if (lane == 63) part[w] = inc;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int i = 0; i < NT / 64; ++i) {
+    const int x = part[i];
+    before += i < w ? x : 0;
+    all += x;
+  }
+  __syncthreads();
+  total = all;
+  return before + inc - v;
+}
+
+// Walk the reference counts in ascending order of page until f has been called for
+// `most` free pages (or `used` ones, FREE false): f(page, ordinal).  Returns how many
+// there were, at most those of the step that reached `most`.
+template <bool FREE, typename F>
+__device__ int walk_pages(const int32_t* ref, int P, int most, int* part, F f) {
+  int seen = 0;
+  for (int p0 = 0; p0 < P && seen < most; p0 += NT * PER) {
+    const int p = p0 + (int)threadIdx.x * PER;
+    int hit[PER], mine = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      hit[i] = p + i < P && (FREE ? ref[p + i] == 0 : ref[p + i] != 0) ? 1 : 0;
+      mine += hit[i];
+    }
+    int total;
+    int at = seen + block_excl(mine, part, total);
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (hit[i]) {
+        if (at < most) f(p + i, at);
+        ++at;
+      }
+    seen += total;
+  }
+  return seen;
+}
+
+__device__ inline int pages_of(int tokens, int lps) {
+  return (int)(((int64_t)tokens + (1 << lps) - 1) >> lps);
+}
+
+// ---- reserve -------------------------------------------------------------------
+__global__ __launch_bounds__(NT) void reserve_kernel(blt_paged_cache c, int lps,
+                                                     const int32_t* seqs, const int32_t* counts,
+                                                     int n) {
+  __shared__ int first[kPageListMax + 1];  // pages wanted by the entries before
+  __shared__ int part[NT / 64];
+  __shared__ int bad;
+  const int tid = threadIdx.x;
+  if (tid == 0) bad = *c.status & kCachePending ? -1 : 0;
+  __syncthreads();
+  if (bad) return;
+  int need_all = 0;
+  for (int i0 = 0; i0 < n; i0 += NT) {
+    const int i = i0 + tid;
+    int need = 0, err = 0;
+    if (i < n) {
+      const int s = seqs ? seqs[i] : i, cnt = counts[i];
+      if (s < 0 || s >= c.max_seqs || cnt < 0) {
+        err = BLT_CACHE_BAD_INDEX;
+      } else {
+        const int old = atomicOr(&c.lens[s], CLAIM);
+        const int len = old & ~CLAIM;
+        if (old & CLAIM) err = BLT_CACHE_BUSY;
+        const int64_t want = ((int64_t)len + cnt + (1 << lps) - 1) >> lps;
+        if (want > c.max_pages) err |= BLT_CACHE_TOO_LONG;
+        else need = (int)want - pages_of(len, lps);
+      }
+    }
+    if (err) atomicOr(&bad, err);
+    int total;
+    const int at = block_excl(need, part, total);
+    if (i < n) first[i] = need_all + at;
+    // past any pool: too many for this call, and no overflow
+    need_all = total > c.num_pages - need_all ? c.num_pages + 1 : need_all + total;
+  }
+  if (tid == 0) first[n] = need_all;
+  __syncthreads();
+  if (!bad && need_all > 0) {
+    const int have = walk_pages<true>(c.refcount, c.num_pages, need_all, part, [](int, int) {});
+    if (have < need_all && tid == 0) bad = BLT_CACHE_FULL;
+    __syncthreads();
+    if (!bad)
+      walk_pages<true>(c.refcount, c.num_pages, need_all, part, [&](int page, int o) {
+        int lo = 0, hi = n;  // the last entry with first[entry] <= o
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          if (first[mid] <= o) lo = mid; else hi = mid;
+        }
+        const int s = seqs ? seqs[lo] : lo;
+        const int col = pages_of(c.lens[s] & ~CLAIM, lps) + o - first[lo];
+        c.page_table[(int64_t)s * c.max_pages + col] = page;
+        c.refcount[page] = 1;
+      });
+  }
+  __syncthreads();
+  for (int i = tid; i < n; i += NT) {
+    const int s = seqs ? seqs[i] : i;
+    if (s < 0 || s >= c.max_seqs) continue;
+    if (bad) atomicAnd(&c.lens[s], ~CLAIM);
+    else c.lens[s] = (c.lens[s] & ~CLAIM) + counts[i];
+  }
+  if (bad && tid == 0) atomicOr(c.status, bad);
+}
+
+// ---- copies --------------------------------------------------------------------
+// The listed pages' first fill[i] tokens (fill NULL: all), in every layer, k and v: 16
+// bytes a lane, four in flight.  A fixed grid walks (pair, layer, k or v).
+__device__ inline void copy_tokens(const blt_paged_cache& c, int64_t src, int64_t dst, int fill,
+                                   int layer, int kv, int es) {
+  const int64_t page_b = (int64_t)c.n_kv_heads * c.page_size * c.head_dim * es;
+  const int64_t head_b = (int64_t)c.page_size * c.head_dim * es;
+  char* base = reinterpret_cast<char*>(kv ? c.v : c.k) + (int64_t)layer * c.num_pages * page_b;
+  const char* from = base + src * page_b;
+  char* to = base + dst * page_b;
+  const int row = fill * c.head_dim * es / 16;  // 16-byte pieces of a head
+  const int all = row * c.n_kv_heads;
+  const bool whole = fill == c.page_size;
+  auto off = [&](int i) -> int64_t {
+    return whole ? (int64_t)i * 16 : (i / row) * head_b + (int64_t)(i % row) * 16;
+  };
+  constexpr int U = 4;
+  for (int i = threadIdx.x; i < all; i += U * 256) {
+    u32x4_t x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i + u * 256 < all) x[u] = *reinterpret_cast<const u32x4_t*>(from + off(i + u * 256));
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i + u * 256 < all) *reinterpret_cast<u32x4_t*>(to + off(i + u * 256)) = x[u];
+  }
+}
+__device__ inline void copy_listed(const blt_paged_cache& c, const Lists& l, int es) {
+  const int64_t items = (int64_t)*l.count * c.n_layers * 2;
+  for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
+    const int64_t i = it / (c.n_layers * 2);
+    const int r = (int)(it - i * (c.n_layers * 2));
+    copy_tokens(c, l.src[i], l.dst[i], l.fill ? l.fill[i] : c.page_size, r >> 1, r & 1, es);
+  }
+}
+__global__ __launch_bounds__(256) void copy_list_kernel(blt_paged_cache c, Lists l, int es) {
+  copy_listed(c, l, es);
+}
+__global__ __launch_bounds__(256) void copy_pages_kernel(blt_paged_cache c, const int32_t* src,
+                                                         const int32_t* dst, int64_t n, int es) {
+  const int64_t items = n * c.n_layers * 2;
+  for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
+    const int64_t i = it / (c.n_layers * 2);
+    const int r = (int)(it - i * (c.n_layers * 2));
+    const int a = src[i], b = dst[i];
+    if (a < 0 || a >= c.num_pages || b < 0 || b >= c.num_pages) {
+      if (r == 0 && threadIdx.x == 0) atomicOr(c.status, BLT_CACHE_BAD_INDEX);
+      continue;
+    }
+    if (a != b) copy_tokens(c, a, b, c.page_size, r >> 1, r & 1, es);
+  }
+}
+
+// ---- fork ----------------------------------------------------------------------
+// Decides: the free page of every pair whose source ends inside a page.  dst[i] is
+// claimed by CLAIM, src may repeat.  l.dst[i] of pair i = its page; the copy list is dense.
+__global__ __launch_bounds__(NT) void fork_kernel(blt_paged_cache c, int lps, const int32_t* src,
+                                                  const int32_t* dst, int n, Lists l) {
+  __shared__ int first[kPageListMax];  // partial pages of the pairs before
+  __shared__ int part[NT / 64];
+  __shared__ int bad;
+  const int tid = threadIdx.x, mask = c.page_size - 1;
+  if (tid == 0) {
+    bad = *c.status & kCachePending ? -1 : 0;
+    *l.count = 0;
+  }
+  __syncthreads();
+  if (bad) return;
+  auto known = [&](int s) { return s >= 0 && s < c.max_seqs; };
+  int need_all = 0;
+  for (int i0 = 0; i0 < n; i0 += NT) {
+    const int i = i0 + tid;
+    int need = 0, err = 0;
+    if (i < n) {
+      const int a = src[i], b = dst[i];
+      if (!known(a) || !known(b)) {
+        err = BLT_CACHE_BAD_INDEX;
+      } else {
+        if (atomicOr(&c.lens[b], CLAIM) != 0) err = BLT_CACHE_BUSY;  // has tokens, or is claimed
+        const int len = c.lens[a] & ~CLAIM;
+        need = len & mask ? 1 : 0;
+      }
+    }
+    if (err) atomicOr(&bad, err);
+    int total;
+    const int at = block_excl(need, part, total);
+    if (i < n) first[i] = need_all + at;
+    need_all += total;
+  }
+  __syncthreads();
+  // no source may be a destination of the same call (read past the L1 cache)
+  for (int i = tid; i < n; i += NT)
+    if (known(src[i]) && (atomicOr(&c.lens[src[i]], 0) & CLAIM)) atomicOr(&bad, BLT_CACHE_BUSY);
+  __syncthreads();
+  if (!bad && need_all > 0) {
+    const int have = walk_pages<true>(c.refcount, c.num_pages, need_all, part,
+                                      [&](int page, int o) { l.dst[o] = page; });
+    if (have < need_all && tid == 0) bad = BLT_CACHE_FULL;
+    __syncthreads();
+    if (!bad) {
+      for (int o = tid; o < need_all; o += NT) c.refcount[l.dst[o]] = 1;
+      for (int i = tid; i < n; i += NT) {
+        const int len = c.lens[src[i]] & ~CLAIM;
+        if (!(len & mask)) continue;
+        const int o = first[i], col = len >> lps;
+        const int page = c.page_table[(int64_t)src[i] * c.max_pages + col];
+        l.src[o] = page < 0 ? 0 : page < c.num_pages ? page : c.num_pages - 1;
+        l.fill[o] = len & mask;
+        c.page_table[(int64_t)dst[i] * c.max_pages + col] = l.dst[o];
+      }
+      if (tid == 0) *l.count = need_all;
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < n; i += NT) {
+    if (!known(dst[i])) continue;
+    if (bad) atomicAnd(&c.lens[dst[i]], ~CLAIM);
+    else c.lens[dst[i]] = c.lens[src[i]];
+  }
+  if (bad && tid == 0) atomicOr(c.status, bad);
+}
+// Shares the full pages (one wave per pair and 64 columns) and copies the partial ones.
+__global__ __launch_bounds__(256) void fork_copy_kernel(blt_paged_cache c, int lps,
+                                                        const int32_t* src, const int32_t* dst,
+                                                        int n, Lists l, int es) {
+  if (*c.status & kCachePending) return;
+  const int64_t threads = (int64_t)gridDim.x * 256;
+  const int cols = c.max_pages;
+  for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < (int64_t)n * cols; x += threads) {
+    const int i = (int)(x / cols), col = (int)(x - (int64_t)i * cols);
+    if (col >= c.lens[dst[i]] >> lps) continue;
+    const int page = c.page_table[(int64_t)src[i] * c.max_pages + col];
+    c.page_table[(int64_t)dst[i] * c.max_pages + col] = page;
+    if (page >= 0 && page < c.num_pages) atomicAdd(&c.refcount[page], 1);
+  }
+  copy_listed(c, l, es);
+}
+
+// ---- trim ----------------------------------------------------------------------
+// One block per entry.  atomicMin hands every entry the length before it, so a
+// sequence listed twice frees each of its pages once.
+__global__ __launch_bounds__(256) void trim_kernel(blt_paged_cache c, int lps, const int32_t* seqs,
+                                                   const int32_t* lens) {
+  __shared__ int old_len;
+  const int i = blockIdx.x;
+  const int s = seqs ? seqs[i] : i, want = lens ? lens[i] : 0;
+  if (s < 0 || s >= c.max_seqs || want < 0) {
+    if (threadIdx.x == 0) atomicOr(c.status, BLT_CACHE_BAD_INDEX);
+    return;
+  }
+  if (threadIdx.x == 0) old_len = atomicMin(&c.lens[s], want);
+  __syncthreads();
+  int hi = pages_of(old_len, lps);
+  if (hi > c.max_pages) hi = c.max_pages;
+  for (int col = pages_of(want, lps) + threadIdx.x; col < hi; col += 256) {
+    const int page = c.page_table[(int64_t)s * c.max_pages + col];
+    if (page >= 0 && page < c.num_pages) atomicSub(&c.refcount[page], 1);
+  }
+}
+// Sequences that now end inside a page that others use get a copy of it.  Those
+// sharers that were cut into the same page in one call each get their own.
+__global__ __launch_bounds__(NT) void trim_split_kernel(blt_paged_cache c, int lps,
+                                                        const int32_t* seqs, int n, Lists l) {
+  __shared__ int first[kPageListMax];  // splits of the entries before; -1: no split
+  __shared__ int part[NT / 64];
+  const int tid = threadIdx.x, mask = c.page_size - 1;
+  auto entry = [&](int64_t s, int len) {
+    const int page = c.page_table[s * c.max_pages + (len >> lps)];
+    return page >= 0 && page < c.num_pages ? page : -1;
+  };
+  int need_all = 0;
+  for (int i0 = 0; i0 < n; i0 += NT) {
+    const int i = i0 + tid;
+    int need = 0;
+    if (i < n) {
+      const int s = seqs ? seqs[i] : i;
+      if (s >= 0 && s < c.max_seqs) {
+        const int old = atomicOr(&c.lens[s], CLAIM);
+        if (!(old & CLAIM) && (old & mask) && (old >> lps) < c.max_pages) {
+          const int page = entry(s, old);
+          need = page >= 0 && c.refcount[page] > 1 ? 1 : 0;
+        }
+      }
+    }
+    int total;
+    const int at = block_excl(need, part, total);
+    if (i < n) first[i] = need ? need_all + at : -1;
+    need_all += total;
+  }
+  __syncthreads();
+  int have = 0;
+  if (need_all > 0)
+    have = walk_pages<true>(c.refcount, c.num_pages, need_all, part,
+                            [&](int page, int o) { l.dst[o] = page; });
+  if (have > need_all) have = need_all;
+  __syncthreads();
+  for (int o = tid; o < have; o += NT) c.refcount[l.dst[o]] = 1;
+  for (int i = tid; i < n; i += NT) {
+    const int o = first[i];
+    if (o < 0) continue;
+    const int s = seqs ? seqs[i] : i;
+    const int len = c.lens[s] & ~CLAIM;
+    const int page = entry(s, len);
+    atomicSub(&c.refcount[page], 1);
+    if (o < have) {
+      l.src[o] = page;
+      l.fill[o] = len & mask;
+      c.page_table[(int64_t)s * c.max_pages + (len >> lps)] = l.dst[o];
+    } else {
+      atomicExch(&c.lens[s], (len & ~mask) | CLAIM);
+    }
+  }
+  if (tid == 0) {
+    *l.count = have;
+    if (have < need_all) atomicOr(c.status, BLT_CACHE_FULL);
+  }
+  __syncthreads();
+  for (int i = tid; i < n; i += NT) {
+    const int s = seqs ? seqs[i] : i;
+    if (s >= 0 && s < c.max_seqs) atomicAnd(&c.lens[s], ~CLAIM);
+  }
+}
+
+// ---- compact -------------------------------------------------------------------
+__global__ __launch_bounds__(NT) void compact_kernel(blt_paged_cache c, Lists l) {
+  __shared__ int part[NT / 64];
+  const int tid = threadIdx.x, P = c.num_pages;
+  const int live = walk_pages<false>(c.refcount, P, P, part, [](int, int) {});
+  // holes: free pages below `live`; as many used ones lie above it
+  const int holes = walk_pages<true>(c.refcount, live, P, part,
+                                     [&](int page, int o) { l.dst[o] = page; });
+  walk_pages<false>(c.refcount + live, P - live, P, part,
+                    [&](int page, int o) { l.src[o] = page + live; });
+  __syncthreads();
+  for (int o = tid; o < holes; o += NT) {
+    const int from = l.src[o], to = l.dst[o];
+    c.refcount[to] = c.refcount[from];
+    c.refcount[from] = 0;
+    l.map[from] = to;
+    l.fill[o] = c.page_size;
+  }
+  if (tid == 0) {
+    l.count[0] = holes;
+    l.count[1] = live;
+  }
+}
+__global__ __launch_bounds__(256) void compact_copy_kernel(blt_paged_cache c, int lps, Lists l,
+                                                           int es) {
+  if (*l.count == 0) return;
+  const int live = l.count[1];
+  const int64_t threads = (int64_t)gridDim.x * 256, cols = c.max_pages;
+  for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < c.max_seqs * cols; x += threads) {
+    const int64_t s = x / cols;
+    if (x - s * cols >= pages_of(c.lens[s], lps)) continue;
+    const int page = c.page_table[x];
+    if (page >= live && page < c.num_pages) c.page_table[x] = l.map[page];
+  }
+  copy_listed(c, l, es);
+}
+
+constexpr int kCopyBlocks = 2048;  // eight 256-thread blocks on each of 256 CUs
+
+}  // namespace
+
+int64_t cache_workspace_bytes(const blt_paged_cache& c, int64_t n) {
+  return (16 + 3 * list_cap(c, n) + (n > 0 ? 0 : (int64_t)c.num_pages)) * 4;
+}
+
+int launch_cache_reserve(const blt_paged_cache& c, const int32_t* seqs, const int32_t* counts,
+                         int64_t n, hipStream_t s) {
+  hipLaunchKernelGGL(reserve_kernel, dim3(1), dim3(NT), 0, s, c, log2_of(c.page_size), seqs,
+                     counts, (int)n);
+  BLT_LAUNCH_CHECK("reserve_kernel");
+  return 0;
+}
+
+inline int elem_size(const blt_paged_cache& c) { return c.dtype == BLT_DTYPE_BF16 ? 2 : 4; }
+inline unsigned copy_blocks(const blt_paged_cache& c, int64_t pairs) {
+  const int64_t items = pairs * c.n_layers * 2;
+  return (unsigned)(items < 1 ? 1 : items < kCopyBlocks ? items : kCopyBlocks);
+}
+
+int launch_cache_trim(const blt_paged_cache& c, const int32_t* seqs, const int32_t* lens,
+                      int64_t n, void* ws, hipStream_t s) {
+  const int lps = log2_of(c.page_size);
+  hipLaunchKernelGGL(trim_kernel, dim3((unsigned)n), dim3(256), 0, s, c, lps, seqs, lens);
+  BLT_LAUNCH_CHECK("trim_kernel");
+  if (lens == nullptr) return 0;
+  const Lists l = lists_of(c, n, ws);
+  hipLaunchKernelGGL(trim_split_kernel, dim3(1), dim3(NT), 0, s, c, lps, seqs, (int)n, l);
+  BLT_LAUNCH_CHECK("trim_split_kernel");
+  hipLaunchKernelGGL(copy_list_kernel, dim3(copy_blocks(c, n)), dim3(256), 0, s, c, l,
+                     elem_size(c));
+  BLT_LAUNCH_CHECK("copy_list_kernel");
+  return 0;
+}
+
+int launch_cache_fork(const blt_paged_cache& c, const int32_t* src, const int32_t* dst, int64_t n,
+                      void* ws, hipStream_t s) {
+  const int lps = log2_of(c.page_size);
+  const Lists l = lists_of(c, n, ws);
+  hipLaunchKernelGGL(fork_kernel, dim3(1), dim3(NT), 0, s, c, lps, src, dst, (int)n, l);
+  BLT_LAUNCH_CHECK("fork_kernel");
+  hipLaunchKernelGGL(fork_copy_kernel, dim3(copy_blocks(c, n)), dim3(256), 0, s, c, lps, src, dst,
+                     (int)n, l, elem_size(c));
+  BLT_LAUNCH_CHECK("fork_copy_kernel");
+  return 0;
+}
+
+int launch_cache_compact(const blt_paged_cache& c, void* ws, hipStream_t s) {
+  const Lists l = lists_of(c, 0, ws);
+  hipLaunchKernelGGL(compact_kernel, dim3(1), dim3(NT), 0, s, c, l);
+  BLT_LAUNCH_CHECK("compact_kernel");
+  hipLaunchKernelGGL(compact_copy_kernel, dim3(copy_blocks(c, c.num_pages / 2)), dim3(256), 0, s, c,
+                     log2_of(c.page_size), l, elem_size(c));
+  BLT_LAUNCH_CHECK("compact_copy_kernel");
+  return 0;
+}
+
+int launch_cache_copy_pages(const blt_paged_cache& c, const int32_t* src, const int32_t* dst,
+                            int64_t n, hipStream_t s) {
+  hipLaunchKernelGGL(copy_pages_kernel, dim3(copy_blocks(c, n)), dim3(256), 0, s, c, src, dst, n,
+                     elem_size(c));
+  BLT_LAUNCH_CHECK("copy_pages_kernel");
+  return 0;
+}
+
+}  // namespace blt

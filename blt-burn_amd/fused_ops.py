@@ -6,15 +6,17 @@ and runs one gfx950 kernel through libblt_hip.so on the current stream.
 Inputs are f32 (Burn's default float) or bf16.  Shape mismatches raise
 (where the reference panics).
 """
+import ctypes
+
 import torch
 
 from . import _lib
 from ._lib import EPS_AFTER_SQRT, EPS_INSIDE_SQRT, BltError, check
-from ._torch import contiguous, require_cuda, stream_ptr
+from ._torch import call_on, contiguous, require_cuda, stream_ptr
 
 __all__ = ["fused_entropy", "fused_rms_norm", "fused_softmax", "fused_l2_norm",
-           "fused_silu_gate", "fused_coherence", "fused_attention", "EPS_AFTER_SQRT",
-           "EPS_INSIDE_SQRT"]
+           "fused_silu_gate", "fused_coherence", "fused_attention", "RotaryPlan", "fused_rotary",
+           "EPS_AFTER_SQRT", "EPS_INSIDE_SQRT"]
 
 
 def _dtype_ok(t):
@@ -171,3 +173,98 @@ def fused_attention(q, k, v, use_causal_mask, window=0, rope_theta=0.0):
         float(rope_theta), ws.data_ptr() if ws is not None else 0, stream_ptr(qb.device)),
         "fused_attention")
     return o if in_dtype == torch.bfloat16 else o.to(in_dtype)
+
+
+class RotaryPlan:
+    """The frequencies of rotary positions, computed once and kept on a device.
+
+    The first rotary_dim values of a head are rotated, in pairs (i, i + rotary_dim / 2)
+    (pairs "half", the model's, model.rs:107-147) or (2 i, 2 i + 1) ("interleaved"), by
+    the angles position * theta^(-2 i / rotary_dim).  Angles hold for any int32
+    position; there is no table to outgrow.  scaling stretches them for contexts
+    longer than a model was trained on (original_len positions, by `factor`):
+      "linear"  every frequency divided by factor
+      "ntk"     theta times factor^(rotary_dim / (rotary_dim - 2))
+      "yarn"    high frequencies kept, low ones divided, a ramp between, and the
+                rotated values times 0.1 ln(factor) + 1"""
+
+    def __init__(self, rotary_dim, theta=10000.0, pairs="half", scaling="none", factor=1.0,
+                 original_len=8192, device=None):
+        if pairs not in ("half", "interleaved"):
+            raise BltError("RotaryPlan: pairs must be 'half' or 'interleaved'")
+        if scaling not in _lib.ROTARY_SCALING:
+            raise BltError("RotaryPlan: scaling must be one of %s" % sorted(_lib.ROTARY_SCALING))
+        n = int(rotary_dim)
+        freq = torch.zeros(max(n // 2, 1), dtype=torch.int64)
+        mag = ctypes.c_float()
+        check(_lib.lib().blt_rotary_frequencies(n, float(theta), _lib.ROTARY_SCALING[scaling],
+                                                float(factor), float(original_len),
+                                                freq.data_ptr(), ctypes.addressof(mag)),
+              "rotary_frequencies")
+        dev = torch.device("cuda" if device is None else device)
+        if dev.index is None:
+            dev = torch.device("cuda", torch.cuda.current_device())
+        self.rotary_dim, self.magnitude, self.device = n, mag.value, dev
+        self.freq = freq.to(dev)
+        self._desc = _lib.Rotary(self.freq.data_ptr(), n, 1 if pairs == "interleaved" else 0,
+                                 mag.value)
+        self._ptr = ctypes.addressof(self._desc)
+
+
+def _unit_stride(t):
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def fused_rotary(q, k, positions, plan, backward=False, out=None):
+    """Rotary positions of q [batch, heads, seq, head_dim] and k (its own number of
+    heads; may be None) in one launch: (q', k').  Any strides with a dense last
+    dimension are read as they are, e.g. views into a packed QKV tensor.
+    positions: int32 [seq] or [batch, seq].  backward=True applies the transposed
+    rotation, which turns gradients of q', k' into those of q, k.  out: (q', k') to
+    write, which may be q and k themselves; other overlaps are not allowed."""
+    require_cuda(q, positions)
+    _dtype_ok(q)
+    if not isinstance(plan, RotaryPlan):
+        raise TypeError("fused_rotary expects a RotaryPlan")
+    if q.dim() != 4:
+        raise BltError("fused_rotary expects q [batch, heads, seq, head_dim]")
+    B, Hq, T, d = q.shape
+    dev = q.device
+    Hk = 0
+    if k is not None:
+        require_cuda(k)
+        if k.dim() != 4 or k.dtype != q.dtype or (k.shape[0], k.shape[2], k.shape[3]) != (B, T, d):
+            raise BltError("fused_rotary: k must be [batch, kv_heads, seq, head_dim] of q's dtype")
+        Hk = k.shape[1]
+    if positions.dtype != torch.int32 or tuple(positions.shape) not in ((T,), (B, T)):
+        raise BltError("fused_rotary: positions must be int32 [seq] or [batch, seq]")
+    if plan.device != dev or positions.device != dev or (k is not None and k.device != dev):
+        raise BltError("fused_rotary: tensors and plan must be on one device")
+    pos = positions if positions.stride(-1) == 1 else positions.contiguous()
+    x = _unit_stride(q)
+    y = _unit_stride(k) if k is not None else None
+    if out is None:
+        qo = torch.empty_like(x)
+        ko = torch.empty_like(y) if y is not None else None
+    else:
+        qo, ko = out
+        if (ko is None) != (k is None):
+            raise BltError("fused_rotary: out must hold a k exactly when k is given")
+        for a, b in ((qo, q), (ko, k)):
+            if b is None:
+                continue
+            require_cuda(a)
+            if not (a.shape == b.shape and a.dtype == b.dtype and a.device == dev and
+                    (a.stride(-1) == 1 or d == 1)):
+                raise BltError("fused_rotary: out tensors must match q and k, with a dense last "
+                               "dimension")
+    xs, qs = x.stride(), qo.stride()
+    ys, ks = (y.stride(), ko.stride()) if y is not None else ((0,) * 4, (0,) * 4)
+    call_on(dev, _lib.lib().blt_fused_rotary, "fused_rotary", x.data_ptr(),
+            y.data_ptr() if y is not None else None, qo.data_ptr(),
+            ko.data_ptr() if y is not None else None,
+            _lib.DTYPE_BF16 if q.dtype == torch.bfloat16 else _lib.DTYPE_F32, B, Hq, Hk, T, d,
+            xs[0], xs[1], xs[2], ys[0], ys[1], ys[2], qs[0], qs[1], qs[2], ks[0], ks[1], ks[2],
+            pos.data_ptr(), pos.stride(0) if pos.dim() == 2 else 0, plan._ptr,
+            1 if backward else 0)
+    return qo, ko

@@ -136,6 +136,151 @@ int blt_fused_attention_f32(const float* q, const float* k, const float* v, floa
 int blt_rope_table_f32(float* out_device, int32_t head_dim, int32_t max_seqlen, double theta,
                        blt_stream_t stream);
 
+/* Rotary positions, the paged cache and attention over it: the incremental form
+ * of the entropy model's attention (no counterpart in the reference, which runs
+ * whole rows, model.rs:620-672). ------------------------------------------- */
+
+typedef enum blt_dtype { BLT_DTYPE_F32 = 0, BLT_DTYPE_BF16 = 1 } blt_dtype;
+
+typedef enum blt_rotary_scaling {
+  BLT_ROTARY_NONE = 0,
+  BLT_ROTARY_LINEAR = 1, /* every frequency divided by factor */
+  BLT_ROTARY_NTK = 2,    /* theta times factor^(rotary_dim / (rotary_dim - 2)) */
+  BLT_ROTARY_YARN = 3    /* per frequency: kept where its wave turns 32 times or more over
+                          * original_len, divided by factor where it turns at most once, a
+                          * linear ramp over the pair index between; the rotated values
+                          * times 0.1 ln(factor) + 1 */
+} blt_rotary_scaling;
+
+/* Rotary frequencies, computed on the host: freq[i] = theta^(-2 i / rotary_dim)
+ * (scaled) in turns per position, as 64-bit fractions of a turn (2^64 = 1 turn),
+ * so that position * freq modulo 2^64 is the angle of any position to 2^-33 of a
+ * turn.  freq [rotary_dim / 2] and magnitude are host memory. */
+int blt_rotary_frequencies(int32_t rotary_dim, double theta, int32_t scaling, double factor,
+                           double original_len, uint64_t* freq, float* magnitude);
+
+typedef struct blt_rotary {
+  const uint64_t* freq; /* device, [rotary_dim / 2], from blt_rotary_frequencies */
+  int32_t rotary_dim;   /* the first rotary_dim values of a head are rotated; even */
+  int32_t interleaved;  /* pairs: 0 = (i, i + rotary_dim / 2), model.rs:107-147; 1 = (2 i, 2 i + 1) */
+  float magnitude;      /* factor on the rotated values */
+} blt_rotary;
+
+/* q [B, Hq, T, d] and k [B, Hk, T, d] rotated by the angles of their positions into
+ * q_out and k_out; any (b, h, t) strides in elements with unit d-stride.  k and
+ * k_out may both be NULL with Hk = 0.  An output may be its input itself (the
+ * same pointer and strides); no other overlap.  positions: int32, token t of row
+ * b at positions[b * sb_pos + t] (sb_pos 0: one row of positions for all); any
+ * value.  backward: the transposed rotation, which turns gradients of the outputs
+ * into gradients of the inputs.  Angles to 2^-32 of a turn, products in f32. */
+int blt_fused_rotary(const void* q, const void* k, void* q_out, void* k_out, int32_t dtype,
+                     int64_t B, int64_t Hq, int64_t Hk, int64_t T, int32_t d, int64_t sb_q,
+                     int64_t sh_q, int64_t st_q, int64_t sb_k, int64_t sh_k, int64_t st_k,
+                     int64_t sb_qo, int64_t sh_qo, int64_t st_qo, int64_t sb_ko, int64_t sh_ko,
+                     int64_t st_ko, const int32_t* positions, int64_t sb_pos,
+                     const blt_rotary* rotary, int32_t backward, blt_stream_t stream);
+
+/* A cache of keys and values in pages of page_size tokens, for several layers and
+ * sequences.  All pointers are caller-owned device memory:
+ *   k, v       [n_layers, num_pages, n_kv_heads, page_size, head_dim], 16-byte aligned
+ *   page_table [max_seqs, max_pages]: page of tokens page_size * c .. of sequence s;
+ *              only the entries below ceil(lens[s] / page_size) have a meaning
+ *   lens       [max_seqs]: tokens of each sequence
+ *   refcount   [num_pages]: sequences that use a page; 0 = free
+ *   status     [1]: failures of the calls below (blt_cache_status bits, 0 = none)
+ * head_dim 64 or 128; page_size a power of two, 8 .. 1024.  A sequence's last page,
+ * where it is partly filled, belongs to it alone; full pages may be shared.  The
+ * calls keep that: they need no host synchronisation and can be captured.  A
+ * call that cannot be carried out sets a status bit and changes nothing (except
+ * as blt_cache_trim says); while one of the first four is set, blt_cache_append writes no keys and values and
+ * blt_cache_reserve and blt_cache_fork do nothing. */
+typedef struct blt_paged_cache {
+  void* k;
+  void* v;
+  int32_t* page_table;
+  int32_t* lens;
+  int32_t* refcount;
+  int32_t* status;
+  int32_t dtype; /* blt_dtype */
+  int32_t n_layers;
+  int32_t num_pages;
+  int32_t n_kv_heads;
+  int32_t page_size;
+  int32_t head_dim;
+  int32_t max_seqs;
+  int32_t max_pages;
+} blt_paged_cache;
+
+typedef enum blt_cache_status {
+  BLT_CACHE_FULL = 1,      /* not enough free pages */
+  BLT_CACHE_TOO_LONG = 2,  /* a sequence would pass max_pages pages */
+  BLT_CACHE_BAD_INDEX = 4, /* a sequence or page index out of range, a negative count */
+  BLT_CACHE_BUSY = 8,      /* a sequence twice in one call, or a fork onto one that has tokens */
+  BLT_CACHE_NO_PAGE = 16   /* tokens appended where the sequence has no page: left out */
+} blt_cache_status;
+
+/* Device bytes of the workspace of blt_cache_trim, blt_cache_fork (n sequences) and
+ * blt_cache_compact (n = 0); no initialisation; calls that share one must be
+ * stream-ordered. */
+int64_t blt_cache_workspace_bytes(const blt_paged_cache* cache, int64_t n);
+/* Grow sequence seqs[i] by counts[i] tokens (seqs NULL: sequence i), i < n <= 8192:
+ * missing pages are taken from the free ones, lowest index first, in the order of
+ * the list.  Their contents are what was there.  All sequences or none. */
+int blt_cache_reserve(const blt_paged_cache* cache, const int32_t* seqs, const int32_t* counts,
+                      int64_t n, blt_stream_t stream);
+/* Cut sequence seqs[i] to new_lens[i] tokens where it is longer (new_lens NULL: to
+ * 0, which needs no workspace); pages no sequence uses any more are free.  A cut
+ * inside a shared page takes a copy of its kept part; where no page is free for
+ * that, the sequence is cut to the page's start and BLT_CACHE_FULL is set.  An index
+ * out of range is skipped and reported. */
+int blt_cache_trim(const blt_paged_cache* cache, const int32_t* seqs, const int32_t* new_lens,
+                   int64_t n, void* workspace, int64_t workspace_bytes, blt_stream_t stream);
+/* Make sequence dst[i], which has no tokens, a continuation of sequence src[i]: its full
+ * pages are shared, a partly filled last page is copied (every layer, its filled
+ * tokens) into the lowest free page.  One src may have several dst; none may be a dst
+ * of the same call.  All or none. */
+int blt_cache_fork(const blt_paged_cache* cache, const int32_t* src, const int32_t* dst, int64_t n,
+                   void* workspace, int64_t workspace_bytes, blt_stream_t stream);
+/* Move the used pages with the highest indices into the free ones with the lowest,
+ * both ascending, until the n used pages are pages 0 .. n - 1. */
+int blt_cache_compact(const blt_paged_cache* cache, void* workspace, int64_t workspace_bytes,
+                      blt_stream_t stream);
+/* Copy page src[i] to page dst[i] in every layer, i < n; no index may appear twice in
+ * dst or in both lists.  Pairs with an index out of range are skipped and reported. */
+int blt_cache_copy_pages(const blt_paged_cache* cache, const int32_t* src, const int32_t* dst,
+                         int64_t n, blt_stream_t stream);
+
+/* Write the new tokens of B sequences into `layer`: row b has the tokens starts[b] ..
+ * starts[b + 1] - 1 (int32 [B + 1], device) of k and v [total, n_kv_heads, head_dim] (token
+ * and head strides in elements), which become the last tokens of sequence
+ * seqs[b] (NULL: b; no sequence twice), whose length already counts them
+ * (blt_cache_reserve).  rotary (may be NULL): k is rotated at its position, and q
+ * [total, Hq, head_dim] into q_out (both may be NULL with Hq = 0; q_out may be q).
+ * Tokens at starts[B] and behind are left alone. */
+int blt_cache_append(const blt_paged_cache* cache, int32_t layer, const void* k, int64_t st_k,
+                     int64_t sh_k, const void* v, int64_t st_v, int64_t sh_v, const void* q,
+                     int64_t st_q, int64_t sh_q, void* q_out, int64_t st_qo, int64_t sh_qo,
+                     int64_t Hq, const int32_t* starts, const int32_t* seqs, int64_t B,
+                     int64_t total, const blt_rotary* rotary, blt_stream_t stream);
+
+/* Attention of the new tokens q [total, Hq, head_dim] of B sequences (starts, seqs as
+ * above; a sequence may appear twice here) over `layer` of the cache, whose lengths
+ * count the new tokens: token i of n sits at position len - n + i.  Query head h reads
+ * key head h / (Hq / n_kv_heads).
+ *   causal: 1 = keys up to the token's own position; 0 = every key of the sequence
+ *   window: W > 0 (with causal) = only the last W of them
+ *   scale: of the scores, > 0
+ * Scores and softmax in f32; a token that sees no key gets 0.  Keys and values
+ * outside the sequences are not read; o [total, Hq, head_dim] behind starts[B] is left
+ * as it was.  Page indices outside the pool are read as its nearest page. */
+int64_t blt_paged_attention_workspace_bytes(const blt_paged_cache* cache, int64_t B, int64_t total,
+                                            int64_t Hq);
+int blt_paged_attention(const blt_paged_cache* cache, int32_t layer, const void* q, int64_t st_q,
+                        int64_t sh_q, void* o, int64_t st_o, int64_t sh_o, int64_t Hq,
+                        const int32_t* starts, const int32_t* seqs, int64_t B, int64_t total,
+                        int32_t causal, int32_t window, float scale, void* workspace,
+                        int64_t workspace_bytes, blt_stream_t stream);
+
 /* Patcher (src/patcher.rs) --------------------------------------------- */
 
 /* patch_start_mask_from_entropy_with_monotonicity (patcher.rs:80-118) fused with
