@@ -21,6 +21,7 @@ EPI_BF16, EPI_F32, EPI_RESID_F32, EPI_QKV_ROPE, EPI_SILU_GATE = 0, 1, 2, 3, 4
 NUM_STAGES = 11
 DTYPE_F32, DTYPE_BF16 = 0, 1
 ROTARY_SCALING = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
+CACHE_SYNC_WORDS = 2048
 # blt_cache_status
 CACHE_FULL, CACHE_TOO_LONG, CACHE_BAD_INDEX, CACHE_BUSY, CACHE_NO_PAGE = 1, 2, 4, 8, 16
 
@@ -149,7 +150,8 @@ class Rotary(ctypes.Structure):
 
 class PagedCacheDesc(ctypes.Structure):
     """blt_paged_cache."""
-    _fields_ = ([(n, c_vp) for n in ("k", "v", "page_table", "lens", "refcount", "status")]
+    _fields_ = ([(n, c_vp) for n in ("k", "v", "page_table", "lens", "refcount", "status",
+                                  "sync")]
                 + [(n, c_i32) for n in ("dtype", "n_layers", "num_pages", "n_kv_heads",
                                         "page_size", "head_dim", "max_seqs", "max_pages")])
 

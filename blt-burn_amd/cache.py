@@ -81,10 +81,11 @@ class PagedCache:
         self.device, self.dtype = k.device, k.dtype
         self.n_layers, self.num_pages, self.n_kv_heads, self.page_size, self.head_dim = k.shape
         self.max_seqs, self.max_pages = page_table.shape
-        self._status = torch.zeros(1, dtype=torch.int32, device=k.device)
+        words = torch.zeros(1 + _lib.CACHE_SYNC_WORDS, dtype=torch.int32, device=k.device)
+        self._status, self._sync = words[:1], words[1:]
         self._desc = _lib.PagedCacheDesc(
             k.data_ptr(), v.data_ptr(), page_table.data_ptr(), lens.data_ptr(),
-            refcount.data_ptr(), self._status.data_ptr(), _TYPES[k.dtype], *k.shape[:3],
+            refcount.data_ptr(), self._status.data_ptr(), self._sync.data_ptr(), _TYPES[k.dtype], *k.shape[:3],
             k.shape[3], k.shape[4], *page_table.shape)
         self._ptr = ctypes.addressof(self._desc)
         self._lib = _lib.lib()

@@ -400,7 +400,7 @@ static int cache_checks(const blt_paged_cache* c, const char* what) {
       c->n_kv_heads < 1 || c->n_kv_heads > 1024 || c->max_seqs < 1 || c->max_seqs > (1 << 20) ||
       c->max_pages < 1 || c->max_pages > (1 << 20))
     return fail(BLT_ERR_SHAPE, w + ": cache sizes out of range");
-  if (!c->k || !c->v || !c->page_table || !c->lens || !c->refcount || !c->status)
+  if (!c->k || !c->v || !c->page_table || !c->lens || !c->refcount || !c->status || !c->sync)
     return fail(BLT_ERR_INVALID, w + ": null cache pointer");
   if (((uintptr_t)c->k | (uintptr_t)c->v) & 15)
     return fail(BLT_ERR_SHAPE, w + ": k and v must be 16-byte aligned");

@@ -6,7 +6,7 @@
 // into rows (row = token * G + head), so one key tile serves all of them and a
 // single token with grouped heads still fills matrix rows.  An item is a row tile of
 // one (sequence, key head) and, where the call has too few of them to fill the chip, a
-// part of its keys; the parts' unnormalised outputs meet in combine_kernel.  Lengths
+// part of its keys; the part that ends last joins the parts' unnormalised outputs (join_parts).  Lengths
 // live on the device (the call can be captured and replayed as they grow), so every wave
 // works out its item itself: the number of key tiles an item may have (C) follows from
 // the total work, then a scan over the sequences finds the item of a block.  The host
@@ -28,11 +28,12 @@ struct KArgs {
   void* o;
   int64_t st_q, sh_q, st_o, sh_o;
   const int32_t *starts, *seqs, *lens, *table;
-  int B, total, H, Hkv, G;
+  int B, total, Hkv, G;
   int max_seqs, max_pages, num_pages, lps, cap;  // cap: tokens max_pages hold
   int causal, window;                            // window 0: none
   float c;        // log2(e) * scale
   int target, cmin;
+  int* sync;      // a counter for every row tile with parts; all zero between calls
   float* part;    // [slots][rows of a tile][D], unnormalised outputs
   float* ml;      // [slots][rows of a tile][2], their max (before the scale) and sum
 };
@@ -70,14 +71,14 @@ __device__ inline void tiles_of(const KArgs& p, const Seq& q, int& nrt, int& kt)
 struct Item {
   Seq q;
   int kvh, rt, split, ns;  // key head, row tile, part and number of parts
-  int nrt, pslot;          // row tiles of the sequence; first partial slot of the sequence
+  int nrt;                 // row tiles of the sequence
+  int pslot, join;         // first partial slot and first counter of the sequence
 };
 __device__ inline int lane_of(int v, int l) { return __builtin_amdgcn_readlane(v, l); }
 
-// The item of block `bid`, false if it has none.  JOIN: the row tiles whose parts have
-// to be joined instead.  Every wave computes it by itself, in the same order, so all
-// agree.
-template <int BQ, int BKV, bool JOIN>
+// The item of block `bid`, false if it has none.  Every wave computes it by itself, in
+// the same order, so all agree.
+template <int BQ, int BKV>
 __device__ bool find_item(const KArgs& p, unsigned bid, Item& it) {
   const int lane = threadIdx.x & 63;
   Seq q;
@@ -92,38 +93,40 @@ __device__ bool find_item(const KArgs& p, unsigned bid, Item& it) {
   // (0.1 % above the exact quotient: the bounds on the grid and the slots hold
   // whatever the rounding of the sums)
   const int C = max(p.cmin, (int)fminf(ceilf(work * (1.001f / (float)p.target)), 1e9f));
-  auto counts = [&](int& ns, int& items, int& parts) {
-    ns = (kt + C - 1) / C;
-    items = JOIN ? (ns > 1 ? nrt * p.Hkv : 0) : nrt * ns * p.Hkv;
-    parts = ns > 1 ? nrt * ns * p.Hkv : 0;
+  int ns, heads;  // parts of a row tile, row tiles over all heads
+  auto counts = [&]() {
+    // (a part costs as much as a few key tiles to write and join: in proportion to its
+    // rows, a quarter of them in the form for 128)
+    const int64_t r = (int64_t)q.n * p.G;
+    const int most = max(C, p.cmin + (int)(r < BQ ? r : BQ) / (BQ >= 128 ? 4 : 16));
+    ns = (kt + most - 1) / most;
+    heads = nrt * p.Hkv;
   };
-  int ns, items, parts;
-  int id = (int)bid;
-  if constexpr (!JOIN) {
-    // dispatch places block i on XCD i % 8: each XCD takes a contiguous run of items, so
-    // the row tiles of one key head share its L2
-    int mine = 0;
-    for (int b0 = 0; b0 < p.B; b0 += 64) {
-      if (p.B > 64) {
-        q = seq_at(p, b0 + lane);
-        tiles_of<BQ, BKV>(p, q, nrt, kt);
-      }
-      counts(ns, items, parts);
-      mine += items;
-    }
-    const int all = lane_of(wave_incl_scan(mine), 63);
-    const int per = (all + 7) >> 3;
-    id = (int)(bid & 7) * per + (int)(bid >> 3);
-    if ((int)(bid >> 3) >= per || id >= all) return false;
-  }
-  int base = 0, pbase = 0;
+  // dispatch places block i on XCD i % 8: each XCD takes a contiguous run of items, so
+  // the row tiles of one key head share its L2
+  int mine = 0;
   for (int b0 = 0; b0 < p.B; b0 += 64) {
     if (p.B > 64) {
       q = seq_at(p, b0 + lane);
       tiles_of<BQ, BKV>(p, q, nrt, kt);
     }
-    counts(ns, items, parts);
-    const int inc = wave_incl_scan(items), pinc = wave_incl_scan(parts);
+    counts();
+    mine += heads * ns;
+  }
+  const int all = lane_of(wave_incl_scan(mine), 63);
+  const int per = (all + 7) >> 3;
+  const int id = (int)(bid & 7) * per + (int)(bid >> 3);
+  if ((int)(bid >> 3) >= per || id >= all) return false;
+  int base = 0, pbase = 0, jbase = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 64) {
+    if (p.B > 64) {
+      q = seq_at(p, b0 + lane);
+      tiles_of<BQ, BKV>(p, q, nrt, kt);
+    }
+    counts();
+    const int items = heads * ns, parts = ns > 1 ? items : 0, joins = ns > 1 ? heads : 0;
+    const int inc = wave_incl_scan(items);
+    const int pinc = wave_incl_scan(parts), jinc = wave_incl_scan(joins);
     const uint64_t above = __ballot(base + inc > id);
     if (above) {
       const int l = __ffsll((unsigned long long)above) - 1;
@@ -131,15 +134,17 @@ __device__ bool find_item(const KArgs& p, unsigned bid, Item& it) {
       it.nrt = lane_of(nrt, l);
       it.ns = lane_of(ns, l);
       it.pslot = pbase + lane_of(pinc - parts, l);
+      it.join = jbase + lane_of(jinc - joins, l);
       int at = id - (base + lane_of(inc - items, l));
       it.rt = it.nrt - 1 - at % it.nrt;  // the longest causal rows first
       at /= it.nrt;
-      it.split = JOIN ? 0 : at % it.ns;
-      it.kvh = JOIN ? at : at / it.ns;
+      it.split = at % it.ns;
+      it.kvh = at / it.ns;
       return true;
     }
     base += lane_of(inc, 63);
     pbase += lane_of(pinc, 63);
+    jbase += lane_of(jinc, 63);
   }
   return false;
 }
@@ -177,17 +182,116 @@ __device__ inline void stage_pages(const KArgs& p, const Seq& q, int base, int* 
   }
 }
 
+// Words of two bf16 values: the largest exponents seen so far; whether one of them is an
+// infinite value's or a NaN's; a word with such values zeroed.
+typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
+__device__ inline uint32_t exponents2(uint32_t seen, uint32_t x) {
+  return __builtin_bit_cast(
+      uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, seen),
+                                          __builtin_bit_cast(u16x2_t, x & 0x7f807f80u)));
+}
+__device__ inline bool not_finite2(uint32_t seen) {
+  return (seen & 0xffffu) == 0x7f80u || (seen >> 16) == 0x7f80u;
+}
+__device__ inline uint32_t finite2(uint32_t x) {
+  x = (x & 0x7f800000u) == 0x7f800000u ? x & 0xffffu : x;
+  return (x & 0x7f80u) == 0x7f80u ? x & 0xffff0000u : x;
+}
+
+// ---- joining the parts of a row tile ----------------------------------------------
+// Every block that has written its part counts itself; the one that finds all others
+// counted joins them, in the order of the parts (so the result does not depend on who
+// is last), and sets the counter back to zero.
+//   o = sum_i w_i o_i / sum_i w_i l_i,  w_i = e^(scale (m_i - max))
+// The blocks may sit on different XCDs, whose L2s are not coherent for ordinary accesses,
+// so parts are written and read by relaxed atomics of agent scope: they pass the L2s, a
+// write is complete when the wave's counter of stores says so.  (Ordinary accesses
+// between fences write back and invalidate whole L2s: 48 single tokens over up to
+// 8192 keys took 333 us that way, 135 with a second launch, see the figures below.)
+__device__ inline void put2(float* at, float x, float y) {
+  const uint64_t v = (uint64_t)__float_as_uint(x) | (uint64_t)__float_as_uint(y) << 32;
+  __hip_atomic_store(reinterpret_cast<uint64_t*>(at), v, __ATOMIC_RELAXED,
+                     __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ inline void put4(float* at, f32x4_t v) {
+  put2(at, v.x, v.y);
+  put2(at + 2, v.z, v.w);
+}
+__device__ inline void get2(const float* at, float& x, float& y) {
+  const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t*>(at), __ATOMIC_RELAXED,
+                                       __HIP_MEMORY_SCOPE_AGENT);
+  x = __uint_as_float((uint32_t)v);
+  y = __uint_as_float((uint32_t)(v >> 32));
+}
+__device__ inline f32x4_t get4(const float* at) {
+  f32x4_t v;
+  float x, y;
+  get2(at, x, y);
+  v.x = x; v.y = y;
+  get2(at + 2, x, y);
+  v.z = x; v.w = y;
+  return v;
+}
+// A thread takes four columns of a row at a time.  Called by all threads of a block of NT.
+template <int D, int BQ, int NT, typename T>
+__device__ void join_parts(const KArgs& p, const Item& it, int nr) {
+  __shared__ int last;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this thread's part, before the count
+  __syncthreads();
+  int* counter = p.sync + it.join + it.kvh * it.nrt + it.rt;
+  if (threadIdx.x == 0) {
+    last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+           it.ns - 1;
+    if (last) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (!last) return;
+  const int64_t step = (int64_t)it.nrt * BQ;
+  for (int i = threadIdx.x; i < nr * (D / 4); i += NT) {
+    const int r = i / (D / 4), dd = (i % (D / 4)) * 4;
+    const int64_t s0 = slot_of(it, 0) * BQ + r;
+    float mx = -INFINITY;
+#pragma unroll 8
+    for (int x = 0; x < it.ns; ++x) {
+      float m, l;
+      get2(p.ml + (s0 + x * step) * 2, m, l);
+      mx = fmaxf(mx, m);
+    }
+    const float mu = mx == -INFINITY ? 0.f : mx;
+    f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+    float lt = 0.f;
+#pragma unroll 8
+    for (int x = 0; x < it.ns; ++x) {
+      float m, l;
+      get2(p.ml + (s0 + x * step) * 2, m, l);
+      const f32x4_t o = get4(p.part + (s0 + x * step) * D + dd);
+      const float w = __builtin_amdgcn_exp2f((m - mu) * p.c);
+      lt = fmaf(w, l, lt);
+      acc += w * o;
+    }
+    const int row = it.rt * BQ + r, t = row / p.G, g = row - t * p.G;
+    const int64_t at =
+        (int64_t)(it.q.s0 + t) * p.st_o + (int64_t)(it.kvh * p.G + g) * p.sh_o + dd;
+    const f32x4_t x = lt == 0.f ? f32x4_t{0.f, 0.f, 0.f, 0.f} : acc / lt;
+    if constexpr (sizeof(T) == 2)
+      *reinterpret_cast<u32x2_t*>((uint16_t*)p.o + at) =
+          u32x2_t{pack_bf16x2(x.x, x.y), pack_bf16x2(x.z, x.w)};
+    else
+      *reinterpret_cast<f32x4_t*>((float*)p.o + at) = x;
+  }
+}
+
 // ---- bf16, tiles of rows ---------------------------------------------------------
-// One block = 4 waves of 32 NQ rows each; key tiles of 64 keys go global -> LDS by DMA
+// One block = 4 waves of 32 rows each; key tiles of 64 keys go global -> LDS by DMA
 // through NST stages shared by the waves.  As in attn_fwd_kernel the scores are taken
 // transposed, S^T = K . Q^T, so a lane owns one row: its max and sum need one
 // cross-lane step, P^T feeds the second product from registers, and V's operand is
 // read with the LDS transposing read.  Unlike there q keeps its own bf16 values (scaling it
 // before its rounding costs as much accuracy as the output's rounding): the scores come
 // out of the matrix core minus the running max, and the scale is one multiply before exp2.
-template <int D, int NQ, int NST>
-__global__ __launch_bounds__(256) void paged_attn_kernel(KArgs p) {
-  constexpr int BKV = 64, QPW = 32 * NQ, BQ = 4 * QPW;
+template <int D, int NST>
+__global__ __launch_bounds__(256, 2) void paged_attn_kernel(KArgs p) {
+  constexpr int BKV = 64, QPW = 32, BQ = 4 * QPW;
   constexpr int TILE = BKV * D;        // elements of a K (or V) tile
   constexpr int STAGE = 2 * TILE;
   constexpr int NOP = 4 * (D / 64);    // DMA instructions of a wave per tile
@@ -196,7 +300,7 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(KArgs p) {
   __shared__ int ptab[PT];
 
   Item it;
-  if (!find_item<BQ, BKV, false>(p, blockIdx.x, it)) return;
+  if (!find_item<BQ, BKV>(p, blockIdx.x, it)) return;
   const Seq& sq = it.q;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -220,30 +324,26 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(KArgs p) {
   const int pos_first = first + rw / p.G;  // lowest position in the wave
   const int lo_last = p.window ? first + rwl / p.G - p.window + 1 : 0;  // highest lower bound
 
-  // Q fragments (B operand): row rw + 32 qq + lrow, d = 16 ks + 8 lhalf .. + 8
-  bf16x8_t qf[NQ][KS];
-  int klo[NQ], khi[NQ];  // the row's visible keys
-#pragma unroll
-  for (int qq = 0; qq < NQ; ++qq) {
-    const int r = min(rw + 32 * qq + lrow, rows - 1);
-    const int t = r / p.G, g = r - t * p.G;
-    const uint16_t* qrow = (const uint16_t*)p.q + (int64_t)(sq.s0 + t) * p.st_q +
-                           (int64_t)(it.kvh * p.G + g) * p.sh_q;
+  // Q fragments (B operand): row rw + lrow, d = 16 ks + 8 lhalf .. + 8
+  bf16x8_t qf[KS];
+  const int row = rw + lrow;
+  const int tok = min(row, rows - 1) / p.G, head = it.kvh * p.G + min(row, rows - 1) - tok * p.G;
+  {
+    const uint16_t* qrow =
+        (const uint16_t*)p.q + (int64_t)(sq.s0 + tok) * p.st_q + (int64_t)head * p.sh_q;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
-      qf[qq][ks] = __builtin_bit_cast(
+      qf[ks] = __builtin_bit_cast(
           bf16x8_t, *reinterpret_cast<const u32x4_t*>(qrow + ks * 16 + lhalf * 8));
-    khi[qq] = p.causal ? min(first + t, sq.len - 1) : sq.len - 1;
-    klo[qq] = p.window ? first + t - p.window + 1 : 0;
   }
-  // consumed here, before any DMA is in flight (see attn_fwd_kernel)
-#pragma unroll
-  for (int qq = 0; qq < NQ; ++qq)
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) asm volatile("" ::"v"(qf[qq][ks]));
-
+  // the row's visible keys
+  const int khi = p.causal ? min(first + tok, sq.len - 1) : sq.len - 1;
+  const int klo = p.window ? first + tok - p.window + 1 : 0;
   int wbase = (t0 * BKV) >> p.lps;
   if (t0 < t1) stage_pages(p, sq, wbase, ptab, tid, 256);
+  // consumed here, before any DMA is in flight (see attn_fwd_kernel)
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) asm volatile("" ::"v"(qf[ks]));
   __syncthreads();
 
   // DMA.  Wave w moves keys 16 w .. 16 w + 15 of a tile, eight (one page) at a time.  LDS
@@ -287,20 +387,12 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(KArgs p) {
              16 * ((lane >> 4) & 1) + 4 * (s16 & 3);
   const int kswz = D == 64 ? (lrow >> 1) & 7 : lrow & 15;
 
-  f32x16_t o[NQ][DS], negm[NQ];
-  float m[NQ], mu[NQ], l[NQ];
+  f32x16_t o[DS];
+  float m = -INFINITY, l = 0.f;  // the row's offset (-inf until its first visible key), its sum
 #pragma unroll
-  for (int qq = 0; qq < NQ; ++qq) {
-    m[qq] = -INFINITY;
-    mu[qq] = 0.f;
-    l[qq] = 0.f;
+  for (int j = 0; j < DS; ++j)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) negm[qq][r] = 0.f;
-#pragma unroll
-    for (int j = 0; j < DS; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) o[qq][j][r] = 0.f;
-  }
+    for (int r = 0; r < 16; ++r) o[j][r] = 0.f;
   const bf16x2_t ones2 = {(__bf16)1.0f, (__bf16)1.0f};
   const float c = p.c, grow_at = 8.f / p.c;
 
@@ -329,90 +421,27 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(KArgs p) {
     if (wave_active && kb <= whi && kb + BKV > wlo) {
       const uint16_t* sk = lds + stage * STAGE;
       const uint16_t* sv = sk + TILE;
-      f32x16_t s[NQ][2];
-#pragma unroll
-      for (int sub = 0; sub < 2; ++sub)
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          const bf16x8_t a = *reinterpret_cast<const bf16x8_t*>(
-              sk + (sub * 32 + lrow) * D + (((2 * ks + lhalf) ^ kswz) << 3));
-#pragma unroll
-          for (int qq = 0; qq < NQ; ++qq)
-            s[qq][sub] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                a, qf[qq][ks], ks == 0 ? negm[qq] : s[qq][sub], 0, 0, 0);
-        }
       const bool mask_hi = kb + BKV - 1 > (p.causal ? pos_first : sq.len - 1) ||
                            kb + BKV > sq.len;
       const bool mask_lo = p.window && kb < lo_last;
-      bf16x8_t pb[NQ][2][2];
+      // All of K's fragments are read before the first product and all of V's under the
+      // softmax: 2 chunks of 2048 over 16384 keys (d = 128) take 0.92 ms, 0.96 with V's
+      // read between the products of the second, 1.70 with K's among those of the first.
+      bf16x8_t f[2][KS];
 #pragma unroll
-      for (int qq = 0; qq < NQ; ++qq) {
-        if (mask_hi) {
-          const int rel = khi[qq] - kb - 4 * lhalf;
+      for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
-          for (int sub = 0; sub < 2; ++sub)
+        for (int ks = 0; ks < KS; ++ks)
+          f[sub][ks] = *reinterpret_cast<const bf16x8_t*>(
+              sk + (sub * 32 + lrow) * D + (((2 * ks + lhalf) ^ kswz) << 3));
+      f32x16_t s[2];
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-              s[qq][sub][r] = sub * 32 + 8 * (r >> 2) + (r & 3) <= rel ? s[qq][sub][r] : -INFINITY;
-        }
-        if (mask_lo) {
-          const int rel = klo[qq] - kb - 4 * lhalf;
+      for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
-          for (int sub = 0; sub < 2; ++sub)
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-              s[qq][sub][r] = sub * 32 + 8 * (r >> 2) + (r & 3) >= rel ? s[qq][sub][r] : -INFINITY;
-        }
-        float mt = -INFINITY;  // this tile's max, relative to mu
-#pragma unroll
-        for (int sub = 0; sub < 2; ++sub)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[qq][sub][r]);
-        {
-          float a, b;
-          swap_pair<32>(mt, a, b);
-          mt = fmaxf(a, b);
-        }
-        // the offset mu moves only when the max grows by more than 2^8 over it
-        const bool grow = mt > grow_at || (m[qq] == -INFINITY && mt > -INFINITY);
-        if (__any(grow)) {
-          const float m_new = fmaxf(m[qq], mt + mu[qq]);
-          const float alpha =
-              m[qq] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((mu[qq] - m_new) * c);
-          m[qq] = m_new;
-          const float mu_new = m_new == -INFINITY ? 0.f : m_new;
-          const float shift = mu_new - mu[qq];
-          mu[qq] = mu_new;
-          l[qq] *= alpha;
-#pragma unroll
-          for (int j = 0; j < DS; ++j)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) o[qq][j][r] *= alpha;
-#pragma unroll
-          for (int sub = 0; sub < 2; ++sub)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[qq][sub][r] -= shift;
-#pragma unroll
-          for (int r = 0; r < 16; ++r) negm[qq][r] = -mu_new;
-        }
-        float ls = l[qq];
-#pragma unroll
-        for (int sub = 0; sub < 2; ++sub)
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            uint32_t w[4];
-#pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-              const float p0 = __builtin_amdgcn_exp2f(s[qq][sub][8 * u + e] * c);
-              const float p1 = __builtin_amdgcn_exp2f(s[qq][sub][8 * u + e + 1] * c);
-              w[e >> 1] = pack_bf16x2(p0, p1);
-              ls = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w[e >> 1]), ones2,
-                                                   ls, false);
-            }
-            pb[qq][sub][u] = __builtin_bit_cast(bf16x8_t, u32x4_t{w[0], w[1], w[2], w[3]});
-          }
-        l[qq] = ls;
-      }
+        for (int ks = 0; ks < KS; ++ks)
+          s[sub] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+              f[sub][ks], qf[ks], ks == 0 ? f32x16_t{} : s[sub], 0, 0, 0);
+      u32x4_t vf[DS][2][2];
 #pragma unroll
       for (int ds = 0; ds < DS; ++ds)
 #pragma unroll
@@ -424,55 +453,444 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(KArgs p) {
                 __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(LDS_PTR(vp)));
             const u32x2_t w1 = __builtin_bit_cast(
                 u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(LDS_PTR(vp + 8 * D)));
-            const bf16x8_t a = __builtin_bit_cast(bf16x8_t, u32x4_t{w0.x, w0.y, w1.x, w1.y});
-#pragma unroll
-            for (int qq = 0; qq < NQ; ++qq)
-              o[qq][ds] =
-                  __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, pb[qq][sub][u], o[qq][ds], 0, 0, 0);
+            vf[ds][sub][u] = u32x4_t{w0.x, w0.y, w1.x, w1.y};
           }
+      if (mask_hi) {
+        const int rel = khi - kb - 4 * lhalf;
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            s[sub][r] = sub * 32 + 8 * (r >> 2) + (r & 3) <= rel ? s[sub][r] : -INFINITY;
+      }
+      if (mask_lo) {
+        const int rel = klo - kb - 4 * lhalf;
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            s[sub][r] = sub * 32 + 8 * (r >> 2) + (r & 3) >= rel ? s[sub][r] : -INFINITY;
+      }
+      // A weight of zero does not silence an infinite or NaN value: where rows see different
+      // keys of a tile that holds one, it is taken out of the product and added to the
+      // rows that see it.
+      if (mask_hi || mask_lo) {
+        uint32_t seen = 0;
+#pragma unroll
+        for (int i = 0; i < DS * 4; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            seen = exponents2(seen, vf[i >> 2][(i >> 1) & 1][i & 1][e]);
+        if (__any(not_finite2(seen))) {
+#pragma unroll
+          for (int i = 0; i < DS * 4; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              vf[i >> 2][(i >> 1) & 1][i & 1][e] = finite2(vf[i >> 2][(i >> 1) & 1][i & 1][e]);
+          for (int j = 0; j < BKV; ++j) {
+            const bool sees = kb + j <= khi && kb + j >= klo;
+            const int swz = 4 * (D == 64 ? (j >> 1) & 1 : j & 3);
+#pragma unroll
+            for (int i = 0; i < DS * 4; ++i) {  // columns 8 i + 4 lhalf .. + 3
+              const u32x2_t x =
+                  *reinterpret_cast<const u32x2_t*>(sv + j * D + ((i ^ swz) << 3) + 4 * lhalf);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float v = bf16_to_f32((uint16_t)(x[e >> 1] >> (16 * (e & 1))));
+                o[i >> 2][4 * (i & 3) + e] += sees && !(fabsf(v) < INFINITY) ? v : 0.f;
+              }
+            }
+          }
+        }
+      }
+      float mt = -INFINITY;
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[sub][r]);
+      {
+        float a, b;
+        swap_pair<32>(mt, a, b);
+        mt = fmaxf(a, b);
+      }
+      // the offset moves only when the max is more than 2^8 over it
+      if (__any(mt > m + grow_at)) {
+        const float m_new = fmaxf(m, mt);
+        const float alpha = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - m_new) * c);
+        m = m_new;
+        l *= alpha;
+#pragma unroll
+        for (int j = 0; j < DS; ++j)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[j][r] *= alpha;
+      }
+      const float mc = m == -INFINITY ? 0.f : -m * c;
+      bf16x8_t pb[2][2];
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          uint32_t w[4];
+#pragma unroll
+          for (int e = 0; e < 8; e += 2) {
+            const float p0 = __builtin_amdgcn_exp2f(fmaf(s[sub][8 * u + e], c, mc));
+            const float p1 = __builtin_amdgcn_exp2f(fmaf(s[sub][8 * u + e + 1], c, mc));
+            w[e >> 1] = pack_bf16x2(p0, p1);
+            l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w[e >> 1]), ones2, l,
+                                                false);
+          }
+          pb[sub][u] = __builtin_bit_cast(bf16x8_t, u32x4_t{w[0], w[1], w[2], w[3]});
+        }
+#pragma unroll
+      for (int ds = 0; ds < DS; ++ds)
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+            o[ds] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                __builtin_bit_cast(bf16x8_t, vf[ds][sub][u]), pb[sub][u], o[ds], 0, 0, 0);
     }
     stage = stage + 1 < NST ? stage + 1 : 0;
   }
 
-  if (!wave_active) return;
+  float a, b;
+  swap_pair<32>(l, a, b);
+  const float lt = a + b;
+  if (row < rows && it.ns > 1) {
+    const int64_t at = slot_of(it, it.split) * BQ + (row - r0);
 #pragma unroll
-  for (int qq = 0; qq < NQ; ++qq) {
-    float a, b;
-    swap_pair<32>(l[qq], a, b);
-    const float lt = a + b;
-    const int r = rw + 32 * qq + lrow;
-    if (r >= rows) continue;
-    if (it.ns > 1) {
-      const int64_t at = slot_of(it, it.split) * BQ + (r - r0);
-      float* dst = p.part + at * D;
+    for (int ds = 0; ds < DS; ++ds)
 #pragma unroll
-      for (int ds = 0; ds < DS; ++ds)
+      for (int j = 0; j < 4; ++j)
+        put4(p.part + at * D + ds * 32 + 8 * j + 4 * lhalf,
+             f32x4_t{o[ds][4 * j], o[ds][4 * j + 1], o[ds][4 * j + 2], o[ds][4 * j + 3]});
+    if (lhalf == 0) put2(p.ml + at * 2, m, lt);
+  } else if (row < rows) {
+    uint16_t* orow = (uint16_t*)p.o + (int64_t)(sq.s0 + tok) * p.st_o + (int64_t)head * p.sh_o;
+    // hardware reciprocal (1 ulp): the output is rounded to bf16
+    const float inv = lt > 0.f ? __builtin_amdgcn_rcpf(lt) : lt == lt ? 0.f : lt;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          *reinterpret_cast<f32x4_t*>(dst + ds * 32 + 8 * j + 4 * lhalf) =
-              f32x4_t{o[qq][ds][4 * j], o[qq][ds][4 * j + 1], o[qq][ds][4 * j + 2],
-                      o[qq][ds][4 * j + 3]};
-      if (lhalf == 0) {
-        p.ml[at * 2] = m[qq] == -INFINITY ? -INFINITY : mu[qq];
-        p.ml[at * 2 + 1] = lt;
+    for (int ds = 0; ds < DS; ++ds)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        u32x2_t w;
+        w.x = pack_bf16x2(o[ds][4 * j] * inv, o[ds][4 * j + 1] * inv);
+        w.y = pack_bf16x2(o[ds][4 * j + 2] * inv, o[ds][4 * j + 3] * inv);
+        *reinterpret_cast<u32x2_t*>(orow + ds * 32 + 8 * j + 4 * lhalf) = w;
       }
-    } else {
-      const int t = r / p.G, g = r - t * p.G;
-      uint16_t* orow = (uint16_t*)p.o + (int64_t)(sq.s0 + t) * p.st_o +
-                       (int64_t)(it.kvh * p.G + g) * p.sh_o;
-      // hardware reciprocal (1 ulp): the output is rounded to bf16
-      const float inv = lt > 0.f ? __builtin_amdgcn_rcpf(lt) : lt == lt ? 0.f : lt;
+  }
+  if (it.ns > 1) join_parts<D, BQ, 256, uint16_t>(p, it, r1 - r0 + 1);
+}
+
+// ---- bf16, few rows ----------------------------------------------------------------
+// Up to 16 NR rows (single tokens, short chunks): bound by reading K and V once, so the
+// four waves of a block share nothing and wait for nothing but their own loads: each takes
+// every NW-th 32-key tile of the item through its own LDS ring of NST tiles, filled by DMA
+// while the tiles before are consumed, and they meet once at the end.  16 x 16 x 32
+// MFMAs, scores transposed as above (a lane owns a row, the key blocks' registers are the
+// second product's operand).  p goes into that product as two bf16 halves (p rounded, and
+// what the rounding left): the matrix cores have nothing else to do, and the output
+// keeps f32 accuracy up to its own rounding.
+template <int N>
+__device__ inline void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+template <int D, int NR, int NW, int NST>
+__global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(KArgs p) {
+  constexpr int KT = 32, BKV = 64, BQ = 16 * NR, TILE = KT * D;
+  constexpr int OPS = 2 * 4 * (D / 64);  // DMA instructions of a tile
+  constexpr int KS = D / 32, DB = D / 16, OP = D + 4, PTF = 1024;
+  constexpr int RING = NW * NST * 2 * TILE;  // elements
+  static_assert(RING * 2 >= NW * BQ * OP * 4, "the waves' outputs fit the rings");
+  __shared__ __attribute__((aligned(1024))) uint16_t lds[RING];
+  __shared__ float sm[NW][BQ], sl[NW][BQ];
+  __shared__ int ptab[PTF];
+
+  Item it;
+  if (!find_item<BQ, BKV>(p, blockIdx.x, it)) return;
+  const Seq& sq = it.q;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15, g4 = lane >> 4;
+  const int rows = sq.n * p.G, first = sq.len - sq.n;
+  const int r0 = it.rt * BQ, r1 = min(r0 + BQ, rows) - 1;
+  int lo, hi;
+  key_range(p, sq, r0, r1, lo, hi);
+  // the item's key tiles [t0, t1), of 32 keys here
+  const int t_lo = lo / KT, cnt = hi < 0 ? 0 : hi / KT - t_lo + 1;
+  const int t0 = t_lo + (int)((int64_t)cnt * it.split / it.ns);
+  const int t1 = t_lo + (int)((int64_t)cnt * (it.split + 1) / it.ns);
+
+  bf16x8_t qf[NR][KS];
+  int klo[NR], khi[NR];
 #pragma unroll
-      for (int ds = 0; ds < DS; ++ds)
+  for (int n = 0; n < NR; ++n) {
+    const int r = min(r0 + 16 * n + col, rows - 1);
+    const int t = r / p.G, g = r - t * p.G;
+    const uint16_t* qrow = (const uint16_t*)p.q + (int64_t)(sq.s0 + t) * p.st_q +
+                           (int64_t)(it.kvh * p.G + g) * p.sh_q;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          u32x2_t w;
-          w.x = pack_bf16x2(o[qq][ds][4 * j] * inv, o[qq][ds][4 * j + 1] * inv);
-          w.y = pack_bf16x2(o[qq][ds][4 * j + 2] * inv, o[qq][ds][4 * j + 3] * inv);
-          *reinterpret_cast<u32x2_t*>(orow + ds * 32 + 8 * j + 4 * lhalf) = w;
+    for (int ks = 0; ks < KS; ++ks)
+      qf[n][ks] = __builtin_bit_cast(
+          bf16x8_t, *reinterpret_cast<const u32x4_t*>(qrow + ks * 32 + g4 * 8));
+    khi[n] = p.causal ? min(first + t, sq.len - 1) : sq.len - 1;
+    klo[n] = p.window ? first + t - p.window + 1 : 0;
+  }
+  // every row sees [all_lo, all_hi]
+  const int all_hi = p.causal ? min(first + r0 / p.G, sq.len - 1) : sq.len - 1;
+  const int all_lo = p.window ? first + r1 / p.G - p.window + 1 : 0;
+
+  // DMA of one tile: eight keys (one page) at a time, chunks swizzled for the operand reads
+  const unsigned ring = (unsigned)(uintptr_t)lds + (unsigned)(w * NST * 2 * TILE * 2);
+  constexpr int CPR = D / 8;
+  const int kin = lane / CPR, slot = lane % CPR;
+  const int kx = slot ^ (D == 64 ? kin >> 1 : kin);
+  const int vx = slot ^ (D == 64 ? 2 * (kin >> 1) : 2 * kin);
+  int wbase = 0;
+  auto issue = [&](int t, int stage) {
+    const unsigned sb = ring + (unsigned)(stage * 2 * TILE * 2);
+    int pg[4], kc[4];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      kc[g] = min(t * KT + 8 * g, (sq.len - 1) & ~7);
+      pg[g] = ptab[(kc[g] >> p.lps) - wbase];
+    }
+    // (also: this wave's operand reads of the stage are done)
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int page = __builtin_amdgcn_readfirstlane(pg[g]);
+      const int64_t off =
+          (((((int64_t)page * p.Hkv + it.kvh) << p.lps) + (kc[g] & ((1 << p.lps) - 1))) * D) * 2;
+      const char* kb = (const char*)p.k + off;
+      const char* vb = (const char*)p.v + off;
+      const int key0 = t * KT + 8 * g;
+      const bool all = key0 + 8 <= sq.len;
+#pragma unroll
+      for (int h = 0; h < D / 64; ++h) {
+        int row = kin + (D == 128 ? 4 * h : 0);
+        if (!all) row = min(key0 + row, sq.len - 1) - kc[g];
+        const int kch = kx ^ (D == 64 ? 4 * (g & 1) : 8 * (g & 1) + 4 * h);
+        const int vch = D == 64 ? vx : vx ^ (8 * h);
+        const unsigned la = sb + (unsigned)(8 * g * D * 2 + h * 1024);
+        dma16_so(kb, (unsigned)(row * D * 2 + kch * 16), la);
+        dma16_so(vb, (unsigned)(row * D * 2 + vch * 16), la + TILE * 2);
+      }
+    }
+  };
+  // operand reads: K row `col` of a 16-key block; V rows 4 g4 + col / 4, 16 columns at 16 db
+  const int kswz = D == 64 ? (col >> 1) & 7 : col;
+  const int vrow = 4 * g4 + (col >> 2);
+  const int vswz = D == 64 ? (vrow >> 1) & 3 : vrow & 7;  // of 16-column blocks
+  const int vlane = vrow * D + 4 * (col & 3);
+
+  f32x4_t o[NR][DB];
+  float l[NR], m[NR];
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+    m[n] = -INFINITY;
+    l[n] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DB; ++d) o[n][d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  const float c = p.c, grow_at = 8.f / p.c;
+
+  auto tile = [&](int t, int stage) {
+    const uint16_t* sk = lds + (w * NST + stage) * 2 * TILE;
+    const uint16_t* sv = sk + TILE;
+    const int kb = t * KT;
+    f32x4_t s[NR][2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const bf16x8_t a = *reinterpret_cast<const bf16x8_t*>(
+            sk + (16 * b + col) * D + (((4 * ks + g4) ^ kswz) << 3));
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+          s[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              a, qf[n][ks], ks == 0 ? f32x4_t{} : s[n][b], 0, 0, 0);
         }
+      }
+    const bool mask = kb + KT - 1 > all_hi || kb < all_lo;
+    bf16x8_t ph[NR], pl[NR];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      if (mask) {
+        const int up = khi[n] - kb - 4 * g4, dn = klo[n] - kb - 4 * g4;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            s[n][b][r] = 16 * b + r <= up && 16 * b + r >= dn ? s[n][b][r] : -INFINITY;
+      }
+      float mt = fmaxf(fmaxf(fmaxf(s[n][0][0], s[n][0][1]), fmaxf(s[n][0][2], s[n][0][3])),
+                       fmaxf(fmaxf(s[n][1][0], s[n][1][1]), fmaxf(s[n][1][2], s[n][1][3])));
+      {
+        float a, b;
+        swap_pair<16>(mt, a, b);
+        mt = fmaxf(a, b);
+        swap_pair<32>(mt, a, b);
+        mt = fmaxf(a, b);
+      }
+      if (__any(mt > m[n] + grow_at)) {
+        const float m_new = fmaxf(m[n], mt);
+        const float alpha = m[n] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m[n] - m_new) * c);
+        m[n] = m_new;
+        l[n] *= alpha;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) o[n][d] *= alpha;
+      }
+      const float mc = m[n] == -INFINITY ? 0.f : -m[n] * c;
+      uint32_t wh[4], wl[4];
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[n][e >> 2][e & 3], c, mc));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(s[n][e >> 2][(e & 3) + 1], c, mc));
+        l[n] += p0 + p1;
+        const uint32_t x = pack_bf16x2(p0, p1);
+        wh[e >> 1] = x;
+        wl[e >> 1] = pack_bf16x2(p0 - __uint_as_float(x << 16),
+                                 p1 - __uint_as_float(x & 0xffff0000u));
+      }
+      ph[n] = __builtin_bit_cast(bf16x8_t, u32x4_t{wh[0], wh[1], wh[2], wh[3]});
+      pl[n] = __builtin_bit_cast(bf16x8_t, u32x4_t{wl[0], wl[1], wl[2], wl[3]});
+    }
+    u32x4_t vf[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d) {
+      const uint16_t* vp = sv + vlane + 16 * (d ^ vswz);
+      const u32x2_t w0 =
+          __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(LDS_PTR(vp)));
+      const u32x2_t w1 = __builtin_bit_cast(
+          u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(LDS_PTR(vp + 16 * D)));
+      vf[d] = u32x4_t{w0.x, w0.y, w1.x, w1.y};
+    }
+    if (mask) {  // (as in paged_attn_kernel: no infinite value behind a mask)
+      uint32_t seen = 0;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) seen = exponents2(seen, vf[d][e]);
+      if (__any(not_finite2(seen))) {
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) vf[d][e] = finite2(vf[d][e]);
+        for (int j = 0; j < KT; ++j) {
+          const int swz = D == 64 ? (j >> 1) & 3 : j & 7;
+#pragma unroll
+          for (int d = 0; d < DB; ++d) {  // columns 16 d + 4 g4 .. + 3
+            const u32x2_t x =
+                *reinterpret_cast<const u32x2_t*>(sv + j * D + 16 * (d ^ swz) + 4 * g4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float v = bf16_to_f32((uint16_t)(x[e >> 1] >> (16 * (e & 1))));
+#pragma unroll
+              for (int n = 0; n < NR; ++n)
+                o[n][d][e] +=
+                    kb + j <= khi[n] && kb + j >= klo[n] && !(fabsf(v) < INFINITY) ? v : 0.f;
+            }
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < DB; ++d) {
+      const bf16x8_t a = __builtin_bit_cast(bf16x8_t, vf[d]);
+#pragma unroll
+      for (int n = 0; n < NR; ++n) {
+        o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, ph[n], o[n][d], 0, 0, 0);
+        o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, pl[n], o[n][d], 0, 0, 0);
+      }
+    }
+  };
+
+  // runs of tiles whose pages ptab holds (one, but for very long parts)
+  const int run = ((PTF - 1) << p.lps) / KT;
+  for (int ta = t0; ta < t1; ta += run) {
+    const int tb = min(ta + run, t1);
+    if (ta > t0) __syncthreads();
+    wbase = (ta * KT) >> p.lps;
+    {
+      const int cols = (sq.len + (1 << p.lps) - 1) >> p.lps;
+      const int n = min(PTF, ((min(tb * KT, sq.len) - 1) >> p.lps) - wbase + 1);
+      for (int i = tid; i < n; i += 64 * NW) {
+        int page = wbase + i < cols ? p.table[(int64_t)sq.slot * p.max_pages + wbase + i] : 0;
+        page = page < 0 ? 0 : page;
+        ptab[i] = page < p.num_pages ? page : p.num_pages - 1;
+      }
+    }
+    __syncthreads();
+    int at = ta + w;  // next tile to issue
+#pragma unroll
+    for (int i = 0; i < NST - 1; ++i, at += NW)
+      if (at < tb) issue(at, i);
+    int stage = 0;
+    for (int t = ta + w; t < tb; t += NW) {
+      if (at < tb) issue(at, stage == 0 ? NST - 1 : stage - 1);
+      at += NW;
+      // tiles behind t that are in flight
+      const int left = min(NST - 1, (tb - 1 - t) / NW);
+      if (left >= 3) wait_loads<3 * OPS < 63 ? 3 * OPS : 63>();
+      else if (left == 2) wait_loads<2 * OPS>();
+      else if (left == 1) wait_loads<OPS>();
+      else wait_loads<0>();
+      tile(t, stage);
+      stage = stage + 1 < NST ? stage + 1 : 0;
     }
   }
+
+  // ---- the waves' partial results ----
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+    float a, b;
+    swap_pair<16>(l[n], a, b);
+    l[n] = a + b;
+    swap_pair<32>(l[n], a, b);
+    l[n] = a + b;
+    if (g4 == 0) {
+      sm[w][16 * n + col] = m[n];
+      sl[w][16 * n + col] = l[n];
+    }
+  }
+  __syncthreads();  // every wave is past its ring
+  float* so = reinterpret_cast<float*>(lds);
+#pragma unroll
+  for (int n = 0; n < NR; ++n)
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+      *reinterpret_cast<f32x4_t*>(so + (w * BQ + 16 * n + col) * OP + 16 * d + 4 * g4) = o[n][d];
+  __syncthreads();
+  const int nr = r1 - r0 + 1;
+  const int64_t at = it.ns > 1 ? slot_of(it, it.split) * BQ : 0;
+  for (int i = tid; i < nr * (D / 4); i += 64 * NW) {
+    const int r = i / (D / 4), dd = (i % (D / 4)) * 4;
+    float mx = sm[0][r];
+#pragma unroll
+    for (int x = 1; x < NW; ++x) mx = fmaxf(mx, sm[x][r]);
+    const float off = mx == -INFINITY ? 0.f : mx;
+    f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+    float lt = 0.f;
+#pragma unroll
+    for (int x = 0; x < NW; ++x) {
+      const float wt = __builtin_amdgcn_exp2f((sm[x][r] - off) * c);
+      lt += wt * sl[x][r];
+      acc += wt * *reinterpret_cast<const f32x4_t*>(so + (x * BQ + r) * OP + dd);
+    }
+    if (it.ns > 1) {
+      put4(p.part + (at + r) * D + dd, acc);
+      if (dd == 0) put2(p.ml + (at + r) * 2, mx, lt);
+    } else {
+      const int t = (r0 + r) / p.G, g = (r0 + r) - t * p.G;
+      uint16_t* dst = (uint16_t*)p.o + (int64_t)(sq.s0 + t) * p.st_o +
+                      (int64_t)(it.kvh * p.G + g) * p.sh_o + dd;
+      const float inv = lt == 0.f ? 0.f : 1.f / lt;
+      *reinterpret_cast<u32x2_t*>(dst) = u32x2_t{pack_bf16x2(acc.x * inv, acc.y * inv),
+                                                 pack_bf16x2(acc.z * inv, acc.w * inv)};
+    }
+  }
+  if (it.ns > 1) join_parts<D, BQ, 64 * NW, uint16_t>(p, it, nr);
 }
 
 // ---- f32 -------------------------------------------------------------------------
@@ -484,8 +902,9 @@ __global__ __launch_bounds__(256) void paged_attn_f32_kernel(KArgs p) {
   constexpr int D = 32 * ND, NW = 4, NC = 4 * ND, OP = D + 4, BQ = 32, BKV = 32;
   __shared__ __attribute__((aligned(16))) float so[NW * 32 * OP];
   __shared__ float sm[NW][32], sl[NW][32];
+  __shared__ int ptab[PT];
   Item it;
-  if (!find_item<BQ, BKV, false>(p, blockIdx.x, it)) return;
+  if (!find_item<BQ, BKV>(p, blockIdx.x, it)) return;
   const Seq& sq = it.q;
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -509,13 +928,12 @@ __global__ __launch_bounds__(256) void paged_attn_f32_kernel(KArgs p) {
 #pragma unroll
     for (int j = 0; j < NC; ++j) qf[j] = *reinterpret_cast<const f32x4_t*>(qrow + 8 * j + 4 * h);
   }
-  const int32_t* table = p.table + (int64_t)sq.slot * p.max_pages;
   const int mask = (1 << p.lps) - 1;
+  int wbase = 0;
   // element offset of a key's row; keys past the end give the last one
   auto row_at = [&](int key) -> int64_t {
     key = min(key, sq.len - 1);
-    int page = table[key >> p.lps];
-    page = page < 0 ? 0 : page < p.num_pages ? page : p.num_pages - 1;
+    const int page = ptab[(key >> p.lps) - wbase];
     return ((((int64_t)page * p.Hkv + it.kvh) << p.lps) + (key & mask)) * D;
   };
   auto load_k = [&](int t) {
@@ -534,8 +952,11 @@ __global__ __launch_bounds__(256) void paged_attn_f32_kernel(KArgs p) {
     for (int i = 0; i < 16; ++i) oacc[n][i] = 0.f;
   float m = -INFINITY, l = 0.f;
   const float c = p.c;
-  if (t0 + w < t1) load_k(t0 + w);
-  for (int t = t0 + w; t < t1; t += NW) {
+  // every row sees [all_lo, all_hi]
+  const int all_hi = p.causal ? min(first + r0 / p.G, sq.len - 1) : sq.len - 1;
+  const int all_lo = p.window ? first + r1 / p.G - p.window + 1 : 0;
+  // one tile; the next one's K (of `next`) is loaded under the second product
+  auto tile = [&](int t, int next) {
     const int k0 = t * BKV;
     // V of key k0 + 8 (i / 4) + 4 h + i % 4: four neighbours lie in one page
     vf_t vf[NV][16];
@@ -566,12 +987,44 @@ __global__ __launch_bounds__(256) void paged_attn_f32_kernel(KArgs p) {
       }
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] += s1[i];
-    load_k(t + NW < t1 ? t + NW : t);
+    load_k(next);
     const int up = khi - k0 - 4 * h, dn = klo - k0 - 4 * h;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const int key = 8 * (i >> 2) + (i & 3);
       s[i] = key <= up && key >= dn ? s[i] : -INFINITY;
+    }
+    if (k0 + BKV - 1 > all_hi || k0 < all_lo) {  // (as in paged_attn_kernel)
+      uint32_t seen = 0;  // the largest magnitude, as bits
+#pragma unroll
+      for (int n = 0; n < NV; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+#pragma unroll
+          for (int u = 0; u < VW; ++u)
+            seen = max(seen, __float_as_uint(vf[n][i][u]) & 0x7fffffffu);
+      if (__any(seen >= 0x7f800000u)) {
+        for (int j = 0; j < BKV; ++j) {
+          const float* vrow = (const float*)p.v + row_at(k0 + j);
+#pragma unroll
+          for (int n = 0; n < ND; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float v =
+                  vrow[VW * (8 * (i >> 2) + 4 * h + (i & 3)) + n % VW + 32 * VW * (n / VW)];
+              oacc[n][i] += k0 + j <= khi && k0 + j >= klo && !(fabsf(v) < INFINITY) ? v : 0.f;
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NV; ++n)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+#pragma unroll
+            for (int u = 0; u < VW; ++u) {
+              const float v = vf[n][i][u];
+              vf[n][i][u] = fabsf(v) < INFINITY ? v : 0.f;
+            }
+      }
     }
     float mt = s[0];
 #pragma unroll
@@ -602,6 +1055,17 @@ __global__ __launch_bounds__(256) void paged_attn_f32_kernel(KArgs p) {
       for (int n = 0; n < ND; ++n)
         oacc[n] =
             __builtin_amdgcn_mfma_f32_32x32x2f32(vf[n / VW][i][n % VW], s[i], oacc[n], 0, 0, 0);
+  };
+  // runs of tiles whose pages ptab holds
+  const int run = ((PT - 1) << p.lps) / BKV;
+  for (int ta = t0; ta < t1; ta += run) {
+    const int tb = min(ta + run, t1);
+    if (ta > t0) __syncthreads();
+    wbase = (ta * BKV) >> p.lps;
+    stage_pages(p, sq, wbase, ptab, tid, 256);
+    __syncthreads();
+    if (ta + w < tb) load_k(ta + w);
+    for (int t = ta + w; t < tb; t += NW) tile(t, t + NW < tb ? t + NW : t);
   }
 
   // ---- the four waves' partial results ----
@@ -641,83 +1105,40 @@ __global__ __launch_bounds__(256) void paged_attn_f32_kernel(KArgs p) {
   __syncthreads();
   const int nq = r1 - r0 + 1;
   const int64_t at = it.ns > 1 ? slot_of(it, it.split) * BQ : 0;
-  for (int i = tid; i < nq * D; i += 256) {
-    const int rr = i / D, cc = i - rr * D;
-    const float* x = so + rr * OP + cc;
-    const float sum = (x[0] + x[32 * OP]) + (x[64 * OP] + x[96 * OP]);
+  for (int i = tid; i < nq * (D / 4); i += 256) {
+    const int rr = i / (D / 4), cc = (i % (D / 4)) * 4;
+    f32x4_t x[NW];
+#pragma unroll
+    for (int k = 0; k < NW; ++k)
+      x[k] = *reinterpret_cast<const f32x4_t*>(so + (k * 32 + rr) * OP + cc);
+    const f32x4_t sum = (x[0] + x[1]) + (x[2] + x[3]);
     const float tot = sl[0][rr];
     if (it.ns > 1) {
-      p.part[(at + rr) * D + cc] = sum;
-      if (cc == 0) {
-        p.ml[(at + rr) * 2] = sm[0][rr];
-        p.ml[(at + rr) * 2 + 1] = tot;
-      }
+      put4(p.part + (at + rr) * D + cc, sum);
+      if (cc == 0) put2(p.ml + (at + rr) * 2, sm[0][rr], tot);
     } else {
       const int t = (r0 + rr) / p.G, gg = (r0 + rr) - t * p.G;
-      ((float*)p.o)[(int64_t)(sq.s0 + t) * p.st_o + (int64_t)(it.kvh * p.G + gg) * p.sh_o + cc] =
-          tot == 0.f ? 0.f : sum / tot;
+      *reinterpret_cast<f32x4_t*>((float*)p.o + (int64_t)(sq.s0 + t) * p.st_o +
+                                  (int64_t)(it.kvh * p.G + gg) * p.sh_o + cc) =
+          tot == 0.f ? f32x4_t{0.f, 0.f, 0.f, 0.f} : sum / tot;
     }
   }
-}
-
-// ---- joining the parts of a row tile ----------------------------------------------
-// One block per row tile with parts, a wave per row: o = sum_i w_i o_i / sum_i w_i l_i,
-// w_i = e^(scale (m_i - max)).
-template <int D, int BQ, int BKV, typename T>
-__global__ __launch_bounds__(256) void combine_kernel(KArgs p) {
-  Item it;
-  if (!find_item<BQ, BKV, true>(p, blockIdx.x, it)) return;
-  constexpr int E = D / 64;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int rows = it.q.n * p.G;
-  const int r0 = it.rt * BQ, nr = min(BQ, rows - r0);
-  const int64_t step = (int64_t)it.nrt * BQ, s0 = slot_of(it, 0) * BQ;
-  for (int r = w; r < nr; r += 4) {
-    float mx = -INFINITY;
-    for (int i = lane; i < it.ns; i += 64) mx = fmaxf(mx, p.ml[(s0 + i * step + r) * 2]);
-    mx = wave_max(mx);
-    const float mu = mx == -INFINITY ? 0.f : mx;
-    float acc[E], lt = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = 0.f;
-    for (int i0 = 0; i0 < it.ns; i0 += 64) {
-      float wt = 0.f;
-      if (i0 + lane < it.ns) {
-        const float* ml = p.ml + (s0 + (i0 + lane) * step + r) * 2;
-        wt = __builtin_amdgcn_exp2f((ml[0] - mu) * p.c);
-        lt += wt * ml[1];
-      }
-      const int n = min(64, it.ns - i0);
-#pragma unroll 8
-      for (int i = 0; i < n; ++i) {
-        const float wi =
-            __builtin_bit_cast(float, lane_of(__builtin_bit_cast(int, wt), i));
-        const float* src = p.part + (s0 + (i0 + i) * step + r) * D + lane * E;
-#pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = fmaf(wi, src[e], acc[e]);
-      }
-    }
-    lt = wave_sum(lt);
-    const int t = (r0 + r) / p.G, g = (r0 + r) - t * p.G;
-    const int64_t at = (int64_t)(it.q.s0 + t) * p.st_o + (int64_t)(it.kvh * p.G + g) * p.sh_o;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float x = lt == 0.f ? 0.f : acc[e] / lt;
-      if constexpr (sizeof(T) == 2) ((uint16_t*)p.o)[at + lane * E + e] = f32_to_bf16(x);
-      else ((float*)p.o)[at + lane * E + e] = x;
-    }
-  }
+  if (it.ns > 1) join_parts<D, BQ, 256, float>(p, it, nq);
 }
 
 // ---- launch ------------------------------------------------------------------------
+enum Form { FORM_TILES, FORM_FEW16, FORM_FEW32, FORM_F32 };
 struct Shape {
+  Form form;
   int bq, bkv, target, cmin;
 };
-// resident blocks: 3 per CU where LDS (48 KB of stages) and registers allow, 2 for
-// head_dim 128 and f32
-Shape shape_of(const blt_paged_cache& c) {
-  if (c.dtype == BLT_DTYPE_F32) return Shape{32, 32, 512, 4};
-  return Shape{128, 64, c.head_dim == 64 ? 768 : 512, 2};
+static_assert(BLT_CACHE_SYNC_WORDS >= 1536, "a counter for every row tile with parts");
+Shape shape_of(const blt_paged_cache& c, int64_t B, int64_t total, int H) {
+  if (c.dtype == BLT_DTYPE_F32) return Shape{FORM_F32, 32, 32, 512, 4};
+  const int64_t rows = total * (H / c.n_kv_heads);  // of all sequences, per key head
+  if (rows <= 16 * B) return Shape{FORM_FEW16, 16, 64, 1536, 2};
+  if (rows <= 32 * B) return Shape{FORM_FEW32, 32, 64, 1536, 2};
+  return Shape{FORM_TILES, 128, 64, 512, 2};
 }
 int64_t row_tiles(const blt_paged_cache& c, int64_t B, int64_t total, int H, int bq) {
   return total * (H / c.n_kv_heads) / bq + B;
@@ -728,16 +1149,37 @@ int64_t slots_of(const blt_paged_cache& c, const Shape& s) {
   return cap <= (int64_t)s.cmin * s.bkv ? 0 : 2 * (int64_t)s.target;
 }
 
+template <int D>
+int run_paged(const KArgs& p, const Shape& sh, unsigned nb, hipStream_t s) {
+  const dim3 grid(nb), block(256);
+  switch (sh.form) {
+    case FORM_TILES:
+      hipLaunchKernelGGL((paged_attn_kernel<D, 2>), grid, block, 0, s, p);
+      break;
+    case FORM_FEW16:
+      hipLaunchKernelGGL((paged_attn_few_kernel<D, 1, 2, 2>), grid, dim3(128), 0, s, p);
+      break;
+    case FORM_FEW32:
+      hipLaunchKernelGGL((paged_attn_few_kernel<D, 2, 2, 2>), grid, dim3(128), 0, s, p);
+      break;
+    default:
+      hipLaunchKernelGGL((paged_attn_f32_kernel<D / 32>), grid, block, 0, s, p);
+  }
+  BLT_LAUNCH_CHECK("paged_attn_kernel");
+  return 0;
+}
+
 }  // namespace
 
-int64_t paged_attention_workspace_bytes(const blt_paged_cache& c, int64_t, int64_t, int) {
-  const Shape s = shape_of(c);
+int64_t paged_attention_workspace_bytes(const blt_paged_cache& c, int64_t B, int64_t total,
+                                        int H) {
+  const Shape s = shape_of(c, B, total, H);
   return slots_of(c, s) * s.bq * (c.head_dim + 2) * 4;
 }
 
 int launch_paged_attention(const blt_paged_cache& c, const PagedAttnArgs& a, void* ws,
                            hipStream_t s) {
-  const Shape sh = shape_of(c);
+  const Shape sh = shape_of(c, a.B, a.total, a.H);
   const int d = c.head_dim;
   KArgs p{};
   const int64_t es = c.dtype == BLT_DTYPE_BF16 ? 2 : 4;
@@ -746,7 +1188,7 @@ int launch_paged_attention(const blt_paged_cache& c, const PagedAttnArgs& a, voi
   p.k = (const char*)c.k + layer; p.v = (const char*)c.v + layer;
   p.st_q = a.st_q; p.sh_q = a.sh_q; p.st_o = a.st_o; p.sh_o = a.sh_o;
   p.starts = a.starts; p.seqs = a.seqs; p.lens = c.lens; p.table = c.page_table;
-  p.B = (int)a.B; p.total = (int)a.total; p.H = a.H; p.Hkv = c.n_kv_heads; p.G = a.H / c.n_kv_heads;
+  p.B = (int)a.B; p.total = (int)a.total; p.Hkv = c.n_kv_heads; p.G = a.H / c.n_kv_heads;
   p.max_seqs = c.max_seqs; p.max_pages = c.max_pages; p.num_pages = c.num_pages;
   p.lps = log2_of(c.page_size); p.cap = c.max_pages * c.page_size;
   p.causal = a.causal; p.window = a.causal ? a.window : 0;
@@ -754,34 +1196,14 @@ int launch_paged_attention(const blt_paged_cache& c, const PagedAttnArgs& a, voi
   p.c = (float)(1.44269504088896340736 * (double)a.scale);
   p.target = sh.target; p.cmin = sh.cmin;
   const int64_t slots = slots_of(c, sh);
+  p.sync = c.sync;
   p.part = (float*)ws;
   p.ml = p.part + slots * sh.bq * d;
   const int64_t rt = row_tiles(c, a.B, a.total, a.H, sh.bq) * c.n_kv_heads;
   const int64_t nb = (rt + (slots ? sh.target : 0) + 7) / 8 * 8;
   if (nb > 0x7fffffff) return fail(BLT_ERR_SHAPE, "paged_attention: too many row tiles");
-  const dim3 grid((unsigned)nb), block(256);
-  const int64_t nj = rt < sh.target ? rt : sh.target;  // row tiles with parts
-  const dim3 jgrid((unsigned)nj);
-  if (c.dtype == BLT_DTYPE_BF16) {
-    if (d == 64) hipLaunchKernelGGL((paged_attn_kernel<64, 1, 3>), grid, block, 0, s, p);
-    else hipLaunchKernelGGL((paged_attn_kernel<128, 1, 2>), grid, block, 0, s, p);
-    BLT_LAUNCH_CHECK("paged_attn_kernel");
-    if (slots) {
-      if (d == 64) hipLaunchKernelGGL((combine_kernel<64, 128, 64, uint16_t>), jgrid, block, 0, s, p);
-      else hipLaunchKernelGGL((combine_kernel<128, 128, 64, uint16_t>), jgrid, block, 0, s, p);
-      BLT_LAUNCH_CHECK("combine_kernel");
-    }
-  } else {
-    if (d == 64) hipLaunchKernelGGL((paged_attn_f32_kernel<2>), grid, block, 0, s, p);
-    else hipLaunchKernelGGL((paged_attn_f32_kernel<4>), grid, block, 0, s, p);
-    BLT_LAUNCH_CHECK("paged_attn_f32_kernel");
-    if (slots) {
-      if (d == 64) hipLaunchKernelGGL((combine_kernel<64, 32, 32, float>), jgrid, block, 0, s, p);
-      else hipLaunchKernelGGL((combine_kernel<128, 32, 32, float>), jgrid, block, 0, s, p);
-      BLT_LAUNCH_CHECK("combine_kernel");
-    }
-  }
-  return 0;
+  return d == 64 ? run_paged<64>(p, sh, (unsigned)nb, s)
+                 : run_paged<128>(p, sh, (unsigned)nb, s);
 }
 
 }  // namespace blt

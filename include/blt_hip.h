@@ -188,12 +188,16 @@ int blt_fused_rotary(const void* q, const void* k, void* q_out, void* k_out, int
  *   lens       [max_seqs]: tokens of each sequence
  *   refcount   [num_pages]: sequences that use a page; 0 = free
  *   status     [1]: failures of the calls below (blt_cache_status bits, 0 = none)
+ *   sync       [BLT_CACHE_SYNC_WORDS]: zero when the cache is made; counters of blocks that
+ *              wait for each other, zero again after every call
  * head_dim 64 or 128; page_size a power of two, 8 .. 1024.  A sequence's last page,
  * where it is partly filled, belongs to it alone; full pages may be shared.  The
- * calls keep that: they need no host synchronisation and can be captured.  A
+ * calls keep that: they need no host synchronisation and can be captured; calls on one
+ * cache must be stream-ordered, attention among them (sync).  A
  * call that cannot be carried out sets a status bit and changes nothing (except
  * as blt_cache_trim says); while one of the first four is set, blt_cache_append writes no keys and values and
  * blt_cache_reserve and blt_cache_fork do nothing. */
+#define BLT_CACHE_SYNC_WORDS 2048
 typedef struct blt_paged_cache {
   void* k;
   void* v;
@@ -201,6 +205,7 @@ typedef struct blt_paged_cache {
   int32_t* lens;
   int32_t* refcount;
   int32_t* status;
+  int32_t* sync;
   int32_t dtype; /* blt_dtype */
   int32_t n_layers;
   int32_t num_pages;

@@ -302,6 +302,42 @@ def test_attention_infinite_keys_are_the_rows_own(dtype):
     assert (np.abs(f64(o[1:]) - want) <= tol).all()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("n,H,window", [(150, 1, 0), (9, 1, 0), (9, 3, 0), (150, 1, 40), (20, 1, 70)])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_attention_masked_values_stay_masked(dtype, d, n, H, window, value):
+    """NaN or infinite keys and values at some positions: the queries that see them have them
+    in their outputs, in that column only for a value, and no other query has."""
+    L = 200
+    m = Made([L], Hkv=1, d=d, dtype=TYPES[dtype])
+    clean_k, clean_v = m.rows(0, 0), m.rows(1, 0)
+    torch.manual_seed(n)
+    q = torch.randn(n, H, d, device=DEV).to(TYPES[dtype])
+    bad_v = {L - 5: 3, L - n // 2: d - 1, max(L - n, 0): 20, 60: 33}  # position: column
+    for pos, colm in bad_v.items():
+        m.kv[1][0, m.table[0, pos // 16], 0, pos % 16, colm] = value
+    o = f64(m.cache.attention(0, q, i32([0, n]), window=window))
+    want, A = R.attention(f64(q), clean_k, np.where(np.isfinite(m.rows(1, 0)), clean_v, 0.0), L, True, window)
+    tol = att_tol(A, f64(q), clean_k, TYPES[dtype], d, d ** -0.5)
+    at = L - n + np.arange(n)
+    hit = np.zeros((n, 1, d), bool)
+    for pos, colm in bad_v.items():
+        see = (pos <= at) & ((pos > at - window) if window else True)
+        hit[see, 0, colm] = True
+    hit = np.broadcast_to(hit, o.shape)
+    assert not np.isfinite(o[hit]).any()
+    assert (np.abs(o - want)[~hit] <= tol[~hit]).all()
+    # a NaN key that only the last tokens see
+    m2 = Made([L], Hkv=1, d=d, dtype=TYPES[dtype])
+    m2.kv[0][0, m2.table[0, (L - 3) // 16], 0, (L - 3) % 16] = float("nan")
+    o = f64(m2.cache.attention(0, q, i32([0, n]), window=window))
+    want, A = R.attention(f64(q), clean_k, clean_v, L, True, window)
+    tol = att_tol(A, f64(q), clean_k, TYPES[dtype], d, d ** -0.5)
+    assert (np.abs(o - want)[:-3] <= tol[:-3]).all()
+    assert np.isnan(o[-3:]).all()
+
+
 def test_attention_bad_indices_stay_in_bounds():
     """Page indices outside the pool, lengths beyond the table and unknown sequences: the
     other rows are what they were, nothing is written for an unknown sequence."""

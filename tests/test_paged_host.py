@@ -15,7 +15,7 @@ P = 0x1000  # a pointer that is never followed: all of these calls end in a chec
 
 
 def desc(**kw):
-    d = dict(k=P, v=P, page_table=P, lens=P, refcount=P, status=P, dtype=1, n_layers=2, num_pages=8,
+    d = dict(k=P, v=P, page_table=P, lens=P, refcount=P, status=P, sync=P, dtype=1, n_layers=2, num_pages=8,
              n_kv_heads=4, page_size=16, head_dim=64, max_seqs=4, max_pages=8)
     d.update(kw)
     return _lib.PagedCacheDesc(**d)
@@ -29,7 +29,7 @@ def addr(s):
     (dict(dtype=7), "dtype"), (dict(head_dim=96), "head_dim"), (dict(page_size=24), "page_size"),
     (dict(page_size=4), "page_size"), (dict(page_size=2048), "page_size"),
     (dict(n_layers=0), "sizes"), (dict(num_pages=0), "sizes"), (dict(max_pages=1 << 21), "sizes"),
-    (dict(k=0), "null"), (dict(status=0), "null"), (dict(v=P + 8), "aligned")])
+    (dict(k=0), "null"), (dict(status=0), "null"), (dict(sync=0), "null"), (dict(v=P + 8), "aligned")])
 def test_bad_caches_are_refused(bad, word):
     d = desc(**bad)
     calls = [lambda: L.blt_cache_reserve(addr(d), None, P, 1, None),
