@@ -19,14 +19,19 @@ def stream_ptr(device=None):
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def call_on(device, fn, what, *args):
-    """fn(*args, stream) on `device` (with an index) and its current stream: the
-    library launches on the current device, which may be another one."""
-    if torch.cuda.current_device() == device.index:
-        check(fn(*args, stream_ptr(device)), what)
+_current_device = torch._C._cuda_getDevice
+
+
+def call_on(device, index, fn, what, *args):
+    """fn(*args, stream) on `device` (whose index is `index`) and its current stream:
+    the library launches on the current device, which may be another one."""
+    if _current_device() == index:
+        rc = fn(*args, stream_ptr(index))
     else:
         with torch.cuda.device(device):
-            check(fn(*args, stream_ptr(device)), what)
+            rc = fn(*args, stream_ptr(index))
+    if rc:
+        check(rc, what)
 
 
 def require_cuda(*tensors):

@@ -13,7 +13,8 @@ bookkeeping is on the device: no call synchronises, and all of them can be
 captured into a graph.  A call that the state does not allow (no free page, a
 sequence too long) sets a bit in the cache's status instead of raising; check()
 waits, raises BltError for it and clears it.  Calls on one cache must be
-stream-ordered.
+stream-ordered, attention among them: they share its workspace and counters (two
+graphs that use one cache must not be replayed at once).
 """
 import ctypes
 
@@ -78,7 +79,7 @@ class PagedCache:
             raise BltError("PagedCache: tensors must be contiguous and on one device")
         self.k, self.v = k, v
         self.page_table, self.lens, self.refcount = page_table, lens, refcount
-        self.device, self.dtype = k.device, k.dtype
+        self.device, self._index, self.dtype = k.device, k.device.index, k.dtype
         self.n_layers, self.num_pages, self.n_kv_heads, self.page_size, self.head_dim = k.shape
         self.max_seqs, self.max_pages = page_table.shape
         words = torch.zeros(1 + _lib.CACHE_SYNC_WORDS, dtype=torch.int32, device=k.device)
@@ -89,11 +90,18 @@ class PagedCache:
             k.shape[3], k.shape[4], *page_table.shape)
         self._ptr = ctypes.addressof(self._desc)
         self._lib = _lib.lib()
-        self._heads = (self.n_kv_heads, self.head_dim)
+        self._piece, self._scale = 16 // k.element_size(), self.head_dim ** -0.5
         if self._lib.blt_cache_workspace_bytes(self._ptr, 0) <= 0:
             raise BltError("PagedCache: bad sizes")
         # the library's own checks, once: an empty list does nothing else
-        call_on(self.device, self._lib.blt_cache_reserve, "PagedCache", self._ptr, None, None, 0)
+        self._call(self._lib.blt_cache_reserve, "PagedCache", self._ptr, None, None, 0)
+        # parts of attention calls, of whichever form needs most
+        self._ws_bytes = max(self._lib.blt_paged_attention_workspace_bytes(
+            self._ptr, 1, rows, self.n_kv_heads) for rows in (1, 32, 1024))
+        self._ws = self._workspace(max(self._ws_bytes, 16))
+
+    def _call(self, fn, what, *args):
+        call_on(self.device, self._index, fn, what, *args)
 
     # ---- status ---------------------------------------------------------------
     def check(self):
@@ -105,12 +113,14 @@ class PagedCache:
 
     # ---- lists of sequences ---------------------------------------------------
     def _list(self, t, what, n=None):
-        require_cuda(t)
-        if t.dtype != torch.int32 or t.dim() != 1 or t.device != self.device or \
+        """(pointer, length) of an int32 list on the cache's device, of length n if given."""
+        if not isinstance(t, torch.Tensor):
+            raise TypeError("expected a torch.Tensor, got %r" % type(t))
+        if t.dtype is not torch.int32 or t.get_device() != self._index or t.dim() != 1 or \
                 not t.is_contiguous() or (n is not None and t.shape[0] != n):
             raise BltError("PagedCache: %s must be a contiguous int32 [%s] on %s"
                            % (what, "n" if n is None else n, self.device))
-        return t.data_ptr()
+        return t.data_ptr(), t.shape[0]
 
     def _workspace(self, nbytes):
         return torch.empty(nbytes, dtype=torch.uint8, device=self.device)
@@ -118,68 +128,71 @@ class PagedCache:
     def reserve(self, counts, seqs=None):
         """Grow sequence seqs[i] (None: i) by counts[i] tokens; missing pages are the free
         ones with the lowest index.  All or, with a status bit, none."""
-        c = self._list(counts, "counts")
-        n = counts.shape[0]
-        s = None if seqs is None else self._list(seqs, "seqs", n)
-        call_on(self.device, self._lib.blt_cache_reserve, "cache_reserve", self._ptr, s, c, n)
+        c, n = self._list(counts, "counts")
+        s = None if seqs is None else self._list(seqs, "seqs", n)[0]
+        self._call(self._lib.blt_cache_reserve, "cache_reserve", self._ptr, s, c, n)
 
     def trim(self, lens, seqs=None):
         """Cut sequence seqs[i] (None: i) to lens[i] tokens where it is longer."""
-        p = self._list(lens, "lens")
-        n = lens.shape[0]
-        s = None if seqs is None else self._list(seqs, "seqs", n)
+        p, n = self._list(lens, "lens")
+        s = None if seqs is None else self._list(seqs, "seqs", n)[0]
         size = self._lib.blt_cache_workspace_bytes(self._ptr, max(n, 1))
         ws = self._workspace(size)
-        call_on(self.device, self._lib.blt_cache_trim, "cache_trim", self._ptr, s, p, n,
-                ws.data_ptr(), size)
+        self._call(self._lib.blt_cache_trim, "cache_trim", self._ptr, s, p, n, ws.data_ptr(), size)
 
     def free(self, seqs):
         """Drop sequences: their pages are free where no other sequence shares them."""
-        s = self._list(seqs, "seqs")
-        call_on(self.device, self._lib.blt_cache_trim, "cache_free", self._ptr, s, None,
-                seqs.shape[0], None, 0)
+        s, n = self._list(seqs, "seqs")
+        self._call(self._lib.blt_cache_trim, "cache_free", self._ptr, s, None, n, None, 0)
 
     def fork(self, src, dst):
         """Make every dst[i] (a sequence without tokens) a continuation of src[i]: full
         pages are shared, a partly filled last page is copied."""
-        a = self._list(src, "src")
-        n = src.shape[0]
-        b = self._list(dst, "dst", n)
+        a, n = self._list(src, "src")
+        b = self._list(dst, "dst", n)[0]
         size = self._lib.blt_cache_workspace_bytes(self._ptr, max(n, 1))
         ws = self._workspace(size)
-        call_on(self.device, self._lib.blt_cache_fork, "cache_fork", self._ptr, a, b, n,
-                ws.data_ptr(), size)
+        self._call(self._lib.blt_cache_fork, "cache_fork", self._ptr, a, b, n, ws.data_ptr(), size)
 
     def compact(self):
         """Move the used pages with the highest indices into the lowest free ones."""
         size = self._lib.blt_cache_workspace_bytes(self._ptr, 0)
         ws = self._workspace(size)
-        call_on(self.device, self._lib.blt_cache_compact, "cache_compact", self._ptr,
-                ws.data_ptr(), size)
+        self._call(self._lib.blt_cache_compact, "cache_compact", self._ptr, ws.data_ptr(), size)
 
     def copy_pages(self, src, dst):
         """Copy page src[i] to page dst[i] in every layer (no index twice in dst, none in
         both)."""
-        a = self._list(src, "src")
-        b = self._list(dst, "dst", src.shape[0])
-        call_on(self.device, self._lib.blt_cache_copy_pages, "cache_copy_pages", self._ptr, a, b,
-                src.shape[0])
+        a, n = self._list(src, "src")
+        b = self._list(dst, "dst", n)[0]
+        self._call(self._lib.blt_cache_copy_pages, "cache_copy_pages", self._ptr, a, b, n)
 
     # ---- tokens ---------------------------------------------------------------
     def _rows(self, starts, seqs):
-        p = self._list(starts, "starts")
-        B = starts.shape[0] - 1
+        p, B = self._list(starts, "starts")
+        B -= 1
         if B < 0:
             raise BltError("PagedCache: starts has one entry more than there are sequences")
-        return p, B, None if seqs is None else self._list(seqs, "seqs", B)
+        return p, B, None if seqs is None else self._list(seqs, "seqs", B)[0]
 
     def _tokens(self, t, what, heads=None):
-        require_cuda(t)
-        if t.dim() != 3 or t.dtype != self.dtype or t.device != self.device or \
-                t.shape[2] != self.head_dim or (heads is not None and t.shape[1] != heads):
+        """t as [tokens, heads, head_dim] with a dense last dimension, and its heads."""
+        if not isinstance(t, torch.Tensor):
+            raise TypeError("expected a torch.Tensor, got %r" % type(t))
+        shape = t.shape
+        if t.dtype is not self.dtype or t.get_device() != self._index or len(shape) != 3 or \
+                shape[2] != self.head_dim or (heads is not None and shape[1] != heads):
             raise BltError("PagedCache: %s must be %s [tokens, %s, %d] on %s"
                            % (what, self.dtype, "heads" if heads is None else heads,
                               self.head_dim, self.device))
+        return t if t.stride(2) == 1 else t.contiguous()
+
+    def _output(self, out, like, total, heads):
+        if out is None:
+            return torch.empty_like(like)
+        if self._tokens(out, "out", heads) is not out or out.shape[0] != total:
+            raise BltError("PagedCache: out must match q, with a dense last dimension")
+        return out
 
     def append(self, layer, k, v, starts, seqs=None, rotary=None, q=None, out=None):
         """Write the new tokens k, v [total, kv_heads, head_dim] into a layer: row b has
@@ -187,46 +200,35 @@ class PagedCache:
         ones of sequence seqs[b] (None: b; none twice), whose length already counts them
         (reserve).  rotary: a RotaryPlan that rotates k at its positions, and q [total, heads,
         head_dim] if given, which is returned (into `out`, which may be q)."""
-        Hk, total = self.n_kv_heads, k.shape[0]
-        self._tokens(k, "k", Hk)
-        self._tokens(v, "v", Hk)
+        k = self._tokens(k, "k", self.n_kv_heads)
+        v = self._tokens(v, "v", self.n_kv_heads)
         p, B, s = self._rows(starts, seqs)
+        total = k.shape[0]
         if v.shape[0] != total:
             raise BltError("PagedCache: k and v must have one number of tokens")
-        if k.stride(2) != 1:
-            k = k.contiguous()
-        if v.stride(2) != 1:
-            v = v.contiguous()
         r = None
         if rotary is not None:
             if not isinstance(rotary, RotaryPlan):
                 raise TypeError("PagedCache.append expects a RotaryPlan")
-            if rotary.device != self.device:
+            if rotary.device.index != self._index:
                 raise BltError("PagedCache: the rotary plan is on another device")
             r = rotary._ptr
         qp, qs, op, os_, Hq = None, (0, 0), None, (0, 0), 0
         if q is not None:
             if rotary is None:
                 raise BltError("PagedCache.append: q is rotated only with a rotary plan")
-            self._tokens(q, "q")
+            q = self._tokens(q, "q")
+            Hq = q.shape[1]
             if q.shape[0] != total:
                 raise BltError("PagedCache: q and k must have one number of tokens")
-            if q.stride(2) != 1:
-                q = q.contiguous()
-            Hq = q.shape[1]
-            if out is None:
-                out = torch.empty_like(q)
-            else:
-                self._tokens(out, "out", Hq)
-                if out.shape[0] != total or out.stride(2) != 1:
-                    raise BltError("PagedCache: out must match q, with a dense last dimension")
+            out = self._output(out, q, total, Hq)
             qp, qs, op, os_ = q.data_ptr(), q.stride(), out.data_ptr(), out.stride()
         elif out is not None:
             raise BltError("PagedCache.append: out without q")
         ks, vs = k.stride(), v.stride()
-        call_on(self.device, self._lib.blt_cache_append, "cache_append", self._ptr, layer,
-                k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], qp, qs[0], qs[1], op,
-                os_[0], os_[1], Hq, p, s, B, total, r)
+        self._call(self._lib.blt_cache_append, "cache_append", self._ptr, layer, k.data_ptr(), ks[0],
+                   ks[1], v.data_ptr(), vs[0], vs[1], qp, qs[0], qs[1], op, os_[0], os_[1], Hq, p, s,
+                   B, total, r)
         return out
 
     def attention(self, layer, q, starts, seqs=None, causal=True, window=0, scale=None, out=None):
@@ -237,28 +239,20 @@ class PagedCache:
         position, with window > 0 only the last `window` of them; causal=False: every
         key.  scale defaults to head_dim^-0.5.  Returns [total, heads, head_dim] (`out` if
         given; tokens at starts[-1] and behind are left as they were there)."""
-        self._tokens(q, "q")
+        q = self._tokens(q, "q")
         p, B, s = self._rows(starts, seqs)
         total, H, d = q.shape
         if H % self.n_kv_heads or H == 0:
             raise BltError("PagedCache: q's heads must be a multiple of the cache's %d"
                            % self.n_kv_heads)
-        es = 16 // q.element_size()
-        st = q.stride()
-        if st[2] != 1 or st[0] % es or st[1] % es or q.data_ptr() % 16:
+        st, qp = q.stride(), q.data_ptr()
+        if (st[0] | st[1]) % self._piece or qp % 16:  # rows that are not 16-byte aligned
             q = q.clone(memory_format=torch.contiguous_format)
-            st = q.stride()
-        if out is None:
-            out = torch.empty((total, H, d), dtype=q.dtype, device=self.device)
-        else:
-            self._tokens(out, "out", H)
-            if out.shape[0] != total or out.stride(2) != 1:
-                raise BltError("PagedCache: out must match q, with a dense last dimension")
+            st, qp = q.stride(), q.data_ptr()
+        out = self._output(out, q, total, H)
         so = out.stride()
-        size = self._lib.blt_paged_attention_workspace_bytes(self._ptr, B, total, H)
-        ws = self._workspace(size) if size else None
-        call_on(self.device, self._lib.blt_paged_attention, "paged_attention", self._ptr, layer,
-                q.data_ptr(), st[0], st[1], out.data_ptr(), so[0], so[1], H, p, s, B, total,
-                1 if causal else 0, window, d ** -0.5 if scale is None else scale,
-                ws.data_ptr() if size else None, size)
+        self._call(self._lib.blt_paged_attention, "paged_attention", self._ptr, layer, qp, st[0],
+                   st[1], out.data_ptr(), so[0], so[1], H, p, s, B, total, 1 if causal else 0,
+                   window, self._scale if scale is None else scale, self._ws.data_ptr(),
+                   self._ws_bytes)
         return out

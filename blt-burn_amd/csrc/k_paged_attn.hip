@@ -10,8 +10,8 @@
 // live on the device (the call can be captured and replayed as they grow), so every wave
 // works out its item itself: the number of key tiles an item may have (C) follows from
 // the total work, then a scan over the sequences finds the item of a block.  The host
-// only bounds the grid: items <= target + row tiles, parts in need of
-// joining <= 2 * target (every one of them has more than half of C).
+// only bounds the grid: items <= 2 * resident + row tiles, parts in need
+// of joining <= 4 * resident (every one of them has more than half of C).
 #include <type_traits>
 
 #include "paged.hpp"
@@ -32,7 +32,7 @@ struct KArgs {
   int max_seqs, max_pages, num_pages, lps, cap;  // cap: tokens max_pages hold
   int causal, window;                            // window 0: none
   float c;        // log2(e) * scale
-  int target, cmin;
+  int resident, cmin;  // blocks the chip holds; key tiles of the smallest part
   int* sync;      // a counter for every row tile with parts; all zero between calls
   float* part;    // [slots][rows of a tile][D], unnormalised outputs
   float* ml;      // [slots][rows of a tile][2], their max (before the scale) and sum
@@ -83,16 +83,23 @@ __device__ bool find_item(const KArgs& p, unsigned bid, Item& it) {
   const int lane = threadIdx.x & 63;
   Seq q;
   int nrt, kt;
-  float work = 0.f;
+  float work = 0.f, tiles = 0.f;
   for (int b0 = 0; b0 < p.B; b0 += 64) {
     q = seq_at(p, b0 + lane);
     tiles_of<BQ, BKV>(p, q, nrt, kt);
     work += (float)nrt * (float)kt;
+    tiles += (float)nrt;
   }
   work = wave_sum(work) * (float)p.Hkv;
-  // (0.1 % above the exact quotient: the bounds on the grid and the slots hold
-  // whatever the rounding of the sums)
-  const int C = max(p.cmin, (int)fminf(ceilf(work * (1.001f / (float)p.target)), 1e9f));
+  tiles = wave_sum(tiles) * (float)p.Hkv;
+  // Items should fill the chip's resident blocks once, or twice where there are so many row
+  // tiles that items of a single round would differ much in size.  Row tiles that are no
+  // whole number of C make half an item more each, on average: so work / C = blocks -
+  // tiles / 2.  (0.1 % above the exact quotient: the bounds on the grid and the slots
+  // hold whatever the rounding of the sums.)
+  const float blocks = 2.f * tiles > (float)p.resident ? 2.f * p.resident : (float)p.resident;
+  const float fill = fmaxf(blocks - 0.5f * tiles, 0.5f * (float)p.resident);
+  const int C = max(p.cmin, (int)fminf(ceilf(work * 1.001f / fill), 1e9f));
   int ns, heads;  // parts of a row tile, row tiles over all heads
   auto counts = [&]() {
     // (a part costs as much as a few key tiles to write and join: in proportion to its
@@ -1130,14 +1137,15 @@ __global__ __launch_bounds__(256) void paged_attn_f32_kernel(KArgs p) {
 enum Form { FORM_TILES, FORM_FEW16, FORM_FEW32, FORM_F32 };
 struct Shape {
   Form form;
-  int bq, bkv, target, cmin;
+  int bq, bkv, resident, cmin;
 };
-static_assert(BLT_CACHE_SYNC_WORDS >= 1536, "a counter for every row tile with parts");
+// (2 * resident <= BLT_CACHE_SYNC_WORDS: a counter for every row tile with parts)
 Shape shape_of(const blt_paged_cache& c, int64_t B, int64_t total, int H) {
   if (c.dtype == BLT_DTYPE_F32) return Shape{FORM_F32, 32, 32, 512, 4};
   const int64_t rows = total * (H / c.n_kv_heads);  // of all sequences, per key head
-  if (rows <= 16 * B) return Shape{FORM_FEW16, 16, 64, 1536, 2};
-  if (rows <= 32 * B) return Shape{FORM_FEW32, 32, 64, 1536, 2};
+  const int few = c.head_dim == 64 ? 1024 : 512;  // 32 and 64 KB of rings
+  if (rows <= 16 * B) return Shape{FORM_FEW16, 16, 64, few, 2};
+  if (rows <= 32 * B) return Shape{FORM_FEW32, 32, 64, few, 2};
   return Shape{FORM_TILES, 128, 64, 512, 2};
 }
 int64_t row_tiles(const blt_paged_cache& c, int64_t B, int64_t total, int H, int bq) {
@@ -1146,7 +1154,7 @@ int64_t row_tiles(const blt_paged_cache& c, int64_t B, int64_t total, int H, int
 // parts: none where not even a full sequence has more than cmin key tiles
 int64_t slots_of(const blt_paged_cache& c, const Shape& s) {
   const int64_t cap = (int64_t)c.max_pages * c.page_size;
-  return cap <= (int64_t)s.cmin * s.bkv ? 0 : 2 * (int64_t)s.target;
+  return cap <= (int64_t)s.cmin * s.bkv ? 0 : 4 * (int64_t)s.resident;
 }
 
 template <int D>
@@ -1194,13 +1202,13 @@ int launch_paged_attention(const blt_paged_cache& c, const PagedAttnArgs& a, voi
   p.causal = a.causal; p.window = a.causal ? a.window : 0;
   if (p.window > (1 << 30)) p.window = 0;  // longer than any sequence
   p.c = (float)(1.44269504088896340736 * (double)a.scale);
-  p.target = sh.target; p.cmin = sh.cmin;
+  p.resident = sh.resident; p.cmin = sh.cmin;
   const int64_t slots = slots_of(c, sh);
   p.sync = c.sync;
   p.part = (float*)ws;
   p.ml = p.part + slots * sh.bq * d;
   const int64_t rt = row_tiles(c, a.B, a.total, a.H, sh.bq) * c.n_kv_heads;
-  const int64_t nb = (rt + (slots ? sh.target : 0) + 7) / 8 * 8;
+  const int64_t nb = (rt + (slots ? 2 * sh.resident : 0) + 7) / 8 * 8;
   if (nb > 0x7fffffff) return fail(BLT_ERR_SHAPE, "paged_attention: too many row tiles");
   return d == 64 ? run_paged<64>(p, sh, (unsigned)nb, s)
                  : run_paged<128>(p, sh, (unsigned)nb, s);

@@ -211,7 +211,7 @@ class RotaryPlan:
         self._ptr = ctypes.addressof(self._desc)
 
 
-def _unit_stride(t):
+def _dense_rows(t):
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
@@ -222,27 +222,30 @@ def fused_rotary(q, k, positions, plan, backward=False, out=None):
     positions: int32 [seq] or [batch, seq].  backward=True applies the transposed
     rotation, which turns gradients of q', k' into those of q, k.  out: (q', k') to
     write, which may be q and k themselves; other overlaps are not allowed."""
-    require_cuda(q, positions)
-    _dtype_ok(q)
     if not isinstance(plan, RotaryPlan):
+        require_cuda(q, positions)
         raise TypeError("fused_rotary expects a RotaryPlan")
+    index, dtype = plan.device.index, q.dtype
+    if q.get_device() != index or positions.get_device() != index:
+        require_cuda(q, positions)
+        raise BltError("fused_rotary: tensors and plan must be on one device")
+    _dtype_ok(q)
     if q.dim() != 4:
         raise BltError("fused_rotary expects q [batch, heads, seq, head_dim]")
     B, Hq, T, d = q.shape
-    dev = q.device
-    Hk = 0
-    if k is not None:
-        require_cuda(k)
-        if k.dim() != 4 or k.dtype != q.dtype or (k.shape[0], k.shape[2], k.shape[3]) != (B, T, d):
-            raise BltError("fused_rotary: k must be [batch, kv_heads, seq, head_dim] of q's dtype")
-        Hk = k.shape[1]
-    if positions.dtype != torch.int32 or tuple(positions.shape) not in ((T,), (B, T)):
+    if positions.dtype != torch.int32 or positions.shape not in ((T,), (B, T)):
         raise BltError("fused_rotary: positions must be int32 [seq] or [batch, seq]")
-    if plan.device != dev or positions.device != dev or (k is not None and k.device != dev):
-        raise BltError("fused_rotary: tensors and plan must be on one device")
-    pos = positions if positions.stride(-1) == 1 else positions.contiguous()
-    x = _unit_stride(q)
-    y = _unit_stride(k) if k is not None else None
+    pos = _dense_rows(positions)
+    x = _dense_rows(q)
+    Hk, y, yp, kop, ys, ks = 0, None, None, None, (0, 0, 0), (0, 0, 0)
+    if k is not None:
+        if k.get_device() != index:
+            require_cuda(k)
+            raise BltError("fused_rotary: tensors and plan must be on one device")
+        if k.dim() != 4 or k.dtype != dtype or k.shape != (B, k.shape[1], T, d):
+            raise BltError("fused_rotary: k must be [batch, kv_heads, seq, head_dim] of q's dtype")
+        Hk, y = k.shape[1], _dense_rows(k)
+        yp, ys = y.data_ptr(), y.stride()
     if out is None:
         qo = torch.empty_like(x)
         ko = torch.empty_like(y) if y is not None else None
@@ -254,17 +257,16 @@ def fused_rotary(q, k, positions, plan, backward=False, out=None):
             if b is None:
                 continue
             require_cuda(a)
-            if not (a.shape == b.shape and a.dtype == b.dtype and a.device == dev and
+            if not (a.shape == b.shape and a.dtype == dtype and a.get_device() == index and
                     (a.stride(-1) == 1 or d == 1)):
                 raise BltError("fused_rotary: out tensors must match q and k, with a dense last "
                                "dimension")
     xs, qs = x.stride(), qo.stride()
-    ys, ks = (y.stride(), ko.stride()) if y is not None else ((0,) * 4, (0,) * 4)
-    call_on(dev, _lib.lib().blt_fused_rotary, "fused_rotary", x.data_ptr(),
-            y.data_ptr() if y is not None else None, qo.data_ptr(),
-            ko.data_ptr() if y is not None else None,
-            _lib.DTYPE_BF16 if q.dtype == torch.bfloat16 else _lib.DTYPE_F32, B, Hq, Hk, T, d,
-            xs[0], xs[1], xs[2], ys[0], ys[1], ys[2], qs[0], qs[1], qs[2], ks[0], ks[1], ks[2],
-            pos.data_ptr(), pos.stride(0) if pos.dim() == 2 else 0, plan._ptr,
+    if ko is not None:
+        kop, ks = ko.data_ptr(), ko.stride()
+    call_on(plan.device, index, _lib.lib().blt_fused_rotary, "fused_rotary", x.data_ptr(), yp,
+            qo.data_ptr(), kop, _lib.DTYPE_BF16 if dtype == torch.bfloat16 else _lib.DTYPE_F32, B,
+            Hq, Hk, T, d, xs[0], xs[1], xs[2], ys[0], ys[1], ys[2], qs[0], qs[1], qs[2], ks[0],
+            ks[1], ks[2], pos.data_ptr(), pos.stride(0) if pos.dim() == 2 else 0, plan._ptr,
             1 if backward else 0)
     return qo, ko
