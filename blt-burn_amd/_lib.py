@@ -53,7 +53,7 @@ EXPORTS = {
     "blt_cache_workspace_bytes": (c_i64, [c_vp, c_i64]),
     "blt_cache_reserve": (c_i32, [c_vp, c_vp, c_vp, c_i64, c_vp]),
     "blt_cache_trim": (c_i32, [c_vp, c_vp, c_vp, c_i64, c_vp, c_i64, c_vp]),
-    "blt_cache_fork": (c_i32, [c_vp, c_vp, c_vp, c_i64, c_vp, c_i64, c_vp]),
+    "blt_cache_fork": (c_i32, [c_vp, c_vp, c_vp, c_i64, c_vp]),
     "blt_cache_compact": (c_i32, [c_vp, c_vp, c_i64, c_vp]),
     "blt_cache_copy_pages": (c_i32, [c_vp, c_vp, c_vp, c_i64, c_vp]),
     "blt_cache_append": (c_i32, [c_vp, c_i32] + [c_vp, c_i64, c_i64] * 4

@@ -150,9 +150,7 @@ class PagedCache:
         pages are shared, a partly filled last page is copied."""
         a, n = self._list(src, "src")
         b = self._list(dst, "dst", n)[0]
-        size = self._lib.blt_cache_workspace_bytes(self._ptr, max(n, 1))
-        ws = self._workspace(size)
-        self._call(self._lib.blt_cache_fork, "cache_fork", self._ptr, a, b, n, ws.data_ptr(), size)
+        self._call(self._lib.blt_cache_fork, "cache_fork", self._ptr, a, b, n)
 
     def compact(self):
         """Move the used pages with the highest indices into the lowest free ones."""

@@ -397,7 +397,7 @@ static int cache_checks(const blt_paged_cache* c, const char* what) {
   if (c->page_size < 8 || c->page_size > 1024 || (c->page_size & (c->page_size - 1)))
     return fail(BLT_ERR_SHAPE, w + ": page_size must be a power of two, 8 .. 1024");
   if (c->n_layers < 1 || c->n_layers > 4096 || c->num_pages < 1 || c->num_pages > (1 << 28) ||
-      c->n_kv_heads < 1 || c->n_kv_heads > 1024 || c->max_seqs < 1 || c->max_seqs > (1 << 20) ||
+      c->n_kv_heads < 1 || c->n_kv_heads > 1024 || c->max_seqs < 1 || c->max_seqs > kMaxSeqs ||
       c->max_pages < 1 || c->max_pages > (1 << 20))
     return fail(BLT_ERR_SHAPE, w + ": cache sizes out of range");
   if (!c->k || !c->v || !c->page_table || !c->lens || !c->refcount || !c->status || !c->sync)
@@ -442,12 +442,11 @@ int blt_cache_trim(const blt_paged_cache* cache, const int32_t* seqs, const int3
   return launch_cache_trim(*cache, seqs, new_lens, n, workspace, STREAM(stream));
 }
 int blt_cache_fork(const blt_paged_cache* cache, const int32_t* src, const int32_t* dst, int64_t n,
-                   void* workspace, int64_t workspace_bytes, blt_stream_t stream) {
+                   blt_stream_t stream) {
   if (int rc = list_checks(cache, n, "cache_fork")) return rc;
   if (n == 0) return BLT_OK;
   if (!src || !dst) return fail(BLT_ERR_INVALID, "cache_fork: null list");
-  if (int rc = workspace_checks(cache, n, workspace, workspace_bytes, "cache_fork")) return rc;
-  return launch_cache_fork(*cache, src, dst, n, workspace, STREAM(stream));
+  return launch_cache_fork(*cache, src, dst, n, STREAM(stream));
 }
 int blt_cache_compact(const blt_paged_cache* cache, void* workspace, int64_t workspace_bytes,
                       blt_stream_t stream) {

@@ -2,15 +2,13 @@
 //
 // All bookkeeping is on the device (page table, lengths, reference counts), so a
 // decode step can grow, branch and drop sequences without the host.  What has to
-// be decided in order (which free page goes to whom) is one block of 1024 threads
+// be decided in order (which free page goes to whom) is a block of 1024 threads
 // walking the reference counts with a block scan: latency-bound, a few us up to
-// some ten thousand pages.  What moves data (page contents of every layer, the shared
-// rows of the table) is a second kernel over many blocks that reads the first one's
-// list.  Free pages are always taken lowest index first, so results do not depend
-// on timing.
-//
-// Lengths hold a claim in their sign bit while a call runs: the first entry that sets
-// it owns the sequence, so a sequence listed twice is seen, not raced on.
+// some ten thousand pages.  Free pages are always taken lowest index first, so results
+// do not depend on timing.  What moves data (page contents of every layer, the shared
+// rows of the table) runs on many blocks: a fork's blocks each decide for themselves,
+// from state that only the one that ends last writes; the others read a list that a
+// first kernel made.
 #include "paged.hpp"
 
 namespace blt {
@@ -19,7 +17,8 @@ namespace {
 
 constexpr int NT = 1024;     // threads of a bookkeeping block
 constexpr int PER = 4;       // reference counts a thread reads per step
-constexpr int CLAIM = (int)0x80000000;
+constexpr int LIST = 4096;   // free pages of one call held in LDS
+constexpr int CLAIM = (int)0x80000000;  // sign bit of a length, while trim_split_kernel runs
 
 // Workspace words: [0] number of copies; then three lists of `cap` words (source page,
 // destination page, tokens to copy) and, for compact, the page map.
@@ -55,18 +54,30 @@ __device__ inline int block_excl(int v, int* part, int& total) {
   return before + inc - v;
 }
 
+struct Refs {
+  int r[PER];
+};
+// reference counts of pages p .. p + PER - 1 (past the end: none free, none used)
+template <bool FREE>
+__device__ inline Refs load_refs(const int32_t* ref, int P, int p) {
+  Refs x;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) x.r[i] = p + i < P ? ref[p + i] : FREE ? 1 : 0;
+  return x;
+}
 // Walk the reference counts in ascending order of page until f has been called for
 // `most` free pages (or `used` ones, FREE false): f(page, ordinal).  Returns how many
-// there were, at most those of the step that reached `most`.
+// there were, at most those of the step that reached `most`.  x: the first step's.
 template <bool FREE, typename F>
-__device__ int walk_pages(const int32_t* ref, int P, int most, int* part, F f) {
+__device__ int walk_pages(const int32_t* ref, int P, int most, int* part, Refs x, F f) {
   int seen = 0;
   for (int p0 = 0; p0 < P && seen < most; p0 += NT * PER) {
     const int p = p0 + (int)threadIdx.x * PER;
+    if (p0) x = load_refs<FREE>(ref, P, p);
     int hit[PER], mine = 0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      hit[i] = p + i < P && (FREE ? ref[p + i] == 0 : ref[p + i] != 0) ? 1 : 0;
+      hit[i] = (FREE ? x.r[i] == 0 : x.r[i] != 0) ? 1 : 0;
       mine += hit[i];
     }
     int total;
@@ -81,6 +92,17 @@ __device__ int walk_pages(const int32_t* ref, int P, int most, int* part, F f) {
   }
   return seen;
 }
+template <bool FREE, typename F>
+__device__ int walk_pages(const int32_t* ref, int P, int most, int* part, F f) {
+  return walk_pages<FREE>(ref, P, most, part, load_refs<FREE>(ref, P, (int)threadIdx.x * PER), f);
+}
+
+// which sequences a call has named: a bit for each, in LDS
+constexpr int kSeqWords = kMaxSeqs / 32;
+__device__ inline bool named_before(uint32_t* bits, int s) {
+  return atomicOr(&bits[s >> 5], 1u << (s & 31)) >> (s & 31) & 1;
+}
+__device__ inline bool named(const uint32_t* bits, int s) { return bits[s >> 5] >> (s & 31) & 1; }
 
 __device__ inline int pages_of(int tokens, int lps) {
   return (int)(((int64_t)tokens + (1 << lps) - 1) >> lps);
@@ -91,10 +113,15 @@ __global__ __launch_bounds__(NT) void reserve_kernel(blt_paged_cache c, int lps,
                                                      const int32_t* seqs, const int32_t* counts,
                                                      int n) {
   __shared__ int first[kPageListMax + 1];  // pages wanted by the entries before
+  __shared__ int held[kPageListMax];       // pages an entry's sequence has
+  __shared__ int list[LIST];
+  __shared__ uint32_t bits[kSeqWords];
   __shared__ int part[NT / 64];
   __shared__ int bad;
   const int tid = threadIdx.x;
+  const Refs refs = load_refs<true>(c.refcount, c.num_pages, tid * PER);
   if (tid == 0) bad = *c.status & kCachePending ? -1 : 0;
+  for (int i = tid; i < kSeqWords; i += NT) bits[i] = 0;
   __syncthreads();
   if (bad) return;
   int need_all = 0;
@@ -106,12 +133,12 @@ __global__ __launch_bounds__(NT) void reserve_kernel(blt_paged_cache c, int lps,
       if (s < 0 || s >= c.max_seqs || cnt < 0) {
         err = BLT_CACHE_BAD_INDEX;
       } else {
-        const int old = atomicOr(&c.lens[s], CLAIM);
-        const int len = old & ~CLAIM;
-        if (old & CLAIM) err = BLT_CACHE_BUSY;
+        const int len = c.lens[s];
+        if (named_before(bits, s)) err = BLT_CACHE_BUSY;
         const int64_t want = ((int64_t)len + cnt + (1 << lps) - 1) >> lps;
         if (want > c.max_pages) err |= BLT_CACHE_TOO_LONG;
         else need = (int)want - pages_of(len, lps);
+        held[i] = pages_of(len, lps);
       }
     }
     if (err) atomicOr(&bad, err);
@@ -121,40 +148,42 @@ __global__ __launch_bounds__(NT) void reserve_kernel(blt_paged_cache c, int lps,
     // past any pool: too many for this call, and no overflow
     need_all = total > c.num_pages - need_all ? c.num_pages + 1 : need_all + total;
   }
-  if (tid == 0) first[n] = need_all;
   __syncthreads();
+  // ordinal o of the new pages: the last entry with first[entry] <= o
+  auto assign = [&](int page, int o) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (first[mid] <= o) lo = mid; else hi = mid;
+    }
+    const int s = seqs ? seqs[lo] : lo;
+    c.page_table[(int64_t)s * c.max_pages + held[lo] + o - first[lo]] = page;
+    c.refcount[page] = 1;
+  };
   if (!bad && need_all > 0) {
-    const int have = walk_pages<true>(c.refcount, c.num_pages, need_all, part, [](int, int) {});
+    const int have = walk_pages<true>(c.refcount, c.num_pages, need_all, part, refs,
+                                      [&](int page, int o) { if (o < LIST) list[o] = page; });
     if (have < need_all && tid == 0) bad = BLT_CACHE_FULL;
     __syncthreads();
-    if (!bad)
-      walk_pages<true>(c.refcount, c.num_pages, need_all, part, [&](int page, int o) {
-        int lo = 0, hi = n;  // the last entry with first[entry] <= o
-        while (hi - lo > 1) {
-          const int mid = (lo + hi) >> 1;
-          if (first[mid] <= o) lo = mid; else hi = mid;
-        }
-        const int s = seqs ? seqs[lo] : lo;
-        const int col = pages_of(c.lens[s] & ~CLAIM, lps) + o - first[lo];
-        c.page_table[(int64_t)s * c.max_pages + col] = page;
-        c.refcount[page] = 1;
-      });
+    if (!bad && need_all <= LIST)
+      for (int o = tid; o < need_all; o += NT) assign(list[o], o);
+    else if (!bad)
+      walk_pages<true>(c.refcount, c.num_pages, need_all, part, refs, assign);
   }
   __syncthreads();
-  for (int i = tid; i < n; i += NT) {
-    const int s = seqs ? seqs[i] : i;
-    if (s < 0 || s >= c.max_seqs) continue;
-    if (bad) atomicAnd(&c.lens[s], ~CLAIM);
-    else c.lens[s] = (c.lens[s] & ~CLAIM) + counts[i];
+  if (bad) {
+    if (tid == 0) atomicOr(c.status, bad);
+  } else {
+    for (int i = tid; i < n; i += NT) c.lens[seqs ? seqs[i] : i] += counts[i];
   }
-  if (bad && tid == 0) atomicOr(c.status, bad);
 }
 
 // ---- copies --------------------------------------------------------------------
 // The listed pages' first fill[i] tokens (fill NULL: all), in every layer, k and v: 16
 // bytes a lane, four in flight.  A fixed grid walks (pair, layer, k or v).
+// (256 threads, this one is `tid`)
 __device__ inline void copy_tokens(const blt_paged_cache& c, int64_t src, int64_t dst, int fill,
-                                   int layer, int kv, int es) {
+                                   int layer, int kv, int es, int tid) {
   const int64_t page_b = (int64_t)c.n_kv_heads * c.page_size * c.head_dim * es;
   const int64_t head_b = (int64_t)c.page_size * c.head_dim * es;
   char* base = reinterpret_cast<char*>(kv ? c.v : c.k) + (int64_t)layer * c.num_pages * page_b;
@@ -167,7 +196,7 @@ __device__ inline void copy_tokens(const blt_paged_cache& c, int64_t src, int64_
     return whole ? (int64_t)i * 16 : (i / row) * head_b + (int64_t)(i % row) * 16;
   };
   constexpr int U = 4;
-  for (int i = threadIdx.x; i < all; i += U * 256) {
+  for (int i = tid; i < all; i += U * 256) {
     u32x4_t x[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -182,7 +211,7 @@ __device__ inline void copy_listed(const blt_paged_cache& c, const Lists& l, int
   for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
     const int64_t i = it / (c.n_layers * 2);
     const int r = (int)(it - i * (c.n_layers * 2));
-    copy_tokens(c, l.src[i], l.dst[i], l.fill ? l.fill[i] : c.page_size, r >> 1, r & 1, es);
+    copy_tokens(c, l.src[i], l.dst[i], l.fill[i], r >> 1, r & 1, es, threadIdx.x);
   }
 }
 __global__ __launch_bounds__(256) void copy_list_kernel(blt_paged_cache c, Lists l, int es) {
@@ -199,93 +228,110 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(blt_paged_cache c, cons
       if (r == 0 && threadIdx.x == 0) atomicOr(c.status, BLT_CACHE_BAD_INDEX);
       continue;
     }
-    if (a != b) copy_tokens(c, a, b, c.page_size, r >> 1, r & 1, es);
+    if (a != b) copy_tokens(c, a, b, c.page_size, r >> 1, r & 1, es, threadIdx.x);
   }
 }
 
 // ---- fork ----------------------------------------------------------------------
-// Decides: the free page of every pair whose source ends inside a page.  dst[i] is
-// claimed by CLAIM, src may repeat.  l.dst[i] of pair i = its page; the copy list is dense.
+// Every block decides for itself, from the lengths and reference counts as they were:
+// the pages of the pairs whose source ends inside one, and whether the call can be carried
+// out.  Then the blocks share the work: entries of the shared rows (their pages are in
+// use, so the counts they raise change no decision) and the copies.  The block that ends
+// last, behind all decisions, writes what they rest on: the new pages' counts and
+// the lengths.  One launch: 24 pairs of 14 layers take 6.9 us; a deciding kernel and
+// a copying one took 10.9.
 __global__ __launch_bounds__(NT) void fork_kernel(blt_paged_cache c, int lps, const int32_t* src,
-                                                  const int32_t* dst, int n, Lists l) {
+                                                  const int32_t* dst, int n, int es) {
   __shared__ int first[kPageListMax];  // partial pages of the pairs before
+  __shared__ int list[kPageListMax];   // their new pages, old pages and tokens, by ordinal
+  __shared__ int olds[kPageListMax];
+  __shared__ short fills[kPageListMax];
+  __shared__ uint32_t bits[kSeqWords];
   __shared__ int part[NT / 64];
-  __shared__ int bad;
+  __shared__ int bad, last;
   const int tid = threadIdx.x, mask = c.page_size - 1;
-  if (tid == 0) {
-    bad = *c.status & kCachePending ? -1 : 0;
-    *l.count = 0;
-  }
+  const Refs refs = load_refs<true>(c.refcount, c.num_pages, tid * PER);
+  if (tid == 0) bad = *c.status & kCachePending ? -1 : 0;
+  for (int i = tid; i < kSeqWords; i += NT) bits[i] = 0;
   __syncthreads();
-  if (bad) return;
-  auto known = [&](int s) { return s >= 0 && s < c.max_seqs; };
+  const bool pending = bad != 0;
+  auto page_at = [&](int s, int col) {
+    const int page = c.page_table[(int64_t)s * c.max_pages + col];
+    return page < 0 ? 0 : page < c.num_pages ? page : c.num_pages - 1;
+  };
   int need_all = 0;
-  for (int i0 = 0; i0 < n; i0 += NT) {
-    const int i = i0 + tid;
-    int need = 0, err = 0;
-    if (i < n) {
-      const int a = src[i], b = dst[i];
-      if (!known(a) || !known(b)) {
-        err = BLT_CACHE_BAD_INDEX;
-      } else {
-        if (atomicOr(&c.lens[b], CLAIM) != 0) err = BLT_CACHE_BUSY;  // has tokens, or is claimed
-        const int len = c.lens[a] & ~CLAIM;
-        need = len & mask ? 1 : 0;
+  if (!pending) {
+    auto known = [&](int s) { return s >= 0 && s < c.max_seqs; };
+    for (int i0 = 0; i0 < n; i0 += NT) {
+      const int i = i0 + tid;
+      int need = 0, err = 0, old = 0, fill = 0;
+      if (i < n) {
+        const int a = src[i], b = dst[i];
+        if (!known(a) || !known(b)) {
+          err = BLT_CACHE_BAD_INDEX;
+        } else {
+          if (named_before(bits, b) || c.lens[b] != 0) err = BLT_CACHE_BUSY;
+          const int len = c.lens[a];
+          fill = len & mask;
+          need = fill ? 1 : 0;
+          if (fill && (len >> lps) < c.max_pages) old = page_at(a, len >> lps);
+        }
       }
+      if (err) atomicOr(&bad, err);
+      int total;
+      const int at = block_excl(need, part, total);
+      if (i < n) first[i] = need_all + at;
+      if (need) {
+        olds[need_all + at] = old;
+        fills[need_all + at] = (short)fill;
+      }
+      need_all += total;
     }
-    if (err) atomicOr(&bad, err);
-    int total;
-    const int at = block_excl(need, part, total);
-    if (i < n) first[i] = need_all + at;
-    need_all += total;
-  }
-  __syncthreads();
-  // no source may be a destination of the same call (read past the L1 cache)
-  for (int i = tid; i < n; i += NT)
-    if (known(src[i]) && (atomicOr(&c.lens[src[i]], 0) & CLAIM)) atomicOr(&bad, BLT_CACHE_BUSY);
-  __syncthreads();
-  if (!bad && need_all > 0) {
-    const int have = walk_pages<true>(c.refcount, c.num_pages, need_all, part,
-                                      [&](int page, int o) { l.dst[o] = page; });
-    if (have < need_all && tid == 0) bad = BLT_CACHE_FULL;
     __syncthreads();
-    if (!bad) {
-      for (int o = tid; o < need_all; o += NT) c.refcount[l.dst[o]] = 1;
-      for (int i = tid; i < n; i += NT) {
-        const int len = c.lens[src[i]] & ~CLAIM;
-        if (!(len & mask)) continue;
-        const int o = first[i], col = len >> lps;
-        const int page = c.page_table[(int64_t)src[i] * c.max_pages + col];
-        l.src[o] = page < 0 ? 0 : page < c.num_pages ? page : c.num_pages - 1;
-        l.fill[o] = len & mask;
-        c.page_table[(int64_t)dst[i] * c.max_pages + col] = l.dst[o];
+    // no source may be a destination of the same call
+    for (int i = tid; i < n; i += NT)
+      if (known(src[i]) && named(bits, src[i])) atomicOr(&bad, BLT_CACHE_BUSY);
+    int have = 0;
+    if (need_all > 0)
+      have = walk_pages<true>(c.refcount, c.num_pages, need_all, part, refs,
+                              [&](int page, int o) { list[o] = page; });
+    if (have < need_all && tid == 0) atomicOr(&bad, BLT_CACHE_FULL);
+    __syncthreads();
+  }
+  if (!bad) {
+    const int64_t cols = c.max_pages;
+    for (int64_t x = (int64_t)blockIdx.x * NT + tid; x < n * cols; x += (int64_t)gridDim.x * NT) {
+      const int i = (int)(x / cols), col = (int)(x - i * cols);
+      const int len = c.lens[src[i]];
+      int page = -1;
+      if (col < len >> lps) {
+        page = page_at(src[i], col);
+        atomicAdd(&c.refcount[page], 1);
+      } else if (col == len >> lps && (len & mask)) {
+        page = list[first[i]];
       }
-      if (tid == 0) *l.count = need_all;
+      if (page >= 0) c.page_table[(int64_t)dst[i] * cols + col] = page;
+    }
+    const int per = c.n_layers * 2;  // four teams of 256 threads
+    for (int64_t it = (int64_t)blockIdx.x * 4 + (tid >> 8); it < (int64_t)need_all * per;
+         it += (int64_t)gridDim.x * 4) {
+      const int o = (int)(it / per), r = (int)(it - (int64_t)o * per);
+      copy_tokens(c, olds[o], list[o], fills[o], r >> 1, r & 1, es, tid & 255);
     }
   }
   __syncthreads();
-  for (int i = tid; i < n; i += NT) {
-    if (!known(dst[i])) continue;
-    if (bad) atomicAnd(&c.lens[dst[i]], ~CLAIM);
-    else c.lens[dst[i]] = c.lens[src[i]];
+  if (tid == 0)
+    last = __hip_atomic_fetch_add(c.sync, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+           (int)gridDim.x - 1;
+  __syncthreads();
+  if (!last) return;
+  if (tid == 0) __hip_atomic_store(c.sync, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (bad) {
+    if (tid == 0 && !pending) atomicOr(c.status, bad);
+    return;
   }
-  if (bad && tid == 0) atomicOr(c.status, bad);
-}
-// Shares the full pages (one wave per pair and 64 columns) and copies the partial ones.
-__global__ __launch_bounds__(256) void fork_copy_kernel(blt_paged_cache c, int lps,
-                                                        const int32_t* src, const int32_t* dst,
-                                                        int n, Lists l, int es) {
-  if (*c.status & kCachePending) return;
-  const int64_t threads = (int64_t)gridDim.x * 256;
-  const int cols = c.max_pages;
-  for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < (int64_t)n * cols; x += threads) {
-    const int i = (int)(x / cols), col = (int)(x - (int64_t)i * cols);
-    if (col >= c.lens[dst[i]] >> lps) continue;
-    const int page = c.page_table[(int64_t)src[i] * c.max_pages + col];
-    c.page_table[(int64_t)dst[i] * c.max_pages + col] = page;
-    if (page >= 0 && page < c.num_pages) atomicAdd(&c.refcount[page], 1);
-  }
-  copy_listed(c, l, es);
+  for (int o = tid; o < need_all; o += NT) c.refcount[list[o]] = 1;
+  for (int i = tid; i < n; i += NT) c.lens[dst[i]] = c.lens[src[i]];
 }
 
 // ---- trim ----------------------------------------------------------------------
@@ -448,14 +494,11 @@ int launch_cache_trim(const blt_paged_cache& c, const int32_t* seqs, const int32
 }
 
 int launch_cache_fork(const blt_paged_cache& c, const int32_t* src, const int32_t* dst, int64_t n,
-                      void* ws, hipStream_t s) {
-  const int lps = log2_of(c.page_size);
-  const Lists l = lists_of(c, n, ws);
-  hipLaunchKernelGGL(fork_kernel, dim3(1), dim3(NT), 0, s, c, lps, src, dst, (int)n, l);
+                      hipStream_t s) {
+  const unsigned nb = (copy_blocks(c, n) + 3) / 4;
+  hipLaunchKernelGGL(fork_kernel, dim3(nb < 256 ? nb : 256), dim3(NT), 0, s, c,
+                     log2_of(c.page_size), src, dst, (int)n, elem_size(c));
   BLT_LAUNCH_CHECK("fork_kernel");
-  hipLaunchKernelGGL(fork_copy_kernel, dim3(copy_blocks(c, n)), dim3(256), 0, s, c, lps, src, dst,
-                     (int)n, l, elem_size(c));
-  BLT_LAUNCH_CHECK("fork_copy_kernel");
   return 0;
 }
 

@@ -43,14 +43,15 @@ constexpr int kCachePending =
     BLT_CACHE_FULL | BLT_CACHE_TOO_LONG | BLT_CACHE_BAD_INDEX | BLT_CACHE_BUSY;
 
 // ---- k_pages.hip -------------------------------------------------------------
-constexpr int64_t kPageListMax = 8192;  // sequences of one maintenance call
+constexpr int kPageListMax = 8192;  // sequences of one maintenance call
+constexpr int kMaxSeqs = 65536;
 int64_t cache_workspace_bytes(const blt_paged_cache& c, int64_t n);
 int launch_cache_reserve(const blt_paged_cache& c, const int32_t* seqs, const int32_t* counts,
                          int64_t n, hipStream_t s);
 int launch_cache_trim(const blt_paged_cache& c, const int32_t* seqs, const int32_t* lens,
                       int64_t n, void* ws, hipStream_t s);
 int launch_cache_fork(const blt_paged_cache& c, const int32_t* src, const int32_t* dst, int64_t n,
-                      void* ws, hipStream_t s);
+                      hipStream_t s);
 int launch_cache_compact(const blt_paged_cache& c, void* ws, hipStream_t s);
 int launch_cache_copy_pages(const blt_paged_cache& c, const int32_t* src, const int32_t* dst,
                             int64_t n, hipStream_t s);

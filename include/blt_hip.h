@@ -190,7 +190,7 @@ int blt_fused_rotary(const void* q, const void* k, void* q_out, void* k_out, int
  *   status     [1]: failures of the calls below (blt_cache_status bits, 0 = none)
  *   sync       [BLT_CACHE_SYNC_WORDS]: zero when the cache is made; counters of blocks that
  *              wait for each other, zero again after every call
- * head_dim 64 or 128; page_size a power of two, 8 .. 1024.  A sequence's last page,
+ * head_dim 64 or 128; page_size a power of two, 8 .. 1024; max_seqs <= 65536.  A sequence's last page,
  * where it is partly filled, belongs to it alone; full pages may be shared.  The
  * calls keep that: they need no host synchronisation and can be captured; calls on one
  * cache must be stream-ordered, attention among them (sync).  A
@@ -224,7 +224,7 @@ typedef enum blt_cache_status {
   BLT_CACHE_NO_PAGE = 16   /* tokens appended where the sequence has no page: left out */
 } blt_cache_status;
 
-/* Device bytes of the workspace of blt_cache_trim, blt_cache_fork (n sequences) and
+/* Device bytes of the workspace of blt_cache_trim (n sequences) and of
  * blt_cache_compact (n = 0); no initialisation; calls that share one must be
  * stream-ordered. */
 int64_t blt_cache_workspace_bytes(const blt_paged_cache* cache, int64_t n);
@@ -245,7 +245,7 @@ int blt_cache_trim(const blt_paged_cache* cache, const int32_t* seqs, const int3
  * tokens) into the lowest free page.  One src may have several dst; none may be a dst
  * of the same call.  All or none. */
 int blt_cache_fork(const blt_paged_cache* cache, const int32_t* src, const int32_t* dst, int64_t n,
-                   void* workspace, int64_t workspace_bytes, blt_stream_t stream);
+                   blt_stream_t stream);
 /* Move the used pages with the highest indices into the free ones with the lowest,
  * both ascending, until the n used pages are pages 0 .. n - 1. */
 int blt_cache_compact(const blt_paged_cache* cache, void* workspace, int64_t workspace_bytes,

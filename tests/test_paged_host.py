@@ -28,13 +28,13 @@ def addr(s):
 @pytest.mark.parametrize("bad,word", [
     (dict(dtype=7), "dtype"), (dict(head_dim=96), "head_dim"), (dict(page_size=24), "page_size"),
     (dict(page_size=4), "page_size"), (dict(page_size=2048), "page_size"),
-    (dict(n_layers=0), "sizes"), (dict(num_pages=0), "sizes"), (dict(max_pages=1 << 21), "sizes"),
+    (dict(n_layers=0), "sizes"), (dict(num_pages=0), "sizes"), (dict(max_pages=1 << 21), "sizes"), (dict(max_seqs=65537), "sizes"),
     (dict(k=0), "null"), (dict(status=0), "null"), (dict(sync=0), "null"), (dict(v=P + 8), "aligned")])
 def test_bad_caches_are_refused(bad, word):
     d = desc(**bad)
     calls = [lambda: L.blt_cache_reserve(addr(d), None, P, 1, None),
              lambda: L.blt_cache_trim(addr(d), None, None, 1, None, 0, None),
-             lambda: L.blt_cache_fork(addr(d), P, P, 1, P, 1 << 20, None),
+             lambda: L.blt_cache_fork(addr(d), P, P, 1, None),
              lambda: L.blt_cache_compact(addr(d), P, 1 << 20, None),
              lambda: L.blt_cache_copy_pages(addr(d), P, P, 1, None),
              lambda: L.blt_cache_append(addr(d), 0, P, 256, 64, P, 256, 64, None, 0, 0, None, 0, 0, 0,
@@ -54,15 +54,16 @@ def test_bad_lists_and_workspaces_are_refused():
     assert L.blt_cache_trim(addr(d), P, P, 2, None, 0, None) == -1
     need = L.blt_cache_workspace_bytes(addr(d), 2)
     assert need > 0 and L.blt_cache_workspace_bytes(addr(d), 0) > 0
-    assert L.blt_cache_fork(addr(d), P, P, 2, P, need - 1, None) == -1
-    assert L.blt_cache_fork(addr(d), P, P, 2, P + 4, need, None) == -1
-    assert L.blt_cache_fork(addr(d), P, None, 2, P, need, None) == -1
+    assert L.blt_cache_trim(addr(d), P, P, 2, P, need - 1, None) == -1
+    assert L.blt_cache_trim(addr(d), P, P, 2, P + 4, need, None) == -1
+    assert L.blt_cache_fork(addr(d), P, None, 2, None) == -1
+    assert L.blt_cache_fork(addr(d), P, P, 8193, None) == -2
     assert L.blt_cache_compact(addr(d), None, 1 << 20, None) == -1
     assert L.blt_cache_copy_pages(addr(d), P, P, -1, None) == -2
     # nothing to do: no launch
     assert L.blt_cache_reserve(addr(d), None, None, 0, None) == 0
     assert L.blt_cache_trim(addr(d), None, None, 0, None, 0, None) == 0
-    assert L.blt_cache_fork(addr(d), None, None, 0, None, 0, None) == 0
+    assert L.blt_cache_fork(addr(d), None, None, 0, None) == 0
     assert L.blt_cache_copy_pages(addr(d), None, None, 0, None) == 0
 
 
