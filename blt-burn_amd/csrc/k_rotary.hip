@@ -126,20 +126,25 @@ __device__ inline void rotate(Piece<T, V>& a, Piece<T, V>& b, const float* c, co
   }
 }
 
+constexpr int HB = 4;  // heads whose pieces a thread has in flight
+
 // How a block's threads are dealt: `units` of a head side by side, `hg` heads (each
 // thread takes every hg-th), then `tb` tokens.
 struct Deal {
   int units, hg, tb;
   int64_t blocks;
 };
-// At least six heads a thread where the tokens fill the chip by themselves, so that
-// the angles (about 150 cycles a pair) are spread over them; every head its own
-// thread below that.
+// Four heads a thread (HB, one batch of loads) where the tokens fill the chip by
+// themselves, so that the angles (about 150 cycles a pair) are spread over them; every
+// head its own thread below that.  [16, 24 heads, 8192, 64] bf16 takes 143 us with four,
+// 146 with three, 151 with six and 159 with twelve.  The angles come before the loads:
+// with the loads issued first, behind the positions and frequencies, it takes 155, and
+// 11,100 appended tokens 46 instead of 40.
 inline Deal deal(int d, int v, int heads, int64_t tokens) {
   Deal t;
   t.units = d / (2 * v);
   const int most = t.units >= 256 ? 1 : 256 / t.units;
-  const int64_t want = tokens * t.units >= (int64_t)256 * 1024 ? (heads + 5) / 6 : heads;
+  const int64_t want = tokens * t.units >= (int64_t)256 * 1024 ? (heads + HB - 1) / HB : heads;
   t.hg = (int)(want < most ? want : most);
   t.tb = 256 / (t.units * t.hg);
   if (t.tb < 1) t.tb = 1;
@@ -147,8 +152,6 @@ inline Deal deal(int d, int v, int heads, int64_t tokens) {
   t.blocks = (tokens + t.tb - 1) / t.tb;
   return t;
 }
-
-constexpr int HB = 4;  // heads whose pieces a thread has in flight
 
 template <typename T, int V>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs p, Deal dl) {
