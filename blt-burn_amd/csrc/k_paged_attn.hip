@@ -72,7 +72,7 @@ struct Item {
   Seq q;
   int kvh, rt, split, ns;  // key head, row tile, part and number of parts
   int nrt;                 // row tiles of the sequence
-  int pslot, join;         // first partial slot and first counter of the sequence
+  int pslot, join;         // first partial slot and first counter of its row tiles
 };
 __device__ inline int lane_of(int v, int l) { return __builtin_amdgcn_readlane(v, l); }
 
@@ -100,53 +100,59 @@ __device__ bool find_item(const KArgs& p, unsigned bid, Item& it) {
   const float blocks = 2.f * tiles > (float)p.resident ? 2.f * p.resident : (float)p.resident;
   const float fill = fmaxf(blocks - 0.5f * tiles, 0.5f * (float)p.resident);
   const int C = max(p.cmin, (int)fminf(ceilf(work * 1.001f / fill), 1e9f));
-  int ns, heads;  // parts of a row tile, row tiles over all heads
-  auto counts = [&]() {
+  int ns;
+  auto parts_of = [&]() {
     // (a part costs as much as a few key tiles to write and join: in proportion to its
     // rows, a quarter of them in the form for 128)
     const int64_t r = (int64_t)q.n * p.G;
     const int most = max(C, p.cmin + (int)(r < BQ ? r : BQ) / (BQ >= 128 ? 4 : 16));
     ns = (kt + most - 1) / most;
-    heads = nrt * p.Hkv;
   };
-  // dispatch places block i on XCD i % 8: each XCD takes a contiguous run of items, so
-  // the row tiles of one key head share its L2
-  int mine = 0;
+  // Items, partial slots and counters of one key head.  Key heads are the outermost order of
+  // the items, and dispatch places block i on XCD i % 8, of which each takes a contiguous
+  // run of items: the row tiles of one (sequence, key head) share an L2, and every XCD gets
+  // its share of the long sequences (2 chunks of 2048 over 16384 and 11854 keys, 8 key
+  // heads: 790 us, 940 with the sequences outermost).
+  int items = 0, parts = 0, joins = 0;
   for (int b0 = 0; b0 < p.B; b0 += 64) {
     if (p.B > 64) {
       q = seq_at(p, b0 + lane);
       tiles_of<BQ, BKV>(p, q, nrt, kt);
     }
-    counts();
-    mine += heads * ns;
+    parts_of();
+    items += nrt * ns;
+    parts += ns > 1 ? nrt * ns : 0;
+    joins += ns > 1 ? nrt : 0;
   }
-  const int all = lane_of(wave_incl_scan(mine), 63);
-  const int per = (all + 7) >> 3;
+  items = lane_of(wave_incl_scan(items), 63);
+  parts = lane_of(wave_incl_scan(parts), 63);
+  joins = lane_of(wave_incl_scan(joins), 63);
+  const int all = items * p.Hkv, per = (all + 7) >> 3;
   const int id = (int)(bid & 7) * per + (int)(bid >> 3);
   if ((int)(bid >> 3) >= per || id >= all) return false;
-  int base = 0, pbase = 0, jbase = 0;
+  it.kvh = id / items;
+  const int rem = id - it.kvh * items;
+  int base = 0, pbase = it.kvh * parts, jbase = it.kvh * joins;
   for (int b0 = 0; b0 < p.B; b0 += 64) {
     if (p.B > 64) {
       q = seq_at(p, b0 + lane);
       tiles_of<BQ, BKV>(p, q, nrt, kt);
     }
-    counts();
-    const int items = heads * ns, parts = ns > 1 ? items : 0, joins = ns > 1 ? heads : 0;
-    const int inc = wave_incl_scan(items);
-    const int pinc = wave_incl_scan(parts), jinc = wave_incl_scan(joins);
-    const uint64_t above = __ballot(base + inc > id);
+    parts_of();
+    const int mine = nrt * ns, split = ns > 1 ? mine : 0, join = ns > 1 ? nrt : 0;
+    const int inc = wave_incl_scan(mine);
+    const int pinc = wave_incl_scan(split), jinc = wave_incl_scan(join);
+    const uint64_t above = __ballot(base + inc > rem);
     if (above) {
       const int l = __ffsll((unsigned long long)above) - 1;
       it.q = Seq{lane_of(q.s0, l), lane_of(q.n, l), lane_of(q.len, l), lane_of(q.slot, l)};
       it.nrt = lane_of(nrt, l);
       it.ns = lane_of(ns, l);
-      it.pslot = pbase + lane_of(pinc - parts, l);
-      it.join = jbase + lane_of(jinc - joins, l);
-      int at = id - (base + lane_of(inc - items, l));
-      it.rt = it.nrt - 1 - at % it.nrt;  // the longest causal rows first
-      at /= it.nrt;
-      it.split = at % it.ns;
-      it.kvh = at / it.ns;
+      it.pslot = pbase + lane_of(pinc - split, l);
+      it.join = jbase + lane_of(jinc - join, l);
+      const int at = rem - (base + lane_of(inc - mine, l));
+      it.split = at / it.nrt;
+      it.rt = it.nrt - 1 - (at - it.split * it.nrt);  // the longest causal rows first
       return true;
     }
     base += lane_of(inc, 63);
@@ -156,7 +162,7 @@ __device__ bool find_item(const KArgs& p, unsigned bid, Item& it) {
   return false;
 }
 __device__ inline int64_t slot_of(const Item& it, int split) {
-  return it.pslot + ((int64_t)it.kvh * it.ns + split) * it.nrt + it.rt;
+  return it.pslot + (int64_t)split * it.nrt + it.rt;
 }
 
 // The keys rows r0 .. r1 (of one sequence) see between them: [lo, hi].
@@ -245,7 +251,7 @@ __device__ void join_parts(const KArgs& p, const Item& it, int nr) {
   __shared__ int last;
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this thread's part, before the count
   __syncthreads();
-  int* counter = p.sync + it.join + it.kvh * it.nrt + it.rt;
+  int* counter = p.sync + it.join + it.rt;
   if (threadIdx.x == 0) {
     last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
            it.ns - 1;
@@ -443,9 +449,9 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(KArgs p) {
               sk + (sub * 32 + lrow) * D + (((2 * ks + lhalf) ^ kswz) << 3));
       f32x16_t s[2];
 #pragma unroll
-      for (int sub = 0; sub < 2; ++sub)
+      for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
+        for (int sub = 0; sub < 2; ++sub)
           s[sub] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
               f[sub][ks], qf[ks], ks == 0 ? f32x16_t{} : s[sub], 0, 0, 0);
       u32x4_t vf[DS][2][2];
@@ -532,7 +538,6 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(KArgs p) {
           for (int r = 0; r < 16; ++r) o[j][r] *= alpha;
       }
       const float mc = m == -INFINITY ? 0.f : -m * c;
-      bf16x8_t pb[2][2];
 #pragma unroll
       for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
@@ -546,16 +551,12 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(KArgs p) {
             l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w[e >> 1]), ones2, l,
                                                 false);
           }
-          pb[sub][u] = __builtin_bit_cast(bf16x8_t, u32x4_t{w[0], w[1], w[2], w[3]});
-        }
+          const bf16x8_t pb = __builtin_bit_cast(bf16x8_t, u32x4_t{w[0], w[1], w[2], w[3]});
 #pragma unroll
-      for (int ds = 0; ds < DS; ++ds)
-#pragma unroll
-        for (int sub = 0; sub < 2; ++sub)
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
+          for (int ds = 0; ds < DS; ++ds)  // (independent chains)
             o[ds] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                __builtin_bit_cast(bf16x8_t, vf[ds][sub][u]), pb[sub][u], o[ds], 0, 0, 0);
+                __builtin_bit_cast(bf16x8_t, vf[ds][sub][u]), pb, o[ds], 0, 0, 0);
+        }
     }
     stage = stage + 1 < NST ? stage + 1 : 0;
   }
