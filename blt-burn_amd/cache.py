@@ -91,8 +91,6 @@ class PagedCache:
         self._ptr = ctypes.addressof(self._desc)
         self._lib = _lib.lib()
         self._piece, self._scale = 16 // k.element_size(), self.head_dim ** -0.5
-        if self._lib.blt_cache_workspace_bytes(self._ptr, 0) <= 0:
-            raise BltError("PagedCache: bad sizes")
         # the library's own checks, once: an empty list does nothing else
         self._call(self._lib.blt_cache_reserve, "PagedCache", self._ptr, None, None, 0)
         # parts of attention calls, of whichever form needs most
@@ -155,8 +153,9 @@ class PagedCache:
     def compact(self):
         """Move the used pages with the highest indices into the lowest free ones."""
         size = self._lib.blt_cache_workspace_bytes(self._ptr, 0)
-        ws = self._workspace(size)
-        self._call(self._lib.blt_cache_compact, "cache_compact", self._ptr, ws.data_ptr(), size)
+        ws = self._workspace(size) if size else None
+        self._call(self._lib.blt_cache_compact, "cache_compact", self._ptr,
+                   ws.data_ptr() if size else None, size)
 
     def copy_pages(self, src, dst):
         """Copy page src[i] to page dst[i] in every layer (no index twice in dst, none in

@@ -414,7 +414,8 @@ static int list_checks(const blt_paged_cache* c, int64_t n, const char* what) {
 }
 static int workspace_checks(const blt_paged_cache* c, int64_t n, const void* ws, int64_t bytes,
                             const char* what) {
-  if (!ws || ((uintptr_t)ws & 15) || bytes < cache_workspace_bytes(*c, n))
+  const int64_t need = cache_workspace_bytes(*c, n);
+  if (need > 0 && (!ws || ((uintptr_t)ws & 15) || bytes < need))
     return fail(BLT_ERR_INVALID, std::string(what) + ": workspace missing, misaligned or too small");
   return 0;
 }

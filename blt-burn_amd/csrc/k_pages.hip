@@ -420,17 +420,73 @@ __global__ __launch_bounds__(NT) void trim_split_kernel(blt_paged_cache c, int l
 }
 
 // ---- compact -------------------------------------------------------------------
+// With n pages in use, the used ones at n and above move into the free ones below, both
+// ascending.  As in a fork every block decides for itself and the last one writes the
+// counts.  The lists are in LDS where the pool is small enough (FIT: one launch); for
+// larger ones compact_kernel writes them, and the map of the pages, for compact_copy_kernel.
+constexpr int FIT = 8192;  // pairs whose lists fit: pools of up to twice as many pages
+// f(page, ordinal) of the holes, g of the movers; returns how many, and n
+template <typename F, typename G>
+__device__ int find_pairs(const blt_paged_cache& c, int* part, int& live, F f, G g) {
+  const int P = c.num_pages;
+  live = walk_pages<false>(c.refcount, P, P, part, [](int, int) {});
+  const int holes = walk_pages<true>(c.refcount, live, P, part, f);
+  const int n = live;
+  walk_pages<false>(c.refcount + n, P - n, P, part, [&](int page, int o) { g(page + n, o); });
+  return holes;
+}
+__global__ __launch_bounds__(NT) void compact_fit_kernel(blt_paged_cache c, int lps, int es) {
+  __shared__ int hole[FIT], mover[FIT];
+  __shared__ int part[NT / 64];
+  __shared__ int last;
+  const int tid = threadIdx.x;
+  int live;
+  const int pairs = find_pairs(
+      c, part, live, [&](int page, int o) { hole[o] = page; },
+      [&](int page, int o) { mover[o] = page; });
+  __syncthreads();
+  if (pairs > 0) {
+    const int64_t cols = c.max_pages, threads = (int64_t)gridDim.x * NT;
+    for (int64_t x = (int64_t)blockIdx.x * NT + tid; x < c.max_seqs * cols; x += threads) {
+      const int64_t s = x / cols;
+      if (x - s * cols >= pages_of(c.lens[s], lps)) continue;
+      const int page = c.page_table[x];
+      if (page < live) continue;
+      int lo = 0, hi = pairs;  // mover[lo] <= page
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (mover[mid] <= page) lo = mid; else hi = mid;
+      }
+      if (mover[lo] == page) c.page_table[x] = hole[lo];
+    }
+    const int per = c.n_layers * 2;  // four teams of 256 threads
+    for (int64_t it = (int64_t)blockIdx.x * 4 + (tid >> 8); it < (int64_t)pairs * per;
+         it += (int64_t)gridDim.x * 4) {
+      const int o = (int)(it / per), r = (int)(it - (int64_t)o * per);
+      copy_tokens(c, mover[o], hole[o], c.page_size, r >> 1, r & 1, es, tid & 255);
+    }
+  }
+  __syncthreads();
+  if (tid == 0)
+    last = __hip_atomic_fetch_add(c.sync, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+           (int)gridDim.x - 1;
+  __syncthreads();
+  if (!last) return;
+  if (tid == 0) __hip_atomic_store(c.sync, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  for (int o = tid; o < pairs; o += NT) {
+    c.refcount[hole[o]] = c.refcount[mover[o]];
+    c.refcount[mover[o]] = 0;
+  }
+}
 __global__ __launch_bounds__(NT) void compact_kernel(blt_paged_cache c, Lists l) {
   __shared__ int part[NT / 64];
-  const int tid = threadIdx.x, P = c.num_pages;
-  const int live = walk_pages<false>(c.refcount, P, P, part, [](int, int) {});
-  // holes: free pages below `live`; as many used ones lie above it
-  const int holes = walk_pages<true>(c.refcount, live, P, part,
-                                     [&](int page, int o) { l.dst[o] = page; });
-  walk_pages<false>(c.refcount + live, P - live, P, part,
-                    [&](int page, int o) { l.src[o] = page + live; });
+  const int tid = threadIdx.x;
+  int live;
+  const int pairs = find_pairs(
+      c, part, live, [&](int page, int o) { l.dst[o] = page; },
+      [&](int page, int o) { l.src[o] = page; });
   __syncthreads();
-  for (int o = tid; o < holes; o += NT) {
+  for (int o = tid; o < pairs; o += NT) {
     const int from = l.src[o], to = l.dst[o];
     c.refcount[to] = c.refcount[from];
     c.refcount[from] = 0;
@@ -438,7 +494,7 @@ __global__ __launch_bounds__(NT) void compact_kernel(blt_paged_cache c, Lists l)
     l.fill[o] = c.page_size;
   }
   if (tid == 0) {
-    l.count[0] = holes;
+    l.count[0] = pairs;
     l.count[1] = live;
   }
 }
@@ -461,6 +517,7 @@ constexpr int kCopyBlocks = 2048;  // eight 256-thread blocks on each of 256 CUs
 }  // namespace
 
 int64_t cache_workspace_bytes(const blt_paged_cache& c, int64_t n) {
+  if (n == 0 && c.num_pages <= 2 * FIT) return 0;
   return (16 + 3 * list_cap(c, n) + (n > 0 ? 0 : (int64_t)c.num_pages)) * 4;
 }
 
@@ -503,6 +560,13 @@ int launch_cache_fork(const blt_paged_cache& c, const int32_t* src, const int32_
 }
 
 int launch_cache_compact(const blt_paged_cache& c, void* ws, hipStream_t s) {
+  if (c.num_pages <= 2 * FIT) {
+    const unsigned nb = (copy_blocks(c, c.num_pages / 2) + 3) / 4;
+    hipLaunchKernelGGL(compact_fit_kernel, dim3(nb < 512 ? nb : 512), dim3(NT), 0, s, c,
+                       log2_of(c.page_size), elem_size(c));
+    BLT_LAUNCH_CHECK("compact_fit_kernel");
+    return 0;
+  }
   const Lists l = lists_of(c, 0, ws);
   hipLaunchKernelGGL(compact_kernel, dim3(1), dim3(NT), 0, s, c, l);
   BLT_LAUNCH_CHECK("compact_kernel");

@@ -225,7 +225,7 @@ typedef enum blt_cache_status {
 } blt_cache_status;
 
 /* Device bytes of the workspace of blt_cache_trim (n sequences) and of
- * blt_cache_compact (n = 0); no initialisation; calls that share one must be
+ * blt_cache_compact (n = 0; none for pools of up to 16384 pages); no initialisation; calls that share one must be
  * stream-ordered. */
 int64_t blt_cache_workspace_bytes(const blt_paged_cache* cache, int64_t n);
 /* Grow sequence seqs[i] by counts[i] tokens (seqs NULL: sequence i), i < n <= 8192:

@@ -504,10 +504,13 @@ def test_pages_random_walk(dtype, page, d, seed):
     assert seen_full
 
 
-def test_pages_larger_than_one_step_and_many_entries():
+@pytest.mark.parametrize("P", [9001, 20003])  # lists in LDS, and in the workspace
+def test_pages_larger_than_one_step_and_many_entries(P):
     """More pages than one block step reads and more entries than threads."""
     S, page = 3000, 8
-    m = Made([0], Hkv=1, d=64, page=page, spare=9001, slots=S, columns=8, seed=2)
+    m = Made([0], Hkv=1, d=64, page=page, spare=P, slots=S, columns=8, seed=2)
+    m.cache.k.nan_to_num_(0.0)
+    m.cache.v.nan_to_num_(0.0)
     c, pool = m.cache, m.pool()
     rng = np.random.default_rng(1)
     cnt = rng.integers(0, 20, S)
@@ -530,9 +533,13 @@ def test_pages_larger_than_one_step_and_many_entries():
     c.trim(i32(lens))
     c.check()
     same(c, pool, False)
+    # contents, told apart by their page
+    c.k.add_(torch.arange(P, device=DEV).view(1, -1, 1, 1, 1) % 251)
+    c.v.add_(torch.arange(P, device=DEV).view(1, -1, 1, 1, 1) % 241)
+    pool.k, pool.v = f64(c.k), f64(c.v)
     pool.compact()
     c.compact()
-    same(c, pool, False)
+    same(c, pool)
 
 
 def test_pages_failures_change_nothing():

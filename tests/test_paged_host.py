@@ -53,12 +53,13 @@ def test_bad_lists_and_workspaces_are_refused():
     assert L.blt_cache_reserve(addr(d), None, P, 5, None) == -2   # more than max_seqs
     assert L.blt_cache_trim(addr(d), P, P, 2, None, 0, None) == -1
     need = L.blt_cache_workspace_bytes(addr(d), 2)
-    assert need > 0 and L.blt_cache_workspace_bytes(addr(d), 0) > 0
+    big = desc(num_pages=20000)
+    assert need > 0 and L.blt_cache_workspace_bytes(addr(big), 0) > 0
     assert L.blt_cache_trim(addr(d), P, P, 2, P, need - 1, None) == -1
     assert L.blt_cache_trim(addr(d), P, P, 2, P + 4, need, None) == -1
     assert L.blt_cache_fork(addr(d), P, None, 2, None) == -1
     assert L.blt_cache_fork(addr(d), P, P, 8193, None) == -2
-    assert L.blt_cache_compact(addr(d), None, 1 << 20, None) == -1
+    assert L.blt_cache_compact(addr(big), None, 1 << 20, None) == -1
     assert L.blt_cache_copy_pages(addr(d), P, P, -1, None) == -2
     # nothing to do: no launch
     assert L.blt_cache_reserve(addr(d), None, None, 0, None) == 0
