@@ -223,6 +223,7 @@ def prepare(case, seed):
         st = dict(case=c, q=x[:, :H], k=x[:, H:], pos=pos)
         if own:
             F = _package("fused_ops")
+            st["fused_rotary"] = F.fused_rotary
             st["plan"] = F.RotaryPlan(c["rot"], theta=THETA, pairs=c["pairs"],
                                       scaling=c["scaling"], factor=c["factor"],
                                       original_len=ORIGINAL, device=DEV)
@@ -294,8 +295,7 @@ def _turned(x, cos, sin, pairs):
 def _rotary(st):
     c = st["case"]
     if own:
-        return _package("fused_ops").fused_rotary(st["q"], st["k"], st["pos"], st["plan"],
-                                                  backward=c["back"])
+        return st["fused_rotary"](st["q"], st["k"], st["pos"], st["plan"], backward=c["back"])
     f, mag = _inv_freq(c["rot"], c["scaling"], c["factor"], ORIGINAL)
     angle = st["pos"].double()[:, None] * f
     cos, sin = (angle.cos() * mag).float(), (angle.sin() * (-mag if c["back"] else mag)).float()
