@@ -219,36 +219,51 @@ __global__ __launch_bounds__(256) void append_kernel(AppendKernelArgs p, Deal dl
   const int tid = threadIdx.x, lane = tid & 63;
   const int u0 = tid % dl.units, rest = tid / dl.units;
   const int h0 = rest % dl.hg, tt = rest / dl.hg;
-  // the sequence of the block's first token: how many starts[1 ..] are at or below
-  // it, counted by every wave for itself
-  const int64_t tok0 = (int64_t)blockIdx.x * dl.tb;
-  int b = 0;
-  for (int64_t i = 0; i < a.B; i += 64) {
-    const bool le = i + lane < a.B && a.starts[i + lane + 1] <= tok0;
-    const uint64_t m = __ballot(le);
-    b += __popcll(m);
-    if (m != ~0ull) break;
+  const int64_t tok0 = (int64_t)blockIdx.x * dl.tb, tok = tok0 + tt;
+  const bool mine = tt < dl.tb && tok < a.total;
+  // The token's row b: the number of starts[1 ..] at or below it; its first token and
+  // length.  Up to 64 rows a wave holds them all, one round of loads ahead of the page's;
+  // beyond that every wave counts for the block's first token and goes on from there.
+  int64_t s0, n;
+  int seq, len;
+  if (a.B <= 64) {
+    const int i = lane < a.B ? lane : (int)a.B - 1;
+    const int lo = a.starts[i], hi = a.starts[i + 1];
+    const int sq = a.seqs ? a.seqs[i] : i;
+    const int ln = c.lens[sq >= 0 && sq < c.max_seqs ? sq : 0];
+    int b = __popcll(__ballot(lane < a.B && hi <= tok0));
+    // (every lane takes part in the shuffles; tokens past the last row stop at 64)
+    for (int next = __shfl(hi, b & 63); __any(b < a.B && next <= tok); next = __shfl(hi, b & 63))
+      b += b < a.B && next <= tok ? 1 : 0;
+    s0 = __shfl(lo, b & 63);
+    n = __shfl(hi, b & 63) - s0;
+    seq = __shfl(sq, b & 63);
+    len = __shfl(ln, b & 63);
+    if (!mine || b >= a.B) return;  // behind the last row
+  } else {
+    int b = 0;
+    for (int64_t i = 0; i < a.B; i += 64) {
+      const bool le = i + lane < a.B && a.starts[i + lane + 1] <= tok0;
+      const uint64_t m = __ballot(le);
+      b += __popcll(m);
+      if (m != ~0ull) break;
+    }
+    if (!mine) return;
+    while (b < a.B && a.starts[b + 1] <= tok) ++b;
+    if (b >= a.B) return;
+    s0 = a.starts[b];
+    n = a.starts[b + 1] - s0;
+    seq = a.seqs ? a.seqs[b] : b;
+    len = c.lens[seq >= 0 && seq < c.max_seqs ? seq : 0];
   }
-  const int64_t tok = tok0 + tt;
-  if (tt >= dl.tb || tok >= a.total) return;
-  while (b < a.B && a.starts[b + 1] <= tok) ++b;
-  if (b >= a.B) return;  // behind the last sequence
-  const int64_t s0 = a.starts[b], n = a.starts[b + 1] - s0;
   if (tok < s0) return;
-  const int seq = a.seqs ? a.seqs[b] : b;
   const bool known = seq >= 0 && seq < c.max_seqs;
-  const int64_t pos = (known ? c.lens[seq] : 0) - n + (tok - s0);
+  const int64_t pos = (known ? len : 0) - n + (tok - s0);
   // where k and v go: no page where an index is out of range or a failure is pending
-  int64_t at = -1;
-  if (known && pos >= 0 && (pos >> p.lps) < c.max_pages) {
-    const int page = c.page_table[(int64_t)seq * c.max_pages + (pos >> p.lps)];
-    if (page >= 0 && page < c.num_pages)
-      at = p.layer0 + (((int64_t)page * c.n_kv_heads) << p.lps) * c.head_dim +
-           (pos & (c.page_size - 1)) * c.head_dim;
-  }
-  const bool bad = at < 0;
-  if (*c.status & kCachePending) at = -1;
-  if (bad && u0 == 0 && h0 == 0) atomicOr(c.status, BLT_CACHE_NO_PAGE);
+  // (looked at behind the angles, which need not wait for it)
+  const bool inside = known && pos >= 0 && (pos >> p.lps) < c.max_pages;
+  const int page = inside ? c.page_table[(int64_t)seq * c.max_pages + (pos >> p.lps)] : -1;
+  const int status = *c.status;
 
   const Unit<V> un = unit_of<V>(u0, a.r);
   float cs[V], sn[V];
@@ -260,8 +275,14 @@ __global__ __launch_bounds__(256) void append_kernel(AppendKernelArgs p, Deal dl
       sn[e] *= a.r.magnitude;
     }
   }
+  const bool bad = page < 0 || page >= c.num_pages;
+  if (bad && u0 == 0 && h0 == 0) atomicOr(c.status, BLT_CACHE_NO_PAGE);
   const int Hk = c.n_kv_heads, heads = a.Hq + 2 * Hk;
   const int64_t sh_page = (int64_t)c.head_dim << p.lps;
+  const int64_t at = bad || (status & kCachePending)
+                         ? -1
+                         : p.layer0 + (int64_t)page * c.n_kv_heads * sh_page +
+                               (pos & (c.page_size - 1)) * c.head_dim;
   for (int hb = h0; hb < heads; hb += HB * dl.hg) {
     Piece<T, V> x[HB], y[HB];
 #pragma unroll
