@@ -263,24 +263,37 @@ __device__ void join_parts(const KArgs& p, const Item& it, int nr) {
   for (int i = threadIdx.x; i < nr * (D / 4); i += NT) {
     const int r = i / (D / 4), dd = (i % (D / 4)) * 4;
     const int64_t s0 = slot_of(it, 0) * BQ + r;
-    float mx = -INFINITY;
-#pragma unroll 8
-    for (int x = 0; x < it.ns; ++x) {
-      float m, l;
-      get2(p.ml + (s0 + x * step) * 2, m, l);
-      mx = fmaxf(mx, m);
-    }
-    const float mu = mx == -INFINITY ? 0.f : mx;
+    // eight parts at a time, everything of them in flight at once (a read that passes the
+    // L2 takes about 2 us), with a running max
+    constexpr int U = 8;
+    float mx = -INFINITY, lt = 0.f;
     f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-    float lt = 0.f;
-#pragma unroll 8
-    for (int x = 0; x < it.ns; ++x) {
-      float m, l;
-      get2(p.ml + (s0 + x * step) * 2, m, l);
-      const f32x4_t o = get4(p.part + (s0 + x * step) * D + dd);
-      const float w = __builtin_amdgcn_exp2f((m - mu) * p.c);
-      lt = fmaf(w, l, lt);
-      acc += w * o;
+    for (int x0 = 0; x0 < it.ns; x0 += U) {
+      float m[U], l[U];
+      f32x4_t o[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t at = s0 + min(x0 + u, it.ns - 1) * step;
+        get2(p.ml + at * 2, m[u], l[u]);
+        o[u] = get4(p.part + at * D + dd);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)  // (past the last part: the last one again, without weight)
+        if (x0 + u >= it.ns) m[u] = -INFINITY;
+      float mn = mx;
+#pragma unroll
+      for (int u = 0; u < U; ++u) mn = fmaxf(mn, m[u]);
+      const float mu = mn == -INFINITY ? 0.f : mn;
+      const float alpha = __builtin_amdgcn_exp2f((mx - mu) * p.c);
+      mx = mn;
+      lt *= alpha;
+      acc *= alpha;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float w = __builtin_amdgcn_exp2f((m[u] - mu) * p.c);
+        lt = fmaf(w, l[u], lt);
+        acc += w * o[u];
+      }
     }
     const int row = it.rt * BQ + r, t = row / p.G, g = row - t * p.G;
     const int64_t at =
