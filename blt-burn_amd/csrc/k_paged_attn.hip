@@ -75,6 +75,9 @@ struct Item {
   int pslot, join;         // first partial slot and first counter of its row tiles
 };
 __device__ inline int lane_of(int v, int l) { return __builtin_amdgcn_readlane(v, l); }
+__device__ inline float uniform(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
+}
 
 // The item of block `bid`, false if it has none.  Every wave computes it by itself, in
 // the same order, so all agree.
@@ -90,8 +93,9 @@ __device__ bool find_item(const KArgs& p, unsigned bid, Item& it) {
     work += (float)nrt * (float)kt;
     tiles += (float)nrt;
   }
-  work = wave_sum(work) * (float)p.Hkv;
-  tiles = wave_sum(tiles) * (float)p.Hkv;
+  // (one value for the wave, in scalar registers: what follows from it stays there too)
+  work = uniform(wave_sum(work)) * (float)p.Hkv;
+  tiles = uniform(wave_sum(tiles)) * (float)p.Hkv;
   // Items should fill the chip's resident blocks once, or twice where there are so many row
   // tiles that items of a single round would differ much in size.  Row tiles that are no
   // whole number of C make half an item more each, on average: so work / C = blocks -
@@ -99,7 +103,7 @@ __device__ bool find_item(const KArgs& p, unsigned bid, Item& it) {
   // hold whatever the rounding of the sums.)
   const float blocks = 2.f * tiles > (float)p.resident ? 2.f * p.resident : (float)p.resident;
   const float fill = fmaxf(blocks - 0.5f * tiles, 0.5f * (float)p.resident);
-  const int C = max(p.cmin, (int)fminf(ceilf(work * 1.001f / fill), 1e9f));
+  int C = max(p.cmin, (int)fminf(ceilf(work * 1.001f / fill), 1e9f));
   int ns;
   auto parts_of = [&]() {
     // (a part costs as much as a few key tiles to write and join: in proportion to its
@@ -113,18 +117,26 @@ __device__ bool find_item(const KArgs& p, unsigned bid, Item& it) {
   // run of items: the row tiles of one (sequence, key head) share an L2, and every XCD gets
   // its share of the long sequences (2 chunks of 2048 over 16384 and 11854 keys, 8 key
   // heads: 790 us, 940 with the sequences outermost).
-  int items = 0, parts = 0, joins = 0;
-  for (int b0 = 0; b0 < p.B; b0 += 64) {
-    if (p.B > 64) {
-      q = seq_at(p, b0 + lane);
-      tiles_of<BQ, BKV>(p, q, nrt, kt);
+  int items, parts, joins;
+  for (int tries = 0;; ++tries) {
+    items = parts = joins = 0;
+    for (int b0 = 0; b0 < p.B; b0 += 64) {
+      if (p.B > 64) {
+        q = seq_at(p, b0 + lane);
+        tiles_of<BQ, BKV>(p, q, nrt, kt);
+      }
+      parts_of();
+      items += nrt * ns;
+      parts += ns > 1 ? nrt * ns : 0;
+      joins += ns > 1 ? nrt : 0;
     }
-    parts_of();
-    items += nrt * ns;
-    parts += ns > 1 ? nrt * ns : 0;
-    joins += ns > 1 ? nrt : 0;
+    items = lane_of(wave_incl_scan(items), 63);
+    // a few items above a whole round would take one of their own: fewer, larger parts
+    // (8 sequences of 49152 keys, 12 heads: 1056 items 295 us, 960 of them 213)
+    const float over = (float)items * (float)p.Hkv / blocks;
+    if (over <= 1.f || tiles > blocks || tries == 3) break;
+    C = max(C + 1, (int)(over * (float)C));
   }
-  items = lane_of(wave_incl_scan(items), 63);
   parts = lane_of(wave_incl_scan(parts), 63);
   joins = lane_of(wave_incl_scan(joins), 63);
   const int all = items * p.Hkv, per = (all + 7) >> 3;
@@ -605,8 +617,8 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(KArgs p) {
 
 // ---- bf16, few rows ----------------------------------------------------------------
 // Up to 16 NR rows (single tokens, short chunks): bound by reading K and V once, so the
-// four waves of a block share nothing and wait for nothing but their own loads: each takes
-// every NW-th 32-key tile of the item through its own LDS ring of NST tiles, filled by DMA
+// waves of a block share nothing and wait for nothing but their own loads: each takes
+// every NW-th 32-key tile of the item through its own LDS ring of two tiles, filled by DMA
 // while the tiles before are consumed, and they meet once at the end.  16 x 16 x 32
 // MFMAs, scores transposed as above (a lane owns a row, the key blocks' registers are the
 // second product's operand).  p goes into that product as two bf16 halves (p rounded, and
@@ -616,10 +628,10 @@ template <int N>
 __device__ inline void wait_loads() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
-template <int D, int NR, int NW, int NST>
+template <int D, int NR, int NW>
 __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(KArgs p) {
-  constexpr int KT = 32, BKV = 64, BQ = 16 * NR, TILE = KT * D;
-  constexpr int OPS = 2 * 4 * (D / 64);  // DMA instructions of a tile
+  constexpr int KT = 32, BKV = 64, BQ = 16 * NR, TILE = KT * D, NST = 2;
+  constexpr int OPS = 4 * (D / 64);  // DMA instructions of a K (or V) tile
   constexpr int KS = D / 32, DB = D / 16, OP = D + 4, PTF = 1024;
   constexpr int RING = NW * NST * 2 * TILE;  // elements
   static_assert(RING * 2 >= NW * BQ * OP * 4, "the waves' outputs fit the rings");
@@ -668,37 +680,47 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(KArgs p) {
   const int kx = slot ^ (D == 64 ? kin >> 1 : kin);
   const int vx = slot ^ (D == 64 ? 2 * (kin >> 1) : 2 * kin);
   int wbase = 0;
-  auto issue = [&](int t, int stage) {
-    const unsigned sb = ring + (unsigned)(stage * 2 * TILE * 2);
-    int pg[4], kc[4];
+  // byte offsets of a tile's groups of eight keys in K and V (past the end: the last group)
+  struct Groups {
+    int64_t at[4];
+  };
+  auto group = [&](int t, int g) { return min(t * KT + 8 * g, (sq.len - 1) & ~7); };
+  auto place = [&](int t) {
+    int pg[4];
+    Groups x;
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      kc[g] = min(t * KT + 8 * g, (sq.len - 1) & ~7);
-      pg[g] = ptab[(kc[g] >> p.lps) - wbase];
-    }
-    // (also: this wave's operand reads of the stage are done)
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    for (int g = 0; g < 4; ++g) pg[g] = ptab[(group(t, g) >> p.lps) - wbase];
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int page = __builtin_amdgcn_readfirstlane(pg[g]);
-      const int64_t off =
-          (((((int64_t)page * p.Hkv + it.kvh) << p.lps) + (kc[g] & ((1 << p.lps) - 1))) * D) * 2;
-      const char* kb = (const char*)p.k + off;
-      const char* vb = (const char*)p.v + off;
+      x.at[g] = (((((int64_t)page * p.Hkv + it.kvh) << p.lps) +
+                  (group(t, g) & ((1 << p.lps) - 1))) * D) * 2;
+    }
+    return x;
+  };
+  auto issue = [&](int t, int stage, const Groups& x, auto of_v) {
+    constexpr bool V = decltype(of_v)::value;
+    const unsigned sb = ring + (unsigned)(stage * 2 * TILE * 2) + (V ? TILE * 2 : 0);
+    // (this wave's operand reads of the stage are done)
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const char* base = (const char*)(V ? p.v : p.k) + x.at[g];
       const int key0 = t * KT + 8 * g;
       const bool all = key0 + 8 <= sq.len;
 #pragma unroll
       for (int h = 0; h < D / 64; ++h) {
         int row = kin + (D == 128 ? 4 * h : 0);
-        if (!all) row = min(key0 + row, sq.len - 1) - kc[g];
-        const int kch = kx ^ (D == 64 ? 4 * (g & 1) : 8 * (g & 1) + 4 * h);
-        const int vch = D == 64 ? vx : vx ^ (8 * h);
-        const unsigned la = sb + (unsigned)(8 * g * D * 2 + h * 1024);
-        dma16_so(kb, (unsigned)(row * D * 2 + kch * 16), la);
-        dma16_so(vb, (unsigned)(row * D * 2 + vch * 16), la + TILE * 2);
+        if (!all) row = min(key0 + row, sq.len - 1) - group(t, g);
+        const int ch = V ? (D == 64 ? vx : vx ^ (8 * h))
+                         : kx ^ (D == 64 ? 4 * (g & 1) : 8 * (g & 1) + 4 * h);
+        dma16_so(base, (unsigned)(row * D * 2 + ch * 16),
+                 sb + (unsigned)(8 * g * D * 2 + h * 1024));
       }
     }
   };
+  constexpr std::false_type of_k{};
+  constexpr std::true_type of_v{};
   // operand reads: K row `col` of a 16-key block; V rows 4 g4 + col / 4, 16 columns at 16 db
   const int kswz = D == 64 ? (col >> 1) & 7 : col;
   const int vrow = 4 * g4 + (col >> 2);
@@ -716,7 +738,11 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(KArgs p) {
   }
   const float c = p.c, grow_at = 8.f / p.c;
 
-  auto tile = [&](int t, int stage) {
+  // Tile t of this wave; `more` follow.  A half of the ring is refilled as soon as
+  // it is read: K of tile t + 2 under the softmax of t, V behind its second product, so
+  // three halves or more are on their way at any time.
+  auto tile = [&](int t, int stage, int more) {
+    if (more >= 1) wait_loads<3 * OPS>(); else wait_loads<OPS>();  // K has landed
     const uint16_t* sk = lds + (w * NST + stage) * 2 * TILE;
     const uint16_t* sv = sk + TILE;
     const int kb = t * KT;
@@ -733,6 +759,11 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(KArgs p) {
               a, qf[n][ks], ks == 0 ? f32x4_t{} : s[n][b], 0, 0, 0);
         }
       }
+    Groups next{};
+    if (more >= 2) {
+      next = place(t + 2 * NW);
+      issue(t + 2 * NW, stage, next, of_k);
+    }
     const bool mask = kb + KT - 1 > all_hi || kb < all_lo;
     bf16x8_t ph[NR], pl[NR];
 #pragma unroll
@@ -777,6 +808,7 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(KArgs p) {
       ph[n] = __builtin_bit_cast(bf16x8_t, u32x4_t{wh[0], wh[1], wh[2], wh[3]});
       pl[n] = __builtin_bit_cast(bf16x8_t, u32x4_t{wl[0], wl[1], wl[2], wl[3]});
     }
+    if (more >= 2) wait_loads<3 * OPS>(); else if (more == 1) wait_loads<2 * OPS>(); else wait_loads<0>();
     u32x4_t vf[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d) {
@@ -825,6 +857,7 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(KArgs p) {
         o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, pl[n], o[n][d], 0, 0, 0);
       }
     }
+    if (more >= 2) issue(t + 2 * NW, stage, next, of_v);
   };
 
   // runs of tiles whose pages ptab holds (one, but for very long parts)
@@ -843,23 +876,15 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(KArgs p) {
       }
     }
     __syncthreads();
-    int at = ta + w;  // next tile to issue
+    const int mine = (tb - ta - w + NW - 1) / NW;  // this wave's tiles
 #pragma unroll
-    for (int i = 0; i < NST - 1; ++i, at += NW)
-      if (at < tb) issue(at, i);
-    int stage = 0;
-    for (int t = ta + w; t < tb; t += NW) {
-      if (at < tb) issue(at, stage == 0 ? NST - 1 : stage - 1);
-      at += NW;
-      // tiles behind t that are in flight
-      const int left = min(NST - 1, (tb - 1 - t) / NW);
-      if (left >= 3) wait_loads<3 * OPS < 63 ? 3 * OPS : 63>();
-      else if (left == 2) wait_loads<2 * OPS>();
-      else if (left == 1) wait_loads<OPS>();
-      else wait_loads<0>();
-      tile(t, stage);
-      stage = stage + 1 < NST ? stage + 1 : 0;
-    }
+    for (int i = 0; i < 2; ++i)
+      if (i < mine) {
+        const Groups x = place(ta + w + i * NW);
+        issue(ta + w + i * NW, i, x, of_k);
+        issue(ta + w + i * NW, i, x, of_v);
+      }
+    for (int i = 0; i < mine; ++i) tile(ta + w + i * NW, i & 1, mine - 1 - i);
   }
 
   // ---- the waves' partial results ----
@@ -1179,10 +1204,10 @@ int run_paged(const KArgs& p, const Shape& sh, unsigned nb, hipStream_t s) {
       hipLaunchKernelGGL((paged_attn_kernel<D, 2>), grid, block, 0, s, p);
       break;
     case FORM_FEW16:
-      hipLaunchKernelGGL((paged_attn_few_kernel<D, 1, 2, 2>), grid, dim3(128), 0, s, p);
+      hipLaunchKernelGGL((paged_attn_few_kernel<D, 1, 2>), grid, dim3(128), 0, s, p);
       break;
     case FORM_FEW32:
-      hipLaunchKernelGGL((paged_attn_few_kernel<D, 2, 2, 2>), grid, dim3(128), 0, s, p);
+      hipLaunchKernelGGL((paged_attn_few_kernel<D, 2, 2>), grid, dim3(128), 0, s, p);
       break;
     default:
       hipLaunchKernelGGL((paged_attn_f32_kernel<D / 32>), grid, block, 0, s, p);
