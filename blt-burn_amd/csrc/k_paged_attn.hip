@@ -1178,9 +1178,14 @@ struct Shape {
   Form form;
   int bq, bkv, resident, cmin;
 };
-// (2 * resident <= BLT_CACHE_SYNC_WORDS: a counter for every row tile with parts)
+// resident: blocks the chip holds at once by their registers and LDS (f32 with d = 128: one
+// per CU; with two assumed, 3 chunks of 100 tokens over 1500 keys, 32 / 8 heads, took 85 us
+// instead of 68).  2 * resident <= BLT_CACHE_SYNC_WORDS: a counter for every row tile with
+// parts.  The form goes by the rows a sequence has on average: a tile of 16 rows costs the
+// matrix cores half of one of 32, and 128 rows share what they read; every form takes any
+// chunk, in more row tiles.
 Shape shape_of(const blt_paged_cache& c, int64_t B, int64_t total, int H) {
-  if (c.dtype == BLT_DTYPE_F32) return Shape{FORM_F32, 32, 32, 512, 4};
+  if (c.dtype == BLT_DTYPE_F32) return Shape{FORM_F32, 32, 32, c.head_dim == 64 ? 512 : 256, 4};
   const int64_t rows = total * (H / c.n_kv_heads);  // of all sequences, per key head
   const int few = c.head_dim == 64 ? 1024 : 512;  // 32 and 64 KB of rings
   if (rows <= 16 * B) return Shape{FORM_FEW16, 16, 64, few, 2};

@@ -243,6 +243,124 @@ def test_attention_long_contexts_in_parts(dtype, d, H, Hkv, page):
     check_attention(m, [1, 1, 5], H, window=4100)
 
 
+def attention_on_device(q, keys, values, length, window=0):
+    """R.attention in 64-bit torch on the GPU, for the large cases."""
+    n, H, d = q.shape
+    out, mag = (torch.zeros(n, H, d, dtype=torch.float64, device=DEV) for _ in range(2))
+    pos = torch.arange(length - n, length, device=DEV)[:, None]
+    j = torch.arange(length, device=DEV)
+    hide = j > pos
+    if window:
+        hide |= j <= pos - window
+    for h in range(H):
+        g = h * keys.shape[1] // H
+        p = (q[:, h].double() @ keys[:, g].double().t()) * d ** -0.5
+        p = torch.softmax(p.masked_fill_(hide, -float("inf")), -1)
+        out[:, h], mag[:, h] = p @ values[:, g].double(), p @ values[:, g].double().abs()
+    return out.cpu().numpy(), mag.cpu().numpy()
+
+
+def device_rows(m, which, s):
+    x, n = m.kv[which][0], m.lens[s]
+    pages = torch.tensor(m.table[s, :-(-n // m.page)], device=DEV, dtype=torch.long)
+    return x[pages].transpose(1, 2).reshape(-1, x.shape[1], x.shape[3])[:n]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_attention_long_items_reload_their_pages(dtype):
+    """So many row tiles that none is split, over more pages of 8 than an item's run of
+    page indices in LDS."""
+    n, L, H = (4100, 8200, 16) if dtype == "bf16" else (1100, 8200, 16)
+    m = Made([L], Hkv=H, d=64, page=8, dtype=TYPES[dtype])
+    torch.manual_seed(2)
+    q = torch.randn(n, H, 64, device=DEV).to(TYPES[dtype])
+    o = m.cache.attention(0, q, i32([0, n]))
+    k, v = device_rows(m, 0, 0), device_rows(m, 1, 0)
+    for a in (0, n // 2, n - 300):  # 300 rows at a time
+        rows = slice(a, a + 300)
+        keep = L - n + a + 300
+        want, A = attention_on_device(q[rows], k[:keep], v[:keep], keep)
+        tol = att_tol(A, f64(q[rows]), f64(k[:keep]), TYPES[dtype], 64, 0.125)
+        assert (np.abs(f64(o[rows]) - want) <= tol).all()
+
+
+def test_attention_long_single_tokens_reload_their_pages():
+    """The same for single tokens: 130 rows over one sequence of 8300 keys, none split."""
+    H = 16
+    m = Made([8300], Hkv=H, d=64, page=8)
+    torch.manual_seed(3)
+    q = torch.randn(130, H, 64, device=DEV).bfloat16()
+    o = m.cache.attention(0, q, i32(np.arange(131)), seqs=i32([0] * 130))
+    k, v = device_rows(m, 0, 0), device_rows(m, 1, 0)
+    for i in (0, 64, 129):
+        want, A = attention_on_device(q[i:i + 1], k, v, 8300)
+        assert (np.abs(f64(o[i:i + 1]) - want) <= 3.25 * 2.0 ** -8 * A).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_attention_mixed_batch_and_repeats_bit_for_bit(dtype):
+    """Single tokens beside one long chunk (in the form for few rows), and the same bits
+    every time: the order in which parts end does not matter."""
+    rng = np.random.default_rng(8)
+    lens = [int(x) for x in rng.integers(1, 3000, 20)] + [2500]
+    m = Made(lens, Hkv=2, d=64, dtype=TYPES[dtype])
+    first = check_attention(m, [1] * 20 + [70], 4)
+    for _ in range(10):
+        assert torch.equal(check_again(m, [1] * 20 + [70], 4), first)
+
+
+def check_again(m, n, H, seed=1, tail=3):
+    torch.manual_seed(seed)
+    q = torch.randn(sum(n) + tail, H, m.cache.head_dim, device=DEV).to(m.cache.dtype)
+    o = torch.full_like(q, 7.0)
+    return m.cache.attention(0, q, i32(np.concatenate([[0], np.cumsum(n)])), seqs=i32(range(len(n))), out=o)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_offsets_past_32_bits(dtype):
+    """A pool whose byte and element offsets pass 2^32: append, attention, fork, copies and
+    compaction on its last pages."""
+    page, Hkv, d = 1024, 8, 128
+    per = page * Hkv * d
+    P = (1 << 32) // per + 40 if dtype == "bf16" else (1 << 31) // per + 40
+    k, v = (torch.empty((1, P, Hkv, page, d), dtype=TYPES[dtype], device=DEV) for _ in range(2))
+    table = np.full((3, 4), -1)
+    table[0, :3] = [P - 1, P - 7, P - 20]
+    refs = np.ones(P, int)
+    refs[[5, 9, P - 3]] = 0
+    n, L = 40, 2 * page + 90
+    c = C.PagedCache.wrap(k, v, i32(table), i32([L, 0, 0]), i32(refs))
+    torch.manual_seed(6)
+    new = torch.randn(L, 2, Hkv, d, device=DEV).to(TYPES[dtype])
+    c.append(0, new[:, 0], new[:, 1], i32([0, L]), seqs=i32([0]))
+    c.check()
+    q = torch.randn(n, Hkv, d, device=DEV).to(TYPES[dtype])
+
+    def right(seq):
+        o = c.attention(0, q, i32([0, n]), seqs=i32([seq]))
+        want, A = attention_on_device(q, new[:, 0], new[:, 1], L)
+        tol = att_tol(A, f64(q), f64(new[:, 0]), TYPES[dtype], d, d ** -0.5)
+        assert (np.abs(f64(o) - want) <= tol).all()
+
+    right(0)
+    c.fork(i32([0]), i32([1]))           # the partial page into page 5
+    c.check()
+    assert c.page_table[1, :3].tolist() == [P - 1, P - 7, 5]
+    right(1)
+    c.free(i32([0]))
+    refs = c.refcount.clone()
+    refs[:P - 30] = 1                    # everything below is in use but pages 9 and 11
+    refs[[9, 11]] = 0
+    c.refcount.copy_(refs)
+    c.copy_pages(i32([P - 7]), i32([P - 20]))
+    assert torch.equal(c.k[0, P - 20], c.k[0, P - 7]) and torch.equal(c.v[0, P - 20], c.v[0, P - 7])
+    c.compact()
+    c.check()
+    live = int((c.refcount > 0).sum())
+    assert int(c.page_table[1, :3].max()) < live and bool((c.refcount[:live] > 0).all())
+    right(1)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_attention_not_causal_and_scaled(dtype):
     m = Made([200, 64, 1], Hkv=2, d=64, dtype=TYPES[dtype])
