@@ -93,9 +93,9 @@ class PagedCache:
         self._piece, self._scale = 16 // k.element_size(), self.head_dim ** -0.5
         # the library's own checks, once: an empty list does nothing else
         self._call(self._lib.blt_cache_reserve, "PagedCache", self._ptr, None, None, 0)
-        # parts of attention calls, of whichever form needs most
+        # parts of attention calls, for the largest call of whichever form needs most
         self._ws_bytes = max(self._lib.blt_paged_attention_workspace_bytes(
-            self._ptr, 1, rows, self.n_kv_heads) for rows in (1, 32, 1024))
+            self._ptr, 65536, 65536 * rows, self.n_kv_heads) for rows in (1, 32, 128))
         self._ws = self._workspace(max(self._ws_bytes, 16))
 
     def _call(self, fn, what, *args):

@@ -1195,10 +1195,23 @@ Shape shape_of(const blt_paged_cache& c, int64_t B, int64_t total, int H) {
 int64_t row_tiles(const blt_paged_cache& c, int64_t B, int64_t total, int H, int bq) {
   return total * (H / c.n_kv_heads) / bq + B;
 }
-// parts: none where not even a full sequence has more than cmin key tiles
-int64_t slots_of(const blt_paged_cache& c, const Shape& s) {
-  const int64_t cap = (int64_t)c.max_pages * c.page_size;
-  return cap <= (int64_t)s.cmin * s.bkv ? 0 : 4 * (int64_t)s.resident;
+// Most parts a row tile can have: one for every cmin key tiles of a full sequence.
+int64_t most_parts(const blt_paged_cache& c, const Shape& s) {
+  const int64_t tiles = ((int64_t)c.max_pages * c.page_size + s.bkv - 1) / s.bkv;
+  return (tiles + s.cmin - 1) / s.cmin;
+}
+// Bounds for what find_item makes of lengths that only the device knows: blocks, and
+// slots for parts (none where no row tile can have two).
+int64_t blocks_of(const blt_paged_cache& c, const Shape& s, int64_t B, int64_t total, int H) {
+  const int64_t rt = row_tiles(c, B, total, H, s.bq) * c.n_kv_heads;
+  const int64_t fill = (2 * rt > s.resident ? 2 : 1) * (int64_t)s.resident;
+  const int64_t most = most_parts(c, s);
+  return most < 2 ? rt : rt * most < rt + fill ? rt * most : rt + fill;
+}
+int64_t slots_of(const blt_paged_cache& c, const Shape& s, int64_t B, int64_t total, int H) {
+  const int64_t rt = row_tiles(c, B, total, H, s.bq) * c.n_kv_heads;
+  const int64_t most = most_parts(c, s), all = 4 * (int64_t)s.resident;
+  return most < 2 ? 0 : rt * most < all ? rt * most : all;
 }
 
 template <int D>
@@ -1226,7 +1239,7 @@ int run_paged(const KArgs& p, const Shape& sh, unsigned nb, hipStream_t s) {
 int64_t paged_attention_workspace_bytes(const blt_paged_cache& c, int64_t B, int64_t total,
                                         int H) {
   const Shape s = shape_of(c, B, total, H);
-  return slots_of(c, s) * s.bq * (c.head_dim + 2) * 4;
+  return slots_of(c, s, B, total, H) * s.bq * (c.head_dim + 2) * 4;
 }
 
 int launch_paged_attention(const blt_paged_cache& c, const PagedAttnArgs& a, void* ws,
@@ -1247,12 +1260,11 @@ int launch_paged_attention(const blt_paged_cache& c, const PagedAttnArgs& a, voi
   if (p.window > (1 << 30)) p.window = 0;  // longer than any sequence
   p.c = (float)(1.44269504088896340736 * (double)a.scale);
   p.resident = sh.resident; p.cmin = sh.cmin;
-  const int64_t slots = slots_of(c, sh);
+  const int64_t slots = slots_of(c, sh, a.B, a.total, a.H);
   p.sync = c.sync;
   p.part = (float*)ws;
   p.ml = p.part + slots * sh.bq * d;
-  const int64_t rt = row_tiles(c, a.B, a.total, a.H, sh.bq) * c.n_kv_heads;
-  const int64_t nb = (rt + (slots ? 2 * sh.resident : 0) + 7) / 8 * 8;
+  const int64_t nb = (blocks_of(c, sh, a.B, a.total, a.H) + 7) / 8 * 8;
   if (nb > 0x7fffffff) return fail(BLT_ERR_SHAPE, "paged_attention: too many row tiles");
   return d == 64 ? run_paged<64>(p, sh, (unsigned)nb, s)
                  : run_paged<128>(p, sh, (unsigned)nb, s);
