@@ -8,8 +8,8 @@
 // modulo a turn, to 2^-33 for any 32-bit position.  The upper word's quarter turn
 // picks the quadrant, its remainder (|x| <= pi / 4) goes through the Taylor series
 // of sine and cosine in f32 (first terms left out: x^11 / 11! and x^12 / 12!, below
-// 2e-9).  Both kernels move bytes; one thread computes the angles of V pairs
-// of a token once and applies them to several heads.
+// 2e-9).  Both kernels move bytes; a block computes the angles of its tokens once, into
+// LDS, and applies them to every head.
 #include <math.h>
 
 #include "paged.hpp"
@@ -17,6 +17,8 @@
 namespace blt {
 
 namespace {
+
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
 
 template <typename T>
 struct Conv;
@@ -94,24 +96,35 @@ __device__ inline Unit<V> unit_of(int u, const blt_rotary& r) {
   return t;
 }
 
+// The (cosine, sine) pairs of a token, times the magnitude, into `out`: its `step` threads
+// take them in turn.
+__device__ inline void token_angles(const blt_rotary& r, int pos, int first, int step,
+                                    bool backward, f32x2_t* out) {
+  for (int i = first; i < r.rotary_dim / 2; i += step) {
+    float c, s;
+    angle_of(pos, r.freq[i], c, s);
+    out[i] = f32x2_t{c * r.magnitude, s * (backward ? -r.magnitude : r.magnitude)};
+  }
+}
+
 // one pair, with its roundings written out: every variant gives the same bits
 __device__ inline void turn(float x, float y, float c, float s, float& a, float& b) {
   a = fmaf(x, c, -(y * s));
   b = fmaf(x, s, y * c);
 }
 template <typename T, int V>
-__device__ inline void rotate(Piece<T, V>& a, Piece<T, V>& b, const float* c, const float* s,
+__device__ inline void rotate(Piece<T, V>& a, Piece<T, V>& b, const f32x2_t* cs,
                               bool interleaved) {
   float p, q;
   if (!interleaved) {
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      turn(Conv<T>::in(a.e[e]), Conv<T>::in(b.e[e]), c[e], s[e], p, q);
+      turn(Conv<T>::in(a.e[e]), Conv<T>::in(b.e[e]), cs[e].x, cs[e].y, p, q);
       a.e[e] = Conv<T>::out(p);
       b.e[e] = Conv<T>::out(q);
     }
   } else if constexpr (V == 1) {
-    turn(Conv<T>::in(a.e[0]), Conv<T>::in(b.e[0]), c[0], s[0], p, q);
+    turn(Conv<T>::in(a.e[0]), Conv<T>::in(b.e[0]), cs[0].x, cs[0].y, p, q);
     a.e[0] = Conv<T>::out(p);
     b.e[0] = Conv<T>::out(q);
   } else {
@@ -119,14 +132,16 @@ __device__ inline void rotate(Piece<T, V>& a, Piece<T, V>& b, const float* c, co
     for (int e = 0; e < V; ++e) {
       Piece<T, V>& w = e < V / 2 ? a : b;
       const int i = 2 * (e % (V / 2));
-      turn(Conv<T>::in(w.e[i]), Conv<T>::in(w.e[i + 1]), c[e], s[e], p, q);
+      turn(Conv<T>::in(w.e[i]), Conv<T>::in(w.e[i + 1]), cs[e].x, cs[e].y, p, q);
       w.e[i] = Conv<T>::out(p);
       w.e[i + 1] = Conv<T>::out(q);
     }
   }
 }
 
-constexpr int HB = 4;  // heads whose pieces a thread has in flight
+// heads whose pieces a thread of rotary_kernel has in flight
+template <typename T>
+constexpr int kBatch = sizeof(T) == 2 ? 4 : 6;
 
 // How a block's threads are dealt: `units` of a head side by side, `hg` heads (each
 // thread takes every hg-th), then `tb` tokens.
@@ -134,17 +149,18 @@ struct Deal {
   int units, hg, tb;
   int64_t blocks;
 };
-// Four heads a thread (HB, one batch of loads) where the tokens fill the chip by
-// themselves, so that the angles (about 150 cycles a pair) are spread over them; every
-// head its own thread below that.  [16, 24 heads, 8192, 64] bf16 takes 143 us with four,
-// 146 with three, 151 with six and 159 with twelve.  The angles come before the loads:
-// with the loads issued first, behind the positions and frequencies, it takes 155, and
-// 11,100 appended tokens 46 instead of 40.
-inline Deal deal(int d, int v, int heads, int64_t tokens) {
+// Where the tokens fill the chip by themselves a thread of rotary_kernel takes one batch of
+// heads, otherwise (and in append_kernel always) every head has its own thread, as far
+// as a block has room.  [16, 24 heads, 8192, 64] bf16 takes 143 us with batches of four,
+// 144 with six, 150 with eight, 169 with one; 5001 f32 gradients of 40 heads of 128, half
+// rotated, 40 us with four and 38 with six.  11,100 tokens of 32 / 8 heads of 128 into the
+// cache take 35 us with one head a thread, 36 with two, 38 with three, 41 with four.
+inline Deal deal(int d, int v, int heads, int64_t tokens, int batch) {
   Deal t;
   t.units = d / (2 * v);
   const int most = t.units >= 256 ? 1 : 256 / t.units;
-  const int64_t want = tokens * t.units >= (int64_t)256 * 1024 ? (heads + HB - 1) / HB : heads;
+  if (tokens * t.units < (int64_t)256 * 1024) batch = 1;
+  const int64_t want = (heads + batch - 1) / batch;
   t.hg = (int)(want < most ? want : most);
   t.tb = 256 / (t.units * t.hg);
   if (t.tb < 1) t.tb = 1;
@@ -158,27 +174,23 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs p, Deal dl) {
   const int tid = threadIdx.x;
   const int u0 = tid % dl.units, rest = tid / dl.units;
   const int h0 = rest % dl.hg, tt = rest / dl.hg;
-  if (tt >= dl.tb) return;
+  __shared__ __attribute__((aligned(16))) f32x2_t angles[256 * V];  // (tb * rotary_dim / 2 of them)
   const int64_t tokens = p.B * p.T;
   const int64_t tok = (int64_t)blockIdx.x * dl.tb + tt;
-  if (tok >= tokens) return;
+  const bool mine = tt < dl.tb && tok < tokens;
   const int64_t b = tok / p.T, t = tok - b * p.T;
-  const int pos = p.pos[b * p.sb_pos + t];
-  const int heads = p.q.heads + p.k.heads;
   const Unit<V> un = unit_of<V>(u0, p.r);
-  float c[V], s[V];
-  if (un.rot) {
+  const f32x2_t* cs = angles + tt * (p.r.rotary_dim / 2) + un.pair;
+  if (mine)
+    token_angles(p.r, p.pos[b * p.sb_pos + t], h0 * dl.units + u0, dl.units * dl.hg, p.backward,
+                 angles + tt * (p.r.rotary_dim / 2));
+  __syncthreads();
+  if (!mine) return;
+  const int heads = p.q.heads + p.k.heads;
+  for (int hb = h0; hb < heads; hb += kBatch<T> * dl.hg) {
+    Piece<T, V> a[kBatch<T>], w[kBatch<T>];
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      angle_of(pos, p.r.freq[un.pair + e], c[e], s[e]);
-      c[e] *= p.r.magnitude;
-      s[e] *= p.backward ? -p.r.magnitude : p.r.magnitude;
-    }
-  }
-  for (int hb = h0; hb < heads; hb += HB * dl.hg) {
-    Piece<T, V> a[HB], w[HB];
-#pragma unroll
-    for (int i = 0; i < HB; ++i) {
+    for (int i = 0; i < kBatch<T>; ++i) {
       const int h = hb + i * dl.hg;
       if (h < heads) {
         const bool iq = h < p.q.heads;
@@ -189,13 +201,13 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs p, Deal dl) {
       }
     }
 #pragma unroll
-    for (int i = 0; i < HB; ++i) {
+    for (int i = 0; i < kBatch<T>; ++i) {
       const int h = hb + i * dl.hg;
       if (h < heads) {
         const bool iq = h < p.q.heads;
         T* y = iq ? (T*)p.q.y + b * p.q.sb_y + t * p.q.st_y + h * p.q.sh_y
                   : (T*)p.k.y + b * p.k.sb_y + t * p.k.st_y + (h - p.q.heads) * p.k.sh_y;
-        if (un.rot) rotate<T, V>(a[i], w[i], c, s, p.r.interleaved);
+        if (un.rot) rotate<T, V>(a[i], w[i], cs, p.r.interleaved);
         store_piece<T, V>(y + un.a, a[i]);
         store_piece<T, V>(y + un.b, w[i]);
       }
@@ -224,8 +236,9 @@ __global__ __launch_bounds__(256) void append_kernel(AppendKernelArgs p, Deal dl
   // The token's row b: the number of starts[1 ..] at or below it; its first token and
   // length.  Up to 64 rows a wave holds them all, one round of loads ahead of the page's;
   // beyond that every wave counts for the block's first token and goes on from there.
-  int64_t s0, n;
-  int seq, len;
+  int64_t s0 = 0, n = 0;
+  int seq = -1, len = 0;
+  bool found = false;
   if (a.B <= 64) {
     const int i = lane < a.B ? lane : (int)a.B - 1;
     const int lo = a.starts[i], hi = a.starts[i + 1];
@@ -239,7 +252,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendKernelArgs p, Deal dl
     n = __shfl(hi, b & 63) - s0;
     seq = __shfl(sq, b & 63);
     len = __shfl(ln, b & 63);
-    if (!mine || b >= a.B) return;  // behind the last row
+    found = mine && b < a.B;  // (else behind the last row)
   } else {
     int b = 0;
     for (int64_t i = 0; i < a.B; i += 64) {
@@ -248,33 +261,32 @@ __global__ __launch_bounds__(256) void append_kernel(AppendKernelArgs p, Deal dl
       b += __popcll(m);
       if (m != ~0ull) break;
     }
-    if (!mine) return;
-    while (b < a.B && a.starts[b + 1] <= tok) ++b;
-    if (b >= a.B) return;
-    s0 = a.starts[b];
-    n = a.starts[b + 1] - s0;
-    seq = a.seqs ? a.seqs[b] : b;
-    len = c.lens[seq >= 0 && seq < c.max_seqs ? seq : 0];
+    while (mine && b < a.B && a.starts[b + 1] <= tok) ++b;
+    found = mine && b < a.B;
+    if (found) {
+      s0 = a.starts[b];
+      n = a.starts[b + 1] - s0;
+      seq = a.seqs ? a.seqs[b] : b;
+      len = c.lens[seq >= 0 && seq < c.max_seqs ? seq : 0];
+    }
   }
-  if (tok < s0) return;
+  found = found && tok >= s0;
   const bool known = seq >= 0 && seq < c.max_seqs;
   const int64_t pos = (known ? len : 0) - n + (tok - s0);
   // where k and v go: no page where an index is out of range or a failure is pending
   // (looked at behind the angles, which need not wait for it)
-  const bool inside = known && pos >= 0 && (pos >> p.lps) < c.max_pages;
+  const bool inside = found && known && pos >= 0 && (pos >> p.lps) < c.max_pages;
   const int page = inside ? c.page_table[(int64_t)seq * c.max_pages + (pos >> p.lps)] : -1;
   const int status = *c.status;
 
   const Unit<V> un = unit_of<V>(u0, a.r);
-  float cs[V], sn[V];
-  if (un.rot) {
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      angle_of((int)pos, a.r.freq[un.pair + e], cs[e], sn[e]);
-      cs[e] *= a.r.magnitude;
-      sn[e] *= a.r.magnitude;
-    }
-  }
+  __shared__ __attribute__((aligned(16))) f32x2_t angles[256 * V];
+  const f32x2_t* cs = angles + tt * (a.r.rotary_dim / 2) + un.pair;
+  if (found)
+    token_angles(a.r, (int)pos, h0 * dl.units + u0, dl.units * dl.hg, false,
+                 angles + tt * (a.r.rotary_dim / 2));
+  __syncthreads();
+  if (!found) return;
   const bool bad = page < 0 || page >= c.num_pages;
   if (bad && u0 == 0 && h0 == 0) atomicOr(c.status, BLT_CACHE_NO_PAGE);
   const int Hk = c.n_kv_heads, heads = a.Hq + 2 * Hk;
@@ -283,37 +295,22 @@ __global__ __launch_bounds__(256) void append_kernel(AppendKernelArgs p, Deal dl
                          ? -1
                          : p.layer0 + (int64_t)page * c.n_kv_heads * sh_page +
                                (pos & (c.page_size - 1)) * c.head_dim;
-  for (int hb = h0; hb < heads; hb += HB * dl.hg) {
-    Piece<T, V> x[HB], y[HB];
-#pragma unroll
-    for (int i = 0; i < HB; ++i) {
-      const int h = hb + i * dl.hg;
-      if (h < heads) {
-        const T* src = h < a.Hq ? (const T*)a.q + tok * a.st_q + h * a.sh_q
-                       : h < a.Hq + Hk
-                           ? (const T*)a.k + tok * a.st_k + (h - a.Hq) * a.sh_k
-                           : (const T*)a.v + tok * a.st_v + (h - a.Hq - Hk) * a.sh_v;
-        x[i] = load_piece<T, V>(src + un.a);
-        y[i] = load_piece<T, V>(src + un.b);
-      }
+  for (int h = h0; h < heads; h += dl.hg) {
+    const T* src = h < a.Hq ? (const T*)a.q + tok * a.st_q + h * a.sh_q
+                   : h < a.Hq + Hk ? (const T*)a.k + tok * a.st_k + (h - a.Hq) * a.sh_k
+                                   : (const T*)a.v + tok * a.st_v + (h - a.Hq - Hk) * a.sh_v;
+    Piece<T, V> x = load_piece<T, V>(src + un.a), y = load_piece<T, V>(src + un.b);
+    T* dst;
+    if (h < a.Hq) {
+      dst = (T*)a.q_out + tok * a.st_qo + h * a.sh_qo;
+    } else {
+      if (at < 0) continue;
+      dst = h < a.Hq + Hk ? (T*)c.k + at + (h - a.Hq) * sh_page
+                          : (T*)c.v + at + (h - a.Hq - Hk) * sh_page;
     }
-#pragma unroll
-    for (int i = 0; i < HB; ++i) {
-      const int h = hb + i * dl.hg;
-      if (h < heads) {
-        T* dst;
-        if (h < a.Hq) {
-          dst = (T*)a.q_out + tok * a.st_qo + h * a.sh_qo;
-        } else {
-          if (at < 0) continue;
-          dst = h < a.Hq + Hk ? (T*)c.k + at + (h - a.Hq) * sh_page
-                              : (T*)c.v + at + (h - a.Hq - Hk) * sh_page;
-        }
-        if (un.rot && h < a.Hq + Hk) rotate<T, V>(x[i], y[i], cs, sn, a.r.interleaved);
-        store_piece<T, V>(dst + un.a, x[i]);
-        store_piece<T, V>(dst + un.b, y[i]);
-      }
-    }
+    if (un.rot && h < a.Hq + Hk) rotate<T, V>(x, y, cs, a.r.interleaved);
+    store_piece<T, V>(dst + un.a, x);
+    store_piece<T, V>(dst + un.b, y);
   }
 }
 
@@ -332,7 +329,8 @@ int launch_rotary(const RotaryArgs& a, int dtype, hipStream_t s) {
     if (x->heads)
       vec = vec && aligned(x->x) && aligned(x->y) && whole(x->sb_x, v) && whole(x->sh_x, v) &&
             whole(x->st_x, v) && whole(x->sb_y, v) && whole(x->sh_y, v) && whole(x->st_y, v);
-  const Deal dl = deal(a.d, vec ? v : 1, heads, tokens);
+  const Deal dl = deal(a.d, vec ? v : 1, heads, tokens,
+                       dtype == BLT_DTYPE_BF16 ? kBatch<uint16_t> : kBatch<float>);
   if (dl.blocks > 0x7fffffff) return fail(BLT_ERR_SHAPE, "fused_rotary: too many tokens");
   const dim3 g((unsigned)dl.blocks), b(256);
   if (dtype == BLT_DTYPE_BF16) {
@@ -355,7 +353,7 @@ int launch_append(const blt_paged_cache& c, const AppendArgs& a, hipStream_t s) 
   if (a.Hq)
     vec = vec && aligned(a.q) && aligned(a.q_out) && whole(a.st_q, v) && whole(a.sh_q, v) &&
           whole(a.st_qo, v) && whole(a.sh_qo, v);
-  const Deal dl = deal(d, vec ? v : 1, a.Hq + 2 * c.n_kv_heads, a.total);
+  const Deal dl = deal(d, vec ? v : 1, a.Hq + 2 * c.n_kv_heads, a.total, 1);
   if (dl.blocks > 0x7fffffff) return fail(BLT_ERR_SHAPE, "cache_append: too many tokens");
   AppendKernelArgs p{a, c, log2_of(c.page_size), 0};
   p.layer0 = (int64_t)a.layer * c.num_pages * c.n_kv_heads * c.page_size * d;
