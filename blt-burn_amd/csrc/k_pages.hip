@@ -179,9 +179,36 @@ __global__ __launch_bounds__(NT) void reserve_kernel(blt_paged_cache c, int lps,
 }
 
 // ---- copies --------------------------------------------------------------------
-// The listed pages' first fill[i] tokens (fill NULL: all), in every layer, k and v: 16
-// bytes a lane, four in flight.  A fixed grid walks (pair, layer, k or v).
-// (256 threads, this one is `tid`)
+// The first `fill` tokens of a page in one layer's k or v, by 256 threads (this one is
+// `tid`): 16 bytes a lane, four in flight.  Callers' grids walk (pair, layer, k or v).
+// Whole pages (compaction, copy_pages) are moved past the caches: 400 MB of them take 167 us
+// so and 175 us through the caches (6.15 TB/s is a large plain copy).  The started pages of a
+// fork or a trim are read by the next step's attention and stay cached.
+template <bool WHOLE>
+__device__ inline void copy_rows(const char* from, char* to, int n_heads, int64_t head_b, int row,
+                                 int tid) {
+  const int all = row * n_heads;
+  auto off = [&](int i) -> int64_t {
+    return WHOLE ? (int64_t)i * 16 : (i / row) * head_b + (int64_t)(i % row) * 16;
+  };
+  constexpr int U = 4;
+  for (int i = tid; i < all; i += U * 256) {
+    u32x4_t x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i + u * 256 < all) {
+        const u32x4_t* p = reinterpret_cast<const u32x4_t*>(from + off(i + u * 256));
+        x[u] = WHOLE ? __builtin_nontemporal_load(p) : *p;
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i + u * 256 < all) {
+        u32x4_t* p = reinterpret_cast<u32x4_t*>(to + off(i + u * 256));
+        if (WHOLE) __builtin_nontemporal_store(x[u], p);
+        else *p = x[u];
+      }
+  }
+}
 __device__ inline void copy_tokens(const blt_paged_cache& c, int64_t src, int64_t dst, int fill,
                                    int layer, int kv, int es, int tid) {
   const int64_t page_b = (int64_t)c.n_kv_heads * c.page_size * c.head_dim * es;
@@ -190,21 +217,8 @@ __device__ inline void copy_tokens(const blt_paged_cache& c, int64_t src, int64_
   const char* from = base + src * page_b;
   char* to = base + dst * page_b;
   const int row = fill * c.head_dim * es / 16;  // 16-byte pieces of a head
-  const int all = row * c.n_kv_heads;
-  const bool whole = fill == c.page_size;
-  auto off = [&](int i) -> int64_t {
-    return whole ? (int64_t)i * 16 : (i / row) * head_b + (int64_t)(i % row) * 16;
-  };
-  constexpr int U = 4;
-  for (int i = tid; i < all; i += U * 256) {
-    u32x4_t x[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (i + u * 256 < all) x[u] = *reinterpret_cast<const u32x4_t*>(from + off(i + u * 256));
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (i + u * 256 < all) *reinterpret_cast<u32x4_t*>(to + off(i + u * 256)) = x[u];
-  }
+  if (fill == c.page_size) copy_rows<true>(from, to, c.n_kv_heads, head_b, row, tid);
+  else copy_rows<false>(from, to, c.n_kv_heads, head_b, row, tid);
 }
 __device__ inline void copy_listed(const blt_paged_cache& c, const Lists& l, int es) {
   const int64_t items = (int64_t)*l.count * c.n_layers * 2;
