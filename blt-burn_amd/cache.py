@@ -196,7 +196,8 @@ class PagedCache:
         tokens starts[b] .. starts[b + 1] - 1 (int32 [rows + 1]) and they become the last
         ones of sequence seqs[b] (None: b; none twice), whose length already counts them
         (reserve).  rotary: a RotaryPlan that rotates k at its positions, and q [total, heads,
-        head_dim] if given, which is returned (into `out`, which may be q)."""
+        head_dim] if given, which is returned (into `out`, which may be q; tokens at
+        starts[-1] and behind are not written).  starts ascends from 0 on."""
         k = self._tokens(k, "k", self.n_kv_heads)
         v = self._tokens(v, "v", self.n_kv_heads)
         p, B, s = self._rows(starts, seqs)
@@ -235,7 +236,9 @@ class PagedCache:
         reads key head h // (heads / kv_heads).  causal: keys up to the token's own
         position, with window > 0 only the last `window` of them; causal=False: every
         key.  scale defaults to head_dim^-0.5.  Returns [total, heads, head_dim] (`out` if
-        given; tokens at starts[-1] and behind are left as they were there)."""
+        given): 0 where a token sees no key; tokens at starts[-1] and behind are not
+        written, nor are those of a row without a sequence, nor any where starts does not
+        ascend within q (both set the status)."""
         q = self._tokens(q, "q")
         p, B, s = self._rows(starts, seqs)
         total, H, d = q.shape
@@ -248,6 +251,8 @@ class PagedCache:
             st, qp = q.stride(), q.data_ptr()
         out = self._output(out, q, total, H)
         so = out.stride()
+        if window > 0x7fffffff:  # longer than any sequence
+            window = 0
         self._call(self._lib.blt_paged_attention, "paged_attention", self._ptr, layer, qp, st[0],
                    st[1], out.data_ptr(), so[0], so[1], H, p, s, B, total, 1 if causal else 0,
                    window, self._scale if scale is None else scale, self._ws.data_ptr(),

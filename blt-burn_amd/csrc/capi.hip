@@ -517,8 +517,8 @@ int blt_paged_attention(const blt_paged_cache* cache, int32_t layer, const void*
   if (Hq < 1 || Hq % cache->n_kv_heads)
     return fail(BLT_ERR_SHAPE, "paged_attention: heads must be a multiple of the cache's");
   if (window < 0) return fail(BLT_ERR_SHAPE, "paged_attention: window must be >= 0");
-  if (!(scale > 0.f) || !(scale < 1e30f))
-    return fail(BLT_ERR_SHAPE, "paged_attention: scale must be positive and finite");
+  if (!(scale >= 1e-30f) || !(scale <= 1e30f))
+    return fail(BLT_ERR_SHAPE, "paged_attention: scale must be within 1e-30 .. 1e30");
   if (!seqs && B > cache->max_seqs)
     return fail(BLT_ERR_SHAPE, "paged_attention: more rows than sequences");
   if (B == 0 || total == 0) return BLT_OK;

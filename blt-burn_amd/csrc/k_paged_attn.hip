@@ -34,6 +34,7 @@ struct KArgs {
   float c;        // log2(e) * scale
   int resident, cmin;  // blocks the chip holds; key tiles of the smallest part
   int* sync;      // a counter for every row tile with parts; all zero between calls
+  int32_t* status;
   float* part;    // [slots][rows of a tile][D], unnormalised outputs
   float* ml;      // [slots][rows of a tile][2], their max (before the scale) and sum
 };
@@ -43,12 +44,17 @@ struct KArgs {
 struct Seq {
   int s0, n, len, slot;  // first token in q, tokens, keys, sequence
 };
-__device__ inline Seq seq_at(const KArgs& p, int b) {
+// lost: a row without a sequence; crossed: starts that do not ascend within q (what bounds
+// the grid and the workspace rests on that)
+__device__ inline Seq seq_at(const KArgs& p, int b, bool& lost, bool& crossed) {
   Seq q{0, 0, 0, 0};
   if (b < p.B) {
     const int a = p.starts[b], e = p.starts[b + 1];
     const int slot = p.seqs ? p.seqs[b] : b;
-    if (a >= 0 && e > a && e <= p.total && slot >= 0 && slot < p.max_seqs) {
+    const bool known = slot >= 0 && slot < p.max_seqs;
+    crossed = crossed || a < 0 || e < a || e > p.total;
+    lost = lost || !known;
+    if (a >= 0 && e > a && e <= p.total && known) {
       int len = p.lens[slot];
       len = len < 0 ? 0 : len > p.cap ? p.cap : len;
       q = Seq{a, e - a, len, slot};
@@ -87,11 +93,16 @@ __device__ bool find_item(const KArgs& p, unsigned bid, Item& it) {
   Seq q;
   int nrt, kt;
   float work = 0.f, tiles = 0.f;
+  bool lost = false, crossed = false;
   for (int b0 = 0; b0 < p.B; b0 += 64) {
-    q = seq_at(p, b0 + lane);
+    q = seq_at(p, b0 + lane, lost, crossed);
     tiles_of<BQ, BKV>(p, q, nrt, kt);
     work += (float)nrt * (float)kt;
     tiles += (float)nrt;
+  }
+  if (__any(lost || crossed)) {
+    if (bid == 0 && threadIdx.x == 0) atomicOr(p.status, BLT_CACHE_BAD_INDEX);
+    if (__any(crossed)) return false;
   }
   // (one value for the wave, in scalar registers: what follows from it stays there too)
   work = uniform(wave_sum(work)) * (float)p.Hkv;
@@ -122,7 +133,7 @@ __device__ bool find_item(const KArgs& p, unsigned bid, Item& it) {
     items = parts = joins = 0;
     for (int b0 = 0; b0 < p.B; b0 += 64) {
       if (p.B > 64) {
-        q = seq_at(p, b0 + lane);
+        q = seq_at(p, b0 + lane, lost, crossed);
         tiles_of<BQ, BKV>(p, q, nrt, kt);
       }
       parts_of();
@@ -147,7 +158,7 @@ __device__ bool find_item(const KArgs& p, unsigned bid, Item& it) {
   int base = 0, pbase = it.kvh * parts, jbase = it.kvh * joins;
   for (int b0 = 0; b0 < p.B; b0 += 64) {
     if (p.B > 64) {
-      q = seq_at(p, b0 + lane);
+      q = seq_at(p, b0 + lane, lost, crossed);
       tiles_of<BQ, BKV>(p, q, nrt, kt);
     }
     parts_of();
@@ -1261,7 +1272,7 @@ int launch_paged_attention(const blt_paged_cache& c, const PagedAttnArgs& a, voi
   p.c = (float)(1.44269504088896340736 * (double)a.scale);
   p.resident = sh.resident; p.cmin = sh.cmin;
   const int64_t slots = slots_of(c, sh, a.B, a.total, a.H);
-  p.sync = c.sync;
+  p.sync = c.sync; p.status = c.status;
   p.part = (float*)ws;
   p.ml = p.part + slots * sh.bq * d;
   const int64_t nb = (blocks_of(c, sh, a.B, a.total, a.H) + 7) / 8 * 8;

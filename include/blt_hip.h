@@ -261,7 +261,7 @@ int blt_cache_copy_pages(const blt_paged_cache* cache, const int32_t* src, const
  * seqs[b] (NULL: b; no sequence twice), whose length already counts them
  * (blt_cache_reserve).  rotary (may be NULL): k is rotated at its position, and q
  * [total, Hq, head_dim] into q_out (both may be NULL with Hq = 0; q_out may be q).
- * Tokens at starts[B] and behind are left alone. */
+ * starts ascends; tokens at starts[B] and behind are left alone. */
 int blt_cache_append(const blt_paged_cache* cache, int32_t layer, const void* k, int64_t st_k,
                      int64_t sh_k, const void* v, int64_t st_v, int64_t sh_v, const void* q,
                      int64_t st_q, int64_t sh_q, void* q_out, int64_t st_qo, int64_t sh_qo,
@@ -274,10 +274,12 @@ int blt_cache_append(const blt_paged_cache* cache, int32_t layer, const void* k,
  * key head h / (Hq / n_kv_heads).
  *   causal: 1 = keys up to the token's own position; 0 = every key of the sequence
  *   window: W > 0 (with causal) = only the last W of them
- *   scale: of the scores, > 0
+ *   scale: of the scores, 1e-30 .. 1e30
  * Scores and softmax in f32; a token that sees no key gets 0.  Keys and values
  * outside the sequences are not read; o [total, Hq, head_dim] behind starts[B] is left
- * as it was.  Page indices outside the pool are read as its nearest page. */
+ * as it was.  Page indices outside the pool are read as its nearest page.  Rows whose
+ * sequence index is out of range are left as they were, all rows where starts does not
+ * ascend within 0 .. total; both set BLT_CACHE_BAD_INDEX. */
 int64_t blt_paged_attention_workspace_bytes(const blt_paged_cache* cache, int64_t B, int64_t total,
                                             int64_t Hq);
 int blt_paged_attention(const blt_paged_cache* cache, int32_t layer, const void* q, int64_t st_q,

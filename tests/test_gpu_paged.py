@@ -233,6 +233,14 @@ def test_attention_window(dtype, window):
     check_attention(m, [2, 64, 300, 1], 4, window=window)
 
 
+def test_attention_window_past_32_bits_is_none():
+    m = Made([90], Hkv=1, d=64)
+    q = torch.randn(3, 1, 64, device=DEV).bfloat16()
+    want = m.cache.attention(0, q, i32([0, 3]))
+    for window in (1 << 30, (1 << 31) - 1, 1 << 31, (1 << 32) + 5):
+        assert torch.equal(m.cache.attention(0, q, i32([0, 3]), window=window), want)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("d,H,Hkv,page", [(64, 12, 12, 16), (128, 8, 1, 32), (64, 3, 1, 8)])
 def test_attention_long_contexts_in_parts(dtype, d, H, Hkv, page):
@@ -474,10 +482,32 @@ def test_attention_bad_indices_stay_in_bounds():
     assert torch.equal(o[1:2], good[1:2]) and bool((o[2:] == 3.0).all())
     o = c.attention(0, q, starts, seqs=i32([3, 1, 2, 0]))
     assert bool((o[0] == 0).all()) and torch.equal(o[1:2], good[1:2])
-    # starts that run backwards or past the tokens are no sequences
-    o = torch.full_like(q, 3.0)
-    c.attention(0, q, i32([0, 1, 0, 9, -1]), seqs=i32([0, 1, 0, 1]), out=o)
-    assert torch.equal(o[:1], good[:1]) and bool((o[1:] == 3.0).all())
+    with pytest.raises(BltError, match="index out of range"):
+        c.check()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_attention_starts_out_of_order_change_nothing(dtype):
+    """The bounds on the grid and the workspace rest on starts that ascend within q: such a
+    call is reported and writes nothing, and the next one finds the counters as they were."""
+    m = Made([900, 40, 700], Hkv=2, d=64, slots=80, dtype=TYPES[dtype])
+    c = m.cache
+    q = torch.randn(40, 8, 64, device=DEV).to(c.dtype)
+    order = i32([0, 1, 2])
+    starts = i32([0, 10, 20, 40])
+    good = c.attention(0, q, starts, seqs=order)
+    c.check()
+    many = i32([0, 40] * 35 + [0])  # far more tokens than q holds
+    for bad in (i32([0, 10, 5, 40]), i32([0, 10, 41, 41]), i32([-1, 10, 20, 40]), many):
+        o = torch.full_like(q, 3.0)
+        seqs = order if len(bad) == 4 else torch.zeros(len(bad) - 1, device=DEV, dtype=torch.int32)
+        c.attention(0, q, bad, seqs=seqs, out=o)
+        assert bool((o == 3.0).all())
+        with pytest.raises(BltError, match="index out of range"):
+            c.check()
+        assert torch.equal(c.attention(0, q, starts, seqs=order), good)
+        c.check()
+    assert int(c._sync.abs().max()) == 0
 
 
 def test_attention_refusals():
@@ -487,7 +517,8 @@ def test_attention_refusals():
     a = m.cache.attention
     for f in (lambda: a(0, q.float(), s), lambda: a(0, q[..., :32], s), lambda: a(0, q[:, :3], s),
               lambda: a(1, q, s), lambda: a(0, q, s.long()), lambda: a(0, q, s, seqs=i32([0, 1])),
-              lambda: a(0, q, s, window=-1), lambda: a(0, q, s, scale=0.0),
+              lambda: a(0, q, s, window=-1), lambda: a(0, q, s, scale=0.0), lambda: a(0, q, s, scale=1e-31),
+              lambda: a(0, q, s, scale=float("inf")),
               lambda: a(0, q, s, out=q[:2]), lambda: a(0, q, s.cpu()), lambda: a(0, q[0], s)):
         with pytest.raises(BltError):
             f()

@@ -79,7 +79,8 @@ def test_bad_attention_calls_are_refused():
     for kw, rc, word in [(dict(layer=2), -2, "layer"), (dict(layer=-1), -2, "layer"),
                          (dict(H=6), -2, "multiple"), (dict(H=0), -2, "multiple"),
                          (dict(window=-1), -2, "window"), (dict(scale=0.0), -2, "scale"),
-                         (dict(scale=float("nan")), -2, "scale"), (dict(B=5), -2, "rows"),
+                         (dict(scale=float("nan")), -2, "scale"), (dict(scale=1e-31), -2, "scale"),
+                         (dict(scale=1e31), -2, "scale"), (dict(B=5), -2, "rows"),
                          (dict(B=70000), -2, "rows"), (dict(total=1 << 30), -2, "int32"),
                          (dict(starts=None), -1, "starts"), (dict(q=None), -1, "null"),
                          (dict(q=P + 2), -2, "aligned"), (dict(st=252), -2, "aligned")]:
