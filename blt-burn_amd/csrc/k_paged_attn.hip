@@ -23,12 +23,29 @@ namespace {
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 #define LDS_PTR(p) ((__attribute__((address_space(3))) s16x4_t*)(p))
 
+// x / d for 0 <= x < 2^31 by one product: m = floor(2^s / d) + 1 with s = 31 + ceil(log2 d)
+// is at most 2^s / d + 1, so x m / 2^s passes x / d by less than 1 / d.
+struct Divisor {
+  uint32_t m;
+  int s;
+};
+inline Divisor divisor_of(int d) {
+  int l = 0;
+  while (((int64_t)1 << l) < d) ++l;
+  return Divisor{(uint32_t)(((uint64_t)1 << (31 + l)) / (uint64_t)d + 1), 31 + l};
+}
+__device__ inline int over(int x, const Divisor& d) {
+  return (int)(((uint64_t)(uint32_t)x * d.m) >> d.s);
+}
+
 struct KArgs {
   const void *q, *k, *v;  // k, v: the layer's first element
   void* o;
   int64_t st_q, sh_q, st_o, sh_o;
   const int32_t *starts, *seqs, *lens, *table;
   int B, total, Hkv, G;
+  Divisor by_g;
+  int tokens_max;  // tokens that a row tile touches, at most
   int max_seqs, max_pages, num_pages, lps, cap;  // cap: tokens max_pages hold
   int causal, window;                            // window 0: none
   float c;        // log2(e) * scale
@@ -49,27 +66,26 @@ struct Seq {
 __device__ inline Seq seq_at(const KArgs& p, int b, bool& lost, bool& crossed) {
   Seq q{0, 0, 0, 0};
   if (b < p.B) {
-    const int a = p.starts[b], e = p.starts[b + 1];
+    // (loads that wait for no comparison: all of them are on their way at once)
     const int slot = p.seqs ? p.seqs[b] : b;
     const bool known = slot >= 0 && slot < p.max_seqs;
+    int len = p.lens[known ? slot : 0];
+    const int a = p.starts[b], e = p.starts[b + 1];
     crossed = crossed || a < 0 || e < a || e > p.total;
     lost = lost || !known;
-    if (a >= 0 && e > a && e <= p.total && known) {
-      int len = p.lens[slot];
-      len = len < 0 ? 0 : len > p.cap ? p.cap : len;
-      q = Seq{a, e - a, len, slot};
-    }
+    len = len < 0 ? 0 : len > p.cap ? p.cap : len;
+    if (a >= 0 && e > a && e <= p.total && known) q = Seq{a, e - a, len, slot};
   }
   return q;
 }
 // row tiles of a sequence, and the key tiles one of them may have to read
 template <int BQ, int BKV>
 __device__ inline void tiles_of(const KArgs& p, const Seq& q, int& nrt, int& kt) {
-  nrt = (int)(((int64_t)q.n * p.G + BQ - 1) / BQ);
-  kt = (q.len + BKV - 1) / BKV;
+  nrt = (int)(((uint32_t)(q.n * p.G) + BQ - 1) / BQ);
+  kt = (int)(((uint32_t)q.len + BKV - 1) / BKV);
   if (p.window) {
-    const int tokens = q.n < BQ / p.G + 2 ? q.n : BQ / p.G + 2;
-    const int most = (p.window + tokens + BKV - 2) / BKV + 1;
+    const int tokens = q.n < p.tokens_max ? q.n : p.tokens_max;
+    const int most = (int)((uint32_t)(p.window + tokens + BKV - 2) / BKV) + 1;
     kt = kt < most ? kt : most;
   }
   kt = kt < 1 ? 1 : kt;
@@ -121,16 +137,16 @@ __device__ bool find_item(const KArgs& p, unsigned bid, Item& it) {
     // rows, a quarter of them in the form for 128)
     const int64_t r = (int64_t)q.n * p.G;
     const int most = max(C, p.cmin + (int)(r < BQ ? r : BQ) / (BQ >= 128 ? 4 : 16));
-    ns = (kt + most - 1) / most;
+    ns = (int)((uint32_t)(kt + most - 1) / (uint32_t)most);
   };
   // Items, partial slots and counters of one key head.  Key heads are the outermost order of
   // the items, and dispatch places block i on XCD i % 8, of which each takes a contiguous
   // run of items: the row tiles of one (sequence, key head) share an L2, and every XCD gets
   // its share of the long sequences (2 chunks of 2048 over 16384 and 11854 keys, 8 key
   // heads: 790 us, 940 with the sequences outermost).
-  int items, parts, joins;
+  int items, inc;  // of all sequences; with up to 64 of them, those up to the lane's own
   for (int tries = 0;; ++tries) {
-    items = parts = joins = 0;
+    items = 0;
     for (int b0 = 0; b0 < p.B; b0 += 64) {
       if (p.B > 64) {
         q = seq_at(p, b0 + lane, lost, crossed);
@@ -138,51 +154,67 @@ __device__ bool find_item(const KArgs& p, unsigned bid, Item& it) {
       }
       parts_of();
       items += nrt * ns;
-      parts += ns > 1 ? nrt * ns : 0;
-      joins += ns > 1 ? nrt : 0;
     }
-    items = lane_of(wave_incl_scan(items), 63);
+    inc = wave_incl_scan(items);
+    items = lane_of(inc, 63);
     // a few items above a whole round would take one of their own: fewer, larger parts
     // (8 sequences of 49152 keys, 12 heads: 1056 items 295 us, 960 of them 213)
-    const float over = (float)items * (float)p.Hkv / blocks;
-    if (over <= 1.f || tiles > blocks || tries == 3) break;
-    C = max(C + 1, (int)(over * (float)C));
+    const float excess = (float)items * (float)p.Hkv / blocks;
+    if (excess <= 1.f || tiles > blocks || tries == 3) break;
+    C = max(C + 1, (int)(excess * (float)C));
   }
-  parts = lane_of(wave_incl_scan(parts), 63);
-  joins = lane_of(wave_incl_scan(joins), 63);
-  const int all = items * p.Hkv, per = (all + 7) >> 3;
-  const int id = (int)(bid & 7) * per + (int)(bid >> 3);
-  if ((int)(bid >> 3) >= per || id >= all) return false;
-  it.kvh = id / items;
-  const int rem = id - it.kvh * items;
-  int base = 0, pbase = it.kvh * parts, jbase = it.kvh * joins;
+  // partial slots, and counters above them: at most 4096 and 2048 of a call
+  auto joined = [&]() { return ns > 1 ? nrt * ns + (nrt << 16) : 0; };
+  int join = 0;
   for (int b0 = 0; b0 < p.B; b0 += 64) {
     if (p.B > 64) {
       q = seq_at(p, b0 + lane, lost, crossed);
       tiles_of<BQ, BKV>(p, q, nrt, kt);
+      parts_of();
     }
-    parts_of();
-    const int mine = nrt * ns, split = ns > 1 ? mine : 0, join = ns > 1 ? nrt : 0;
-    const int inc = wave_incl_scan(mine);
-    const int pinc = wave_incl_scan(split), jinc = wave_incl_scan(join);
+    join += joined();
+  }
+  int jinc = wave_incl_scan(join);
+  const int joins = lane_of(jinc, 63);
+  const int all = items * p.Hkv, per = (all + 7) >> 3;
+  const int id = (int)(bid & 7) * per + (int)(bid >> 3);
+  if ((int)(bid >> 3) >= per || id >= all) return false;
+  it.kvh = (int)((uint32_t)id / (uint32_t)items);
+  const int rem = id - it.kvh * items;
+  int base = 0, jbase = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 64) {
+    if (p.B > 64) {
+      q = seq_at(p, b0 + lane, lost, crossed);
+      tiles_of<BQ, BKV>(p, q, nrt, kt);
+      parts_of();
+      join = joined();
+      inc = wave_incl_scan(nrt * ns);
+      jinc = wave_incl_scan(join);
+    }
     const uint64_t above = __ballot(base + inc > rem);
     if (above) {
       const int l = __ffsll((unsigned long long)above) - 1;
       it.q = Seq{lane_of(q.s0, l), lane_of(q.n, l), lane_of(q.len, l), lane_of(q.slot, l)};
       it.nrt = lane_of(nrt, l);
       it.ns = lane_of(ns, l);
-      it.pslot = pbase + lane_of(pinc - split, l);
-      it.join = jbase + lane_of(jinc - join, l);
-      const int at = rem - (base + lane_of(inc - mine, l));
-      it.split = at / it.nrt;
+      const int before = jbase + lane_of(jinc - join, l);
+      it.pslot = it.kvh * (joins & 0xffff) + (before & 0xffff);
+      it.join = it.kvh * (joins >> 16) + (before >> 16);
+      const int at = rem - (base + lane_of(inc - nrt * ns, l));
+      it.split = (int)((uint32_t)at / (uint32_t)it.nrt);
       it.rt = it.nrt - 1 - (at - it.split * it.nrt);  // the longest causal rows first
       return true;
     }
     base += lane_of(inc, 63);
-    pbase += lane_of(pinc, 63);
     jbase += lane_of(jinc, 63);
   }
   return false;
+}
+// The key tiles [t0, t1) of an item: its part of the `cnt` ones from t_lo on.
+__device__ inline void part_of(const Item& it, int t_lo, int cnt, int& t0, int& t1) {
+  const int each = (int)((uint32_t)cnt / (uint32_t)it.ns), more = cnt - each * it.ns;
+  t0 = t_lo + it.split * each + min(it.split, more);
+  t1 = t0 + each + (it.split < more ? 1 : 0);
 }
 __device__ inline int64_t slot_of(const Item& it, int split) {
   return it.pslot + (int64_t)split * it.nrt + it.rt;
@@ -194,10 +226,10 @@ __device__ inline void key_range(const KArgs& p, const Seq& q, int r0, int r1, i
   hi = q.len - 1;
   lo = 0;
   if (p.causal) {
-    const int last = first + r1 / p.G;
+    const int last = first + over(r1, p.by_g);
     hi = last < hi ? last : hi;
     if (p.window) {
-      const int l = first + r0 / p.G - p.window + 1;
+      const int l = first + over(r0, p.by_g) - p.window + 1;
       lo = l > 0 ? l : 0;
     }
   }
@@ -318,7 +350,7 @@ __device__ void join_parts(const KArgs& p, const Item& it, int nr) {
         acc += w * o[u];
       }
     }
-    const int row = it.rt * BQ + r, t = row / p.G, g = row - t * p.G;
+    const int row = it.rt * BQ + r, t = over(row, p.by_g), g = row - t * p.G;
     const int64_t at =
         (int64_t)(it.q.s0 + t) * p.st_o + (int64_t)(it.kvh * p.G + g) * p.sh_o + dd;
     const f32x4_t x = lt == 0.f ? f32x4_t{0.f, 0.f, 0.f, 0.f} : acc / lt;
@@ -366,21 +398,21 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(KArgs p) {
   const int r0 = it.rt * BQ, r1 = min(r0 + BQ, rows) - 1;
   key_range(p, sq, r0, r1, lo, hi);
   const int t_lo = lo / BKV, cnt = hi < 0 ? 0 : hi / BKV - t_lo + 1;
-  const int t0 = t_lo + (int)((int64_t)cnt * it.split / it.ns);
-  const int t1 = t_lo + (int)((int64_t)cnt * (it.split + 1) / it.ns);
+  int t0, t1;
+  part_of(it, t_lo, cnt, t0, t1);
   // the wave's
   const int rw = r0 + wid * QPW;
   const bool wave_active = rw < rows;
   int wlo = 0, whi = -1;
   const int rwl = min(rw + QPW, rows) - 1;
   if (wave_active) key_range(p, sq, rw, rwl, wlo, whi);
-  const int pos_first = first + rw / p.G;  // lowest position in the wave
-  const int lo_last = p.window ? first + rwl / p.G - p.window + 1 : 0;  // highest lower bound
+  const int pos_first = first + over(rw, p.by_g);  // lowest position in the wave
+  const int lo_last = p.window ? first + over(rwl, p.by_g) - p.window + 1 : 0;  // highest lower bound
 
   // Q fragments (B operand): row rw + lrow, d = 16 ks + 8 lhalf .. + 8
   bf16x8_t qf[KS];
   const int row = rw + lrow;
-  const int tok = min(row, rows - 1) / p.G, head = it.kvh * p.G + min(row, rows - 1) - tok * p.G;
+  const int tok = over(min(row, rows - 1), p.by_g), head = it.kvh * p.G + min(row, rows - 1) - tok * p.G;
   {
     const uint16_t* qrow =
         (const uint16_t*)p.q + (int64_t)(sq.s0 + tok) * p.st_q + (int64_t)head * p.sh_q;
@@ -670,15 +702,15 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(KArgs p) {
   key_range(p, sq, r0, r1, lo, hi);
   // the item's key tiles [t0, t1), of 32 keys here
   const int t_lo = lo / KT, cnt = hi < 0 ? 0 : hi / KT - t_lo + 1;
-  const int t0 = t_lo + (int)((int64_t)cnt * it.split / it.ns);
-  const int t1 = t_lo + (int)((int64_t)cnt * (it.split + 1) / it.ns);
+  int t0, t1;
+  part_of(it, t_lo, cnt, t0, t1);
 
   bf16x8_t qf[NR][KS];
   int klo[NR], khi[NR];
 #pragma unroll
   for (int n = 0; n < NR; ++n) {
     const int r = min(r0 + 16 * n + col, rows - 1);
-    const int t = r / p.G, g = r - t * p.G;
+    const int t = over(r, p.by_g), g = r - t * p.G;
     const uint16_t* qrow = (const uint16_t*)p.q + (int64_t)(sq.s0 + t) * p.st_q +
                            (int64_t)(it.kvh * p.G + g) * p.sh_q;
 #pragma unroll
@@ -689,8 +721,8 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(KArgs p) {
     klo[n] = p.window ? first + t - p.window + 1 : 0;
   }
   // every row sees [all_lo, all_hi]
-  const int all_hi = p.causal ? min(first + r0 / p.G, sq.len - 1) : sq.len - 1;
-  const int all_lo = p.window ? first + r1 / p.G - p.window + 1 : 0;
+  const int all_hi = p.causal ? min(first + over(r0, p.by_g), sq.len - 1) : sq.len - 1;
+  const int all_lo = p.window ? first + over(r1, p.by_g) - p.window + 1 : 0;
 
   // DMA of one tile: eight keys (one page) at a time, chunks swizzled for the operand reads
   const unsigned ring = (unsigned)(uintptr_t)lds + (unsigned)(w * NST * 2 * TILE * 2);
@@ -947,7 +979,7 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(KArgs p) {
       put4(p.part + (at + r) * D + dd, acc);
       if (dd == 0) put2(p.ml + (at + r) * 2, mx, lt);
     } else {
-      const int t = (r0 + r) / p.G, g = (r0 + r) - t * p.G;
+      const int t = over(r0 + r, p.by_g), g = (r0 + r) - t * p.G;
       uint16_t* dst = (uint16_t*)p.o + (int64_t)(sq.s0 + t) * p.st_o +
                       (int64_t)(it.kvh * p.G + g) * p.sh_o + dd;
       const float inv = lt == 0.f ? 0.f : 1.f / lt;
@@ -981,11 +1013,11 @@ __global__ __launch_bounds__(256) void paged_attn_f32_kernel(KArgs p) {
   int lo, hi;
   key_range(p, sq, r0, r1, lo, hi);
   const int t_lo = lo / BKV, cnt = hi < 0 ? 0 : hi / BKV - t_lo + 1;
-  const int t0 = t_lo + (int)((int64_t)cnt * it.split / it.ns);
-  const int t1 = t_lo + (int)((int64_t)cnt * (it.split + 1) / it.ns);
+  int t0, t1;
+  part_of(it, t_lo, cnt, t0, t1);
 
   const int r = min(r0 + l31, rows - 1);
-  const int tok = r / p.G, g = r - tok * p.G;
+  const int tok = over(r, p.by_g), g = r - tok * p.G;
   const int khi = p.causal ? min(first + tok, sq.len - 1) : sq.len - 1;
   const int klo = p.window ? first + tok - p.window + 1 : 0;
   f32x4_t qf[NC], kf[NC];
@@ -1020,8 +1052,8 @@ __global__ __launch_bounds__(256) void paged_attn_f32_kernel(KArgs p) {
   float m = -INFINITY, l = 0.f;
   const float c = p.c;
   // every row sees [all_lo, all_hi]
-  const int all_hi = p.causal ? min(first + r0 / p.G, sq.len - 1) : sq.len - 1;
-  const int all_lo = p.window ? first + r1 / p.G - p.window + 1 : 0;
+  const int all_hi = p.causal ? min(first + over(r0, p.by_g), sq.len - 1) : sq.len - 1;
+  const int all_lo = p.window ? first + over(r1, p.by_g) - p.window + 1 : 0;
   // one tile; the next one's K (of `next`) is loaded under the second product
   auto tile = [&](int t, int next) {
     const int k0 = t * BKV;
@@ -1184,7 +1216,7 @@ __global__ __launch_bounds__(256) void paged_attn_f32_kernel(KArgs p) {
       put4(p.part + (at + rr) * D + cc, sum);
       if (cc == 0) put2(p.ml + (at + rr) * 2, sm[0][rr], tot);
     } else {
-      const int t = (r0 + rr) / p.G, gg = (r0 + rr) - t * p.G;
+      const int t = over(r0 + rr, p.by_g), gg = (r0 + rr) - t * p.G;
       *reinterpret_cast<f32x4_t*>((float*)p.o + (int64_t)(sq.s0 + t) * p.st_o +
                                   (int64_t)(it.kvh * p.G + gg) * p.sh_o + cc) =
           tot == 0.f ? f32x4_t{0.f, 0.f, 0.f, 0.f} : sum / tot;
@@ -1275,6 +1307,8 @@ int launch_paged_attention(const blt_paged_cache& c, const PagedAttnArgs& a, voi
   p.st_q = a.st_q; p.sh_q = a.sh_q; p.st_o = a.st_o; p.sh_o = a.sh_o;
   p.starts = a.starts; p.seqs = a.seqs; p.lens = c.lens; p.table = c.page_table;
   p.B = (int)a.B; p.total = (int)a.total; p.Hkv = c.n_kv_heads; p.G = a.H / c.n_kv_heads;
+  p.by_g = divisor_of(p.G);
+  p.tokens_max = sh.bq / p.G + 2;
   p.max_seqs = c.max_seqs; p.max_pages = c.max_pages; p.num_pages = c.num_pages;
   p.lps = log2_of(c.page_size); p.cap = c.max_pages * c.page_size;
   p.causal = a.causal; p.window = a.causal ? a.window : 0;
