@@ -26,7 +26,7 @@ def call_on(device, index, fn, what, *args):
     """fn(*args, stream) on `device` (whose index is `index`) and its current stream:
     the library launches on the current device, which may be another one."""
     if _current_device() == index:
-        rc = fn(*args, stream_ptr(index))
+        rc = fn(*args, _raw_stream(index) if _raw_stream is not None else stream_ptr(index))
     else:
         with torch.cuda.device(device):
             rc = fn(*args, stream_ptr(index))

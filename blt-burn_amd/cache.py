@@ -17,6 +17,7 @@ stream-ordered, attention among them: they share its workspace and counters (two
 graphs that use one cache must not be replayed at once).
 """
 import ctypes
+import functools
 
 import torch
 
@@ -90,6 +91,7 @@ class PagedCache:
             k.shape[3], k.shape[4], *page_table.shape)
         self._ptr = ctypes.addressof(self._desc)
         self._lib = _lib.lib()
+        self._call = functools.partial(call_on, self.device, self._index)
         self._piece, self._scale = 16 // k.element_size(), self.head_dim ** -0.5
         # the library's own checks, once: an empty list does nothing else
         self._call(self._lib.blt_cache_reserve, "PagedCache", self._ptr, None, None, 0)
@@ -97,9 +99,6 @@ class PagedCache:
         self._ws_bytes = max(self._lib.blt_paged_attention_workspace_bytes(
             self._ptr, 65536, 65536 * rows, self.n_kv_heads) for rows in (1, 32, 128))
         self._ws = self._workspace(max(self._ws_bytes, 16))
-
-    def _call(self, fn, what, *args):
-        call_on(self.device, self._index, fn, what, *args)
 
     # ---- status ---------------------------------------------------------------
     def check(self):

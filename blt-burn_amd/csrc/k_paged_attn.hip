@@ -134,9 +134,11 @@ __device__ bool find_item(const KArgs& p, unsigned bid, Item& it) {
   int ns;
   auto parts_of = [&]() {
     // (a part costs as much as a few key tiles to write and join: in proportion to its
-    // rows, a quarter of them in the form for 128)
-    const int64_t r = (int64_t)q.n * p.G;
-    const int most = max(C, p.cmin + (int)(r < BQ ? r : BQ) / (BQ >= 128 ? 4 : 16));
+    // rows, a quarter of them in the form for 128; and the more there are of one row tile,
+    // the longer their joining takes: one token over 8192 keys, 12 heads, 16.0 us in parts of
+    // four tiles and 17.8 in parts of two, over 1000 keys 10.4 and 8.7)
+    const int r = q.n * p.G, long_row = BKV < 64 || kt < 64 ? 0 : max(2, kt >> 6);
+    const int most = max(C, p.cmin + long_row + (r < BQ ? r : BQ) / (BQ >= 128 ? 4 : 16));
     ns = (int)((uint32_t)(kt + most - 1) / (uint32_t)most);
   };
   // Items, partial slots and counters of one key head.  Key heads are the outermost order of
@@ -300,9 +302,23 @@ __device__ inline f32x4_t get4(const float* at) {
   v.z = x; v.w = y;
   return v;
 }
-// A thread takes four columns of a row at a time.  Called by all threads of a block of NT.
+// A thread takes four columns of a row at a time; where that leaves threads over and there
+// are many parts, groups of threads take runs of them and meet in `room` (6 NT words of LDS
+// that nobody uses any more).  Called by all threads of a block of NT.
+struct Joined {
+  float m, l;
+  f32x4_t o;
+};
+__device__ inline void join(Joined& a, const Joined& b, float c) {
+  const float mx = fmaxf(a.m, b.m), off = mx == -INFINITY ? 0.f : mx;
+  const float wa = __builtin_amdgcn_exp2f((a.m - off) * c);
+  const float wb = __builtin_amdgcn_exp2f((b.m - off) * c);
+  a.m = mx;
+  a.l = fmaf(a.l, wa, wb * b.l);
+  a.o = a.o * wa + wb * b.o;
+}
 template <int D, int BQ, int NT, typename T>
-__device__ void join_parts(const KArgs& p, const Item& it, int nr) {
+__device__ void join_parts(const KArgs& p, const Item& it, int nr, float* room) {
   __shared__ int last;
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this thread's part, before the count
   __syncthreads();
@@ -314,52 +330,81 @@ __device__ void join_parts(const KArgs& p, const Item& it, int nr) {
   }
   __syncthreads();
   if (!last) return;
+  // U parts at a time, everything of them in flight at once (a read that passes the L2 takes
+  // about 1 us), with a running max; past the last part: the last one again, without weight
   const int64_t step = (int64_t)it.nrt * BQ;
-  for (int i = threadIdx.x; i < nr * (D / 4); i += NT) {
-    const int r = i / (D / 4), dd = (i % (D / 4)) * 4;
-    const int64_t s0 = slot_of(it, 0) * BQ + r;
-    // eight parts at a time, everything of them in flight at once (a read that passes the
-    // L2 takes about 2 us), with a running max
-    constexpr int U = 8;
-    float mx = -INFINITY, lt = 0.f;
-    f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-    for (int x0 = 0; x0 < it.ns; x0 += U) {
+  auto run = [&](int i, int x0, int x1, auto at_once) {
+    constexpr int U = decltype(at_once)::value;
+    const int64_t s0 = slot_of(it, 0) * BQ + i / (D / 4);
+    const int dd = (i % (D / 4)) * 4;
+    Joined a{-INFINITY, 0.f, f32x4_t{0.f, 0.f, 0.f, 0.f}};
+    for (int x = x0; x < x1; x += U) {
       float m[U], l[U];
       f32x4_t o[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int64_t at = s0 + min(x0 + u, it.ns - 1) * step;
+        const int64_t at = s0 + min(x + u, x1 - 1) * step;
         get2(p.ml + at * 2, m[u], l[u]);
         o[u] = get4(p.part + at * D + dd);
       }
 #pragma unroll
-      for (int u = 0; u < U; ++u)  // (past the last part: the last one again, without weight)
-        if (x0 + u >= it.ns) m[u] = -INFINITY;
-      float mn = mx;
+      for (int u = 0; u < U; ++u)
+        if (x + u >= x1) m[u] = -INFINITY;
+      float mn = a.m;
 #pragma unroll
       for (int u = 0; u < U; ++u) mn = fmaxf(mn, m[u]);
       const float mu = mn == -INFINITY ? 0.f : mn;
-      const float alpha = __builtin_amdgcn_exp2f((mx - mu) * p.c);
-      mx = mn;
-      lt *= alpha;
-      acc *= alpha;
+      const float alpha = __builtin_amdgcn_exp2f((a.m - mu) * p.c);
+      a.m = mn;
+      a.l *= alpha;
+      a.o *= alpha;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const float w = __builtin_amdgcn_exp2f((m[u] - mu) * p.c);
-        lt = fmaf(w, l[u], lt);
-        acc += w * o[u];
+        a.l = fmaf(w, l[u], a.l);
+        a.o += w * o[u];
       }
     }
+    return a;
+  };
+  auto store = [&](int i, const Joined& a) {
+    const int r = i / (D / 4), dd = (i % (D / 4)) * 4;
     const int row = it.rt * BQ + r, t = over(row, p.by_g), g = row - t * p.G;
     const int64_t at =
         (int64_t)(it.q.s0 + t) * p.st_o + (int64_t)(it.kvh * p.G + g) * p.sh_o + dd;
-    const f32x4_t x = lt == 0.f ? f32x4_t{0.f, 0.f, 0.f, 0.f} : acc / lt;
+    const f32x4_t x = a.l == 0.f ? f32x4_t{0.f, 0.f, 0.f, 0.f} : a.o / a.l;
     if constexpr (sizeof(T) == 2)
       *reinterpret_cast<u32x2_t*>((uint16_t*)p.o + at) =
           u32x2_t{pack_bf16x2(x.x, x.y), pack_bf16x2(x.z, x.w)};
     else
       *reinterpret_cast<f32x4_t*>((float*)p.o + at) = x;
+  };
+  constexpr std::integral_constant<int, 8> eight{};
+  constexpr std::integral_constant<int, BQ <= 32 && sizeof(T) == 2 ? 16 : 8> more{};
+  const int work = nr * (D / 4);
+  if (it.ns <= 8) {
+    for (int i = threadIdx.x; i < work; i += NT) store(i, run(i, 0, it.ns, eight));
+    return;
   }
+  if (2 * work > NT) {
+    for (int i = threadIdx.x; i < work; i += NT) store(i, run(i, 0, it.ns, more));
+    return;
+  }
+  const int groups = NT / work, per = (it.ns + groups - 1) / groups;
+  const int i = threadIdx.x % work, g = threadIdx.x / work;
+  const int x0 = min(g * per, it.ns);
+  Joined a = run(i, x0, g < groups ? min(x0 + per, it.ns) : x0, eight);
+  *reinterpret_cast<f32x4_t*>(room + threadIdx.x * 4) = a.o;
+  room[4 * NT + threadIdx.x] = a.m;
+  room[5 * NT + threadIdx.x] = a.l;
+  __syncthreads();
+  if (g > 0) return;
+  for (int x = 1; x < groups; ++x) {
+    const int th = i + x * work;
+    join(a, Joined{room[4 * NT + th], room[5 * NT + th], *reinterpret_cast<f32x4_t*>(room + th * 4)},
+         p.c);
+  }
+  store(i, a);
 }
 
 // ---- bf16, tiles of rows ---------------------------------------------------------
@@ -659,7 +704,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(KArgs p) {
         *reinterpret_cast<u32x2_t*>(orow + ds * 32 + 8 * j + 4 * lhalf) = w;
       }
   }
-  if (it.ns > 1) join_parts<D, BQ, 256, uint16_t>(p, it, r1 - r0 + 1);
+  if (it.ns > 1) join_parts<D, BQ, 256, uint16_t>(p, it, r1 - r0 + 1, reinterpret_cast<float*>(lds));
 }
 
 // ---- bf16, few rows ----------------------------------------------------------------
@@ -987,7 +1032,7 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(KArgs p) {
                                                  pack_bf16x2(acc.z * inv, acc.w * inv)};
     }
   }
-  if (it.ns > 1) join_parts<D, BQ, 64 * NW, uint16_t>(p, it, nr);
+  if (it.ns > 1) join_parts<D, BQ, 64 * NW, uint16_t>(p, it, nr, so);
 }
 
 // ---- f32 -------------------------------------------------------------------------
@@ -1222,7 +1267,7 @@ __global__ __launch_bounds__(256) void paged_attn_f32_kernel(KArgs p) {
           tot == 0.f ? f32x4_t{0.f, 0.f, 0.f, 0.f} : sum / tot;
     }
   }
-  if (it.ns > 1) join_parts<D, BQ, 256, float>(p, it, nq);
+  if (it.ns > 1) join_parts<D, BQ, 256, float>(p, it, nq, so);
 }
 
 // ---- launch ------------------------------------------------------------------------
