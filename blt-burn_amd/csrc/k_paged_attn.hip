@@ -10,8 +10,9 @@
 // live on the device (the call can be captured and replayed as they grow), so every wave
 // works out its item itself: the number of key tiles an item may have (C) follows from
 // the total work, then a scan over the sequences finds the item of a block.  The host
-// only bounds the grid: items <= 2 * resident + row tiles, parts in need
-// of joining <= 4 * resident (every one of them has more than half of C).
+// only bounds the grid: items <= row tiles + the blocks that are to be filled (2 * resident,
+// where find_item spills 4 * resident), parts in need of joining <= twice those blocks (every
+// one of them has more than half of C).
 #include <type_traits>
 
 #include "paged.hpp"
@@ -49,7 +50,7 @@ struct KArgs {
   int max_seqs, max_pages, num_pages, lps, cap;  // cap: tokens max_pages hold
   int causal, window;                            // window 0: none
   float c;        // log2(e) * scale
-  int resident, cmin;  // blocks the chip holds; key tiles of the smallest part
+  int resident, cmin, spill;  // see Shape
   int* sync;      // a counter for every row tile with parts; all zero between calls
   int32_t* status;
   float* part;    // [slots][rows of a tile][D], unnormalised outputs
@@ -108,12 +109,13 @@ __device__ bool find_item(const KArgs& p, unsigned bid, Item& it) {
   const int lane = threadIdx.x & 63;
   Seq q;
   int nrt, kt;
-  float work = 0.f, tiles = 0.f;
+  float work = 0.f, tiles = 0.f, longest = 0.f;
   bool lost = false, crossed = false;
   for (int b0 = 0; b0 < p.B; b0 += 64) {
     q = seq_at(p, b0 + lane, lost, crossed);
     tiles_of<BQ, BKV>(p, q, nrt, kt);
     work += (float)nrt * (float)kt;
+    longest = fmaxf(longest, nrt ? (float)kt : 0.f);
     tiles += (float)nrt;
   }
   if (__any(lost || crossed)) {
@@ -128,9 +130,19 @@ __device__ bool find_item(const KArgs& p, unsigned bid, Item& it) {
   // whole number of C make half an item more each, on average: so work / C = blocks -
   // tiles / 2.  (0.1 % above the exact quotient: the bounds on the grid and the slots
   // hold whatever the rounding of the sums.)
-  const float blocks = 2.f * tiles > (float)p.resident ? 2.f * p.resident : (float)p.resident;
+  // Row tiles just above one round would leave the next one nearly empty: four rounds of parts,
+  // where these are not too short (see shape_of).
+  const bool spill = p.spill && tiles > (float)p.resident && tiles <= 1.5f * (float)p.resident &&
+                     work >= 32.f * tiles;
+  const float blocks = (spill ? 4.f : 2.f * tiles > (float)p.resident ? 2.f : 1.f) * p.resident;
   const float fill = fmaxf(blocks - 0.5f * tiles, 0.5f * (float)p.resident);
   int C = max(p.cmin, (int)fminf(ceilf(work * 1.001f / fill), 1e9f));
+  // Row tiles that fill a round between them and are of about one length stay whole: parts of
+  // them would only add a round that is not full (16 chunks of 128 over 8192 keys, 32 / 8
+  // heads of 128: 308 us, 380 in parts; with a window of 3000 keys 113 and 210).
+  longest = uniform(wave_max(longest));
+  if ((BQ >= 128 || tiles <= (float)p.resident) && !spill && longest * (float)p.resident <= 1.25f * work)
+    C = max(C, (int)longest);
   int ns;
   auto parts_of = [&]() {
     // (a part costs as much as a few key tiles to write and join: in proportion to its
@@ -165,7 +177,7 @@ __device__ bool find_item(const KArgs& p, unsigned bid, Item& it) {
     if (excess <= 1.f || tiles > blocks || tries == 3) break;
     C = max(C + 1, (int)(excess * (float)C));
   }
-  // partial slots, and counters above them: at most 4096 and 2048 of a call
+  // partial slots, and counters above them: at most 8192 and 2048 of a call
   auto joined = [&]() { return ns > 1 ? nrt * ns + (nrt << 16) : 0; };
   int join = 0;
   for (int b0 = 0; b0 < p.B; b0 += 64) {
@@ -1274,24 +1286,34 @@ __global__ __launch_bounds__(256) void paged_attn_f32_kernel(KArgs p) {
 enum Form { FORM_TILES, FORM_FEW16, FORM_FEW32, FORM_F32 };
 struct Shape {
   Form form;
-  int bq, bkv, resident, cmin;
+  int bq, bkv;
+  int resident;  // blocks the chip holds at once
+  int cmin;      // key tiles of the smallest part
+  int spill;     // the row tiles may be just above one round
 };
 // resident: blocks the chip holds at once by their registers and LDS (f32 with d = 128: one
 // per CU; with two assumed, 3 chunks of 100 tokens over 1500 keys, 32 / 8 heads, took 85 us
-// instead of 68).  2 * resident <= BLT_CACHE_SYNC_WORDS: a counter for every row tile with
-// parts.  The form goes by the rows a sequence has on average: a tile of 16 rows costs the
+// instead of 68).  A counter for every row tile with parts: at most 2 * resident (two parts
+// or more of each) or, with a spill, 1.5 * resident of them, <= BLT_CACHE_SYNC_WORDS.  The form goes by the rows a sequence has on average: a tile of 16 rows costs the
 // matrix cores half of one of 32, and 128 rows share what they read; every form takes any
 // chunk, in more row tiles.
-Shape shape_of(const blt_paged_cache& c, int64_t B, int64_t total, int H) {
-  if (c.dtype == BLT_DTYPE_F32) return Shape{FORM_F32, 32, 32, c.head_dim == 64 ? 512 : 256, 4};
-  const int64_t rows = total * (H / c.n_kv_heads);  // of all sequences, per key head
-  const int few = c.head_dim == 64 ? 1024 : 512;  // 32 and 64 KB of rings
-  if (rows <= 16 * B) return Shape{FORM_FEW16, 16, 64, few, 2};
-  if (rows <= 32 * B) return Shape{FORM_FEW32, 32, 64, few, 2};
-  return Shape{FORM_TILES, 128, 64, 512, 2};
-}
 int64_t row_tiles(const blt_paged_cache& c, int64_t B, int64_t total, int H, int bq) {
   return total * (H / c.n_kv_heads) / bq + B;
+}
+// spill: 72 single tokens over 8000 keys, 32 / 8 heads of 128, are 576 row tiles for 512
+// blocks: 590 us in two rounds, 432 in four; 96 over 4000 keys, 12 heads, 266 and 224.  From
+// half a round more on it costs (128: 291 and 309), and in the form for 128 rows always
+// (5 chunks of 512 over 8192 keys, 32 / 8 heads: 415 and 455).
+Shape shape_of(const blt_paged_cache& c, int64_t B, int64_t total, int H) {
+  const int64_t rows = total * (H / c.n_kv_heads);  // of all sequences, per key head
+  const int few = c.head_dim == 64 ? 1024 : 512;  // 32 and 64 KB of rings
+  Shape s{FORM_TILES, 128, 64, 512, 2, 0};
+  if (c.dtype == BLT_DTYPE_F32) s = Shape{FORM_F32, 32, 32, few / 2, 4, 0};
+  else if (rows <= 16 * B) s = Shape{FORM_FEW16, 16, 64, few, 2, 0};
+  else if (rows <= 32 * B) s = Shape{FORM_FEW32, 32, 64, few, 2, 0};
+  s.spill = s.form != FORM_TILES && 5 * B * c.n_kv_heads <= 7 * s.resident &&
+            row_tiles(c, B, total, H, s.bq) * c.n_kv_heads > s.resident;
+  return s;
 }
 // Most parts a row tile can have: one for every cmin key tiles of a full sequence.
 int64_t most_parts(const blt_paged_cache& c, const Shape& s) {
@@ -1302,13 +1324,13 @@ int64_t most_parts(const blt_paged_cache& c, const Shape& s) {
 // slots for parts (none where no row tile can have two).
 int64_t blocks_of(const blt_paged_cache& c, const Shape& s, int64_t B, int64_t total, int H) {
   const int64_t rt = row_tiles(c, B, total, H, s.bq) * c.n_kv_heads;
-  const int64_t fill = (2 * rt > s.resident ? 2 : 1) * (int64_t)s.resident;
+  const int64_t fill = (s.spill ? 4 : 2 * rt > s.resident ? 2 : 1) * (int64_t)s.resident;
   const int64_t most = most_parts(c, s);
   return most < 2 ? rt : rt * most < rt + fill ? rt * most : rt + fill;
 }
 int64_t slots_of(const blt_paged_cache& c, const Shape& s, int64_t B, int64_t total, int H) {
   const int64_t rt = row_tiles(c, B, total, H, s.bq) * c.n_kv_heads;
-  const int64_t most = most_parts(c, s), all = 4 * (int64_t)s.resident;
+  const int64_t most = most_parts(c, s), all = (s.form == FORM_TILES ? 4 : 8) * (int64_t)s.resident;
   return most < 2 ? 0 : rt * most < all ? rt * most : all;
 }
 
@@ -1342,7 +1364,7 @@ int64_t paged_attention_workspace_bytes(const blt_paged_cache& c, int64_t B, int
 
 int launch_paged_attention(const blt_paged_cache& c, const PagedAttnArgs& a, void* ws,
                            hipStream_t s) {
-  const Shape sh = shape_of(c, a.B, a.total, a.H);
+  Shape sh = shape_of(c, a.B, a.total, a.H);
   const int d = c.head_dim;
   KArgs p{};
   const int64_t es = c.dtype == BLT_DTYPE_BF16 ? 2 : 4;
@@ -1359,7 +1381,8 @@ int launch_paged_attention(const blt_paged_cache& c, const PagedAttnArgs& a, voi
   p.causal = a.causal; p.window = a.causal ? a.window : 0;
   if (p.window > (1 << 30)) p.window = 0;  // longer than any sequence
   p.c = (float)(1.44269504088896340736 * (double)a.scale);
-  p.resident = sh.resident; p.cmin = sh.cmin;
+  if (p.window && p.window < 24 * sh.bkv) sh.spill = 0;  // (too short: its blocks would only exit)
+  p.resident = sh.resident; p.cmin = sh.cmin; p.spill = sh.spill;
   const int64_t slots = slots_of(c, sh, a.B, a.total, a.H);
   p.sync = c.sync; p.status = c.status;
   p.part = (float*)ws;

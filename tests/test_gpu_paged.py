@@ -403,6 +403,33 @@ def test_attention_more_sequences_than_lanes(dtype):
     check_attention(m, n, 4)
 
 
+@pytest.mark.parametrize("dtype,d,H,Hkv,B", [("bf16", 64, 12, 12, 96), ("bf16", 128, 8, 8, 70),
+                                             ("f32", 64, 12, 12, 44), ("f32", 128, 4, 4, 70)])
+def test_attention_row_tiles_just_above_a_round(dtype, d, H, Hkv, B):
+    # (more row tiles than blocks the card holds, by less than half: four rounds of parts)
+    m = Made([2200 + (7 * i) % 41 for i in range(B)], Hkv=Hkv, d=d, page=64, dtype=TYPES[dtype])
+    some = [0, 1, B // 2, B - 1]
+    torch.manual_seed(3)
+    q = torch.randn(B, H, d, device=DEV).to(m.cache.dtype)
+    o = m.cache.attention(0, q, i32(np.arange(B + 1)))
+    assert torch.equal(o, m.cache.attention(0, q, i32(np.arange(B + 1))))
+    for s in some:
+        x = f64(q[s:s + 1])
+        want, A = R.attention(x, m.rows(0, s), m.rows(1, s), m.lens[s])
+        assert (np.abs(f64(o[s:s + 1]) - want) <= att_tol(A, x, m.rows(0, s), m.cache.dtype, d,
+                                                          d ** -0.5) + 1e-30).all(), s
+    assert int(m.cache._sync.abs().max()) == 0
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("lens", [[1500], [5000], [9000], [20000], [700, 9000, 65]])
+def test_attention_of_one_token_joins_many_parts(dtype, lens):
+    m = Made(lens, Hkv=2, d=64, page=16, dtype=TYPES[dtype])
+    check_attention(m, [1] * len(lens), 2)
+    check_attention(m, [1] * len(lens), 6)
+    check_attention(m, [2] * len(lens), 4, window=1400)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_attention_peaked_and_large_scores(dtype):
     """Scores far above and below each other (the running max moves by thousands)."""
