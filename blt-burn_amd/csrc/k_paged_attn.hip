@@ -157,7 +157,7 @@ __device__ bool find_item(const KArgs& p, unsigned bid, Item& it) {
   // the items, and dispatch places block i on XCD i % 8, of which each takes a contiguous
   // run of items: the row tiles of one (sequence, key head) share an L2, and every XCD gets
   // its share of the long sequences (2 chunks of 2048 over 16384 and 11854 keys, 8 key
-  // heads: 790 us, 940 with the sequences outermost).
+  // heads: 795 us, 940 with the sequences outermost).
   int items, inc;  // of all sequences; with up to 64 of them, those up to the lane's own
   for (int tries = 0;; ++tries) {
     items = 0;
@@ -289,7 +289,7 @@ __device__ inline uint32_t finite2(uint32_t x) {
 // so parts are written and read by relaxed atomics of agent scope: they pass the L2s, a
 // write is complete when the wave's counter of stores says so.  (Ordinary accesses
 // between fences write back and invalidate whole L2s: 48 single tokens over up to 8192
-// keys, 12 heads, took 333 us that way, 135 with a second launch that joins, 130 so.)
+// keys, 12 heads, took 333 us that way, 135 with a second launch that joins, 128 so.)
 __device__ inline void put2(float* at, float x, float y) {
   const uint64_t v = (uint64_t)__float_as_uint(x) | (uint64_t)__float_as_uint(y) << 32;
   __hip_atomic_store(reinterpret_cast<uint64_t*>(at), v, __ATOMIC_RELAXED,
@@ -427,7 +427,10 @@ __device__ void join_parts(const KArgs& p, const Item& it, int nr, float* room) 
 // read with the LDS transposing read.  Unlike there q keeps its own bf16 values (scaling it
 // before its rounding costs as much accuracy as the output's rounding): the scores come
 // out of the matrix core minus the running max, and the scale is one multiply before exp2.
-// Chunks of 2048 and 1598 tokens over 16384 and 11854 keys, 32 / 8 heads of 128: 800 us,
+// p is rounded to bf16 for the second product, and the sum takes the rounded values: the
+// outputs are 2.3e-3 off (relative, rms; their own rounding alone is 1.7e-3).  As two halves,
+// as in the form below, the chunks named next take 1080 us.
+// Chunks of 2048 and 1598 tokens over 16384 and 11854 keys, 32 / 8 heads of 128: 795 us,
 // 1.0 PFLOP/s of the visible pairs (an 8192^3 library product reaches 1.4); the matrix cores
 // are busy 46 % of the time and the vector units 43 %, hardly ever both.  With 64 rows a wave
 // (1.2 ms for 0.96 then), three stages, or 32-key tiles at three waves a SIMD it was slower.
@@ -728,10 +731,10 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(KArgs p) {
 // second product's operand).  p goes into that product as two bf16 halves (p rounded, and
 // what the rounding left): the matrix cores have nothing else to do, and the output
 // keeps f32 accuracy up to its own rounding.
-// 48 single tokens over up to 8192 keys, 12 heads of 64: 130 us, 5.0 TB/s; 16 over up to 32768
+// 48 single tokens over up to 8192 keys, 12 heads of 64: 128 us, 5.0 TB/s; 16 over up to 32768
 // keys, 32 / 8 heads of 128: 169 us, 5.5 TB/s (a large copy: 6.15).  One token over 1000 keys,
-// 12 heads: 9.0 us of dependent steps: launch 1.7, find_item 0.7, pages 0.6, tiles 2.1, the
-// waves' merge 1.3, join 2.6.
+// 12 heads: 8.7 us of dependent steps: launch 1.7, find_item 0.5, pages 0.6, tiles 2.1, the
+// waves' merge 1.3, join 2.6; over 8192 keys 15.4 us, over 32768 26.8.
 template <int N>
 __device__ inline void wait_loads() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
@@ -1051,7 +1054,7 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(KArgs p) {
 // As attn_f32_kernel (k_attn.hip): both products on the f32 matrix cores, one block = 32
 // rows, its four waves take every fourth 32-key tile with operands straight from global
 // memory, and meet once at the end.  Chunks of 100, 97 and 87 tokens over 1500, 350 and 87 keys,
-// 12 heads: 22.7 us; two tiles a wave, each 64 MFMAs of 64 cycles behind its loads, then the
+// 12 heads: 22.3 us; two tiles a wave, each 64 MFMAs of 64 cycles behind its loads, then the
 // merge and the join.
 template <int ND>
 __global__ __launch_bounds__(256) void paged_attn_f32_kernel(KArgs p) {
