@@ -504,7 +504,10 @@ int blt_cache_append(const blt_paged_cache* cache, int32_t layer, const void* k,
 
 int64_t blt_paged_attention_workspace_bytes(const blt_paged_cache* cache, int64_t B, int64_t total,
                                             int64_t Hq) {
-  if (!cache || cache->n_kv_heads < 1 || Hq < 0 || B < 0 || total < 0) return 0;
+  // (0 for what blt_paged_attention refuses)
+  if (cache_checks(cache, "paged_attention_workspace_bytes") || Hq < 0 || Hq > 0xffff || B < 0 ||
+      B > 65536 || total < 0 || total > 0x7fffffff)
+    return 0;
   return paged_attention_workspace_bytes(*cache, B, total, (int)Hq);
 }
 int blt_paged_attention(const blt_paged_cache* cache, int32_t layer, const void* q, int64_t st_q,

@@ -89,6 +89,10 @@ def test_bad_attention_calls_are_refused():
     long = desc(max_pages=1 << 16)
     assert L.blt_paged_attention_workspace_bytes(addr(long), 1, 1, 4) > 0
     assert attend(long, ws=None) == -1 and "workspace" in pkg.last_error()
+    for cache, B, total, H in ((None, 1, 1, 4), (desc(page_size=0), 1, 1, 4),
+                               (desc(n_kv_heads=0), 1, 1, 4), (long, -1, 1, 4), (long, 1, -1, 4),
+                               (long, 1, 1 << 40, 4), (long, 1 << 20, 1, 4), (long, 1, 1, 1 << 40)):
+        assert L.blt_paged_attention_workspace_bytes(cache and addr(cache), B, total, H) == 0
     assert attend(d, B=0) == 0 and attend(d, total=0) == 0
 
 
