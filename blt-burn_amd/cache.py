@@ -99,6 +99,7 @@ class PagedCache:
         self._ws_bytes = max(self._lib.blt_paged_attention_workspace_bytes(
             self._ptr, 65536, 65536 * rows, self.n_kv_heads) for rows in (1, 32, 128))
         self._ws = self._workspace(max(self._ws_bytes, 16))
+        self._wsp = self._ws.data_ptr()
 
     # ---- status ---------------------------------------------------------------
     def check(self):
@@ -165,14 +166,15 @@ class PagedCache:
 
     # ---- tokens ---------------------------------------------------------------
     def _rows(self, starts, seqs):
-        p, B = self._list(starts, "starts")
-        B -= 1
-        if B < 0:
+        """(starts pointer, rows, seqs pointer or None)."""
+        p, n = self._list(starts, "starts")
+        if n < 1:
             raise BltError("PagedCache: starts has one entry more than there are sequences")
-        return p, B, None if seqs is None else self._list(seqs, "seqs", B)[0]
+        return p, n - 1, None if seqs is None else self._list(seqs, "seqs", n - 1)[0]
 
     def _tokens(self, t, what, heads=None):
-        """t as [tokens, heads, head_dim] with a dense last dimension, and its heads."""
+        """t [tokens, heads, head_dim] with a dense last dimension: itself or a copy, its
+        pointer, tokens, heads and strides."""
         if not isinstance(t, torch.Tensor):
             raise TypeError("expected a torch.Tensor, got %r" % type(t))
         shape = t.shape
@@ -181,14 +183,22 @@ class PagedCache:
             raise BltError("PagedCache: %s must be %s [tokens, %s, %d] on %s"
                            % (what, self.dtype, "heads" if heads is None else heads,
                               self.head_dim, self.device))
-        return t if t.stride(2) == 1 else t.contiguous()
+        st, sh, sd = t.stride()
+        if sd != 1:
+            t = t.contiguous()
+            st, sh, sd = t.stride()
+        return t, t.data_ptr(), shape[0], shape[1], st, sh
 
     def _output(self, out, like, total, heads):
+        """(out, or a new tensor like `like`; its pointer and strides)"""
         if out is None:
-            return torch.empty_like(like)
-        if self._tokens(out, "out", heads) is not out or out.shape[0] != total:
+            out = torch.empty_like(like)
+            st, sh, _ = out.stride()
+            return out, out.data_ptr(), st, sh
+        t, p, n, _, st, sh = self._tokens(out, "out", heads)
+        if t is not out or n != total:
             raise BltError("PagedCache: out must match q, with a dense last dimension")
-        return out
+        return out, p, st, sh
 
     def append(self, layer, k, v, starts, seqs=None, rotary=None, q=None, out=None):
         """Write the new tokens k, v [total, kv_heads, head_dim] into a layer: row b has
@@ -197,35 +207,29 @@ class PagedCache:
         (reserve).  rotary: a RotaryPlan that rotates k at its positions, and q [total, heads,
         head_dim] if given, which is returned (into `out`, which may be q; tokens at
         starts[-1] and behind are not written).  starts ascends from 0 on."""
-        k = self._tokens(k, "k", self.n_kv_heads)
-        v = self._tokens(v, "v", self.n_kv_heads)
+        k, kp, total, _, ks, kh = self._tokens(k, "k", self.n_kv_heads)
+        v, vp, n, _, vs, vh = self._tokens(v, "v", self.n_kv_heads)
         p, B, s = self._rows(starts, seqs)
-        total = k.shape[0]
-        if v.shape[0] != total:
+        if n != total:
             raise BltError("PagedCache: k and v must have one number of tokens")
-        r = None
+        r, qp, qs, qh, op, os_, oh, Hq = None, None, 0, 0, None, 0, 0, 0
         if rotary is not None:
             if not isinstance(rotary, RotaryPlan):
                 raise TypeError("PagedCache.append expects a RotaryPlan")
-            if rotary.device.index != self._index:
+            if rotary._index != self._index:
                 raise BltError("PagedCache: the rotary plan is on another device")
             r = rotary._ptr
-        qp, qs, op, os_, Hq = None, (0, 0), None, (0, 0), 0
         if q is not None:
             if rotary is None:
                 raise BltError("PagedCache.append: q is rotated only with a rotary plan")
-            q = self._tokens(q, "q")
-            Hq = q.shape[1]
-            if q.shape[0] != total:
+            q, qp, n, Hq, qs, qh = self._tokens(q, "q")
+            if n != total:
                 raise BltError("PagedCache: q and k must have one number of tokens")
-            out = self._output(out, q, total, Hq)
-            qp, qs, op, os_ = q.data_ptr(), q.stride(), out.data_ptr(), out.stride()
+            out, op, os_, oh = self._output(out, q, total, Hq)
         elif out is not None:
             raise BltError("PagedCache.append: out without q")
-        ks, vs = k.stride(), v.stride()
-        self._call(self._lib.blt_cache_append, "cache_append", self._ptr, layer, k.data_ptr(), ks[0],
-                   ks[1], v.data_ptr(), vs[0], vs[1], qp, qs[0], qs[1], op, os_[0], os_[1], Hq, p, s,
-                   B, total, r)
+        self._call(self._lib.blt_cache_append, "cache_append", self._ptr, layer, kp, ks, kh, vp, vs,
+                   vh, qp, qs, qh, op, os_, oh, Hq, p, s, B, total, r)
         return out
 
     def attention(self, layer, q, starts, seqs=None, causal=True, window=0, scale=None, out=None):
@@ -238,22 +242,19 @@ class PagedCache:
         given): 0 where a token sees no key; tokens at starts[-1] and behind are not
         written, nor are those of a row without a sequence, nor any where starts does not
         ascend within q (both set the status)."""
-        q = self._tokens(q, "q")
+        q, qp, total, H, qs, qh = self._tokens(q, "q")
         p, B, s = self._rows(starts, seqs)
-        total, H, d = q.shape
         if H % self.n_kv_heads or H == 0:
             raise BltError("PagedCache: q's heads must be a multiple of the cache's %d"
                            % self.n_kv_heads)
-        st, qp = q.stride(), q.data_ptr()
-        if (st[0] | st[1]) % self._piece or qp % 16:  # rows that are not 16-byte aligned
+        if (qs | qh) % self._piece or qp % 16:  # rows that are not 16-byte aligned
             q = q.clone(memory_format=torch.contiguous_format)
-            st, qp = q.stride(), q.data_ptr()
-        out = self._output(out, q, total, H)
-        so = out.stride()
+            qs, qh, _ = q.stride()
+            qp = q.data_ptr()
+        out, op, os_, oh = self._output(out, q, total, H)
         if window > 0x7fffffff:  # longer than any sequence
             window = 0
-        self._call(self._lib.blt_paged_attention, "paged_attention", self._ptr, layer, qp, st[0],
-                   st[1], out.data_ptr(), so[0], so[1], H, p, s, B, total, 1 if causal else 0,
-                   window, self._scale if scale is None else scale, self._ws.data_ptr(),
-                   self._ws_bytes)
+        self._call(self._lib.blt_paged_attention, "paged_attention", self._ptr, layer, qp, qs, qh, op,
+                   os_, oh, H, p, s, B, total, 1 if causal else 0, window,
+                   self._scale if scale is None else scale, self._wsp, self._ws_bytes)
         return out

@@ -205,6 +205,7 @@ class RotaryPlan:
         if dev.index is None:
             dev = torch.device("cuda", torch.cuda.current_device())
         self.rotary_dim, self.magnitude, self.device = n, mag.value, dev
+        self._index, self._lib = dev.index, _lib.lib()
         self.freq = freq.to(dev)
         self._desc = _lib.Rotary(self.freq.data_ptr(), n, 1 if pairs == "interleaved" else 0,
                                  mag.value)
@@ -225,7 +226,7 @@ def fused_rotary(q, k, positions, plan, backward=False, out=None):
     if not isinstance(plan, RotaryPlan):
         require_cuda(q, positions)
         raise TypeError("fused_rotary expects a RotaryPlan")
-    index, dtype = plan.device.index, q.dtype
+    index, dtype = plan._index, q.dtype
     if q.get_device() != index or positions.get_device() != index:
         require_cuda(q, positions)
         raise BltError("fused_rotary: tensors and plan must be on one device")
@@ -233,7 +234,9 @@ def fused_rotary(q, k, positions, plan, backward=False, out=None):
     if q.dim() != 4:
         raise BltError("fused_rotary expects q [batch, heads, seq, head_dim]")
     B, Hq, T, d = q.shape
-    if positions.dtype != torch.int32 or positions.shape not in ((T,), (B, T)):
+    rows = positions.shape
+    if positions.dtype is not torch.int32 or len(rows) not in (1, 2) or rows[-1] != T or \
+            (len(rows) == 2 and rows[0] != B):
         raise BltError("fused_rotary: positions must be int32 [seq] or [batch, seq]")
     pos = _dense_rows(positions)
     x = _dense_rows(q)
@@ -242,9 +245,10 @@ def fused_rotary(q, k, positions, plan, backward=False, out=None):
         if k.get_device() != index:
             require_cuda(k)
             raise BltError("fused_rotary: tensors and plan must be on one device")
-        if k.dim() != 4 or k.dtype != dtype or k.shape != (B, k.shape[1], T, d):
+        Bk, Hk, Tk, dk = k.shape if k.dim() == 4 else (-1, 0, 0, 0)
+        if k.dtype is not dtype or Bk != B or Tk != T or dk != d:
             raise BltError("fused_rotary: k must be [batch, kv_heads, seq, head_dim] of q's dtype")
-        Hk, y = k.shape[1], _dense_rows(k)
+        y = _dense_rows(k)
         yp, ys = y.data_ptr(), y.stride()
     if out is None:
         qo = torch.empty_like(x)
@@ -264,9 +268,9 @@ def fused_rotary(q, k, positions, plan, backward=False, out=None):
     xs, qs = x.stride(), qo.stride()
     if ko is not None:
         kop, ks = ko.data_ptr(), ko.stride()
-    call_on(plan.device, index, _lib.lib().blt_fused_rotary, "fused_rotary", x.data_ptr(), yp,
+    call_on(plan.device, index, plan._lib.blt_fused_rotary, "fused_rotary", x.data_ptr(), yp,
             qo.data_ptr(), kop, _lib.DTYPE_BF16 if dtype == torch.bfloat16 else _lib.DTYPE_F32, B,
             Hq, Hk, T, d, xs[0], xs[1], xs[2], ys[0], ys[1], ys[2], qs[0], qs[1], qs[2], ks[0],
-            ks[1], ks[2], pos.data_ptr(), pos.stride(0) if pos.dim() == 2 else 0, plan._ptr,
+            ks[1], ks[2], pos.data_ptr(), pos.stride(0) if len(rows) == 2 else 0, plan._ptr,
             1 if backward else 0)
     return qo, ko
