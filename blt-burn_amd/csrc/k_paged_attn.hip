@@ -126,15 +126,17 @@ __device__ bool find_item(const KArgs& p, unsigned bid, Item& it) {
   work = uniform(wave_sum(work)) * (float)p.Hkv;
   tiles = uniform(wave_sum(tiles)) * (float)p.Hkv;
   // Items should fill the chip's resident blocks once, or twice where there are so many row
-  // tiles that items of a single round would differ much in size.  Row tiles that are no
-  // whole number of C make half an item more each, on average: so work / C = blocks -
-  // tiles / 2.  (0.1 % above the exact quotient: the bounds on the grid and the slots
-  // hold whatever the rounding of the sums.)
+  // tiles that items of a single round would differ much in size and that round is a long
+  // one (64 single tokens over up to 3000 keys, 12 heads, 56 us in one round and 52 in two;
+  // over up to 500, 15 and 19).  Row tiles that are no whole number of C make half an
+  // item more each, on average: so work / C = blocks - tiles / 2.  (0.1 % above the exact
+  // quotient: the bounds on the grid and the slots hold whatever the rounding of the sums.)
   // Row tiles just above one round would leave the next one nearly empty: four rounds of parts,
   // where these are not too short (see shape_of).
   const bool spill = p.spill && tiles > (float)p.resident && tiles <= 1.5f * (float)p.resident &&
                      work >= 32.f * tiles;
-  const float blocks = (spill ? 4.f : 2.f * tiles > (float)p.resident ? 2.f : 1.f) * p.resident;
+  const bool twice = 2.f * tiles > (float)p.resident && work >= 12.f * p.resident;
+  const float blocks = (spill ? 4.f : twice ? 2.f : 1.f) * p.resident;
   const float fill = fmaxf(blocks - 0.5f * tiles, 0.5f * (float)p.resident);
   int C = max(p.cmin, (int)fminf(ceilf(work * 1.001f / fill), 1e9f));
   // Row tiles that fill a round between them and are of about one length stay whole: parts of
