@@ -147,12 +147,12 @@ __device__ bool find_item(const KArgs& p, unsigned bid, Item& it) {
     C = max(C, (int)longest);
   int ns;
   auto parts_of = [&]() {
-    // (a part costs as much as a few key tiles to write and join: in proportion to its
-    // rows, a quarter of them in the form for 128; and the more there are of one row tile,
-    // the longer their joining takes: one token over 8192 keys, 12 heads, 16.0 us in parts of
+    // (a part costs as much as a few key tiles to write and join, in proportion to its rows:
+    // one chunk of 1578, 12 heads, 28 us with a quarter of them, 21 with a sixteenth; and the
+    // more there are of one row tile, the longer their joining takes: one token over 8192 keys, 12 heads, 16.0 us in parts of
     // four tiles and 17.8 in parts of two, over 1000 keys 10.4 and 8.7)
     const int r = q.n * p.G, long_row = BKV < 64 || kt < 64 ? 0 : max(2, kt >> 6);
-    const int most = max(C, p.cmin + long_row + (r < BQ ? r : BQ) / (BQ >= 128 ? 4 : 16));
+    const int most = max(C, p.cmin + long_row + (r < BQ ? r : BQ) / 16);
     ns = (int)((uint32_t)(kt + most - 1) / (uint32_t)most);
   };
   // Items, partial slots and counters of one key head.  Key heads are the outermost order of
@@ -316,6 +316,21 @@ __device__ inline f32x4_t get4(const float* at) {
   v.z = x; v.w = y;
   return v;
 }
+// Every thread of the block has written its share of the part: is it the last one?
+__device__ inline bool last_part(const KArgs& p, const Item& it) {
+  __shared__ int last;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this thread's share, before the count
+  __syncthreads();
+  int* counter = p.sync + it.join + it.rt;
+  if (threadIdx.x == 0) {
+    last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+           it.ns - 1;
+    if (last) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  return last;
+}
+// The forms for few rows: parts [rows][D].
 // A thread takes four columns of a row at a time; where that leaves threads over and there
 // are many parts, groups of threads take runs of them and meet in `room` (6 NT words of LDS
 // that nobody uses any more).  Called by all threads of a block of NT.
@@ -333,17 +348,7 @@ __device__ inline void join(Joined& a, const Joined& b, float c) {
 }
 template <int D, int BQ, int NT, typename T>
 __device__ void join_parts(const KArgs& p, const Item& it, int nr, float* room) {
-  __shared__ int last;
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this thread's part, before the count
-  __syncthreads();
-  int* counter = p.sync + it.join + it.rt;
-  if (threadIdx.x == 0) {
-    last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
-           it.ns - 1;
-    if (last) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  }
-  __syncthreads();
-  if (!last) return;
+  if (!last_part(p, it)) return;
   // U parts at a time, everything of them in flight at once (a read that passes the L2 takes
   // about 1 us), with a running max; past the last part: the last one again, without weight
   const int64_t step = (int64_t)it.nrt * BQ;
@@ -698,19 +703,65 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(KArgs p) {
   float a, b;
   swap_pair<32>(l, a, b);
   const float lt = a + b;
-  if (row < rows && it.ns > 1) {
-    const int64_t at = slot_of(it, it.split) * BQ + (row - r0);
+  float total = lt;
+  if (it.ns > 1) {
+    // A part is laid out as the threads hold it, [D / 4][256] pairs, so that whole lines are
+    // written and read: the last block's threads take up the values of their own rows.  (By
+    // rows, with every lane's 16 bytes in another line, 4 chunks of 512 over 4096 keys, 12
+    // heads, took 64 us instead of 53.)
+    constexpr int PAIRS = D / 4;
+    const int trow = wid * QPW + lrow;
+    if (wave_active) {
+      const int64_t slot = slot_of(it, it.split);
+      float* at = p.part + slot * BQ * D + tid * 2;
 #pragma unroll
-    for (int ds = 0; ds < DS; ++ds)
+      for (int k = 0; k < PAIRS; ++k)
+        put2(at + k * 512, o[k >> 3][2 * (k & 7)], o[k >> 3][2 * (k & 7) + 1]);
+      if (lhalf == 0) put2(p.ml + (slot * BQ + trow) * 2, m, lt);
+    }
+    if (!last_part(p, it) || !wave_active) return;
+    constexpr int U = 2;  // parts in flight at once (more would cost a block a CU)
+    float mx = -INFINITY;
+    total = 0.f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        put4(p.part + at * D + ds * 32 + 8 * j + 4 * lhalf,
-             f32x4_t{o[ds][4 * j], o[ds][4 * j + 1], o[ds][4 * j + 2], o[ds][4 * j + 3]});
-    if (lhalf == 0) put2(p.ml + at * 2, m, lt);
-  } else if (row < rows) {
+    for (int j = 0; j < DS; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[j][r] = 0.f;
+    for (int x0 = 0; x0 < it.ns; x0 += U) {
+      float pm[U], pl[U], v[U][D / 2];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {  // (past the last part: the last one again, left out)
+        const int64_t slot = slot_of(it, min(x0 + u, it.ns - 1));
+        const float* at = p.part + slot * BQ * D + tid * 2;
+        get2(p.ml + (slot * BQ + trow) * 2, pm[u], pl[u]);
+#pragma unroll
+        for (int k = 0; k < PAIRS; ++k) get2(at + k * 512, v[u][2 * k], v[u][2 * k + 1]);
+      }
+      float mn = mx;
+#pragma unroll
+      for (int u = 0; u < U; ++u) mn = fmaxf(mn, pm[u]);
+      const float mu = mn == -INFINITY ? 0.f : mn;
+      const float alpha = __builtin_amdgcn_exp2f((mx - mu) * c);
+      mx = mn;
+      total *= alpha;
+#pragma unroll
+      for (int j = 0; j < DS; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[j][r] *= alpha;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (x0 + u < it.ns) {
+          const float w = __builtin_amdgcn_exp2f((pm[u] - mu) * c);
+          total = fmaf(w, pl[u], total);
+#pragma unroll
+          for (int k = 0; k < D / 2; ++k) o[k >> 4][k & 15] = fmaf(w, v[u][k], o[k >> 4][k & 15]);
+        }
+    }
+  }
+  if (row < rows) {
     uint16_t* orow = (uint16_t*)p.o + (int64_t)(sq.s0 + tok) * p.st_o + (int64_t)head * p.sh_o;
     // hardware reciprocal (1 ulp): the output is rounded to bf16
-    const float inv = lt > 0.f ? __builtin_amdgcn_rcpf(lt) : lt == lt ? 0.f : lt;
+    const float inv = total > 0.f ? __builtin_amdgcn_rcpf(total) : total == total ? 0.f : total;
 #pragma unroll
     for (int ds = 0; ds < DS; ++ds)
 #pragma unroll
@@ -721,7 +772,6 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(KArgs p) {
         *reinterpret_cast<u32x2_t*>(orow + ds * 32 + 8 * j + 4 * lhalf) = w;
       }
   }
-  if (it.ns > 1) join_parts<D, BQ, 256, uint16_t>(p, it, r1 - r0 + 1, reinterpret_cast<float*>(lds));
 }
 
 // ---- bf16, few rows ----------------------------------------------------------------
@@ -1298,7 +1348,8 @@ struct Shape {
 };
 // resident: blocks the chip holds at once by their registers and LDS (f32 with d = 128: one
 // per CU; with two assumed, 3 chunks of 100 tokens over 1500 keys, 32 / 8 heads, took 85 us
-// instead of 68).  A counter for every row tile with parts: at most 2 * resident (two parts
+// instead of 68; tiles of 128 rows with d = 64 three, one chunk of 1473 over 8319 keys, 12
+// heads, 69 us with two assumed and 62).  A counter for every row tile with parts: at most 2 * resident (two parts
 // or more of each) or, with a spill, 1.5 * resident of them, <= BLT_CACHE_SYNC_WORDS.  The form goes by the rows a sequence has on average: a tile of 16 rows costs the
 // matrix cores half of one of 32, and 128 rows share what they read; every form takes any
 // chunk, in more row tiles.
@@ -1312,7 +1363,7 @@ int64_t row_tiles(const blt_paged_cache& c, int64_t B, int64_t total, int H, int
 Shape shape_of(const blt_paged_cache& c, int64_t B, int64_t total, int H) {
   const int64_t rows = total * (H / c.n_kv_heads);  // of all sequences, per key head
   const int few = c.head_dim == 64 ? 1024 : 512;  // 32 and 64 KB of rings
-  Shape s{FORM_TILES, 128, 64, 512, 2, 0};
+  Shape s{FORM_TILES, 128, 64, c.head_dim == 64 ? 768 : 512, 2, 0};
   if (c.dtype == BLT_DTYPE_F32) s = Shape{FORM_F32, 32, 32, few / 2, 4, 0};
   else if (rows <= 16 * B) s = Shape{FORM_FEW16, 16, 64, few, 2, 0};
   else if (rows <= 32 * B) s = Shape{FORM_FEW32, 32, 64, few, 2, 0};
