@@ -426,6 +426,65 @@ __device__ void join_parts(const KArgs& p, const Item& it, int nr, float* room) 
   store(i, a);
 }
 
+// The forms for 128 rows, a wave with 32 of them and o in the accumulators' layout.  A part is
+// laid out as the threads hold it, [D / 4][256] pairs, so that whole lines are written and
+// read: the last block's threads take up the values of their own rows.  (By rows, with every
+// lane's 16 bytes in another line, 4 chunks of 512 over 4096 keys, 12 heads, took 64 us
+// instead of 53.)  False where the thread has nothing to store; else o, total are the row's.
+template <int D>
+__device__ inline bool join_tiles(const KArgs& p, const Item& it, bool active,
+                                  f32x16_t (&o)[D / 32], float m, float& total) {
+  constexpr int BQ = 128, PAIRS = D / 4;
+  const int tid = threadIdx.x, trow = (tid >> 6) * 32 + (tid & 31);
+  if (active) {
+    const int64_t slot = slot_of(it, it.split);
+    float* at = p.part + slot * BQ * D + tid * 2;
+#pragma unroll
+    for (int k = 0; k < PAIRS; ++k)
+      put2(at + k * 512, o[k >> 3][2 * (k & 7)], o[k >> 3][2 * (k & 7) + 1]);
+    if (!(tid & 32)) put2(p.ml + (slot * BQ + trow) * 2, m, total);
+  }
+  if (!last_part(p, it) || !active) return false;
+  constexpr int U = 2;  // parts in flight at once (more would cost a block a CU)
+  float mx = -INFINITY;
+  total = 0.f;
+#pragma unroll
+  for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[j][r] = 0.f;
+  for (int x0 = 0; x0 < it.ns; x0 += U) {
+    float pm[U], pl[U], v[U][D / 2];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {  // (past the last part: the last one again, left out)
+      const int64_t slot = slot_of(it, min(x0 + u, it.ns - 1));
+      const float* at = p.part + slot * BQ * D + tid * 2;
+      get2(p.ml + (slot * BQ + trow) * 2, pm[u], pl[u]);
+#pragma unroll
+      for (int k = 0; k < PAIRS; ++k) get2(at + k * 512, v[u][2 * k], v[u][2 * k + 1]);
+    }
+    float mn = mx;
+#pragma unroll
+    for (int u = 0; u < U; ++u) mn = fmaxf(mn, pm[u]);
+    const float mu = mn == -INFINITY ? 0.f : mn;
+    const float alpha = __builtin_amdgcn_exp2f((mx - mu) * p.c);
+    mx = mn;
+    total *= alpha;
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[j][r] *= alpha;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (x0 + u < it.ns) {
+        const float w = __builtin_amdgcn_exp2f((pm[u] - mu) * p.c);
+        total = fmaf(w, pl[u], total);
+#pragma unroll
+        for (int k = 0; k < D / 2; ++k) o[k >> 4][k & 15] = fmaf(w, v[u][k], o[k >> 4][k & 15]);
+      }
+  }
+  return true;
+}
+
 // ---- bf16, tiles of rows ---------------------------------------------------------
 // One block = 4 waves of 32 rows each; key tiles of 64 keys go global -> LDS by DMA
 // through NST stages shared by the waves.  As in attn_fwd_kernel the scores are taken
@@ -704,60 +763,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(KArgs p) {
   swap_pair<32>(l, a, b);
   const float lt = a + b;
   float total = lt;
-  if (it.ns > 1) {
-    // A part is laid out as the threads hold it, [D / 4][256] pairs, so that whole lines are
-    // written and read: the last block's threads take up the values of their own rows.  (By
-    // rows, with every lane's 16 bytes in another line, 4 chunks of 512 over 4096 keys, 12
-    // heads, took 64 us instead of 53.)
-    constexpr int PAIRS = D / 4;
-    const int trow = wid * QPW + lrow;
-    if (wave_active) {
-      const int64_t slot = slot_of(it, it.split);
-      float* at = p.part + slot * BQ * D + tid * 2;
-#pragma unroll
-      for (int k = 0; k < PAIRS; ++k)
-        put2(at + k * 512, o[k >> 3][2 * (k & 7)], o[k >> 3][2 * (k & 7) + 1]);
-      if (lhalf == 0) put2(p.ml + (slot * BQ + trow) * 2, m, lt);
-    }
-    if (!last_part(p, it) || !wave_active) return;
-    constexpr int U = 2;  // parts in flight at once (more would cost a block a CU)
-    float mx = -INFINITY;
-    total = 0.f;
-#pragma unroll
-    for (int j = 0; j < DS; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) o[j][r] = 0.f;
-    for (int x0 = 0; x0 < it.ns; x0 += U) {
-      float pm[U], pl[U], v[U][D / 2];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {  // (past the last part: the last one again, left out)
-        const int64_t slot = slot_of(it, min(x0 + u, it.ns - 1));
-        const float* at = p.part + slot * BQ * D + tid * 2;
-        get2(p.ml + (slot * BQ + trow) * 2, pm[u], pl[u]);
-#pragma unroll
-        for (int k = 0; k < PAIRS; ++k) get2(at + k * 512, v[u][2 * k], v[u][2 * k + 1]);
-      }
-      float mn = mx;
-#pragma unroll
-      for (int u = 0; u < U; ++u) mn = fmaxf(mn, pm[u]);
-      const float mu = mn == -INFINITY ? 0.f : mn;
-      const float alpha = __builtin_amdgcn_exp2f((mx - mu) * c);
-      mx = mn;
-      total *= alpha;
-#pragma unroll
-      for (int j = 0; j < DS; ++j)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[j][r] *= alpha;
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (x0 + u < it.ns) {
-          const float w = __builtin_amdgcn_exp2f((pm[u] - mu) * c);
-          total = fmaf(w, pl[u], total);
-#pragma unroll
-          for (int k = 0; k < D / 2; ++k) o[k >> 4][k & 15] = fmaf(w, v[u][k], o[k >> 4][k & 15]);
-        }
-    }
-  }
+  if (it.ns > 1 && !join_tiles<D>(p, it, wave_active, o, m, total)) return;
   if (row < rows) {
     uint16_t* orow = (uint16_t*)p.o + (int64_t)(sq.s0 + tok) * p.st_o + (int64_t)head * p.sh_o;
     // hardware reciprocal (1 ulp): the output is rounded to bf16
@@ -1337,8 +1343,243 @@ __global__ __launch_bounds__(256) void paged_attn_f32_kernel(KArgs p) {
   if (it.ns > 1) join_parts<D, BQ, 256, float>(p, it, nq, so);
 }
 
+// ---- f32, tiles of rows ----------------------------------------------------------
+// Many long chunks with d = 128, where the form above has one block a CU: as in
+// paged_attn_kernel a block has 4 waves of 32 rows each that share key tiles (of 32 keys here)
+// moved by LDS DMA through two stages, two blocks a CU, with the f32 products of the form
+// above; a quarter of its reads of K and V, and nothing to merge.  32 / 8 heads: chunks of up
+// to 107 tokens in 25 sequences 50 us (80 in the form above), of up to 1025 over up to 2045
+// keys in two, window 300, 125 (182), 4 of up to 1024 265 (316).  With few row tiles their keys
+// take too long one after the other (7 chunks of up to 566, 4 / 2 heads, 61 and 53), and with
+// d = 64 the form above has two blocks a CU itself (10 of up to 400, 12 heads, 58 and 39).
+__global__ __launch_bounds__(256, 2) void paged_attn_f32_tiles_kernel(KArgs p) {
+  constexpr int D = 128, BKV = 32, QPW = 32, BQ = 4 * QPW, ND = D / 32, NC = D / 8;
+  constexpr int TILE = BKV * D, STAGE = 2 * TILE, NST = 2;
+  constexpr int CPR = D / 4, RPI = 64 / CPR, NI = 8 / RPI;  // chunks of a row; rows of a DMA
+  constexpr int VW = 4, NV = ND / VW;                       // V's columns as in the form above
+  typedef float vf_t __attribute__((ext_vector_type(VW)));
+  __shared__ __attribute__((aligned(1024))) float lds[NST * STAGE];
+  __shared__ int ptab[PT];
+
+  Item it;
+  if (!find_item<BQ, BKV>(p, blockIdx.x, it)) return;
+  const Seq& sq = it.q;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l31 = lane & 31, h = lane >> 5;
+  const int rows = sq.n * p.G, first = sq.len - sq.n;
+  int lo, hi;
+  const int r0 = it.rt * BQ, r1 = min(r0 + BQ, rows) - 1;
+  key_range(p, sq, r0, r1, lo, hi);
+  const int t_lo = lo / BKV, cnt = hi < 0 ? 0 : hi / BKV - t_lo + 1;
+  int t0, t1;
+  part_of(it, t_lo, cnt, t0, t1);
+  // the wave's rows and keys
+  const int rw = r0 + wid * QPW, rwl = min(rw + QPW, rows) - 1;
+  const bool wave_active = rw < rows;
+  int wlo = 0, whi = -1;
+  if (wave_active) key_range(p, sq, rw, rwl, wlo, whi);
+  const int pos_first = first + over(rw, p.by_g);
+  const int lo_last = p.window ? first + over(rwl, p.by_g) - p.window + 1 : 0;
+
+  const int row = min(rw + l31, rows - 1);
+  const int tok = over(row, p.by_g), head = it.kvh * p.G + row - tok * p.G;
+  const int khi = p.causal ? min(first + tok, sq.len - 1) : sq.len - 1;
+  const int klo = p.window ? first + tok - p.window + 1 : 0;
+  f32x4_t qf[NC];
+  {
+    const float* qrow =
+        (const float*)p.q + (int64_t)(sq.s0 + tok) * p.st_q + (int64_t)head * p.sh_q;
+#pragma unroll
+    for (int j = 0; j < NC; ++j) qf[j] = *reinterpret_cast<const f32x4_t*>(qrow + 8 * j + 4 * h);
+  }
+  int wbase = (t0 * BKV) >> p.lps;
+  if (t0 < t1) stage_pages(p, sq, wbase, ptab, tid, 256);
+  // consumed here, before any DMA is in flight
+#pragma unroll
+  for (int j = 0; j < NC; ++j) asm volatile("" ::"v"(qf[j]));
+  __syncthreads();
+
+  // DMA.  Wave w moves keys 8 w .. 8 w + 7 of a tile (one page), RPI at a time.  16-byte
+  // chunk c of K's row k is stored at c ^ (k & 15), so that 16 lanes' reads of one chunk
+  // of 16 rows spread over all banks; V is read along its rows.
+  const unsigned lds_base = (unsigned)(uintptr_t)lds;
+  const int kin = lane / CPR, slot = lane % CPR;
+  auto issue = [&](int t, int stage) {
+    const int key0 = t * BKV + 8 * wid;
+    const int kc = min(key0, (sq.len - 1) & ~7);  // the group that is read
+    const int page = __builtin_amdgcn_readfirstlane(ptab[(kc >> p.lps) - wbase]);
+    const int64_t off =
+        (((((int64_t)page * p.Hkv + it.kvh) << p.lps) + (kc & ((1 << p.lps) - 1))) * D) * 4;
+    const unsigned la = lds_base + (unsigned)(stage * STAGE + 8 * wid * D) * 4;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int k = kin + RPI * i;
+      // rows past the end read the last key
+      const int from = key0 + 8 <= sq.len ? k : min(key0 + k, sq.len - 1) - kc;
+      const int kch = slot ^ ((8 * wid + k) & 15);
+      dma16_so((const char*)p.k + off, (unsigned)(from * D * 4 + kch * 16), la + i * 1024);
+      dma16_so((const char*)p.v + off, (unsigned)(from * D * 4 + slot * 16),
+               la + TILE * 4 + i * 1024);
+    }
+  };
+  f32x16_t o[ND];
+#pragma unroll
+  for (int n = 0; n < ND; ++n)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[n][i] = 0.f;
+  float m = -INFINITY, l = 0.f;
+  const float c = p.c;
+
+  // operand reads are not moved over it: all of a tile's would not fit the registers
+  auto some_at_once = [] { asm volatile("" ::: "memory"); };
+  auto need = [&](int t) {  // (as in paged_attn_kernel)
+    const int last = min(t * BKV + BKV - 1, sq.len - 1) >> p.lps;
+    if (last >= wbase + PT) {
+      wbase = (t * BKV) >> p.lps;
+      stage_pages(p, sq, wbase, ptab, tid, 256);
+      __syncthreads();
+    }
+  };
+  if (t0 < t1) issue(t0, 0);
+  int stage = 0;
+  for (int t = t0; t < t1; ++t) {
+    // tile t has landed and every wave is past tile t - 1, whose stage is free
+    dma_wait_barrier<0>();
+    if (t + 1 < t1) {
+      need(t + 1);
+      issue(t + 1, stage ^ 1);
+    }
+    const int kb = t * BKV;
+    if (wave_active && kb <= whi && kb + BKV > wlo) {
+      const float* sk = lds + stage * STAGE;
+      const float* sv = sk + TILE;
+      const bool mask = kb + BKV - 1 > (p.causal ? pos_first : sq.len - 1) ||
+                        kb + BKV > sq.len || kb < lo_last;
+      f32x16_t s, s1;  // two chains of alternate chunks: less rounding in each
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = s1[i] = 0.f;
+#pragma unroll
+      for (int j = 0; j < NC; ++j) {
+        const f32x4_t kf =
+            *reinterpret_cast<const f32x4_t*>(sk + l31 * D + (((2 * j + h) ^ (l31 & 15)) << 2));
+        f32x16_t& a = j & 1 ? s1 : s;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          a = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[e], qf[j][e], a, 0, 0, 0);
+        if ((j & 3) == 3) some_at_once();
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] += s1[i];
+      if (mask) {
+        const int up = khi - kb - 4 * h, dn = klo - kb - 4 * h;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int key = 8 * (i >> 2) + (i & 3);
+          s[i] = key <= up && key >= dn ? s[i] : -INFINITY;
+        }
+      }
+      float mt = s[0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) mt = fmaxf(mt, s[i]);
+      {
+        float a, b;
+        swap_pair<32>(mt, a, b);
+        mt = fmaxf(a, b);
+      }
+      if (__any(mt > m)) {
+        const float m_new = fmaxf(m, mt);
+        const float alpha = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - m_new) * c);
+        m = m_new;
+        l *= alpha;
+#pragma unroll
+        for (int n = 0; n < ND; ++n)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[n][i] *= alpha;
+      }
+      const float mu = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[i] = __builtin_amdgcn_exp2f((s[i] - mu) * c);
+        l += s[i];
+      }
+      // V of key kb + 8 (i / 4) + 4 h + i % 4
+      auto v_at = [&](int i, int n) {
+        return *reinterpret_cast<const vf_t*>(sv + (8 * (i >> 2) + 4 * h + (i & 3)) * D +
+                                              VW * l31 + 32 * VW * n);
+      };
+      bool odd = false;  // a value that is not finite, where rows see different keys
+      if (mask) {
+        uint32_t seen = 0;  // the largest magnitude, as bits
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+#pragma unroll
+          for (int n = 0; n < NV; ++n) {
+            const vf_t x = v_at(i, n);
+#pragma unroll
+            for (int u = 0; u < VW; ++u) seen = max(seen, __float_as_uint(x[u]) & 0x7fffffffu);
+          }
+        odd = __any(seen >= 0x7f800000u);
+      }
+      if (!odd) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+#pragma unroll
+          for (int n = 0; n < NV; ++n) {
+            const vf_t x = v_at(i, n);
+#pragma unroll
+            for (int u = 0; u < VW; ++u)
+              o[n * VW + u] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[u], s[i], o[n * VW + u], 0, 0, 0);
+          }
+          if ((i & 3) == 3) some_at_once();
+        }
+      } else {  // (as in paged_attn_kernel: added to the rows that see it, out of the product)
+        for (int j = 0; j < BKV; ++j) {
+          const bool sees = kb + j <= khi && kb + j >= klo;
+#pragma unroll
+          for (int n = 0; n < ND; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float x =
+                  sv[j * D + VW * (8 * (i >> 2) + 4 * h + (i & 3)) + n % VW + 32 * VW * (n / VW)];
+              o[n][i] += sees && !(fabsf(x) < INFINITY) ? x : 0.f;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+#pragma unroll
+          for (int n = 0; n < NV; ++n) {
+            const vf_t x = v_at(i, n);
+#pragma unroll
+            for (int u = 0; u < VW; ++u)
+              o[n * VW + u] = __builtin_amdgcn_mfma_f32_32x32x2f32(
+                  fabsf(x[u]) < INFINITY ? x[u] : 0.f, s[i], o[n * VW + u], 0, 0, 0);
+          }
+      }
+    }
+    stage ^= 1;
+  }
+
+  float a, b;
+  swap_pair<32>(l, a, b);
+  float total = a + b;
+  if (it.ns > 1 && !join_tiles<D>(p, it, wave_active, o, m, total)) return;
+  if (rw + l31 < rows) {
+    float* orow = (float*)p.o + (int64_t)(sq.s0 + tok) * p.st_o + (int64_t)head * p.sh_o;
+#pragma unroll
+    for (int n = 0; n < NV; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        vf_t x;
+#pragma unroll
+        for (int u = 0; u < VW; ++u) x[u] = total == 0.f ? 0.f : o[n * VW + u][i] / total;
+        *reinterpret_cast<vf_t*>(orow + VW * (8 * (i >> 2) + 4 * h + (i & 3)) + 32 * VW * n) = x;
+      }
+  }
+}
+
 // ---- launch ------------------------------------------------------------------------
-enum Form { FORM_TILES, FORM_FEW16, FORM_FEW32, FORM_F32 };
+enum Form { FORM_TILES, FORM_FEW16, FORM_FEW32, FORM_F32, FORM_F32_TILES };
 struct Shape {
   Form form;
   int bq, bkv;
@@ -1364,10 +1605,14 @@ Shape shape_of(const blt_paged_cache& c, int64_t B, int64_t total, int H) {
   const int64_t rows = total * (H / c.n_kv_heads);  // of all sequences, per key head
   const int few = c.head_dim == 64 ? 1024 : 512;  // 32 and 64 KB of rings
   Shape s{FORM_TILES, 128, 64, c.head_dim == 64 ? 768 : 512, 2, 0};
-  if (c.dtype == BLT_DTYPE_F32) s = Shape{FORM_F32, 32, 32, few / 2, 4, 0};
+  // (enough of the larger row tiles for half the chip, with d = 128: see the form)
+  if (c.dtype == BLT_DTYPE_F32 && c.head_dim == 128 && rows > 64 * B &&
+      row_tiles(c, B, total, H, 128) * c.n_kv_heads >= 256)
+    s = Shape{FORM_F32_TILES, 128, 32, 512, 4, 0};
+  else if (c.dtype == BLT_DTYPE_F32) s = Shape{FORM_F32, 32, 32, few / 2, 4, 0};
   else if (rows <= 16 * B) s = Shape{FORM_FEW16, 16, 64, few, 2, 0};
   else if (rows <= 32 * B) s = Shape{FORM_FEW32, 32, 64, few, 2, 0};
-  s.spill = s.form != FORM_TILES && 5 * B * c.n_kv_heads <= 7 * s.resident &&
+  s.spill = s.bq < 128 && 5 * B * c.n_kv_heads <= 7 * s.resident &&
             row_tiles(c, B, total, H, s.bq) * c.n_kv_heads > s.resident;
   return s;
 }
@@ -1386,7 +1631,7 @@ int64_t blocks_of(const blt_paged_cache& c, const Shape& s, int64_t B, int64_t t
 }
 int64_t slots_of(const blt_paged_cache& c, const Shape& s, int64_t B, int64_t total, int H) {
   const int64_t rt = row_tiles(c, B, total, H, s.bq) * c.n_kv_heads;
-  const int64_t most = most_parts(c, s), all = (s.form == FORM_TILES ? 4 : 8) * (int64_t)s.resident;
+  const int64_t most = most_parts(c, s), all = (s.bq < 128 ? 8 : 4) * (int64_t)s.resident;
   return most < 2 ? 0 : rt * most < all ? rt * most : all;
 }
 
@@ -1402,6 +1647,9 @@ int run_paged(const KArgs& p, const Shape& sh, unsigned nb, hipStream_t s) {
       break;
     case FORM_FEW32:
       hipLaunchKernelGGL((paged_attn_few_kernel<D, 2, 2>), grid, dim3(128), 0, s, p);
+      break;
+    case FORM_F32_TILES:
+      hipLaunchKernelGGL(paged_attn_f32_tiles_kernel, grid, block, 0, s, p);
       break;
     default:
       hipLaunchKernelGGL((paged_attn_f32_kernel<D / 32>), grid, block, 0, s, p);

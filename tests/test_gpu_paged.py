@@ -421,6 +421,33 @@ def test_attention_row_tiles_just_above_a_round(dtype, d, H, Hkv, B):
     assert int(m.cache._sync.abs().max()) == 0
 
 
+@pytest.mark.parametrize("page,window,causal", [(8, 0, True), (32, 130, True), (16, 0, False)])
+def test_attention_f32_of_many_long_chunks(page, window, causal):
+    # (its own form: tiles of 128 rows, d = 128; a chunk of nothing and one of one token too)
+    lens = [1100, 700, 130, 90, 2100, 640, 1, 333]
+    m = Made(lens, Hkv=8, d=128, page=page, dtype=torch.float32, seed=page)
+    check_attention(m, [300, 700, 130, 0, 257, 129, 1, 64], 32, window=window, causal=causal)
+    check_attention(m, [200, 65, 130, 90, 999, 129, 1, 333], 16, window=window, causal=causal,
+                    strided=True)
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_attention_f32_of_many_long_chunks_masked_values(value):
+    m = Made([600, 500, 700, 650], Hkv=8, d=128, dtype=torch.float32)
+    m.kv[1][0, m.table[0, 599 // 16], :, 599 % 16, 3] = value  # seen by the last token alone
+    torch.manual_seed(1)
+    q = torch.randn(1800, 16, 128, device=DEV)
+    n = [600, 300, 500, 400]
+    starts = i32(np.concatenate([[0], np.cumsum(n)]))
+    got = f64(m.cache.attention(0, q, starts))
+    m.kv[1][0, m.table[0, 599 // 16], :, 599 % 16, 3] = 0.5
+    want = f64(m.cache.attention(0, q, starts))
+    ok = np.ones(got.shape, bool)
+    ok[599, :, 3] = False
+    assert np.array_equal(got[ok], want[ok])
+    assert not np.isfinite(got[599, :, 3]).any()
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("lens", [[1500], [5000], [9000], [20000], [700, 9000, 65]])
 def test_attention_of_one_token_joins_many_parts(dtype, lens):
