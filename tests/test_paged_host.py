@@ -178,3 +178,16 @@ def test_host_pool_model():
     p.compact()
     assert p.refs.tolist() == [1, 1, 1, 0, 0, 0] and p.table[2, :2].tolist() == [0, 1]
     assert not p.reserve([0], [8 * 4])
+
+
+def test_the_largest_calls_need_the_most_workspace():
+    """What PagedCache allocates (the largest call of every form) covers every call."""
+    rng = np.random.default_rng(0)
+    for _ in range(3000):
+        K, d, dtype = int(rng.choice([1, 2, 4, 8, 12])), int(rng.choice([64, 128])), int(rng.integers(2))
+        c = desc(dtype=dtype, n_kv_heads=K, head_dim=d, page_size=int(rng.choice([8, 64, 1024])),
+                 max_pages=int(rng.choice([1, 3, 40, 5000])), max_seqs=65536)
+        size = lambda B, total, H: L.blt_paged_attention_workspace_bytes(addr(c), B, total, H)
+        most = max(size(65536, 65536 * rows, K) for rows in (1, 32, 128))
+        B, G = int(rng.choice([1, 2, 20, 70, 300, 65536])), int(rng.choice([1, 2, 4, 7]))
+        assert size(B, B * int(rng.choice([1, 2, 7, 33, 64, 65, 200])), K * G) <= most
