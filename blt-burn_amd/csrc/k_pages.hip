@@ -180,19 +180,48 @@ __global__ __launch_bounds__(NT) void reserve_kernel(blt_paged_cache c, int lps,
 
 // ---- copies --------------------------------------------------------------------
 // The first `fill` tokens of a page in one layer's k or v, by 256 threads (this one is
-// `tid`): 16 bytes a lane, four in flight.  Callers' grids walk (pair, layer, k or v).
+// `tid`): 16 bytes a lane, four in flight.  Callers' grids walk (pair, layer, k or v, part):
+// a few pages of more than 32 KB go in parts, so that they are not a few teams' work (one
+// started 393 KB page in 14 layers: a fork of four, growth and drop 36 us in one part, 18 so).
 // Whole pages (compaction, copy_pages) are moved past the caches: 400 MB of them take 167 us
 // so and 175 us through the caches (6.15 TB/s is a large plain copy).  The started pages of a
 // fork or a trim are read by the next step's attention and stay cached.
+struct Parts {
+  int n, pieces;  // parts of a page, 16-byte pieces of each
+};
+// pages: of one layer's k or v, to be copied
+__host__ __device__ inline Parts page_parts(const blt_paged_cache& c, int64_t pages, int es) {
+  const int pieces = c.n_kv_heads * (c.page_size * c.head_dim * es / 16);
+  const int most = (pieces + 2047) / 2048;
+  if (most == 1 || pages >= 1024) return Parts{1, pieces};
+  const int n = pages < 1 ? most : 2048 / (int)pages;
+  const int parts = n < most ? n : most;
+  return Parts{parts, (pieces + parts - 1) / parts};
+}
+// Item `it` of a walk: its pair, layer, k or v, and first piece.
+struct CopyItem {
+  int64_t pair;
+  int layer, kv, first;
+};
+__device__ inline CopyItem copy_item(int64_t it, int n_layers, const Parts& parts) {
+  if (it >> 32) {  // (parts.n is 1 where there are so many)
+    const int64_t pair = it / (n_layers * 2);
+    const int r = (int)(it - pair * (n_layers * 2));
+    return CopyItem{pair, r >> 1, r & 1, 0};
+  }
+  const uint32_t page = parts.n == 1 ? (uint32_t)it : (uint32_t)it / (uint32_t)parts.n;
+  const uint32_t pair = page / (uint32_t)(n_layers * 2);
+  const int r = (int)(page - pair * (n_layers * 2));
+  return CopyItem{pair, r >> 1, r & 1, (int)((uint32_t)it - page * parts.n) * parts.pieces};
+}
 template <bool WHOLE>
-__device__ inline void copy_rows(const char* from, char* to, int n_heads, int64_t head_b, int row,
-                                 int tid) {
-  const int all = row * n_heads;
+__device__ inline void copy_rows(const char* from, char* to, int64_t head_b, int row, int first,
+                                 int all, int tid) {
   auto off = [&](int i) -> int64_t {
     return WHOLE ? (int64_t)i * 16 : (i / row) * head_b + (int64_t)(i % row) * 16;
   };
   constexpr int U = 4;
-  for (int i = tid; i < all; i += U * 256) {
+  for (int i = first + tid; i < all; i += U * 256) {
     u32x4_t x[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -209,40 +238,46 @@ __device__ inline void copy_rows(const char* from, char* to, int n_heads, int64_
       }
   }
 }
+template <bool WHOLE>
 __device__ inline void copy_tokens(const blt_paged_cache& c, int64_t src, int64_t dst, int fill,
-                                   int layer, int kv, int es, int tid) {
+                                   const CopyItem& x, const Parts& parts, int es, int tid) {
   const int64_t page_b = (int64_t)c.n_kv_heads * c.page_size * c.head_dim * es;
   const int64_t head_b = (int64_t)c.page_size * c.head_dim * es;
-  char* base = reinterpret_cast<char*>(kv ? c.v : c.k) + (int64_t)layer * c.num_pages * page_b;
+  char* base =
+      reinterpret_cast<char*>(x.kv ? c.v : c.k) + (int64_t)x.layer * c.num_pages * page_b;
   const char* from = base + src * page_b;
   char* to = base + dst * page_b;
   const int row = fill * c.head_dim * es / 16;  // 16-byte pieces of a head
-  if (fill == c.page_size) copy_rows<true>(from, to, c.n_kv_heads, head_b, row, tid);
-  else copy_rows<false>(from, to, c.n_kv_heads, head_b, row, tid);
+  const int all = min(row * c.n_kv_heads, x.first + parts.pieces);
+  copy_rows<WHOLE>(from, to, head_b, row, x.first, all, tid);
 }
+template <bool WHOLE>
 __device__ inline void copy_listed(const blt_paged_cache& c, const Lists& l, int es) {
-  const int64_t items = (int64_t)*l.count * c.n_layers * 2;
+  const int64_t pages = (int64_t)*l.count * c.n_layers * 2;
+  const Parts parts = page_parts(c, pages, es);
+  const int64_t items = pages * parts.n;
   for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
-    const int64_t i = it / (c.n_layers * 2);
-    const int r = (int)(it - i * (c.n_layers * 2));
-    copy_tokens(c, l.src[i], l.dst[i], l.fill[i], r >> 1, r & 1, es, threadIdx.x);
+    const CopyItem x = copy_item(it, c.n_layers, parts);
+    copy_tokens<WHOLE>(c, l.src[x.pair], l.dst[x.pair], WHOLE ? c.page_size : l.fill[x.pair], x,
+                       parts, es, threadIdx.x);
   }
 }
 __global__ __launch_bounds__(256) void copy_list_kernel(blt_paged_cache c, Lists l, int es) {
-  copy_listed(c, l, es);
+  copy_listed<false>(c, l, es);
 }
 __global__ __launch_bounds__(256) void copy_pages_kernel(blt_paged_cache c, const int32_t* src,
                                                          const int32_t* dst, int64_t n, int es) {
-  const int64_t items = n * c.n_layers * 2;
+  const Parts parts = page_parts(c, n * c.n_layers * 2, es);
+  const int64_t items = n * c.n_layers * 2 * parts.n;
   for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
-    const int64_t i = it / (c.n_layers * 2);
-    const int r = (int)(it - i * (c.n_layers * 2));
-    const int a = src[i], b = dst[i];
+    const CopyItem x = copy_item(it, c.n_layers, parts);
+    const int a = src[x.pair], b = dst[x.pair];
     if (a < 0 || a >= c.num_pages || b < 0 || b >= c.num_pages) {
-      if (r == 0 && threadIdx.x == 0) atomicOr(c.status, BLT_CACHE_BAD_INDEX);
+      if (threadIdx.x == 0 && x.layer + x.kv + x.first == 0)
+        atomicOr(c.status, BLT_CACHE_BAD_INDEX);
       continue;
     }
-    if (a != b) copy_tokens(c, a, b, c.page_size, r >> 1, r & 1, es, threadIdx.x);
+    if (a != b) copy_tokens<true>(c, a, b, c.page_size, x, parts, es, threadIdx.x);
   }
 }
 
@@ -326,11 +361,13 @@ __global__ __launch_bounds__(NT) void fork_kernel(blt_paged_cache c, int lps, co
       }
       if (page >= 0) c.page_table[(int64_t)dst[i] * cols + col] = page;
     }
-    const int per = c.n_layers * 2;  // four teams of 256 threads
-    for (int64_t it = (int64_t)blockIdx.x * 4 + (tid >> 8); it < (int64_t)need_all * per;
+    const int64_t pages = (int64_t)need_all * c.n_layers * 2;  // four teams of 256 threads
+    const Parts parts = page_parts(c, pages, es);
+    const int64_t items = pages * parts.n;
+    for (int64_t it = (int64_t)blockIdx.x * 4 + (tid >> 8); it < items;
          it += (int64_t)gridDim.x * 4) {
-      const int o = (int)(it / per), r = (int)(it - (int64_t)o * per);
-      copy_tokens(c, olds[o], list[o], fills[o], r >> 1, r & 1, es, tid & 255);
+      const CopyItem x = copy_item(it, c.n_layers, parts);
+      copy_tokens<false>(c, olds[x.pair], list[x.pair], fills[x.pair], x, parts, es, tid & 255);
     }
   }
   __syncthreads();
@@ -474,11 +511,13 @@ __global__ __launch_bounds__(NT) void compact_fit_kernel(blt_paged_cache c, int 
       }
       if (mover[lo] == page) c.page_table[x] = hole[lo];
     }
-    const int per = c.n_layers * 2;  // four teams of 256 threads
-    for (int64_t it = (int64_t)blockIdx.x * 4 + (tid >> 8); it < (int64_t)pairs * per;
+    const int64_t pages = (int64_t)pairs * c.n_layers * 2;  // four teams of 256 threads
+    const Parts parts = page_parts(c, pages, es);
+    const int64_t items = pages * parts.n;
+    for (int64_t it = (int64_t)blockIdx.x * 4 + (tid >> 8); it < items;
          it += (int64_t)gridDim.x * 4) {
-      const int o = (int)(it / per), r = (int)(it - (int64_t)o * per);
-      copy_tokens(c, mover[o], hole[o], c.page_size, r >> 1, r & 1, es, tid & 255);
+      const CopyItem x = copy_item(it, c.n_layers, parts);
+      copy_tokens<true>(c, mover[x.pair], hole[x.pair], c.page_size, x, parts, es, tid & 255);
     }
   }
   __syncthreads();
@@ -506,7 +545,6 @@ __global__ __launch_bounds__(NT) void compact_kernel(blt_paged_cache c, Lists l)
     c.refcount[to] = c.refcount[from];
     c.refcount[from] = 0;
     l.map[from] = to;
-    l.fill[o] = c.page_size;
   }
   if (tid == 0) {
     l.count[0] = pairs;
@@ -524,7 +562,7 @@ __global__ __launch_bounds__(256) void compact_copy_kernel(blt_paged_cache c, in
     const int page = c.page_table[x];
     if (page >= live && page < c.num_pages) c.page_table[x] = l.map[page];
   }
-  copy_listed(c, l, es);
+  copy_listed<true>(c, l, es);
 }
 
 constexpr int kCopyBlocks = 2048;  // eight 256-thread blocks on each of 256 CUs
@@ -546,7 +584,8 @@ int launch_cache_reserve(const blt_paged_cache& c, const int32_t* seqs, const in
 
 inline int elem_size(const blt_paged_cache& c) { return c.dtype == BLT_DTYPE_BF16 ? 2 : 4; }
 inline unsigned copy_blocks(const blt_paged_cache& c, int64_t pairs) {
-  const int64_t items = pairs * c.n_layers * 2;
+  // (at most `pairs`: fewer may be cut into more parts)
+  const int64_t items = pairs * c.n_layers * 2 * page_parts(c, 1, elem_size(c)).n;
   return (unsigned)(items < 1 ? 1 : items < kCopyBlocks ? items : kCopyBlocks);
 }
 

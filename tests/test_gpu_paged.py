@@ -707,6 +707,42 @@ def test_pages_random_walk(dtype, page, d, seed):
     assert seen_full
 
 
+@pytest.mark.parametrize("dtype,page,d,Hkv", [("f32", 512, 64, 2), ("bf16", 256, 128, 3), ("f32", 128, 128, 1)])
+def test_large_pages_are_copied_in_parts(dtype, page, d, Hkv):
+    """Pages of up to 262 KB: a few of them are cut into parts, by a fork (part of a page), a
+    trim, a compaction and copy_pages (whole ones)."""
+    m = Made([0], Hkv=Hkv, d=d, page=page, dtype=TYPES[dtype], layers=2, spare=16, slots=6, columns=6)
+    c = m.cache
+    c.k.copy_(torch.randn(c.k.shape, device=DEV))
+    c.v.copy_(torch.randn(c.v.shape, device=DEV))
+    pool = m.pool()
+
+    def both(what, *lists):
+        getattr(c, what)(*(i32(x) for x in lists))
+        if what == "reserve":
+            pool.reserve(lists[1], np.array(lists[0]))
+        elif what == "fork":
+            pool.fork(*lists)
+        elif what == "trim":
+            pool.trim(lists[1], lists[0])
+        elif what == "free":
+            pool.trim(lists[0], [0] * len(lists[0]))
+        else:
+            pool.compact()
+        c.check()
+        same(c, pool)
+
+    both("reserve", [2 * page + page // 3, page + 1, 40], [0, 1, 2])
+    both("fork", [0, 0, 2], [3, 4, 5])
+    both("trim", [page + page // 2 + 1, 17], [3, 4])
+    both("free", [0, 1])
+    both("compact")
+    k, v = c.k.clone(), c.v.clone()
+    c.copy_pages(i32([0, 1]), i32([15, 13]))
+    k[:, [15, 13]], v[:, [15, 13]] = k[:, [0, 1]], v[:, [0, 1]]
+    assert torch.equal(c.k, k) and torch.equal(c.v, v)
+
+
 @pytest.mark.parametrize("P", [9001, 20003])  # lists in LDS, and in the workspace
 def test_pages_larger_than_one_step_and_many_entries(P):
     """More pages than one block step reads and more entries than threads."""
