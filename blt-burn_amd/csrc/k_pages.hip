@@ -120,10 +120,12 @@ __global__ __launch_bounds__(NT) void reserve_kernel(blt_paged_cache c, int lps,
   __shared__ int bad;
   const int tid = threadIdx.x;
   const Refs refs = load_refs<true>(c.refcount, c.num_pages, tid * PER);
-  if (tid == 0) bad = *c.status & kCachePending ? -1 : 0;
+  // (in a register: `bad` takes the entries' errors as soon as the barrier is passed)
+  const bool pending = *c.status & kCachePending;
+  if (tid == 0) bad = 0;
   for (int i = tid; i < kSeqWords; i += NT) bits[i] = 0;
   __syncthreads();
-  if (bad) return;
+  if (pending) return;
   int need_all = 0;
   for (int i0 = 0; i0 < n; i0 += NT) {
     const int i = i0 + tid;
@@ -300,10 +302,11 @@ __global__ __launch_bounds__(NT) void fork_kernel(blt_paged_cache c, int lps, co
   __shared__ int bad, last;
   const int tid = threadIdx.x, mask = c.page_size - 1;
   const Refs refs = load_refs<true>(c.refcount, c.num_pages, tid * PER);
-  if (tid == 0) bad = *c.status & kCachePending ? -1 : 0;
+  // (in a register, as in reserve_kernel; the status changes behind all blocks' reads)
+  const bool pending = *c.status & kCachePending;
+  if (tid == 0) bad = 0;
   for (int i = tid; i < kSeqWords; i += NT) bits[i] = 0;
   __syncthreads();
-  const bool pending = bad != 0;
   auto page_at = [&](int s, int col) {
     const int page = c.page_table[(int64_t)s * c.max_pages + col];
     return page < 0 ? 0 : page < c.num_pages ? page : c.num_pages - 1;
@@ -347,7 +350,8 @@ __global__ __launch_bounds__(NT) void fork_kernel(blt_paged_cache c, int lps, co
     if (have < need_all && tid == 0) atomicOr(&bad, BLT_CACHE_FULL);
     __syncthreads();
   }
-  if (!bad) {
+  const bool go = !pending && !bad;
+  if (go) {
     const int64_t cols = c.max_pages;
     for (int64_t x = (int64_t)blockIdx.x * NT + tid; x < n * cols; x += (int64_t)gridDim.x * NT) {
       const int i = (int)(x / cols), col = (int)(x - i * cols);
@@ -377,7 +381,7 @@ __global__ __launch_bounds__(NT) void fork_kernel(blt_paged_cache c, int lps, co
   __syncthreads();
   if (!last) return;
   if (tid == 0) __hip_atomic_store(c.sync, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  if (bad) {
+  if (!go) {
     if (tid == 0 && !pending) atomicOr(c.status, bad);
     return;
   }
