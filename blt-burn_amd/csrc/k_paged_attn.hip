@@ -350,7 +350,8 @@ template <int D, int BQ, int NT, typename T>
 __device__ void join_parts(const KArgs& p, const Item& it, int nr, float* room) {
   if (!last_part(p, it)) return;
   // U parts at a time, everything of them in flight at once (a read that passes the L2 takes
-  // about 1 us), with a running max; past the last part: the last one again, without weight
+  // about 1 us), with a running max; past the last part: the last one again, as an empty part (a
+  // weight of zero alone would make its infinite values NaN)
   const int64_t step = (int64_t)it.nrt * BQ;
   auto run = [&](int i, int x0, int x1, auto at_once) {
     constexpr int U = decltype(at_once)::value;
@@ -367,8 +368,13 @@ __device__ void join_parts(const KArgs& p, const Item& it, int nr, float* room) 
         o[u] = get4(p.part + at * D + dd);
       }
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (x + u >= x1) m[u] = -INFINITY;
+      for (int u = 0; u < U; ++u) {
+        const bool mine = x + u < x1;
+        m[u] = mine ? m[u] : -INFINITY;
+        l[u] = mine ? l[u] : 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[u][e] = mine ? o[u][e] : 0.f;
+      }
       float mn = a.m;
 #pragma unroll
       for (int u = 0; u < U; ++u) mn = fmaxf(mn, m[u]);

@@ -40,3 +40,32 @@ def test_a_bad_entry_among_many_is_always_reported(n):
                     c.check()
     assert torch.equal(c.lens, lens) and torch.equal(c.refcount, refs)
     assert torch.equal(c.page_table, table) and int(c._sync.abs().max()) == 0
+
+
+# ---- values that are not finite -------------------------------------------------------
+
+ODD = [float("inf"), -float("inf"), float("nan")]
+
+
+def same_value(got, value):
+    """Every one of `got` is +inf, -inf or NaN, as `value` is."""
+    return bool(np.isnan(got).all() if np.isnan(value) else (got == value).all())
+
+
+@pytest.mark.parametrize("value", ODD)
+@pytest.mark.parametrize("d,H,Hkv", [(64, 2, 2), (128, 4, 1)])
+@pytest.mark.parametrize("L", [64 * k for k in (3, 5, 9, 17, 33, 67, 140)])
+def test_attention_f32_infinite_values_in_the_last_part(L, d, H, Hkv, value):
+    """One token over L keys in parts, with a value that is not finite in the last one's
+    last tile, which the token sees whole: it comes through the join as it is, whatever
+    the number of parts."""
+    m = Made([L], Hkv=Hkv, d=d, dtype=torch.float32)
+    torch.manual_seed(L)
+    q = torch.randn(1, H, d, device=DEV)
+    want = f64(m.cache.attention(0, q, i32([0, 1])))
+    pos = L - 7
+    m.kv[1][0, m.table[0, pos // 16], :, pos % 16, 5] = value
+    got = f64(m.cache.attention(0, q, i32([0, 1])))
+    assert same_value(got[:, :, 5], value)
+    rest = np.arange(d) != 5
+    assert np.array_equal(got[..., rest], want[..., rest])
