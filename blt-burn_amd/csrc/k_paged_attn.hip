@@ -1217,6 +1217,7 @@ __global__ __launch_bounds__(256) void paged_attn_f32_kernel(KArgs p) {
       const int key = 8 * (i >> 2) + (i & 3);
       s[i] = key <= up && key >= dn ? s[i] : -INFINITY;
     }
+    bool odd = false;  // a value that is not finite, where rows see different keys
     if (k0 + BKV - 1 > all_hi || k0 < all_lo) {  // (as in paged_attn_kernel)
       uint32_t seen = 0;  // the largest magnitude, as bits
 #pragma unroll
@@ -1226,18 +1227,8 @@ __global__ __launch_bounds__(256) void paged_attn_f32_kernel(KArgs p) {
 #pragma unroll
           for (int u = 0; u < VW; ++u)
             seen = max(seen, __float_as_uint(vf[n][i][u]) & 0x7fffffffu);
-      if (__any(seen >= 0x7f800000u)) {
-        for (int j = 0; j < BKV; ++j) {
-          const float* vrow = (const float*)p.v + row_at(k0 + j);
-#pragma unroll
-          for (int n = 0; n < ND; ++n)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float v =
-                  vrow[VW * (8 * (i >> 2) + 4 * h + (i & 3)) + n % VW + 32 * VW * (n / VW)];
-              oacc[n][i] += k0 + j <= khi && k0 + j >= klo && !(fabsf(v) < INFINITY) ? v : 0.f;
-            }
-        }
+      odd = __any(seen >= 0x7f800000u);
+      if (odd)
 #pragma unroll
         for (int n = 0; n < NV; ++n)
 #pragma unroll
@@ -1247,7 +1238,6 @@ __global__ __launch_bounds__(256) void paged_attn_f32_kernel(KArgs p) {
               const float v = vf[n][i][u];
               vf[n][i][u] = fabsf(v) < INFINITY ? v : 0.f;
             }
-      }
     }
     float mt = s[0];
 #pragma unroll
@@ -1272,6 +1262,19 @@ __global__ __launch_bounds__(256) void paged_attn_f32_kernel(KArgs p) {
     for (int n = 0; n < ND; ++n)
 #pragma unroll
       for (int i = 0; i < 16; ++i) oacc[n][i] *= alpha;
+    if (odd) {  // (behind the rescaling: the row's first tile has a factor of zero there)
+      for (int j = 0; j < BKV; ++j) {
+        const float* vrow = (const float*)p.v + row_at(k0 + j);
+#pragma unroll
+        for (int n = 0; n < ND; ++n)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float v =
+                vrow[VW * (8 * (i >> 2) + 4 * h + (i & 3)) + n % VW + 32 * VW * (n / VW)];
+            oacc[n][i] += k0 + j <= khi && k0 + j >= klo && !(fabsf(v) < INFINITY) ? v : 0.f;
+          }
+      }
+    }
 #pragma unroll
     for (int i = 0; i < 16; ++i)
 #pragma unroll

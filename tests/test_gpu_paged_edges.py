@@ -69,3 +69,38 @@ def test_attention_f32_infinite_values_in_the_last_part(L, d, H, Hkv, value):
     assert same_value(got[:, :, 5], value)
     rest = np.arange(d) != 5
     assert np.array_equal(got[..., rest], want[..., rest])
+
+
+def check_odd_values(m, q, bad, value, window=0, n=None, rows=None):
+    """A copy of `value` at (position, column) pairs `bad` of sequence 0's values: the rows that
+    see one have it in that column, as it is, and everything else is the rest's attention."""
+    L, d = int(m.lens[0]), q.shape[-1]
+    n = len(q) if n is None else n
+    k, v = m.rows(0, 0), m.rows(1, 0)
+    for pos, col in bad:
+        m.kv[1][0, m.table[0, pos // m.page], :, pos % m.page, col] = value
+        v[pos, :, col] = 0.0
+    o = f64(m.cache.attention(0, q, i32([0, n]), seqs=i32([0]), window=window))
+    at = L - n + np.arange(n)
+    hit = np.zeros((n, 1, d), bool)
+    for pos, col in bad:
+        hit[(pos <= at) & ((pos > at - window) if window else True), 0, col] = True
+    hit = np.broadcast_to(hit, o.shape)
+    assert hit.any() and same_value(o[hit], value)
+    want, A = R.attention(f64(q), k, v, L, True, window)
+    tol = att_tol(A, f64(q), k, m.cache.dtype, d, d ** -0.5)
+    # (a column with the value taken out has no weight of its own there: not compared)
+    assert (np.abs(o - want)[~hit] <= tol[~hit] + 1e-30).all()
+    return o
+
+
+@pytest.mark.parametrize("value", ODD)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("L,n,window", [(1, 1, 0), (5, 5, 0), (31, 31, 0), (31, 1, 0), (200, 150, 0),
+                                        (200, 9, 0), (200, 150, 40), (200, 20, 70)])
+def test_attention_f32_infinite_values_are_seen_as_they_are(L, n, window, d, value):
+    """Also in the first tile that a row sees, where it sees only a part of it."""
+    m = Made([L], Hkv=1, d=d, dtype=torch.float32, seed=L)
+    torch.manual_seed(n)
+    q = torch.randn(n, 2, d, device=DEV)
+    check_odd_values(m, q, {(L - 1, 3), (max(L - n, 0), 20), (L // 2, d - 1)}, value, window)
