@@ -688,9 +688,30 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(KArgs p) {
           for (int r = 0; r < 16; ++r)
             s[sub][r] = sub * 32 + 8 * (r >> 2) + (r & 3) >= rel ? s[sub][r] : -INFINITY;
       }
+      float mt = -INFINITY;
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[sub][r]);
+      {
+        float a, b;
+        swap_pair<32>(mt, a, b);
+        mt = fmaxf(a, b);
+      }
+      // the offset moves only when the max is more than 2^8 over it
+      if (__any(mt > m + grow_at)) {
+        const float m_new = fmaxf(m, mt);
+        const float alpha = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - m_new) * c);
+        m = m_new;
+        l *= alpha;
+#pragma unroll
+        for (int j = 0; j < DS; ++j)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[j][r] *= alpha;
+      }
       // A weight of zero does not silence an infinite or NaN value: where rows see different
       // keys of a tile that holds one, it is taken out of the product and added to the
-      // rows that see it.
+      // rows that see it (behind the rescaling, whose factor may be zero).
       if (mask_hi || mask_lo) {
         uint32_t seen = 0;
 #pragma unroll
@@ -719,27 +740,6 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(KArgs p) {
             }
           }
         }
-      }
-      float mt = -INFINITY;
-#pragma unroll
-      for (int sub = 0; sub < 2; ++sub)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[sub][r]);
-      {
-        float a, b;
-        swap_pair<32>(mt, a, b);
-        mt = fmaxf(a, b);
-      }
-      // the offset moves only when the max is more than 2^8 over it
-      if (__any(mt > m + grow_at)) {
-        const float m_new = fmaxf(m, mt);
-        const float alpha = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - m_new) * c);
-        m = m_new;
-        l *= alpha;
-#pragma unroll
-        for (int j = 0; j < DS; ++j)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) o[j][r] *= alpha;
       }
       const float mc = m == -INFINITY ? 0.f : -m * c;
 #pragma unroll

@@ -104,3 +104,31 @@ def test_attention_f32_infinite_values_are_seen_as_they_are(L, n, window, d, val
     torch.manual_seed(n)
     q = torch.randn(n, 2, d, device=DEV)
     check_odd_values(m, q, {(L - 1, 3), (max(L - n, 0), 20), (L // 2, d - 1)}, value, window)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("value", ODD)
+@pytest.mark.parametrize("d,n,H", [(64, 150, 1), (128, 150, 1)])
+def test_attention_infinite_value_of_a_key_far_above_the_others(d, n, H, value, dtype):
+    """The key's score is 200 above those of the tiles before, whose outputs are rescaled to
+    nothing: its value is not."""
+    L, pos = 200, 195
+    m = Made([L], Hkv=1, d=d, dtype=TYPES[dtype])
+    m.kv[0][0, :, :, :, 0] = 0.0
+    m.kv[0][0, m.table[0, pos // 16], 0, pos % 16, 0] = 25.0 * d ** 0.5
+    torch.manual_seed(n)
+    q = torch.randn(n, H, d, device=DEV).to(TYPES[dtype])
+    q[:, :, 0] = 8.0
+    o = check_odd_values(m, q, {(pos, 3)}, value)
+    assert np.isfinite(o[:n - 5]).all()
+
+
+@pytest.mark.parametrize("value", ODD)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("L,n,window", [(40, 40, 0), (200, 150, 0), (200, 150, 40), (700, 100, 0)])
+def test_attention_bf16_tiles_infinite_values_are_seen_as_they_are(L, n, window, d, value):
+    """(more than 32 rows: the form for tiles of 128 rows)"""
+    m = Made([L], Hkv=1, d=d, seed=L)
+    torch.manual_seed(n)
+    q = torch.randn(n, 2, d, device=DEV).bfloat16()
+    check_odd_values(m, q, {(L - 1, 3), (max(L - n, 0), 20), (L // 2, d - 1)}, value, window)
