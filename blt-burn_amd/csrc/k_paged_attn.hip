@@ -792,13 +792,16 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(KArgs p) {
 // every NW-th 32-key tile of the item through its own LDS ring of two tiles, filled by DMA
 // while the tiles before are consumed, and they meet once at the end.  16 x 16 x 32
 // MFMAs, scores transposed as above (a lane owns a row, the key blocks' registers are the
-// second product's operand).  p goes into that product as two bf16 halves (p rounded, and
-// what the rounding left): the matrix cores have nothing else to do, and the output
-// keeps f32 accuracy up to its own rounding.
+// second product's operand).  p goes into that product as two bf16 halves (p cut off, and
+// what that left, rounded): the matrix cores have nothing else to do, and p is off by 2^-15 at
+// most, against 2^-8 of the output's own rounding.  Cut off and not rounded, and the rest with
+// 2^-22 p on top, so that both halves are above zero: an infinite value times zero or a
+// negative rest would be NaN (below p = 2^-104, where the rest may vanish, it still is).
 // 48 single tokens over up to 8192 keys, 12 heads of 64: 128 us, 5.0 TB/s; 16 over up to 32768
 // keys, 32 / 8 heads of 128: 169 us, 5.5 TB/s (a large copy: 6.15).  One token over 1000 keys,
 // 12 heads: 8.7 us of dependent steps: launch 1.7, find_item 0.5, pages 0.6, tiles 2.1, the
 // waves' merge 1.3, join 2.6; over 8192 keys 15.4 us, over 32768 26.8.
+constexpr float kAbove1 = 1.f + 0x1p-22f;
 template <int N>
 __device__ inline void wait_loads() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
@@ -975,10 +978,10 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(KArgs p) {
         const float p0 = __builtin_amdgcn_exp2f(fmaf(s[n][e >> 2][e & 3], c, mc));
         const float p1 = __builtin_amdgcn_exp2f(fmaf(s[n][e >> 2][(e & 3) + 1], c, mc));
         l[n] += p0 + p1;
-        const uint32_t x = pack_bf16x2(p0, p1);
-        wh[e >> 1] = x;
-        wl[e >> 1] = pack_bf16x2(p0 - __uint_as_float(x << 16),
-                                 p1 - __uint_as_float(x & 0xffff0000u));
+        const uint32_t x0 = __float_as_uint(p0), x1 = __float_as_uint(p1);
+        wh[e >> 1] = __builtin_amdgcn_perm(x1, x0, 0x07060302);  // their upper halves
+        wl[e >> 1] = pack_bf16x2(fmaf(p0, kAbove1, -__uint_as_float(x0 & 0xffff0000u)),
+                                 fmaf(p1, kAbove1, -__uint_as_float(x1 & 0xffff0000u)));
       }
       ph[n] = __builtin_bit_cast(bf16x8_t, u32x4_t{wh[0], wh[1], wh[2], wh[3]});
       pl[n] = __builtin_bit_cast(bf16x8_t, u32x4_t{wl[0], wl[1], wl[2], wl[3]});

@@ -132,3 +132,24 @@ def test_attention_bf16_tiles_infinite_values_are_seen_as_they_are(L, n, window,
     torch.manual_seed(n)
     q = torch.randn(n, 2, d, device=DEV).bfloat16()
     check_odd_values(m, q, {(L - 1, 3), (max(L - n, 0), 20), (L // 2, d - 1)}, value, window)
+
+
+@pytest.mark.parametrize("value", ODD)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("L,n,H,window", [(1, 1, 1, 0), (20, 1, 2, 0), (64, 1, 1, 0), (700, 1, 1, 0), (700, 1, 12, 0),
+                                          (3000, 1, 4, 0), (200, 9, 2, 0), (200, 20, 1, 70), (700, 30, 1, 0)])
+def test_attention_bf16_few_rows_infinite_values_are_seen_as_they_are(L, n, H, window, d, value):
+    """(up to 32 rows: the forms for few rows) in tiles that a row sees whole as well as in others,
+    of either sign of what rounding the weight leaves."""
+    m = Made([L], Hkv=1, d=d, seed=L)
+    torch.manual_seed(n)
+    q = torch.randn(n, H, d, device=DEV).bfloat16()
+    lo = max(L - n - (window or L) + 1, 0)
+    bad = {(L - 1, 3), (max(L - n, 0), 20)} | {(lo + i * 7 % (L - lo), 21 + i) for i in range(16)}
+    check_odd_values(m, q, bad, value, window)
+
+
+@pytest.mark.parametrize("value", ODD)
+@pytest.mark.parametrize("d,H", [(64, 1), (128, 3)])
+def test_attention_few_rows_infinite_value_of_a_key_far_above_the_others(d, H, value):
+    test_attention_infinite_value_of_a_key_far_above_the_others(d, 9, H, value, "bf16")
