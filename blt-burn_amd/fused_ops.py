@@ -194,6 +194,9 @@ class RotaryPlan:
             raise BltError("RotaryPlan: pairs must be 'half' or 'interleaved'")
         if scaling not in _lib.ROTARY_SCALING:
             raise BltError("RotaryPlan: scaling must be one of %s" % sorted(_lib.ROTARY_SCALING))
+        dev = torch.device("cuda" if device is None else device)
+        if dev.type != "cuda":
+            raise BltError("RotaryPlan: the table must live on a GPU (got device %s)" % dev)
         n = int(rotary_dim)
         freq = torch.zeros(max(n // 2, 1), dtype=torch.int64)
         mag = ctypes.c_float()
@@ -201,7 +204,6 @@ class RotaryPlan:
                                                 float(factor), float(original_len),
                                                 freq.data_ptr(), ctypes.addressof(mag)),
               "rotary_frequencies")
-        dev = torch.device("cuda" if device is None else device)
         if dev.index is None:
             dev = torch.device("cuda", torch.cuda.current_device())
         self.rotary_dim, self.magnitude, self.device = n, mag.value, dev
