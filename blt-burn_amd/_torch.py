@@ -19,7 +19,8 @@ def stream_ptr(device=None):
     return torch.cuda.current_stream(device).cuda_stream
 
 
-_current_device = torch._C._cuda_getDevice
+# (the same without a lazy initialisation and a Python frame on every call)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def call_on(device, index, fn, what, *args):

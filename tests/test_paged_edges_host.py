@@ -1,9 +1,12 @@
 """Refusals and host parts of the incremental operators that need no GPU, beside those of
 test_paged_host."""
+import importlib.util
+
 import pytest
+import torch
 
 import blt_burn_amd as pkg
-from blt_burn_amd import fused_ops as F
+from blt_burn_amd import _torch as T, fused_ops as F
 
 
 @pytest.mark.parametrize("device", ["cpu", "cpu:0", "meta"])
@@ -11,3 +14,19 @@ def test_a_rotary_table_outside_the_gpu_is_refused(device):
     """Its index alone would pass for a GPU's, and a kernel would follow a host pointer."""
     with pytest.raises(pkg.BltError, match="GPU"):
         F.RotaryPlan(64, device=device)
+
+
+@pytest.mark.parametrize("missing", [["_cuda_getDevice"], ["_cuda_getCurrentRawStream"],
+                                     ["_cuda_getDevice", "_cuda_getCurrentRawStream"]])
+def test_a_torch_without_its_private_names_will_do(missing, monkeypatch):
+    """The quick handles are private names of torch: without them the public calls serve."""
+    for name in missing:
+        monkeypatch.delattr(torch._C, name, raising=False)
+    spec = importlib.util.spec_from_file_location("blt_burn_amd._torch_again", T.__file__)
+    again = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(again)
+    monkeypatch.setattr(again, "_current_device", lambda: 3)
+    monkeypatch.setattr(again, "_raw_stream", lambda index: 77)
+    got = []
+    again.call_on(torch.device("cuda", 3), 3, lambda *a: got.append(a) or 0, "call", 1, 2)
+    assert got == [(1, 2, 77)]
