@@ -14,7 +14,8 @@ captured into a graph.  A call that the state does not allow (no free page, a
 sequence too long) sets a bit in the cache's status instead of raising; check()
 waits, raises BltError for it and clears it.  Calls on one cache must be
 stream-ordered, attention among them: they share its workspace and counters (two
-graphs that use one cache must not be replayed at once).
+graphs that use one cache must not be replayed at once).  Autograd does not follow
+them: what they return carries no gradient.
 """
 import ctypes
 import functools

@@ -218,16 +218,42 @@ def _dense_rows(t):
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+class _RotaryGradient(torch.autograd.Function):
+    """fused_rotary for inputs that need a gradient: the transposed rotation of the outputs'."""
+
+    @staticmethod
+    def forward(ctx, q, k, positions, plan, backward):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(positions)
+        ctx.plan, ctx.turned = plan, backward
+        return fused_rotary(q, k, positions, plan, backward)
+
+    @staticmethod
+    def backward(ctx, gq, gk):
+        (positions,) = ctx.saved_tensors
+        if gq is None and gk is not None:
+            gk, _ = fused_rotary(gk, None, positions, ctx.plan, not ctx.turned)
+        elif gq is not None:
+            gq, gk = fused_rotary(gq, gk, positions, ctx.plan, not ctx.turned)
+        return gq, gk, None, None, None
+
+
 def fused_rotary(q, k, positions, plan, backward=False, out=None):
     """Rotary positions of q [batch, heads, seq, head_dim] and k (its own number of
     heads; may be None) in one launch: (q', k').  Any strides with a dense last
     dimension are read as they are, e.g. views into a packed QKV tensor.
     positions: int32 [seq] or [batch, seq].  backward=True applies the transposed
-    rotation, which turns gradients of q', k' into those of q, k.  out: (q', k') to
-    write, which may be q and k themselves; other overlaps are not allowed."""
+    rotation, which turns gradients of q', k' into those of q, k; autograd does so by
+    itself for inputs that need a gradient.  out: (q', k') to write, which may be q and k
+    themselves; other overlaps are not allowed, nor are inputs that need a gradient."""
     if not isinstance(plan, RotaryPlan):
         require_cuda(q, positions)
         raise TypeError("fused_rotary expects a RotaryPlan")
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        if out is not None:
+            raise BltError("fused_rotary: out takes no inputs that need a gradient (use "
+                           "torch.no_grad())")
+        return _RotaryGradient.apply(q, k, positions, plan, backward)
     index, dtype = plan._index, q.dtype
     if q.get_device() != index or positions.get_device() != index:
         require_cuda(q, positions)

@@ -7,7 +7,7 @@ import torch
 
 import paged_ref as R
 from blt_burn_amd import BltError, cache as C, fused_ops as F
-from test_gpu_paged import DEV, TYPES, Made, att_tol, check_attention, f64, i32
+from test_gpu_paged import DEV, TYPES, Made, att_tol, check_attention, check_rotary, f64, i32
 
 pytestmark = pytest.mark.gpu
 
@@ -153,3 +153,102 @@ def test_attention_bf16_few_rows_infinite_values_are_seen_as_they_are(L, n, H, w
 @pytest.mark.parametrize("d,H", [(64, 1), (128, 3)])
 def test_attention_few_rows_infinite_value_of_a_key_far_above_the_others(d, H, value):
     test_attention_infinite_value_of_a_key_far_above_the_others(d, 9, H, value, "bf16")
+
+
+# ---- gradients ------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("pairs,d,rot", [("half", 64, 64), ("interleaved", 128, 32), ("half", 10, 4)])
+@pytest.mark.parametrize("back", [False, True])
+def test_rotary_passes_gradients(dtype, pairs, d, rot, back):
+    """Autograd's gradients of q and k are the transposed rotation of the outputs' ones."""
+    torch.manual_seed(rot)
+    kw = dict(scaling="yarn", factor=4.0)
+    plan = F.RotaryPlan(rot, pairs=pairs, **kw)
+    pos = torch.randint(0, 9000, (2, 7), dtype=torch.int32, device=DEV)
+    x = torch.randn(2, 7, 5, d, device=DEV).to(TYPES[dtype]).requires_grad_()
+    q, k = x.transpose(1, 2)[:, :3], x.transpose(1, 2)[:, 3:]
+    qo, ko = F.fused_rotary(q, k, pos, plan, backward=back)
+    with torch.no_grad():
+        plain = F.fused_rotary(q, k, pos, plan, backward=back)
+    assert torch.equal(qo, plain[0]) and torch.equal(ko, plain[1])
+    gq, gk = torch.randn_like(qo), torch.randn_like(ko)
+    (gx,) = torch.autograd.grad([qo, ko], x, [gq, gk], retain_graph=True)
+    at = pos.cpu().numpy()[:, None]
+    check_rotary(gx.transpose(1, 2)[:, :3], gq, at, rot, pairs, not back, **kw)
+    check_rotary(gx.transpose(1, 2)[:, 3:], gk, at, rot, pairs, not back, **kw)
+    # one output alone: the other input's part is zero
+    for out, g, mine in ((qo, gq, slice(0, 3)), (ko, gk, slice(3, 5))):
+        (g1,) = torch.autograd.grad(out, x, g, retain_graph=True)
+        assert torch.equal(g1.transpose(1, 2)[:, mine], gx.transpose(1, 2)[:, mine])
+        assert int((g1 != 0).sum()) <= g1.transpose(1, 2)[:, mine].numel()
+
+
+def test_rotary_gradients_of_shared_and_broadcast_inputs():
+    torch.manual_seed(5)
+    plan = F.RotaryPlan(64)
+    pos = torch.arange(100, 109, dtype=torch.int32, device=DEV)
+    one = torch.randn(1, 1, 9, 64, device=DEV, requires_grad=True)
+    q = one.expand(2, 4, 9, 64)
+    qo, none = F.fused_rotary(q, None, pos, plan)
+    assert none is None
+    qo.sum().backward()  # an expanded gradient
+    want = R.rotate(np.ones((1, 1, 9, 64)), pos.cpu().numpy(), *R.frequencies(64), "half", True) * 8
+    # eight values of at most 2 (6 u + 2e-9) off each, summed in f32
+    assert (np.abs(f64(one.grad) - want) <= 8 * 2 * (6 * 2.0 ** -24 + 2e-9 + 8 * 2.0 ** -24)).all()
+    # only k needs one; the second derivative is the rotation again
+    k = torch.randn(2, 1, 9, 64, device=DEV, requires_grad=True)
+    ko = F.fused_rotary(q.detach(), k, pos, plan)[1]
+    g = torch.randn_like(ko).requires_grad_()
+    (gk,) = torch.autograd.grad(ko, k, g, create_graph=True)
+    e = torch.randn_like(gk)
+    (gg,) = torch.autograd.grad(gk, g, e)
+    assert torch.equal(gg, F.fused_rotary(e, None, pos, plan)[0])
+    # against differences: the rotation is linear
+    e = torch.randn_like(k)
+    y0, y1 = ko.detach(), F.fused_rotary(k.detach() + e, None, pos, plan)[0]
+    lhs, rhs = ((y1 - y0).double() * g.double()).sum(), (e.double() * gk.double()).sum()
+    bound = 32 * 2.0 ** -24 * ((k.abs() + e.abs() + y1.abs()).double() * g.abs().double()).sum()
+    assert abs(lhs - rhs) <= bound
+    for f in (lambda: F.fused_rotary(one, None, pos, plan, out=(one, None)),
+              lambda: F.fused_rotary(q.detach(), k, pos, plan, out=(q.detach().clone(), k))):
+        with pytest.raises(BltError, match="gradient"):
+            f()
+    with torch.no_grad():
+        z = one.detach().clone()
+        F.fused_rotary(one, None, pos, plan, out=(z, None))
+        assert torch.equal(z, F.fused_rotary(one, None, pos, plan)[0])
+
+
+def test_rotary_gradient_in_a_captured_graph():
+    """Forward and gradient captured and replayed with eager work between, against the eager
+    ones; the leaf is used by nothing else while it is captured."""
+    torch.manual_seed(6)
+    plan = F.RotaryPlan(64, pairs="interleaved")
+    pos = torch.arange(9, dtype=torch.int32, device=DEV)
+    x = torch.randn(2, 3, 9, 64, device=DEV, requires_grad=True)
+    g = torch.randn(2, 3, 9, 64, device=DEV)
+
+    def step(x, g):
+        y, _ = F.fused_rotary(x, None, pos, plan)
+        return y, torch.autograd.grad(y, x, g)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step(x, g)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, gx = step(x, g)
+    for i in range(5):
+        with torch.no_grad():
+            x.copy_(torch.randn_like(x))
+        g.copy_(torch.randn_like(g))
+        graph.replay()
+        if i % 2:
+            torch.cuda.synchronize()
+        e = x.detach().clone().requires_grad_()
+        want = step(e, g)
+        assert torch.equal(y, want[0]) and torch.equal(gx, want[1]), i
