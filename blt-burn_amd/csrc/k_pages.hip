@@ -138,7 +138,8 @@ __global__ __launch_bounds__(NT) void reserve_kernel(blt_paged_cache c, int lps,
         const int len = c.lens[s];
         if (named_before(bits, s)) err = BLT_CACHE_BUSY;
         const int64_t want = ((int64_t)len + cnt + (1 << lps) - 1) >> lps;
-        if (want > c.max_pages) err |= BLT_CACHE_TOO_LONG;
+        if (len < 0) err |= BLT_CACHE_BAD_INDEX;  // (a column before the sequence's row)
+        else if (want > c.max_pages) err |= BLT_CACHE_TOO_LONG;
         else need = (int)want - pages_of(len, lps);
         held[i] = pages_of(len, lps);
       }
@@ -324,9 +325,13 @@ __global__ __launch_bounds__(NT) void fork_kernel(blt_paged_cache c, int lps, co
         } else {
           if (named_before(bits, b) || c.lens[b] != 0) err = BLT_CACHE_BUSY;
           const int len = c.lens[a];
-          fill = len & mask;
-          need = fill ? 1 : 0;
-          if (fill && (len >> lps) < c.max_pages) old = page_at(a, len >> lps);
+          if (len < 0 || pages_of(len, lps) > c.max_pages) {
+            err |= BLT_CACHE_BAD_INDEX;
+          } else {
+            fill = len & mask;
+            need = fill ? 1 : 0;
+            if (fill) old = page_at(a, len >> lps);
+          }
         }
       }
       if (err) atomicOr(&bad, err);
@@ -401,7 +406,13 @@ __global__ __launch_bounds__(256) void trim_kernel(blt_paged_cache c, int lps, c
     if (threadIdx.x == 0) atomicOr(c.status, BLT_CACHE_BAD_INDEX);
     return;
   }
-  if (threadIdx.x == 0) old_len = atomicMin(&c.lens[s], want);
+  if (threadIdx.x == 0) {
+    old_len = atomicMin(&c.lens[s], want);
+    if (old_len < 0) {  // no length: none from here on (trim_split_kernel uses the sign)
+      atomicMax(&c.lens[s], 0);
+      atomicOr(c.status, BLT_CACHE_BAD_INDEX);
+    }
+  }
   __syncthreads();
   int hi = pages_of(old_len, lps);
   if (hi > c.max_pages) hi = c.max_pages;

@@ -219,7 +219,9 @@ typedef struct blt_paged_cache {
 typedef enum blt_cache_status {
   BLT_CACHE_FULL = 1,      /* not enough free pages */
   BLT_CACHE_TOO_LONG = 2,  /* a sequence would pass max_pages pages */
-  BLT_CACHE_BAD_INDEX = 4, /* a sequence or page index out of range, a negative count */
+  BLT_CACHE_BAD_INDEX = 4, /* a sequence or page index out of range, a negative count, a length
+                            * in lens that no sequence can have (blt_cache_trim makes a
+                            * negative one 0) */
   BLT_CACHE_BUSY = 8,      /* a sequence twice in one call, or a fork onto one that has tokens */
   BLT_CACHE_NO_PAGE = 16   /* tokens appended where the sequence has no page: left out */
 } blt_cache_status;

@@ -252,3 +252,45 @@ def test_rotary_gradient_in_a_captured_graph():
         e = x.detach().clone().requires_grad_()
         want = step(e, g)
         assert torch.equal(y, want[0]) and torch.equal(gx, want[1]), i
+
+
+# ---- lengths that no sequence can have ---------------------------------------------------
+
+def test_lengths_out_of_range_stay_in_bounds():
+    """A negative length, or one past the table, in the caller's tensors: reserve, fork and trim
+    report it and touch nothing outside the sequences' own rows."""
+    page, S, cols, P = 8, 4, 6, 20
+    kv = [torch.randn(2, P, 1, page, 64, device=DEV).bfloat16() for _ in range(2)]
+    around = torch.full((3, S, cols), -77, dtype=torch.int32, device=DEV)
+    table, lens, refs = around[1], i32([13, 0, 0, 5]), torch.zeros(P, dtype=torch.int32, device=DEV)
+    table[0, :2], table[3, :1] = i32([4, 9]), i32([2])
+    refs[[4, 9, 2]] = 1
+    c = C.PagedCache.wrap(*kv, table, lens, refs)
+    for bad in (-1, -8, -9, -100, -2 ** 31, cols * page + 1, 2 ** 31 - 1):
+        lens[0] = bad
+        keep = [t.clone() for t in (*kv, around, lens, refs)]
+        for call in (lambda: c.reserve(i32([9, 1]), i32([0, 3])), lambda: c.reserve(i32([300]), i32([0])),
+                     lambda: c.fork(i32([0, 3]), i32([1, 2])), lambda: c.fork(i32([3, 0]), i32([1, 2]))):
+            call()
+            with pytest.raises(BltError, match="range|page table"):
+                c.check()
+            assert all(torch.equal(a, b) for a, b in zip(keep, (*kv, around, lens, refs)))
+        if bad < 0:
+            for cut in ([0, 0], [3, 0], [0, 3]):
+                lens[0] = bad
+                c.trim(i32([3, 4]), i32(cut))
+                with pytest.raises(BltError, match="range"):
+                    c.check()
+                assert int(lens[0]) == 0 and lens[1:3].tolist() == [0, 0]
+                assert torch.equal(around[0], keep[2][0]) and torch.equal(around[2], keep[2][2])
+                lens[3] = 5
+            lens[0] = bad
+            c.free(i32([0]))
+            with pytest.raises(BltError, match="range"):
+                c.check()
+            assert int(lens[0]) == 0 and torch.equal(refs, keep[4])
+    # and a sound one again
+    lens[0] = 13
+    c.fork(i32([0]), i32([1]))
+    c.check()
+    assert lens.tolist() == [13, 13, 0, 5] and table[1, :2].tolist() == [4, 0]
