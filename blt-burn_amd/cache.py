@@ -173,6 +173,12 @@ class PagedCache:
             raise BltError("PagedCache: starts has one entry more than there are sequences")
         return p, n - 1, None if seqs is None else self._list(seqs, "seqs", n - 1)[0]
 
+    def _layer(self, layer):
+        # (here too: past 32 bits the call would see its low bits)
+        if not 0 <= layer < self.n_layers:
+            raise BltError("PagedCache: no such layer (%r of %d)" % (layer, self.n_layers))
+        return layer
+
     def _tokens(self, t, what, heads=None):
         """t [tokens, heads, head_dim] with a dense last dimension: itself or a copy, its
         pointer, tokens, heads and strides."""
@@ -208,6 +214,7 @@ class PagedCache:
         (reserve).  rotary: a RotaryPlan that rotates k at its positions, and q [total, heads,
         head_dim] if given, which is returned (into `out`, which may be q; tokens at
         starts[-1] and behind are not written).  starts ascends from 0 on."""
+        layer = self._layer(layer)
         k, kp, total, _, ks, kh = self._tokens(k, "k", self.n_kv_heads)
         v, vp, n, _, vs, vh = self._tokens(v, "v", self.n_kv_heads)
         p, B, s = self._rows(starts, seqs)
@@ -243,6 +250,7 @@ class PagedCache:
         given): 0 where a token sees no key; tokens at starts[-1] and behind are not
         written, nor are those of a row without a sequence, nor any where starts does not
         ascend within q (both set the status)."""
+        layer = self._layer(layer)
         q, qp, total, H, qs, qh = self._tokens(q, "q")
         p, B, s = self._rows(starts, seqs)
         if H % self.n_kv_heads or H == 0:
@@ -253,6 +261,8 @@ class PagedCache:
             qs, qh, _ = q.stride()
             qp = q.data_ptr()
         out, op, os_, oh = self._output(out, q, total, H)
+        if window < 0:
+            raise BltError("PagedCache.attention: window must be >= 0")
         if window > 0x7fffffff:  # longer than any sequence
             window = 0
         self._call(self._lib.blt_paged_attention, "paged_attention", self._ptr, layer, qp, qs, qh, op,

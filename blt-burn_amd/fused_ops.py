@@ -198,6 +198,8 @@ class RotaryPlan:
         if dev.type != "cuda":
             raise BltError("RotaryPlan: the table must live on a GPU (got device %s)" % dev)
         n = int(rotary_dim)
+        if not 2 <= n <= 512:  # (here too: past 32 bits the call would see its low bits)
+            raise BltError("RotaryPlan: rotary_dim must be even, 2 .. 512")
         freq = torch.zeros(max(n // 2, 1), dtype=torch.int64)
         mag = ctypes.c_float()
         check(_lib.lib().blt_rotary_frequencies(n, float(theta), _lib.ROTARY_SCALING[scaling],

@@ -294,3 +294,19 @@ def test_lengths_out_of_range_stay_in_bounds():
     c.fork(i32([0]), i32([1]))
     c.check()
     assert lens.tolist() == [13, 13, 0, 5] and table[1, :2].tolist() == [4, 0]
+
+
+def test_arguments_past_32_bits_are_not_cut():
+    m = Made([20, 9], Hkv=2, d=64, layers=2)
+    c = m.cache
+    q = torch.zeros(3, 4, 64, device=DEV, dtype=torch.bfloat16)
+    k, v = c.k.clone(), c.v.clone()
+    for layer in (-1, 2, 1 << 32, (1 << 32) + 1, -(1 << 32), 1 << 70):
+        with pytest.raises(BltError, match="layer"):
+            c.attention(layer, q, i32([0, 3]))
+        with pytest.raises(BltError, match="layer"):
+            c.append(layer, q[:, :2], q[:, :2], i32([0, 3]))
+    for window in (-1, -(1 << 32), 5 - (1 << 32), -(1 << 70)):
+        with pytest.raises(BltError, match="window"):
+            c.attention(0, q, i32([0, 3]), window=window)
+    assert torch.equal(c.k.nan_to_num(), k.nan_to_num()) and torch.equal(c.v.nan_to_num(), v.nan_to_num())

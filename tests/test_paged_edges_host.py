@@ -16,6 +16,12 @@ def test_a_rotary_table_outside_the_gpu_is_refused(device):
         F.RotaryPlan(64, device=device)
 
 
+@pytest.mark.parametrize("rot", [0, 1, 63, 514, -64, (1 << 32) + 64, -(1 << 32) + 64])
+def test_rotary_dimensions_out_of_range_are_refused(rot):
+    with pytest.raises(pkg.BltError, match="rotary_dim"):
+        F.RotaryPlan(rot)
+
+
 @pytest.mark.parametrize("missing", [["_cuda_getDevice"], ["_cuda_getCurrentRawStream"],
                                      ["_cuda_getDevice", "_cuda_getCurrentRawStream"]])
 def test_a_torch_without_its_private_names_will_do(missing, monkeypatch):
