@@ -41,7 +41,11 @@ class PagedCache:
     """k, v [n_layers, num_pages, n_kv_heads, page_size, head_dim] (f32 or bf16) with
     page_table [max_seqs, max_pages], lens [max_seqs] and refcount [num_pages], all
     int32 tensors of the cache's device that may be read at any time (stream-ordered).
-    head_dim 64 or 128, page_size a power of two from 8 to 1024."""
+    head_dim 64 or 128, page_size a power of two from 8 to 1024.
+
+    Beside them a cache keeps the workspace of its attention calls, as large as the calls
+    so far have needed: some MB for single tokens, at most 104 MB (head_dim 64) or 136 MB
+    (128).  The first call of a size may allocate."""
 
     def __init__(self, n_layers, n_kv_heads, head_dim, num_pages, max_seqs, max_len, page_size=16,
                  dtype=torch.bfloat16, device=None):
@@ -96,11 +100,26 @@ class PagedCache:
         self._piece, self._scale = 16 // k.element_size(), self.head_dim ** -0.5
         # the library's own checks, once: an empty list does nothing else
         self._call(self._lib.blt_cache_reserve, "PagedCache", self._ptr, None, None, 0)
-        # parts of attention calls, for the largest call of whichever form needs most
-        self._ws_bytes = max(self._lib.blt_paged_attention_workspace_bytes(
+        # attention's workspace (parts of its work, see _room): none yet
+        self._ws, self._wsp, self._ws_bytes, self._ws_for = [], None, 0, None
+        self._ws_most = max(self._lib.blt_paged_attention_workspace_bytes(
             self._ptr, 65536, 65536 * rows, self.n_kv_heads) for rows in (1, 32, 128))
-        self._ws = self._workspace(max(self._ws_bytes, 16))
-        self._wsp = self._ws.data_ptr()
+
+    def _room(self, rows, total, heads):
+        """Workspace for attention calls of this size.  It grows by steps of four or more and
+        never past the largest call's; what it was before stays, for the graphs that use it."""
+        need = self._lib.blt_paged_attention_workspace_bytes(self._ptr, rows, total, heads)
+        if need > self._ws_bytes:
+            size = max(need, min(4 * self._ws_bytes, self._ws_most))
+            self._ws.append(self._workspace(size))
+            self._wsp, self._ws_bytes = self._ws[-1].data_ptr(), size
+        self._ws_for = (rows, total, heads)
+
+    def record_stream(self, stream):
+        """Tensor.record_stream for everything the cache holds: for a cache that is dropped
+        while another stream than the one it was made on still uses it."""
+        for t in [self.k, self.v, self.page_table, self.lens, self.refcount, self._status] + self._ws:
+            t.record_stream(stream)
 
     # ---- status ---------------------------------------------------------------
     def check(self):
@@ -261,6 +280,8 @@ class PagedCache:
             qs, qh, _ = q.stride()
             qp = q.data_ptr()
         out, op, os_, oh = self._output(out, q, total, H)
+        if self._ws_for != (B, total, H):
+            self._room(B, total, H)
         if window < 0:
             raise BltError("PagedCache.attention: window must be >= 0")
         if window > 0x7fffffff:  # longer than any sequence

@@ -310,3 +310,78 @@ def test_arguments_past_32_bits_are_not_cut():
         with pytest.raises(BltError, match="window"):
             c.attention(0, q, i32([0, 3]), window=window)
     assert torch.equal(c.k.nan_to_num(), k.nan_to_num()) and torch.equal(c.v.nan_to_num(), v.nan_to_num())
+
+
+# ---- the workspace ---------------------------------------------------------------------
+
+def test_attention_workspace_grows_with_the_calls():
+    """A cache takes no more memory than its calls need; larger and smaller ones in any order
+    give what a fresh cache gives."""
+    base = torch.cuda.memory_allocated()
+    m = Made([3000, 900], Hkv=12, d=64)
+    size = sum(t.numel() * t.element_size() for t in m.kv)
+    assert torch.cuda.memory_allocated() - base < size + (4 << 20)
+    torch.manual_seed(1)
+    q = torch.randn(1000, 12, 64, device=DEV).bfloat16()
+
+    def call(cache, n):
+        return cache.attention(0, q[:sum(n)], i32(np.concatenate([[0], np.cumsum(n)])))
+
+    one = call(m.cache, [1, 1])
+    assert torch.cuda.memory_allocated() - base < size + (24 << 20)
+    for n in ([500, 500], [1, 1], [900, 100], [3, 2], [0, 1], [1, 1]):
+        fresh = C.PagedCache.wrap(*m.kv, m.cache.page_table, m.cache.lens, m.cache.refcount)
+        assert torch.equal(call(m.cache, n), call(fresh, n)), n
+    assert torch.equal(call(m.cache, [1, 1]), one)
+    assert torch.cuda.memory_allocated() - base < size + (160 << 20)
+
+
+def test_a_captured_call_keeps_its_workspace():
+    """A graph captured while the workspace was small is right after it has grown, with eager
+    calls of the larger size between its replays."""
+    m = Made([5000, 4000], Hkv=4, d=64)
+    q = torch.randn(2, 4, 64, device=DEV).bfloat16()
+    many = torch.randn(1500, 4, 64, device=DEV).bfloat16()
+    one, lots = i32([0, 1, 2]), i32([0, 1000, 1500])
+    m.cache.attention(0, q, one)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = m.cache.attention(0, q, one)
+    for i in range(6):
+        q.copy_(torch.randn_like(q))
+        want_many = m.cache.attention(0, many, lots)
+        graph.replay()
+        if i % 2:
+            torch.cuda.synchronize()
+        assert torch.equal(m.cache.attention(0, many, lots), want_many)
+        assert torch.equal(out, m.cache.attention(0, q, one)), i
+    # and one captured before any call
+    m2 = Made([700], Hkv=4, d=64)
+    qs, s1 = q[:1], i32([0, 1])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = m2.cache.attention(0, qs, s1)
+    for i in range(4):
+        q.copy_(torch.randn_like(q))
+        graph.replay()
+        assert torch.equal(out, m2.cache.attention(0, qs, s1)), i
+
+
+def test_a_cache_dropped_while_another_stream_uses_it():
+    """record_stream: the memory is not handed out again before that stream is done."""
+    m = Made([4000] * 8, Hkv=8, d=64)
+    side = torch.cuda.Stream()
+    q, starts = torch.randn(8, 8, 64, device=DEV).bfloat16(), i32(np.arange(9))
+    want = m.cache.attention(0, q, starts)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            out = m.cache.attention(0, q, starts)
+    for t in (q, starts):
+        t.record_stream(side)
+    m.cache.record_stream(side)
+    sizes = [(t.shape, t.dtype) for t in m.kv] + [(t.shape, t.dtype) for t in m.cache._ws]
+    del m
+    fill = [torch.full(s, 7, dtype=d, device=DEV) for s, d in sizes]
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(out, want) and all(bool((f == 7).all()) for f in fill)
