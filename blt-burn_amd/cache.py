@@ -44,8 +44,8 @@ class PagedCache:
     head_dim 64 or 128, page_size a power of two from 8 to 1024.
 
     Beside them a cache keeps the workspace of its attention calls, as large as the calls
-    so far have needed: some MB for single tokens, at most 104 MB (head_dim 64) or 136 MB
-    (128).  The first call of a size may allocate."""
+    so far have needed: at most 35 MB for single tokens, 104 MB (head_dim 64) or 136 MB (128)
+    for any call.  The first call of a size may allocate."""
 
     def __init__(self, n_layers, n_kv_heads, head_dim, num_pages, max_seqs, max_len, page_size=16,
                  dtype=torch.bfloat16, device=None):
