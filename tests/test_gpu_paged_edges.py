@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import paged_ref as R
-from blt_burn_amd import BltError, cache as C, fused_ops as F
+from blt_burn_amd import BltError, cache as C, fused_ops as F, model as M, synth
 from test_gpu_paged import DEV, TYPES, Made, att_tol, check_attention, check_rotary, f64, i32
 
 pytestmark = pytest.mark.gpu
@@ -385,3 +385,69 @@ def test_a_cache_dropped_while_another_stream_uses_it():
     fill = [torch.full(s, 7, dtype=d, device=DEV) for s, d in sizes]
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(out, want) and all(bool((f == 7).all()) for f in fill)
+
+
+# ---- the entropy model, byte by byte -----------------------------------------------------
+
+@pytest.mark.parametrize("dtype,times", [("f32", 1), ("bf16", 2)])
+@pytest.mark.parametrize("window,T", [(0, 150), (100, 300)])
+def test_the_entropy_model_through_the_cache(window, T, dtype, times):
+    """All 14 layers of the entropy model at its sizes over a document that arrives in chunks and
+    single bytes, with a continuation forked on the way, against the model's whole-row forward.
+
+    Tolerances: the forward is held to 2e-2 (entropies) and 1e-2 of the largest value
+    (embeddings, logits) of an f32 computation, for its bf16 operands.  Through an f32 cache
+    everything here is f32: the same bounds.  Through a bf16 one q, k, v and the attention's
+    weights and outputs are rounded as the forward rounds them, and nothing else: twice them."""
+    cfg = M.entropy_model_config()
+    w = M.random_weights(cfg, 4, hidden=2048)
+    text = synth.tokens(synth.config_seed(4) + 9, (2, T))
+    fork_at = T // 2
+    text[1, :fork_at] = text[0, :fork_at]
+    tok = torch.from_numpy(text).to(DEV)
+    whole = M.LMTransformer(cfg, w, device=0, max_tokens=2 * T, window=window)
+    want = whole.forward_with_embeddings(tok)
+    f = {n: torch.from_numpy(synth.bf16_to_f32(x)).to(DEV) for n, x in w.items()}
+    H, d, t = cfg.resolved_n_heads(), cfg.resolved_head_dim(), TYPES[dtype]
+    c = C.PagedCache(cfg.n_layers, H, d, num_pages=64, max_seqs=4, max_len=T, dtype=t)
+    plan = F.RotaryPlan(d, theta=cfg.rope_theta)
+
+    def norm(x, weight):
+        return F.fused_rms_norm(x[None], weight, cfg.norm_eps)[0]
+
+    def step(rows, seqs, a, b):
+        n, s = b - a, i32(seqs)
+        starts = i32(np.arange(len(seqs) + 1) * n)
+        c.reserve(i32([n] * len(seqs)), s)
+        x = f["tok_embeddings"][tok[rows, a:b].reshape(-1).long()]
+        for i in range(cfg.n_layers):
+            h = norm(x, f["attention_norm"][i])
+            q, k, v = ((h @ f[p][i]).view(-1, H, d).to(t) for p in ("wq", "wk", "wv"))
+            q = c.append(i, k, v, starts, seqs=s, rotary=plan, q=q)
+            o = c.attention(i, q, starts, seqs=s, window=window)
+            x = x + o.float().view(-1, H * d) @ f["wo"][i]
+            h = norm(x, f["ffn_norm"][i])
+            x = x + F.fused_silu_gate((h @ f["w1"][i])[None], (h @ f["w3"][i])[None])[0] @ f["w2"][i]
+        logits = norm(x, f["norm"]) @ f["output"]
+        entropy = F.fused_entropy(logits[None], cfg.vocab_size)[0]
+        return [y.view(len(rows), n, -1) for y in (x, logits, entropy)]
+
+    parts = [[], []]
+    for a, b in ((0, 1), (1, fork_at - 1), (fork_at - 1, fork_at)):
+        y = step([0], [2], a, b)
+        for row in parts:
+            row.append([z[0] for z in y])
+    c.fork(i32([2]), i32([0]))
+    for a, b in ((fork_at, fork_at + 1), (fork_at + 1, T - 2), (T - 2, T - 1), (T - 1, T)):
+        y = step([0, 1], [2, 0], a, b)
+        for r in range(2):
+            parts[r].append([z[r] for z in y])
+    c.check()
+    x, logits, entropy = (torch.stack([torch.cat([p[j] for p in row]) for row in parts]) for j in range(3))
+
+    def off(got, ref):
+        return float((got - ref).abs().max() / ref.abs().max())
+
+    assert off(x, want.pre_norm_embeddings) < times * 1e-2
+    assert off(logits, want.logits) < times * 1e-2
+    assert float((entropy[..., 0] - want.entropies).abs().max()) < times * 2e-2
