@@ -451,3 +451,88 @@ def test_the_entropy_model_through_the_cache(window, T, dtype, times):
     assert off(x, want.pre_norm_embeddings) < times * 1e-2
     assert off(logits, want.logits) < times * 1e-2
     assert float((entropy[..., 0] - want.entropies).abs().max()) < times * 2e-2
+
+
+# ---- accuracy of the forms for few rows ----------------------------------------------------
+
+def few_tol(want, A, q, keys, d, scale):
+    """Up to 32 rows a key head: the weights are two bf16 halves (2^-15 + 2^-22 of each), scores,
+    sums and joins f32 as in the f32 forms, and the output is rounded once (2^-8)."""
+    return (A * (2.0 ** -15 + 2.0 ** -22) + att_tol(A, q, keys, torch.float32, d, scale)) * 1.01 \
+        + 2.0 ** -8 * np.abs(want)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("n,H,Hkv", [(1, 1, 1), (1, 12, 12), (1, 8, 2), (9, 2, 2), (4, 8, 1), (32, 1, 1)])
+@pytest.mark.parametrize("window,causal", [(0, True), (100, True), (0, False)])
+def test_attention_few_rows_is_rounded_once(d, n, H, Hkv, window, causal):
+    lens = [32, 33, 64, 700, 3000, 6000]
+    m = Made(lens, Hkv=Hkv, d=d, seed=n)
+    torch.manual_seed(n + H)
+    total = n * len(lens)
+    q = torch.randn(total, H, d, device=DEV).bfloat16()
+    starts = i32(np.arange(len(lens) + 1) * n)
+    o = f64(m.cache.attention(0, q, starts, window=window, causal=causal))
+    x = f64(q)
+    for s, L in enumerate(lens):
+        keys, vals, rows = m.rows(0, s), m.rows(1, s), slice(s * n, s * n + n)
+        want, A = R.attention(x[rows], keys, vals, L, causal, window)
+        err, tol = np.abs(o[rows] - want), few_tol(want, A, x[rows], keys, d, d ** -0.5)
+        assert (err <= tol).all(), (L, (err / tol).max())
+
+
+# ---- many rows ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("B,H,Hkv", [(64, 4, 2), (65, 4, 2), (257, 4, 2), (1000, 2, 1), (4096, 4, 2)])
+def test_many_rows(dtype, B, H, Hkv):
+    """Rows beyond a wave's lanes, in any order of sequences, some without tokens: what append
+    writes, in one call and in calls of 50 rows, and attention of them all."""
+    rng = np.random.default_rng(B)
+    d, page, t = 64, 8, TYPES[dtype]
+    lens = rng.integers(1, 49, B)
+    n = np.minimum(rng.integers(0, 4, B), lens)
+    order = rng.permutation(B)
+    m = Made(lens.tolist(), Hkv=Hkv, d=d, page=page, dtype=t, seed=B)
+    c = m.cache
+    starts = np.concatenate([[0], np.cumsum(n[order])])
+    total = int(starts[-1])
+    torch.manual_seed(B)
+    x = torch.randn(total + 2, H + 2 * Hkv, d, device=DEV).to(t)
+    q, k, v = x[:, :H], x[:, H:H + Hkv], x[:, H + Hkv:]
+    plan = F.RotaryPlan(32, pairs="interleaved")
+    again = C.PagedCache.wrap(c.k.clone(), c.v.clone(), c.page_table, c.lens, c.refcount)
+    qo = c.append(0, k, v, i32(starts), seqs=i32(order), rotary=plan, q=q, out=torch.full_like(q, 5.0))
+    assert bool((qo[total:] == 5.0).all())
+    for a in range(0, B, 50):
+        b, at = min(a + 50, B), slice(int(starts[a]), int(starts[min(a + 50, B)]))
+        qs = again.append(0, k[at], v[at], i32(starts[a:b + 1] - starts[a]), seqs=i32(order[a:b]),
+                          rotary=plan, q=q[at])
+        assert torch.equal(qs, qo[at])
+    assert torch.equal(c.k.nan_to_num(), again.k.nan_to_num())
+    assert torch.equal(c.v.nan_to_num(), again.v.nan_to_num())
+    out = torch.full_like(qo, 7.0)
+    c.attention(0, qo, i32(starts), seqs=i32(order), out=out)
+    c.check()
+    assert bool((out[total:] == 7.0).all()) and int(c._sync.abs().max()) == 0
+    # 64-bit reference: every sequence's keys side by side
+    row = torch.tensor(np.repeat(order, n[order]), device=DEV)
+    length = torch.tensor(lens, device=DEV)
+    pos = length[row] - torch.tensor(np.concatenate([np.arange(z, 0, -1) for z in n[order]] or [[]]),
+                                     device=DEV)
+    pages = c.page_table.clamp(min=0).long()
+    keys, vals = (y[0][pages].transpose(2, 3).reshape(B, -1, Hkv, d).nan_to_num().double()
+                  for y in (c.k, c.v))
+    see = torch.arange(keys.shape[1], device=DEV)[None] <= pos[:, None]
+    for h in range(H):
+        g = h * Hkv // H
+        s = (keys[row, :, g] * qo[:total, None, h].double()).sum(-1) * d ** -0.5
+        p = torch.softmax(s.masked_fill(~see, -float("inf")), -1)[..., None]
+        want, A = (p * vals[row, :, g]).sum(1), (p * vals[row, :, g].abs()).sum(1)
+        smax = float(qo.double().abs().sum(-1).max() * keys.abs().max()) * d ** -0.5
+        u = 2.0 ** -24
+        tol = u * (2 * (d + 4) * smax + 16 * (1 + smax) + keys.shape[1] + 16) * A
+        if dtype == "bf16":  # (1.5 tokens a sequence: a form for few rows)
+            tol = (tol + A * (2.0 ** -15 + 2.0 ** -22)) * 1.01 + 2.0 ** -8 * want.abs()
+        err = (out[:total, h].double() - want).abs()
+        assert bool((err <= tol).all()), float((err / tol).max())
