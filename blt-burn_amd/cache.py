@@ -219,7 +219,10 @@ class PagedCache:
         """(out, or a new tensor like `like`; its pointer and strides)"""
         if out is None:
             out = torch.empty_like(like)
-            st, sh, _ = out.stride()
+            st, sh, sd = out.stride()
+            if sd != 1:  # (of overlapping rows)
+                out = torch.empty_like(like, memory_format=torch.contiguous_format)
+                st, sh, sd = out.stride()
             return out, out.data_ptr(), st, sh
         t, p, n, _, st, sh = self._tokens(out, "out", heads)
         if t is not out or n != total:

@@ -220,6 +220,13 @@ def _dense_rows(t):
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+def _output_like(t):
+    """A new tensor of t's order of dimensions whose last one is dense (that of overlapping
+    rows need not be, in empty_like)."""
+    y = torch.empty_like(t)
+    return y if y.stride(-1) == 1 else torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 class _RotaryGradient(torch.autograd.Function):
     """fused_rotary for inputs that need a gradient: the transposed rotation of the outputs'."""
 
@@ -281,8 +288,8 @@ def fused_rotary(q, k, positions, plan, backward=False, out=None):
         y = _dense_rows(k)
         yp, ys = y.data_ptr(), y.stride()
     if out is None:
-        qo = torch.empty_like(x)
-        ko = torch.empty_like(y) if y is not None else None
+        qo = _output_like(x)
+        ko = _output_like(y) if y is not None else None
     else:
         qo, ko = out
         if (ko is None) != (k is None):

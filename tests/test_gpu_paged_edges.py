@@ -536,3 +536,27 @@ def test_many_rows(dtype, B, H, Hkv):
             tol = (tol + A * (2.0 ** -15 + 2.0 ** -22)) * 1.01 + 2.0 ** -8 * want.abs()
         err = (out[:total, h].double() - want).abs()
         assert bool((err <= tol).all()), float((err / tol).max())
+
+
+# ---- layouts -----------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_overlapping_rows_are_read_as_they_are(dtype):
+    """Rows that overlap (windows of a signal): the new outputs are dense along a head all the
+    same, where empty_like lays them out otherwise."""
+    torch.manual_seed(2)
+    t, T, H, d = TYPES[dtype], 9, 4, 64
+    signal = torch.randn(4000, device=DEV).to(t)
+    plan, pos = F.RotaryPlan(d), torch.arange(T, dtype=torch.int32, device=DEV)
+    m = Made([T], Hkv=H, d=d, dtype=t)
+    kv = torch.randn(T, 2, H, d, device=DEV).to(t)
+    for st, sh in ((1, 1), (1, d), (8, 1), (64, 32), (0, 0), (0, 64), (1, 0), (24, 8)):
+        x = signal.as_strided((T, H, d), (st, sh, 1))
+        q = x.transpose(0, 1)[None]
+        want, _ = F.fused_rotary(q.contiguous(), None, pos, plan)
+        got, k = F.fused_rotary(q, q, pos, plan)
+        assert torch.equal(got, want) and torch.equal(k, want), (st, sh)
+        got = m.cache.append(0, kv[:, 0], kv[:, 1], i32([0, T]), rotary=plan, q=x)
+        assert torch.equal(got, want[0].transpose(0, 1)), (st, sh)
+        assert torch.equal(m.cache.attention(0, x, i32([0, T])),
+                           m.cache.attention(0, x.contiguous(), i32([0, T]))), (st, sh)
