@@ -255,6 +255,9 @@ def fused_rotary(q, k, positions, plan, backward=False, out=None):
     rotation, which turns gradients of q', k' into those of q, k; autograd does so by
     itself for inputs that need a gradient.  out: (q', k') to write, which may be q and k
     themselves; other overlaps are not allowed, nor are inputs that need a gradient."""
+    for t in (q, positions) if k is None else (q, k, positions):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError("expected a torch.Tensor, got %r" % type(t))
     if not isinstance(plan, RotaryPlan):
         require_cuda(q, positions)
         raise TypeError("fused_rotary expects a RotaryPlan")

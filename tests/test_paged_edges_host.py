@@ -22,6 +22,17 @@ def test_rotary_dimensions_out_of_range_are_refused(rot):
         F.RotaryPlan(rot)
 
 
+def test_rotary_of_something_else_than_tensors_is_a_type_error():
+    x, pos = torch.zeros(1, 1, 1, 64), torch.zeros(1, dtype=torch.int32)
+    plan = object.__new__(F.RotaryPlan)  # (no table: nothing of it is looked at)
+    plan._index = 0
+    for q, k, p in (([1.0], None, pos), (x, [1.0], pos), (x, None, [0]), (None, x, pos), (x, x, None)):
+        with pytest.raises(TypeError, match="torch.Tensor"):
+            F.fused_rotary(q, k, p, plan)
+    with pytest.raises(pkg.BltError, match="GPU"):
+        F.fused_rotary(x, x, pos, plan)
+
+
 @pytest.mark.parametrize("missing", [["_cuda_getDevice"], ["_cuda_getCurrentRawStream"],
                                      ["_cuda_getDevice", "_cuda_getCurrentRawStream"]])
 def test_a_torch_without_its_private_names_will_do(missing, monkeypatch):
