@@ -269,9 +269,16 @@ class PagedCache:
         reads key head h // (heads / kv_heads).  causal: keys up to the token's own
         position, with window > 0 only the last `window` of them; causal=False: every
         key.  scale defaults to head_dim^-0.5.  Returns [total, heads, head_dim] (`out` if
-        given): 0 where a token sees no key; tokens at starts[-1] and behind are not
-        written, nor are those of a row without a sequence, nor any where starts does not
-        ascend within q (both set the status)."""
+        given, whose rows are 16-byte aligned): 0 where a token sees no key; tokens at
+        starts[-1] and behind are not written, nor are those of a row without a sequence,
+        nor any where starts does not ascend within q (both set the status).
+
+        A key whose score is -inf weighs nothing.  Scores, sums and f32 outputs are f32
+        throughout; in bf16 the softmax's weights are rounded to bf16 where the rows have more
+        than 32 tokens on average (heads per key head counted as tokens), and to 2^-15 of
+        them below.  That average also chooses the kernel, so a long chunk is best issued
+        apart from many single tokens; and calls of more than some hundred rows are best cut
+        into several (a call's cost has a part that grows with the square of its rows)."""
         layer = self._layer(layer)
         q, qp, total, H, qs, qh = self._tokens(q, "q")
         p, B, s = self._rows(starts, seqs)

@@ -102,7 +102,10 @@ __device__ inline float uniform(float v) {
   return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
 }
 
-// The item of block `bid`, false if it has none.  Every wave computes it by itself, in
+// The item of block `bid`, false if it has none.  (Up to 64 rows a lane holds each; beyond that
+// every wave walks all rows three times or more, so that a call grows with the square of its
+// rows: single tokens over up to 200 keys, 12 heads, 64 of them 10 us, 256 50, 1024 406,
+// 4096 5200.)  Every wave computes it by itself, in
 // the same order, so all agree.
 template <int BQ, int BKV>
 __device__ bool find_item(const KArgs& p, unsigned bid, Item& it) {
@@ -806,7 +809,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(KArgs p) {
 // negative rest would be NaN (below p = 2^-104, where the rest may vanish, it still is).
 // 48 single tokens over up to 8192 keys, 12 heads of 64: 128 us, 5.0 TB/s; 16 over up to 32768
 // keys, 32 / 8 heads of 128: 169 us, 5.5 TB/s (a large copy: 6.15).  One token over 1000 keys,
-// 12 heads: 8.7 us of dependent steps: launch 1.7, find_item 0.5, pages 0.6, tiles 2.1, the
+// 12 heads: 8.8 us of dependent steps: launch 1.7, find_item 0.5, pages 0.6, tiles 2.1, the
 // waves' merge 1.3, join 2.6; over 8192 keys 15.4 us, over 32768 26.8.
 constexpr float kAbove1 = 1.f + 0x1p-22f;
 template <int N>
@@ -1128,8 +1131,8 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(KArgs p) {
 // As attn_f32_kernel (k_attn.hip): both products on the f32 matrix cores, one block = 32
 // rows, its four waves take every fourth 32-key tile with operands straight from global
 // memory, and meet once at the end.  Chunks of 100, 97 and 87 tokens over 1500, 350 and 87 keys,
-// 12 heads: 22.3 us; two tiles a wave, each 64 MFMAs of 64 cycles behind its loads, then the
-// merge and the join.
+// 12 heads: 22.5 us; two tiles a wave, each 64 MFMAs of 64 cycles behind its loads, then the
+// merge and the join.  A single token fills a whole tile of 32 rows: one over 8192 keys 22.4 us.
 template <int ND>
 __global__ __launch_bounds__(256) void paged_attn_f32_kernel(KArgs p) {
   constexpr int D = 32 * ND, NW = 4, NC = 4 * ND, OP = D + 4, BQ = 32, BKV = 32;
@@ -1371,6 +1374,8 @@ __global__ __launch_bounds__(256) void paged_attn_f32_kernel(KArgs p) {
 // keys in two, window 300, 125 (182), 4 of up to 1024 265 (316).  With few row tiles their keys
 // take too long one after the other (7 chunks of up to 566, 4 / 2 heads, 61 and 53), and with
 // d = 64 the form above has two blocks a CU itself (10 of up to 400, 12 heads, 58 and 39).
+// At 256 registers 91 values a lane stay in scratch memory, in the main loop (q's fragments,
+// scores and outputs alone are 160).
 __global__ __launch_bounds__(256, 2) void paged_attn_f32_tiles_kernel(KArgs p) {
   constexpr int D = 128, BKV = 32, QPW = 32, BQ = 4 * QPW, ND = D / 32, NC = D / 8;
   constexpr int TILE = BKV * D, STAGE = 2 * TILE, NST = 2;
@@ -1612,7 +1617,8 @@ struct Shape {
 // heads, 69 us with two assumed and 62).  A counter for every row tile with parts: at most 2 * resident (two parts
 // or more of each) or, with a spill, 1.5 * resident of them, <= BLT_CACHE_SYNC_WORDS.  The form goes by the rows a sequence has on average: a tile of 16 rows costs the
 // matrix cores half of one of 32, and 128 rows share what they read; every form takes any
-// chunk, in more row tiles.
+// chunk, in more row tiles (63 single tokens and a chunk of 900 over 4000 keys: 194 us in one
+// call, 192 in two, 12 heads; 285 and 263, 32 / 8 heads of 128).
 int64_t row_tiles(const blt_paged_cache& c, int64_t B, int64_t total, int H, int bq) {
   return total * (H / c.n_kv_heads) / bq + B;
 }

@@ -277,7 +277,8 @@ int blt_cache_append(const blt_paged_cache* cache, int32_t layer, const void* k,
  *   causal: 1 = keys up to the token's own position; 0 = every key of the sequence
  *   window: W > 0 (with causal) = only the last W of them
  *   scale: of the scores, 1e-30 .. 1e30
- * Scores and softmax in f32; a token that sees no key gets 0.  Keys and values
+ * Scores and softmax in f32; a key whose score is -inf weighs nothing, a token that sees no
+ * key gets 0, infinite and NaN values come through where they are seen.  Keys and values
  * outside the sequences are not read; o [total, Hq, head_dim] behind starts[B] is left
  * as it was.  Page indices outside the pool are read as its nearest page.  Rows whose
  * sequence index is out of range are left as they were, all rows where starts does not
