@@ -501,14 +501,19 @@ __device__ inline bool join_tiles(const KArgs& p, const Item& it, bool active,
   return true;
 }
 
+// p = 2^(s c - m c) is one fma with m c rounded, which is off by 2^-24 |m c| in the exponent: much
+// where scores are large (beyond 2^31 the largest key's p would overflow or vanish).  From here
+// on m is taken from s first, which is exact.  Only looked at where a wave's offsets move.
+constexpr float kFar = 1024.f;
+
 // ---- bf16, tiles of rows ---------------------------------------------------------
 // One block = 4 waves of 32 rows each; key tiles of 64 keys go global -> LDS by DMA
 // through NST stages shared by the waves.  As in attn_fwd_kernel the scores are taken
 // transposed, S^T = K . Q^T, so a lane owns one row: its max and sum need one
 // cross-lane step, P^T feeds the second product from registers, and V's operand is
 // read with the LDS transposing read.  Unlike there q keeps its own bf16 values (scaling it
-// before its rounding costs as much accuracy as the output's rounding): the scores come
-// out of the matrix core minus the running max, and the scale is one multiply before exp2.
+// before its rounding costs as much accuracy as the output's rounding): the scale and the
+// running max go into one fma before exp2.
 // p is rounded to bf16 for the second product, and the sum takes the rounded values: the
 // outputs are 2.3e-3 off (relative, rms; their own rounding alone is 1.7e-3).  As two halves,
 // as in the form below, the chunks named next take 1080 us.
@@ -616,6 +621,8 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(KArgs p) {
 
   f32x16_t o[DS];
   float m = -INFINITY, l = 0.f;  // the row's offset (-inf until its first visible key), its sum
+  float mc = 0.f;                // -m c, or 0 where m is taken from the scores themselves (far)
+  bool far = false;
 #pragma unroll
   for (int j = 0; j < DS; ++j)
 #pragma unroll
@@ -708,8 +715,8 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(KArgs p) {
         swap_pair<32>(mt, a, b);
         mt = fmaxf(a, b);
       }
-      // the offset moves only when the max is more than 2^8 over it
-      if (__any(mt > m + grow_at)) {
+      // the offset moves only when the max is more than 2^8 over it (far: in every tile)
+      if (__any(mt > m + grow_at) || far) {
         const float m_new = fmaxf(m, mt);
         const float alpha = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - m_new) * c);
         m = m_new;
@@ -718,6 +725,16 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(KArgs p) {
         for (int j = 0; j < DS; ++j)
 #pragma unroll
           for (int r = 0; r < 16; ++r) o[j][r] *= alpha;
+        mc = m == -INFINITY ? 0.f : -m * c;
+        far = __any(fabsf(mc) > kFar);
+        if (__builtin_expect(far, false)) {
+          const float mu = m == -INFINITY ? 0.f : m;
+          mc = 0.f;
+#pragma unroll
+          for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[sub][r] -= mu;
+        }
       }
       // A weight of zero does not silence an infinite or NaN value: where rows see different
       // keys of a tile that holds one, it is taken out of the product and added to the
@@ -751,7 +768,6 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(KArgs p) {
           }
         }
       }
-      const float mc = m == -INFINITY ? 0.f : -m * c;
 #pragma unroll
       for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
@@ -917,9 +933,13 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(KArgs p) {
 
   f32x4_t o[NR][DB];
   float l[NR], m[NR];
+  float mc[NR];  // (as in paged_attn_kernel)
+  bool far[NR];
 #pragma unroll
   for (int n = 0; n < NR; ++n) {
     m[n] = -INFINITY;
+    mc[n] = 0.f;
+    far[n] = false;
     l[n] = 0.f;
 #pragma unroll
     for (int d = 0; d < DB; ++d) o[n][d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -973,20 +993,29 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(KArgs p) {
         swap_pair<32>(mt, a, b);
         mt = fmaxf(a, b);
       }
-      if (__any(mt > m[n] + grow_at)) {
+      if (__any(mt > m[n] + grow_at) || far[n]) {
         const float m_new = fmaxf(m[n], mt);
         const float alpha = m[n] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m[n] - m_new) * c);
         m[n] = m_new;
         l[n] *= alpha;
 #pragma unroll
         for (int d = 0; d < DB; ++d) o[n][d] *= alpha;
+        mc[n] = m_new == -INFINITY ? 0.f : -m_new * c;
+        far[n] = __any(fabsf(mc[n]) > kFar);
+        if (__builtin_expect(far[n], false)) {
+          const float mu = m_new == -INFINITY ? 0.f : m_new;
+          mc[n] = 0.f;
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[n][b][r] -= mu;
+        }
       }
-      const float mc = m[n] == -INFINITY ? 0.f : -m[n] * c;
       uint32_t wh[4], wl[4];
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
-        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[n][e >> 2][e & 3], c, mc));
-        const float p1 = __builtin_amdgcn_exp2f(fmaf(s[n][e >> 2][(e & 3) + 1], c, mc));
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[n][e >> 2][e & 3], c, mc[n]));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(s[n][e >> 2][(e & 3) + 1], c, mc[n]));
         l[n] += p0 + p1;
         const uint32_t x0 = __float_as_uint(p0), x1 = __float_as_uint(p1);
         wh[e >> 1] = __builtin_amdgcn_perm(x1, x0, 0x07060302);  // their upper halves

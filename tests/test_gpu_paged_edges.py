@@ -7,7 +7,7 @@ import torch
 
 import paged_ref as R
 from blt_burn_amd import BltError, cache as C, fused_ops as F, model as M, synth
-from test_gpu_paged import DEV, TYPES, Made, att_tol, check_attention, check_rotary, f64, i32
+from test_gpu_paged import DEV, TYPES, Made, att_tol, check_attention, check_rotary, device_rows, f64, i32
 
 pytestmark = pytest.mark.gpu
 
@@ -560,3 +560,38 @@ def test_overlapping_rows_are_read_as_they_are(dtype):
         assert torch.equal(got, want[0].transpose(0, 1)), (st, sh)
         assert torch.equal(m.cache.attention(0, x, i32([0, T])),
                            m.cache.attention(0, x.contiguous(), i32([0, T]))), (st, sh)
+
+
+# ---- large scores ------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("d,n,H,Hkv", [(64, 1, 2, 2), (128, 1, 4, 1), (64, 20, 1, 1), (64, 150, 2, 1), (128, 90, 2, 2),
+                                       (128, 400, 16, 8)])
+@pytest.mark.parametrize("scale,size", [(300.0, 1.0), (1e6, 1.0), (1e12, 1.0), (1e25, 1.0), (0.125, 1e6), (1e-4, 1e10)])
+def test_attention_of_large_scores_takes_the_largest(scale, size, d, n, H, Hkv, dtype):
+    """Where the largest score is far enough above the next for f32 to tell them apart, by more
+    than the softmax can see beside it, the output is that key's value, bit for bit."""
+    L = max(700, n)
+    m = Made([L], Hkv=Hkv, d=d, dtype=TYPES[dtype], seed=n)
+    m.kv[0].mul_(size)
+    torch.manual_seed(n + d)
+    q = (torch.randn(n, H, d, device=DEV) * size).to(TYPES[dtype])
+    o = m.cache.attention(0, q, i32([0, n]), scale=scale)
+    k, v = device_rows(m, 0, 0).double(), device_rows(m, 1, 0)
+    see = torch.arange(L, device=DEV)[None] <= torch.arange(L - n, L, device=DEV)[:, None]
+    told = 0
+    for h in range(H):
+        g = h * Hkv // H
+        s = (q[:, h].double() @ k[:, g].t()).masked_fill(~see, -float("inf"))
+        # f32 sums of d products: (d + 4) half steps of the sum of their magnitudes
+        off = (d + 4) * 2.0 ** -24 * (q[:, h].double().abs() @ k[:, g].abs().t()).amax(-1)
+        top = s.topk(2, -1)
+        gap = top.values[:, 0] - top.values[:, 1] - 2 * off
+        # 700 weights of 2^-140 together are below half a step of any bf16 or f32 value of a
+        # normal distribution's size that is not itself below 2^-100
+        sure = gap * scale > 100.0
+        told += int(sure.sum())
+        want = v[top.indices[:, 0], g]
+        assert torch.equal(o[:, h][sure], want[sure])
+    assert bool(torch.isfinite(o).all()) and float(o.float().abs().max()) <= float(v.float().abs().max()) * 1.01
+    assert told * 3 > n * H  # (a third of the rows and more can be told)
