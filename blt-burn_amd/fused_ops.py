@@ -235,7 +235,10 @@ class _RotaryGradient(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(positions)
         ctx.plan, ctx.turned = plan, backward
-        return fused_rotary(q, k, positions, plan, backward)
+        out = fused_rotary(q, k, positions, plan, backward)
+        ctx.mark_non_differentiable(*[y for y, need in zip(out, ctx.needs_input_grad)
+                                      if y is not None and not need])
+        return out
 
     @staticmethod
     def backward(ctx, gq, gk):

@@ -220,6 +220,21 @@ def test_rotary_gradients_of_shared_and_broadcast_inputs():
         assert torch.equal(z, F.fused_rotary(one, None, pos, plan)[0])
 
 
+def test_rotary_outputs_need_a_gradient_as_their_inputs_do():
+    plan, pos = F.RotaryPlan(64), torch.arange(9, dtype=torch.int32, device=DEV)
+    for nq, nk in ((False, False), (True, False), (False, True), (True, True)):
+        q = torch.randn(1, 2, 9, 64, device=DEV, requires_grad=nq)
+        k = torch.randn(1, 1, 9, 64, device=DEV, requires_grad=nk)
+        qo, ko = F.fused_rotary(q, k, pos, plan)
+        assert (qo.requires_grad, ko.requires_grad) == (nq, nk)
+        if nq or nk:
+            (qo.sum() + 2 * ko.sum()).backward()
+        want = [F.fused_rotary(torch.full_like(x, g).detach(), None, pos, plan, backward=True)[0]
+                for x, g in ((q, 1.0), (k, 2.0))]
+        for x, need, w in ((q, nq, want[0]), (k, nk, want[1])):
+            assert torch.equal(x.grad, w) if need else x.grad is None
+
+
 def test_rotary_gradient_in_a_captured_graph():
     """Forward and gradient captured and replayed with eager work between, against the eager
     ones; the leaf is used by nothing else while it is captured."""
