@@ -235,7 +235,8 @@ class PagedCache:
         ones of sequence seqs[b] (None: b; none twice), whose length already counts them
         (reserve).  rotary: a RotaryPlan that rotates k at its positions, and q [total, heads,
         head_dim] if given, which is returned (into `out`, which may be q; tokens at
-        starts[-1] and behind are not written).  starts ascends from 0 on."""
+        starts[-1] and behind are not written).  starts ascends from 0 on within the
+        tokens (else the status is set)."""
         layer = self._layer(layer)
         k, kp, total, _, ks, kh = self._tokens(k, "k", self.n_kv_heads)
         v, vp, n, _, vs, vh = self._tokens(v, "v", self.n_kv_heads)

@@ -241,11 +241,13 @@ __global__ __launch_bounds__(256) void append_kernel(AppendKernelArgs p, Deal dl
   int64_t s0 = 0, n = 0;
   int seq = -1, len = 0;
   bool found = false;
+  bool crossed = false;  // starts that do not ascend within the tokens
   if (a.B <= 64) {
     const int i = lane < a.B ? lane : (int)a.B - 1;
     const int lo = a.starts[i], hi = a.starts[i + 1];
     const int sq = a.seqs ? a.seqs[i] : i;
     const int ln = c.lens[sq >= 0 && sq < c.max_seqs ? sq : 0];
+    crossed = lo < 0 || hi < lo || hi > a.total;
     int b = __popcll(__ballot(lane < a.B && hi <= tok0));
     // (every lane takes part in the shuffles; tokens past the last row stop at 64)
     for (int next = __shfl(hi, b & 63); __any(b < a.B && next <= tok); next = __shfl(hi, b & 63))
@@ -264,6 +266,10 @@ __global__ __launch_bounds__(256) void append_kernel(AppendKernelArgs p, Deal dl
       if (m != ~0ull) break;
     }
     while (mine && b < a.B && a.starts[b + 1] <= tok) ++b;
+    if (blockIdx.x == 0)
+      for (int64_t i = tid; i < a.B; i += 256)
+        crossed = crossed || a.starts[i] < 0 || a.starts[i + 1] < a.starts[i] ||
+                  a.starts[i + 1] > a.total;
     found = mine && b < a.B;
     if (found) {
       s0 = a.starts[b];
@@ -287,6 +293,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendKernelArgs p, Deal dl
   if (found)
     token_angles(a.r, (int)pos, h0 * dl.units + u0, dl.units * dl.hg, false,
                  angles + tt * (a.r.rotary_dim / 2));
+  if (blockIdx.x == 0 && __any(crossed) && lane == 0) atomicOr(c.status, BLT_CACHE_BAD_INDEX);
   __syncthreads();
   if (!found) return;
   const bool bad = page < 0 || page >= c.num_pages;

@@ -263,7 +263,9 @@ int blt_cache_copy_pages(const blt_paged_cache* cache, const int32_t* src, const
  * seqs[b] (NULL: b; no sequence twice), whose length already counts them
  * (blt_cache_reserve).  rotary (may be NULL): k is rotated at its position, and q
  * [total, Hq, head_dim] into q_out (both may be NULL with Hq = 0; q_out may be q).
- * starts ascends; tokens at starts[B] and behind are left alone. */
+ * starts ascends from 0 within the tokens; tokens at starts[B] and behind are left alone.
+ * Starts that do not set BLT_CACHE_BAD_INDEX; which tokens are written then, at places
+ * of their rows' sequences, is not specified. */
 int blt_cache_append(const blt_paged_cache* cache, int32_t layer, const void* k, int64_t st_k,
                      int64_t sh_k, const void* v, int64_t st_v, int64_t sh_v, const void* q,
                      int64_t st_q, int64_t sh_q, void* q_out, int64_t st_qo, int64_t sh_qo,

@@ -610,3 +610,39 @@ def test_attention_of_large_scores_takes_the_largest(scale, size, d, n, H, Hkv, 
         assert torch.equal(o[:, h][sure], want[sure])
     assert bool(torch.isfinite(o).all()) and float(o.float().abs().max()) <= float(v.float().abs().max()) * 1.01
     assert told * 3 > n * H  # (a third of the rows and more can be told)
+
+
+# ---- starts ------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("B", [3, 64, 65, 300])
+def test_append_reports_starts_out_of_order(B):
+    """As attention does: starts that descend, begin below 0 or pass the tokens set the status, and
+    nothing outside the rows' own sequences is touched."""
+    n, page = 2, 8
+    m = Made([20] * B, Hkv=1, d=64, page=page, slots=B + 1)
+    c = m.cache
+    total = n * B
+    x = torch.randn(total, 1, 64, device=DEV).bfloat16()
+    free = [p for p in range(c.num_pages) if int(c.refcount[p]) == 0]
+    good = np.arange(B + 1) * n
+    c.append(0, x, x, i32(good))
+    c.check()
+    for at, value in ((B, total + 1), (B, total + 1000), (0, -1), (B // 2, total), (B // 2, total + 5), (1, 0),
+                      (B, 0)):
+        bad = good.copy()
+        bad[at] = value
+        ascends = (np.diff(bad) >= 0).all() and bad[0] >= 0 and bad[-1] <= total
+        for reps in range(3):
+            c.append(0, x, x, i32(bad))
+            if ascends:
+                c.check()
+            else:
+                with pytest.raises(BltError, match="out of range"):
+                    c.check()
+    assert bool(torch.isnan(c.k[0, free]).all()) and bool(torch.isnan(c.v[0, free]).all())
+    lens = c.lens.tolist()
+    assert lens[:B] == [20] * B
+    # tokens before the last `total` places of a sequence are what they were
+    for s in range(0, B, max(1, B // 7)):
+        first = m.rows(1, s)[:max(0, 20 - total)]
+        assert np.isfinite(first).all()
