@@ -354,8 +354,8 @@ __device__ void join_parts(const KArgs& p, const Item& it, int nr, float* room) 
   if (!last_part(p, it)) return;
   // U parts at a time, everything of them in flight at once (a read that passes the L2 takes
   // about 1 us), with a running max; past the last part: the last one again, without weight.
-  // Its infinite values become NaN by that: where a sum is none, once more with such parts empty
-  // (at once for all of them: one token over 1000 keys 8.9 us for 8.7).
+  // Its infinite values become NaN by that: where a sum is none, the parts are added up once
+  // more, those past the last as empty ones (0.2 us a call if it is always done so).
   const int64_t step = (int64_t)it.nrt * BQ;
   auto sum = [&](int i, int x0, int x1, auto at_once, auto odd) {
     constexpr int U = decltype(at_once)::value;
@@ -825,7 +825,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(KArgs p) {
 // negative rest would be NaN (below p = 2^-104, where the rest may vanish, it still is).
 // 48 single tokens over up to 8192 keys, 12 heads of 64: 128 us, 5.0 TB/s; 16 over up to 32768
 // keys, 32 / 8 heads of 128: 169 us, 5.5 TB/s (a large copy: 6.15).  One token over 1000 keys,
-// 12 heads: 8.8 us of dependent steps: launch 1.7, find_item 0.5, pages 0.6, tiles 2.1, the
+// 12 heads: 8.9 us of dependent steps: launch 1.7, find_item 0.5, pages 0.6, tiles 2.1, the
 // waves' merge 1.3, join 2.6; over 8192 keys 15.4 us, over 32768 26.8.
 constexpr float kAbove1 = 1.f + 0x1p-22f;
 template <int N>
