@@ -12,6 +12,7 @@
 #include <vector>
 
 #include "model.hpp"
+#include "packed.hpp"
 #include "paged.hpp"
 
 namespace blt {
@@ -290,6 +291,97 @@ int blt_fused_attention_f32(const float* q, const float* k, const float* v, floa
   if (!q || !o || (Tkv > 0 && (!k || !v)))
     return fail(BLT_ERR_INVALID, "attention_f32: null pointer");
   return launch_attention_f32(q, k, v, o, B, H, Tq, Tkv, d, causal, STREAM(stream));
+}
+
+static int packed_checks(int32_t dtype, int64_t total, int64_t Hq, int64_t Hkv, int32_t d,
+                         const int32_t* starts, int64_t B, int32_t window, float scale,
+                         const char* what) {
+  const std::string w(what);
+  if (dtype != BLT_DTYPE_F32 && dtype != BLT_DTYPE_BF16)
+    return fail(BLT_ERR_INVALID, w + ": bad dtype");
+  if (d != 64 && d != 128) return fail(BLT_ERR_SHAPE, w + ": head_dim must be 64 or 128");
+  if (Hkv < 1 || Hq < 1 || Hq > 0xffff || Hq % Hkv)
+    return fail(BLT_ERR_SHAPE, w + ": heads must be a multiple of kv_heads, at most 65535");
+  if (B < 0 || B > 0x7ffffffe || total < 0 || total > 0x7ffe0000 || Hq * total > 0x7ffe0000)
+    return fail(BLT_ERR_SHAPE, w + ": heads * tokens must fit int32");
+  if (window < 0) return fail(BLT_ERR_SHAPE, w + ": window must be >= 0");
+  if (!(scale >= 1e-30f) || !(scale <= 1e30f))
+    return fail(BLT_ERR_SHAPE, w + ": scale must be within 1e-30 .. 1e30");
+  if (total > 0 && !starts) return fail(BLT_ERR_INVALID, w + ": null starts");
+  return 0;
+}
+// rows of 16-byte alignment whose token stride leaves a tile's offsets in 32 bits
+static int packed_heads_check(const void* x, int64_t st, int64_t sh, int32_t dtype,
+                              const char* what) {
+  const std::string w(what);
+  const int64_t v = dtype == BLT_DTYPE_BF16 ? 8 : 4;
+  if (!x) return fail(BLT_ERR_INVALID, w + ": null pointer");
+  if (((uintptr_t)x & 15) || st % v || sh % v)
+    return fail(BLT_ERR_SHAPE, w + ": rows must be 16-byte aligned");
+  if (st < 0 || sh < 0 || st > (1 << 23) || sh > ((int64_t)1 << 40))
+    return fail(BLT_ERR_SHAPE, w + ": strides must not be negative, a token's at most 2^23");
+  return 0;
+}
+
+int blt_packed_attention(const void* q, int64_t st_q, int64_t sh_q, const void* k, int64_t st_k,
+                         int64_t sh_k, const void* v, int64_t st_v, int64_t sh_v, void* o,
+                         int64_t st_o, int64_t sh_o, float* lse, int32_t dtype, int64_t total,
+                         int64_t Hq, int64_t Hkv, int32_t d, const int32_t* starts, int64_t B,
+                         int32_t causal, int32_t window, float scale, int32_t tail,
+                         blt_stream_t stream) {
+  const char* what = "packed_attention";
+  if (int rc = packed_checks(dtype, total, Hq, Hkv, d, starts, B, window, scale, what)) return rc;
+  if (total == 0) return BLT_OK;
+  if (int rc = packed_heads_check(q, st_q, sh_q, dtype, what)) return rc;
+  if (int rc = packed_heads_check(k, st_k, sh_k, dtype, what)) return rc;
+  if (int rc = packed_heads_check(v, st_v, sh_v, dtype, what)) return rc;
+  if (int rc = packed_heads_check(o, st_o, sh_o, dtype, what)) return rc;
+  PackedAttnArgs a{};
+  a.q = PackedHeads{q, st_q, sh_q}; a.k = PackedHeads{k, st_k, sh_k};
+  a.v = PackedHeads{v, st_v, sh_v}; a.o = PackedHeads{o, st_o, sh_o};
+  a.lse = lse; a.dtype = dtype; a.total = total; a.H = (int)Hq; a.Hkv = (int)Hkv; a.d = d;
+  a.starts = starts; a.B = B; a.causal = causal ? 1 : 0; a.window = window; a.scale = scale;
+  a.tail = tail ? 1 : 0;
+  return launch_packed_attention(a, STREAM(stream));
+}
+
+int64_t blt_packed_attention_backward_workspace_bytes(int64_t total, int64_t Hq, int64_t Hkv) {
+  // (0 for what blt_packed_attention_backward refuses)
+  if (Hkv < 1 || Hq < 1 || Hq > 0xffff || Hq % Hkv || total < 0 || total > 0x7ffe0000 ||
+      Hq * total > 0x7ffe0000)
+    return 0;
+  return packed_attention_backward_workspace_bytes(total, (int)Hq, (int)Hkv);
+}
+int blt_packed_attention_backward(
+    const void* grad_o, int64_t st_go, int64_t sh_go, const void* q, int64_t st_q, int64_t sh_q,
+    const void* k, int64_t st_k, int64_t sh_k, const void* v, int64_t st_v, int64_t sh_v,
+    const void* o, int64_t st_o, int64_t sh_o, const float* lse, void* dq, int64_t st_dq,
+    int64_t sh_dq, void* dk, int64_t st_dk, int64_t sh_dk, void* dv, int64_t st_dv, int64_t sh_dv,
+    int32_t dtype, int64_t total, int64_t Hq, int64_t Hkv, int32_t d, const int32_t* starts,
+    int64_t B, int32_t causal, int32_t window, float scale, void* workspace,
+    int64_t workspace_bytes, blt_stream_t stream) {
+  const char* what = "packed_attention_backward";
+  if (int rc = packed_checks(dtype, total, Hq, Hkv, d, starts, B, window, scale, what)) return rc;
+  if (total == 0) return BLT_OK;
+  const PackedHeads x[8] = {{grad_o, st_go, sh_go}, {q, st_q, sh_q},    {k, st_k, sh_k},
+                            {v, st_v, sh_v},        {o, st_o, sh_o},    {dq, st_dq, sh_dq},
+                            {dk, st_dk, sh_dk},     {dv, st_dv, sh_dv}};
+  for (const PackedHeads& h : x)
+    if (int rc = packed_heads_check(h.x, h.st, h.sh, dtype, what)) return rc;
+  const int64_t G = Hq / Hkv;
+  if (sh_q > ((int64_t)1 << 29) / G || sh_go > ((int64_t)1 << 29) / G)
+    return fail(BLT_ERR_SHAPE, std::string(what) + ": head strides of q and grad_o too large");
+  if (!lse) return fail(BLT_ERR_INVALID, std::string(what) + ": null pointer");
+  if (!workspace || ((uintptr_t)workspace & 15) ||
+      workspace_bytes < packed_attention_backward_workspace_bytes(total, (int)Hq, (int)Hkv))
+    return fail(BLT_ERR_INVALID, std::string(what) + ": workspace missing, misaligned or too small");
+  PackedAttnArgs a{};
+  a.q = x[1]; a.k = x[2]; a.v = x[3]; a.o = x[4];
+  a.lse = const_cast<float*>(lse); a.dtype = dtype; a.total = total; a.H = (int)Hq;
+  a.Hkv = (int)Hkv; a.d = d; a.starts = starts; a.B = B; a.causal = causal ? 1 : 0;
+  a.window = window; a.scale = scale;
+  return launch_packed_attention_backward(a, PackedGradArgs{x[0], x[5], x[6], x[7]}, workspace,
+                                          STREAM(stream));
 }
 
 int blt_rope_table_f32(float* out_device, int32_t head_dim, int32_t max_seqlen, double theta,

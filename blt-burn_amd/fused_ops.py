@@ -15,7 +15,8 @@ from ._lib import EPS_AFTER_SQRT, EPS_INSIDE_SQRT, BltError, check
 from ._torch import call_on, contiguous, require_cuda, stream_ptr
 
 __all__ = ["fused_entropy", "fused_rms_norm", "fused_softmax", "fused_l2_norm",
-           "fused_silu_gate", "fused_coherence", "fused_attention", "RotaryPlan", "fused_rotary",
+           "fused_silu_gate", "fused_coherence", "fused_attention", "fused_packed_attention",
+           "fused_packed_attention_backward", "RotaryPlan", "fused_rotary",
            "EPS_AFTER_SQRT", "EPS_INSIDE_SQRT"]
 
 
@@ -173,6 +174,150 @@ def fused_attention(q, k, v, use_causal_mask, window=0, rope_theta=0.0):
         float(rope_theta), ws.data_ptr() if ws is not None else 0, stream_ptr(qb.device)),
         "fused_attention")
     return o if in_dtype == torch.bfloat16 else o.to(in_dtype)
+
+
+def _packed_heads(t, what, like=None, heads=None):
+    """t [total, heads, head_dim] with 16-byte aligned rows: itself or a copy, its pointer and
+    strides."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("expected a torch.Tensor, got %r" % type(t))
+    if like is None:
+        require_cuda(t)
+        _dtype_ok(t)
+        if t.dim() != 3 or t.shape[2] not in (64, 128):
+            raise BltError("fused_packed_attention: %s must be [tokens, heads, head_dim 64 or 128]"
+                           % what)
+    elif t.device != like.device or t.dtype != like.dtype or t.dim() != 3 or \
+            t.shape[0] != like.shape[0] or t.shape[2] != like.shape[2] or \
+            (heads is not None and t.shape[1] != heads):
+        raise BltError("fused_packed_attention: %s must be %s [%d, %s, %d] on %s"
+                       % (what, like.dtype, like.shape[0], "heads" if heads is None else heads,
+                          like.shape[2], like.device))
+    st, sh, sd = t.stride()
+    if sd != 1 or (st | sh) % (16 // t.element_size()) or t.data_ptr() % 16 or st > 1 << 23:
+        t = t.clone(memory_format=torch.contiguous_format)
+        st, sh, sd = t.stride()
+    return t, t.data_ptr(), st, sh
+
+
+def _packed_setting(q, k, starts, window, scale):
+    H, Hkv = q.shape[1], k.shape[1]
+    if Hkv == 0 or H == 0 or H % Hkv:
+        raise BltError("fused_packed_attention: heads must be a multiple of kv_heads")
+    if not isinstance(starts, torch.Tensor):
+        raise TypeError("expected a torch.Tensor, got %r" % type(starts))
+    if starts.dtype is not torch.int32 or starts.device != q.device or starts.dim() != 1 or \
+            not starts.is_contiguous() or starts.shape[0] < 1:
+        raise BltError("fused_packed_attention: starts must be a contiguous int32 [sequences + 1] "
+                       "on %s" % q.device)
+    if window < 0:
+        raise BltError("fused_packed_attention: window must be >= 0")
+    # (here too: past 32 bits the call would see its low bits)
+    return (0 if window > 0x7fffffff else window), (q.shape[2] ** -0.5 if scale is None else scale)
+
+
+class _PackedGradient(torch.autograd.Function):
+    """fused_packed_attention for inputs that need a gradient."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, starts, causal, window, scale):
+        o, lse = fused_packed_attention(q, k, v, starts, causal, window, scale, return_lse=True)
+        ctx.save_for_backward(q, k, v, o, lse, starts)
+        ctx.setting = causal, window, scale
+        ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)
+        return o, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_o, _):
+        if grad_o is None:
+            return (None,) * 7
+        q, k, v, o, lse, starts = ctx.saved_tensors
+        out = fused_packed_attention_backward(grad_o, q, k, v, o, lse, starts, *ctx.setting)
+        return tuple(g if need else None
+                     for g, need in zip(out, ctx.needs_input_grad)) + (None,) * 4
+
+
+def fused_packed_attention(q, k, v, starts, causal=True, window=0, scale=None, out=None,
+                           return_lse=False):
+    """Attention of whole sequences of different lengths, packed behind each other: q [tokens,
+    heads, head_dim], k and v [tokens, kv_heads, head_dim] (f32 or bf16, head_dim 64 or 128,
+    heads a multiple of kv_heads; any strides, e.g. views into a packed QKV tensor, are
+    read as they are where rows are dense and 16-byte aligned).  Sequence b has the tokens starts[b] ..
+    starts[b + 1] - 1 (int32 [sequences + 1], ascending from 0).  causal: a token sees the keys of its
+    sequence up to its own, with window > 0 only the last `window` of them; causal=False: all
+    of them.  scale defaults to head_dim^-0.5.
+
+    Returns o [tokens, heads, head_dim]; with return_lse also the logarithms of the softmax's sums,
+    f32 [tokens, heads] (-inf for none), which fused_packed_attention_backward takes.  Tokens at
+    starts[-1] and behind get 0 in a new tensor and are left alone in `out`.  Scores and sums
+    are f32 throughout; in bf16 the weights are rounded to bf16.  Autograd follows it for o
+    (once; `out` takes no inputs that need a gradient)."""
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad
+                                       for t in (q, k, v)):
+        if out is not None:
+            raise BltError("fused_packed_attention: out takes no inputs that need a gradient (use "
+                           "torch.no_grad())")
+        both = _PackedGradient.apply(q, k, v, starts, causal, window, scale)
+        return both if return_lse else both[0]
+    q, qp, qs, qh = _packed_heads(q, "q")
+    k, kp, ks, kh = _packed_heads(k, "k", q)
+    v, vp, vs, vh = _packed_heads(v, "v", q, k.shape[1])
+    window, scale = _packed_setting(q, k, starts, window, scale)
+    total, H, d = q.shape
+    tail = 1 if out is None else 0
+    if out is None:
+        out = torch.empty((total, H, d), dtype=q.dtype, device=q.device)
+        op, os_, oh = out.data_ptr(), H * d, d
+    else:
+        t, op, os_, oh = _packed_heads(out, "out", q, H)
+        if t is not out:
+            raise BltError("fused_packed_attention: out needs dense, 16-byte aligned rows")
+    lse = lp = None
+    if return_lse:
+        lse = torch.empty((total, H), dtype=torch.float32, device=q.device)
+        lp = lse.data_ptr()
+    call_on(q.device, q.get_device(), _lib.lib().blt_packed_attention, "packed_attention", qp, qs,
+            qh, kp, ks, kh, vp, vs, vh, op, os_, oh, lp,
+            _lib.DTYPE_BF16 if q.dtype == torch.bfloat16 else _lib.DTYPE_F32, total, H, k.shape[1],
+            d, starts.data_ptr(), starts.shape[0] - 1, 1 if causal else 0, window, scale, tail)
+    return (out, lse) if return_lse else out
+
+
+def fused_packed_attention_backward(grad_o, q, k, v, o, lse, starts, causal=True, window=0,
+                                    scale=None):
+    """(dq, dk, dv) of fused_packed_attention from its output's gradient, its o and lse, and its
+    other arguments; tokens at starts[-1] and behind get 0.  Sums are f32, in bf16 the weights and
+    their gradients are rounded to bf16; the same bits in every run."""
+    q, qp, qs, qh = _packed_heads(q, "q")
+    total, H, d = q.shape
+    k, kp, ks, kh = _packed_heads(k, "k", q)
+    Hkv = k.shape[1]
+    v, vp, vs, vh = _packed_heads(v, "v", q, Hkv)
+    o, op, os_, oh = _packed_heads(o, "o", q, H)
+    grad_o, gp, gs, gh = _packed_heads(grad_o, "grad_o", q, H)
+    window, scale = _packed_setting(q, k, starts, window, scale)
+    if max(qh, gh) * (H // Hkv) > 1 << 29:
+        q, grad_o = (t.clone(memory_format=torch.contiguous_format) for t in (q, grad_o))
+        qp, gp, qs, gs, qh, gh = q.data_ptr(), grad_o.data_ptr(), H * d, H * d, d, d
+    if not isinstance(lse, torch.Tensor):
+        raise TypeError("expected a torch.Tensor, got %r" % type(lse))
+    if lse.dtype != torch.float32 or lse.device != q.device or lse.shape != (total, H):
+        raise BltError("fused_packed_attention_backward: lse must be f32 [tokens, heads]")
+    lse = contiguous(lse)
+    L = _lib.lib()
+    dq = torch.empty((total, H, d), dtype=q.dtype, device=q.device)
+    dk, dv = (torch.empty((total, Hkv, d), dtype=q.dtype, device=q.device) for _ in range(2))
+    size = L.blt_packed_attention_backward_workspace_bytes(total, H, Hkv)
+    ws = torch.empty(size, dtype=torch.uint8, device=q.device)
+    call_on(q.device, q.get_device(), L.blt_packed_attention_backward, "packed_attention_backward",
+            gp, gs, gh, qp, qs, qh, kp, ks, kh, vp, vs, vh, op, os_, oh, lse.data_ptr(),
+            dq.data_ptr(), H * d, d, dk.data_ptr(), Hkv * d, d, dv.data_ptr(), Hkv * d, d,
+            _lib.DTYPE_BF16 if q.dtype == torch.bfloat16 else _lib.DTYPE_F32, total, H, Hkv, d,
+            starts.data_ptr(), starts.shape[0] - 1, 1 if causal else 0, window, scale,
+            ws.data_ptr(), size)
+    return dq, dk, dv
 
 
 class RotaryPlan:

@@ -131,6 +131,42 @@ int blt_fused_attention_f32(const float* q, const float* k, const float* v, floa
                             int64_t H, int64_t Tq, int64_t Tkv, int32_t d, int32_t causal,
                             blt_stream_t stream);
 
+/* Attention of B whole sequences packed behind each other (no counterpart in the reference,
+ * whose rows are one [B, H, T, d] shape): q, o [total, Hq, d] and k, v [total, Hkv, d] with
+ * token and head strides in elements, unit d-stride; rows 16-byte aligned, token strides at
+ * most 2^23.  Sequence b has the tokens starts[b] .. starts[b + 1] - 1 (int32 [B + 1], device,
+ * ascending from 0 within the tokens; otherwise the outputs are not specified).  Query head h
+ * reads key head h / (Hq / Hkv).  d 64 or 128.
+ *   causal: 1 = keys of the token's sequence up to its own position; 0 = every key of it
+ *   window: W > 0 (with causal) = only the last W of them
+ *   scale:  of the scores, 1e-30 .. 1e30
+ *   lse:    (may be NULL) f32 [total, Hq], log of the sum of e^score, -inf where it is 0
+ *   tail:   tokens at starts[B] and behind: 0 = left alone, 1 = outputs 0, lse -inf
+ * Scores, softmax and sums in f32; in bf16 the weights are rounded to bf16.  A key whose
+ * score is -inf weighs nothing; infinite and NaN values come through where they are seen. */
+int blt_packed_attention(const void* q, int64_t st_q, int64_t sh_q, const void* k, int64_t st_k,
+                         int64_t sh_k, const void* v, int64_t st_v, int64_t sh_v, void* o,
+                         int64_t st_o, int64_t sh_o, float* lse, int32_t dtype, int64_t total,
+                         int64_t Hq, int64_t Hkv, int32_t d, const int32_t* starts, int64_t B,
+                         int32_t causal, int32_t window, float scale, int32_t tail,
+                         blt_stream_t stream);
+
+/* Gradients of blt_packed_attention's q, k and v from that of its output, with its o and lse;
+ * the other arguments as there, a head stride of q and grad_o times Hq / Hkv at most 2^29.  dq
+ * [total, Hq, d], dk and dv [total, Hkv, d] are written whole: 0 at starts[B] and behind.
+ * Sums in f32, the weights and their gradients rounded to bf16 in bf16; the same bits
+ * in every run.  workspace: blt_packed_attention_backward_workspace_bytes, 16-byte aligned, no
+ * initialisation; calls that share one must be stream-ordered. */
+int64_t blt_packed_attention_backward_workspace_bytes(int64_t total, int64_t Hq, int64_t Hkv);
+int blt_packed_attention_backward(
+    const void* grad_o, int64_t st_go, int64_t sh_go, const void* q, int64_t st_q, int64_t sh_q,
+    const void* k, int64_t st_k, int64_t sh_k, const void* v, int64_t st_v, int64_t sh_v,
+    const void* o, int64_t st_o, int64_t sh_o, const float* lse, void* dq, int64_t st_dq,
+    int64_t sh_dq, void* dk, int64_t st_dk, int64_t sh_dk, void* dv, int64_t st_dv, int64_t sh_dv,
+    int32_t dtype, int64_t total, int64_t Hq, int64_t Hkv, int32_t d, const int32_t* starts,
+    int64_t B, int32_t causal, int32_t window, float scale, void* workspace,
+    int64_t workspace_bytes, blt_stream_t stream);
+
 /* RoPE table, precompute_freqs_cis (model.rs:24-52): out [max_seqlen, head_dim/2, 2]
  * f32 (cos, sin), computed on the host in the reference's f32 order, copied to device. */
 int blt_rope_table_f32(float* out_device, int32_t head_dim, int32_t max_seqlen, double theta,
