@@ -46,6 +46,9 @@ EXPORTS = {
                                  + [c_i64] * 9 + [c_i32, c_i32, c_f32, c_vp, c_vp]),
     "blt_fused_attention_f32": (c_i32, [c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_i32,
                                         c_i32, c_vp]),
+    "blt_fused_sample_workspace_bytes": (c_i64, [c_i64, c_i32]),
+    "blt_fused_sample": (c_i32, [c_vp, c_i64, c_i32, c_i64, c_i32, c_vp, c_f64, c_vp, c_i32, c_vp,
+                                 c_f64, c_vp, c_f64, c_vp, c_vp, c_vp, c_i64, c_vp]),
     "blt_packed_attention": (c_i32, [c_vp, c_i64, c_i64] * 4 + [c_vp, c_i32] + [c_i64] * 3
                              + [c_i32, c_vp, c_i64, c_i32, c_i32, c_f32, c_i32, c_vp]),
     "blt_packed_attention_backward_workspace_bytes": (c_i64, [c_i64] * 3),

@@ -14,6 +14,7 @@
 #include "model.hpp"
 #include "packed.hpp"
 #include "paged.hpp"
+#include "sample.hpp"
 
 namespace blt {
 
@@ -382,6 +383,40 @@ int blt_packed_attention_backward(
   a.window = window; a.scale = scale;
   return launch_packed_attention_backward(a, PackedGradArgs{x[0], x[5], x[6], x[7]}, workspace,
                                           STREAM(stream));
+}
+
+int64_t blt_fused_sample_workspace_bytes(int64_t rows, int32_t vocab) {
+  // (0 for what blt_fused_sample refuses)
+  return rows < 0 || rows > 0x7fffffff || vocab < 1 || vocab > kSampleVocab
+             ? 0
+             : sample_workspace_bytes(rows, vocab);
+}
+int blt_fused_sample(const void* logits, int64_t row_stride, int32_t dtype, int64_t rows,
+                     int32_t vocab, const float* uniform, double temperature,
+                     const float* temperatures, int32_t top_k, const int32_t* top_ks, double top_p,
+                     const float* top_ps, double min_p, const float* min_ps, int32_t* tokens,
+                     void* workspace, int64_t workspace_bytes, blt_stream_t stream) {
+  if (dtype != BLT_DTYPE_F32 && dtype != BLT_DTYPE_BF16)
+    return fail(BLT_ERR_INVALID, "fused_sample: bad dtype");
+  if (rows < 0 || rows > 0x7fffffff || vocab < 1 || vocab > kSampleVocab)
+    return fail(BLT_ERR_SHAPE, "fused_sample: vocab must be 1 .. 2^20");
+  if (row_stride < 0) return fail(BLT_ERR_SHAPE, "fused_sample: negative row stride");
+  if (!temperatures && !(temperature >= 0. && temperature < (double)INFINITY))
+    return fail(BLT_ERR_SHAPE, "fused_sample: temperature must be finite and >= 0");
+  if (!top_ks && top_k < 0) return fail(BLT_ERR_SHAPE, "fused_sample: top_k must be >= 0");
+  if (!top_ps && !(top_p > 0.)) return fail(BLT_ERR_SHAPE, "fused_sample: top_p must be > 0");
+  if (!min_ps && !(min_p >= 0. && min_p <= 1.))
+    return fail(BLT_ERR_SHAPE, "fused_sample: min_p must be within 0 .. 1");
+  if (rows == 0) return BLT_OK;
+  if (!logits || !uniform || !tokens) return fail(BLT_ERR_INVALID, "fused_sample: null pointer");
+  const int64_t need = sample_workspace_bytes(rows, vocab);
+  if (need > 0 && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need))
+    return fail(BLT_ERR_INVALID, "fused_sample: workspace missing, misaligned or too small");
+  SampleArgs a{};
+  a.logits = logits; a.row_stride = row_stride; a.dtype = dtype; a.rows = rows; a.vocab = vocab;
+  a.uniform = uniform; a.out = tokens;
+  a.set = SampleSetting{temperature, top_p, min_p, top_k, temperatures, top_ps, min_ps, top_ks};
+  return launch_sample(a, workspace, STREAM(stream));
 }
 
 int blt_rope_table_f32(float* out_device, int32_t head_dim, int32_t max_seqlen, double theta,

@@ -1,0 +1,816 @@
+// One token a row from logits, by temperature, top-k, top-p and min-p, from given random
+// numbers.
+//
+// With tokens ranked by logit (descending, equal ones by index) and weights
+// w_i = e^((x_i - max) / temperature), the tokens kept are the first n ranks: at most top_k;
+// those whose running sum before them is below top_p times the sum of the top_k; those with
+// w >= min_p.  The token drawn is the lowest index whose running sum of kept weights, in the order
+// of the indices, passes u times their sum.
+//
+// No sorting: all three rules keep a prefix of the ranks, so a row's choice is a cut, the last
+// kept (logit, index), found by counting.  Weights are exponentials in 64 bits rounded to
+// fixed point (2^SCALE = 1, so that a row's sum stays below 2^63): sums of integers do not
+// depend on their order, so the tokens are the same bits in every run whatever adds up first, and off
+// by at most vocab / 2^(SCALE + 1) of the largest weight.
+//
+// By the size of the vocabulary: up to 1024 a wave holds a row in registers and bisects
+// the cut over the bits of the logits; up to 16384 a block holds it in LDS and counts bins; above that rows are
+// cut into parts, in five launches (the largest logit, the parts' bins, the cut, the kept
+// sums of the parts, the token).
+#include "sample.hpp"
+
+namespace blt {
+
+namespace {
+
+struct SArgs {
+  const void* x;
+  int64_t st;  // row stride
+  int64_t rows;
+  int V;
+  const float* u;
+  SampleSetting s;
+  int32_t* out;
+  int scale;
+  // parts of rows
+  int parts;
+  float* pmax;      // [rows][parts], NaN where a logit is
+  uint64_t* pmass;  // [rows][parts]
+  uint64_t* hm;     // [rows][parts][NB]
+  uint32_t* hc;     // [rows][parts][NB]
+  int2* cut;        // [rows]: see Cut
+};
+
+template <typename T>
+__device__ inline float logit(const void* x, int64_t i) {
+  if constexpr (sizeof(T) == 2) return bf16_to_f32(((const uint16_t*)x)[i]);
+  else return ((const float*)x)[i];
+}
+// an integer that orders as the value does (-0 as 0), and back
+__device__ inline uint32_t key_of(float x) {
+  const uint32_t b = __float_as_uint(x + 0.f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ inline float value_of(uint32_t key) {
+  return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
+}
+// the last kept (logit, index): tokens with a larger key, or the same and an index up to this
+struct Cut {
+  uint32_t key;
+  int index;
+};
+__device__ inline bool kept(const Cut& c, uint32_t key, int i) {
+  return key > c.key || (key == c.key && i <= c.index);
+}
+
+// ---- a row's rules ---------------------------------------------------------------------
+struct Rules {
+  double a;     // log2(e) / temperature
+  double p;     // top_p; 1 or more: off
+  uint64_t m;   // smallest weight kept
+  int k;        // 0: off
+  float bins;   // bins per logit (see bin_of)
+  bool good;
+};
+constexpr int NB = 2048;
+__device__ inline Rules rules_of(const SArgs& g, int64_t row) {
+  const SampleSetting& s = g.s;
+  const double t = s.temperatures ? (double)s.temperatures[row] : s.temperature;
+  const double p = s.top_ps ? (double)s.top_ps[row] : s.top_p;
+  const double m = s.min_ps ? (double)s.min_ps[row] : s.min_p;
+  const int k = s.top_ks ? s.top_ks[row] : s.top_k;
+  Rules r;
+  r.good = t >= 0. && t < (double)INFINITY && p > 0. && m >= 0. && m <= 1. && k >= 0 &&
+           g.u[row] == g.u[row];
+  r.a = t > 0. ? 1.4426950408889634074 / t : 1.;
+  r.p = p;
+  r.m = (uint64_t)ceil(ldexp(m, g.scale));
+  r.k = t > 0. ? k : 1;  // (temperature 0: the first of the largest)
+  if (r.k >= g.V) r.k = 0;
+  // weights below 2^-63 share the last bin
+  r.bins = (float)((NB - 1) / 63. * r.a);
+  return r;
+}
+__device__ inline uint64_t weight(float x, float top, const Rules& r, int scale) {
+  if (x == top) return (uint64_t)1 << scale;
+  const double y = (double)scale - ((double)top - (double)x) * r.a;
+  return y > -2. ? (uint64_t)rint(exp2(y)) : 0;
+}
+// a bin of about the same logits, the largest ones first; the order of bins is that of logits
+__device__ inline int bin_of(float x, float top, const Rules& r) {
+  const float t = (top - x) * r.bins;
+  return x == top ? 0 : t < (float)(NB - 1) ? (int)t : NB - 1;
+}
+__device__ inline uint64_t wanted(double p, uint64_t sum) {  // least running sum >= p * sum
+  const double x = ceil(p * (double)sum);
+  return x >= (double)sum ? sum : x < 1. ? 1 : (uint64_t)x;
+}
+// u of the sum: the token is the first whose running sum is above
+__device__ inline uint64_t aim_of(float u, uint64_t sum) {
+  const double x = floor((double)fminf(fmaxf(u, 0.f), 1.f) * (double)sum);
+  return x >= (double)sum ? sum - 1 : (uint64_t)x;
+}
+
+// ---- 64-bit sums over a wave -------------------------------------------------------------
+template <int CTRL, int ROWS>
+__device__ inline uint64_t dpp_u64(uint64_t x) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, CTRL, ROWS, 0xF, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(x >> 32), CTRL, ROWS, 0xF, false);
+  return (uint64_t)hi << 32 | lo;
+}
+__device__ inline uint64_t lane_u64(uint64_t x, int l) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), l) << 32 |
+         (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, l);
+}
+__device__ inline uint64_t incl_scan_u64(uint64_t v) {  // (as wave_incl_scan)
+  v += dpp_u64<0x111, 0xF>(v);
+  v += dpp_u64<0x112, 0xF>(v);
+  v += dpp_u64<0x114, 0xF>(v);
+  v += dpp_u64<0x118, 0xF>(v);
+  v += dpp_u64<0x142, 0xA>(v);
+  v += dpp_u64<0x143, 0xC>(v);
+  return v;
+}
+__device__ inline uint64_t sum_u64(uint64_t v) { return lane_u64(incl_scan_u64(v), 63); }
+__device__ inline uint32_t wave_min_u32(uint32_t x) {
+  return ~((uint32_t)wave_max_i32((int)(~x ^ 0x80000000u)) ^ 0x80000000u);
+}
+__device__ inline uint32_t wave_max_u32(uint32_t x) {
+  return (uint32_t)wave_max_i32((int)(x ^ 0x80000000u)) ^ 0x80000000u;
+}
+__device__ inline int below(uint64_t mask) {  // set bits below this lane
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32),
+                                   __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+}
+__device__ inline int bits(uint64_t mask) { return __popcll((unsigned long long)mask); }
+
+// ---- up to 1024 tokens: one wave a row ------------------------------------------------------
+template <typename T, int N>
+__global__ __launch_bounds__(256) void sample_wave_kernel(SArgs g) {
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= g.rows) return;
+  const int lane = threadIdx.x & 63;
+  const char* x = (const char*)g.x + row * g.st * (int64_t)sizeof(T);
+  float v[N];
+  uint32_t key[N];
+  float top = -INFINITY;
+  bool nan = false;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    v[j] = lane + 64 * j < g.V ? logit<T>(x, lane + 64 * j) : -INFINITY;
+    nan |= v[j] != v[j];
+    key[j] = lane + 64 * j < g.V ? key_of(v[j]) : 0;  // (a logit's is never 0)
+    top = fmaxf(top, v[j]);
+  }
+  top = wave_max(top);
+  const Rules r = rules_of(g, row);
+  if (__any(nan) || top == -INFINITY || !r.good) {
+    if (lane == 0) g.out[row] = -1;
+    return;
+  }
+  uint64_t w[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) w[j] = weight(v[j], top, r, g.scale);
+  auto count = [&](uint32_t c) {
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) n += bits(__ballot(key[j] >= c));
+    return n;
+  };
+  auto mass = [&](uint32_t c) {
+    uint64_t m = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) m += key[j] >= c ? w[j] : 0;
+    return sum_u64(m);
+  };
+  // The largest c whose tokens of key >= c are enough, as far as it matters: down to one
+  // token or one key between lo (enough) and hi (not); `over` tokens at or above hi.
+  uint32_t lo = 1;
+  int at = g.V;            // tokens of key >= lo
+  int ties = 0x7fffffff;   // kept ones of the smallest key >= lo
+  if (r.k) {
+    uint32_t hi = key_of(top) + 1;
+    int over = 0;
+    while (hi - lo > 1 && at - over > 1 && at != r.k) {
+      const uint32_t mid = lo + ((hi - lo) >> 1);
+      const int n = count(mid);
+      if (n >= r.k) {
+        lo = mid;
+        at = n;
+      } else {
+        hi = mid;
+        over = n;
+      }
+    }
+    if (at != r.k) ties = r.k - over;  // (of at - over with the one key that is left)
+  }
+  if (r.p < 1.) {
+    uint64_t sum = mass(lo);
+    if (ties < 0x7fffffff) {
+      const uint64_t above = mass(lo + 1);
+      sum = above + (sum - above) / (uint64_t)(at - (r.k - ties)) * (uint64_t)ties;
+    }
+    const uint64_t want = wanted(r.p, sum);
+    const uint32_t first = lo;
+    uint32_t hi = key_of(top) + 1;
+    int over = 0;
+    uint64_t above = 0;
+    while (hi - lo > 1 && at - over > 1) {
+      const uint32_t mid = lo + ((hi - lo) >> 1);
+      const uint64_t m = mass(mid);
+      if (m >= want) {
+        lo = mid;
+        at = count(mid);
+      } else {
+        hi = mid;
+        over = count(mid);
+        above = m;
+      }
+    }
+    // one key is left; its tokens' weight is not 0, for with them the sum reaches `want`
+    const uint64_t each = (mass(lo) - above) / (uint64_t)(at - over);
+    const uint64_t need = (want - above + each - 1) / each;
+    const int n = need < (uint64_t)(at - over) ? (int)need : at - over;
+    ties = lo == first ? min(ties, n) : n;
+  }
+  // kept weights, the ties in the order of their indices
+  uint64_t total = 0;
+  {
+    uint32_t tie = 0xffffffffu;
+#pragma unroll
+    for (int j = 0; j < N; ++j) tie = key[j] >= lo ? min(tie, key[j]) : tie;
+    tie = wave_min_u32(tie);
+    int before = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const uint64_t here = __ballot(key[j] == tie);
+      const bool in = key[j] > tie || (key[j] == tie && before + below(here) < ties);
+      w[j] = in && w[j] >= r.m ? w[j] : 0;
+      before += bits(here);
+      total += w[j];
+    }
+  }
+  total = sum_u64(total);
+  const uint64_t aim = aim_of(g.u[row], total);
+  uint64_t run = 0;
+  int token = -1;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const uint64_t s = incl_scan_u64(w[j]);
+    const uint64_t hit = __ballot(run + s > aim);
+    if (token < 0 && hit) token = 64 * j + __ffsll((unsigned long long)hit) - 1;
+    run += lane_u64(s, 63);
+  }
+  if (lane == 0) g.out[row] = token;
+}
+
+// ---- blocks of 1024 threads ------------------------------------------------------------------
+constexpr int NT = 1024, NW = NT / 64;
+constexpr int PART = 16 * NT;  // tokens that a block holds in registers
+
+// Tokens [0, n) of a row in the registers of a block, or in memory; wave w has a run of them, so
+// that the waves' runs, and the groups of 64 within one, follow each other. each(f) calls
+// f(x, index, j) in that order in all lanes, with index < 0 where there is no token; j counts
+// the calls.
+template <typename T, int N>
+struct Held {
+  float x[N];
+  int first, n;
+  __device__ inline Held(const void* row, int64_t from, int n_) : n(n_) {
+    first = (int)(threadIdx.x >> 6) * 64 * N + (int)(threadIdx.x & 63);
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      x[j] = first + 64 * j < n ? logit<T>(row, from + first + 64 * j) : -INFINITY;
+  }
+  template <typename F>
+  __device__ inline void each(F f) const {
+#pragma unroll
+    for (int j = 0; j < N; ++j) f(x[j], first + 64 * j < n ? first + 64 * j : -1, j);
+  }
+};
+template <typename T>
+struct InMemory {
+  const void* row;
+  int n, run;
+  __device__ inline InMemory(const void* row_, int n_) : row(row_), n(n_) {
+    run = ((n + NW - 1) / NW + 63) & ~63;
+  }
+  template <typename F>
+  __device__ inline void each(F f) const {
+    const int a = (int)(threadIdx.x >> 6) * run, lane = threadIdx.x & 63;
+    for (int j = 0; j < run; j += 64 * 8) {
+      float x[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int i = a + j + 64 * u + lane;
+        x[u] = j + 64 * u < run && i < n ? logit<T>(row, i) : -INFINITY;
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int i = a + j + 64 * u + lane;
+        f(x[u], j + 64 * u < run && i < n ? i : -1, j / 64 + u);
+      }
+    }
+  }
+};
+
+struct Room {
+  uint64_t m[NB];  // bins: sum of weights and tokens
+  uint32_t c[NB];
+  uint32_t lk[NT];  // a bin's tokens
+  uint64_t lw[NT];
+  int li[NT];
+  uint64_t wm[NW];  // of the waves
+  uint32_t wc[NW], wx[NW];
+  int n;
+  Cut cut;
+  uint64_t sum;
+  // a bin, and what lies above it
+  int bin;
+  uint32_t above_c, in_c;
+  uint64_t above_m;
+};
+__device__ inline void zero_bins(Room& s) {
+  for (int i = threadIdx.x; i < NB; i += NT) {
+    s.m[i] = 0;
+    s.c[i] = 0;
+  }
+}
+__device__ inline void add_to_bin(Room& s, int b, uint64_t w) {
+  atomicAdd(&s.c[b], 1u);
+  if (w) atomicAdd((unsigned long long*)&s.m[b], (unsigned long long)w);
+}
+// Two bins of a thread and what lies above them.
+struct Bins {
+  uint32_t c[2], above_c;
+  uint64_t m[2], above_m;
+  uint64_t total_m;
+};
+// of the bins in s, complete; a barrier before and two within
+__device__ inline Bins scan_bins(Room& s) {
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  Bins b;
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    b.c[q] = s.c[2 * tid + q];
+    b.m[q] = s.m[2 * tid + q];
+  }
+  const uint32_t ic = (uint32_t)wave_incl_scan((int)(b.c[0] + b.c[1]));
+  const uint64_t im = incl_scan_u64(b.m[0] + b.m[1]);
+  if (lane == 63) {
+    s.wc[w] = ic;
+    s.wm[w] = im;
+  }
+  __syncthreads();
+  b.above_c = ic - b.c[0] - b.c[1];
+  b.above_m = im - b.m[0] - b.m[1];
+  b.total_m = 0;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) {
+    if (i < w) {
+      b.above_c += s.wc[i];
+      b.above_m += s.wm[i];
+    }
+    b.total_m += s.wm[i];
+  }
+  __syncthreads();
+  return b;
+}
+// The bin where the running count (or sum) reaches `want`, into s.
+__device__ inline void locate(Room& s, const Bins& b, bool by_count, uint64_t want) {
+  uint32_t c = b.above_c;
+  uint64_t m = b.above_m;
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const uint64_t at = by_count ? c : m, here = by_count ? b.c[q] : b.m[q];
+    if (at < want && want <= at + here) {
+      s.bin = 2 * (int)threadIdx.x + q;
+      s.above_c = c;
+      s.above_m = m;
+      s.in_c = b.c[q];
+    }
+    c += b.c[q];
+    m += b.m[q];
+  }
+  __syncthreads();
+}
+// The t-th token with this key, in the order of the indices.
+template <typename Row>
+__device__ int tie_index(const Row& row, Room& s, uint32_t key, uint32_t t) {
+  const int w = threadIdx.x >> 6;
+  uint32_t n = 0;
+  row.each([&](float x, int i, int) { n += bits(__ballot(i >= 0 && key_of(x) == key)); });
+  if ((threadIdx.x & 63) == 0) s.wc[w] = n;
+  if (threadIdx.x == 0) s.n = 0;
+  __syncthreads();
+  uint32_t before = 0;
+  for (int i = 0; i < w; ++i) before += s.wc[i];
+  if (before < t && t <= before + n)
+    row.each([&](float x, int i, int) {
+      const bool tie = i >= 0 && key_of(x) == key;
+      const uint64_t all = __ballot(tie);
+      if (tie && before + (uint32_t)below(all) + 1 == t) s.n = i;
+      before += bits(all);
+    });
+  __syncthreads();
+  const int at = s.n;
+  __syncthreads();
+  return at;
+}
+// The token in bin s.bin where the running count (or sum) reaches `want`: with few tokens in it each
+// finds its own rank among them; with more, bins of bins over the bits of the keys, at most
+// three times, until they are few or have one key.  `sum`: the running sum with it.
+template <typename Row>
+__device__ Cut refine(const Row& row, Room& s, const Rules& r, float top, int scale,
+                      bool by_count, uint64_t want, uint64_t& sum) {
+  const int tid = threadIdx.x, bin = s.bin;
+  uint32_t lo = 0, hi = 0xffffffffu;
+  auto member = [&](float x, int i) {
+    const uint32_t k = key_of(x);
+    return i >= 0 && k >= lo && k <= hi && bin_of(x, top, r) == bin;
+  };
+  for (bool first = true;; first = false) {
+    const uint32_t n = s.in_c, above_c = s.above_c;
+    const uint64_t above_m = s.above_m;
+    if (n <= NT) {
+      if (tid == 0) s.n = 0;
+      __syncthreads();
+      row.each([&](float x, int i, int) {
+        if (member(x, i)) {
+          const int at = atomicAdd(&s.n, 1);
+          s.lk[at] = key_of(x);
+          s.li[at] = i;
+          s.lw[at] = weight(x, top, r, scale);
+        }
+      });
+      __syncthreads();
+      if (tid < (int)n) {
+        const uint32_t k = s.lk[tid];
+        const int at = s.li[tid];
+        uint32_t rank = above_c;
+        uint64_t before = above_m;
+        for (int j = 0; j < (int)n; ++j) {
+          const uint32_t kj = s.lk[j];
+          const bool better = kj > k || (kj == k && s.li[j] < at);
+          rank += better ? 1 : 0;
+          before += better ? s.lw[j] : 0;
+        }
+        const uint64_t w = s.lw[tid];
+        if (by_count ? rank + 1 == (uint32_t)want : before < want && want <= before + w) {
+          s.cut = Cut{k, at};
+          s.sum = before + w;
+        }
+      }
+      __syncthreads();
+      const Cut c = s.cut;
+      sum = s.sum;
+      __syncthreads();
+      return c;
+    }
+    if (first) {
+      uint32_t a = 0xffffffffu, b = 0;
+      row.each([&](float x, int i, int) {
+        if (member(x, i)) {
+          a = min(a, key_of(x));
+          b = max(b, key_of(x));
+        }
+      });
+      a = wave_min_u32(a);
+      b = wave_max_u32(b);
+      if ((tid & 63) == 0) {
+        s.wc[tid >> 6] = a;
+        s.wx[tid >> 6] = b;
+      }
+      __syncthreads();
+      lo = 0xffffffffu;
+      hi = 0;
+      for (int i = 0; i < NW; ++i) {
+        lo = min(lo, s.wc[i]);
+        hi = max(hi, s.wx[i]);
+      }
+      __syncthreads();
+    }
+    if (lo == hi) {
+      const uint64_t w = weight(value_of(lo), top, r, scale);
+      // (by sums the bin's weight is not 0)
+      const uint64_t t = by_count ? want - above_c : (want - above_m + w - 1) / w;
+      sum = above_m + t * w;
+      return Cut{lo, tie_index(row, s, lo, (uint32_t)t)};
+    }
+    const int shift = max(0, 32 - __clz((int)(hi - lo)) - 11);
+    zero_bins(s);
+    __syncthreads();
+    row.each([&](float x, int i, int) {
+      if (member(x, i))
+        add_to_bin(s, NB - 1 - (int)((key_of(x) - lo) >> shift), weight(x, top, r, scale));
+    });
+    __syncthreads();
+    const Bins b = scan_bins(s);
+    locate(s, b, by_count, want - (by_count ? above_c : above_m));
+    const uint32_t base = lo + ((uint32_t)(NB - 1 - s.bin) << shift);
+    lo = base;
+    hi = min(hi, base + ((1u << shift) - 1));
+    __syncthreads();
+    if (tid == 0) {
+      s.above_c += above_c;
+      s.above_m += above_m;
+    }
+    __syncthreads();
+  }
+}
+// The cut of a row whose bins are in s.
+template <typename Row>
+__device__ Cut find_cut(const Row& row, Room& s, const Rules& r, float top, int scale) {
+  Cut c{0, 0x7fffffff};
+  if (!r.k && !(r.p < 1.)) return c;
+  const Bins b = scan_bins(s);
+  uint64_t sum = b.total_m, unused;
+  if (r.k) {
+    locate(s, b, true, (uint64_t)r.k);
+    c = refine(row, s, r, top, scale, true, (uint64_t)r.k, sum);
+  }
+  if (r.p < 1.) {
+    const uint64_t want = wanted(r.p, sum);
+    locate(s, b, false, want);
+    c = refine(row, s, r, top, scale, false, want, unused);
+  }
+  return c;
+}
+// The token of tokens [0, n): the first whose running sum of kept weights is above u times
+// their sum or (known) above `aim`.
+template <typename Row, int N>
+__device__ int draw(const Row& row, Room& s, const Rules& r, float top, int scale, const Cut& cut,
+                    float u, bool known, uint64_t aim) {
+  const int wid = threadIdx.x >> 6;
+  uint64_t w[N], mine = 0;
+  row.each([&](float x, int i, int j) {
+    const uint64_t y = i >= 0 && kept(cut, key_of(x), i) ? weight(x, top, r, scale) : 0;
+    w[j] = y >= r.m ? y : 0;
+    mine += w[j];
+  });
+  mine = sum_u64(mine);
+  if ((threadIdx.x & 63) == 0) s.wm[wid] = mine;
+  if (threadIdx.x == 0) s.n = -1;
+  __syncthreads();
+  uint64_t run = 0, total = 0;
+  for (int i = 0; i < NW; ++i) {
+    run += i < wid ? s.wm[i] : 0;
+    total += s.wm[i];
+  }
+  if (!known) aim = aim_of(u, total);
+  if (run <= aim && aim < run + mine) {
+    int token = -1;
+    row.each([&](float, int i, int j) {
+      const uint64_t at = incl_scan_u64(w[j]);
+      const uint64_t hit = __ballot(run + at > aim);
+      if (token < 0 && hit) token = __builtin_amdgcn_readlane(i, __ffsll((unsigned long long)hit) - 1);
+      run += lane_u64(at, 63);
+    });
+    if ((threadIdx.x & 63) == 0) s.n = token;
+  }
+  __syncthreads();
+  return s.n;
+}
+// the largest over a block; NaN where one is
+__device__ inline float block_top(Room& s, float x, bool nan) {
+  x = wave_max(x);
+  if (__any(nan)) x = NAN;
+  if ((threadIdx.x & 63) == 0) s.wc[threadIdx.x >> 6] = __float_as_uint(x);
+  __syncthreads();
+  float top = -INFINITY;
+  bool bad = false;
+  for (int i = 0; i < NW; ++i) {
+    const float y = __uint_as_float(s.wc[i]);
+    bad |= y != y;
+    top = fmaxf(top, y);
+  }
+  __syncthreads();
+  return bad ? NAN : top;
+}
+
+// ---- up to 16384 tokens: one block a row -------------------------------------------------------
+template <typename T, int N>
+__global__ __launch_bounds__(NT) void sample_block_kernel(SArgs g) {
+  __shared__ Room s;
+  const int64_t row = blockIdx.x;
+  const Held<T, N> x((const char*)g.x + row * g.st * (int64_t)sizeof(T), 0, g.V);
+  float m = -INFINITY;
+  bool nan = false;
+  x.each([&](float v, int, int) {
+    m = fmaxf(m, v);
+    nan |= v != v;
+  });
+  const float top = block_top(s, m, nan);
+  const Rules r = rules_of(g, row);
+  if (!(top > -INFINITY) || !r.good) {
+    if (threadIdx.x == 0) g.out[row] = -1;
+    return;
+  }
+  if (r.k || r.p < 1.) {
+    zero_bins(s);
+    __syncthreads();
+    x.each([&](float v, int i, int) {
+      if (i >= 0) add_to_bin(s, bin_of(v, top, r), weight(v, top, r, g.scale));
+    });
+    __syncthreads();
+  }
+  const Cut cut = find_cut(x, s, r, top, g.scale);
+  const int token = draw<Held<T, N>, N>(x, s, r, top, g.scale, cut, g.u[row], false, 0);
+  if (threadIdx.x == 0) g.out[row] = token;
+}
+
+// ---- more: parts of rows ------------------------------------------------------------------------
+__device__ inline float row_top(const SArgs& g, int64_t row) {
+  float m = -INFINITY;
+  bool nan = false;
+  for (int i = threadIdx.x & 63; i < g.parts; i += 64) {
+    const float x = g.pmax[row * g.parts + i];
+    m = fmaxf(m, x);
+    nan |= x != x;
+  }
+  m = wave_max(m);
+  return __any(nan) ? NAN : m;
+}
+template <typename T>
+__device__ inline Held<T, 16> part_of(const SArgs& g, int64_t row, int part) {
+  return Held<T, 16>((const char*)g.x + row * g.st * (int64_t)sizeof(T), (int64_t)part * PART,
+                     min(PART, g.V - part * PART));
+}
+template <typename T>
+__global__ __launch_bounds__(NT) void sample_top_kernel(SArgs g) {
+  __shared__ Room s;
+  const int64_t row = blockIdx.x / g.parts;
+  const int part = (int)(blockIdx.x - row * g.parts);
+  const Held<T, 16> x = part_of<T>(g, row, part);
+  float m = -INFINITY;
+  bool nan = false;
+  x.each([&](float v, int, int) {
+    m = fmaxf(m, v);
+    nan |= v != v;
+  });
+  const float top = block_top(s, m, nan);
+  if (threadIdx.x == 0) g.pmax[row * g.parts + part] = top;
+}
+template <typename T>
+__global__ __launch_bounds__(NT) void sample_bins_kernel(SArgs g) {
+  __shared__ Room s;
+  const int64_t row = blockIdx.x / g.parts;
+  const int part = (int)(blockIdx.x - row * g.parts);
+  const float top = row_top(g, row);
+  const Rules r = rules_of(g, row);
+  if (!(top > -INFINITY) || !r.good || (!r.k && !(r.p < 1.))) return;
+  const Held<T, 16> x = part_of<T>(g, row, part);
+  zero_bins(s);
+  __syncthreads();
+  x.each([&](float v, int i, int) {
+    if (i >= 0) add_to_bin(s, bin_of(v, top, r), weight(v, top, r, g.scale));
+  });
+  __syncthreads();
+  const int64_t at = (row * g.parts + part) * NB;
+  for (int i = threadIdx.x; i < NB; i += NT) {
+    g.hm[at + i] = s.m[i];
+    g.hc[at + i] = s.c[i];
+  }
+}
+template <typename T>
+__global__ __launch_bounds__(NT) void sample_cut_kernel(SArgs g) {
+  __shared__ Room s;
+  const int64_t row = blockIdx.x;
+  const float top = row_top(g, row);
+  const Rules r = rules_of(g, row);
+  if (!(top > -INFINITY) || !r.good) return;
+  if (r.k || r.p < 1.) {
+    for (int i = threadIdx.x; i < NB; i += NT) {
+      uint64_t m = 0;
+      uint32_t c = 0;
+      for (int part = 0; part < g.parts; ++part) {
+        const int64_t at = (row * g.parts + part) * NB + i;
+        m += g.hm[at];
+        c += g.hc[at];
+      }
+      s.m[i] = m;
+      s.c[i] = c;
+    }
+    __syncthreads();
+  }
+  const InMemory<T> x((const char*)g.x + row * g.st * (int64_t)sizeof(T), g.V);
+  const Cut c = find_cut(x, s, r, top, g.scale);
+  if (threadIdx.x == 0) g.cut[row] = int2{(int)c.key, c.index};
+}
+__device__ inline Cut cut_in(const SArgs& g, int64_t row, int part) {
+  const int2 c = g.cut[row];
+  return Cut{(uint32_t)c.x, c.y - part * PART};
+}
+template <typename T>
+__global__ __launch_bounds__(NT) void sample_mass_kernel(SArgs g) {
+  __shared__ uint64_t wm[NW];
+  const int64_t row = blockIdx.x / g.parts;
+  const int part = (int)(blockIdx.x - row * g.parts);
+  const float top = row_top(g, row);
+  const Rules r = rules_of(g, row);
+  if (!(top > -INFINITY) || !r.good) return;
+  const Cut cut = cut_in(g, row, part);
+  const Held<T, 16> x = part_of<T>(g, row, part);
+  uint64_t m = 0;
+  x.each([&](float v, int i, int) {
+    const uint64_t y = i >= 0 && kept(cut, key_of(v), i) ? weight(v, top, r, g.scale) : 0;
+    m += y >= r.m ? y : 0;
+  });
+  m = sum_u64(m);
+  if ((threadIdx.x & 63) == 0) wm[threadIdx.x >> 6] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    uint64_t all = 0;
+    for (int i = 0; i < NW; ++i) all += wm[i];
+    g.pmass[row * g.parts + part] = all;
+  }
+}
+template <typename T>
+__global__ __launch_bounds__(NT) void sample_pick_kernel(SArgs g) {
+  __shared__ Room s;
+  const int64_t row = blockIdx.x;
+  const float top = row_top(g, row);
+  const Rules r = rules_of(g, row);
+  if (!(top > -INFINITY) || !r.good) {
+    if (threadIdx.x == 0) g.out[row] = -1;
+    return;
+  }
+  const int lane = threadIdx.x & 63;
+  // (parts <= 64: 2^20 tokens)
+  const uint64_t m = lane < g.parts ? g.pmass[row * g.parts + lane] : 0;
+  const uint64_t at = incl_scan_u64(m);
+  const uint64_t aim = aim_of(g.u[row], lane_u64(at, 63));
+  const uint64_t hit = __ballot(at > aim);
+  const int part = __ffsll((unsigned long long)hit) - 1;
+  const uint64_t before = lane_u64(at - m, part);
+  const Held<T, 16> x = part_of<T>(g, row, part);
+  const int token = draw<Held<T, 16>, 16>(x, s, r, top, g.scale, cut_in(g, row, part), 0.f, true,
+                                          aim - before);
+  if (threadIdx.x == 0) g.out[row] = part * PART + token;
+}
+
+int parts_of(int vocab) { return vocab <= PART ? 0 : (vocab + PART - 1) / PART; }
+
+template <typename T>
+int run(const SArgs& g, hipStream_t s) {
+  if (g.V <= 1024) {
+    const dim3 grid(ceil_div(g.rows, 4)), block(256);
+    if (g.V <= 64)
+      hipLaunchKernelGGL((sample_wave_kernel<T, 1>), grid, block, 0, s, g);
+    else if (g.V <= 128)
+      hipLaunchKernelGGL((sample_wave_kernel<T, 2>), grid, block, 0, s, g);
+    else if (g.V <= 320)
+      hipLaunchKernelGGL((sample_wave_kernel<T, 5>), grid, block, 0, s, g);
+    else if (g.V <= 512)
+      hipLaunchKernelGGL((sample_wave_kernel<T, 8>), grid, block, 0, s, g);
+    else
+      hipLaunchKernelGGL((sample_wave_kernel<T, 16>), grid, block, 0, s, g);
+  } else if (g.V <= PART) {
+    const dim3 grid((unsigned)g.rows), block(NT);
+    if (g.V <= 4 * NT)
+      hipLaunchKernelGGL((sample_block_kernel<T, 4>), grid, block, 0, s, g);
+    else if (g.V <= 8 * NT)
+      hipLaunchKernelGGL((sample_block_kernel<T, 8>), grid, block, 0, s, g);
+    else
+      hipLaunchKernelGGL((sample_block_kernel<T, 16>), grid, block, 0, s, g);
+  } else {
+    const dim3 all((unsigned)(g.rows * g.parts)), one((unsigned)g.rows), block(NT);
+    hipLaunchKernelGGL((sample_top_kernel<T>), all, block, 0, s, g);
+    hipLaunchKernelGGL((sample_bins_kernel<T>), all, block, 0, s, g);
+    hipLaunchKernelGGL((sample_cut_kernel<T>), one, block, 0, s, g);
+    hipLaunchKernelGGL((sample_mass_kernel<T>), all, block, 0, s, g);
+    hipLaunchKernelGGL((sample_pick_kernel<T>), one, block, 0, s, g);
+  }
+  BLT_LAUNCH_CHECK("sample");
+  return 0;
+}
+
+}  // namespace
+
+int64_t sample_workspace_bytes(int64_t rows, int vocab) {
+  const int64_t parts = parts_of(vocab);
+  return parts ? rows * (parts * (12 * (int64_t)NB + 16) + 16) : 0;
+}
+
+int launch_sample(const SampleArgs& a, void* ws, hipStream_t s) {
+  SArgs g{};
+  g.x = a.logits; g.st = a.row_stride; g.rows = a.rows; g.V = a.vocab; g.u = a.uniform;
+  g.s = a.set; g.out = a.out;
+  int l = 0;
+  while (((int64_t)1 << l) < a.vocab) ++l;
+  g.scale = 62 - l;
+  g.parts = parts_of(a.vocab);
+  const int64_t n = a.rows * g.parts;
+  if (n > 0x7fffffff || a.rows > 0x7fffffff)
+    return fail(BLT_ERR_SHAPE, "fused_sample: too many rows");
+  if (g.parts) {
+    g.hm = (uint64_t*)ws;
+    g.pmass = g.hm + n * NB;
+    g.cut = (int2*)(g.pmass + n);
+    g.hc = (uint32_t*)(g.cut + a.rows);
+    g.pmax = (float*)(g.hc + n * NB);
+  }
+  return a.dtype == BLT_DTYPE_BF16 ? run<uint16_t>(g, s) : run<float>(g, s);
+}
+
+}  // namespace blt

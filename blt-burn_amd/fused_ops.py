@@ -15,8 +15,8 @@ from ._lib import EPS_AFTER_SQRT, EPS_INSIDE_SQRT, BltError, check
 from ._torch import call_on, contiguous, require_cuda, stream_ptr
 
 __all__ = ["fused_entropy", "fused_rms_norm", "fused_softmax", "fused_l2_norm",
-           "fused_silu_gate", "fused_coherence", "fused_attention", "fused_packed_attention",
-           "fused_packed_attention_backward", "RotaryPlan", "fused_rotary",
+           "fused_silu_gate", "fused_coherence", "fused_attention", "fused_sample",
+           "fused_packed_attention", "fused_packed_attention_backward", "RotaryPlan", "fused_rotary",
            "EPS_AFTER_SQRT", "EPS_INSIDE_SQRT"]
 
 
@@ -174,6 +174,70 @@ def fused_attention(q, k, v, use_causal_mask, window=0, rope_theta=0.0):
         float(rope_theta), ws.data_ptr() if ws is not None else 0, stream_ptr(qb.device)),
         "fused_attention")
     return o if in_dtype == torch.bfloat16 else o.to(in_dtype)
+
+
+def _row_setting(x, what, like, dtype, lo, hi):
+    """A number of all rows, or a tensor of one each: (number, pointer or None, what to keep)."""
+    if isinstance(x, torch.Tensor):
+        if x.dtype != dtype or x.device != like.device or x.shape != like.shape:
+            raise BltError("fused_sample: %s must be a number or %s %s on %s"
+                           % (what, dtype, tuple(like.shape), like.device))
+        x = contiguous(x)
+        return 0, x.data_ptr(), x
+    if not lo <= x <= hi:  # (here too: past 32 bits the call would see its low bits)
+        raise BltError("fused_sample: %s out of range (%r)" % (what, x))
+    return x, None, None
+
+
+def fused_sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None):
+    """One token a row of logits [..., vocab] (f32 or bf16, vocab up to 2^20), int32 [...], from
+    given random numbers uniform [...] (f32 in [0, 1)), beside fused_softmax and fused_entropy of
+    the same rows.
+
+    With tokens ranked by logit (descending, equal ones by index) and weights
+    e^((logit - max) / temperature), the tokens kept are those among the first top_k (0: all), whose running
+    sum of the ranks before them is below top_p times the sum of those (1: all), with a weight of at least
+    min_p; drawn is the lowest index whose running sum of kept weights, in the order of the indices,
+    is above uniform times their sum.  temperature 0 takes the first of the largest.  Each setting is a number
+    or a tensor like uniform (f32; top_k int32) of one for every row.
+
+    A logit of -inf is never drawn.  A row with a NaN, without a logit above -inf or with a setting
+    of its own out of range gives -1.  Weights are exact to 2^-42 of the largest or better, sums
+    of them exact: the same tokens in every run."""
+    require_cuda(logits, uniform)
+    _dtype_ok(logits)
+    if logits.dim() == 0 or not 1 <= logits.shape[-1] <= 1 << 20:
+        raise BltError("fused_sample expects logits [..., vocab], vocab 1 .. 2^20")
+    shape, V = logits.shape[:-1], logits.shape[-1]
+    if uniform.dtype != torch.float32 or uniform.shape != shape or uniform.device != logits.device:
+        raise BltError("fused_sample: uniform must be f32 %s on %s" % (tuple(shape), logits.device))
+    x = logits if logits.dim() == 2 and (logits.stride(1) == 1 or V == 1) and \
+        logits.stride(0) >= 0 else contiguous(logits)
+    u = contiguous(uniform)
+    big = float("inf")
+    t, tp, t_ = _row_setting(temperature, "temperature", u, torch.float32, 0, 1.7e308)
+    k, kp, k_ = _row_setting(top_k, "top_k", u, torch.int32, 0, big)
+    p, pp, p_ = _row_setting(top_p, "top_p", u, torch.float32, 5e-324, big)
+    m, mp, m_ = _row_setting(min_p, "min_p", u, torch.float32, 0, 1)
+    if out is None:
+        out = torch.empty(shape, dtype=torch.int32, device=x.device)
+    elif not isinstance(out, torch.Tensor):
+        raise TypeError("expected a torch.Tensor, got %r" % type(out))
+    elif out.dtype != torch.int32 or out.shape != shape or out.device != x.device or \
+            not out.is_contiguous():
+        raise BltError("fused_sample: out must be contiguous int32 %s on %s"
+                       % (tuple(shape), x.device))
+    rows, L, ws, size = u.numel(), _lib.lib(), None, 0
+    if V > 1024:
+        size = L.blt_fused_sample_workspace_bytes(rows, V)
+        if size:
+            ws = torch.empty(size, dtype=torch.uint8, device=x.device)
+    call_on(x.device, x.get_device(), L.blt_fused_sample, "fused_sample", x.data_ptr(),
+            x.stride(0) if x.dim() == 2 else V,
+            _lib.DTYPE_BF16 if x.dtype == torch.bfloat16 else _lib.DTYPE_F32, rows, V, u.data_ptr(),
+            t, tp, min(k, V), kp, p, pp, m, mp, out.data_ptr(), None if ws is None else ws.data_ptr(),
+            size)
+    return out
 
 
 def _packed_heads(t, what, like=None, heads=None):

@@ -131,6 +131,27 @@ int blt_fused_attention_f32(const float* q, const float* k, const float* v, floa
                             int64_t H, int64_t Tq, int64_t Tkv, int32_t d, int32_t causal,
                             blt_stream_t stream);
 
+/* One token a row of logits [rows, vocab] (row stride in elements, vocab up to 2^20) from the given
+ * random numbers uniform [rows] in [0, 1) (no counterpart in the reference, which answers with
+ * patches).  With tokens ranked by logit, descending, equal ones by index, and weights w =
+ * e^((logit - max) / temperature), the tokens kept are those among the first top_k ranks (0: all), whose
+ * running sum of the ranks before is below top_p times the sum of those (1 or more: all), with w >=
+ * min_p; the token is the lowest index whose running sum of kept weights, by index, is above
+ * uniform times their sum.  temperature 0: the first of the largest logits.  Each setting is that
+ * of all rows, or row r's in the device array beside it where that is not NULL.  A logit of -inf is
+ * never drawn; one of +inf takes everything with its like.  tokens: int32 [rows]; -1 for a row with a NaN,
+ * without a logit above -inf, or with a setting out of range (temperature >= 0 and finite, top_k >= 0,
+ * top_p > 0, min_p 0 .. 1).
+ * Weights are rounded to 2^(ceil(log2 vocab) - 63) of the largest and summed exactly: the same
+ * tokens in every run.  workspace: blt_fused_sample_workspace_bytes (0 up to vocab 16384), 16-byte
+ * aligned, no initialisation; calls that share one must be stream-ordered. */
+int64_t blt_fused_sample_workspace_bytes(int64_t rows, int32_t vocab);
+int blt_fused_sample(const void* logits, int64_t row_stride, int32_t dtype, int64_t rows,
+                     int32_t vocab, const float* uniform, double temperature,
+                     const float* temperatures, int32_t top_k, const int32_t* top_ks, double top_p,
+                     const float* top_ps, double min_p, const float* min_ps, int32_t* tokens,
+                     void* workspace, int64_t workspace_bytes, blt_stream_t stream);
+
 /* Attention of B whole sequences packed behind each other (no counterpart in the reference,
  * whose rows are one [B, H, T, d] shape): q, o [total, Hq, d] and k, v [total, Hkv, d] with
  * token and head strides in elements, unit d-stride; rows 16-byte aligned, token strides at
