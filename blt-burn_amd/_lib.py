@@ -72,6 +72,11 @@ EXPORTS = {
     "blt_paged_attention": (c_i32, [c_vp, c_i32] + [c_vp, c_i64, c_i64] * 2
                             + [c_i64, c_vp, c_vp, c_i64, c_i64, c_i32, c_i32, c_f32, c_vp, c_i64,
                                c_vp]),
+    "blt_cache_common_prefix": (c_i32, [c_vp, c_vp, c_i64, c_vp, c_vp]),
+    "blt_paged_attention_prefix_workspace_bytes": (c_i64, [c_vp, c_i64, c_i64, c_i64]),
+    "blt_paged_attention_prefix": (c_i32, [c_vp, c_i32] + [c_vp, c_i64, c_i64] * 2
+                                   + [c_i64, c_vp, c_vp, c_i64, c_i64, c_i32, c_f32, c_vp, c_vp,
+                                      c_i64, c_vp]),
     "blt_patch_boundaries": (c_i32, [c_vp, c_i64, c_i64, c_f32, c_i32, c_vp, c_vp, c_vp, c_vp,
                                      c_vp]),
     "blt_patch_mask_starts": (c_i32, [c_vp, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp]),

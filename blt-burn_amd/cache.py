@@ -45,8 +45,8 @@ class PagedCache:
 
     Beside them a cache keeps the workspace of its attention calls, as large as the calls
     so far have needed: at most 35 MB for single tokens, 104 MB (head_dim 64) or 136 MB (128)
-    for any call, and up to a third more where it has grown.  The first call of a size may
-    allocate."""
+    for any call, and up to a third more where it has grown; a call with a prefix takes 4
+    (head_dim + 2) bytes more for every token and head.  The first call of a size may allocate."""
 
     def __init__(self, n_layers, n_kv_heads, head_dim, num_pages, max_seqs, max_len, page_size=16,
                  dtype=torch.bfloat16, device=None):
@@ -106,15 +106,18 @@ class PagedCache:
         self._ws_most = max(self._lib.blt_paged_attention_workspace_bytes(
             self._ptr, 65536, 65536 * rows, self.n_kv_heads) for rows in (1, 32, 128))
 
-    def _room(self, rows, total, heads):
-        """Workspace for attention calls of this size.  It grows by steps of four or more and
-        never past the largest call's; what it was before stays, for the graphs that use it."""
-        need = self._lib.blt_paged_attention_workspace_bytes(self._ptr, rows, total, heads)
+    def _room(self, rows, total, heads, prefix):
+        """Workspace for attention calls of this size.  It grows by steps of four or more and, but
+        for calls with a prefix, never past the largest call's; what it was before stays, for the
+        graphs that use it."""
+        f = (self._lib.blt_paged_attention_prefix_workspace_bytes if prefix
+             else self._lib.blt_paged_attention_workspace_bytes)
+        need = f(self._ptr, rows, total, heads)
         if need > self._ws_bytes:
             size = max(need, min(4 * self._ws_bytes, self._ws_most))
             self._ws.append(self._workspace(size))
             self._wsp, self._ws_bytes = self._ws[-1].data_ptr(), size
-        self._ws_for = (rows, total, heads)
+        self._ws_for = (rows, total, heads, prefix)
 
     def record_stream(self, stream):
         """Tensor.record_stream for everything the cache holds: for a cache that is dropped
@@ -264,7 +267,21 @@ class PagedCache:
                    vh, qp, qs, qh, op, os_, oh, Hq, p, s, B, total, r)
         return out
 
-    def attention(self, layer, q, starts, seqs=None, causal=True, window=0, scale=None, out=None):
+    def common_prefix(self, seqs=None, out=None):
+        """Tokens that the listed sequences (None: all) have in common, as an int32 [1] tensor
+        of the device (`out` if given): the leading whole pages that are the same pages, as fork
+        leaves them.  Sequences without tokens are left out; 0 with fewer than two.  For attention's
+        `prefix`: it stays right for all layers and steps until one of these sequences is
+        cut, dropped or replaced, or pages are moved."""
+        s, n = (None, self.max_seqs) if seqs is None else self._list(seqs, "seqs")
+        if out is None:
+            out = torch.empty(1, dtype=torch.int32, device=self.device)
+        p = self._list(out, "out", 1)[0]
+        self._call(self._lib.blt_cache_common_prefix, "cache_common_prefix", self._ptr, s, n, p)
+        return out
+
+    def attention(self, layer, q, starts, seqs=None, causal=True, window=0, scale=None, out=None,
+                  prefix=None):
         """Attention of new tokens q [total, heads, head_dim] over a layer of the cache,
         whose lengths already count them (rows as in append; a sequence may appear twice):
         the last of a row's n tokens sits at its sequence's last position.  Query head h
@@ -280,7 +297,12 @@ class PagedCache:
         than 32 tokens on average (heads per key head counted as tokens), and to 2^-15 of
         them below.  That average also chooses the kernel, so a long chunk is best issued
         apart from many single tokens; and calls of more than some hundred rows are best cut
-        into several (a call's cost has a part that grows with the square of its rows)."""
+        into several (a call's cost has a part that grows with the square of its rows).
+
+        prefix: what common_prefix said of a list that holds these sequences.  The keys that they
+        share are then read once for all rows, which pays where several rows have a long
+        prefix; the outputs are those without it, up to their rounding.  (It is not used with a
+        window, whose rows do not see all of it.)"""
         layer = self._layer(layer)
         q, qp, total, H, qs, qh = self._tokens(q, "q")
         p, B, s = self._rows(starts, seqs)
@@ -292,12 +314,22 @@ class PagedCache:
             qs, qh, _ = q.stride()
             qp = q.data_ptr()
         out, op, os_, oh = self._output(out, q, total, H)
-        if self._ws_for != (B, total, H):
-            self._room(B, total, H)
         if window < 0:
             raise BltError("PagedCache.attention: window must be >= 0")
         if window > 0x7fffffff:  # longer than any sequence
             window = 0
+        share = None
+        if prefix is not None:
+            share = self._list(prefix, "prefix", 1)[0]
+            if causal and window:
+                share = None
+        if self._ws_for != (B, total, H, share is not None):
+            self._room(B, total, H, share is not None)
+        if share is not None:
+            self._call(self._lib.blt_paged_attention_prefix, "paged_attention", self._ptr, layer, qp,
+                       qs, qh, op, os_, oh, H, p, s, B, total, 1 if causal else 0,
+                       self._scale if scale is None else scale, share, self._wsp, self._ws_bytes)
+            return out
         self._call(self._lib.blt_paged_attention, "paged_attention", self._ptr, layer, qp, qs, qh, op,
                    os_, oh, H, p, s, B, total, 1 if causal else 0, window,
                    self._scale if scale is None else scale, self._wsp, self._ws_bytes)

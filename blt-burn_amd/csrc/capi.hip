@@ -629,19 +629,27 @@ int blt_cache_append(const blt_paged_cache* cache, int32_t layer, const void* k,
   return launch_append(*cache, a, STREAM(stream));
 }
 
-int64_t blt_paged_attention_workspace_bytes(const blt_paged_cache* cache, int64_t B, int64_t total,
-                                            int64_t Hq) {
+static int64_t attention_bytes(const blt_paged_cache* cache, int64_t B, int64_t total, int64_t Hq,
+                               bool prefix) {
   // (0 for what blt_paged_attention refuses)
   if (cache_checks(cache, "paged_attention_workspace_bytes") || Hq < 0 || Hq > 0xffff || B < 0 ||
       B > 65536 || total < 0 || total > 0x7fffffff)
     return 0;
-  return paged_attention_workspace_bytes(*cache, B, total, (int)Hq);
+  return paged_attention_workspace_bytes(*cache, B, total, (int)Hq, prefix);
 }
-int blt_paged_attention(const blt_paged_cache* cache, int32_t layer, const void* q, int64_t st_q,
+int64_t blt_paged_attention_workspace_bytes(const blt_paged_cache* cache, int64_t B, int64_t total,
+                                            int64_t Hq) {
+  return attention_bytes(cache, B, total, Hq, false);
+}
+int64_t blt_paged_attention_prefix_workspace_bytes(const blt_paged_cache* cache, int64_t B,
+                                                   int64_t total, int64_t Hq) {
+  return attention_bytes(cache, B, total, Hq, true);
+}
+static int attention(const blt_paged_cache* cache, int32_t layer, const void* q, int64_t st_q,
                         int64_t sh_q, void* o, int64_t st_o, int64_t sh_o, int64_t Hq,
                         const int32_t* starts, const int32_t* seqs, int64_t B, int64_t total,
-                        int32_t causal, int32_t window, float scale, void* workspace,
-                        int64_t workspace_bytes, blt_stream_t stream) {
+                        int32_t causal, int32_t window, float scale, const int32_t* prefix,
+                        void* workspace, int64_t workspace_bytes, blt_stream_t stream) {
   if (int rc = cache_checks(cache, "paged_attention")) return rc;
   if (int rc = chunk_checks(cache, layer, Hq, starts, B, total, "paged_attention")) return rc;
   if (Hq < 1 || Hq % cache->n_kv_heads)
@@ -656,14 +664,40 @@ int blt_paged_attention(const blt_paged_cache* cache, int32_t layer, const void*
   const int64_t v = cache->dtype == BLT_DTYPE_BF16 ? 8 : 4;
   if (((uintptr_t)q & 15) || ((uintptr_t)o & 15) || st_q % v || sh_q % v || st_o % v || sh_o % v)
     return fail(BLT_ERR_SHAPE, "paged_attention: q and o need 16-byte aligned rows");
-  const int64_t need = paged_attention_workspace_bytes(*cache, B, total, (int)Hq);
+  const int64_t need = paged_attention_workspace_bytes(*cache, B, total, (int)Hq, prefix);
   if (need > 0 && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need))
     return fail(BLT_ERR_INVALID, "paged_attention: workspace missing, misaligned or too small");
   PagedAttnArgs a{};
   a.q = q; a.o = o; a.st_q = st_q; a.sh_q = sh_q; a.st_o = st_o; a.sh_o = sh_o;
   a.H = (int)Hq; a.starts = starts; a.seqs = seqs; a.B = B; a.total = total;
   a.layer = layer; a.causal = causal ? 1 : 0; a.window = window; a.scale = scale;
+  a.prefix = prefix;
   return launch_paged_attention(*cache, a, workspace, STREAM(stream));
+}
+int blt_paged_attention(const blt_paged_cache* cache, int32_t layer, const void* q, int64_t st_q,
+                        int64_t sh_q, void* o, int64_t st_o, int64_t sh_o, int64_t Hq,
+                        const int32_t* starts, const int32_t* seqs, int64_t B, int64_t total,
+                        int32_t causal, int32_t window, float scale, void* workspace,
+                        int64_t workspace_bytes, blt_stream_t stream) {
+  return attention(cache, layer, q, st_q, sh_q, o, st_o, sh_o, Hq, starts, seqs, B, total, causal,
+                   window, scale, nullptr, workspace, workspace_bytes, stream);
+}
+int blt_paged_attention_prefix(const blt_paged_cache* cache, int32_t layer, const void* q,
+                               int64_t st_q, int64_t sh_q, void* o, int64_t st_o, int64_t sh_o,
+                               int64_t Hq, const int32_t* starts, const int32_t* seqs, int64_t B,
+                               int64_t total, int32_t causal, float scale, const int32_t* prefix,
+                               void* workspace, int64_t workspace_bytes, blt_stream_t stream) {
+  if (!prefix) return fail(BLT_ERR_INVALID, "paged_attention_prefix: null prefix");
+  return attention(cache, layer, q, st_q, sh_q, o, st_o, sh_o, Hq, starts, seqs, B, total, causal,
+                   0, scale, prefix, workspace, workspace_bytes, stream);
+}
+int blt_cache_common_prefix(const blt_paged_cache* cache, const int32_t* seqs, int64_t n,
+                            int32_t* tokens, blt_stream_t stream) {
+  if (int rc = cache_checks(cache, "cache_common_prefix")) return rc;
+  if (n < 0 || n > 65536 || (!seqs && n > cache->max_seqs))
+    return fail(BLT_ERR_SHAPE, "cache_common_prefix: more entries than sequences, or than 65536");
+  if (!tokens) return fail(BLT_ERR_INVALID, "cache_common_prefix: null pointer");
+  return launch_cache_common_prefix(*cache, seqs, n, tokens, STREAM(stream));
 }
 
 // ---- patcher -----------------------------------------------------------------

@@ -13,6 +13,12 @@
 // only bounds the grid: items <= row tiles + the blocks that are to be filled (2 * resident,
 // where find_item spills 4 * resident), parts in need of joining <= twice those blocks (every
 // one of them has more than half of C).
+//
+// A prefix that all sequences share (the same pages) is read once for all of them, in two
+// launches of the same kernels: PREFIX takes the tokens of all sequences as the rows of one, over
+// the keys of the prefix, which they all see whole, and leaves their unnormalised outputs,
+// maxima and sums in memory; TAILS takes each sequence's keys from there on and joins the two.
+#include <algorithm>
 #include <type_traits>
 
 #include "attn_tiles.hpp"
@@ -21,6 +27,8 @@
 namespace blt {
 
 namespace {
+
+enum Mode { WHOLE, PREFIX, TAILS };
 
 struct KArgs {
   const void *q, *k, *v;  // k, v: the layer's first element
@@ -38,6 +46,9 @@ struct KArgs {
   int32_t* status;
   float* part;    // [slots][rows of a tile][D], unnormalised outputs
   float* ml;      // [slots][rows of a tile][2], their max (before the scale) and sum
+  const int32_t* prefix;  // tokens that all sequences share
+  float* pre_o;           // [total][heads][D] and [total][heads][2], as part and ml, of the prefix
+  float* pre_ml;
 };
 
 // ---- which item ----------------------------------------------------------------
@@ -64,9 +75,9 @@ __device__ inline Seq seq_at(const KArgs& p, int b, bool& lost, bool& crossed) {
 }
 // row tiles of a sequence, and the key tiles one of them may have to read
 template <int BQ, int BKV>
-__device__ inline void tiles_of(const KArgs& p, const Seq& q, int& nrt, int& kt) {
+__device__ inline void tiles_of(const KArgs& p, const Seq& q, int from, int& nrt, int& kt) {
   nrt = (int)(((uint32_t)(q.n * p.G) + BQ - 1) / BQ);
-  kt = (int)(((uint32_t)q.len + BKV - 1) / BKV);
+  kt = (int)(((uint32_t)q.len + BKV - 1) / BKV) - from / BKV;
   if (p.window) {
     const int tokens = q.n < p.tokens_max ? q.n : p.tokens_max;
     const int most = (int)((uint32_t)(p.window + tokens + BKV - 2) / BKV) + 1;
@@ -79,6 +90,7 @@ struct Item {
   int kvh, rt, split, ns;  // key head, row tile, part and number of parts
   int nrt;                 // row tiles of the sequence
   int pslot, join;         // first partial slot and first counter of its row tiles
+  int from;                // first key (0, or TAILS: the first that is not shared)
 };
 __device__ inline int lane_of(int v, int l) { return __builtin_amdgcn_readlane(v, l); }
 
@@ -87,16 +99,37 @@ __device__ inline int lane_of(int v, int l) { return __builtin_amdgcn_readlane(v
 // rows: single tokens over up to 200 keys, 12 heads, 64 of them 10 us, 256 50, 1024 406,
 // 4096 5200.)  Every wave computes it by itself, in
 // the same order, so all agree.
-template <int BQ, int BKV>
+template <int BQ, int BKV, int MODE>
 __device__ bool find_item(const KArgs& p, unsigned bid, Item& it) {
   const int lane = threadIdx.x & 63;
+  const int B = MODE == PREFIX ? 1 : p.B;
   Seq q;
-  int nrt, kt;
+  int nrt, kt, from = 0;
   float work = 0.f, tiles = 0.f, longest = 0.f;
   bool lost = false, crossed = false;
-  for (int b0 = 0; b0 < p.B; b0 += 64) {
-    q = seq_at(p, b0 + lane, lost, crossed);
-    tiles_of<BQ, BKV>(p, q, nrt, kt);
+  if constexpr (MODE != WHOLE) {
+    // the shared keys, whole pages, as far as they lie before every row's tokens (so that all
+    // see all of them, whatever `prefix` says), and a sequence that has them
+    int room = 0x7fffffff, slot = -1;
+    for (int b0 = 0; b0 < p.B; b0 += 64) {
+      q = seq_at(p, b0 + lane, lost, crossed);
+      if (q.n) room = min(room, q.len - q.n);
+      const uint64_t any = __ballot(q.n > 0);
+      if (slot < 0 && any) slot = lane_of(q.slot, __ffsll((unsigned long long)any) - 1);
+    }
+    room = min(p.prefix[0], -wave_max_i32(-room));
+    from = __builtin_amdgcn_readfirstlane(room > 0 ? room >> p.lps << p.lps : 0);
+    if constexpr (MODE == PREFIX) {
+      if (__any(crossed) || slot < 0) return false;  // (TAILS reports it)
+      const int a = p.starts[0], e = p.starts[p.B];
+      q = lane == 0 ? Seq{a, e - a, from, slot} : Seq{0, 0, 0, 0};
+      from = 0;
+      lost = false;
+    }
+  }
+  for (int b0 = 0; b0 < B; b0 += 64) {
+    if (MODE == WHOLE || B > 64) q = seq_at(p, b0 + lane, lost, crossed);
+    tiles_of<BQ, BKV>(p, q, from, nrt, kt);
     work += (float)nrt * (float)kt;
     longest = fmaxf(longest, nrt ? (float)kt : 0.f);
     tiles += (float)nrt;
@@ -146,10 +179,10 @@ __device__ bool find_item(const KArgs& p, unsigned bid, Item& it) {
   int items, inc;  // of all sequences; with up to 64 of them, those up to the lane's own
   for (int tries = 0;; ++tries) {
     items = 0;
-    for (int b0 = 0; b0 < p.B; b0 += 64) {
-      if (p.B > 64) {
+    for (int b0 = 0; b0 < B; b0 += 64) {
+      if (B > 64) {
         q = seq_at(p, b0 + lane, lost, crossed);
-        tiles_of<BQ, BKV>(p, q, nrt, kt);
+        tiles_of<BQ, BKV>(p, q, from, nrt, kt);
       }
       parts_of();
       items += nrt * ns;
@@ -165,10 +198,10 @@ __device__ bool find_item(const KArgs& p, unsigned bid, Item& it) {
   // partial slots, and counters above them: at most 8192 and 2048 of a call
   auto joined = [&]() { return ns > 1 ? nrt * ns + (nrt << 16) : 0; };
   int join = 0;
-  for (int b0 = 0; b0 < p.B; b0 += 64) {
-    if (p.B > 64) {
+  for (int b0 = 0; b0 < B; b0 += 64) {
+    if (B > 64) {
       q = seq_at(p, b0 + lane, lost, crossed);
-      tiles_of<BQ, BKV>(p, q, nrt, kt);
+      tiles_of<BQ, BKV>(p, q, from, nrt, kt);
       parts_of();
     }
     join += joined();
@@ -181,10 +214,10 @@ __device__ bool find_item(const KArgs& p, unsigned bid, Item& it) {
   it.kvh = (int)((uint32_t)id / (uint32_t)items);
   const int rem = id - it.kvh * items;
   int base = 0, jbase = 0;
-  for (int b0 = 0; b0 < p.B; b0 += 64) {
-    if (p.B > 64) {
+  for (int b0 = 0; b0 < B; b0 += 64) {
+    if (B > 64) {
       q = seq_at(p, b0 + lane, lost, crossed);
-      tiles_of<BQ, BKV>(p, q, nrt, kt);
+      tiles_of<BQ, BKV>(p, q, from, nrt, kt);
       parts_of();
       join = joined();
       inc = wave_incl_scan(nrt * ns);
@@ -194,6 +227,7 @@ __device__ bool find_item(const KArgs& p, unsigned bid, Item& it) {
     if (above) {
       const int l = __ffsll((unsigned long long)above) - 1;
       it.q = Seq{lane_of(q.s0, l), lane_of(q.n, l), lane_of(q.len, l), lane_of(q.slot, l)};
+      it.from = from;
       it.nrt = lane_of(nrt, l);
       it.ns = lane_of(ns, l);
       const int before = jbase + lane_of(jinc - join, l);
@@ -220,10 +254,12 @@ __device__ inline int64_t slot_of(const Item& it, int split) {
 }
 
 // The keys rows r0 .. r1 (of one sequence) see between them: [lo, hi].
-__device__ inline void key_range(const KArgs& p, const Seq& q, int r0, int r1, int& lo, int& hi) {
+__device__ inline void key_range(const KArgs& p, const Item& it, int r0, int r1, int& lo,
+                                 int& hi) {
+  const Seq& q = it.q;
   const int first = q.len - q.n;  // position of token 0
   hi = q.len - 1;
-  lo = 0;
+  lo = it.from;
   if (p.causal) {
     const int last = first + over(r1, p.by_g);
     hi = last < hi ? last : hi;
@@ -313,7 +349,26 @@ __device__ inline void join(Joined& a, const Joined& b, float c) {
   a.l = fmaf(a.l, wa, wb * b.l);
   a.o = a.o * wa + wb * b.o;
 }
-template <int D, int BQ, int NT, typename T>
+// Four columns of a row of head `head`: PREFIX leaves them for TAILS (true: nothing more to do),
+// which takes them up.
+template <int D, int MODE>
+__device__ inline bool shared_part(const KArgs& p, int token, int head, int dd, Joined& a) {
+  if constexpr (MODE == WHOLE) return false;
+  const int64_t at = (int64_t)token * (p.Hkv * p.G) + head;
+  f32x4_t* o = reinterpret_cast<f32x4_t*>(p.pre_o + at * D + dd);
+  float* ml = p.pre_ml + at * 2;
+  if constexpr (MODE == PREFIX) {
+    *o = a.o;
+    if (dd == 0) {
+      ml[0] = a.m;
+      ml[1] = a.l;
+    }
+    return true;
+  }
+  join(a, Joined{ml[0], ml[1], *o}, p.c);
+  return false;
+}
+template <int D, int BQ, int NT, typename T, int MODE>
 __device__ void join_parts(const KArgs& p, const Item& it, int nr, float* room) {
   if (!last_part(p, it)) return;
   // U parts at a time, everything of them in flight at once (a read that passes the L2 takes
@@ -366,9 +421,10 @@ __device__ void join_parts(const KArgs& p, const Item& it, int nr, float* room) 
     const float all = (a.o.x + a.o.y) + (a.o.z + a.o.w) + a.l;
     return all == all ? a : sum(i, x0, x1, at_once, std::true_type{});
   };
-  auto store = [&](int i, const Joined& a) {
+  auto store = [&](int i, Joined a) {
     const int r = i / (D / 4), dd = (i % (D / 4)) * 4;
     const int row = it.rt * BQ + r, t = over(row, p.by_g), g = row - t * p.G;
+    if (shared_part<D, MODE>(p, it.q.s0 + t, it.kvh * p.G + g, dd, a)) return;
     const int64_t at =
         (int64_t)(it.q.s0 + t) * p.st_o + (int64_t)(it.kvh * p.G + g) * p.sh_o + dd;
     const f32x4_t x = a.l == 0.f ? f32x4_t{0.f, 0.f, 0.f, 0.f} : a.o / a.l;
@@ -410,10 +466,10 @@ __device__ void join_parts(const KArgs& p, const Item& it, int nr, float* room) 
 // laid out as the threads hold it, [D / 4][256] pairs, so that whole lines are written and
 // read: the last block's threads take up the values of their own rows.  (By rows, with every
 // lane's 16 bytes in another line, 4 chunks of 512 over 4096 keys, 12 heads, took 64 us
-// instead of 53.)  False where the thread has nothing to store; else o, total are the row's.
+// instead of 53.)  False where the thread has nothing to store; else o, m, total are the row's.
 template <int D>
 __device__ inline bool join_tiles(const KArgs& p, const Item& it, bool active,
-                                  f32x16_t (&o)[D / 32], float m, float& total) {
+                                  f32x16_t (&o)[D / 32], float& m, float& total) {
   constexpr int BQ = 128, PAIRS = D / 4;
   const int tid = threadIdx.x, trow = (tid >> 6) * 32 + (tid & 31);
   if (active) {
@@ -462,7 +518,49 @@ __device__ inline bool join_tiles(const KArgs& p, const Item& it, bool active,
         for (int k = 0; k < D / 2; ++k) o[k >> 4][k & 15] = fmaf(w, v[u][k], o[k >> 4][k & 15]);
       }
   }
+  m = mx;
   return true;
+}
+
+// As shared_part, a row in the accumulators' layout: of bf16's form for 128 rows, or of f32's.
+template <int D, int MODE, bool F32>
+__device__ inline bool shared_row(const KArgs& p, int token, int head, int half, float m,
+                                  float& total, f32x16_t (&o)[D / 32]) {
+  if constexpr (MODE == WHOLE) return false;
+  const int64_t at = (int64_t)token * (p.Hkv * p.G) + head;
+  float* to = p.pre_o + at * D;
+  float* ml = p.pre_ml + at * 2;
+  auto col = [&](int j) { return F32 ? 4 * (8 * (j >> 2) + 4 * half + (j & 3)) : 8 * j + 4 * half; };
+  if constexpr (MODE == PREFIX) {
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j) {
+      f32x4_t x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = F32 ? o[e & (D / 32 - 1)][j & 15] : o[j >> 2][4 * (j & 3) + e];
+      *reinterpret_cast<f32x4_t*>(to + col(j)) = x;
+    }
+    if (half == 0) {
+      ml[0] = m;
+      ml[1] = total;
+    }
+    return true;
+  }
+  const float pm = ml[0], mx = fmaxf(m, pm), off = mx == -INFINITY ? 0.f : mx;
+  const float wa = __builtin_amdgcn_exp2f((m - off) * p.c);
+  const float wb = __builtin_amdgcn_exp2f((pm - off) * p.c);
+  total = fmaf(total, wa, wb * ml[1]);
+#pragma unroll
+  for (int j = 0; j < D / 8; ++j) {
+    const f32x4_t x = *reinterpret_cast<const f32x4_t*>(to + col(j));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (F32)
+        o[e & (D / 32 - 1)][j & 15] = fmaf(o[e & (D / 32 - 1)][j & 15], wa, wb * x[e]);
+      else
+        o[j >> 2][4 * (j & 3) + e] = fmaf(o[j >> 2][4 * (j & 3) + e], wa, wb * x[e]);
+    }
+  }
+  return false;
 }
 
 // ---- bf16, tiles of rows ---------------------------------------------------------
@@ -480,7 +578,7 @@ __device__ inline bool join_tiles(const KArgs& p, const Item& it, bool active,
 // 1.0 PFLOP/s of the visible pairs (an 8192^3 library product reaches 1.4); the matrix cores
 // are busy 46 % of the time and the vector units 43 %, hardly ever both.  With 64 rows a wave
 // (1.2 ms for 0.96 then), three stages, or 32-key tiles at three waves a SIMD it was slower.
-template <int D, int NST>
+template <int D, int NST, int MODE>
 __global__ __launch_bounds__(256, 2) void paged_attn_kernel(KArgs p) {
   constexpr int BKV = 64, QPW = 32, BQ = 4 * QPW;
   constexpr int TILE = BKV * D;        // elements of a K (or V) tile
@@ -491,7 +589,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(KArgs p) {
   __shared__ int ptab[PT];
 
   Item it;
-  if (!find_item<BQ, BKV>(p, blockIdx.x, it)) return;
+  if (!find_item<BQ, BKV, MODE>(p, blockIdx.x, it)) return;
   const Seq& sq = it.q;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -502,7 +600,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(KArgs p) {
   // the block's key tiles [t0, t1)
   int lo, hi;
   const int r0 = it.rt * BQ, r1 = min(r0 + BQ, rows) - 1;
-  key_range(p, sq, r0, r1, lo, hi);
+  key_range(p, it, r0, r1, lo, hi);
   const int t_lo = lo / BKV, cnt = hi < 0 ? 0 : hi / BKV - t_lo + 1;
   int t0, t1;
   part_of(it, t_lo, cnt, t0, t1);
@@ -511,9 +609,9 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(KArgs p) {
   const bool wave_active = rw < rows;
   int wlo = 0, whi = -1;
   const int rwl = min(rw + QPW, rows) - 1;
-  if (wave_active) key_range(p, sq, rw, rwl, wlo, whi);
+  if (wave_active) key_range(p, it, rw, rwl, wlo, whi);
   const int pos_first = first + over(rw, p.by_g);  // lowest position in the wave
-  const int lo_last = p.window ? first + over(rwl, p.by_g) - p.window + 1 : 0;  // highest lower bound
+  const int lo_last = p.window ? first + over(rwl, p.by_g) - p.window + 1 : it.from;  // highest lower bound
 
   // Q fragments (B operand): row rw + lrow, d = 16 ks + 8 lhalf .. + 8
   bf16x8_t qf[KS];
@@ -529,7 +627,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(KArgs p) {
   }
   // the row's visible keys
   const int khi = p.causal ? min(first + tok, sq.len - 1) : sq.len - 1;
-  const int klo = p.window ? first + tok - p.window + 1 : 0;
+  const int klo = p.window ? first + tok - p.window + 1 : it.from;
   int wbase = (t0 * BKV) >> p.lps;
   if (t0 < t1) stage_pages(p, sq, wbase, ptab, tid, 256);
   // consumed here, before any DMA is in flight (see attn_fwd_kernel)
@@ -616,7 +714,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(KArgs p) {
       const uint16_t* sv = sk + TILE;
       const bool mask_hi = kb + BKV - 1 > (p.causal ? pos_first : sq.len - 1) ||
                            kb + BKV > sq.len;
-      const bool mask_lo = p.window && kb < lo_last;
+      const bool mask_lo = kb < lo_last;
       // All of K's fragments are read before the first product and all of V's under the
       // softmax: against that, 2 chunks over up to 16384 keys (d = 128) take 4 % longer with
       // V's read between the products of the second, 85 % with K's among those of the first.
@@ -756,6 +854,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(KArgs p) {
   float total = lt;
   if (it.ns > 1 && !join_tiles<D>(p, it, wave_active, o, m, total)) return;
   if (row < rows) {
+    if (shared_row<D, MODE, false>(p, sq.s0 + tok, head, lhalf, m, total, o)) return;
     uint16_t* orow = (uint16_t*)p.o + (int64_t)(sq.s0 + tok) * p.st_o + (int64_t)head * p.sh_o;
     // hardware reciprocal (1 ulp): the output is rounded to bf16
     const float inv = total > 0.f ? __builtin_amdgcn_rcpf(total) : total == total ? 0.f : total;
@@ -791,7 +890,7 @@ template <int N>
 __device__ inline void wait_loads() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
-template <int D, int NR, int NW>
+template <int D, int NR, int NW, int MODE>
 __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(KArgs p) {
   constexpr int KT = 32, BKV = 64, BQ = 16 * NR, TILE = KT * D, NST = 2;
   constexpr int OPS = 4 * (D / 64);  // DMA instructions of a K (or V) tile
@@ -803,7 +902,7 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(KArgs p) {
   __shared__ int ptab[PTF];
 
   Item it;
-  if (!find_item<BQ, BKV>(p, blockIdx.x, it)) return;
+  if (!find_item<BQ, BKV, MODE>(p, blockIdx.x, it)) return;
   const Seq& sq = it.q;
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -811,7 +910,7 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(KArgs p) {
   const int rows = sq.n * p.G, first = sq.len - sq.n;
   const int r0 = it.rt * BQ, r1 = min(r0 + BQ, rows) - 1;
   int lo, hi;
-  key_range(p, sq, r0, r1, lo, hi);
+  key_range(p, it, r0, r1, lo, hi);
   // the item's key tiles [t0, t1), of 32 keys here
   const int t_lo = lo / KT, cnt = hi < 0 ? 0 : hi / KT - t_lo + 1;
   int t0, t1;
@@ -830,11 +929,11 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(KArgs p) {
       qf[n][ks] = __builtin_bit_cast(
           bf16x8_t, *reinterpret_cast<const u32x4_t*>(qrow + ks * 32 + g4 * 8));
     khi[n] = p.causal ? min(first + t, sq.len - 1) : sq.len - 1;
-    klo[n] = p.window ? first + t - p.window + 1 : 0;
+    klo[n] = p.window ? first + t - p.window + 1 : it.from;
   }
   // every row sees [all_lo, all_hi]
   const int all_hi = p.causal ? min(first + over(r0, p.by_g), sq.len - 1) : sq.len - 1;
-  const int all_lo = p.window ? first + over(r1, p.by_g) - p.window + 1 : 0;
+  const int all_lo = p.window ? first + over(r1, p.by_g) - p.window + 1 : it.from;
 
   // DMA of one tile: eight keys (one page) at a time, chunks swizzled for the operand reads
   const unsigned ring = (unsigned)(uintptr_t)lds + (unsigned)(w * NST * 2 * TILE * 2);
@@ -1105,6 +1204,12 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(KArgs p) {
       if (dd == 0) put2(p.ml + (at + r) * 2, mx, lt);
     } else {
       const int t = over(r0 + r, p.by_g), g = (r0 + r) - t * p.G;
+      if constexpr (MODE != WHOLE) {
+        Joined a{mx, lt, acc};
+        if (shared_part<D, MODE>(p, sq.s0 + t, it.kvh * p.G + g, dd, a)) continue;
+        lt = a.l;
+        acc = a.o;
+      }
       uint16_t* dst = (uint16_t*)p.o + (int64_t)(sq.s0 + t) * p.st_o +
                       (int64_t)(it.kvh * p.G + g) * p.sh_o + dd;
       const float inv = lt == 0.f ? 0.f : 1.f / lt;
@@ -1112,7 +1217,7 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(KArgs p) {
                                                  pack_bf16x2(acc.z * inv, acc.w * inv)};
     }
   }
-  if (it.ns > 1) join_parts<D, BQ, 64 * NW, uint16_t>(p, it, nr, so);
+  if (it.ns > 1) join_parts<D, BQ, 64 * NW, uint16_t, MODE>(p, it, nr, so);
 }
 
 // ---- f32 -------------------------------------------------------------------------
@@ -1121,14 +1226,14 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(KArgs p) {
 // memory, and meet once at the end.  Chunks of 100, 97 and 87 tokens over 1500, 350 and 87 keys,
 // 12 heads: 22.5 us; two tiles a wave, each 64 MFMAs of 64 cycles behind its loads, then the
 // merge and the join.  A single token fills a whole tile of 32 rows: one over 8192 keys 22.4 us.
-template <int ND>
+template <int ND, int MODE>
 __global__ __launch_bounds__(256) void paged_attn_f32_kernel(KArgs p) {
   constexpr int D = 32 * ND, NW = 4, NC = 4 * ND, OP = D + 4, BQ = 32, BKV = 32;
   __shared__ __attribute__((aligned(16))) float so[NW * 32 * OP];
   __shared__ float sm[NW][32], sl[NW][32];
   __shared__ int ptab[PT];
   Item it;
-  if (!find_item<BQ, BKV>(p, blockIdx.x, it)) return;
+  if (!find_item<BQ, BKV, MODE>(p, blockIdx.x, it)) return;
   const Seq& sq = it.q;
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -1136,7 +1241,7 @@ __global__ __launch_bounds__(256) void paged_attn_f32_kernel(KArgs p) {
   const int rows = sq.n * p.G, first = sq.len - sq.n;
   const int r0 = it.rt * BQ, r1 = min(r0 + BQ, rows) - 1;
   int lo, hi;
-  key_range(p, sq, r0, r1, lo, hi);
+  key_range(p, it, r0, r1, lo, hi);
   const int t_lo = lo / BKV, cnt = hi < 0 ? 0 : hi / BKV - t_lo + 1;
   int t0, t1;
   part_of(it, t_lo, cnt, t0, t1);
@@ -1144,7 +1249,7 @@ __global__ __launch_bounds__(256) void paged_attn_f32_kernel(KArgs p) {
   const int r = min(r0 + l31, rows - 1);
   const int tok = over(r, p.by_g), g = r - tok * p.G;
   const int khi = p.causal ? min(first + tok, sq.len - 1) : sq.len - 1;
-  const int klo = p.window ? first + tok - p.window + 1 : 0;
+  const int klo = p.window ? first + tok - p.window + 1 : it.from;
   f32x4_t qf[NC], kf[NC];
   {
     const float* qrow = (const float*)p.q + (int64_t)(sq.s0 + tok) * p.st_q +
@@ -1178,7 +1283,7 @@ __global__ __launch_bounds__(256) void paged_attn_f32_kernel(KArgs p) {
   const float c = p.c;
   // every row sees [all_lo, all_hi]
   const int all_hi = p.causal ? min(first + over(r0, p.by_g), sq.len - 1) : sq.len - 1;
-  const int all_lo = p.window ? first + over(r1, p.by_g) - p.window + 1 : 0;
+  const int all_lo = p.window ? first + over(r1, p.by_g) - p.window + 1 : it.from;
   // one tile; the next one's K (of `next`) is loaded under the second product
   auto tile = [&](int t, int next) {
     const int k0 = t * BKV;
@@ -1338,19 +1443,25 @@ __global__ __launch_bounds__(256) void paged_attn_f32_kernel(KArgs p) {
 #pragma unroll
     for (int k = 0; k < NW; ++k)
       x[k] = *reinterpret_cast<const f32x4_t*>(so + (k * 32 + rr) * OP + cc);
-    const f32x4_t sum = (x[0] + x[1]) + (x[2] + x[3]);
-    const float tot = sl[0][rr];
+    f32x4_t sum = (x[0] + x[1]) + (x[2] + x[3]);
+    float tot = sl[0][rr];
     if (it.ns > 1) {
       put4(p.part + (at + rr) * D + cc, sum);
       if (cc == 0) put2(p.ml + (at + rr) * 2, sm[0][rr], tot);
     } else {
       const int t = over(r0 + rr, p.by_g), gg = (r0 + rr) - t * p.G;
+      if constexpr (MODE != WHOLE) {
+        Joined a{sm[0][rr], tot, sum};
+        if (shared_part<D, MODE>(p, sq.s0 + t, it.kvh * p.G + gg, cc, a)) continue;
+        tot = a.l;
+        sum = a.o;
+      }
       *reinterpret_cast<f32x4_t*>((float*)p.o + (int64_t)(sq.s0 + t) * p.st_o +
                                   (int64_t)(it.kvh * p.G + gg) * p.sh_o + cc) =
           tot == 0.f ? f32x4_t{0.f, 0.f, 0.f, 0.f} : sum / tot;
     }
   }
-  if (it.ns > 1) join_parts<D, BQ, 256, float>(p, it, nq, so);
+  if (it.ns > 1) join_parts<D, BQ, 256, float, MODE>(p, it, nq, so);
 }
 
 // ---- f32, tiles of rows ----------------------------------------------------------
@@ -1364,6 +1475,7 @@ __global__ __launch_bounds__(256) void paged_attn_f32_kernel(KArgs p) {
 // d = 64 the form above has two blocks a CU itself (10 of up to 400, 12 heads, 58 and 39).
 // At 256 registers 91 values a lane stay in scratch memory, in the main loop (q's fragments,
 // scores and outputs alone are 160).
+template <int MODE>
 __global__ __launch_bounds__(256, 2) void paged_attn_f32_tiles_kernel(KArgs p) {
   constexpr int D = 128, BKV = 32, QPW = 32, BQ = 4 * QPW, ND = D / 32, NC = D / 8;
   constexpr int TILE = BKV * D, STAGE = 2 * TILE, NST = 2;
@@ -1374,7 +1486,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_f32_tiles_kernel(KArgs p) {
   __shared__ int ptab[PT];
 
   Item it;
-  if (!find_item<BQ, BKV>(p, blockIdx.x, it)) return;
+  if (!find_item<BQ, BKV, MODE>(p, blockIdx.x, it)) return;
   const Seq& sq = it.q;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -1382,7 +1494,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_f32_tiles_kernel(KArgs p) {
   const int rows = sq.n * p.G, first = sq.len - sq.n;
   int lo, hi;
   const int r0 = it.rt * BQ, r1 = min(r0 + BQ, rows) - 1;
-  key_range(p, sq, r0, r1, lo, hi);
+  key_range(p, it, r0, r1, lo, hi);
   const int t_lo = lo / BKV, cnt = hi < 0 ? 0 : hi / BKV - t_lo + 1;
   int t0, t1;
   part_of(it, t_lo, cnt, t0, t1);
@@ -1390,14 +1502,14 @@ __global__ __launch_bounds__(256, 2) void paged_attn_f32_tiles_kernel(KArgs p) {
   const int rw = r0 + wid * QPW, rwl = min(rw + QPW, rows) - 1;
   const bool wave_active = rw < rows;
   int wlo = 0, whi = -1;
-  if (wave_active) key_range(p, sq, rw, rwl, wlo, whi);
+  if (wave_active) key_range(p, it, rw, rwl, wlo, whi);
   const int pos_first = first + over(rw, p.by_g);
-  const int lo_last = p.window ? first + over(rwl, p.by_g) - p.window + 1 : 0;
+  const int lo_last = p.window ? first + over(rwl, p.by_g) - p.window + 1 : it.from;
 
   const int row = min(rw + l31, rows - 1);
   const int tok = over(row, p.by_g), head = it.kvh * p.G + row - tok * p.G;
   const int khi = p.causal ? min(first + tok, sq.len - 1) : sq.len - 1;
-  const int klo = p.window ? first + tok - p.window + 1 : 0;
+  const int klo = p.window ? first + tok - p.window + 1 : it.from;
   f32x4_t qf[NC];
   {
     const float* qrow =
@@ -1577,6 +1689,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_f32_tiles_kernel(KArgs p) {
   float total = a + b;
   if (it.ns > 1 && !join_tiles<D>(p, it, wave_active, o, m, total)) return;
   if (rw + l31 < rows) {
+    if (shared_row<D, MODE, true>(p, sq.s0 + tok, head, h, m, total, o)) return;
     float* orow = (float*)p.o + (int64_t)(sq.s0 + tok) * p.st_o + (int64_t)head * p.sh_o;
 #pragma unroll
     for (int n = 0; n < NV; ++n)
@@ -1648,24 +1761,24 @@ int64_t slots_of(const blt_paged_cache& c, const Shape& s, int64_t B, int64_t to
   return most < 2 ? 0 : rt * most < all ? rt * most : all;
 }
 
-template <int D>
+template <int D, int MODE>
 int run_paged(const KArgs& p, const Shape& sh, unsigned nb, hipStream_t s) {
   const dim3 grid(nb), block(256);
   switch (sh.form) {
     case FORM_TILES:
-      hipLaunchKernelGGL((paged_attn_kernel<D, 2>), grid, block, 0, s, p);
+      hipLaunchKernelGGL((paged_attn_kernel<D, 2, MODE>), grid, block, 0, s, p);
       break;
     case FORM_FEW16:
-      hipLaunchKernelGGL((paged_attn_few_kernel<D, 1, 2>), grid, dim3(128), 0, s, p);
+      hipLaunchKernelGGL((paged_attn_few_kernel<D, 1, 2, MODE>), grid, dim3(128), 0, s, p);
       break;
     case FORM_FEW32:
-      hipLaunchKernelGGL((paged_attn_few_kernel<D, 2, 2>), grid, dim3(128), 0, s, p);
+      hipLaunchKernelGGL((paged_attn_few_kernel<D, 2, 2, MODE>), grid, dim3(128), 0, s, p);
       break;
     case FORM_F32_TILES:
-      hipLaunchKernelGGL(paged_attn_f32_tiles_kernel, grid, block, 0, s, p);
+      hipLaunchKernelGGL(paged_attn_f32_tiles_kernel<MODE>, grid, block, 0, s, p);
       break;
     default:
-      hipLaunchKernelGGL((paged_attn_f32_kernel<D / 32>), grid, block, 0, s, p);
+      hipLaunchKernelGGL((paged_attn_f32_kernel<D / 32, MODE>), grid, block, 0, s, p);
   }
   BLT_LAUNCH_CHECK("paged_attn_kernel");
   return 0;
@@ -1673,15 +1786,23 @@ int run_paged(const KArgs& p, const Shape& sh, unsigned nb, hipStream_t s) {
 
 }  // namespace
 
-int64_t paged_attention_workspace_bytes(const blt_paged_cache& c, int64_t B, int64_t total,
-                                        int H) {
+static int64_t parts_bytes(const blt_paged_cache& c, int64_t B, int64_t total, int H) {
   const Shape s = shape_of(c, B, total, H);
   return slots_of(c, s, B, total, H) * s.bq * (c.head_dim + 2) * 4;
 }
+int64_t paged_attention_workspace_bytes(const blt_paged_cache& c, int64_t B, int64_t total, int H,
+                                        bool prefix) {
+  const int64_t own = parts_bytes(c, B, total, H);
+  if (!prefix) return own;
+  // the prefix' outputs, and the parts of one launch after the other
+  return total * H * (c.head_dim + 2) * 4 + std::max(own, parts_bytes(c, 1, total, H));
+}
 
-int launch_paged_attention(const blt_paged_cache& c, const PagedAttnArgs& a, void* ws,
-                           hipStream_t s) {
-  Shape sh = shape_of(c, a.B, a.total, a.H);
+// One launch; with a prefix its own (mode PREFIX) and the sequences' (TAILS).
+static int launch_mode(const blt_paged_cache& c, const PagedAttnArgs& a, int mode, void* ws,
+                       hipStream_t s) {
+  const int64_t B = mode == PREFIX ? 1 : a.B;  // (what the shape and the grid go by)
+  Shape sh = shape_of(c, B, a.total, a.H);
   const int d = c.head_dim;
   KArgs p{};
   const int64_t es = c.dtype == BLT_DTYPE_BF16 ? 2 : 4;
@@ -1695,19 +1816,37 @@ int launch_paged_attention(const blt_paged_cache& c, const PagedAttnArgs& a, voi
   p.tokens_max = sh.bq / p.G + 2;
   p.max_seqs = c.max_seqs; p.max_pages = c.max_pages; p.num_pages = c.num_pages;
   p.lps = log2_of(c.page_size); p.cap = c.max_pages * c.page_size;
-  p.causal = a.causal; p.window = a.causal ? a.window : 0;
+  p.causal = mode == PREFIX ? 0 : a.causal;  // (every row sees all of the prefix)
+  p.window = p.causal ? a.window : 0;
   if (p.window > (1 << 30)) p.window = 0;  // longer than any sequence
   p.c = (float)(1.44269504088896340736 * (double)a.scale);
   if (p.window && p.window < 24 * sh.bkv) sh.spill = 0;  // (too short: its blocks would only exit)
   p.resident = sh.resident; p.cmin = sh.cmin; p.spill = sh.spill;
-  const int64_t slots = slots_of(c, sh, a.B, a.total, a.H);
+  const int64_t slots = slots_of(c, sh, B, a.total, a.H);
   p.sync = c.sync; p.status = c.status;
   p.part = (float*)ws;
+  if (mode != WHOLE) {
+    p.prefix = a.prefix;
+    p.pre_o = p.part;
+    p.pre_ml = p.pre_o + a.total * a.H * d;
+    p.part = p.pre_ml + a.total * a.H * 2;
+  }
   p.ml = p.part + slots * sh.bq * d;
-  const int64_t nb = (blocks_of(c, sh, a.B, a.total, a.H) + 7) / 8 * 8;
+  const int64_t nb = (blocks_of(c, sh, B, a.total, a.H) + 7) / 8 * 8;
   if (nb > 0x7fffffff) return fail(BLT_ERR_SHAPE, "paged_attention: too many row tiles");
-  return d == 64 ? run_paged<64>(p, sh, (unsigned)nb, s)
-                 : run_paged<128>(p, sh, (unsigned)nb, s);
+  const unsigned n = (unsigned)nb;
+  switch (mode) {
+    case PREFIX: return d == 64 ? run_paged<64, PREFIX>(p, sh, n, s) : run_paged<128, PREFIX>(p, sh, n, s);
+    case TAILS: return d == 64 ? run_paged<64, TAILS>(p, sh, n, s) : run_paged<128, TAILS>(p, sh, n, s);
+    default: return d == 64 ? run_paged<64, WHOLE>(p, sh, n, s) : run_paged<128, WHOLE>(p, sh, n, s);
+  }
+}
+
+int launch_paged_attention(const blt_paged_cache& c, const PagedAttnArgs& a, void* ws,
+                           hipStream_t s) {
+  if (!a.prefix) return launch_mode(c, a, WHOLE, ws, s);
+  if (int rc = launch_mode(c, a, PREFIX, ws, s)) return rc;
+  return launch_mode(c, a, TAILS, ws, s);
 }
 
 }  // namespace blt

@@ -53,6 +53,8 @@ int launch_cache_trim(const blt_paged_cache& c, const int32_t* seqs, const int32
 int launch_cache_fork(const blt_paged_cache& c, const int32_t* src, const int32_t* dst, int64_t n,
                       hipStream_t s);
 int launch_cache_compact(const blt_paged_cache& c, void* ws, hipStream_t s);
+int launch_cache_common_prefix(const blt_paged_cache& c, const int32_t* seqs, int64_t n,
+                               int32_t* tokens, hipStream_t s);
 int launch_cache_copy_pages(const blt_paged_cache& c, const int32_t* src, const int32_t* dst,
                             int64_t n, hipStream_t s);
 
@@ -66,9 +68,10 @@ struct PagedAttnArgs {
   int64_t B, total;
   int layer, causal, window;
   float scale;
+  const int32_t* prefix;  // tokens that the sequences share, or null
 };
-int64_t paged_attention_workspace_bytes(const blt_paged_cache& c, int64_t B, int64_t total,
-                                        int H);
+int64_t paged_attention_workspace_bytes(const blt_paged_cache& c, int64_t B, int64_t total, int H,
+                                        bool prefix);
 int launch_paged_attention(const blt_paged_cache& c, const PagedAttnArgs& a, void* ws,
                            hipStream_t s);
 

@@ -350,6 +350,25 @@ int blt_paged_attention(const blt_paged_cache* cache, int32_t layer, const void*
                         int32_t causal, int32_t window, float scale, void* workspace,
                         int64_t workspace_bytes, blt_stream_t stream);
 
+/* Tokens that the sequences seqs[i], i < n <= 65536 (NULL: sequence i), have in common: their leading
+ * whole pages that are the same pages, as after blt_cache_fork, into tokens [1] (device).
+ * Sequences without tokens are left out; 0 with fewer than two.  An index out of range gives 0 and
+ * sets BLT_CACHE_BAD_INDEX. */
+int blt_cache_common_prefix(const blt_paged_cache* cache, const int32_t* seqs, int64_t n,
+                            int32_t* tokens, blt_stream_t stream);
+/* blt_paged_attention without a window for sequences that share their first prefix[0] tokens (int32
+ * [1], device, from blt_cache_common_prefix of a list that holds these sequences): the shared
+ * keys are read once for all rows, in a launch of their own.  What is no whole page, and what does not lie
+ * before every row's new tokens, is not taken as shared, so any number is safe; but where the first
+ * pages are not the same ones, rows see those of the first row that has tokens. */
+int64_t blt_paged_attention_prefix_workspace_bytes(const blt_paged_cache* cache, int64_t B,
+                                                   int64_t total, int64_t Hq);
+int blt_paged_attention_prefix(const blt_paged_cache* cache, int32_t layer, const void* q,
+                               int64_t st_q, int64_t sh_q, void* o, int64_t st_o, int64_t sh_o,
+                               int64_t Hq, const int32_t* starts, const int32_t* seqs, int64_t B,
+                               int64_t total, int32_t causal, float scale, const int32_t* prefix,
+                               void* workspace, int64_t workspace_bytes, blt_stream_t stream);
+
 /* Patcher (src/patcher.rs) --------------------------------------------- */
 
 /* patch_start_mask_from_entropy_with_monotonicity (patcher.rs:80-118) fused with
