@@ -30,6 +30,8 @@ FILE_FLAGS = {
     # a v_accvgpr read/write per value per tile (the GEMMs keep their
     # accumulators in AGPRs where the 4-wave tiles need the room)
     "k_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    # (and the f32 form fits two waves a SIMD, the gradient's no longer spill)
+    "k_packed_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 

@@ -8,6 +8,8 @@
 // because a sequence ends in it: tiles of rows run over the ends of sequences, so that the grid
 // follows from the number of tokens alone and many short sequences share a tile.  A wave passes the
 // key tiles that none of its rows sees.
+#include <type_traits>
+
 #include "attn_tiles.hpp"
 #include "packed.hpp"
 
@@ -120,6 +122,20 @@ struct Transposed {
     return u32x4_t{w0.x, w0.y, w1.x, w1.y};
   }
 };
+// The order of a block's LDS reads and matrix products: `ahead` reads, then `each` reads behind every
+// one of the first `n` products.  (Left alone the compiler reads an operand right before its
+// product and waits for it every time.)
+template <int AHEAD, int N, int EACH, int LAST>
+__device__ inline void reads_ahead() {
+  constexpr int MFMA = 0x008, READ = 0x100;
+  __builtin_amdgcn_sched_group_barrier(READ, AHEAD, 0);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(READ, EACH, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(MFMA, LAST, 0);
+}
 __device__ inline bf16x8_t bf8(u32x4_t x) { return __builtin_bit_cast(bf16x8_t, x); }
 
 // Bounds of the keys that the rows of a wave and of its block see.
@@ -694,9 +710,7 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(GArgs ga) {
     }
   };
   const Transposed<D> tr(lane);
-  f32x16_t acc[DS], nd;  // nd: -D of the row, where a chain of dP starts
-#pragma unroll
-  for (int r = 0; r < 16; ++r) nd[r] = -delta;
+  f32x16_t acc[DS];
 #pragma unroll
   for (int j = 0; j < DS; ++j)
 #pragma unroll
@@ -713,7 +727,7 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(GArgs ga) {
       const uint16_t* sk = lds + stage * STAGE;
       const uint16_t* sv = sk + TILE;
       const bool mask = kb + BKV - 1 > bd.hi_min || kb < bd.lo_max;
-#pragma unroll
+#pragma unroll 1
       for (int sub = 0; sub < 2; ++sub) {
         f32x16_t s, dp;
 #pragma unroll
@@ -722,8 +736,8 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(GArgs ga) {
               row_chunk<D>(sk, sub * 32 + lrow, 2 * ks + lhalf), qf[ks],
               ks == 0 ? f32x16_t{} : s, 0, 0, 0);
           dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-              row_chunk<D>(sv, sub * 32 + lrow, 2 * ks + lhalf), gf[ks], ks == 0 ? nd : dp, 0, 0,
-              0);
+              row_chunk<D>(sv, sub * 32 + lrow, 2 * ks + lhalf), gf[ks], ks == 0 ? f32x16_t{} : dp, 0,
+              0, 0);
         }
         u32x4_t kt[DS][2];
 #pragma unroll
@@ -732,7 +746,7 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(GArgs ga) {
           for (int u = 0; u < 2; ++u) kt[ds][u] = tr.read(sk, sub * 32 + u * 16, ds);
         float e[16];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) e[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, mc)) * dp[r];
+        for (int r = 0; r < 16; ++r) e[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, mc)) * (dp[r] - delta);
         if (mask) {
           const int up = khi - kb - sub * 32 - 4 * lhalf, dn = klo - kb - sub * 32 - 4 * lhalf;
 #pragma unroll
@@ -793,41 +807,46 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(GArgs ga) {
   }
 }
 
-// dk and dv, bf16.  One block = 4 waves of 32 keys each; tiles of 64 rows, Q beside dO, pass
-// through LDS.  S = Q . K^T and dP = dO . V^T put a key into a lane and rows into registers,
-// from which P and dS feed dV^T = dO^T . P and dK^T = Q^T . dS.
-template <int D>
-__global__ __launch_bounds__(256, D == 64 ? 2 : 1) void packed_dkdv_kernel(GArgs ga) {
+// dk and dv, bf16.  One block = 4 x 2 waves: 32 keys each, and one half of the rows of a tile
+// each; tiles of BR rows, Q beside dO, pass through LDS.  S = Q . K^T and dP = dO . V^T put a key into
+// a lane and rows into registers, from which P and dS feed dV^T = dO^T . P and dK^T = Q^T . dS.
+// The two halves are added up at the end.
+template <int D, int RW, int BR>
+__global__ __launch_bounds__(256 * RW, D == 64 ? 3 : 2) void packed_dkdv_kernel(GArgs ga) {
   const PArgs& p = ga.a;
-  constexpr int BR = 64, KPW = 32, BK = 4 * KPW;
+  constexpr int NW = 4 * RW, KPW = 32, BK = 4 * KPW, SHARE = BR / RW;
+  constexpr bool V_LDS = D == 128;  // (its fragments would not fit the registers)
   constexpr int TILE = BR * D, STAGE = 2 * TILE + 512, NST = 2;  // 512: 1 KB of stats
-  constexpr int KS = D / 16, DS = D / 32, CPR = D / 8, RPI = 64 / CPR;
-  __shared__ __attribute__((aligned(1024))) uint16_t lds[NST * STAGE];
+  constexpr int KS = D / 16, DS = D / 32, CPR = D / 8, RPI = 64 / CPR, RPW = BR / NW;
+  // (the sums that meet: 4 x 64 x DS x 16 floats)
+  static_assert(RW == 1 || NST * STAGE >= 4 * 64 * DS * 32, "they fit the stages");
+  __shared__ __attribute__((aligned(1024))) uint16_t lds[NST * STAGE + (V_LDS ? BK * D : 0)];
 
   int kvh, tile;
   if (!tile_of(p, kvh, tile)) return;
   tile = p.tiles - 1 - tile;  // (long causal columns first)
   const int tid = threadIdx.x, lane = tid & 63;
-  const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wid = __builtin_amdgcn_readfirstlane(tid >> 6), wk = wid & 3, wr = wid >> 2;
   const int lrow = lane & 31, lhalf = lane >> 5;
-  const int kw = tile * BK + wid * KPW;
+  const int kw = tile * BK + wk * KPW;
   const int key = min(kw + lrow, p.total - 1);
-  bf16x8_t kf[KS], vf[KS];
+  bf16x8_t kf[KS], vf[V_LDS ? 1 : KS];
   {
     const uint16_t* krow = (const uint16_t*)p.k + (int64_t)key * p.st_k + (int64_t)kvh * p.sh_k;
     const uint16_t* vrow = (const uint16_t*)p.v + (int64_t)key * p.st_v + (int64_t)kvh * p.sh_v;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       kf[ks] = bf8(*reinterpret_cast<const u32x4_t*>(krow + ks * 16 + lhalf * 8));
-      vf[ks] = bf8(*reinterpret_cast<const u32x4_t*>(vrow + ks * 16 + lhalf * 8));
+      if constexpr (!V_LDS)
+        vf[ks] = bf8(*reinterpret_cast<const u32x4_t*>(vrow + ks * 16 + lhalf * 8));
     }
   }
   int rlo, rhi;
   const bool in = rows_of(p, key, rlo, rhi);
-  const Bounds bd = bounds_of<4>(rlo, rhi, in);
+  const Bounds bd = bounds_of<NW>(rlo, rhi, in);
   const int t0 = bd.hi < 0 ? 0 : bd.lo / BR, t1 = bd.hi < 0 ? 0 : bd.hi / BR + 1;
 #pragma unroll
-  for (int ks = 0; ks < KS; ++ks) asm volatile("" ::"v"(kf[ks]), "v"(vf[ks]));
+  for (int ks = 0; ks < KS; ++ks) asm volatile("" ::"v"(kf[ks]), "v"(vf[V_LDS ? 0 : ks]));
 
   const unsigned lds_base = (unsigned)(uintptr_t)lds;
   const int kin = lane / CPR, slot = lane % CPR;
@@ -840,18 +859,33 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void packed_dkdv_kernel(GArgs
     const char* qt = qbase + (int64_t)tok0 * p.st_q * 2;
     const char* gt = gbase + (int64_t)tok0 * ga.st_g * 2;
 #pragma unroll
-    for (int i = 0; i < 16 / RPI; ++i) {
-      const int r = 16 * wid + RPI * i + kin, from = min(t * BR + r, p.rows - 1);
+    for (int i = 0; i < RPW / RPI; ++i) {
+      const int r = RPW * wid + RPI * i + kin, from = min(t * BR + r, p.rows - 1);
       const int tok = over(from, p.by_g), g = from - tok * p.G;
       const unsigned ch = (unsigned)((slot ^ swz<D>(r)) * 16);
-      const unsigned la = sb + (unsigned)((16 * wid + RPI * i) * D * 2);
+      const unsigned la = sb + (unsigned)((RPW * wid + RPI * i) * D * 2);
       dma16_so(qt, (unsigned)((tok - tok0) * (int)p.st_q + g * (int)p.sh_q) * 2u + ch, la);
       dma16_so(gt, (unsigned)((tok - tok0) * (int)ga.st_g + g * (int)ga.sh_g) * 2u + ch,
                la + TILE * 2);
     }
-    if (wid == 0)  // (a tile's 512 bytes, twice)
-      dma16_so(sbase + (int64_t)t * 512, (unsigned)(lane & 31) * 16, sb + 2 * TILE * 2);
+    // the stats of 64 rows are 512 bytes (twice, where a tile has no more; behind the last: the
+    // last ones)
+    if (wid == 0) {
+      const int at = min(t * (BR / 64) + (BR == 128 ? lane >> 5 : 0), ga.stat_tiles - 1);
+      dma16_so(sbase + (int64_t)t * (BR / 64) * 512,
+               (unsigned)((at - t * (BR / 64)) * 512 + (lane & 31) * 16), sb + 2 * TILE * 2);
+    }
   };
+  const uint16_t* sv = lds + NST * STAGE;  // V of the block's keys
+  if (V_LDS && t0 < t1) {
+    const char* vt = (const char*)p.v + ((int64_t)tile * BK * p.st_v + (int64_t)kvh * p.sh_v) * 2;
+#pragma unroll
+    for (int i = 0; i < BK / NW / RPI; ++i) {
+      const int r = BK / NW * wid + RPI * i + kin, from = min(r, p.total - 1 - tile * BK);
+      dma16_so(vt, (unsigned)from * (unsigned)(p.st_v * 2) + (unsigned)((slot ^ swz<D>(r)) * 16),
+               lds_base + (unsigned)(NST * STAGE + (BK / NW * wid + RPI * i) * D) * 2);
+    }
+  }
   const Transposed<D> tr(lane);
   f32x16_t dk[DS], dv[DS];
 #pragma unroll
@@ -860,114 +894,166 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void packed_dkdv_kernel(GArgs
     for (int r = 0; r < 16; ++r) dk[j][r] = dv[j][r] = 0.f;
   const float c = p.c;
 
-  if (t0 < t1) issue(t0, 0);
-  int stage = 0;
-  for (int t = t0; t < t1; ++t) {
-    dma_wait_barrier<0>();
-    if (t + 1 < t1) issue(t + 1, stage ^ 1);
-    const int rb = t * BR;
-    if (rb <= bd.whi && rb + BR > bd.wlo) {
-      const uint16_t* sq = lds + stage * STAGE;
-      const uint16_t* sg = sq + TILE;
-      const float* st = reinterpret_cast<const float*>(sg + TILE);
-      const bool mask = rb + BR - 1 > bd.hi_min || rb < bd.lo_max;
+  // P and dS of 32 rows at row r0 of the tile at sq, as the second products' operands: false
+  // where no row of them sees a key.  odd: values that are not finite are to be left out.
+  auto first = [&](int t, const uint16_t* sq, int r0, bf16x8_t (&bw)[2], bf16x8_t (&be)[2],
+                   bool& odd) {
+    const uint16_t* sg = sq + TILE;
+    const int rb = t * BR + r0;
+    odd = false;
+    if (rb > bd.whi || rb + 32 <= bd.wlo) return false;
+    const float* st = reinterpret_cast<const float*>(sg + TILE) + (r0 >> 6) * 128 + (r0 & 63);
+    const bool mask = rb + 31 > bd.hi_min || rb < bd.lo_max;
+    f32x16_t s, dp;
 #pragma unroll
-      for (int sub = 0; sub < 2; ++sub) {
-        f32x16_t s, dp;
-        float mc[16];
+    for (int j = 0; j < 4; ++j) {  // (dP starts from -D)
+      const f32x4_t x = *reinterpret_cast<const f32x4_t*>(st + 64 + 8 * j + 4 * lhalf);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const f32x4_t x = *reinterpret_cast<const f32x4_t*>(st + sub * 32 + 8 * j + 4 * lhalf);
-          const f32x4_t y =
-              *reinterpret_cast<const f32x4_t*>(st + 64 + sub * 32 + 8 * j + 4 * lhalf);
+      for (int i = 0; i < 4; ++i) dp[4 * j + i] = x[i];
+    }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            mc[4 * j + i] = x[i];
-            dp[4 * j + i] = y[i];
-          }
-        }
+    for (int ks = 0; ks < KS; ++ks) {
+      s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(row_chunk<D>(sq, r0 + lrow, 2 * ks + lhalf),
+                                                  kf[ks], ks == 0 ? f32x16_t{} : s, 0, 0, 0);
+      dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+          row_chunk<D>(sg, r0 + lrow, 2 * ks + lhalf),
+          V_LDS ? row_chunk<D>(sv, wk * 32 + lrow, 2 * ks + lhalf) : vf[V_LDS ? 0 : ks], dp, 0, 0,
+          0);
+    }
+    // (2 KS products, 2 KS reads and the 4 of -D; with D = 128 there are no registers for it)
+    if constexpr (!V_LDS) reads_ahead<8, 2 * KS - 4, 1, 4>();
+    float w[16], e[16];
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-              row_chunk<D>(sq, sub * 32 + lrow, 2 * ks + lhalf), kf[ks],
-              ks == 0 ? f32x16_t{} : s, 0, 0, 0);
-          dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-              row_chunk<D>(sg, sub * 32 + lrow, 2 * ks + lhalf), vf[ks], dp, 0, 0, 0);
-        }
-        float w[16], e[16];
+    for (int j = 0; j < 4; ++j) {
+      const f32x4_t x = *reinterpret_cast<const f32x4_t*>(st + 8 * j + 4 * lhalf);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          w[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, mc[r]));
-          e[r] = w[r] * dp[r];
-        }
-        bool odd = false;
-        if (mask) {
-          const int up = rhi - rb - sub * 32 - 4 * lhalf, dn = rlo - rb - sub * 32 - 4 * lhalf;
+      for (int i = 0; i < 4; ++i) {
+        const int r = 4 * j + i;
+        w[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, x[i]));
+        e[r] = w[r] * dp[r];
+      }
+    }
+    if (mask) {
+      const int up = rhi - rb - 4 * lhalf, dn = rlo - rb - 4 * lhalf;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int at = 8 * (r >> 2) + (r & 3);
-            const bool sees = at <= up && at >= dn;
-            w[r] = sees ? w[r] : 0.f;
-            e[r] = sees ? e[r] : 0.f;
-          }
-          // values that are not finite in rows that do not see the key (as in packed_dq_kernel)
-          uint32_t seen = 0;
+      for (int r = 0; r < 16; ++r) {
+        const int at = 8 * (r >> 2) + (r & 3);
+        const bool sees = at <= up && at >= dn;
+        w[r] = sees ? w[r] : 0.f;
+        e[r] = sees ? e[r] : 0.f;
+      }
+      // values that are not finite in rows that do not see the key (as in packed_dq_kernel)
+      uint32_t seen = 0;
 #pragma unroll
-          for (int i = 0; i < DS * 2; ++i) {
-            const u32x4_t x = tr.read(sg, sub * 32 + (i & 1) * 16, i >> 1);
-            const u32x4_t y = tr.read(sq, sub * 32 + (i & 1) * 16, i >> 1);
+      for (int i = 0; i < DS * 2; ++i) {
+        const u32x4_t x = tr.read(sg, r0 + (i & 1) * 16, i >> 1);
+        const u32x4_t y = tr.read(sq, r0 + (i & 1) * 16, i >> 1);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) seen = exponents2(exponents2(seen, x[j]), y[j]);
-          }
-          odd = __any(not_finite2(seen));
-          if (odd) {
-            for (int j = 32 * sub; j < 32 * sub + 32; ++j) {
-              const bool sees = rb + j <= rhi && rb + j >= rlo;
+        for (int j = 0; j < 4; ++j) seen = exponents2(exponents2(seen, x[j]), y[j]);
+      }
+      odd = __any(not_finite2(seen));
+      if (odd) {
+        for (int j = r0; j < r0 + 32; ++j) {
+          const bool sees = t * BR + j <= rhi && t * BR + j >= rlo;
 #pragma unroll
-              for (int i = 0; i < DS * 4; ++i) {
-                const int at = j * D + ((i ^ swz<D>(j)) << 3) + 4 * lhalf;
-                const u32x2_t x = *reinterpret_cast<const u32x2_t*>(sg + at);
-                const u32x2_t y = *reinterpret_cast<const u32x2_t*>(sq + at);
+          for (int i = 0; i < DS * 4; ++i) {
+            const int at = j * D + ((i ^ swz<D>(j)) << 3) + 4 * lhalf;
+            const u32x2_t x = *reinterpret_cast<const u32x2_t*>(sg + at);
+            const u32x2_t y = *reinterpret_cast<const u32x2_t*>(sq + at);
 #pragma unroll
-                for (int z = 0; z < 4; ++z) {
-                  const float a = bf16_to_f32((uint16_t)(x[z >> 1] >> (16 * (z & 1))));
-                  const float b = bf16_to_f32((uint16_t)(y[z >> 1] >> (16 * (z & 1))));
-                  dv[i >> 2][4 * (i & 3) + z] += sees && !(fabsf(a) < INFINITY) ? a : 0.f;
-                  dk[i >> 2][4 * (i & 3) + z] += sees ? b - b : 0.f;
-                }
-              }
+            for (int z = 0; z < 4; ++z) {
+              const float a = bf16_to_f32((uint16_t)(x[z >> 1] >> (16 * (z & 1))));
+              const float b = bf16_to_f32((uint16_t)(y[z >> 1] >> (16 * (z & 1))));
+              dv[i >> 2][4 * (i & 3) + z] += sees && !(fabsf(a) < INFINITY) ? a : 0.f;
+              dk[i >> 2][4 * (i & 3) + z] += sees ? b - b : 0.f;
             }
-          }
-        }
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          uint32_t pw[4], pe[4];
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            pw[x] = pack_bf16x2(w[8 * u + 2 * x], w[8 * u + 2 * x + 1]);
-            pe[x] = pack_bf16x2(e[8 * u + 2 * x], e[8 * u + 2 * x + 1]);
-          }
-          const bf16x8_t bw = bf8(u32x4_t{pw[0], pw[1], pw[2], pw[3]});
-          const bf16x8_t be = bf8(u32x4_t{pe[0], pe[1], pe[2], pe[3]});
-#pragma unroll
-          for (int ds = 0; ds < DS; ++ds) {
-            u32x4_t x = tr.read(sg, sub * 32 + u * 16, ds), y = tr.read(sq, sub * 32 + u * 16, ds);
-            if (__builtin_expect(odd, false)) {
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                x[j] = finite2(x[j]);
-                y[j] = finite2(y[j]);
-              }
-            }
-            dv[ds] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bf8(x), bw, dv[ds], 0, 0, 0);
-            dk[ds] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bf8(y), be, dk[ds], 0, 0, 0);
           }
         }
       }
     }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      uint32_t pw[4], pe[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        pw[x] = pack_bf16x2(w[8 * u + 2 * x], w[8 * u + 2 * x + 1]);
+        pe[x] = pack_bf16x2(e[8 * u + 2 * x], e[8 * u + 2 * x + 1]);
+      }
+      bw[u] = bf8(u32x4_t{pw[0], pw[1], pw[2], pw[3]});
+      be[u] = bf8(u32x4_t{pe[0], pe[1], pe[2], pe[3]});
+    }
+    return true;
+  };
+  auto products = [&](const uint16_t* sq, int r0, const bf16x8_t (&bw)[2],
+                      const bf16x8_t (&be)[2], auto some_odd) {
+    const uint16_t* sg = sq + TILE;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int ds = 0; ds < DS; ++ds) {
+        u32x4_t x = tr.read(sg, r0 + u * 16, ds), y = tr.read(sq, r0 + u * 16, ds);
+        if constexpr (decltype(some_odd)::value) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            x[j] = finite2(x[j]);
+            y[j] = finite2(y[j]);
+          }
+        }
+        dv[ds] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bf8(x), bw[u], dv[ds], 0, 0, 0);
+        dk[ds] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bf8(y), be[u], dk[ds], 0, 0, 0);
+      }
+    // (4 DS products and 8 DS reads)
+    if constexpr (!decltype(some_odd)::value) reads_ahead<8, 4 * DS - 4, 2, 4>();
+  };
+  auto second = [&](const uint16_t* sq, int r0, const bf16x8_t (&bw)[2], const bf16x8_t (&be)[2],
+                    bool odd) {
+    if (__builtin_expect(odd, false))
+      products(sq, r0, bw, be, std::true_type{});
+    else
+      products(sq, r0, bw, be, std::false_type{});
+  };
+
+  if (t0 < t1) issue(t0, 0);
+  int stage = 0;
+  for (int t = t0; t < t1; ++t) {
+    // tile t has landed and every wave is past tile t - 1, whose stage is free
+    dma_wait_barrier<0>();
+    if (t + 1 < t1) issue(t + 1, stage ^ 1);
+    const uint16_t* sq = lds + stage * STAGE;
     stage ^= 1;
+#pragma unroll 1
+    for (int r0 = wr * SHARE; r0 < wr * SHARE + SHARE; r0 += 32) {
+      bf16x8_t bw[2], be[2];
+      bool odd = false;
+      if (first(t, sq, r0, bw, be, odd)) second(sq, r0, bw, be, odd);
+    }
   }
-  if (kw + lrow < p.total) {
+  // the second halves' sums, through LDS
+  float* meet = reinterpret_cast<float*>(lds) + (wk * 64 + lane) * 4;
+  auto add = [&](f32x16_t (&x)[DS]) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < DS * 4; ++i) {
+      f32x4_t* at = reinterpret_cast<f32x4_t*>(meet + i * 1024);
+      if (wr) {
+        *at = f32x4_t{x[i >> 2][4 * (i & 3)], x[i >> 2][4 * (i & 3) + 1], x[i >> 2][4 * (i & 3) + 2],
+                      x[i >> 2][4 * (i & 3) + 3]};
+      }
+    }
+    __syncthreads();
+    if (wr) return;
+#pragma unroll
+    for (int i = 0; i < DS * 4; ++i) {
+      const f32x4_t y = *reinterpret_cast<f32x4_t*>(meet + i * 1024);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[i >> 2][4 * (i & 3) + e] += y[e];
+    }
+  };
+  if constexpr (RW == 2) {
+    add(dk);
+    add(dv);
+  }
+  if (wr == 0 && kw + lrow < p.total) {
     uint16_t* ok = (uint16_t*)ga.dk + (int64_t)key * ga.st_dk + (int64_t)kvh * ga.sh_dk;
     uint16_t* ov = (uint16_t*)ga.dv + (int64_t)key * ga.st_dv + (int64_t)kvh * ga.sh_dv;
 #pragma unroll
@@ -1346,10 +1432,10 @@ int launch_packed_attention_backward(const PackedAttnArgs& a, const PackedGradAr
     hipLaunchKernelGGL((packed_dkdv_f32_kernel<4>), gk, block, 0, s, pk);
   } else if (a.d == 64) {
     hipLaunchKernelGGL((packed_dq_kernel<64>), gq, block, 0, s, p);
-    hipLaunchKernelGGL((packed_dkdv_kernel<64>), gk, block, 0, s, pk);
+    hipLaunchKernelGGL((packed_dkdv_kernel<64, 1, 64>), gk, block, 0, s, pk);
   } else {
     hipLaunchKernelGGL((packed_dq_kernel<128>), gq, block, 0, s, p);
-    hipLaunchKernelGGL((packed_dkdv_kernel<128>), gk, block, 0, s, pk);
+    hipLaunchKernelGGL((packed_dkdv_kernel<128, 2, 64>), gk, dim3(512), 0, s, pk);
   }
   BLT_LAUNCH_CHECK("packed_dq_kernel, packed_dkdv_kernel");
   return 0;
