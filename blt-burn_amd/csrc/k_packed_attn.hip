@@ -640,6 +640,10 @@ __device__ inline bool rows_of(const PArgs& p, int key, int& rlo, int& rhi) {
 
 // dq, bf16: as packed_attn_kernel, with two score products, V . dO^T beside K . Q^T, and
 // dQ^T = K^T . dS^T, whose first operand is read by transposing reads of the same K tile.
+// dS goes into its product as two bf16 halves (cut off, and what that left, rounded), and as it
+// adds up to 0 over a row but for what D is off by, with o rounded to bf16, that sum corrects D for the
+// other kernel.  So both gradients are 2.3e-3 off or less (relative, rms; their own rounding is
+// 1.7e-3), and not 2.5e-3 or, in short sequences, 3e-3.
 template <int D>
 __global__ __launch_bounds__(256, 2) void packed_dq_kernel(GArgs ga) {
   const PArgs& p = ga.a;
@@ -678,16 +682,11 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(GArgs ga) {
     delta = a + b;
   }
   const float mc = offset_of(p.lse[(int64_t)tok * p.H + head]);
-  if (lhalf == 0 && rw + lrow < p.rows) {
-    float* st = stats_of(ga, kvh, row);
-    st[0] = mc;
-    st[64] = -delta;
-  }
   int klo, khi;
   const bool in = keys_of(p, tok, klo, khi);
   const Bounds bd = bounds_of<4>(klo, khi, in);
   const int t0 = bd.hi < 0 ? 0 : bd.lo / BKV, t1 = bd.hi < 0 ? 0 : bd.hi / BKV + 1;
-  // (everything consumed and stored before any DMA is in flight)
+  // (everything consumed before any DMA is in flight)
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) asm volatile("" ::"v"(qf[ks]), "v"(gf[ks]));
 
@@ -716,6 +715,7 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(GArgs ga) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[j][r] = 0.f;
   const float c = p.c;
+  float rest = 0.f;  // sum of the row's dS
 
   if (t0 < t1) issue(t0, 0);
   int stage = 0;
@@ -744,6 +744,15 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(GArgs ga) {
         for (int ds = 0; ds < DS; ++ds)
 #pragma unroll
           for (int u = 0; u < 2; ++u) kt[ds][u] = tr.read(sk, sub * 32 + u * 16, ds);
+        // A weight of zero does not silence a key that is not finite (as in packed_attn_kernel),
+        // which shows in every row's score of it; where it is seen the result is NaN.
+        bool odd = false;
+        if (mask) {
+          float sum = 0.f;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) sum = fmaf(s[r], 0.f, sum);
+          odd = __any(sum != sum);
+        }
         float e[16];
 #pragma unroll
         for (int r = 0; r < 16; ++r) e[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, mc)) * (dp[r] - delta);
@@ -754,14 +763,7 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(GArgs ga) {
             const int key = 8 * (r >> 2) + (r & 3);
             e[r] = key <= up && key >= dn ? e[r] : 0.f;
           }
-          // a weight of zero does not silence a key that is not finite (as in
-          // packed_attn_kernel); where it is seen the result is NaN
-          uint32_t seen = 0;
-#pragma unroll
-          for (int i = 0; i < DS * 2; ++i)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) seen = exponents2(seen, kt[i >> 1][i & 1][x]);
-          if (__any(not_finite2(seen))) {
+          if (odd) {
 #pragma unroll
             for (int i = 0; i < DS * 2; ++i)
 #pragma unroll
@@ -783,17 +785,38 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(GArgs ga) {
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          uint32_t w[4];
+          uint32_t w[4], l[4];
 #pragma unroll
-          for (int x = 0; x < 4; ++x) w[x] = pack_bf16x2(e[8 * u + 2 * x], e[8 * u + 2 * x + 1]);
-          const bf16x8_t b = bf8(u32x4_t{w[0], w[1], w[2], w[3]});
+          for (int x = 0; x < 4; ++x) {
+            const float e0 = e[8 * u + 2 * x], e1 = e[8 * u + 2 * x + 1];
+            const uint32_t x0 = __float_as_uint(e0), x1 = __float_as_uint(e1);
+            rest += e0 + e1;
+            w[x] = __builtin_amdgcn_perm(x1, x0, 0x07060302);  // their upper halves
+            l[x] = pack_bf16x2(e0 - __uint_as_float(x0 & 0xffff0000u),
+                               e1 - __uint_as_float(x1 & 0xffff0000u));
+          }
+          const bf16x8_t hi = bf8(u32x4_t{w[0], w[1], w[2], w[3]});
+          const bf16x8_t lo = bf8(u32x4_t{l[0], l[1], l[2], l[3]});
 #pragma unroll
           for (int ds = 0; ds < DS; ++ds)
-            acc[ds] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bf8(kt[ds][u]), b, acc[ds], 0, 0, 0);
+            acc[ds] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bf8(kt[ds][u]), hi, acc[ds], 0, 0, 0);
+#pragma unroll
+          for (int ds = 0; ds < DS; ++ds)
+            acc[ds] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bf8(kt[ds][u]), lo, acc[ds], 0, 0, 0);
         }
       }
     }
     stage ^= 1;
+  }
+  {
+    float a, b;
+    swap_pair<32>(rest, a, b);
+    rest = a + b;
+  }
+  if (lhalf == 0 && rw + lrow < p.rows) {
+    float* st = stats_of(ga, kvh, row);
+    st[0] = mc;
+    st[64] = -(delta + rest);
   }
   if (rw + lrow < p.rows) {
     uint16_t* out = (uint16_t*)ga.dq + (int64_t)tok * ga.st_dq + (int64_t)head * ga.sh_dq;
@@ -811,22 +834,22 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(GArgs ga) {
 // each; tiles of BR rows, Q beside dO, pass through LDS.  S = Q . K^T and dP = dO . V^T put a key into
 // a lane and rows into registers, from which P and dS feed dV^T = dO^T . P and dK^T = Q^T . dS.
 // The two halves are added up at the end.
-template <int D, int RW, int BR>
-__global__ __launch_bounds__(256 * RW, D == 64 ? 3 : 2) void packed_dkdv_kernel(GArgs ga) {
+template <int D, int KW, int RW, int BR>
+__global__ __launch_bounds__(64 * KW * RW, D == 64 ? 3 : 2) void packed_dkdv_kernel(GArgs ga) {
   const PArgs& p = ga.a;
-  constexpr int NW = 4 * RW, KPW = 32, BK = 4 * KPW, SHARE = BR / RW;
+  constexpr int NW = KW * RW, KPW = 32, BK = KW * KPW, SHARE = BR / RW;
   constexpr bool V_LDS = D == 128;  // (its fragments would not fit the registers)
   constexpr int TILE = BR * D, STAGE = 2 * TILE + 512, NST = 2;  // 512: 1 KB of stats
   constexpr int KS = D / 16, DS = D / 32, CPR = D / 8, RPI = 64 / CPR, RPW = BR / NW;
-  // (the sums that meet: 4 x 64 x DS x 16 floats)
-  static_assert(RW == 1 || NST * STAGE >= 4 * 64 * DS * 32, "they fit the stages");
+  // (the sums that meet: (RW - 1) x KW x 64 x DS x 16 floats)
+  static_assert(NST * STAGE >= (RW - 1) * KW * 64 * DS * 32, "they fit the stages");
   __shared__ __attribute__((aligned(1024))) uint16_t lds[NST * STAGE + (V_LDS ? BK * D : 0)];
 
   int kvh, tile;
   if (!tile_of(p, kvh, tile)) return;
   tile = p.tiles - 1 - tile;  // (long causal columns first)
   const int tid = threadIdx.x, lane = tid & 63;
-  const int wid = __builtin_amdgcn_readfirstlane(tid >> 6), wk = wid & 3, wr = wid >> 2;
+  const int wid = __builtin_amdgcn_readfirstlane(tid >> 6), wk = wid % KW, wr = wid / KW;
   const int lrow = lane & 31, lhalf = lane >> 5;
   const int kw = tile * BK + wk * KPW;
   const int key = min(kw + lrow, p.total - 1);
@@ -922,6 +945,14 @@ __global__ __launch_bounds__(256 * RW, D == 64 ? 3 : 2) void packed_dkdv_kernel(
     }
     // (2 KS products, 2 KS reads and the 4 of -D; with D = 128 there are no registers for it)
     if constexpr (!V_LDS) reads_ahead<8, 2 * KS - 4, 1, 4>();
+    if (mask) {
+      // A weight of zero does not silence a row of Q or dO that is not finite, to the keys that
+      // it does not see (as in packed_attn_kernel); such a row shows in S or dP of every key.
+      float sum = 0.f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sum = fmaf(s[r], 0.f, fmaf(dp[r], 0.f, sum));
+      odd = __any(sum != sum);
+    }
     float w[16], e[16];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -942,16 +973,6 @@ __global__ __launch_bounds__(256 * RW, D == 64 ? 3 : 2) void packed_dkdv_kernel(
         w[r] = sees ? w[r] : 0.f;
         e[r] = sees ? e[r] : 0.f;
       }
-      // values that are not finite in rows that do not see the key (as in packed_dq_kernel)
-      uint32_t seen = 0;
-#pragma unroll
-      for (int i = 0; i < DS * 2; ++i) {
-        const u32x4_t x = tr.read(sg, r0 + (i & 1) * 16, i >> 1);
-        const u32x4_t y = tr.read(sq, r0 + (i & 1) * 16, i >> 1);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) seen = exponents2(exponents2(seen, x[j]), y[j]);
-      }
-      odd = __any(not_finite2(seen));
       if (odd) {
         for (int j = r0; j < r0 + 32; ++j) {
           const bool sees = t * BR + j <= rhi && t * BR + j >= rlo;
@@ -1028,28 +1049,30 @@ __global__ __launch_bounds__(256 * RW, D == 64 ? 3 : 2) void packed_dkdv_kernel(
       if (first(t, sq, r0, bw, be, odd)) second(sq, r0, bw, be, odd);
     }
   }
-  // the second halves' sums, through LDS
+  // the rows' shares meet, through LDS
   float* meet = reinterpret_cast<float*>(lds) + (wk * 64 + lane) * 4;
+  constexpr int PIECE = KW * 64 * 4, ALL = DS * 4 * PIECE;
   auto add = [&](f32x16_t (&x)[DS]) {
     __syncthreads();
+    if (wr) {
 #pragma unroll
-    for (int i = 0; i < DS * 4; ++i) {
-      f32x4_t* at = reinterpret_cast<f32x4_t*>(meet + i * 1024);
-      if (wr) {
-        *at = f32x4_t{x[i >> 2][4 * (i & 3)], x[i >> 2][4 * (i & 3) + 1], x[i >> 2][4 * (i & 3) + 2],
-                      x[i >> 2][4 * (i & 3) + 3]};
-      }
+      for (int i = 0; i < DS * 4; ++i)
+        *reinterpret_cast<f32x4_t*>(meet + (wr - 1) * ALL + i * PIECE) =
+            f32x4_t{x[i >> 2][4 * (i & 3)], x[i >> 2][4 * (i & 3) + 1], x[i >> 2][4 * (i & 3) + 2],
+                    x[i >> 2][4 * (i & 3) + 3]};
     }
     __syncthreads();
     if (wr) return;
 #pragma unroll
-    for (int i = 0; i < DS * 4; ++i) {
-      const f32x4_t y = *reinterpret_cast<f32x4_t*>(meet + i * 1024);
+    for (int i = 0; i < DS * 4; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[i >> 2][4 * (i & 3) + e] += y[e];
-    }
+      for (int w = 0; w < RW - 1; ++w) {
+        const f32x4_t y = *reinterpret_cast<f32x4_t*>(meet + w * ALL + i * PIECE);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[i >> 2][4 * (i & 3) + e] += y[e];
+      }
   };
-  if constexpr (RW == 2) {
+  if constexpr (RW > 1) {
     add(dk);
     add(dv);
   }
@@ -1419,8 +1442,12 @@ int launch_packed_attention_backward(const PackedAttnArgs& a, const PackedGradAr
   p.stat_tiles = (p.a.rows + 63) / 64;
   const bool f32 = a.dtype == BLT_DTYPE_F32;
   const int64_t nq = plan_tiles(p.a, p.a.rows, f32 ? 32 : 128, a.Hkv);
+  // Keys of a tile.  With few tiles the longest takes longer than a CU's share of the work:
+  // half as many keys, and twice the rows at a time (32 / 8 heads of 128: one sequence of 4096
+  // 311 us, 433 with 128 keys; four of up to 4096, 9 k tokens, 676 and 738; four of 4096 1254 and 1164).
+  const int bk = f32 ? 32 : a.d == 128 && (int64_t)a.Hkv * ((a.total + 127) / 128) <= 768 ? 64 : 128;
   GArgs pk = p;
-  const int64_t nk = plan_tiles(pk.a, p.a.total, f32 ? 32 : 128, a.Hkv);
+  const int64_t nk = plan_tiles(pk.a, p.a.total, bk, a.Hkv);
   if (nq > 0x7fffffff || nk > 0x7fffffff)
     return fail(BLT_ERR_SHAPE, "packed_attention_backward: too many tiles");
   const dim3 gq((unsigned)nq), gk((unsigned)nk), block(256);
@@ -1432,10 +1459,13 @@ int launch_packed_attention_backward(const PackedAttnArgs& a, const PackedGradAr
     hipLaunchKernelGGL((packed_dkdv_f32_kernel<4>), gk, block, 0, s, pk);
   } else if (a.d == 64) {
     hipLaunchKernelGGL((packed_dq_kernel<64>), gq, block, 0, s, p);
-    hipLaunchKernelGGL((packed_dkdv_kernel<64, 1, 64>), gk, block, 0, s, pk);
+    hipLaunchKernelGGL((packed_dkdv_kernel<64, 4, 1, 64>), gk, block, 0, s, pk);
   } else {
     hipLaunchKernelGGL((packed_dq_kernel<128>), gq, block, 0, s, p);
-    hipLaunchKernelGGL((packed_dkdv_kernel<128, 2, 64>), gk, dim3(512), 0, s, pk);
+    if (bk == 64)
+      hipLaunchKernelGGL((packed_dkdv_kernel<128, 2, 4, 128>), gk, dim3(512), 0, s, pk);
+    else
+      hipLaunchKernelGGL((packed_dkdv_kernel<128, 4, 2, 64>), gk, dim3(512), 0, s, pk);
   }
   BLT_LAUNCH_CHECK("packed_dq_kernel, packed_dkdv_kernel");
   return 0;
