@@ -15,14 +15,15 @@
 //
 // By the size of the vocabulary: up to 1024 a wave holds a row in registers and bisects
 // the cut over the bits of the logits; up to 16384 a block holds it in LDS and counts bins; above that rows are
-// cut into parts, in five launches (the largest logit, the parts' bins, the cut, the kept
-// sums of the parts, the token).
+// cut into parts, in five launches.
 #include "sample.hpp"
 
 namespace blt {
 
 namespace {
 
+struct Found;
+struct Entry;
 struct SArgs {
   const void* x;
   int64_t st;  // row stride
@@ -38,7 +39,9 @@ struct SArgs {
   uint64_t* pmass;  // [rows][parts]
   uint64_t* hm;     // [rows][parts][NB]
   uint32_t* hc;     // [rows][parts][NB]
-  int2* cut;        // [rows]: see Cut
+  Found* found;  // [rows]
+  Entry* list;   // [rows][parts][NT]
+  int* count;           // [rows][parts]: entries of it
 };
 
 template <typename T>
@@ -46,13 +49,10 @@ __device__ inline float logit(const void* x, int64_t i) {
   if constexpr (sizeof(T) == 2) return bf16_to_f32(((const uint16_t*)x)[i]);
   else return ((const float*)x)[i];
 }
-// an integer that orders as the value does (-0 as 0), and back
+// an integer that orders as the value does (-0 as 0)
 __device__ inline uint32_t key_of(float x) {
   const uint32_t b = __float_as_uint(x + 0.f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
-}
-__device__ inline float value_of(uint32_t key) {
-  return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
 }
 // the last kept (logit, index): tokens with a larger key, or the same and an index up to this
 struct Cut {
@@ -66,6 +66,7 @@ __device__ inline bool kept(const Cut& c, uint32_t key, int i) {
 // ---- a row's rules ---------------------------------------------------------------------
 struct Rules {
   double a;     // log2(e) / temperature
+  float a32;
   double p;     // top_p; 1 or more: off
   uint64_t m;   // smallest weight kept
   int k;        // 0: off
@@ -83,6 +84,7 @@ __device__ inline Rules rules_of(const SArgs& g, int64_t row) {
   r.good = t >= 0. && t < (double)INFINITY && p > 0. && m >= 0. && m <= 1. && k >= 0 &&
            g.u[row] == g.u[row];
   r.a = t > 0. ? 1.4426950408889634074 / t : 1.;
+  r.a32 = (float)r.a;
   r.p = p;
   r.m = (uint64_t)ceil(ldexp(m, g.scale));
   r.k = t > 0. ? k : 1;  // (temperature 0: the first of the largest)
@@ -91,10 +93,31 @@ __device__ inline Rules rules_of(const SArgs& g, int64_t row) {
   r.bins = (float)((NB - 1) / 63. * r.a);
   return r;
 }
-__device__ inline uint64_t weight(float x, float top, const Rules& r, int scale) {
+// 2^(j / 64), which a block keeps in LDS
+struct Powers {
+  double of[64];
+};
+__device__ inline void fill(Powers& p) {  // (a barrier before their use)
+  if (threadIdx.x < 64) p.of[threadIdx.x] = exp2((double)threadIdx.x / 64.);
+}
+// 2^(scale - (top - x) a) as an integer: 2^y with y = k / 64 + f, |f| <= 1 / 128, is 2^(k / 64) times
+// the series of 2^f up to f^4, off by less than 2^-44; its mantissa is shifted to its place.
+// The largest logit has 2^scale exactly, equal ones equal weights.
+__device__ inline uint64_t weight(float x, float top, const Rules& r, int scale, const Powers& pw) {
   if (x == top) return (uint64_t)1 << scale;
-  const double y = (double)scale - ((double)top - (double)x) * r.a;
-  return y > -2. ? (uint64_t)rint(exp2(y)) : 0;
+  if (!((x - top) * r.a32 > -70.f)) return 0;  // (below 2^-70: scale <= 62)
+  constexpr double L = 0.693147180559945309417;
+  constexpr double c2 = L * L / 2, c3 = c2 * L / 3, c4 = c3 * L / 4;
+  constexpr double M = 1.5 * 70368744177664.;  // 2^46: the sum below is a multiple of 1 / 64
+  const double y = ((double)x - (double)top) * r.a;
+  const double t = y + M, f = y - (t - M);
+  const int k = (int)(uint32_t)__double_as_longlong(t);
+  const double v = pw.of[k & 63] * fma(fma(fma(fma(c4, f, c3), f, c2), f, L), f, 1.);
+  const uint64_t b = (uint64_t)__double_as_longlong(v);
+  // mantissa times 2^(exponent - 52 + k / 64 + scale), half of the last place up
+  const uint64_t m = (b & 0xfffffffffffffull) | 0x10000000000000ull;
+  const int shift = 52 + 1023 - scale - (int)(b >> 52) - (k >> 6);  // >= -10
+  return shift > 0 ? ((m >> (min(shift, 55) - 1)) + 1) >> 1 : m << -shift;
 }
 // a bin of about the same logits, the largest ones first; the order of bins is that of logits
 __device__ inline int bin_of(float x, float top, const Rules& r) {
@@ -147,6 +170,9 @@ __device__ inline int bits(uint64_t mask) { return __popcll((unsigned long long)
 // ---- up to 1024 tokens: one wave a row ------------------------------------------------------
 template <typename T, int N>
 __global__ __launch_bounds__(256) void sample_wave_kernel(SArgs g) {
+  __shared__ Powers pw;
+  fill(pw);
+  __syncthreads();
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= g.rows) return;
   const int lane = threadIdx.x & 63;
@@ -170,7 +196,7 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(SArgs g) {
   }
   uint64_t w[N];
 #pragma unroll
-  for (int j = 0; j < N; ++j) w[j] = weight(v[j], top, r, g.scale);
+  for (int j = 0; j < N; ++j) w[j] = weight(v[j], top, r, g.scale, pw);
   auto count = [&](uint32_t c) {
     int n = 0;
 #pragma unroll
@@ -288,6 +314,22 @@ struct Held {
     for (int j = 0; j < N; ++j) f(x[j], first + 64 * j < n ? first + 64 * j : -1, j);
   }
 };
+struct InLds {
+  const float* x;
+  int n, run;
+  __device__ inline InLds(const float* x_, int n_) : x(x_), n(n_) {
+    run = ((n + NW - 1) / NW + 63) & ~63;
+  }
+  template <typename F>
+  __device__ inline void each(F f) const {
+    const int a = (int)(threadIdx.x >> 6) * run, lane = threadIdx.x & 63;
+#pragma unroll 2
+    for (int j = 0; j < run; j += 64) {
+      const int i = a + j + lane;
+      f(i < n ? x[i] : -INFINITY, i < n ? i : -1, j / 64);
+    }
+  }
+};
 template <typename T>
 struct InMemory {
   const void* row;
@@ -314,21 +356,20 @@ struct InMemory {
   }
 };
 
+constexpr int FEW = 64;
 struct Room {
   uint64_t m[NB];  // bins: sum of weights and tokens
   uint32_t c[NB];
-  uint32_t lk[NT];  // a bin's tokens
-  uint64_t lw[NT];
-  int li[NT];
-  uint64_t wm[NW];  // of the waves
+  uint64_t lc[FEW], lw[FEW];  // a bin's tokens, when they are few
+  uint64_t wm[NW];            // of the waves
   uint32_t wc[NW], wx[NW];
   int n;
-  Cut cut;
-  uint64_t sum;
+  uint64_t code, sum;
   // a bin, and what lies above it
-  int bin;
+  int bin, bin0;
   uint32_t above_c, in_c;
   uint64_t above_m;
+  Powers pw;
 };
 __device__ inline void zero_bins(Room& s) {
   for (int i = threadIdx.x; i < NB; i += NT) {
@@ -336,8 +377,8 @@ __device__ inline void zero_bins(Room& s) {
     s.c[i] = 0;
   }
 }
-__device__ inline void add_to_bin(Room& s, int b, uint64_t w) {
-  atomicAdd(&s.c[b], 1u);
+__device__ inline void add_to_bin(Room& s, int b, uint64_t w, bool count = true) {
+  if (count) atomicAdd(&s.c[b], 1u);
   if (w) atomicAdd((unsigned long long*)&s.m[b], (unsigned long long)w);
 }
 // Two bins of a thread and what lies above them.
@@ -394,122 +435,104 @@ __device__ inline void locate(Room& s, const Bins& b, bool by_count, uint64_t wa
   }
   __syncthreads();
 }
-// The t-th token with this key, in the order of the indices.
-template <typename Row>
-__device__ int tie_index(const Row& row, Room& s, uint32_t key, uint32_t t) {
-  const int w = threadIdx.x >> 6;
-  uint32_t n = 0;
-  row.each([&](float x, int i, int) { n += bits(__ballot(i >= 0 && key_of(x) == key)); });
-  if ((threadIdx.x & 63) == 0) s.wc[w] = n;
-  if (threadIdx.x == 0) s.n = 0;
-  __syncthreads();
-  uint32_t before = 0;
-  for (int i = 0; i < w; ++i) before += s.wc[i];
-  if (before < t && t <= before + n)
-    row.each([&](float x, int i, int) {
-      const bool tie = i >= 0 && key_of(x) == key;
-      const uint64_t all = __ballot(tie);
-      if (tie && before + (uint32_t)below(all) + 1 == t) s.n = i;
-      before += bits(all);
-    });
-  __syncthreads();
-  const int at = s.n;
-  __syncthreads();
-  return at;
+// Tokens have a code, an integer of their own whose order is that of the selection:
+// their rank's (logits descending, then indices ascending) or their index.
+__device__ inline uint64_t rank_code(float x, int i) {
+  return (uint64_t)~key_of(x) << 32 | (uint32_t)i;
 }
-// The token in bin s.bin where the running count (or sum) reaches `want`: with few tokens in it each
-// finds its own rank among them; with more, bins of bins over the bits of the keys, at most
-// three times, until they are few or have one key.  `sum`: the running sum with it.
-template <typename Row>
-__device__ Cut refine(const Row& row, Room& s, const Rules& r, float top, int scale,
-                      bool by_count, uint64_t want, uint64_t& sum) {
-  const int tid = threadIdx.x, bin = s.bin;
-  uint32_t lo = 0, hi = 0xffffffffu;
-  auto member = [&](float x, int i) {
-    const uint32_t k = key_of(x);
-    return i >= 0 && k >= lo && k <= hi && bin_of(x, top, r) == bin;
-  };
+__device__ inline Cut cut_of(uint64_t code) {
+  return Cut{~(uint32_t)(code >> 32), (int)(uint32_t)code};
+}
+// The code at which the running count (or sum of weights) of the tokens that code_of takes
+// (it gives false for others) reaches `want`, in the order of the codes, and that sum.  s.in_c: how many they
+// are, at most (with in_c above FEW any number); s.above_c, s.above_m: what counts as before
+// them.  More than a few are put into bins over the bits of their codes, until there are
+// few in one; those find their own places.
+template <typename Row, typename Code>
+__device__ uint64_t select(const Row& row, Room& s, Code code_of, bool by_count, uint64_t want,
+                           uint64_t& sum) {
+  const int tid = threadIdx.x;
+  uint64_t lo = 0, hi = ~(uint64_t)0;
   for (bool first = true;; first = false) {
     const uint32_t n = s.in_c, above_c = s.above_c;
     const uint64_t above_m = s.above_m;
-    if (n <= NT) {
+    if (n <= FEW) {
       if (tid == 0) s.n = 0;
       __syncthreads();
       row.each([&](float x, int i, int) {
-        if (member(x, i)) {
+        uint64_t c, w;
+        if (i >= 0 && code_of(x, i, c, w) && c >= lo && c <= hi) {
           const int at = atomicAdd(&s.n, 1);
-          s.lk[at] = key_of(x);
-          s.li[at] = i;
-          s.lw[at] = weight(x, top, r, scale);
+          s.lc[at] = c;
+          s.lw[at] = w;
         }
       });
       __syncthreads();
-      if (tid < (int)n) {
-        const uint32_t k = s.lk[tid];
-        const int at = s.li[tid];
+      const int m = s.n;
+      if (tid < m) {
+        const uint64_t c = s.lc[tid], w = s.lw[tid];
         uint32_t rank = above_c;
         uint64_t before = above_m;
-        for (int j = 0; j < (int)n; ++j) {
-          const uint32_t kj = s.lk[j];
-          const bool better = kj > k || (kj == k && s.li[j] < at);
+        for (int j = 0; j < m; ++j) {
+          const bool better = s.lc[j] < c;
           rank += better ? 1 : 0;
           before += better ? s.lw[j] : 0;
         }
-        const uint64_t w = s.lw[tid];
         if (by_count ? rank + 1 == (uint32_t)want : before < want && want <= before + w) {
-          s.cut = Cut{k, at};
+          s.code = c;
           s.sum = before + w;
         }
       }
       __syncthreads();
-      const Cut c = s.cut;
+      const uint64_t c = s.code;
       sum = s.sum;
       __syncthreads();
       return c;
     }
-    if (first) {
-      uint32_t a = 0xffffffffu, b = 0;
+    if (first) {  // the range of their upper halves, and of the lower ones if those are equal
+      uint32_t a = 0xffffffffu, b = 0, a0 = 0xffffffffu, b0 = 0;
       row.each([&](float x, int i, int) {
-        if (member(x, i)) {
-          a = min(a, key_of(x));
-          b = max(b, key_of(x));
+        uint64_t c, w;
+        if (i >= 0 && code_of(x, i, c, w)) {
+          a = min(a, (uint32_t)(c >> 32));
+          b = max(b, (uint32_t)(c >> 32));
+          a0 = min(a0, (uint32_t)c);
+          b0 = max(b0, (uint32_t)c);
         }
       });
+      if (tid == 0) {
+        s.wc[0] = s.wx[0] = 0xffffffffu;
+        s.wc[1] = s.wx[1] = 0;
+      }
       a = wave_min_u32(a);
       b = wave_max_u32(b);
+      a0 = wave_min_u32(a0);
+      b0 = wave_max_u32(b0);
+      __syncthreads();
       if ((tid & 63) == 0) {
-        s.wc[tid >> 6] = a;
-        s.wx[tid >> 6] = b;
+        atomicMin(&s.wc[0], a);
+        atomicMax(&s.wc[1], b);
+        atomicMin(&s.wx[0], a0);
+        atomicMax(&s.wx[1], b0);
       }
       __syncthreads();
-      lo = 0xffffffffu;
-      hi = 0;
-      for (int i = 0; i < NW; ++i) {
-        lo = min(lo, s.wc[i]);
-        hi = max(hi, s.wx[i]);
-      }
+      const bool one = s.wc[0] == s.wc[1];
+      lo = (uint64_t)s.wc[0] << 32 | (one ? s.wx[0] : 0);
+      hi = (uint64_t)s.wc[1] << 32 | (one ? s.wx[1] : 0xffffffffu);
       __syncthreads();
     }
-    if (lo == hi) {
-      const uint64_t w = weight(value_of(lo), top, r, scale);
-      // (by sums the bin's weight is not 0)
-      const uint64_t t = by_count ? want - above_c : (want - above_m + w - 1) / w;
-      sum = above_m + t * w;
-      return Cut{lo, tie_index(row, s, lo, (uint32_t)t)};
-    }
-    const int shift = max(0, 32 - __clz((int)(hi - lo)) - 11);
+    const int shift = max(0, 64 - __clzll((long long)(hi - lo)) - 11);
     zero_bins(s);
     __syncthreads();
     row.each([&](float x, int i, int) {
-      if (member(x, i))
-        add_to_bin(s, NB - 1 - (int)((key_of(x) - lo) >> shift), weight(x, top, r, scale));
+      uint64_t c, w;
+      if (i >= 0 && code_of(x, i, c, w) && c >= lo && c <= hi) add_to_bin(s, (int)((c - lo) >> shift), w);
     });
     __syncthreads();
     const Bins b = scan_bins(s);
     locate(s, b, by_count, want - (by_count ? above_c : above_m));
-    const uint32_t base = lo + ((uint32_t)(NB - 1 - s.bin) << shift);
-    lo = base;
-    hi = min(hi, base + ((1u << shift) - 1));
+    lo += (uint64_t)s.bin << shift;
+    hi = min(hi, lo + (((uint64_t)1 << shift) - 1));
     __syncthreads();
     if (tid == 0) {
       s.above_c += above_c;
@@ -525,29 +548,34 @@ __device__ Cut find_cut(const Row& row, Room& s, const Rules& r, float top, int 
   if (!r.k && !(r.p < 1.)) return c;
   const Bins b = scan_bins(s);
   uint64_t sum = b.total_m, unused;
-  if (r.k) {
-    locate(s, b, true, (uint64_t)r.k);
-    c = refine(row, s, r, top, scale, true, (uint64_t)r.k, sum);
-  }
-  if (r.p < 1.) {
-    const uint64_t want = wanted(r.p, sum);
-    locate(s, b, false, want);
-    c = refine(row, s, r, top, scale, false, want, unused);
-  }
+  auto in_bin = [&](float x, int i, uint64_t& code, uint64_t& w) {
+    if (bin_of(x, top, r) != s.bin0) return false;
+    code = rank_code(x, i);
+    w = weight(x, top, r, scale, s.pw);
+    return true;
+  };
+  auto end_of = [&](bool by_count, uint64_t want, uint64_t& upto) {
+    locate(s, b, by_count, want);
+    if (threadIdx.x == 0) s.bin0 = s.bin;
+    __syncthreads();
+    return cut_of(select(row, s, in_bin, by_count, want, upto));
+  };
+  if (r.k) c = end_of(true, (uint64_t)r.k, sum);
+  if (r.p < 1.) c = end_of(false, wanted(r.p, sum), unused);
   return c;
 }
 // The token of tokens [0, n): the first whose running sum of kept weights is above u times
 // their sum or (known) above `aim`.
-template <typename Row, int N>
+template <typename Row>
 __device__ int draw(const Row& row, Room& s, const Rules& r, float top, int scale, const Cut& cut,
                     float u, bool known, uint64_t aim) {
   const int wid = threadIdx.x >> 6;
-  uint64_t w[N], mine = 0;
-  row.each([&](float x, int i, int j) {
-    const uint64_t y = i >= 0 && kept(cut, key_of(x), i) ? weight(x, top, r, scale) : 0;
-    w[j] = y >= r.m ? y : 0;
-    mine += w[j];
-  });
+  auto mass = [&](float x, int i) {
+    const uint64_t w = i >= 0 && kept(cut, key_of(x), i) ? weight(x, top, r, scale, s.pw) : 0;
+    return w >= r.m ? w : 0;
+  };
+  uint64_t mine = 0;
+  row.each([&](float x, int i, int) { mine += mass(x, i); });
   mine = sum_u64(mine);
   if ((threadIdx.x & 63) == 0) s.wm[wid] = mine;
   if (threadIdx.x == 0) s.n = -1;
@@ -558,10 +586,10 @@ __device__ int draw(const Row& row, Room& s, const Rules& r, float top, int scal
     total += s.wm[i];
   }
   if (!known) aim = aim_of(u, total);
-  if (run <= aim && aim < run + mine) {
+  if (run <= aim && aim < run + mine) {  // (one wave's run)
     int token = -1;
-    row.each([&](float, int i, int j) {
-      const uint64_t at = incl_scan_u64(w[j]);
+    row.each([&](float x, int i, int) {
+      const uint64_t at = incl_scan_u64(mass(x, i));
       const uint64_t hit = __ballot(run + at > aim);
       if (token < 0 && hit) token = __builtin_amdgcn_readlane(i, __ffsll((unsigned long long)hit) - 1);
       run += lane_u64(at, 63);
@@ -589,37 +617,69 @@ __device__ inline float block_top(Room& s, float x, bool nan) {
 }
 
 // ---- up to 16384 tokens: one block a row -------------------------------------------------------
-template <typename T, int N>
+template <typename T>
 __global__ __launch_bounds__(NT) void sample_block_kernel(SArgs g) {
   __shared__ Room s;
+  __shared__ float held[PART];
   const int64_t row = blockIdx.x;
-  const Held<T, N> x((const char*)g.x + row * g.st * (int64_t)sizeof(T), 0, g.V);
+  fill(s.pw);
   float m = -INFINITY;
   bool nan = false;
-  x.each([&](float v, int, int) {
-    m = fmaxf(m, v);
-    nan |= v != v;
-  });
+  {
+    const char* from = (const char*)g.x + row * g.st * (int64_t)sizeof(T);
+    float v[PART / NT];
+#pragma unroll
+    for (int j = 0; j < PART / NT; ++j) {
+      const int i = (int)threadIdx.x + NT * j;
+      v[j] = i < g.V ? logit<T>(from, i) : -INFINITY;
+    }
+#pragma unroll
+    for (int j = 0; j < PART / NT; ++j) {
+      if ((int)threadIdx.x + NT * j < g.V) held[threadIdx.x + NT * j] = v[j];
+      m = fmaxf(m, v[j]);
+      nan |= v[j] != v[j];
+    }
+  }
   const float top = block_top(s, m, nan);
   const Rules r = rules_of(g, row);
   if (!(top > -INFINITY) || !r.good) {
     if (threadIdx.x == 0) g.out[row] = -1;
     return;
   }
+  const InLds x(held, g.V);
   if (r.k || r.p < 1.) {
     zero_bins(s);
     __syncthreads();
     x.each([&](float v, int i, int) {
-      if (i >= 0) add_to_bin(s, bin_of(v, top, r), weight(v, top, r, g.scale));
+      if (i >= 0) add_to_bin(s, bin_of(v, top, r), r.p < 1. ? weight(v, top, r, g.scale, s.pw) : 0);
     });
     __syncthreads();
   }
   const Cut cut = find_cut(x, s, r, top, g.scale);
-  const int token = draw<Held<T, N>, N>(x, s, r, top, g.scale, cut, g.u[row], false, 0);
+  const int token = draw(x, s, r, top, g.scale, cut, g.u[row], false, 0);
   if (threadIdx.x == 0) g.out[row] = token;
 }
 
 // ---- more: parts of rows ------------------------------------------------------------------------
+// The launches: every part's largest logit; the bins of every part; for every row the bins in
+// which its rules end, from their sums; of every part the tokens that decide (listed) and the
+// weights that are kept whatever they decide; for every row the token.  What is listed:
+//   with top_k     all tokens down to the bin in which it ends: they decide everything
+//   with top_p     those of the bin in which it ends; what lies above is kept
+// Where that are more than a block ranks at once, the cut is found by passes over the row.
+enum Way { ALL, TOP, BIN, CUT };  // (no rule but min_p; lists; a cut that is known)
+struct Found {
+  int way, bin;
+  uint32_t above_c, key;
+  int index;
+  uint32_t pad;
+  uint64_t above_m, want;  // want: of top_p
+};
+struct Entry {
+  float x;
+  int index;
+  uint64_t w;
+};
 __device__ inline float row_top(const SArgs& g, int64_t row) {
   float m = -INFINITY;
   bool nan = false;
@@ -656,65 +716,114 @@ __global__ __launch_bounds__(NT) void sample_bins_kernel(SArgs g) {
   __shared__ Room s;
   const int64_t row = blockIdx.x / g.parts;
   const int part = (int)(blockIdx.x - row * g.parts);
+  const Held<T, 16> x = part_of<T>(g, row, part);
   const float top = row_top(g, row);
   const Rules r = rules_of(g, row);
   if (!(top > -INFINITY) || !r.good || (!r.k && !(r.p < 1.))) return;
-  const Held<T, 16> x = part_of<T>(g, row, part);
+  fill(s.pw);
   zero_bins(s);
   __syncthreads();
   x.each([&](float v, int i, int) {
-    if (i >= 0) add_to_bin(s, bin_of(v, top, r), weight(v, top, r, g.scale));
+    if (i >= 0)
+      add_to_bin(s, bin_of(v, top, r), r.p < 1. ? weight(v, top, r, g.scale, s.pw) : 0, r.k > 0);
   });
   __syncthreads();
   const int64_t at = (row * g.parts + part) * NB;
   for (int i = threadIdx.x; i < NB; i += NT) {
-    g.hm[at + i] = s.m[i];
-    g.hc[at + i] = s.c[i];
+    if (r.p < 1.) g.hm[at + i] = s.m[i];
+    if (r.k) g.hc[at + i] = s.c[i];
   }
 }
 template <typename T>
-__global__ __launch_bounds__(NT) void sample_cut_kernel(SArgs g) {
+__global__ __launch_bounds__(NT) void sample_find_kernel(SArgs g) {
   __shared__ Room s;
   const int64_t row = blockIdx.x;
   const float top = row_top(g, row);
   const Rules r = rules_of(g, row);
   if (!(top > -INFINITY) || !r.good) return;
+  Found f{};
+  f.way = ALL;
   if (r.k || r.p < 1.) {
-    for (int i = threadIdx.x; i < NB; i += NT) {
-      uint64_t m = 0;
-      uint32_t c = 0;
-      for (int part = 0; part < g.parts; ++part) {
-        const int64_t at = (row * g.parts + part) * NB + i;
-        m += g.hm[at];
-        c += g.hc[at];
+    uint64_t m[2] = {0, 0};
+    uint32_t c[2] = {0, 0};
+    for (int part = 0; part < g.parts; ++part) {
+      const int64_t at = (row * g.parts + part) * NB + 2 * threadIdx.x;
+      if (r.p < 1.) {
+        m[0] += g.hm[at];
+        m[1] += g.hm[at + 1];
       }
-      s.m[i] = m;
-      s.c[i] = c;
+      if (r.k) {
+        c[0] += g.hc[at];
+        c[1] += g.hc[at + 1];
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      s.m[2 * threadIdx.x + q] = m[q];
+      s.c[2 * threadIdx.x + q] = c[q];
     }
     __syncthreads();
+    const Bins b = scan_bins(s);
+    if (r.k) {
+      locate(s, b, true, (uint64_t)r.k);
+      f.way = s.above_c + s.in_c <= NT ? TOP : CUT;
+      f.bin = s.bin;
+    } else {
+      f.want = wanted(r.p, b.total_m);
+      locate(s, b, false, f.want);
+      f.way = BIN;
+      f.bin = s.bin;
+      f.above_m = s.above_m;
+    }
+    if (f.way == CUT) {  // (top_k beyond a list)
+      const InMemory<T> x((const char*)g.x + row * g.st * (int64_t)sizeof(T), g.V);
+      fill(s.pw);
+      __syncthreads();
+      const Cut cut = find_cut(x, s, r, top, g.scale);
+      f.key = cut.key;
+      f.index = cut.index;
+    }
   }
-  const InMemory<T> x((const char*)g.x + row * g.st * (int64_t)sizeof(T), g.V);
-  const Cut c = find_cut(x, s, r, top, g.scale);
-  if (threadIdx.x == 0) g.cut[row] = int2{(int)c.key, c.index};
+  if (threadIdx.x == 0) g.found[row] = f;
 }
-__device__ inline Cut cut_in(const SArgs& g, int64_t row, int part) {
-  const int2 c = g.cut[row];
-  return Cut{(uint32_t)c.x, c.y - part * PART};
-}
+// weights kept of a part, and its list
 template <typename T>
-__global__ __launch_bounds__(NT) void sample_mass_kernel(SArgs g) {
+__global__ __launch_bounds__(NT) void sample_part_kernel(SArgs g) {
   __shared__ uint64_t wm[NW];
+  __shared__ int listed;
+  __shared__ Powers pw;
   const int64_t row = blockIdx.x / g.parts;
   const int part = (int)(blockIdx.x - row * g.parts);
+  const Held<T, 16> x = part_of<T>(g, row, part);
   const float top = row_top(g, row);
   const Rules r = rules_of(g, row);
   if (!(top > -INFINITY) || !r.good) return;
-  const Cut cut = cut_in(g, row, part);
-  const Held<T, 16> x = part_of<T>(g, row, part);
+  const Found f = g.found[row];
+  if (threadIdx.x == 0) listed = 0;
+  fill(pw);
+  __syncthreads();
+  const Cut cut{f.key, f.index - part * PART};
+  Entry* list = g.list + (row * g.parts + part) * NT;
   uint64_t m = 0;
+  // (without min_p the weights above the bin are those of the part's bins)
+  const bool sums = f.way == BIN && r.m == 0;
+  if (sums) {
+    const uint64_t* bins = g.hm + (row * g.parts + part) * NB;
+    for (int i = threadIdx.x; i < f.bin; i += NT) m += bins[i];
+  }
   x.each([&](float v, int i, int) {
-    const uint64_t y = i >= 0 && kept(cut, key_of(v), i) ? weight(v, top, r, g.scale) : 0;
-    m += y >= r.m ? y : 0;
+    if (i < 0) return;
+    const int bin = f.way == CUT || f.way == ALL ? 0 : bin_of(v, top, r);
+    const bool list_it = f.way == TOP ? bin <= f.bin : f.way == BIN && bin == f.bin;
+    const bool keep = f.way == ALL || (f.way == CUT && kept(cut, key_of(v), i)) ||
+                      (f.way == BIN && bin < f.bin && !sums);
+    if (!list_it && !keep) return;
+    const uint64_t w = weight(v, top, r, g.scale, pw);
+    if (keep) m += w >= r.m ? w : 0;
+    if (list_it) {
+      const int at = atomicAdd(&listed, 1);
+      if (at < NT) list[at] = Entry{v, part * PART + i, w};
+    }
   });
   m = sum_u64(m);
   if ((threadIdx.x & 63) == 0) wm[threadIdx.x >> 6] = m;
@@ -723,11 +832,20 @@ __global__ __launch_bounds__(NT) void sample_mass_kernel(SArgs g) {
     uint64_t all = 0;
     for (int i = 0; i < NW; ++i) all += wm[i];
     g.pmass[row * g.parts + part] = all;
+    g.count[row * g.parts + part] = listed;
   }
 }
+// the lists' tokens, one each in a thread's registers
+struct Listed {
+  float x;
+  int index;  // -1: none
+  template <typename F>
+  __device__ inline void each(F f) const { f(x, index, 0); }
+};
 template <typename T>
 __global__ __launch_bounds__(NT) void sample_pick_kernel(SArgs g) {
   __shared__ Room s;
+  __shared__ uint64_t extra[64];  // kept weights of the bin, by parts
   const int64_t row = blockIdx.x;
   const float top = row_top(g, row);
   const Rules r = rules_of(g, row);
@@ -735,18 +853,101 @@ __global__ __launch_bounds__(NT) void sample_pick_kernel(SArgs g) {
     if (threadIdx.x == 0) g.out[row] = -1;
     return;
   }
-  const int lane = threadIdx.x & 63;
-  // (parts <= 64: 2^20 tokens)
-  const uint64_t m = lane < g.parts ? g.pmass[row * g.parts + lane] : 0;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const Found f = g.found[row];
+  Cut cut{f.key, f.way == ALL ? 0x7fffffff : f.index};
+  fill(s.pw);
+  if (tid < 64) extra[tid] = 0;
+  if (f.way == TOP || f.way == BIN) {
+    // the parts' lists one behind the other (parts <= 64: 2^20 tokens)
+    const int n_of = lane < g.parts ? g.count[row * g.parts + lane] : 0;
+    const bool over = __any(n_of > NT);
+    const int upto = wave_incl_scan(min(n_of, NT)), n = __builtin_amdgcn_readlane(upto, 63);
+    if (tid == 0) {
+      s.above_c = 0;
+      s.above_m = f.way == BIN ? f.above_m : 0;
+      s.in_c = over ? 0xffffffffu : (uint32_t)n;
+    }
+    __syncthreads();
+    uint64_t sum;
+    if (over || n > NT) {  // (top_p's bin beyond a list)
+      const InMemory<T> x((const char*)g.x + row * g.st * (int64_t)sizeof(T), g.V);
+      auto in_bin = [&](float v, int i, uint64_t& c, uint64_t& w) {
+        if (bin_of(v, top, r) != f.bin) return false;
+        c = rank_code(v, i);
+        w = weight(v, top, r, g.scale, s.pw);
+        return true;
+      };
+      cut = cut_of(select(x, s, in_bin, false, f.want, sum));
+      x.each([&](float v, int i, int) {
+        if (i < 0 || bin_of(v, top, r) != f.bin || !kept(cut, key_of(v), i)) return;
+        const uint64_t w = weight(v, top, r, g.scale, s.pw);
+        if (w >= r.m) atomicAdd((unsigned long long*)&extra[i / PART], (unsigned long long)w);
+      });
+    } else {
+      int part = 0, before_part = 0;
+      for (int i = 0; i < g.parts; ++i) {
+        const int end = __builtin_amdgcn_readlane(upto, i);
+        part += end <= tid ? 1 : 0;
+        before_part = end <= tid ? end : before_part;
+      }
+      Entry e{0.f, -1, 0};
+      if (tid < n) e = g.list[(row * g.parts + part) * NT + tid - before_part];
+      const Listed x{e.x, e.index};
+      auto by_rank = [&](float v, int i, uint64_t& c, uint64_t& w) {
+        c = rank_code(v, i);
+        w = e.w;
+        return true;
+      };
+      auto restart = [&] {
+        if (tid == 0) {
+          s.above_c = 0;
+          s.above_m = f.way == BIN ? f.above_m : 0;
+          s.in_c = (uint32_t)n;
+        }
+        __syncthreads();
+      };
+      uint64_t want = f.want;
+      if (f.way == TOP) {
+        cut = cut_of(select(x, s, by_rank, true, (uint64_t)r.k, sum));
+        want = wanted(r.p, sum);
+      }
+      if (f.way == BIN || r.p < 1.) {
+        if (f.way == TOP) restart();
+        cut = cut_of(select(x, s, by_rank, false, want, sum));
+      }
+      const bool in = e.index >= 0 && kept(cut, key_of(e.x), e.index) && e.w >= r.m;
+      if (f.way == TOP) {  // the list has all that are kept: by index it decides
+        sum = sum_u64(in ? e.w : 0);
+        if (lane == 0) s.wm[tid >> 6] = sum;
+        __syncthreads();
+        sum = 0;
+        for (int i = 0; i < NW; ++i) sum += s.wm[i];
+        restart();
+        const uint64_t aim = aim_of(g.u[row], sum);
+        auto by_index = [&](float, int i, uint64_t& c, uint64_t& w) {
+          c = (uint32_t)i;
+          w = e.w;
+          return in;
+        };
+        const uint64_t token = select(x, s, by_index, false, aim + 1, sum);
+        if (tid == 0) g.out[row] = (int)token;
+        return;
+      }
+      if (in) atomicAdd((unsigned long long*)&extra[e.index / PART], (unsigned long long)e.w);
+    }
+  }
+  __syncthreads();
+  const uint64_t m = lane < g.parts ? g.pmass[row * g.parts + lane] + extra[lane] : 0;
   const uint64_t at = incl_scan_u64(m);
   const uint64_t aim = aim_of(g.u[row], lane_u64(at, 63));
   const uint64_t hit = __ballot(at > aim);
   const int part = __ffsll((unsigned long long)hit) - 1;
   const uint64_t before = lane_u64(at - m, part);
   const Held<T, 16> x = part_of<T>(g, row, part);
-  const int token = draw<Held<T, 16>, 16>(x, s, r, top, g.scale, cut_in(g, row, part), 0.f, true,
-                                          aim - before);
-  if (threadIdx.x == 0) g.out[row] = part * PART + token;
+  const int token = draw(x, s, r, top, g.scale, Cut{cut.key, cut.index - part * PART}, 0.f, true,
+                         aim - before);
+  if (tid == 0) g.out[row] = part * PART + token;
 }
 
 int parts_of(int vocab) { return vocab <= PART ? 0 : (vocab + PART - 1) / PART; }
@@ -766,19 +967,16 @@ int run(const SArgs& g, hipStream_t s) {
     else
       hipLaunchKernelGGL((sample_wave_kernel<T, 16>), grid, block, 0, s, g);
   } else if (g.V <= PART) {
-    const dim3 grid((unsigned)g.rows), block(NT);
-    if (g.V <= 4 * NT)
-      hipLaunchKernelGGL((sample_block_kernel<T, 4>), grid, block, 0, s, g);
-    else if (g.V <= 8 * NT)
-      hipLaunchKernelGGL((sample_block_kernel<T, 8>), grid, block, 0, s, g);
-    else
-      hipLaunchKernelGGL((sample_block_kernel<T, 16>), grid, block, 0, s, g);
+    hipLaunchKernelGGL((sample_block_kernel<T>), dim3((unsigned)g.rows), dim3(NT), 0, s, g);
   } else {
     const dim3 all((unsigned)(g.rows * g.parts)), one((unsigned)g.rows), block(NT);
     hipLaunchKernelGGL((sample_top_kernel<T>), all, block, 0, s, g);
-    hipLaunchKernelGGL((sample_bins_kernel<T>), all, block, 0, s, g);
-    hipLaunchKernelGGL((sample_cut_kernel<T>), one, block, 0, s, g);
-    hipLaunchKernelGGL((sample_mass_kernel<T>), all, block, 0, s, g);
+    // (without top_k and top_p for any row there is nothing to find)
+    if (g.s.top_ks || g.s.top_ps || g.s.temperatures || g.s.temperature == 0. || g.s.top_k > 0 ||
+        g.s.top_p < 1.)
+      hipLaunchKernelGGL((sample_bins_kernel<T>), all, block, 0, s, g);
+    hipLaunchKernelGGL((sample_find_kernel<T>), one, block, 0, s, g);
+    hipLaunchKernelGGL((sample_part_kernel<T>), all, block, 0, s, g);
     hipLaunchKernelGGL((sample_pick_kernel<T>), one, block, 0, s, g);
   }
   BLT_LAUNCH_CHECK("sample");
@@ -789,7 +987,7 @@ int run(const SArgs& g, hipStream_t s) {
 
 int64_t sample_workspace_bytes(int64_t rows, int vocab) {
   const int64_t parts = parts_of(vocab);
-  return parts ? rows * (parts * (12 * (int64_t)NB + 16) + 16) : 0;
+  return parts ? rows * (parts * (12 * (int64_t)NB + sizeof(Entry) * NT + 16) + sizeof(Found)) : 0;
 }
 
 int launch_sample(const SampleArgs& a, void* ws, hipStream_t s) {
@@ -806,9 +1004,11 @@ int launch_sample(const SampleArgs& a, void* ws, hipStream_t s) {
   if (g.parts) {
     g.hm = (uint64_t*)ws;
     g.pmass = g.hm + n * NB;
-    g.cut = (int2*)(g.pmass + n);
-    g.hc = (uint32_t*)(g.cut + a.rows);
+    g.list = (Entry*)(g.pmass + n);
+    g.found = (Found*)(g.list + n * NT);
+    g.hc = (uint32_t*)(g.found + a.rows);
     g.pmax = (float*)(g.hc + n * NB);
+    g.count = (int*)(g.pmax + n);
   }
   return a.dtype == BLT_DTYPE_BF16 ? run<uint16_t>(g, s) : run<float>(g, s);
 }
