@@ -120,10 +120,11 @@ __device__ inline uint64_t weight(float x, float top, const Rules& r, int scale,
   return shift > 0 ? ((m >> (min(shift, 55) - 1)) + 1) >> 1 : m << -shift;
 }
 // a bin of about the same logits, the largest ones first; the order of bins is that of logits
-__device__ inline int bin_of(float x, float top, const Rules& r) {
+__device__ inline float place_of(float x, float top, const Rules& r) {
   const float t = (top - x) * r.bins;
-  return x == top ? 0 : t < (float)(NB - 1) ? (int)t : NB - 1;
+  return x == top ? 0.f : t < (float)(NB - 1) ? t : (float)(NB - 1);
 }
+__device__ inline int bin_of(float x, float top, const Rules& r) { return (int)place_of(x, top, r); }
 __device__ inline uint64_t wanted(double p, uint64_t sum) {  // least running sum >= p * sum
   const double x = ceil(p * (double)sum);
   return x >= (double)sum ? sum : x < 1. ? 1 : (uint64_t)x;
@@ -340,18 +341,10 @@ struct InMemory {
   template <typename F>
   __device__ inline void each(F f) const {
     const int a = (int)(threadIdx.x >> 6) * run, lane = threadIdx.x & 63;
-    for (int j = 0; j < run; j += 64 * 8) {
-      float x[8];
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const int i = a + j + 64 * u + lane;
-        x[u] = j + 64 * u < run && i < n ? logit<T>(row, i) : -INFINITY;
-      }
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const int i = a + j + 64 * u + lane;
-        f(x[u], j + 64 * u < run && i < n ? i : -1, j / 64 + u);
-      }
+#pragma unroll 2
+    for (int j = 0; j < run; j += 64) {  // (longer unrolled the kernels' code takes longer to fetch)
+      const int i = a + j + lane;
+      f(i < n ? logit<T>(row, i) : -INFINITY, i < n ? i : -1, j / 64);
     }
   }
 };
@@ -564,11 +557,10 @@ __device__ Cut find_cut(const Row& row, Room& s, const Rules& r, float top, int 
   if (r.p < 1.) c = end_of(false, wanted(r.p, sum), unused);
   return c;
 }
-// The token of tokens [0, n): the first whose running sum of kept weights is above u times
-// their sum or (known) above `aim`.
+// The token: the first whose running sum of kept weights is above u times their sum.
 template <typename Row>
 __device__ int draw(const Row& row, Room& s, const Rules& r, float top, int scale, const Cut& cut,
-                    float u, bool known, uint64_t aim) {
+                    float u) {
   const int wid = threadIdx.x >> 6;
   auto mass = [&](float x, int i) {
     const uint64_t w = i >= 0 && kept(cut, key_of(x), i) ? weight(x, top, r, scale, s.pw) : 0;
@@ -585,7 +577,7 @@ __device__ int draw(const Row& row, Room& s, const Rules& r, float top, int scal
     run += i < wid ? s.wm[i] : 0;
     total += s.wm[i];
   }
-  if (!known) aim = aim_of(u, total);
+  const uint64_t aim = aim_of(u, total);
   if (run <= aim && aim < run + mine) {  // (one wave's run)
     int token = -1;
     row.each([&](float x, int i, int) {
@@ -595,6 +587,39 @@ __device__ int draw(const Row& row, Room& s, const Rules& r, float top, int scal
       run += lane_u64(at, 63);
     });
     if ((threadIdx.x & 63) == 0) s.n = token;
+  }
+  __syncthreads();
+  return s.n;
+}
+// The same for up to PART tokens of a row, the thread's ones beside each other, where the
+// sum is known: the first above `aim`.
+template <typename T>
+__device__ int draw_part(const void* row, int64_t from, int n, Room& s, const Rules& r, float top,
+                         int scale, const Cut& cut, uint64_t aim) {
+  constexpr int E = PART / NT;
+  const int tid = threadIdx.x, lane = tid & 63, i0 = tid * E;
+  auto mass = [&](float x, int i) {
+    const uint64_t w = i < n && kept(cut, key_of(x), i) ? weight(x, top, r, scale, s.pw) : 0;
+    return w >= r.m ? w : 0;
+  };
+  uint64_t mine = 0;
+  float x[E];
+#pragma unroll
+  for (int j = 0; j < E; ++j) x[j] = i0 + j < n ? logit<T>(row, from + i0 + j) : -INFINITY;
+#pragma unroll
+  for (int j = 0; j < E; ++j) mine += mass(x[j], i0 + j);
+  const uint64_t at = incl_scan_u64(mine);
+  if (lane == 63) s.wm[tid >> 6] = at;
+  __syncthreads();
+  uint64_t run = at - mine;
+  for (int i = 0; i < (tid >> 6); ++i) run += s.wm[i];
+  const uint64_t here = __ballot(run <= aim && aim < run + mine);
+  if (here) {  // one thread's tokens: one each for lanes of its wave
+    const int l = __ffsll((unsigned long long)here) - 1, i = __builtin_amdgcn_readlane(i0, l) + lane;
+    const bool has = lane < E && i < n;
+    const uint64_t w = has ? mass(logit<T>(row, from + i), i) : 0;
+    const uint64_t hit = __ballot(has && lane_u64(run, l) + incl_scan_u64(w) > aim);
+    if (lane == 0) s.n = i + __ffsll((unsigned long long)hit) - 1;
   }
   __syncthreads();
   return s.n;
@@ -656,7 +681,7 @@ __global__ __launch_bounds__(NT) void sample_block_kernel(SArgs g) {
     __syncthreads();
   }
   const Cut cut = find_cut(x, s, r, top, g.scale);
-  const int token = draw(x, s, r, top, g.scale, cut, g.u[row], false, 0);
+  const int token = draw(x, s, r, top, g.scale, cut, g.u[row]);
   if (threadIdx.x == 0) g.out[row] = token;
 }
 
@@ -811,20 +836,37 @@ __global__ __launch_bounds__(NT) void sample_part_kernel(SArgs g) {
     const uint64_t* bins = g.hm + (row * g.parts + part) * NB;
     for (int i = threadIdx.x; i < f.bin; i += NT) m += bins[i];
   }
-  x.each([&](float v, int i, int) {
-    if (i < 0) return;
-    const int bin = f.way == CUT || f.way == ALL ? 0 : bin_of(v, top, r);
-    const bool list_it = f.way == TOP ? bin <= f.bin : f.way == BIN && bin == f.bin;
-    const bool keep = f.way == ALL || (f.way == CUT && kept(cut, key_of(v), i)) ||
-                      (f.way == BIN && bin < f.bin && !sums);
-    if (!list_it && !keep) return;
-    const uint64_t w = weight(v, top, r, g.scale, pw);
-    if (keep) m += w >= r.m ? w : 0;
-    if (list_it) {
-      const int at = atomicAdd(&listed, 1);
-      if (at < NT) list[at] = Entry{v, part * PART + i, w};
+  auto enter = [&](float v, int i) {
+    const int at = atomicAdd(&listed, 1);
+    if (at < NT) list[at] = Entry{v, part * PART + i, weight(v, top, r, g.scale, pw)};
+  };
+  if (sums) {
+    const float from = (float)f.bin, end = from + 1.f;
+    uint32_t hits = 0;
+    x.each([&](float v, int i, int j) {
+      const float t = place_of(v, top, r);
+      hits |= t >= from && t < end && i >= 0 ? 1u << j : 0;
+    });
+    while (hits) {
+      const int i = x.first + 64 * (__ffs((int)hits) - 1);
+      hits &= hits - 1;
+      enter(logit<T>((const char*)g.x + row * g.st * (int64_t)sizeof(T), (int64_t)part * PART + i), i);
     }
-  });
+  } else {
+    const InMemory<T> again((const char*)g.x + (row * g.st + (int64_t)part * PART) * (int64_t)sizeof(T),
+                            x.n);
+    again.each([&](float v, int i, int) {
+      if (i < 0) return;
+      const int bin = f.way == CUT || f.way == ALL ? 0 : bin_of(v, top, r);
+      const bool keep = f.way == ALL || (f.way == CUT && kept(cut, key_of(v), i)) ||
+                        (f.way == BIN && bin < f.bin);
+      if (keep) {
+        const uint64_t w = weight(v, top, r, g.scale, pw);
+        m += w >= r.m ? w : 0;
+      }
+      if (f.way == TOP ? bin <= f.bin : f.way == BIN && bin == f.bin) enter(v, i);
+    });
+  }
   m = sum_u64(m);
   if ((threadIdx.x & 63) == 0) wm[threadIdx.x >> 6] = m;
   __syncthreads();
@@ -847,20 +889,23 @@ __global__ __launch_bounds__(NT) void sample_pick_kernel(SArgs g) {
   __shared__ Room s;
   __shared__ uint64_t extra[64];  // kept weights of the bin, by parts
   const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63;
+  // (everything whose address is known is on its way at once; of a row without a token it is
+  // whatever lies there)
+  const Found f = g.found[row];
+  const int n_of = lane < g.parts ? g.count[row * g.parts + lane] : 0;
+  const uint64_t above = lane < g.parts ? g.pmass[row * g.parts + lane] : 0;
   const float top = row_top(g, row);
   const Rules r = rules_of(g, row);
   if (!(top > -INFINITY) || !r.good) {
     if (threadIdx.x == 0) g.out[row] = -1;
     return;
   }
-  const int tid = threadIdx.x, lane = tid & 63;
-  const Found f = g.found[row];
   Cut cut{f.key, f.way == ALL ? 0x7fffffff : f.index};
   fill(s.pw);
   if (tid < 64) extra[tid] = 0;
   if (f.way == TOP || f.way == BIN) {
     // the parts' lists one behind the other (parts <= 64: 2^20 tokens)
-    const int n_of = lane < g.parts ? g.count[row * g.parts + lane] : 0;
     const bool over = __any(n_of > NT);
     const int upto = wave_incl_scan(min(n_of, NT)), n = __builtin_amdgcn_readlane(upto, 63);
     if (tid == 0) {
@@ -894,59 +939,60 @@ __global__ __launch_bounds__(NT) void sample_pick_kernel(SArgs g) {
       Entry e{0.f, -1, 0};
       if (tid < n) e = g.list[(row * g.parts + part) * NT + tid - before_part];
       const Listed x{e.x, e.index};
-      auto by_rank = [&](float v, int i, uint64_t& c, uint64_t& w) {
-        c = rank_code(v, i);
-        w = e.w;
-        return true;
-      };
-      auto restart = [&] {
+      // the selections of the list, one after the other: where top_k ends, where top_p ends,
+      // and of a list of all that is kept the token
+      enum { BY_K, BY_P, TOKEN };
+      uint64_t want = f.way == TOP ? (uint64_t)r.k : f.want;
+      bool in = true;
+      int stage = f.way == TOP ? BY_K : BY_P;
+      for (;;) {
+        const uint64_t code =
+            select(x, s,
+                   [&](float v, int i, uint64_t& c, uint64_t& w) {
+                     c = stage == TOKEN ? (uint32_t)i : rank_code(v, i);
+                     w = e.w;
+                     return in;
+                   },
+                   stage == BY_K, want, sum);
+        if (stage == TOKEN) {
+          if (tid == 0) g.out[row] = (int)code;
+          return;
+        }
+        cut = cut_of(code);
+        if (stage == BY_K && r.p < 1.) {
+          stage = BY_P;
+          want = wanted(r.p, sum);
+        } else {
+          in = e.index >= 0 && kept(cut, key_of(e.x), e.index) && e.w >= r.m;
+          if (f.way == BIN) break;
+          stage = TOKEN;
+          sum = sum_u64(in ? e.w : 0);
+          if (lane == 0) s.wm[tid >> 6] = sum;
+          __syncthreads();
+          sum = 0;
+          for (int i = 0; i < NW; ++i) sum += s.wm[i];
+          want = aim_of(g.u[row], sum) + 1;
+        }
         if (tid == 0) {
           s.above_c = 0;
-          s.above_m = f.way == BIN ? f.above_m : 0;
+          s.above_m = 0;
           s.in_c = (uint32_t)n;
         }
         __syncthreads();
-      };
-      uint64_t want = f.want;
-      if (f.way == TOP) {
-        cut = cut_of(select(x, s, by_rank, true, (uint64_t)r.k, sum));
-        want = wanted(r.p, sum);
-      }
-      if (f.way == BIN || r.p < 1.) {
-        if (f.way == TOP) restart();
-        cut = cut_of(select(x, s, by_rank, false, want, sum));
-      }
-      const bool in = e.index >= 0 && kept(cut, key_of(e.x), e.index) && e.w >= r.m;
-      if (f.way == TOP) {  // the list has all that are kept: by index it decides
-        sum = sum_u64(in ? e.w : 0);
-        if (lane == 0) s.wm[tid >> 6] = sum;
-        __syncthreads();
-        sum = 0;
-        for (int i = 0; i < NW; ++i) sum += s.wm[i];
-        restart();
-        const uint64_t aim = aim_of(g.u[row], sum);
-        auto by_index = [&](float, int i, uint64_t& c, uint64_t& w) {
-          c = (uint32_t)i;
-          w = e.w;
-          return in;
-        };
-        const uint64_t token = select(x, s, by_index, false, aim + 1, sum);
-        if (tid == 0) g.out[row] = (int)token;
-        return;
       }
       if (in) atomicAdd((unsigned long long*)&extra[e.index / PART], (unsigned long long)e.w);
     }
   }
   __syncthreads();
-  const uint64_t m = lane < g.parts ? g.pmass[row * g.parts + lane] + extra[lane] : 0;
+  const uint64_t m = above + extra[lane];
   const uint64_t at = incl_scan_u64(m);
   const uint64_t aim = aim_of(g.u[row], lane_u64(at, 63));
   const uint64_t hit = __ballot(at > aim);
   const int part = __ffsll((unsigned long long)hit) - 1;
   const uint64_t before = lane_u64(at - m, part);
-  const Held<T, 16> x = part_of<T>(g, row, part);
-  const int token = draw(x, s, r, top, g.scale, Cut{cut.key, cut.index - part * PART}, 0.f, true,
-                         aim - before);
+  const int token = draw_part<T>((const char*)g.x + row * g.st * (int64_t)sizeof(T),
+                                 (int64_t)part * PART, min(PART, g.V - part * PART), s, r, top,
+                                 g.scale, Cut{cut.key, cut.index - part * PART}, aim - before);
   if (tid == 0) g.out[row] = part * PART + token;
 }
 
