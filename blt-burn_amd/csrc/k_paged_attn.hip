@@ -16,8 +16,10 @@
 //
 // A prefix that all sequences share (the same pages) is read once for all of them, in two
 // launches of the same kernels: PREFIX takes the tokens of all sequences as the rows of one, over
-// the keys of the prefix, which they all see whole, and leaves their unnormalised outputs,
-// maxima and sums in memory; TAILS takes each sequence's keys from there on and joins the two.
+// the keys of the prefix, which they all see whole, in parts whose unnormalised outputs,
+// maxima and sums it leaves in memory; TAILS takes each sequence's keys from there on, and joins its
+// rows' parts of the prefix to them.  (Joined by the block whose part ends last, as others are, one block
+// had all rows of a key head to join.)
 #include <algorithm>
 #include <type_traits>
 
@@ -47,8 +49,10 @@ struct KArgs {
   float* part;    // [slots][rows of a tile][D], unnormalised outputs
   float* ml;      // [slots][rows of a tile][2], their max (before the scale) and sum
   const int32_t* prefix;  // tokens that all sequences share
-  float* pre_o;           // [total][heads][D] and [total][heads][2], as part and ml, of the prefix
+  // the prefix' parts: [key heads][pre_tiles][pre_parts][pre_rows][D] and [..][2], as part and ml
+  float* pre_o;
   float* pre_ml;
+  int pre_tiles, pre_parts, pre_rows, pre_keys;  // pre_keys: of a key tile
 };
 
 // ---- which item ----------------------------------------------------------------
@@ -92,6 +96,15 @@ struct Item {
   int pslot, join;         // first partial slot and first counter of its row tiles
   int from;                // first key (0, or TAILS: the first that is not shared)
 };
+// How many parts the `from` shared keys are in: at least two key tiles each.
+__device__ inline int prefix_parts(const KArgs& p, int from) {
+  const int tiles = (from + p.pre_keys - 1) / p.pre_keys;
+  const int each = max(2, (tiles + p.pre_parts - 1) / p.pre_parts);
+  return (tiles + each - 1) / each;
+}
+__device__ inline int64_t prefix_slot(const KArgs& p, int kvh, int rt, int part) {
+  return ((int64_t)kvh * p.pre_tiles + rt) * p.pre_parts + part;
+}
 __device__ inline int lane_of(int v, int l) { return __builtin_amdgcn_readlane(v, l); }
 
 // The item of block `bid`, false if it has none.  (Up to 64 rows a lane holds each; beyond that
@@ -102,7 +115,7 @@ __device__ inline int lane_of(int v, int l) { return __builtin_amdgcn_readlane(v
 template <int BQ, int BKV, int MODE>
 __device__ bool find_item(const KArgs& p, unsigned bid, Item& it) {
   const int lane = threadIdx.x & 63;
-  const int B = MODE == PREFIX ? 1 : p.B;
+  const int B = p.B;
   Seq q;
   int nrt, kt, from = 0;
   float work = 0.f, tiles = 0.f, longest = 0.f;
@@ -120,11 +133,22 @@ __device__ bool find_item(const KArgs& p, unsigned bid, Item& it) {
     room = min(p.prefix[0], -wave_max_i32(-room));
     from = __builtin_amdgcn_readfirstlane(room > 0 ? room >> p.lps << p.lps : 0);
     if constexpr (MODE == PREFIX) {
-      if (__any(crossed) || slot < 0) return false;  // (TAILS reports it)
+      if (__any(crossed) || slot < 0 || from == 0) return false;  // (TAILS reports it)
       const int a = p.starts[0], e = p.starts[p.B];
-      q = lane == 0 ? Seq{a, e - a, from, slot} : Seq{0, 0, 0, 0};
-      from = 0;
-      lost = false;
+      it.q = Seq{a, e - a, from, slot};
+      it.nrt = (int)(((uint32_t)(it.q.n * p.G) + BQ - 1) / BQ);
+      it.ns = prefix_parts(p, from);
+      it.from = 0;
+      it.pslot = it.join = 0;
+      // the row tiles of a part beside each other on one XCD
+      const int all = p.Hkv * it.ns * it.nrt, per = (all + 7) >> 3;
+      const int id = (int)(bid & 7) * per + (int)(bid >> 3);
+      if ((int)(bid >> 3) >= per || id >= all) return false;
+      const int x = (int)((uint32_t)id / (uint32_t)it.nrt);
+      it.rt = id - x * it.nrt;
+      it.kvh = (int)((uint32_t)x / (uint32_t)it.ns);
+      it.split = x - it.kvh * it.ns;
+      return true;
     }
   }
   for (int b0 = 0; b0 < B; b0 += 64) {
@@ -349,23 +373,56 @@ __device__ inline void join(Joined& a, const Joined& b, float c) {
   a.l = fmaf(a.l, wa, wb * b.l);
   a.o = a.o * wa + wb * b.o;
 }
-// Four columns of a row of head `head`: PREFIX leaves them for TAILS (true: nothing more to do),
-// which takes them up.
+// Parts x0 .. x1 - 1 of the prefix, U in flight: ml, o of a row's four columns in the first one.
+template <int D, int U>
+__device__ inline void add_parts(const KArgs& p, const float* ml, const float* o, int x0, int x1,
+                                 Joined& a) {
+  for (int x = x0; x < x1; x += U) {
+    float pm[U], pl[U];
+    f32x4_t po[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {  // (past the last: the last one again, left out)
+      const int64_t step = (int64_t)min(x + u, x1 - 1) * p.pre_rows;
+      pm[u] = ml[step * 2];
+      pl[u] = ml[step * 2 + 1];
+      po[u] = *reinterpret_cast<const f32x4_t*>(o + step * D);
+    }
+    float mx = a.m;
+#pragma unroll
+    for (int u = 0; u < U; ++u) mx = fmaxf(mx, x + u < x1 ? pm[u] : -INFINITY);
+    const float off = mx == -INFINITY ? 0.f : mx;
+    const float w0 = __builtin_amdgcn_exp2f((a.m - off) * p.c);
+    a.m = mx;
+    a.l *= w0;
+    a.o *= w0;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (x + u < x1) {
+        const float w = __builtin_amdgcn_exp2f((pm[u] - off) * p.c);
+        a.l = fmaf(w, pl[u], a.l);
+        a.o += w * po[u];
+      }
+  }
+}
+// Four columns of a row's part: PREFIX leaves them for TAILS (true: nothing more to do), which
+// joins all of them.
 template <int D, int MODE>
-__device__ inline bool shared_part(const KArgs& p, int token, int head, int dd, Joined& a) {
+__device__ inline bool shared_part(const KArgs& p, const Item& it, int token, int g, int dd,
+                                   Joined& a) {
   if constexpr (MODE == WHOLE) return false;
-  const int64_t at = (int64_t)token * (p.Hkv * p.G) + head;
-  f32x4_t* o = reinterpret_cast<f32x4_t*>(p.pre_o + at * D + dd);
+  const int row = (token - p.starts[0]) * p.G + g, rt = row / p.pre_rows, r = row - rt * p.pre_rows;
+  const int64_t at = prefix_slot(p, it.kvh, rt, MODE == PREFIX ? it.split : 0) * p.pre_rows + r;
+  float* o = p.pre_o + at * D + dd;
   float* ml = p.pre_ml + at * 2;
   if constexpr (MODE == PREFIX) {
-    *o = a.o;
+    *reinterpret_cast<f32x4_t*>(o) = a.o;
     if (dd == 0) {
       ml[0] = a.m;
       ml[1] = a.l;
     }
     return true;
   }
-  join(a, Joined{ml[0], ml[1], *o}, p.c);
+  add_parts<D, 8>(p, ml, o, 0, prefix_parts(p, it.from), a);
   return false;
 }
 template <int D, int BQ, int NT, typename T, int MODE>
@@ -424,7 +481,7 @@ __device__ void join_parts(const KArgs& p, const Item& it, int nr, float* room) 
   auto store = [&](int i, Joined a) {
     const int r = i / (D / 4), dd = (i % (D / 4)) * 4;
     const int row = it.rt * BQ + r, t = over(row, p.by_g), g = row - t * p.G;
-    if (shared_part<D, MODE>(p, it.q.s0 + t, it.kvh * p.G + g, dd, a)) return;
+    shared_part<D, MODE>(p, it, it.q.s0 + t, g, dd, a);
     const int64_t at =
         (int64_t)(it.q.s0 + t) * p.st_o + (int64_t)(it.kvh * p.G + g) * p.sh_o + dd;
     const f32x4_t x = a.l == 0.f ? f32x4_t{0.f, 0.f, 0.f, 0.f} : a.o / a.l;
@@ -522,45 +579,31 @@ __device__ inline bool join_tiles(const KArgs& p, const Item& it, bool active,
   return true;
 }
 
-// As shared_part, a row in the accumulators' layout: of bf16's form for 128 rows, or of f32's.
+// The same for a row in the accumulators' layout: of bf16's form for 128 rows, or of f32's.
 template <int D, int MODE, bool F32>
-__device__ inline bool shared_row(const KArgs& p, int token, int head, int half, float m,
-                                  float& total, f32x16_t (&o)[D / 32]) {
+__device__ inline bool shared_row(const KArgs& p, const Item& it, int token, int g, int half,
+                                  float& m, float& total, f32x16_t (&o)[D / 32]) {
   if constexpr (MODE == WHOLE) return false;
-  const int64_t at = (int64_t)token * (p.Hkv * p.G) + head;
-  float* to = p.pre_o + at * D;
-  float* ml = p.pre_ml + at * 2;
-  auto col = [&](int j) { return F32 ? 4 * (8 * (j >> 2) + 4 * half + (j & 3)) : 8 * j + 4 * half; };
-  if constexpr (MODE == PREFIX) {
-#pragma unroll
-    for (int j = 0; j < D / 8; ++j) {
-      f32x4_t x;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = F32 ? o[e & (D / 32 - 1)][j & 15] : o[j >> 2][4 * (j & 3) + e];
-      *reinterpret_cast<f32x4_t*>(to + col(j)) = x;
-    }
-    if (half == 0) {
-      ml[0] = m;
-      ml[1] = total;
-    }
-    return true;
-  }
-  const float pm = ml[0], mx = fmaxf(m, pm), off = mx == -INFINITY ? 0.f : mx;
-  const float wa = __builtin_amdgcn_exp2f((m - off) * p.c);
-  const float wb = __builtin_amdgcn_exp2f((pm - off) * p.c);
-  total = fmaf(total, wa, wb * ml[1]);
+  const float m0 = m, l0 = total;
 #pragma unroll
   for (int j = 0; j < D / 8; ++j) {
-    const f32x4_t x = *reinterpret_cast<const f32x4_t*>(to + col(j));
+    Joined a{m0, l0, {}};
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      a.o[e] = F32 ? o[e & (D / 32 - 1)][j & 15] : o[j >> 2][4 * (j & 3) + e];
+    const int col = F32 ? 4 * (8 * (j >> 2) + 4 * half + (j & 3)) : 8 * j + 4 * half;
+    if (shared_part<D, MODE>(p, it, token, g, col, a)) continue;
+    m = a.m;
+    total = a.l;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       if constexpr (F32)
-        o[e & (D / 32 - 1)][j & 15] = fmaf(o[e & (D / 32 - 1)][j & 15], wa, wb * x[e]);
+        o[e & (D / 32 - 1)][j & 15] = a.o[e];
       else
-        o[j >> 2][4 * (j & 3) + e] = fmaf(o[j >> 2][4 * (j & 3) + e], wa, wb * x[e]);
+        o[j >> 2][4 * (j & 3) + e] = a.o[e];
     }
   }
-  return false;
+  return MODE == PREFIX;
 }
 
 // ---- bf16, tiles of rows ---------------------------------------------------------
@@ -852,9 +895,10 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(KArgs p) {
   swap_pair<32>(l, a, b);
   const float lt = a + b;
   float total = lt;
-  if (it.ns > 1 && !join_tiles<D>(p, it, wave_active, o, m, total)) return;
+  if (MODE != PREFIX && it.ns > 1 && !join_tiles<D>(p, it, wave_active, o, m, total)) return;
   if (row < rows) {
-    if (shared_row<D, MODE, false>(p, sq.s0 + tok, head, lhalf, m, total, o)) return;
+    if (shared_row<D, MODE, false>(p, it, sq.s0 + tok, head - it.kvh * p.G, lhalf, m, total, o))
+      return;
     uint16_t* orow = (uint16_t*)p.o + (int64_t)(sq.s0 + tok) * p.st_o + (int64_t)head * p.sh_o;
     // hardware reciprocal (1 ulp): the output is rounded to bf16
     const float inv = total > 0.f ? __builtin_amdgcn_rcpf(total) : total == total ? 0.f : total;
@@ -1199,14 +1243,14 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(KArgs p) {
       lt += wt * sl[x][r];
       acc += wt * *reinterpret_cast<const f32x4_t*>(so + (x * BQ + r) * OP + dd);
     }
-    if (it.ns > 1) {
+    if (MODE != PREFIX && it.ns > 1) {
       put4(p.part + (at + r) * D + dd, acc);
       if (dd == 0) put2(p.ml + (at + r) * 2, mx, lt);
     } else {
       const int t = over(r0 + r, p.by_g), g = (r0 + r) - t * p.G;
       if constexpr (MODE != WHOLE) {
         Joined a{mx, lt, acc};
-        if (shared_part<D, MODE>(p, sq.s0 + t, it.kvh * p.G + g, dd, a)) continue;
+        if (shared_part<D, MODE>(p, it, sq.s0 + t, g, dd, a)) continue;
         lt = a.l;
         acc = a.o;
       }
@@ -1217,7 +1261,7 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(KArgs p) {
                                                  pack_bf16x2(acc.z * inv, acc.w * inv)};
     }
   }
-  if (it.ns > 1) join_parts<D, BQ, 64 * NW, uint16_t, MODE>(p, it, nr, so);
+  if (MODE != PREFIX && it.ns > 1) join_parts<D, BQ, 64 * NW, uint16_t, MODE>(p, it, nr, so);
 }
 
 // ---- f32 -------------------------------------------------------------------------
@@ -1445,14 +1489,14 @@ __global__ __launch_bounds__(256) void paged_attn_f32_kernel(KArgs p) {
       x[k] = *reinterpret_cast<const f32x4_t*>(so + (k * 32 + rr) * OP + cc);
     f32x4_t sum = (x[0] + x[1]) + (x[2] + x[3]);
     float tot = sl[0][rr];
-    if (it.ns > 1) {
+    if (MODE != PREFIX && it.ns > 1) {
       put4(p.part + (at + rr) * D + cc, sum);
       if (cc == 0) put2(p.ml + (at + rr) * 2, sm[0][rr], tot);
     } else {
       const int t = over(r0 + rr, p.by_g), gg = (r0 + rr) - t * p.G;
       if constexpr (MODE != WHOLE) {
         Joined a{sm[0][rr], tot, sum};
-        if (shared_part<D, MODE>(p, sq.s0 + t, it.kvh * p.G + gg, cc, a)) continue;
+        if (shared_part<D, MODE>(p, it, sq.s0 + t, gg, cc, a)) continue;
         tot = a.l;
         sum = a.o;
       }
@@ -1461,7 +1505,7 @@ __global__ __launch_bounds__(256) void paged_attn_f32_kernel(KArgs p) {
           tot == 0.f ? f32x4_t{0.f, 0.f, 0.f, 0.f} : sum / tot;
     }
   }
-  if (it.ns > 1) join_parts<D, BQ, 256, float, MODE>(p, it, nq, so);
+  if (MODE != PREFIX && it.ns > 1) join_parts<D, BQ, 256, float, MODE>(p, it, nq, so);
 }
 
 // ---- f32, tiles of rows ----------------------------------------------------------
@@ -1687,9 +1731,9 @@ __global__ __launch_bounds__(256, 2) void paged_attn_f32_tiles_kernel(KArgs p) {
   float a, b;
   swap_pair<32>(l, a, b);
   float total = a + b;
-  if (it.ns > 1 && !join_tiles<D>(p, it, wave_active, o, m, total)) return;
+  if (MODE != PREFIX && it.ns > 1 && !join_tiles<D>(p, it, wave_active, o, m, total)) return;
   if (rw + l31 < rows) {
-    if (shared_row<D, MODE, true>(p, sq.s0 + tok, head, h, m, total, o)) return;
+    if (shared_row<D, MODE, true>(p, it, sq.s0 + tok, head - it.kvh * p.G, h, m, total, o)) return;
     float* orow = (float*)p.o + (int64_t)(sq.s0 + tok) * p.st_o + (int64_t)head * p.sh_o;
 #pragma unroll
     for (int n = 0; n < NV; ++n)
@@ -1790,19 +1834,33 @@ static int64_t parts_bytes(const blt_paged_cache& c, int64_t B, int64_t total, i
   const Shape s = shape_of(c, B, total, H);
   return slots_of(c, s, B, total, H) * s.bq * (c.head_dim + 2) * 4;
 }
+// The prefix' row tiles (of all tokens as one sequence), and the parts it may be in: enough to fill the
+// chip, few enough that joining them takes no longer than their keys.
+struct PrefixShape {
+  Shape s;
+  int64_t tiles;  // of a key head
+  int parts;
+};
+static PrefixShape prefix_shape(const blt_paged_cache& c, int64_t total, int H) {
+  PrefixShape x{shape_of(c, 1, total, H), 0, 1};
+  x.tiles = (total * (H / c.n_kv_heads) + x.s.bq - 1) / x.s.bq;
+  const int64_t fill = 768 / std::max<int64_t>(1, x.tiles * c.n_kv_heads);
+  x.parts = (int)std::max<int64_t>(1, std::min<int64_t>(32, fill));
+  return x;
+}
 int64_t paged_attention_workspace_bytes(const blt_paged_cache& c, int64_t B, int64_t total, int H,
                                         bool prefix) {
   const int64_t own = parts_bytes(c, B, total, H);
   if (!prefix) return own;
-  // the prefix' outputs, and the parts of one launch after the other
-  return total * H * (c.head_dim + 2) * 4 + std::max(own, parts_bytes(c, 1, total, H));
+  const PrefixShape x = prefix_shape(c, total, H);
+  return own + c.n_kv_heads * x.tiles * x.parts * x.s.bq * (c.head_dim + 2) * 4;
 }
 
 // One launch; with a prefix its own (mode PREFIX) and the sequences' (TAILS).
 static int launch_mode(const blt_paged_cache& c, const PagedAttnArgs& a, int mode, void* ws,
                        hipStream_t s) {
-  const int64_t B = mode == PREFIX ? 1 : a.B;  // (what the shape and the grid go by)
-  Shape sh = shape_of(c, B, a.total, a.H);
+  const PrefixShape pre = mode == WHOLE ? PrefixShape{} : prefix_shape(c, a.total, a.H);
+  Shape sh = mode == PREFIX ? pre.s : shape_of(c, a.B, a.total, a.H);
   const int d = c.head_dim;
   KArgs p{};
   const int64_t es = c.dtype == BLT_DTYPE_BF16 ? 2 : 4;
@@ -1822,17 +1880,23 @@ static int launch_mode(const blt_paged_cache& c, const PagedAttnArgs& a, int mod
   p.c = (float)(1.44269504088896340736 * (double)a.scale);
   if (p.window && p.window < 24 * sh.bkv) sh.spill = 0;  // (too short: its blocks would only exit)
   p.resident = sh.resident; p.cmin = sh.cmin; p.spill = sh.spill;
-  const int64_t slots = slots_of(c, sh, B, a.total, a.H);
+  const int64_t slots = mode == PREFIX ? 0 : slots_of(c, sh, a.B, a.total, a.H);
   p.sync = c.sync; p.status = c.status;
   p.part = (float*)ws;
   if (mode != WHOLE) {
     p.prefix = a.prefix;
+    p.pre_tiles = (int)pre.tiles;
+    p.pre_parts = pre.parts;
+    p.pre_rows = pre.s.bq;
+    p.pre_keys = pre.s.bkv;
+    const int64_t rows = c.n_kv_heads * pre.tiles * pre.parts * pre.s.bq;
     p.pre_o = p.part;
-    p.pre_ml = p.pre_o + a.total * a.H * d;
-    p.part = p.pre_ml + a.total * a.H * 2;
+    p.pre_ml = p.pre_o + rows * d;
+    p.part = p.pre_ml + rows * 2;
   }
   p.ml = p.part + slots * sh.bq * d;
-  const int64_t nb = (blocks_of(c, sh, B, a.total, a.H) + 7) / 8 * 8;
+  const int64_t nb = ((mode == PREFIX ? c.n_kv_heads * pre.tiles * pre.parts
+                                      : blocks_of(c, sh, a.B, a.total, a.H)) + 7) / 8 * 8;
   if (nb > 0x7fffffff) return fail(BLT_ERR_SHAPE, "paged_attention: too many row tiles");
   const unsigned n = (unsigned)nb;
   switch (mode) {

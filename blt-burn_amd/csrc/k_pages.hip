@@ -584,8 +584,8 @@ constexpr int kCopyBlocks = 2048;  // eight 256-thread blocks on each of 256 CUs
 
 // ---- common prefix -----------------------------------------------------------------
 // Whole pages that all listed sequences with tokens have in common, in tokens (0 with fewer than
-// two of them).  One block: a thread compares one column of the table over every few
-// sequences, eight at a time in flight (48 sequences of 512 pages: 100 KB).
+// two of them).  One block, once a step: what it costs are the rounds of loads (48 sequences of 512 pages,
+// 100 KB: a thread has 24 entries).
 __global__ __launch_bounds__(NT) void common_prefix_kernel(blt_paged_cache c, int lps,
                                                            const int32_t* seqs, int n,
                                                            int32_t* tokens) {
@@ -624,33 +624,37 @@ __global__ __launch_bounds__(NT) void common_prefix_kernel(blt_paged_cache c, in
     return;
   }
   const int32_t* own = c.page_table + (int64_t)(seqs ? seqs[first] : first) * c.max_pages;
-  // W columns at a time, groups of threads share the sequences
-  int W = NT;
-  while (W > 64 && W / 2 >= full) W /= 2;
-  const int col = tid & (W - 1), group = tid / W, groups = NT / W;
+  // 1024 sequences at a time, a thread has entries (sequence, column) of all of them
   for (int i0 = 0; i0 < n; i0 += NT) {
     int pages;
     __syncthreads();
     slots[tid] = i0 + tid < n ? slot_at(i0 + tid, &pages) : -1;
     __syncthreads();
-    const int m = min(NT, n - i0);
-    for (int at = col; at < full; at += W) {
-      const int page = own[at];
-      bool same = true;
-      for (int j = group; j < m; j += 8 * groups) {
-        int x[8];
+    const int cols = full;  // (it may shrink below: what lies behind does not matter then)
+    const int64_t all = (int64_t)min(NT, n - i0) * cols;
+    int j = cols ? tid / cols : 0, at = cols ? tid - j * cols : 0;
+    const int dj = cols ? NT / cols : 0, dat = cols ? NT - dj * cols : 0;
+    constexpr int U = 16;  // entries in flight
+    for (int64_t e = tid; e < all; e += (int64_t)U * NT) {
+      int x[U], y[U], col[U];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const int s = j + u * groups < m ? slots[j + u * groups] : -1;
-          x[u] = s < 0 ? page : c.page_table[(int64_t)s * c.max_pages + at];
+      for (int u = 0; u < U; ++u) {
+        const int s = e + (int64_t)u * NT < all ? slots[j] : -1;
+        col[u] = at;
+        x[u] = s < 0 ? 0 : own[at];
+        y[u] = s < 0 ? 0 : c.page_table[(int64_t)s * c.max_pages + at];
+        j += dj;
+        at += dat;
+        if (at >= cols) {
+          at -= cols;
+          ++j;
         }
+        j = min(j, NT - 1);
+      }
+      int most = 0x7fffffff;
 #pragma unroll
-        for (int u = 0; u < 8; ++u) same &= x[u] == page;
-      }
-      if (!same) {
-        atomicMin(&full, at);
-        break;
-      }
+      for (int u = 0; u < U; ++u) most = x[u] != y[u] ? min(most, col[u]) : most;
+      if (most != 0x7fffffff) atomicMin(&full, most);
     }
   }
   __syncthreads();
