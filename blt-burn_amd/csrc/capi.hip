@@ -324,12 +324,20 @@ static int packed_heads_check(const void* x, int64_t st, int64_t sh, int32_t dty
   return 0;
 }
 
+int64_t blt_packed_attention_workspace_bytes(int64_t B, int64_t total, int64_t Hq, int64_t Hkv,
+                                             int32_t dtype) {
+  // (0 for what blt_packed_attention refuses)
+  if (Hkv < 1 || Hq < 1 || Hq > 0xffff || Hq % Hkv || B < 0 || total < 0 || total > 0x7ffe0000 ||
+      Hq * total > 0x7ffe0000)
+    return 0;
+  return packed_attention_workspace_bytes(B, total, (int)Hq, (int)Hkv, dtype);
+}
 int blt_packed_attention(const void* q, int64_t st_q, int64_t sh_q, const void* k, int64_t st_k,
                          int64_t sh_k, const void* v, int64_t st_v, int64_t sh_v, void* o,
                          int64_t st_o, int64_t sh_o, float* lse, int32_t dtype, int64_t total,
                          int64_t Hq, int64_t Hkv, int32_t d, const int32_t* starts, int64_t B,
                          int32_t causal, int32_t window, float scale, int32_t tail,
-                         blt_stream_t stream) {
+                         void* workspace, int64_t workspace_bytes, blt_stream_t stream) {
   const char* what = "packed_attention";
   if (int rc = packed_checks(dtype, total, Hq, Hkv, d, starts, B, window, scale, what)) return rc;
   if (total == 0) return BLT_OK;
@@ -337,13 +345,16 @@ int blt_packed_attention(const void* q, int64_t st_q, int64_t sh_q, const void* 
   if (int rc = packed_heads_check(k, st_k, sh_k, dtype, what)) return rc;
   if (int rc = packed_heads_check(v, st_v, sh_v, dtype, what)) return rc;
   if (int rc = packed_heads_check(o, st_o, sh_o, dtype, what)) return rc;
+  const int64_t need = packed_attention_workspace_bytes(B, total, (int)Hq, (int)Hkv, dtype);
+  if (need > 0 && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need))
+    return fail(BLT_ERR_INVALID, std::string(what) + ": workspace missing, misaligned or too small");
   PackedAttnArgs a{};
   a.q = PackedHeads{q, st_q, sh_q}; a.k = PackedHeads{k, st_k, sh_k};
   a.v = PackedHeads{v, st_v, sh_v}; a.o = PackedHeads{o, st_o, sh_o};
   a.lse = lse; a.dtype = dtype; a.total = total; a.H = (int)Hq; a.Hkv = (int)Hkv; a.d = d;
   a.starts = starts; a.B = B; a.causal = causal ? 1 : 0; a.window = window; a.scale = scale;
   a.tail = tail ? 1 : 0;
-  return launch_packed_attention(a, STREAM(stream));
+  return launch_packed_attention(a, workspace, STREAM(stream));
 }
 
 int64_t blt_packed_attention_backward_workspace_bytes(int64_t total, int64_t Hq, int64_t Hkv) {

@@ -29,20 +29,24 @@ struct PArgs {
   float scale, c;      // c: log2(e) * scale
   int tail;
   int tiles, residues, units;  // row (or key) tiles; see tile_of
+  const int* order;            // the tiles, longest first, or null: see packed_order_kernel
 };
 
 // The key head and the tile of block `bid`.  Dispatch places block i on XCD i % 8; a
 // unit, the tiles of one key head with one residue modulo `residues`, belongs to one XCD, whose L2 its
 // keys share.  Every XCD has the same number of units (`units`), and residues rather than
-// runs so that all units have about the same work.
-__device__ inline bool tile_of(const PArgs& p, int& kvh, int& tile) {
+// runs so that all units have about the same work.  Without an order, the last tiles first (`down`)
+// or the first ones: the long ones of a single causal sequence.
+__device__ inline bool tile_of(const PArgs& p, bool down, int& kvh, int& tile) {
   const uint32_t x = blockIdx.x & 7, l = blockIdx.x >> 3;
   const uint32_t step = l / (uint32_t)p.units;
   const uint32_t u = x * (uint32_t)p.units + (l - step * (uint32_t)p.units);
   kvh = (int)(u / (uint32_t)p.residues);
   const int residue = (int)(u - (uint32_t)kvh * (uint32_t)p.residues);
-  tile = p.tiles - 1 - residue - p.residues * (int)step;  // (long causal rows first)
-  return tile >= 0;
+  const int rank = residue + p.residues * (int)step;
+  if (rank >= p.tiles) return false;
+  tile = p.order ? p.order[rank] : down ? p.tiles - 1 - rank : rank;
+  return true;
 }
 
 // The sequence [a, e) of token `tok`, false if it lies in none.  Starts that do not ascend
@@ -84,6 +88,88 @@ __device__ inline bool keys_of(const PArgs& p, int tok, int& klo, int& khi) {
     khi = -1;
   }
   return in;
+}
+
+// Tiles by their lengths, longest first, so that the blocks that start last are short ones (12
+// documents of up to 8192 tokens, 12 heads of 64: 423 us in the order of the tokens, whose last blocks are
+// the first document's long ones, MEASURED so; the order itself takes 5).  Block 0: the row tiles,
+// block 1: the key tiles (null: not asked for).  Tiles of one of 256 lengths in any order: it does not change
+// what they hold.
+constexpr int kOrderTiles = 8192, kOrderStarts = 4096;
+__global__ __launch_bounds__(1024) void packed_order_kernel(PArgs p, int rows, int keys, int* row_order,
+                                                            int* key_order) {
+  constexpr int PER = kOrderTiles / 1024;
+  __shared__ int starts[kOrderStarts + 1], hist[256], longest;
+  const bool of_rows = blockIdx.x == 0;
+  int* out = of_rows ? row_order : key_order;
+  if (!out) return;
+  const int each = of_rows ? rows : keys, n = of_rows ? p.rows : p.total;
+  const int tiles = (n + each - 1) / each, tid = threadIdx.x;
+  const int32_t* at = p.starts;
+  if (p.B <= kOrderStarts) {
+    for (int i = tid; i <= p.B; i += 1024) starts[i] = p.starts[i];
+    at = starts;
+  }
+  if (tid < 256) hist[tid] = 0;
+  if (tid == 0) longest = 1;
+  __syncthreads();
+  // the sequence of a token (the last one for those behind it)
+  auto sequence = [&](int tok, int& a, int& e) {
+    int lo = 0, hi = p.B - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (at[mid + 1] > tok) hi = mid; else lo = mid + 1;
+    }
+    a = min(max(at[lo], 0), tok);
+    e = max(at[lo + 1], tok + 1);
+  };
+  int length[PER], most = 1;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int i = tid + 1024 * j;
+    length[j] = 0;
+    if (i >= tiles) continue;
+    const int x0 = i * each, x1 = min(x0 + each, n) - 1;
+    const int t0 = of_rows ? over(x0, p.by_g) : x0, t1 = of_rows ? over(x1, p.by_g) : x1;
+    int a, e, a1, e1;
+    sequence(t0, a, e);
+    sequence(t1, a1, e1);
+    int64_t lo, hi;  // tokens on the other side
+    if (of_rows) {
+      lo = p.window ? max(a, t0 - p.window + 1) : a;
+      hi = p.causal ? t1 : e1 - 1;
+    } else {
+      lo = p.causal ? t0 : a;
+      hi = p.window ? min((int64_t)e1 - 1, (int64_t)t1 + p.window - 1) : e1 - 1;
+    }
+    length[j] = (int)min((hi - lo) / 32 + 1, (int64_t)1 << 24);
+    most = max(most, length[j]);
+  }
+  most = wave_max_i32(most);
+  if ((tid & 63) == 0) atomicMax(&longest, most);
+  __syncthreads();
+  int cls[PER];
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    cls[j] = 255 - (int)((int64_t)length[j] * 255 / longest);
+    if (tid + 1024 * j < tiles) atomicAdd(&hist[cls[j]], 1);
+  }
+  __syncthreads();
+  if (tid < 64) {  // exclusive sums of 256 counts
+    int v[4], sum = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] = sum;
+      sum += hist[4 * tid + i];
+    }
+    const int before = wave_incl_scan(sum) - sum;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) hist[4 * tid + i] = before + v[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < PER; ++j)
+    if (tid + 1024 * j < tiles) out[atomicAdd(&hist[cls[j]], 1)] = tid + 1024 * j;
 }
 
 // LDS tiles have rows of D elements without padding; 16-byte chunk c of row r is stored at
@@ -187,7 +273,7 @@ __global__ __launch_bounds__(256, 2) void packed_attn_kernel(PArgs p) {
   __shared__ __attribute__((aligned(1024))) uint16_t lds[NST * STAGE];
 
   int kvh, tile;
-  if (!tile_of(p, kvh, tile)) return;
+  if (!tile_of(p, true, kvh, tile)) return;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lrow = lane & 31, lhalf = lane >> 5;
@@ -403,7 +489,7 @@ __global__ __launch_bounds__(256) void packed_attn_f32_kernel(PArgs p) {
   __shared__ __attribute__((aligned(16))) float so[NW * 32 * OP];
   __shared__ float sm[NW][32], sl[NW][32];
   int kvh, rt;
-  if (!tile_of(p, kvh, rt)) return;
+  if (!tile_of(p, true, kvh, rt)) return;
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l31 = lane & 31, h = lane >> 5;
@@ -653,7 +739,7 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(GArgs ga) {
   __shared__ __attribute__((aligned(1024))) uint16_t lds[NST * STAGE];
 
   int kvh, tile;
-  if (!tile_of(p, kvh, tile)) return;
+  if (!tile_of(p, true, kvh, tile)) return;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lrow = lane & 31, lhalf = lane >> 5;
@@ -846,8 +932,7 @@ __global__ __launch_bounds__(64 * KW * RW, D == 64 ? 3 : 2) void packed_dkdv_ker
   __shared__ __attribute__((aligned(1024))) uint16_t lds[NST * STAGE + (V_LDS ? BK * D : 0)];
 
   int kvh, tile;
-  if (!tile_of(p, kvh, tile)) return;
-  tile = p.tiles - 1 - tile;  // (long causal columns first)
+  if (!tile_of(p, false, kvh, tile)) return;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6), wk = wid % KW, wr = wid / KW;
   const int lrow = lane & 31, lhalf = lane >> 5;
@@ -1134,7 +1219,7 @@ __global__ __launch_bounds__(256) void packed_dq_f32_kernel(GArgs ga) {
   typedef float vf_t __attribute__((ext_vector_type(VW)));
   __shared__ __attribute__((aligned(16))) float so[NW * 32 * OP];
   int kvh, rt;
-  if (!tile_of(p, kvh, rt)) return;
+  if (!tile_of(p, true, kvh, rt)) return;
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int l31 = lane & 31, h = lane >> 5;
@@ -1262,8 +1347,7 @@ __global__ __launch_bounds__(256) void packed_dkdv_f32_kernel(GArgs ga) {
   typedef float vf_t __attribute__((ext_vector_type(VW)));
   __shared__ __attribute__((aligned(16))) float so[NW * 32 * OP];
   int kvh, tile;
-  if (!tile_of(p, kvh, tile)) return;
-  tile = p.tiles - 1 - tile;  // (long causal columns first)
+  if (!tile_of(p, false, kvh, tile)) return;
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int l31 = lane & 31, h = lane >> 5;
@@ -1402,13 +1486,37 @@ PArgs args_of(const PackedAttnArgs& a) {
   return p;
 }
 
+// An order for n rows (or keys) in tiles of `each`: for several sequences, where the blocks are
+// more than two of a CU and there is room for it.
+bool ordered(int64_t B, int64_t n, int each, int Hkv) {
+  const int64_t tiles = (n + each - 1) / each;
+  return B > 1 && tiles * Hkv >= 512 && tiles <= kOrderTiles;
+}
+// Keys of a tile of dk and dv.  With few tiles the longest takes longer than a CU's share of the work:
+// half as many keys, and twice the rows at a time (32 / 8 heads of 128: one sequence of 4096
+// 311 us, 433 with 128 keys; four of up to 4096, 9 k tokens, 676 and 738; four of 4096 1254 and 1164).
+int key_tile(int64_t total, int Hkv, int d, bool f32) {
+  return f32 ? 32 : d == 128 && Hkv * ((total + 127) / 128) <= 768 ? 64 : 128;
+}
+
 }  // namespace
 
-int launch_packed_attention(const PackedAttnArgs& a, hipStream_t s) {
+int64_t packed_attention_workspace_bytes(int64_t B, int64_t total, int H, int Hkv, int dtype) {
+  const int64_t rows = total * (H / Hkv);
+  const int each = dtype == BLT_DTYPE_F32 ? 32 : 128;
+  return ordered(B, rows, each, Hkv) ? (rows + each - 1) / each * 4 : 0;
+}
+
+int launch_packed_attention(const PackedAttnArgs& a, void* ws, hipStream_t s) {
   PArgs p = args_of(a);
   const bool f32 = a.dtype == BLT_DTYPE_F32;
-  const int64_t nb = plan_tiles(p, p.rows, f32 ? 32 : 128, a.Hkv);
+  const int each = f32 ? 32 : 128;
+  const int64_t nb = plan_tiles(p, p.rows, each, a.Hkv);
   if (nb > 0x7fffffff) return fail(BLT_ERR_SHAPE, "packed_attention: too many tiles");
+  if (ordered(a.B, p.rows, each, a.Hkv)) {
+    hipLaunchKernelGGL(packed_order_kernel, dim3(1), dim3(1024), 0, s, p, each, 0, (int*)ws, nullptr);
+    p.order = (const int*)ws;
+  }
   const dim3 grid((unsigned)nb), block(256);
   if (f32 && a.d == 64)
     hipLaunchKernelGGL((packed_attn_f32_kernel<2>), grid, block, 0, s, p);
@@ -1426,8 +1534,9 @@ int launch_packed_attention(const PackedAttnArgs& a, hipStream_t s) {
   return 0;
 }
 
+// the stats of 64 rows each, then the orders of row and key tiles
 int64_t packed_attention_backward_workspace_bytes(int64_t total, int H, int Hkv) {
-  return (int64_t)Hkv * ((total * (H / Hkv) + 63) / 64) * 512;
+  return (int64_t)Hkv * ((total * (H / Hkv) + 63) / 64) * 512 + 2 * kOrderTiles * 4;
 }
 
 int launch_packed_attention_backward(const PackedAttnArgs& a, const PackedGradArgs& g, void* ws,
@@ -1441,13 +1550,18 @@ int launch_packed_attention_backward(const PackedAttnArgs& a, const PackedGradAr
   p.stats = (float*)ws;
   p.stat_tiles = (p.a.rows + 63) / 64;
   const bool f32 = a.dtype == BLT_DTYPE_F32;
-  const int64_t nq = plan_tiles(p.a, p.a.rows, f32 ? 32 : 128, a.Hkv);
-  // Keys of a tile.  With few tiles the longest takes longer than a CU's share of the work:
-  // half as many keys, and twice the rows at a time (32 / 8 heads of 128: one sequence of 4096
-  // 311 us, 433 with 128 keys; four of up to 4096, 9 k tokens, 676 and 738; four of 4096 1254 and 1164).
-  const int bk = f32 ? 32 : a.d == 128 && (int64_t)a.Hkv * ((a.total + 127) / 128) <= 768 ? 64 : 128;
+  const int bk = key_tile(a.total, a.Hkv, a.d, f32), bq = f32 ? 32 : 128;
+  int* orders = (int*)(p.stats + (int64_t)a.Hkv * p.stat_tiles * 128);
+  const bool by_rows = ordered(a.B, p.a.rows, bq, a.Hkv), by_keys = ordered(a.B, a.total, bk, a.Hkv);
+  if (by_rows || by_keys) {
+    hipLaunchKernelGGL(packed_order_kernel, dim3(2), dim3(1024), 0, s, p.a, bq, bk,
+                       by_rows ? orders : nullptr, by_keys ? orders + kOrderTiles : nullptr);
+  }
   GArgs pk = p;
-  const int64_t nk = plan_tiles(pk.a, p.a.total, bk, a.Hkv);
+  const int64_t nq = plan_tiles(p.a, p.a.rows, bq, a.Hkv);
+  const int64_t nk = plan_tiles(pk.a, a.total, bk, a.Hkv);
+  if (by_rows) p.a.order = orders;
+  if (by_keys) pk.a.order = orders + kOrderTiles;
   if (nq > 0x7fffffff || nk > 0x7fffffff)
     return fail(BLT_ERR_SHAPE, "packed_attention_backward: too many tiles");
   const dim3 gq((unsigned)nq), gk((unsigned)nk), block(256);

@@ -22,7 +22,8 @@ struct PackedAttnArgs {
   float scale;
   int tail;  // tokens behind the last sequence: 0 = left alone, 1 = zeros
 };
-int launch_packed_attention(const PackedAttnArgs& a, hipStream_t s);
+int64_t packed_attention_workspace_bytes(int64_t B, int64_t total, int H, int Hkv, int dtype);
+int launch_packed_attention(const PackedAttnArgs& a, void* ws, hipStream_t s);
 
 // a.o and a.lse are the forward's; g: the output's gradient; dq, dk, dv are written
 struct PackedGradArgs {

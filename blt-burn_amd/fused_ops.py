@@ -342,10 +342,17 @@ def fused_packed_attention(q, k, v, starts, causal=True, window=0, scale=None, o
     if return_lse:
         lse = torch.empty((total, H), dtype=torch.float32, device=q.device)
         lp = lse.data_ptr()
-    call_on(q.device, q.get_device(), _lib.lib().blt_packed_attention, "packed_attention", qp, qs,
-            qh, kp, ks, kh, vp, vs, vh, op, os_, oh, lp,
-            _lib.DTYPE_BF16 if q.dtype == torch.bfloat16 else _lib.DTYPE_F32, total, H, k.shape[1],
-            d, starts.data_ptr(), starts.shape[0] - 1, 1 if causal else 0, window, scale, tail)
+    L, Hkv, B = _lib.lib(), k.shape[1], starts.shape[0] - 1
+    dtype = _lib.DTYPE_BF16 if q.dtype == torch.bfloat16 else _lib.DTYPE_F32
+    size, wp = 0, None
+    if B > 1 and total * H > 1 << 13:
+        size = L.blt_packed_attention_workspace_bytes(B, total, H, Hkv, dtype)
+        if size:
+            ws = torch.empty(size, dtype=torch.uint8, device=q.device)
+            wp = ws.data_ptr()
+    call_on(q.device, q.get_device(), L.blt_packed_attention, "packed_attention", qp, qs, qh, kp, ks,
+            kh, vp, vs, vh, op, os_, oh, lp, dtype, total, H, Hkv, d, starts.data_ptr(), B,
+            1 if causal else 0, window, scale, tail, wp, size)
     return (out, lse) if return_lse else out
 
 

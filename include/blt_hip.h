@@ -164,13 +164,17 @@ int blt_fused_sample(const void* logits, int64_t row_stride, int32_t dtype, int6
  *   lse:    (may be NULL) f32 [total, Hq], log of the sum of e^score, -inf where it is 0
  *   tail:   tokens at starts[B] and behind: 0 = left alone, 1 = outputs 0, lse -inf
  * Scores, softmax and sums in f32; in bf16 the weights are rounded to bf16.  A key whose
- * score is -inf weighs nothing; infinite and NaN values come through where they are seen. */
+ * score is -inf weighs nothing; infinite and NaN values come through where they are seen.
+ * workspace: blt_packed_attention_workspace_bytes (0 for small calls and one sequence), 16-byte
+ * aligned, no initialisation; calls that share one must be stream-ordered. */
+int64_t blt_packed_attention_workspace_bytes(int64_t B, int64_t total, int64_t Hq, int64_t Hkv,
+                                             int32_t dtype);
 int blt_packed_attention(const void* q, int64_t st_q, int64_t sh_q, const void* k, int64_t st_k,
                          int64_t sh_k, const void* v, int64_t st_v, int64_t sh_v, void* o,
                          int64_t st_o, int64_t sh_o, float* lse, int32_t dtype, int64_t total,
                          int64_t Hq, int64_t Hkv, int32_t d, const int32_t* starts, int64_t B,
                          int32_t causal, int32_t window, float scale, int32_t tail,
-                         blt_stream_t stream);
+                         void* workspace, int64_t workspace_bytes, blt_stream_t stream);
 
 /* Gradients of blt_packed_attention's q, k and v from that of its output, with its o and lse;
  * the other arguments as there, a head stride of q and grad_o times Hq / Hkv at most 2^29.  dq
