@@ -52,7 +52,7 @@ EXPORTS = {
     "blt_packed_attention": (c_i32, [c_vp, c_i64, c_i64] * 4 + [c_vp, c_i32] + [c_i64] * 3
                              + [c_i32, c_vp, c_i64, c_i32, c_i32, c_f32, c_i32, c_vp, c_i64, c_vp]),
     "blt_packed_attention_workspace_bytes": (c_i64, [c_i64] * 4 + [c_i32]),
-    "blt_packed_attention_backward_workspace_bytes": (c_i64, [c_i64] * 3),
+    "blt_packed_attention_backward_workspace_bytes": (c_i64, [c_i64] * 3 + [c_i32] * 2),
     "blt_packed_attention_backward": (c_i32, [c_vp, c_i64, c_i64] * 5 + [c_vp]
                                       + [c_vp, c_i64, c_i64] * 3 + [c_i32] + [c_i64] * 3
                                       + [c_i32, c_vp, c_i64, c_i32, c_i32, c_f32, c_vp, c_i64,

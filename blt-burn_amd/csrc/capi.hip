@@ -357,12 +357,14 @@ int blt_packed_attention(const void* q, int64_t st_q, int64_t sh_q, const void* 
   return launch_packed_attention(a, workspace, STREAM(stream));
 }
 
-int64_t blt_packed_attention_backward_workspace_bytes(int64_t total, int64_t Hq, int64_t Hkv) {
+int64_t blt_packed_attention_backward_workspace_bytes(int64_t total, int64_t Hq, int64_t Hkv,
+                                                      int32_t d, int32_t dtype) {
   // (0 for what blt_packed_attention_backward refuses)
   if (Hkv < 1 || Hq < 1 || Hq > 0xffff || Hq % Hkv || total < 0 || total > 0x7ffe0000 ||
-      Hq * total > 0x7ffe0000)
+      Hq * total > 0x7ffe0000 || (d != 64 && d != 128) ||
+      (dtype != BLT_DTYPE_F32 && dtype != BLT_DTYPE_BF16))
     return 0;
-  return packed_attention_backward_workspace_bytes(total, (int)Hq, (int)Hkv);
+  return packed_attention_backward_workspace_bytes(total, (int)Hq, (int)Hkv, d, dtype);
 }
 int blt_packed_attention_backward(
     const void* grad_o, int64_t st_go, int64_t sh_go, const void* q, int64_t st_q, int64_t sh_q,
@@ -385,7 +387,8 @@ int blt_packed_attention_backward(
     return fail(BLT_ERR_SHAPE, std::string(what) + ": head strides of q and grad_o too large");
   if (!lse) return fail(BLT_ERR_INVALID, std::string(what) + ": null pointer");
   if (!workspace || ((uintptr_t)workspace & 15) ||
-      workspace_bytes < packed_attention_backward_workspace_bytes(total, (int)Hq, (int)Hkv))
+      workspace_bytes <
+          packed_attention_backward_workspace_bytes(total, (int)Hq, (int)Hkv, d, dtype))
     return fail(BLT_ERR_INVALID, std::string(what) + ": workspace missing, misaligned or too small");
   PackedAttnArgs a{};
   a.q = x[1]; a.k = x[2]; a.v = x[3]; a.o = x[4];

@@ -8,6 +8,7 @@
 // because a sequence ends in it: tiles of rows run over the ends of sequences, so that the grid
 // follows from the number of tokens alone and many short sequences share a tile.  A wave passes the
 // key tiles that none of its rows sees.
+#include <algorithm>
 #include <type_traits>
 
 #include "attn_tiles.hpp"
@@ -695,6 +696,7 @@ struct GArgs {
   // for 64 rows each: -L log2(e) of them, then -D
   float* stats;
   int stat_tiles;  // of a key head
+  float* part;     // dk and dv of one of several blocks of a tile's rows: see packed_join_kernel
 };
 __device__ inline float* stats_of(const GArgs& p, int kvh, int row) {
   return p.stats + (((int64_t)kvh * p.stat_tiles + (row >> 6)) * 128 + (row & 63));
@@ -1181,8 +1183,8 @@ __global__ __launch_bounds__(64 * KW * RW, D == 64 ? 3 : 2) void packed_dkdv_ker
 
 // f32, as packed_attn_f32_kernel: a block has 32 rows (dq) or 32 keys (dk, dv) in registers, its four
 // waves take every fourth tile of 32 of the others from global memory and add up at the end.
-// Sum of the four waves' [D][32] results, scaled, into rows out(i).
-template <int ND, typename F>
+// Sum of the waves' [D][32] results, scaled, into rows out(i).
+template <int ND, int NW, typename F>
 __device__ inline void add_waves(float* so, const f32x16_t (&acc)[ND], float scale, F out) {
   constexpr int D = 32 * ND, OP = D + 4, VW = ND % 4 == 0 ? 4 : 2, NV = ND / VW;
   typedef float vf_t __attribute__((ext_vector_type(VW)));
@@ -1199,15 +1201,17 @@ __device__ inline void add_waves(float* so, const f32x16_t (&acc)[ND], float sca
       *reinterpret_cast<vf_t*>(row + VW * (8 * (i >> 2) + 4 * h + (i & 3)) + 32 * VW * n) = x;
     }
   __syncthreads();
-  for (int i = tid; i < 32 * (D / 4); i += 256) {
+  for (int i = tid; i < 32 * (D / 4); i += 64 * NW) {
     const int rr = i / (D / 4), cc = (i % (D / 4)) * 4;
     float* to = out(rr);
     if (!to) continue;
-    f32x4_t x[4];
+    f32x4_t x[NW];
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
+    for (int k = 0; k < NW; ++k)
       x[k] = *reinterpret_cast<const f32x4_t*>(so + (k * 32 + rr) * OP + cc);
-    *reinterpret_cast<f32x4_t*>(to + cc) = ((x[0] + x[1]) + (x[2] + x[3])) * scale;
+    f32x4_t sum = (x[0] + x[1]) + (x[2] + x[3]);
+    if constexpr (NW == 8) sum += (x[4] + x[5]) + (x[6] + x[7]);
+    *reinterpret_cast<f32x4_t*>(to + cc) = sum * scale;
   }
 }
 
@@ -1332,17 +1336,21 @@ __global__ __launch_bounds__(256) void packed_dq_f32_kernel(GArgs ga) {
       }
     }
   }
-  add_waves<ND>(so, acc, p.scale, [&](int rr) -> float* {
+  add_waves<ND, NW>(so, acc, p.scale, [&](int rr) -> float* {
     if (r0 + rr >= p.rows) return nullptr;
     const int t = over(r0 + rr, p.by_g), g = r0 + rr - t * p.G;
     return (float*)ga.dq + (int64_t)t * ga.st_dq + (int64_t)(kvh * p.G + g) * ga.sh_dq;
   });
 }
 
-template <int ND>
-__global__ __launch_bounds__(256) void packed_dkdv_f32_kernel(GArgs ga) {
+__device__ inline int64_t part_at(const PArgs& p, int slice, int kvh, int tile) {
+  return ((int64_t)slice * (p.H / p.G) + kvh) * p.tiles + tile;
+}
+
+template <int ND, int NW>
+__global__ __launch_bounds__(64 * NW) void packed_dkdv_f32_kernel(GArgs ga) {
   const PArgs& p = ga.a;
-  constexpr int D = 32 * ND, NW = 4, NC = 4 * ND, OP = D + 4, BR = 32;
+  constexpr int D = 32 * ND, NC = 4 * ND, OP = D + 4, BR = 32;
   constexpr int VW = ND % 4 == 0 ? 4 : 2, NV = ND / VW;
   typedef float vf_t __attribute__((ext_vector_type(VW)));
   __shared__ __attribute__((aligned(16))) float so[NW * 32 * OP];
@@ -1376,7 +1384,8 @@ __global__ __launch_bounds__(256) void packed_dkdv_f32_kernel(GArgs ga) {
   for (int n = 0; n < ND; ++n)
 #pragma unroll
     for (int i = 0; i < 16; ++i) dk[n][i] = dv[n][i] = 0.f;
-  for (int t = t0 + w; t < t1; t += NW) {
+  const int slice = (int)blockIdx.y, slices = (int)gridDim.y;
+  for (int t = t0 + slice * NW + w; t < t1; t += NW * slices) {
     const int rb = t * BR;
     const float* qr = row_at(p.q, p.st_q, p.sh_q, rb + l31);
     const float* gr = row_at(ga.g, ga.st_g, ga.sh_g, rb + l31);
@@ -1455,11 +1464,37 @@ __global__ __launch_bounds__(256) void packed_dkdv_f32_kernel(GArgs ga) {
       }
     }
   }
+  if (slices > 1) {
+    float* to = ga.part + part_at(p, slice, kvh, tile) * (2 * 32 * D);
+    add_waves<ND, NW>(so, dk, 1.f, [&](int i) { return to + i * D; });
+    add_waves<ND, NW>(so, dv, 1.f, [&](int i) { return to + (32 + i) * D; });
+    return;
+  }
   auto out = [&](void* x, int64_t st, int64_t sh, int i) -> float* {
     return j0 + i < p.total ? (float*)x + (int64_t)(j0 + i) * st + (int64_t)kvh * sh : nullptr;
   };
-  add_waves<ND>(so, dk, p.scale, [&](int i) { return out(ga.dk, ga.st_dk, ga.sh_dk, i); });
-  add_waves<ND>(so, dv, 1.f, [&](int i) { return out(ga.dv, ga.st_dv, ga.sh_dv, i); });
+  add_waves<ND, NW>(so, dk, p.scale, [&](int i) { return out(ga.dk, ga.st_dk, ga.sh_dk, i); });
+  add_waves<ND, NW>(so, dv, 1.f, [&](int i) { return out(ga.dv, ga.st_dv, ga.sh_dv, i); });
+}
+
+// dk and dv of a tile from the parts of its `slices` blocks, in their order
+template <int ND>
+__global__ __launch_bounds__(256) void packed_join_kernel(GArgs ga, int slices) {
+  const PArgs& p = ga.a;
+  constexpr int D = 32 * ND;
+  const int tile = (int)blockIdx.x, kvh = (int)blockIdx.y, what = (int)blockIdx.z;
+  void* x = what ? ga.dv : ga.dk;
+  const int64_t st = what ? ga.st_dv : ga.st_dk, sh = what ? ga.sh_dv : ga.sh_dk;
+  for (int i = (int)threadIdx.x; i < 32 * D / 4; i += 256) {
+    const int rr = i / (D / 4), cc = i % (D / 4) * 4, key = tile * 32 + rr;
+    if (key >= p.total) return;
+    f32x4_t sum = {};
+    for (int k = 0; k < slices; ++k)
+      sum += *reinterpret_cast<const f32x4_t*>(
+          ga.part + part_at(p, k, kvh, tile) * (2 * 32 * D) + (32 * what + rr) * D + cc);
+    *reinterpret_cast<f32x4_t*>((float*)x + (int64_t)key * st + (int64_t)kvh * sh + cc) =
+        sum * (what ? 1.f : p.scale);
+  }
 }
 
 // ---- launch ----------------------------------------------------------------------------
@@ -1534,9 +1569,22 @@ int launch_packed_attention(const PackedAttnArgs& a, void* ws, hipStream_t s) {
   return 0;
 }
 
-// the stats of 64 rows each, then the orders of row and key tiles
-int64_t packed_attention_backward_workspace_bytes(int64_t total, int H, int Hkv) {
+// Blocks that share a key tile's rows in f32: as many as give every SIMD four waves, at most 8 (12 / 4
+// heads of 64, sequences of 1000, 77 and 439: 114 us with the join, 191 alone; 8 heads of
+// 128 over one key head, two of 2000: 828 and 1880; where tiles are many two blocks were
+// slower, 472 and 445).
+int key_slices(int64_t total, int Hkv, int d, bool f32) {
+  const int64_t blocks = (total + 31) / 32 * Hkv, fill = d == 64 ? 512 : 1024;
+  return f32 && blocks > 0 && blocks < fill ? (int)std::min<int64_t>(fill / blocks, 8) : 1;
+}
+// the stats of 64 rows each, the orders of row and key tiles, then the parts of dk and dv
+int64_t stats_bytes(int64_t total, int H, int Hkv) {
   return (int64_t)Hkv * ((total * (H / Hkv) + 63) / 64) * 512 + 2 * kOrderTiles * 4;
+}
+int64_t packed_attention_backward_workspace_bytes(int64_t total, int H, int Hkv, int d, int dtype) {
+  const int slices = key_slices(total, Hkv, d, dtype == BLT_DTYPE_F32);
+  return stats_bytes(total, H, Hkv) +
+         (slices > 1 ? slices * ((total + 31) / 32) * Hkv * (2 * 32 * 4) * d : 0);
 }
 
 int launch_packed_attention_backward(const PackedAttnArgs& a, const PackedGradArgs& g, void* ws,
@@ -1564,13 +1612,18 @@ int launch_packed_attention_backward(const PackedAttnArgs& a, const PackedGradAr
   if (by_keys) pk.a.order = orders + kOrderTiles;
   if (nq > 0x7fffffff || nk > 0x7fffffff)
     return fail(BLT_ERR_SHAPE, "packed_attention_backward: too many tiles");
-  const dim3 gq((unsigned)nq), gk((unsigned)nk), block(256);
+  const int slices = key_slices(a.total, a.Hkv, a.d, f32);
+  pk.part = (float*)((char*)ws + stats_bytes(a.total, a.H, a.Hkv));
+  const dim3 gq((unsigned)nq), gk((unsigned)nk, slices), block(256);
+  const dim3 gj(pk.a.tiles, a.Hkv, 2);
   if (f32 && a.d == 64) {
     hipLaunchKernelGGL((packed_dq_f32_kernel<2>), gq, block, 0, s, p);
-    hipLaunchKernelGGL((packed_dkdv_f32_kernel<2>), gk, block, 0, s, pk);
+    hipLaunchKernelGGL((packed_dkdv_f32_kernel<2, 8>), gk, dim3(512), 0, s, pk);
+    if (slices > 1) hipLaunchKernelGGL((packed_join_kernel<2>), gj, block, 0, s, pk, slices);
   } else if (f32) {
     hipLaunchKernelGGL((packed_dq_f32_kernel<4>), gq, block, 0, s, p);
-    hipLaunchKernelGGL((packed_dkdv_f32_kernel<4>), gk, block, 0, s, pk);
+    hipLaunchKernelGGL((packed_dkdv_f32_kernel<4, 4>), gk, block, 0, s, pk);
+    if (slices > 1) hipLaunchKernelGGL((packed_join_kernel<4>), gj, block, 0, s, pk, slices);
   } else if (a.d == 64) {
     hipLaunchKernelGGL((packed_dq_kernel<64>), gq, block, 0, s, p);
     hipLaunchKernelGGL((packed_dkdv_kernel<64, 4, 1, 64>), gk, block, 0, s, pk);

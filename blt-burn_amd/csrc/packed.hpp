@@ -29,7 +29,7 @@ int launch_packed_attention(const PackedAttnArgs& a, void* ws, hipStream_t s);
 struct PackedGradArgs {
   PackedHeads g, dq, dk, dv;
 };
-int64_t packed_attention_backward_workspace_bytes(int64_t total, int H, int Hkv);
+int64_t packed_attention_backward_workspace_bytes(int64_t total, int H, int Hkv, int d, int dtype);
 int launch_packed_attention_backward(const PackedAttnArgs& a, const PackedGradArgs& g, void* ws,
                                      hipStream_t s);
 

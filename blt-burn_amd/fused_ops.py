@@ -318,8 +318,9 @@ def fused_packed_attention(q, k, v, starts, causal=True, window=0, scale=None, o
     starts[-1] and behind get 0 in a new tensor and are left alone in `out`.  Scores and sums
     are f32 throughout; in bf16 the weights are rounded to bf16.  Autograd follows it for o
     (once; `out` takes no inputs that need a gradient)."""
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad
-                                       for t in (q, k, v)):
+    if torch.is_grad_enabled() and (getattr(q, "requires_grad", False)
+                                    or getattr(k, "requires_grad", False)
+                                    or getattr(v, "requires_grad", False)):
         if out is not None:
             raise BltError("fused_packed_attention: out takes no inputs that need a gradient (use "
                            "torch.no_grad())")
@@ -380,13 +381,13 @@ def fused_packed_attention_backward(grad_o, q, k, v, o, lse, starts, causal=True
     L = _lib.lib()
     dq = torch.empty((total, H, d), dtype=q.dtype, device=q.device)
     dk, dv = (torch.empty((total, Hkv, d), dtype=q.dtype, device=q.device) for _ in range(2))
-    size = L.blt_packed_attention_backward_workspace_bytes(total, H, Hkv)
+    dtype = _lib.DTYPE_BF16 if q.dtype == torch.bfloat16 else _lib.DTYPE_F32
+    size = L.blt_packed_attention_backward_workspace_bytes(total, H, Hkv, d, dtype)
     ws = torch.empty(size, dtype=torch.uint8, device=q.device)
     call_on(q.device, q.get_device(), L.blt_packed_attention_backward, "packed_attention_backward",
             gp, gs, gh, qp, qs, qh, kp, ks, kh, vp, vs, vh, op, os_, oh, lse.data_ptr(),
-            dq.data_ptr(), H * d, d, dk.data_ptr(), Hkv * d, d, dv.data_ptr(), Hkv * d, d,
-            _lib.DTYPE_BF16 if q.dtype == torch.bfloat16 else _lib.DTYPE_F32, total, H, Hkv, d,
-            starts.data_ptr(), starts.shape[0] - 1, 1 if causal else 0, window, scale,
+            dq.data_ptr(), H * d, d, dk.data_ptr(), Hkv * d, d, dv.data_ptr(), Hkv * d, d, dtype,
+            total, H, Hkv, d, starts.data_ptr(), starts.shape[0] - 1, 1 if causal else 0, window, scale,
             ws.data_ptr(), size)
     return dq, dk, dv
 

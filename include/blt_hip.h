@@ -182,7 +182,8 @@ int blt_packed_attention(const void* q, int64_t st_q, int64_t sh_q, const void* 
  * Sums in f32, the weights and their gradients rounded to bf16 in bf16; the same bits
  * in every run.  workspace: blt_packed_attention_backward_workspace_bytes, 16-byte aligned, no
  * initialisation; calls that share one must be stream-ordered. */
-int64_t blt_packed_attention_backward_workspace_bytes(int64_t total, int64_t Hq, int64_t Hkv);
+int64_t blt_packed_attention_backward_workspace_bytes(int64_t total, int64_t Hq, int64_t Hkv,
+                                                      int32_t d, int32_t dtype);
 int blt_packed_attention_backward(
     const void* grad_o, int64_t st_go, int64_t sh_go, const void* q, int64_t st_q, int64_t sh_q,
     const void* k, int64_t st_k, int64_t sh_k, const void* v, int64_t st_v, int64_t sh_v,
