@@ -93,7 +93,7 @@ __device__ inline bool keys_of(const PArgs& p, int tok, int& klo, int& khi) {
 
 // Tiles by their lengths, longest first, so that the blocks that start last are short ones (12
 // documents of up to 8192 tokens, 12 heads of 64: 423 us in the order of the tokens, whose last blocks are
-// the first document's long ones, MEASURED so; the order itself takes 5).  Block 0: the row tiles,
+// the first document's long ones, and 403 in this one; the order itself takes 5).  Block 0: the row tiles,
 // block 1: the key tiles (null: not asked for).  Tiles of one of 256 lengths in any order: it does not change
 // what they hold.
 constexpr int kOrderTiles = 8192, kOrderStarts = 4096;
@@ -918,11 +918,16 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(GArgs ga) {
   }
 }
 
+// Where a slice's part of dk (0) or dv (1) of a key lies, in rows of head_dim f32.
+__device__ inline int64_t part_at(const PArgs& p, int slice, int kvh, int what, int key) {
+  return (((int64_t)slice * (p.H / p.G) + kvh) * 2 + what) * p.total + key;
+}
+
 // dk and dv, bf16.  One block = 4 x 2 waves: 32 keys each, and one half of the rows of a tile
 // each; tiles of BR rows, Q beside dO, pass through LDS.  S = Q . K^T and dP = dO . V^T put a key into
 // a lane and rows into registers, from which P and dS feed dV^T = dO^T . P and dK^T = Q^T . dS.
 // The two halves are added up at the end.
-template <int D, int KW, int RW, int BR>
+template <int D, int KW, int RW, int BR, bool SLICED>
 __global__ __launch_bounds__(64 * KW * RW, D == 64 ? 3 : 2) void packed_dkdv_kernel(GArgs ga) {
   const PArgs& p = ga.a;
   constexpr int NW = KW * RW, KPW = 32, BK = KW * KPW, SHARE = BR / RW;
@@ -987,12 +992,14 @@ __global__ __launch_bounds__(64 * KW * RW, D == 64 ? 3 : 2) void packed_dkdv_ker
     }
   };
   const uint16_t* sv = lds + NST * STAGE;  // V of the block's keys
-  if (V_LDS && t0 < t1) {
+  const int slices = SLICED ? (int)gridDim.y : 1;
+  const int from = SLICED ? t0 + (int)blockIdx.y : t0;  // (and every slices-th tile)
+  if (V_LDS && from < t1) {
     const char* vt = (const char*)p.v + ((int64_t)tile * BK * p.st_v + (int64_t)kvh * p.sh_v) * 2;
 #pragma unroll
     for (int i = 0; i < BK / NW / RPI; ++i) {
-      const int r = BK / NW * wid + RPI * i + kin, from = min(r, p.total - 1 - tile * BK);
-      dma16_so(vt, (unsigned)from * (unsigned)(p.st_v * 2) + (unsigned)((slot ^ swz<D>(r)) * 16),
+      const int r = BK / NW * wid + RPI * i + kin, row = min(r, p.total - 1 - tile * BK);
+      dma16_so(vt, (unsigned)row * (unsigned)(p.st_v * 2) + (unsigned)((slot ^ swz<D>(r)) * 16),
                lds_base + (unsigned)(NST * STAGE + (BK / NW * wid + RPI * i) * D) * 2);
     }
   }
@@ -1121,12 +1128,12 @@ __global__ __launch_bounds__(64 * KW * RW, D == 64 ? 3 : 2) void packed_dkdv_ker
       products(sq, r0, bw, be, std::false_type{});
   };
 
-  if (t0 < t1) issue(t0, 0);
+  if (from < t1) issue(from, 0);
   int stage = 0;
-  for (int t = t0; t < t1; ++t) {
-    // tile t has landed and every wave is past tile t - 1, whose stage is free
+  for (int t = from; t < t1; t += slices) {
+    // tile t has landed and every wave is past the one before, whose stage is free
     dma_wait_barrier<0>();
-    if (t + 1 < t1) issue(t + 1, stage ^ 1);
+    if (t + slices < t1) issue(t + slices, stage ^ 1);
     const uint16_t* sq = lds + stage * STAGE;
     stage ^= 1;
 #pragma unroll 1
@@ -1163,7 +1170,19 @@ __global__ __launch_bounds__(64 * KW * RW, D == 64 ? 3 : 2) void packed_dkdv_ker
     add(dk);
     add(dv);
   }
-  if (wr == 0 && kw + lrow < p.total) {
+  if (SLICED && wr == 0 && kw + lrow < p.total) {
+    float* ok = ga.part + part_at(p, (int)blockIdx.y, kvh, 0, key) * D + 4 * lhalf;
+    float* ov = ga.part + part_at(p, (int)blockIdx.y, kvh, 1, key) * D + 4 * lhalf;
+#pragma unroll
+    for (int ds = 0; ds < DS; ++ds)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        *reinterpret_cast<f32x4_t*>(ok + ds * 32 + 8 * j) = f32x4_t{
+            dk[ds][4 * j], dk[ds][4 * j + 1], dk[ds][4 * j + 2], dk[ds][4 * j + 3]};
+        *reinterpret_cast<f32x4_t*>(ov + ds * 32 + 8 * j) = f32x4_t{
+            dv[ds][4 * j], dv[ds][4 * j + 1], dv[ds][4 * j + 2], dv[ds][4 * j + 3]};
+      }
+  } else if (wr == 0 && kw + lrow < p.total) {
     uint16_t* ok = (uint16_t*)ga.dk + (int64_t)key * ga.st_dk + (int64_t)kvh * ga.sh_dk;
     uint16_t* ov = (uint16_t*)ga.dv + (int64_t)key * ga.st_dv + (int64_t)kvh * ga.sh_dv;
 #pragma unroll
@@ -1343,10 +1362,6 @@ __global__ __launch_bounds__(256) void packed_dq_f32_kernel(GArgs ga) {
   });
 }
 
-__device__ inline int64_t part_at(const PArgs& p, int slice, int kvh, int tile) {
-  return ((int64_t)slice * (p.H / p.G) + kvh) * p.tiles + tile;
-}
-
 template <int ND, int NW>
 __global__ __launch_bounds__(64 * NW) void packed_dkdv_f32_kernel(GArgs ga) {
   const PArgs& p = ga.a;
@@ -1465,9 +1480,11 @@ __global__ __launch_bounds__(64 * NW) void packed_dkdv_f32_kernel(GArgs ga) {
     }
   }
   if (slices > 1) {
-    float* to = ga.part + part_at(p, slice, kvh, tile) * (2 * 32 * D);
-    add_waves<ND, NW>(so, dk, 1.f, [&](int i) { return to + i * D; });
-    add_waves<ND, NW>(so, dv, 1.f, [&](int i) { return to + (32 + i) * D; });
+    auto part = [&](int what, int i) {
+      return j0 + i < p.total ? ga.part + part_at(p, slice, kvh, what, j0 + i) * D : nullptr;
+    };
+    add_waves<ND, NW>(so, dk, 1.f, [&](int i) { return part(0, i); });
+    add_waves<ND, NW>(so, dv, 1.f, [&](int i) { return part(1, i); });
     return;
   }
   auto out = [&](void* x, int64_t st, int64_t sh, int i) -> float* {
@@ -1477,24 +1494,25 @@ __global__ __launch_bounds__(64 * NW) void packed_dkdv_f32_kernel(GArgs ga) {
   add_waves<ND, NW>(so, dv, 1.f, [&](int i) { return out(ga.dv, ga.st_dv, ga.sh_dv, i); });
 }
 
-// dk and dv of a tile from the parts of its `slices` blocks, in their order
-template <int ND>
+// dk and dv from the parts of their tiles' blocks, in the blocks' order: a thread 4 values of one
+template <int D, typename T>
 __global__ __launch_bounds__(256) void packed_join_kernel(GArgs ga, int slices) {
   const PArgs& p = ga.a;
-  constexpr int D = 32 * ND;
-  const int tile = (int)blockIdx.x, kvh = (int)blockIdx.y, what = (int)blockIdx.z;
-  void* x = what ? ga.dv : ga.dk;
-  const int64_t st = what ? ga.st_dv : ga.st_dk, sh = what ? ga.sh_dv : ga.sh_dk;
-  for (int i = (int)threadIdx.x; i < 32 * D / 4; i += 256) {
-    const int rr = i / (D / 4), cc = i % (D / 4) * 4, key = tile * 32 + rr;
-    if (key >= p.total) return;
-    f32x4_t sum = {};
-    for (int k = 0; k < slices; ++k)
-      sum += *reinterpret_cast<const f32x4_t*>(
-          ga.part + part_at(p, k, kvh, tile) * (2 * 32 * D) + (32 * what + rr) * D + cc);
-    *reinterpret_cast<f32x4_t*>((float*)x + (int64_t)key * st + (int64_t)kvh * sh + cc) =
-        sum * (what ? 1.f : p.scale);
-  }
+  const int kvh = (int)blockIdx.y, what = (int)blockIdx.z;
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= (int64_t)p.total * D) return;
+  const float* x = ga.part + part_at(p, 0, kvh, what, 0) * D + i;
+  const int64_t step = part_at(p, 1, 0, 0, 0) * D;
+  f32x4_t sum = *reinterpret_cast<const f32x4_t*>(x);
+  for (int k = 1; k < slices; ++k) sum += *reinterpret_cast<const f32x4_t*>(x + k * step);
+  if (!what) sum *= p.scale;
+  T* to = (T*)(what ? ga.dv : ga.dk) + i / D * (what ? ga.st_dv : ga.st_dk) +
+          kvh * (what ? ga.sh_dv : ga.sh_dk) + i % D;
+  if constexpr (std::is_same<T, float>::value)
+    *reinterpret_cast<f32x4_t*>(to) = sum;
+  else
+    *reinterpret_cast<u32x2_t*>(to) =
+        u32x2_t{pack_bf16x2(sum[0], sum[1]), pack_bf16x2(sum[2], sum[3])};
 }
 
 // ---- launch ----------------------------------------------------------------------------
@@ -1529,9 +1547,9 @@ bool ordered(int64_t B, int64_t n, int each, int Hkv) {
 }
 // Keys of a tile of dk and dv.  With few tiles the longest takes longer than a CU's share of the work:
 // half as many keys, and twice the rows at a time (32 / 8 heads of 128: one sequence of 4096
-// 311 us, 433 with 128 keys; four of up to 4096, 9 k tokens, 676 and 738; four of 4096 1254 and 1164).
+// 331 us, 440 with 128 keys; four of up to 4096, 10.8 k tokens, 696 and 665).
 int key_tile(int64_t total, int Hkv, int d, bool f32) {
-  return f32 ? 32 : d == 128 && Hkv * ((total + 127) / 128) <= 768 ? 64 : 128;
+  return f32 ? 32 : d == 128 && Hkv * ((total + 127) / 128) <= 512 ? 64 : 128;
 }
 
 }  // namespace
@@ -1569,22 +1587,32 @@ int launch_packed_attention(const PackedAttnArgs& a, void* ws, hipStream_t s) {
   return 0;
 }
 
-// Blocks that share a key tile's rows in f32: as many as give every SIMD four waves, at most 8 (12 / 4
-// heads of 64, sequences of 1000, 77 and 439: 114 us with the join, 191 alone; 8 heads of
-// 128 over one key head, two of 2000: 828 and 1880; where tiles are many two blocks were
-// slower, 472 and 445).
-int key_slices(int64_t total, int Hkv, int d, bool f32) {
-  const int64_t blocks = (total + 31) / 32 * Hkv, fill = d == 64 ? 512 : 1024;
-  return f32 && blocks > 0 && blocks < fill ? (int)std::min<int64_t>(fill / blocks, 8) : 1;
+// Blocks that share a key tile's rows, each every so-many-th row tile: where the tiles are fewer than
+// keep the device even, at most 8 (`seen`: about how many rows a key has, 0 for unknown: a block
+// gets 256 of them or more).  Their parts cost a join of 4 to 10 us.  dk and dv, sliced with the join
+// and in one block:
+//   f32   12 / 4 heads of 64: 1000 + 77 + 439 tokens 119 and 191 us, 1000 + 780 + 439 147 and 195,
+//         4 x 1000 284 and 313; 8 / 1 heads of 128: 2 x 2000 822 and 1880; but with 1.5 times
+//         the blocks 12 / 12 of 64, 2 x 1000, 153 and 130
+//   bf16  12 / 4 heads of 64: the first of these 33 and 87, 8 x 1000 78 and 120; 12 heads: 1 x
+//         4096 99 and 131; 8 / 1 heads of 128: 2 x 2000 89 and 268; 32 / 8 of 128: 1 x 2048 106 and
+//         133, but 4 x 500 68 and 52 (so fewer where keys have few rows), 4 x 100 31 and 20
+int key_slices(int64_t total, int Hkv, int d, bool f32, int64_t seen) {
+  const int each = key_tile(total, Hkv, d, f32);
+  const int64_t blocks = (total + each - 1) / each * Hkv;
+  const int64_t fill = f32 ? 1024 : d == 64 ? 768 : seen == 0 || seen >= 4096 ? 512 : 256;
+  if (blocks < 1 || blocks >= fill) return 1;
+  const int64_t most = seen > 0 ? std::max<int64_t>(seen / 256, 1) : 8;
+  return (int)std::min<int64_t>(std::min<int64_t>(fill / blocks, 8), most);
 }
 // the stats of 64 rows each, the orders of row and key tiles, then the parts of dk and dv
 int64_t stats_bytes(int64_t total, int H, int Hkv) {
   return (int64_t)Hkv * ((total * (H / Hkv) + 63) / 64) * 512 + 2 * kOrderTiles * 4;
 }
 int64_t packed_attention_backward_workspace_bytes(int64_t total, int H, int Hkv, int d, int dtype) {
-  const int slices = key_slices(total, Hkv, d, dtype == BLT_DTYPE_F32);
+  const int slices = key_slices(total, Hkv, d, dtype == BLT_DTYPE_F32, 0);
   return stats_bytes(total, H, Hkv) +
-         (slices > 1 ? slices * ((total + 31) / 32) * Hkv * (2 * 32 * 4) * d : 0);
+         (slices > 1 ? slices * total * Hkv * 8 * d : 0);
 }
 
 int launch_packed_attention_backward(const PackedAttnArgs& a, const PackedGradArgs& g, void* ws,
@@ -1612,27 +1640,43 @@ int launch_packed_attention_backward(const PackedAttnArgs& a, const PackedGradAr
   if (by_keys) pk.a.order = orders + kOrderTiles;
   if (nq > 0x7fffffff || nk > 0x7fffffff)
     return fail(BLT_ERR_SHAPE, "packed_attention_backward: too many tiles");
-  const int slices = key_slices(a.total, a.Hkv, a.d, f32);
+  const int64_t mean = a.total / std::max<int64_t>(a.B, 1);
+  const int64_t seen = std::max<int64_t>(p.a.window ? std::min<int64_t>(mean, p.a.window + bk) : mean,
+                                         1) * p.a.G;
+  const int slices = key_slices(a.total, a.Hkv, a.d, f32, seen);
   pk.part = (float*)((char*)ws + stats_bytes(a.total, a.H, a.Hkv));
   const dim3 gq((unsigned)nq), gk((unsigned)nk, slices), block(256);
-  const dim3 gj(pk.a.tiles, a.Hkv, 2);
   if (f32 && a.d == 64) {
     hipLaunchKernelGGL((packed_dq_f32_kernel<2>), gq, block, 0, s, p);
     hipLaunchKernelGGL((packed_dkdv_f32_kernel<2, 8>), gk, dim3(512), 0, s, pk);
-    if (slices > 1) hipLaunchKernelGGL((packed_join_kernel<2>), gj, block, 0, s, pk, slices);
   } else if (f32) {
     hipLaunchKernelGGL((packed_dq_f32_kernel<4>), gq, block, 0, s, p);
     hipLaunchKernelGGL((packed_dkdv_f32_kernel<4, 4>), gk, block, 0, s, pk);
-    if (slices > 1) hipLaunchKernelGGL((packed_join_kernel<4>), gj, block, 0, s, pk, slices);
   } else if (a.d == 64) {
     hipLaunchKernelGGL((packed_dq_kernel<64>), gq, block, 0, s, p);
-    hipLaunchKernelGGL((packed_dkdv_kernel<64, 4, 1, 64>), gk, block, 0, s, pk);
+    if (slices > 1)
+      hipLaunchKernelGGL((packed_dkdv_kernel<64, 4, 1, 64, true>), gk, block, 0, s, pk);
+    else
+      hipLaunchKernelGGL((packed_dkdv_kernel<64, 4, 1, 64, false>), gk, block, 0, s, pk);
   } else {
     hipLaunchKernelGGL((packed_dq_kernel<128>), gq, block, 0, s, p);
-    if (bk == 64)
-      hipLaunchKernelGGL((packed_dkdv_kernel<128, 2, 4, 128>), gk, dim3(512), 0, s, pk);
+    if (slices > 1)  // (never where tiles have 128 keys: they are too many for it)
+      hipLaunchKernelGGL((packed_dkdv_kernel<128, 2, 4, 128, true>), gk, dim3(512), 0, s, pk);
+    else if (bk == 64)
+      hipLaunchKernelGGL((packed_dkdv_kernel<128, 2, 4, 128, false>), gk, dim3(512), 0, s, pk);
     else
-      hipLaunchKernelGGL((packed_dkdv_kernel<128, 4, 2, 64>), gk, dim3(512), 0, s, pk);
+      hipLaunchKernelGGL((packed_dkdv_kernel<128, 4, 2, 64, false>), gk, dim3(512), 0, s, pk);
+  }
+  if (slices > 1) {
+    const dim3 grid((unsigned)((a.total * a.d + 1023) / 1024), (unsigned)a.Hkv, 2);
+    if (f32 && a.d == 64)
+      hipLaunchKernelGGL((packed_join_kernel<64, float>), grid, block, 0, s, pk, slices);
+    else if (f32)
+      hipLaunchKernelGGL((packed_join_kernel<128, float>), grid, block, 0, s, pk, slices);
+    else if (a.d == 64)
+      hipLaunchKernelGGL((packed_join_kernel<64, uint16_t>), grid, block, 0, s, pk, slices);
+    else
+      hipLaunchKernelGGL((packed_join_kernel<128, uint16_t>), grid, block, 0, s, pk, slices);
   }
   BLT_LAUNCH_CHECK("packed_dq_kernel, packed_dkdv_kernel");
   return 0;

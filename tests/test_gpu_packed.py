@@ -74,6 +74,25 @@ def test_longer_ones(dtype, lens, window):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("d,H,K", [(64, 12, 4), (64, 8, 1), (128, 8, 1), (128, 12, 4)])
+@pytest.mark.parametrize("lens,causal,window", [([700, 0, 500, 45], True, 0), ([900, 300], True, 400),
+                                                ([1, 640], False, 0)])
+def test_rows_shared_by_several_blocks(dtype, d, H, K, lens, causal, window):
+    """Few keys of many rows: their gradients come from several blocks."""
+    q, k, v, do = made(lens, 30, H, K, d, TYPES[dtype], seed=d + H)
+    out = both(q, k, v, do, starts_of(lens), causal=causal, window=window)
+    assert not any(x[sum(lens):].any() for x in (out[0],) + out[2:])
+
+
+@pytest.mark.parametrize("dtype,d", [("bf16", 64), ("bf16", 128), ("f32", 64)])
+def test_many_tiles_in_an_order_of_their_own(dtype, d):
+    lens = [900, 1, 640, 0, 159]
+    q, k, v, do = made(lens, 11, 40, 40, d, TYPES[dtype], seed=2)
+    out = both(q, k, v, do, starts_of(lens))
+    assert not any(x[sum(lens):].any() for x in (out[0],) + out[2:])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_layouts(dtype):
     """Rows of any order and alignment give the bits of dense ones."""
     t, d, H, K, lens = TYPES[dtype], 64, 4, 2, [70, 33]
@@ -178,6 +197,25 @@ def test_not_finite_stays_where_it_is_seen(dtype, value, where, d, H, K, window)
     if where == "do":
         assert bool((~torch.isfinite(got[4][first:at + 1, 0, 5])).all())
         assert bool((~torch.isfinite(got[2][at, 0])).all())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_not_finite_with_rows_shared_by_several_blocks(dtype, d):
+    """(as above: one bad dO, one bad q; 8 heads of one key head, sequences of 600 and 500)"""
+    st, at, t = [0, 600, 1100], 700, TYPES[dtype]
+    q, k, v, do = (x.clone() for x in made([600, 500], 0, 8, 1, d, t))
+    r = R.attention(q, k, v, st, do=do, u=U[t])
+    q[at, 3, 1], do[at, 5, 2] = math.inf, math.nan
+    o, lse = F.fused_packed_attention(q, k, v, i32(st), return_lse=True)
+    dq, dk, dv = F.fused_packed_attention_backward(do, q, k, v, o, lse, i32(st))
+    i = torch.arange(1100)
+    rows, keys = i == at, (i >= 600) & (i <= at)
+    for name, x in (("o", o), ("lse", lse), ("dq", dq), ("dk", dk), ("dv", dv)):
+        keep = ~(keys if name in ("dk", "dv") else rows)
+        near(x[keep.to(DEV)], {name: r[name][keep], "tol_" + name: r["tol_" + name][keep]}, name)
+    assert bool(torch.isnan(dv[600:at + 1, 0, 2]).all())
+    assert bool((~torch.isfinite(dk[600:at + 1, 0])).all())
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
