@@ -179,7 +179,7 @@ def fused_attention(q, k, v, use_causal_mask, window=0, rope_theta=0.0):
 def _row_setting(x, what, like, dtype, lo, hi):
     """A number of all rows, or a tensor of one each: (number, pointer or None, what to keep)."""
     if isinstance(x, torch.Tensor):
-        if x.dtype != dtype or x.device != like.device or x.shape != like.shape:
+        if x.dtype is not dtype or x.get_device() != like.get_device() or x.shape != like.shape:
             raise BltError("fused_sample: %s must be a number or %s %s on %s"
                            % (what, dtype, tuple(like.shape), like.device))
         x = contiguous(x)
@@ -209,7 +209,8 @@ def fused_sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0
     if logits.dim() == 0 or not 1 <= logits.shape[-1] <= 1 << 20:
         raise BltError("fused_sample expects logits [..., vocab], vocab 1 .. 2^20")
     shape, V = logits.shape[:-1], logits.shape[-1]
-    if uniform.dtype != torch.float32 or uniform.shape != shape or uniform.device != logits.device:
+    if uniform.dtype is not torch.float32 or uniform.shape != shape or \
+            uniform.get_device() != logits.get_device():
         raise BltError("fused_sample: uniform must be f32 %s on %s" % (tuple(shape), logits.device))
     x = logits if logits.dim() == 2 and (logits.stride(1) == 1 or V == 1) and \
         logits.stride(0) >= 0 else contiguous(logits)
@@ -245,23 +246,27 @@ def _packed_heads(t, what, like=None, heads=None):
     strides."""
     if not isinstance(t, torch.Tensor):
         raise TypeError("expected a torch.Tensor, got %r" % type(t))
+    shape = t.shape
     if like is None:
         require_cuda(t)
         _dtype_ok(t)
-        if t.dim() != 3 or t.shape[2] not in (64, 128):
+        if len(shape) != 3 or shape[2] not in (64, 128):
             raise BltError("fused_packed_attention: %s must be [tokens, heads, head_dim 64 or 128]"
                            % what)
-    elif t.device != like.device or t.dtype != like.dtype or t.dim() != 3 or \
-            t.shape[0] != like.shape[0] or t.shape[2] != like.shape[2] or \
-            (heads is not None and t.shape[1] != heads):
-        raise BltError("fused_packed_attention: %s must be %s [%d, %s, %d] on %s"
-                       % (what, like.dtype, like.shape[0], "heads" if heads is None else heads,
-                          like.shape[2], like.device))
+    else:
+        n, _, d = like.shape
+        if t.get_device() != like.get_device() or t.dtype is not like.dtype or len(shape) != 3 or \
+                shape[0] != n or shape[2] != d or (heads is not None and shape[1] != heads):
+            raise BltError("fused_packed_attention: %s must be %s [%d, %s, %d] on %s"
+                           % (what, like.dtype, n, "heads" if heads is None else heads, d,
+                              like.device))
     st, sh, sd = t.stride()
-    if sd != 1 or (st | sh) % (16 // t.element_size()) or t.data_ptr() % 16 or st > 1 << 23:
+    p = t.data_ptr()
+    if sd != 1 or (st | sh) & (3 if t.dtype is torch.float32 else 7) or p & 15 or st > 1 << 23:
         t = t.clone(memory_format=torch.contiguous_format)
-        st, sh, sd = t.stride()
-    return t, t.data_ptr(), st, sh
+        st, sh, _ = t.stride()
+        p = t.data_ptr()
+    return t, p, st, sh
 
 
 def _packed_setting(q, k, starts, window, scale):
@@ -270,8 +275,8 @@ def _packed_setting(q, k, starts, window, scale):
         raise BltError("fused_packed_attention: heads must be a multiple of kv_heads")
     if not isinstance(starts, torch.Tensor):
         raise TypeError("expected a torch.Tensor, got %r" % type(starts))
-    if starts.dtype is not torch.int32 or starts.device != q.device or starts.dim() != 1 or \
-            not starts.is_contiguous() or starts.shape[0] < 1:
+    if starts.dtype is not torch.int32 or starts.get_device() != q.get_device() or \
+            starts.dim() != 1 or not starts.is_contiguous() or starts.shape[0] < 1:
         raise BltError("fused_packed_attention: starts must be a contiguous int32 [sequences + 1] "
                        "on %s" % q.device)
     if window < 0:
