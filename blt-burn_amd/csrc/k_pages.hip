@@ -629,8 +629,10 @@ __global__ __launch_bounds__(NT) void common_prefix_kernel(blt_paged_cache c, in
     int pages;
     __syncthreads();
     slots[tid] = i0 + tid < n ? slot_at(i0 + tid, &pages) : -1;
+    // (the same for all threads, which divide the entries by it: read before the barrier, behind
+    // which `full` may shrink; what lies behind does not matter then)
+    const int cols = full;
     __syncthreads();
-    const int cols = full;  // (it may shrink below: what lies behind does not matter then)
     const int64_t all = (int64_t)min(NT, n - i0) * cols;
     int j = cols ? tid / cols : 0, at = cols ? tid - j * cols : 0;
     const int dj = cols ? NT / cols : 0, dat = cols ? NT - dj * cols : 0;

@@ -91,6 +91,25 @@ def test_common_prefix_of_many(n, cols):
         assert c.common_prefix().tolist() == [8 * at]
 
 
+def test_common_prefix_where_every_sequence_parts_elsewhere():
+    """Threads that find a difference early must not leave what others have yet to compare."""
+    c = C.PagedCache(1, 1, 64, num_pages=16, max_seqs=700, max_len=8 * 640, page_size=8)
+    r = np.random.RandomState(4)
+    table = np.zeros((700, c.max_pages), np.int32)  # (page numbers that nothing reads)
+    c.lens.fill_(8 * 640)
+    for _ in range(20):
+        table[:] = 1
+        first = r.randint(1, 640, 700)
+        first[r.randint(0, 700)] = 0
+        low = int(r.randint(0, 300))
+        for b in range(1, 700):  # one sequence parts at `low`, the others behind it
+            table[b, low + first[b] % (640 - low):] = 2
+        b = r.randint(1, 700)
+        table[b, low] = 3
+        c.page_table.copy_(i32(table))
+        assert c.common_prefix().tolist() == [8 * low]
+
+
 # ---- attention with it ------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
