@@ -9,13 +9,16 @@
 //
 // No sorting: all three rules keep a prefix of the ranks, so a row's choice is a cut, the last
 // kept (logit, index), found by counting.  Weights are exponentials in 64 bits rounded to
-// fixed point (2^SCALE = 1, so that a row's sum stays below 2^63): sums of integers do not
-// depend on their order, so the tokens are the same bits in every run whatever adds up first, and off
-// by at most vocab / 2^(SCALE + 1) of the largest weight.
+// fixed point (the largest is 2^scale, scale = 62 - ceil(log2 vocab), so that a row's sum stays below
+// 2^63): sums of integers do not depend on their order, so the tokens are the same in every run
+// whatever adds up first.  A weight is off by less than 2^-44 of itself (see weight) and by its
+// rounding, 2^-(scale + 1) of the largest.
 //
 // By the size of the vocabulary: up to 1024 a wave holds a row in registers and bisects
 // the cut over the bits of the logits; up to 16384 a block holds it in LDS and counts bins; above that rows are
 // cut into parts, in five launches.
+#include <algorithm>
+
 #include "sample.hpp"
 
 namespace blt {
@@ -1031,32 +1034,48 @@ int run(const SArgs& g, hipStream_t s) {
 
 }  // namespace
 
+// Rows of one round of launches: where they are in parts, 8192 of these fill the chip four times, and
+// what they leave behind (41 KB each) stays below 340 MB.
+static int64_t rows_at_once(int64_t rows, int64_t parts) {
+  return parts ? std::min<int64_t>(rows, 8192 / parts) : rows;
+}
 int64_t sample_workspace_bytes(int64_t rows, int vocab) {
   const int64_t parts = parts_of(vocab);
+  rows = rows_at_once(rows, parts);
   return parts ? rows * (parts * (12 * (int64_t)NB + sizeof(Entry) * NT + 16) + sizeof(Found)) : 0;
 }
 
 int launch_sample(const SampleArgs& a, void* ws, hipStream_t s) {
   SArgs g{};
-  g.x = a.logits; g.st = a.row_stride; g.rows = a.rows; g.V = a.vocab; g.u = a.uniform;
-  g.s = a.set; g.out = a.out;
+  g.st = a.row_stride; g.V = a.vocab; g.s = a.set;
   int l = 0;
   while (((int64_t)1 << l) < a.vocab) ++l;
   g.scale = 62 - l;
   g.parts = parts_of(a.vocab);
-  const int64_t n = a.rows * g.parts;
-  if (n > 0x7fffffff || a.rows > 0x7fffffff)
-    return fail(BLT_ERR_SHAPE, "fused_sample: too many rows");
+  if (a.rows > 0x7fffffff) return fail(BLT_ERR_SHAPE, "fused_sample: too many rows");
+  const int64_t each = rows_at_once(a.rows, g.parts), n = each * g.parts;
   if (g.parts) {
     g.hm = (uint64_t*)ws;
     g.pmass = g.hm + n * NB;
     g.list = (Entry*)(g.pmass + n);
     g.found = (Found*)(g.list + n * NT);
-    g.hc = (uint32_t*)(g.found + a.rows);
+    g.hc = (uint32_t*)(g.found + each);
     g.pmax = (float*)(g.hc + n * NB);
     g.count = (int*)(g.pmax + n);
   }
-  return a.dtype == BLT_DTYPE_BF16 ? run<uint16_t>(g, s) : run<float>(g, s);
+  const bool bf16 = a.dtype == BLT_DTYPE_BF16;
+  for (int64_t row = 0; row < a.rows; row += each) {
+    g.rows = std::min(each, a.rows - row);
+    g.x = (const char*)a.logits + row * a.row_stride * (bf16 ? 2 : 4);
+    g.u = a.uniform + row;
+    g.out = a.out + row;
+    if (a.set.temperatures) g.s.temperatures = a.set.temperatures + row;
+    if (a.set.top_ps) g.s.top_ps = a.set.top_ps + row;
+    if (a.set.min_ps) g.s.min_ps = a.set.min_ps + row;
+    if (a.set.top_ks) g.s.top_ks = a.set.top_ks + row;
+    if (int rc = bf16 ? run<uint16_t>(g, s) : run<float>(g, s)) return rc;
+  }
+  return 0;
 }
 
 }  // namespace blt

@@ -142,8 +142,8 @@ int blt_fused_attention_f32(const float* q, const float* k, const float* v, floa
  * never drawn; one of +inf takes everything with its like.  tokens: int32 [rows]; -1 for a row with a NaN,
  * without a logit above -inf, or with a setting out of range (temperature >= 0 and finite, top_k >= 0,
  * top_p > 0, min_p 0 .. 1).
- * Weights are rounded to 2^(ceil(log2 vocab) - 63) of the largest and summed exactly: the same
- * tokens in every run.  workspace: blt_fused_sample_workspace_bytes (0 up to vocab 16384), 16-byte
+ * Weights are off by less than 2^-42 of the largest and summed exactly: the same tokens in
+ * every run.  workspace: blt_fused_sample_workspace_bytes (0 up to vocab 16384), 16-byte
  * aligned, no initialisation; calls that share one must be stream-ordered. */
 int64_t blt_fused_sample_workspace_bytes(int64_t rows, int32_t vocab);
 int blt_fused_sample(const void* logits, int64_t row_stride, int32_t dtype, int64_t rows,

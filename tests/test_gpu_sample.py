@@ -169,6 +169,31 @@ def test_many_tokens_between_two_bins(V):
             assert torch.equal(F.fused_sample(x, u, **names(s)).cpu(), reference(x, u, **s)), s
 
 
+@pytest.mark.parametrize("V", [300, 2000, 20000])
+@pytest.mark.parametrize("t", [1e-6, 1e-300, 5e-324, 1e30, 1e300])
+def test_extreme_temperatures(V, t):
+    """Only the largest logits are left, or all are alike."""
+    x, u = logits_of(6, V, torch.float32, seed=V)
+    x[:3, V // 3] = x[:3, V // 2] = x[:3].amax(1) + 1  # (two largest ones)
+    for s in (dict(t=t), dict(t=t, p=0.7), dict(t=t, k=5, m=0.1)):
+        assert torch.equal(F.fused_sample(x, u, **names(s)).cpu(), reference(x, u, **s)), s
+
+
+def test_more_rows_than_one_round_of_launches():
+    """Rows of 17000 tokens are in two parts, 4096 rows a round: each row as in a call of its own."""
+    n, V = 4100, 17000
+    x, u = logits_of(n, V, torch.bfloat16, seed=8)
+    t = torch.rand(n, device=DEV) + 0.5
+    k = torch.arange(n, dtype=torch.int32, device=DEV) % 60
+    p, m = 1 - 0.5 * torch.rand(n, device=DEV), 0.01 * torch.rand(n, device=DEV)
+    got = F.fused_sample(x, u, t, k, p, m)
+    for rows in (slice(0, 40), slice(4080, 4100)):
+        want = reference(x[rows], u[rows], *(y[rows].double().cpu().numpy() for y in (t, k, p, m)))
+        assert torch.equal(got[rows].cpu(), want)
+        assert torch.equal(got[rows], F.fused_sample(x[rows], u[rows], t[rows], k[rows], p[rows],
+                                                     m[rows]))
+
+
 def test_all_tokens_in_turn():
     """u over a fine grid draws every kept token as often as its weight says."""
     x, _ = logits_of(1, 260, torch.float32, seed=9, spread=1.0)
