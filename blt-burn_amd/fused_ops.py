@@ -342,8 +342,8 @@ def fused_packed_attention(q, k, v, starts, causal=True, window=0, scale=None, o
         op, os_, oh = out.data_ptr(), H * d, d
     else:
         t, op, os_, oh = _packed_heads(out, "out", q, H)
-        if t is not out:
-            raise BltError("fused_packed_attention: out needs dense, 16-byte aligned rows")
+        if t is not out or (os_ == 0 and total > 1) or (oh == 0 and H > 1):
+            raise BltError("fused_packed_attention: out needs dense, 16-byte aligned rows of their own")
     lse = lp = None
     if return_lse:
         lse = torch.empty((total, H), dtype=torch.float32, device=q.device)
@@ -351,7 +351,7 @@ def fused_packed_attention(q, k, v, starts, causal=True, window=0, scale=None, o
     L, Hkv, B = _lib.lib(), k.shape[1], starts.shape[0] - 1
     dtype = _lib.DTYPE_BF16 if q.dtype == torch.bfloat16 else _lib.DTYPE_F32
     size, wp = 0, None
-    if B > 1 and total * H > 1 << 13:
+    if B > 1 and (total * H >> 5) + Hkv >= 512:  # (below that it takes none)
         size = L.blt_packed_attention_workspace_bytes(B, total, H, Hkv, dtype)
         if size:
             ws = torch.empty(size, dtype=torch.uint8, device=q.device)

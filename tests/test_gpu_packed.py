@@ -151,6 +151,13 @@ def test_large_offsets(dtype):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_many_heads_of_few_tokens(dtype):
+    """(as many tiles as a pack of many tokens has, and an order of them)"""
+    q, k, v, do = made([2, 1], 2, 512, 512, 64, TYPES[dtype])
+    both(q, k, v, do, [0, 2, 3])
+
+
 # ---- values that are not finite ----------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
@@ -377,6 +384,8 @@ def test_refusals():
               lambda: F.fused_packed_attention(q, k, v, s, scale=math.nan),
               lambda: F.fused_packed_attention(q, k, v, s, out=torch.empty_like(k)),
               lambda: F.fused_packed_attention(q, k, v, s, out=o.float()),
+              lambda: F.fused_packed_attention(q, k, v, s, out=o[:, :1].expand(-1, 4, -1)),
+              lambda: F.fused_packed_attention(q, k, v, s, out=o[:1].expand(10, -1, -1)),
               lambda: F.fused_packed_attention(q, k, v, s, out=torch.empty(10, 4, 65, device=DEV,
                                                                            dtype=q.dtype)[..., 1:]),
               lambda: F.fused_packed_attention(q.cpu(), k.cpu(), v.cpu(), s.cpu()),
