@@ -422,7 +422,7 @@ __device__ inline bool shared_part(const KArgs& p, const Item& it, int token, in
     }
     return true;
   }
-  add_parts<D, 8>(p, ml, o, 0, prefix_parts(p, it.from), a);
+  add_parts<D, 16>(p, ml, o, 0, prefix_parts(p, it.from), a);
   return false;
 }
 template <int D, int BQ, int NT, typename T, int MODE>
