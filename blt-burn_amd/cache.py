@@ -45,8 +45,9 @@ class PagedCache:
 
     Beside them a cache keeps the workspace of its attention calls, as large as the calls
     so far have needed: at most 35 MB for single tokens, 104 MB (head_dim 64) or 136 MB (128)
-    for any call, and up to a third more where it has grown; a call with a prefix takes 4
-    (head_dim + 2) bytes more for every token and head.  The first call of a size may allocate."""
+    for any call, and up to a third more where it has grown; a call with a prefix takes
+    up to 26 or 52 MB more, or 8 (head_dim + 2) bytes for every token and head (rounded up to 128
+    a key head) where that is more.  The first call of a size may allocate."""
 
     def __init__(self, n_layers, n_kv_heads, head_dim, num_pages, max_seqs, max_len, page_size=16,
                  dtype=torch.bfloat16, device=None):

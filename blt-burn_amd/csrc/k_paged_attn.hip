@@ -14,12 +14,13 @@
 // where find_item spills 4 * resident), parts in need of joining <= twice those blocks (every
 // one of them has more than half of C).
 //
-// A prefix that all sequences share (the same pages) is read once for all of them, in two
-// launches of the same kernels: PREFIX takes the tokens of all sequences as the rows of one, over
-// the keys of the prefix, which they all see whole, in parts whose unnormalised outputs,
-// maxima and sums it leaves in memory; TAILS takes each sequence's keys from there on, and joins its
-// rows' parts of the prefix to them.  (Joined by the block whose part ends last, as others are, one block
-// had all rows of a key head to join.)
+// A prefix that all sequences share (the same pages) is read once for all of them, by the same
+// code: PREFIX takes the tokens of all sequences as the rows of one, over the keys of the
+// prefix, which they all see whole, in parts whose unnormalised outputs, maxima and sums it leaves
+// in memory.  Each sequence's keys from there on are either a launch behind it (TAILS), which joins its
+// rows' parts of the prefix to them, or (bf16, 33 rows or more in all, up to 32 of a sequence) blocks
+// beside it (OWN), with a launch that joins both.  (Joined by the block whose part ends
+// last, as others are, one block had all rows of a key head to join.)
 #include <algorithm>
 #include <type_traits>
 
@@ -30,7 +31,7 @@ namespace blt {
 
 namespace {
 
-enum Mode { WHOLE, PREFIX, TAILS };
+enum Mode { WHOLE, PREFIX, TAILS, OWN };
 
 struct KArgs {
   const void *q, *k, *v;  // k, v: the layer's first element
@@ -53,6 +54,11 @@ struct KArgs {
   float* pre_o;
   float* pre_ml;
   int pre_tiles, pre_parts, pre_rows, pre_keys;  // pre_keys: of a key tile
+  // OWN: what a row has of its own, [key heads][pre_tiles][pre_rows][D] and [..][2], and the number
+  // of keys that PREFIX took
+  float* own_o;
+  float* own_ml;
+  int* taken;
 };
 
 // ---- which item ----------------------------------------------------------------
@@ -133,6 +139,7 @@ __device__ bool find_item(const KArgs& p, unsigned bid, Item& it) {
     room = min(p.prefix[0], -wave_max_i32(-room));
     from = __builtin_amdgcn_readfirstlane(room > 0 ? room >> p.lps << p.lps : 0);
     if constexpr (MODE == PREFIX) {
+      if (p.taken && bid == 0 && threadIdx.x == 0) *p.taken = __any(crossed) ? 0 : from;
       if (__any(crossed) || slot < 0 || from == 0) return false;  // (TAILS reports it)
       const int a = p.starts[0], e = p.starts[p.B];
       it.q = Seq{a, e - a, from, slot};
@@ -404,13 +411,23 @@ __device__ inline void add_parts(const KArgs& p, const float* ml, const float* o
       }
   }
 }
-// Four columns of a row's part: PREFIX leaves them for TAILS (true: nothing more to do), which
-// joins all of them.
+// Four columns of a row's part: PREFIX leaves them for TAILS, which joins all of them, or, with
+// OWN's, for paged_attn_join_kernel (true: nothing more to do).
 template <int D, int MODE>
 __device__ inline bool shared_part(const KArgs& p, const Item& it, int token, int g, int dd,
                                    Joined& a) {
   if constexpr (MODE == WHOLE) return false;
-  const int row = (token - p.starts[0]) * p.G + g, rt = row / p.pre_rows, r = row - rt * p.pre_rows;
+  const int row = (token - p.starts[0]) * p.G + g;
+  if constexpr (MODE == OWN) {
+    const int64_t own = (int64_t)it.kvh * p.pre_tiles * p.pre_rows + row;
+    *reinterpret_cast<f32x4_t*>(p.own_o + own * D + dd) = a.o;
+    if (dd == 0) {
+      p.own_ml[own * 2] = a.m;
+      p.own_ml[own * 2 + 1] = a.l;
+    }
+    return true;
+  }
+  const int rt = row / p.pre_rows, r = row - rt * p.pre_rows;
   const int64_t at = prefix_slot(p, it.kvh, rt, MODE == PREFIX ? it.split : 0) * p.pre_rows + r;
   float* o = p.pre_o + at * D + dd;
   float* ml = p.pre_ml + at * 2;
@@ -481,7 +498,7 @@ __device__ void join_parts(const KArgs& p, const Item& it, int nr, float* room) 
   auto store = [&](int i, Joined a) {
     const int r = i / (D / 4), dd = (i % (D / 4)) * 4;
     const int row = it.rt * BQ + r, t = over(row, p.by_g), g = row - t * p.G;
-    shared_part<D, MODE>(p, it, it.q.s0 + t, g, dd, a);
+    if (shared_part<D, MODE>(p, it, it.q.s0 + t, g, dd, a)) return;
     const int64_t at =
         (int64_t)(it.q.s0 + t) * p.st_o + (int64_t)(it.kvh * p.G + g) * p.sh_o + dd;
     const f32x4_t x = a.l == 0.f ? f32x4_t{0.f, 0.f, 0.f, 0.f} : a.o / a.l;
@@ -622,17 +639,15 @@ __device__ inline bool shared_row(const KArgs& p, const Item& it, int token, int
 // are busy 46 % of the time and the vector units 43 %, hardly ever both.  With 64 rows a wave
 // (1.2 ms for 0.96 then), three stages, or 32-key tiles at three waves a SIMD it was slower.
 template <int D, int NST, int MODE>
-__global__ __launch_bounds__(256, 2) void paged_attn_kernel(KArgs p) {
+__device__ __forceinline__ void tiles_body(const KArgs& p, unsigned bid, uint16_t* lds, int* ptab) {
   constexpr int BKV = 64, QPW = 32, BQ = 4 * QPW;
   constexpr int TILE = BKV * D;        // elements of a K (or V) tile
   constexpr int STAGE = 2 * TILE;
   constexpr int NOP = 4 * (D / 64);    // DMA instructions of a wave per tile
   constexpr int KS = D / 16, DS = D / 32;
-  __shared__ __attribute__((aligned(1024))) uint16_t lds[NST * STAGE];
-  __shared__ int ptab[PT];
 
   Item it;
-  if (!find_item<BQ, BKV, MODE>(p, blockIdx.x, it)) return;
+  if (!find_item<BQ, BKV, MODE>(p, bid, it)) return;
   const Seq& sq = it.q;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -913,6 +928,12 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(KArgs p) {
       }
   }
 }
+template <int D, int NST, int MODE>
+__global__ __launch_bounds__(256, 2) void paged_attn_kernel(KArgs p) {
+  __shared__ __attribute__((aligned(1024))) uint16_t lds[NST * 2 * 64 * D];
+  __shared__ int ptab[PT];
+  tiles_body<D, NST, MODE>(p, blockIdx.x, lds, ptab);
+}
 
 // ---- bf16, few rows ----------------------------------------------------------------
 // Up to 16 NR rows (single tokens, short chunks): bound by reading K and V once, so the
@@ -934,19 +955,20 @@ template <int N>
 __device__ inline void wait_loads() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
+constexpr int PTF = 1024;
+constexpr int few_ring(int D, int NW) { return NW * 2 * 2 * 32 * D; }  // elements
+// lds: few_ring elements; sm, sl: a value of each wave and row; ptab: PTF entries
 template <int D, int NR, int NW, int MODE>
-__global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(KArgs p) {
+__device__ __forceinline__ void few_body(const KArgs& p, unsigned bid, uint16_t* lds,
+                                         float (*sm)[16 * NR], float (*sl)[16 * NR], int* ptab) {
   constexpr int KT = 32, BKV = 64, BQ = 16 * NR, TILE = KT * D, NST = 2;
   constexpr int OPS = 4 * (D / 64);  // DMA instructions of a K (or V) tile
-  constexpr int KS = D / 32, DB = D / 16, OP = D + 4, PTF = 1024;
-  constexpr int RING = NW * NST * 2 * TILE;  // elements
-  static_assert(RING * 2 >= NW * BQ * OP * 4, "the waves' outputs fit the rings");
-  __shared__ __attribute__((aligned(1024))) uint16_t lds[RING];
-  __shared__ float sm[NW][BQ], sl[NW][BQ];
-  __shared__ int ptab[PTF];
+  constexpr int KS = D / 32, DB = D / 16, OP = D + 4;
+  static_assert(few_ring(D, NW) == NW * NST * 2 * TILE, "the rings");
+  static_assert(few_ring(D, NW) * 2 >= NW * BQ * OP * 4, "the waves' outputs fit the rings");
 
   Item it;
-  if (!find_item<BQ, BKV, MODE>(p, blockIdx.x, it)) return;
+  if (!find_item<BQ, BKV, MODE>(p, bid, it)) return;
   const Seq& sq = it.q;
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -1262,6 +1284,86 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(KArgs p) {
     }
   }
   if (MODE != PREFIX && it.ns > 1) join_parts<D, BQ, 64 * NW, uint16_t, MODE>(p, it, nr, so);
+}
+template <int D, int NR, int NW, int MODE>
+__global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(KArgs p) {
+  __shared__ __attribute__((aligned(1024))) uint16_t lds[few_ring(D, NW)];
+  __shared__ float sm[NW][16 * NR], sl[NW][16 * NR];
+  __shared__ int ptab[PTF];
+  few_body<D, NR, NW, MODE>(p, blockIdx.x, lds, sm, sl, ptab);
+}
+
+// ---- bf16, a prefix and few rows of each sequence --------------------------------------
+// PREFIX and what the sequences have of their own in one launch, side by side, since neither fills
+// the chip for long; the first `first` blocks (a multiple of 8) are PREFIX's, of the others only two waves
+// stay.  With the join, against PREFIX and TAILS behind each other: 48 single tokens over 8192 shared
+// and up to 200 own keys, 12 heads, 25.0 and 28.5 us (PREFIX alone 13.4, 25 MB of keys and values:
+// dependent steps); 16 drafts of up to 6 over 30001 and up to 900, 32 / 8 heads of 128, 73 and 81 (46 alone,
+// 123 MB: 2.6 TB/s, and 27 GFLOP), of up to 9 92 and 123; 64 single tokens over 4000 and
+// 300, 8 / 1 heads of 128, 20.6 and 32.4, where without a prefix they take 22.2.
+template <int D, int NR>
+__global__ __launch_bounds__(256, 2) void paged_attn_both_kernel(KArgs pre, KArgs own,
+                                                                 unsigned first) {
+  static_assert(few_ring(D, 2) <= 2 * 2 * 64 * D && PTF >= PT, "one serves both");
+  __shared__ __attribute__((aligned(1024))) uint16_t lds[2 * 2 * 64 * D];
+  __shared__ float sm[2][16 * NR], sl[2][16 * NR];
+  __shared__ int ptab[PTF];
+  if (blockIdx.x < first) {
+    tiles_body<D, 2, PREFIX>(pre, blockIdx.x, lds, ptab);
+  } else {
+    if (threadIdx.x >= 128) return;  // (a barrier waits for the waves that are left)
+    few_body<D, NR, 2, OWN>(own, blockIdx.x - first, lds, sm, sl, ptab);
+  }
+}
+// Their parts joined: a block has 64 / (D / 4) rows of a key head, four columns a lane, each of
+// its waves a quarter of the prefix' parts.
+template <int D>
+__global__ __launch_bounds__(256) void paged_attn_join_kernel(KArgs p) {
+  constexpr int C = D / 4, RW = 64 / C;
+  __shared__ float sm[4][64], sl[4][64];
+  __shared__ f32x4_t so[4][64];
+  const int lane = threadIdx.x & 63, kvh = (int)blockIdx.y;
+  const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int row0 = (int)blockIdx.x * RW, row = row0 + lane / C, dd = lane % C * 4;
+  const int a0 = p.starts[0], from = p.taken[0], ns = from ? prefix_parts(p, from) : 0;
+  Joined a{-INFINITY, 0.f, f32x4_t{0.f, 0.f, 0.f, 0.f}};
+  if (w == 0) {
+    const int64_t own = (int64_t)kvh * p.pre_tiles * p.pre_rows + row;
+    a.m = p.own_ml[own * 2];
+    a.l = p.own_ml[own * 2 + 1];
+    a.o = *reinterpret_cast<const f32x4_t*>(p.own_o + own * D + dd);
+  }
+  const int rt = row / p.pre_rows, per = (ns + 3) >> 2;
+  const int64_t at = prefix_slot(p, kvh, rt, 0) * p.pre_rows + row - rt * p.pre_rows;
+  add_parts<D, 8>(p, p.pre_ml + at * 2, p.pre_o + at * D + dd, min(w * per, ns), min((w + 1) * per, ns),
+                  a);
+  sm[w][lane] = a.m;
+  sl[w][lane] = a.l;
+  so[w][lane] = a.o;
+  __syncthreads();
+  if (w) return;
+  // rows of a known sequence, nothing where the starts do not ascend within q (as find_item)
+  uint32_t known = 0;
+  bool crossed = false;
+  for (int b0 = 0; b0 < p.B; b0 += 64) {
+    const int b = b0 + lane;
+    const int s = b < p.B ? p.starts[b] : 0, e = b < p.B ? p.starts[b + 1] : 0;
+    const int slot = b >= p.B ? -1 : p.seqs ? p.seqs[b] : b;
+    crossed = crossed || s < 0 || e < s || e > p.total;
+#pragma unroll
+    for (int r = 0; r < RW; ++r) {
+      const int t = a0 + over(row0 + r, p.by_g);
+      if (__any(s <= t && t < e && slot >= 0 && slot < p.max_seqs)) known |= 1u << r;
+    }
+  }
+  if (__any(crossed) || !(known >> (lane / C) & 1)) return;
+#pragma unroll
+  for (int x = 1; x < 4; ++x) join(a, Joined{sm[x][lane], sl[x][lane], so[x][lane]}, p.c);
+  const int t = over(row, p.by_g), g = row - t * p.G;
+  uint16_t* dst = (uint16_t*)p.o + (int64_t)(a0 + t) * p.st_o + (int64_t)(kvh * p.G + g) * p.sh_o + dd;
+  const float inv = a.l == 0.f ? 0.f : 1.f / a.l;
+  *reinterpret_cast<u32x2_t*>(dst) =
+      u32x2_t{pack_bf16x2(a.o.x * inv, a.o.y * inv), pack_bf16x2(a.o.z * inv, a.o.w * inv)};
 }
 
 // ---- f32 -------------------------------------------------------------------------
@@ -1834,8 +1936,10 @@ static int64_t parts_bytes(const blt_paged_cache& c, int64_t B, int64_t total, i
   const Shape s = shape_of(c, B, total, H);
   return slots_of(c, s, B, total, H) * s.bq * (c.head_dim + 2) * 4;
 }
-// The prefix' row tiles (of all tokens as one sequence), and the parts it may be in: enough to fill the
-// chip, few enough that joining them takes no longer than their keys.
+// The prefix' row tiles (of all tokens as one sequence), and the parts it may be in: enough to give
+// every CU two blocks (with three the drafts above took 6 us more, those of up to 9), few enough that joining
+// them takes no longer than their keys (64 for 32: 14 single tokens over 16000 keys, 32 / 8
+// heads of 128, 34 us for 26; 24: 29).
 struct PrefixShape {
   Shape s;
   int64_t tiles;  // of a key head
@@ -1844,7 +1948,7 @@ struct PrefixShape {
 static PrefixShape prefix_shape(const blt_paged_cache& c, int64_t total, int H) {
   PrefixShape x{shape_of(c, 1, total, H), 0, 1};
   x.tiles = (total * (H / c.n_kv_heads) + x.s.bq - 1) / x.s.bq;
-  const int64_t fill = 768 / std::max<int64_t>(1, x.tiles * c.n_kv_heads);
+  const int64_t fill = 512 / std::max<int64_t>(1, x.tiles * c.n_kv_heads);
   x.parts = (int)std::max<int64_t>(1, std::min<int64_t>(32, fill));
   return x;
 }
@@ -1853,12 +1957,16 @@ int64_t paged_attention_workspace_bytes(const blt_paged_cache& c, int64_t B, int
   const int64_t own = parts_bytes(c, B, total, H);
   if (!prefix) return own;
   const PrefixShape x = prefix_shape(c, total, H);
-  return own + c.n_kv_heads * x.tiles * x.parts * x.s.bq * (c.head_dim + 2) * 4;
+  return own + 16 + c.n_kv_heads * x.tiles * (x.parts + 1) * x.s.bq * (c.head_dim + 2) * 4;
 }
 
-// One launch; with a prefix its own (mode PREFIX) and the sequences' (TAILS).
-static int launch_mode(const blt_paged_cache& c, const PagedAttnArgs& a, int mode, void* ws,
-                       hipStream_t s) {
+// One launch's arguments; with a prefix its own (mode PREFIX) and the sequences' (TAILS or OWN).
+struct Launch {
+  KArgs p;
+  Shape sh;
+  int64_t blocks;
+};
+static Launch launch_of(const blt_paged_cache& c, const PagedAttnArgs& a, int mode, void* ws) {
   const PrefixShape pre = mode == WHOLE ? PrefixShape{} : prefix_shape(c, a.total, a.H);
   Shape sh = mode == PREFIX ? pre.s : shape_of(c, a.B, a.total, a.H);
   const int d = c.head_dim;
@@ -1889,28 +1997,55 @@ static int launch_mode(const blt_paged_cache& c, const PagedAttnArgs& a, int mod
     p.pre_parts = pre.parts;
     p.pre_rows = pre.s.bq;
     p.pre_keys = pre.s.bkv;
-    const int64_t rows = c.n_kv_heads * pre.tiles * pre.parts * pre.s.bq;
-    p.pre_o = p.part;
-    p.pre_ml = p.pre_o + rows * d;
-    p.part = p.pre_ml + rows * 2;
+    const int64_t rows = c.n_kv_heads * pre.tiles * pre.s.bq;
+    p.taken = (int*)ws;
+    p.own_o = (float*)ws + 4;
+    p.own_ml = p.own_o + rows * d;
+    p.pre_o = p.own_ml + rows * 2;
+    p.pre_ml = p.pre_o + rows * pre.parts * d;
+    p.part = p.pre_ml + rows * pre.parts * 2;
   }
   p.ml = p.part + slots * sh.bq * d;
-  const int64_t nb = ((mode == PREFIX ? c.n_kv_heads * pre.tiles * pre.parts
-                                      : blocks_of(c, sh, a.B, a.total, a.H)) + 7) / 8 * 8;
-  if (nb > 0x7fffffff) return fail(BLT_ERR_SHAPE, "paged_attention: too many row tiles");
-  const unsigned n = (unsigned)nb;
-  switch (mode) {
-    case PREFIX: return d == 64 ? run_paged<64, PREFIX>(p, sh, n, s) : run_paged<128, PREFIX>(p, sh, n, s);
-    case TAILS: return d == 64 ? run_paged<64, TAILS>(p, sh, n, s) : run_paged<128, TAILS>(p, sh, n, s);
-    default: return d == 64 ? run_paged<64, WHOLE>(p, sh, n, s) : run_paged<128, WHOLE>(p, sh, n, s);
-  }
+  const int64_t nb = mode == PREFIX ? c.n_kv_heads * pre.tiles * pre.parts
+                                    : blocks_of(c, sh, a.B, a.total, a.H);
+  return Launch{p, sh, (nb + 7) / 8 * 8};
+}
+static int too_many() { return fail(BLT_ERR_SHAPE, "paged_attention: too many row tiles"); }
+template <int D, int MODE>
+static int launch_one(const Launch& x, hipStream_t s) {
+  return x.blocks > 0x7fffffff ? too_many() : run_paged<D, MODE>(x.p, x.sh, (unsigned)x.blocks, s);
+}
+template <int D>
+static int launch_both(const Launch& pre, const Launch& own, int64_t total, hipStream_t s) {
+  if (pre.blocks + own.blocks > 0x7fffffff) return too_many();
+  const unsigned first = (unsigned)pre.blocks;
+  const dim3 grid(first + (unsigned)own.blocks);
+  if (own.sh.form == FORM_FEW16)
+    hipLaunchKernelGGL((paged_attn_both_kernel<D, 1>), grid, dim3(256), 0, s, pre.p, own.p, first);
+  else
+    hipLaunchKernelGGL((paged_attn_both_kernel<D, 2>), grid, dim3(256), 0, s, pre.p, own.p, first);
+  constexpr int rows = 64 / (D / 4);
+  hipLaunchKernelGGL((paged_attn_join_kernel<D>),
+                     dim3((unsigned)((total * own.p.G + rows - 1) / rows), (unsigned)own.p.Hkv),
+                     dim3(256), 0, s, own.p);
+  BLT_LAUNCH_CHECK("paged_attn_both_kernel");
+  return 0;
 }
 
 int launch_paged_attention(const blt_paged_cache& c, const PagedAttnArgs& a, void* ws,
                            hipStream_t s) {
-  if (!a.prefix) return launch_mode(c, a, WHOLE, ws, s);
-  if (int rc = launch_mode(c, a, PREFIX, ws, s)) return rc;
-  return launch_mode(c, a, TAILS, ws, s);
+  const bool narrow = c.head_dim == 64;
+  if (!a.prefix) {
+    const Launch x = launch_of(c, a, WHOLE, ws);
+    return narrow ? launch_one<64, WHOLE>(x, s) : launch_one<128, WHOLE>(x, s);
+  }
+  Launch pre = launch_of(c, a, PREFIX, ws);
+  const Launch own = launch_of(c, a, TAILS, ws);
+  if (pre.sh.form == FORM_TILES && (own.sh.form == FORM_FEW16 || own.sh.form == FORM_FEW32))
+    return narrow ? launch_both<64>(pre, own, a.total, s) : launch_both<128>(pre, own, a.total, s);
+  pre.p.taken = nullptr;
+  if (int rc = narrow ? launch_one<64, PREFIX>(pre, s) : launch_one<128, PREFIX>(pre, s)) return rc;
+  return narrow ? launch_one<64, TAILS>(own, s) : launch_one<128, TAILS>(own, s);
 }
 
 }  // namespace blt

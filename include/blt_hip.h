@@ -363,7 +363,7 @@ int blt_cache_common_prefix(const blt_paged_cache* cache, const int32_t* seqs, i
                             int32_t* tokens, blt_stream_t stream);
 /* blt_paged_attention without a window for sequences that share their first prefix[0] tokens (int32
  * [1], device, from blt_cache_common_prefix of a list that holds these sequences): the shared
- * keys are read once for all rows, in a launch of their own.  What is no whole page, and what does not lie
+ * keys are read once for all rows (two launches).  What is no whole page, and what does not lie
  * before every row's new tokens, is not taken as shared, so any number is safe; but where the first
  * pages are not the same ones, rows see those of the first row that has tokens. */
 int64_t blt_paged_attention_prefix_workspace_bytes(const blt_paged_cache* cache, int64_t B,
