@@ -256,6 +256,89 @@ def test_bad_rows_are_reported():
         c.attention(0, q, i32([0, 1, 2, 3]), prefix=96)
 
 
+@pytest.mark.parametrize("d,H,Hkv,chunk", [(64, 4, 4, 1), (64, 8, 2, 6), (128, 4, 1, 2), (128, 8, 2, 7)])
+@pytest.mark.parametrize("B", [40, 90])
+def test_many_rows_in_one_launch_with_their_prefix(d, H, Hkv, chunk, B):
+    """Many short rows: any number as the prefix, rows without tokens, a sequence twice, unknown
+    ones, starts that do not ascend, first tokens and last ones that belong to nobody."""
+    rng = np.random.default_rng(B + d)
+    m = shared(300, rng.integers(8, 40, B).tolist(), Hkv=Hkv, d=d, page=16)
+    c = m.cache
+    n = rng.integers(0, chunk + 1, B).tolist()
+    n[3], n[5] = 0, chunk
+    # (18 pages are shared; every row has 19 and more behind it, so a number of 304 would be taken, and wrong)
+    for number in (0, -3, 5, 160, 288, 300):
+        check(m, n, H, prefix=i32([number]))
+    seqs = list(range(B))
+    seqs[7] = seqs[20] = 5
+    check(m, n, H, seqs=seqs)
+    # tokens in front of the first sequence, unknown sequences
+    starts = np.concatenate([[0], np.cumsum(n)]) + 9
+    q = torch.randn(int(starts[-1]) + 5, H, d, device=DEV).bfloat16()
+    want = c.attention(0, q, i32(starts), out=torch.full_like(q, 7.0))
+    assert bool((want[:9] == 7).all() and (want[-5:] == 7).all())
+    prefix = c.common_prefix()
+    got = c.attention(0, q, i32(starts), prefix=prefix, out=torch.full_like(q, 7.0))
+    # (both are off by their own rounding and the weights' at most)
+    assert bool(((got.float() - want.float()).abs() <= 2 ** -6 * want.float().abs().amax()).all())
+    assert bool((got[:9] == 7).all() and (got[-5:] == 7).all())
+    bad = list(range(B))
+    bad[5], bad[11] = -1, 5000
+    o = c.attention(0, q, i32(starts), seqs=i32(bad), prefix=prefix, out=torch.full_like(q, 7.0))
+    with pytest.raises(BltError, match="range"):
+        c.check()
+    lost = torch.zeros(len(q), dtype=torch.bool)
+    for b in (5, 11):
+        lost[starts[b]:starts[b + 1]] = True
+    lost = lost.to(DEV)
+    assert bool((o[lost] == 7).all()) and bool((o[~lost] == got[~lost]).all())
+    crossed = starts.copy()
+    crossed[B // 2] = crossed[-1] + 1
+    o = c.attention(0, q, i32(crossed), prefix=prefix, out=torch.full_like(q, 7.0))
+    with pytest.raises(BltError, match="range"):
+        c.check()
+    assert bool((o == 7).all())
+
+
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+def test_not_finite_in_one_launch_with_their_prefix(value):
+    m = shared(320, [8] * 50, Hkv=1, d=64, page=16)
+    m.kv[1][0, m.table[9, 20], 0, 7, 7] = value  # a sequence's last token
+    q = torch.randn(50, 2, 64, device=DEV).bfloat16()
+    run = lambda: m.cache.attention(0, q, i32(range(51)), prefix=m.cache.common_prefix())
+    o = run()
+    assert not bool(torch.isfinite(o[9, :, 7]).any())
+    o[9, :, 7] = 0
+    assert bool(torch.isfinite(o).all())
+    m.kv[1][0, m.table[0, 3], 0, 5, 9] = value  # of the prefix
+    got = run()[:, :, 9]
+    assert bool(torch.isnan(got).all() if math.isnan(value) else (got == value).all())
+
+
+def test_one_launch_in_a_graph_and_on_another_stream():
+    m = shared(3000, [60] * 50, Hkv=2, d=64, page=16)
+    c, s = m.cache, i32(range(51))
+    q = torch.randn(50, 8, 64, device=DEV).bfloat16()
+    run = lambda: c.attention(0, q, s, prefix=c.common_prefix())
+    want = run()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = run()
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(want, other)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = run()
+    for n in range(4):
+        q.normal_()
+        c.lens[:4].copy_(i32([3000 + 7 * n, 3060, 3001, 2500 - 400 * n]))
+        fresh = run()
+        torch.cuda.synchronize()
+        graph.replay()
+        assert torch.equal(held, fresh)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_same_bits_and_in_a_graph(dtype):
     """Captured with its common_prefix; lengths and pages change between the replays."""
