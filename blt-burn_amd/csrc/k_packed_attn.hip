@@ -266,6 +266,11 @@ __device__ inline Bounds bounds_of(int klo, int khi, bool in) {
 // registers; V's operand is read with the LDS transposing read.  p is rounded to bf16 for the second
 // product, and without LSE the sum takes the rounded values, so that the weights of a row
 // add up to one; with it the sum is of p itself, which a gradient's weights go by.
+// d = 64: bound by the vector units (an exponential, and 2.5 more instructions, for each score
+// take longer than its 256 FLOP): 12 sequences of up to 8192, 12 heads, 403 us, 0.77 PFLOP/s, vector units
+// 65 % and matrix cores 39 % busy, rarely both.  d = 128: two sequences of 16384 and 11603, 32 / 8
+// heads, 3.07 ms, 1.08 PFLOP/s (the library's 8192^3 product: 1.21), 49 % and 55 %.  Short ones: 156 tokens of
+// 12 heads 7.2 us, a launch and three tiles' dependent steps.
 template <int D, bool LSE>
 __global__ __launch_bounds__(256, 2) void packed_attn_kernel(PArgs p) {
   constexpr int BKV = 64, QPW = 32, BQ = 4 * QPW;
@@ -484,6 +489,8 @@ __global__ __launch_bounds__(256, 2) void packed_attn_kernel(PArgs p) {
 // ---- f32 -----------------------------------------------------------------------------
 // Both products on the f32 matrix cores, one block = 32 rows, its four waves take every
 // fourth 32-key tile with operands straight from global memory, and meet once at the end.
+// Bound by the loads in front of the products, with two waves a SIMD to cover them: five sequences of up to
+// 1501, 12 heads of 64, 142 us, 79 TFLOP/s (an f32 library product: 136), matrix cores 53 % busy.
 template <int ND>
 __global__ __launch_bounds__(256) void packed_attn_f32_kernel(PArgs p) {
   constexpr int D = 32 * ND, NW = 4, NC = 4 * ND, OP = D + 4, BKV = 32;
@@ -732,6 +739,9 @@ __device__ inline bool rows_of(const PArgs& p, int key, int& rlo, int& rhi) {
 // adds up to 0 over a row but for what D is off by, with o rounded to bf16, that sum corrects D for the
 // other kernel.  So both gradients are 2.3e-3 off or less (relative, rms; their own rounding is
 // 1.7e-3), and not 2.5e-3 or, in short sequences, 3e-3.
+// Four sequences of up to 4096 (9 k tokens), 32 / 8 heads of 128: 435 us, four products (dS twice) at
+// 1.1 PFLOP/s, matrix cores 54 % and vector units 48 % busy; eleven of up to 2047, window 512, 12 heads of
+// 64: 52 us, 24 % and 47 %: ten key tiles behind each other in 1.5 rounds of blocks.
 template <int D>
 __global__ __launch_bounds__(256, 2) void packed_dq_kernel(GArgs ga) {
   const PArgs& p = ga.a;
@@ -923,10 +933,15 @@ __device__ inline int64_t part_at(const PArgs& p, int slice, int kvh, int what, 
   return (((int64_t)slice * (p.H / p.G) + kvh) * 2 + what) * p.total + key;
 }
 
-// dk and dv, bf16.  One block = 4 x 2 waves: 32 keys each, and one half of the rows of a tile
+// dk and dv, bf16.  One block = KW x RW waves: 32 keys each, and one RW-th of the rows of a tile
 // each; tiles of BR rows, Q beside dO, pass through LDS.  S = Q . K^T and dP = dO . V^T put a key into
 // a lane and rows into registers, from which P and dS feed dV^T = dO^T . P and dK^T = Q^T . dS.
-// The two halves are added up at the end.
+// The shares are added up at the end; with SLICED a block takes every gridDim.y-th row tile and leaves its sums
+// to packed_join_kernel (a kernel of its own: the few registers more would be spilled, beside DMA in
+// flight, by all calls).  For d = 128, K and the two sums fill the registers and V is read from LDS.
+// Same calls as dq's above: 515 us, four products at 0.94 PFLOP/s, matrix cores 43 % busy, the rest waits
+// for LDS operands (16 reads of 16 bytes for 16 products of 32 cycles) and the exponentials between them;
+// and 53 us, 22 %.
 template <int D, int KW, int RW, int BR, bool SLICED>
 __global__ __launch_bounds__(64 * KW * RW, D == 64 ? 3 : 2) void packed_dkdv_kernel(GArgs ga) {
   const PArgs& p = ga.a;
@@ -1201,7 +1216,10 @@ __global__ __launch_bounds__(64 * KW * RW, D == 64 ? 3 : 2) void packed_dkdv_ker
 }
 
 // f32, as packed_attn_f32_kernel: a block has 32 rows (dq) or 32 keys (dk, dv) in registers, its four
-// waves take every fourth tile of 32 of the others from global memory and add up at the end.
+// waves (dk and dv with d = 64: eight, 491 us for 521 over eight sequences of 1000, 12 heads; dq took 332 for 263)
+// take every fourth tile of 32 of the others from global memory and add up at the end.  Bound by
+// those loads: 12 heads of 64, five sequences of up to 1501, dq 223 us, 76 TFLOP/s, dk and dv 422, 54;
+// 12 / 4 heads, 1000 + 780 + 439 tokens, 70 and 149.
 // Sum of the waves' [D][32] results, scaled, into rows out(i).
 template <int ND, int NW, typename F>
 __device__ inline void add_waves(float* so, const f32x16_t (&acc)[ND], float scale, F out) {

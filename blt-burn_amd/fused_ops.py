@@ -366,7 +366,7 @@ def fused_packed_attention_backward(grad_o, q, k, v, o, lse, starts, causal=True
                                     scale=None):
     """(dq, dk, dv) of fused_packed_attention from its output's gradient, its o and lse, and its
     other arguments; tokens at starts[-1] and behind get 0.  Sums are f32, in bf16 the weights and
-    their gradients are rounded to bf16; the same bits in every run."""
+    (as two halves for dq) their gradients are rounded to bf16; the same bits in every run."""
     q, qp, qs, qh = _packed_heads(q, "q")
     total, H, d = q.shape
     k, kp, ks, kh = _packed_heads(k, "k", q)

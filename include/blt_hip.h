@@ -179,8 +179,9 @@ int blt_packed_attention(const void* q, int64_t st_q, int64_t sh_q, const void* 
 /* Gradients of blt_packed_attention's q, k and v from that of its output, with its o and lse;
  * the other arguments as there, a head stride of q and grad_o times Hq / Hkv at most 2^29.  dq
  * [total, Hq, d], dk and dv [total, Hkv, d] are written whole: 0 at starts[B] and behind.
- * Sums in f32, the weights and their gradients rounded to bf16 in bf16; the same bits
- * in every run.  workspace: blt_packed_attention_backward_workspace_bytes, 16-byte aligned, no
+ * Sums in f32; in bf16 the weights and (as two halves for dq) their gradients are rounded to bf16;
+ * the same bits in every run.  Weights are e^(score - lse): with scores of 2^k and more, lse's own
+ * 24 bits leave them 2^(k - 24) off.  workspace: blt_packed_attention_backward_workspace_bytes, 16-byte aligned, no
  * initialisation; calls that share one must be stream-ordered. */
 int64_t blt_packed_attention_backward_workspace_bytes(int64_t total, int64_t Hq, int64_t Hkv,
                                                       int32_t d, int32_t dtype);
