@@ -1216,12 +1216,11 @@ __global__ __launch_bounds__(64 * KW * RW, D == 64 ? 3 : 2) void packed_dkdv_ker
 }
 
 // f32, as packed_attn_f32_kernel: a block has 32 rows (dq) or 32 keys (dk, dv) in registers, its four
-// waves (dk and dv with d = 64: eight, 491 us for 521 over eight sequences of 1000, 12 heads; dq took 332 for 263)
-// take every fourth tile of 32 of the others from global memory and add up at the end.  Bound by
-// those loads: 12 heads of 64, five sequences of up to 1501, dq 223 us, 76 TFLOP/s, dk and dv 422, 54;
-// 12 / 4 heads, 1000 + 780 + 439 tokens, 70 and 149.
+// waves take every fourth tile of 32 of the others from global memory and add up at the end.  Bound by
+// those loads: 12 heads of 64, five sequences of up to 1501, dq 223 us, 76 TFLOP/s, dk and dv 370, 61 (one
+// wave a SIMD 440, blocks of eight waves 422); 12 / 4 heads, 1000 + 780 + 439 tokens, 70 and 139.
 // Sum of the waves' [D][32] results, scaled, into rows out(i).
-template <int ND, int NW, typename F>
+template <int ND, typename F>
 __device__ inline void add_waves(float* so, const f32x16_t (&acc)[ND], float scale, F out) {
   constexpr int D = 32 * ND, OP = D + 4, VW = ND % 4 == 0 ? 4 : 2, NV = ND / VW;
   typedef float vf_t __attribute__((ext_vector_type(VW)));
@@ -1238,17 +1237,15 @@ __device__ inline void add_waves(float* so, const f32x16_t (&acc)[ND], float sca
       *reinterpret_cast<vf_t*>(row + VW * (8 * (i >> 2) + 4 * h + (i & 3)) + 32 * VW * n) = x;
     }
   __syncthreads();
-  for (int i = tid; i < 32 * (D / 4); i += 64 * NW) {
+  for (int i = tid; i < 32 * (D / 4); i += 256) {
     const int rr = i / (D / 4), cc = (i % (D / 4)) * 4;
     float* to = out(rr);
     if (!to) continue;
-    f32x4_t x[NW];
+    f32x4_t x[4];
 #pragma unroll
-    for (int k = 0; k < NW; ++k)
+    for (int k = 0; k < 4; ++k)
       x[k] = *reinterpret_cast<const f32x4_t*>(so + (k * 32 + rr) * OP + cc);
-    f32x4_t sum = (x[0] + x[1]) + (x[2] + x[3]);
-    if constexpr (NW == 8) sum += (x[4] + x[5]) + (x[6] + x[7]);
-    *reinterpret_cast<f32x4_t*>(to + cc) = sum * scale;
+    *reinterpret_cast<f32x4_t*>(to + cc) = ((x[0] + x[1]) + (x[2] + x[3])) * scale;
   }
 }
 
@@ -1373,17 +1370,18 @@ __global__ __launch_bounds__(256) void packed_dq_f32_kernel(GArgs ga) {
       }
     }
   }
-  add_waves<ND, NW>(so, acc, p.scale, [&](int rr) -> float* {
+  add_waves<ND>(so, acc, p.scale, [&](int rr) -> float* {
     if (r0 + rr >= p.rows) return nullptr;
     const int t = over(r0 + rr, p.by_g), g = r0 + rr - t * p.G;
     return (float*)ga.dq + (int64_t)t * ga.st_dq + (int64_t)(kvh * p.G + g) * ga.sh_dq;
   });
 }
 
-template <int ND, int NW>
-__global__ __launch_bounds__(64 * NW) void packed_dkdv_f32_kernel(GArgs ga) {
+// (d = 64: 256 registers, so that a SIMD has two waves; the compiler takes two more unasked)
+template <int ND>
+__global__ __launch_bounds__(256, ND == 2 ? 2 : 1) void packed_dkdv_f32_kernel(GArgs ga) {
   const PArgs& p = ga.a;
-  constexpr int D = 32 * ND, NC = 4 * ND, OP = D + 4, BR = 32;
+  constexpr int D = 32 * ND, NW = 4, NC = 4 * ND, OP = D + 4, BR = 32;
   constexpr int VW = ND % 4 == 0 ? 4 : 2, NV = ND / VW;
   typedef float vf_t __attribute__((ext_vector_type(VW)));
   __shared__ __attribute__((aligned(16))) float so[NW * 32 * OP];
@@ -1501,15 +1499,15 @@ __global__ __launch_bounds__(64 * NW) void packed_dkdv_f32_kernel(GArgs ga) {
     auto part = [&](int what, int i) {
       return j0 + i < p.total ? ga.part + part_at(p, slice, kvh, what, j0 + i) * D : nullptr;
     };
-    add_waves<ND, NW>(so, dk, 1.f, [&](int i) { return part(0, i); });
-    add_waves<ND, NW>(so, dv, 1.f, [&](int i) { return part(1, i); });
+    add_waves<ND>(so, dk, 1.f, [&](int i) { return part(0, i); });
+    add_waves<ND>(so, dv, 1.f, [&](int i) { return part(1, i); });
     return;
   }
   auto out = [&](void* x, int64_t st, int64_t sh, int i) -> float* {
     return j0 + i < p.total ? (float*)x + (int64_t)(j0 + i) * st + (int64_t)kvh * sh : nullptr;
   };
-  add_waves<ND, NW>(so, dk, p.scale, [&](int i) { return out(ga.dk, ga.st_dk, ga.sh_dk, i); });
-  add_waves<ND, NW>(so, dv, 1.f, [&](int i) { return out(ga.dv, ga.st_dv, ga.sh_dv, i); });
+  add_waves<ND>(so, dk, p.scale, [&](int i) { return out(ga.dk, ga.st_dk, ga.sh_dk, i); });
+  add_waves<ND>(so, dv, 1.f, [&](int i) { return out(ga.dv, ga.st_dv, ga.sh_dv, i); });
 }
 
 // dk and dv from the parts of their tiles' blocks, in the blocks' order: a thread 4 values of one
@@ -1609,9 +1607,9 @@ int launch_packed_attention(const PackedAttnArgs& a, void* ws, hipStream_t s) {
 // keep the device even, at most 8 (`seen`: about how many rows a key has, 0 for unknown: a block
 // gets 256 of them or more).  Their parts cost a join of 4 to 10 us.  dk and dv, sliced with the join
 // and in one block:
-//   f32   12 / 4 heads of 64: 1000 + 77 + 439 tokens 119 and 191 us, 1000 + 780 + 439 147 and 195,
-//         4 x 1000 284 and 313; 8 / 1 heads of 128: 2 x 2000 822 and 1880; but with 1.5 times
-//         the blocks 12 / 12 of 64, 2 x 1000, 153 and 130
+//   f32   12 / 4 heads of 64: 1000 + 77 + 439 tokens 110 and 191 us, 1000 + 780 + 439 139 and 195;
+//         8 / 1 heads of 128: 2 x 2000 827 and 1880; but with more blocks 12 / 12 of 64, 2 x 1000,
+//         133 and 124
 //   bf16  12 / 4 heads of 64: the first of these 33 and 87, 8 x 1000 78 and 120; 12 heads: 1 x
 //         4096 99 and 131; 8 / 1 heads of 128: 2 x 2000 89 and 268; 32 / 8 of 128: 1 x 2048 106 and
 //         133, but 4 x 500 68 and 52 (so fewer where keys have few rows), 4 x 100 31 and 20
@@ -1666,10 +1664,10 @@ int launch_packed_attention_backward(const PackedAttnArgs& a, const PackedGradAr
   const dim3 gq((unsigned)nq), gk((unsigned)nk, slices), block(256);
   if (f32 && a.d == 64) {
     hipLaunchKernelGGL((packed_dq_f32_kernel<2>), gq, block, 0, s, p);
-    hipLaunchKernelGGL((packed_dkdv_f32_kernel<2, 8>), gk, dim3(512), 0, s, pk);
+    hipLaunchKernelGGL((packed_dkdv_f32_kernel<2>), gk, block, 0, s, pk);
   } else if (f32) {
     hipLaunchKernelGGL((packed_dq_f32_kernel<4>), gq, block, 0, s, p);
-    hipLaunchKernelGGL((packed_dkdv_f32_kernel<4, 4>), gk, block, 0, s, pk);
+    hipLaunchKernelGGL((packed_dkdv_f32_kernel<4>), gk, block, 0, s, pk);
   } else if (a.d == 64) {
     hipLaunchKernelGGL((packed_dq_kernel<64>), gq, block, 0, s, p);
     if (slices > 1)
