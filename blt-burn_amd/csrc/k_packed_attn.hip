@@ -1643,8 +1643,12 @@ int launch_packed_attention_backward(const PackedAttnArgs& a, const PackedGradAr
   p.stat_tiles = (p.a.rows + 63) / 64;
   const bool f32 = a.dtype == BLT_DTYPE_F32;
   const int bk = key_tile(a.total, a.Hkv, a.d, f32), bq = f32 ? 32 : 128;
+  const int64_t mean = a.total / std::max<int64_t>(a.B, 1);
+  const int64_t seen = std::max<int64_t>(p.a.window ? std::min<int64_t>(mean, p.a.window + bk) : mean,
+                                         1) * p.a.G;
+  const int slices = key_slices(a.total, a.Hkv, a.d, f32, seen);
   int* orders = (int*)(p.stats + (int64_t)a.Hkv * p.stat_tiles * 128);
-  const bool by_rows = ordered(a.B, p.a.rows, bq, a.Hkv), by_keys = ordered(a.B, a.total, bk, a.Hkv);
+  const bool by_rows = ordered(a.B, p.a.rows, bq, a.Hkv), by_keys = ordered(a.B, a.total, bk, a.Hkv * slices);
   if (by_rows || by_keys) {
     hipLaunchKernelGGL(packed_order_kernel, dim3(2), dim3(1024), 0, s, p.a, bq, bk,
                        by_rows ? orders : nullptr, by_keys ? orders + kOrderTiles : nullptr);
@@ -1656,10 +1660,6 @@ int launch_packed_attention_backward(const PackedAttnArgs& a, const PackedGradAr
   if (by_keys) pk.a.order = orders + kOrderTiles;
   if (nq > 0x7fffffff || nk > 0x7fffffff)
     return fail(BLT_ERR_SHAPE, "packed_attention_backward: too many tiles");
-  const int64_t mean = a.total / std::max<int64_t>(a.B, 1);
-  const int64_t seen = std::max<int64_t>(p.a.window ? std::min<int64_t>(mean, p.a.window + bk) : mean,
-                                         1) * p.a.G;
-  const int slices = key_slices(a.total, a.Hkv, a.d, f32, seen);
   pk.part = (float*)((char*)ws + stats_bytes(a.total, a.H, a.Hkv));
   const dim3 gq((unsigned)nq), gk((unsigned)nk, slices), block(256);
   if (f32 && a.d == 64) {
