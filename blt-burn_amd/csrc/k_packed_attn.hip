@@ -366,15 +366,24 @@ __global__ __launch_bounds__(256, 2) void packed_attn_kernel(PArgs p) {
         for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
           for (int u = 0; u < 2; ++u) vf[ds][sub][u] = tr.read(sv, sub * 32 + u * 16, ds);
-      if (mask_hi || mask_lo) {
-        const int up = khi - kb - 4 * lhalf, dn = klo - kb - 4 * lhalf;
+      // (d = 64: one side at a time, since hardly a tile needs both: eleven sequences of up to 2047,
+      // window 512, 12 heads, 38.7 us for 41.2; d = 128: 201 for 195)
+      const int up = khi - kb - 4 * lhalf, dn = klo - kb - 4 * lhalf;
+      if (D == 64 ? mask_hi : mask_hi || mask_lo) {
 #pragma unroll
         for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int key = sub * 32 + 8 * (r >> 2) + (r & 3);
-            s[sub][r] = key <= up && key >= dn ? s[sub][r] : -INFINITY;
+            s[sub][r] = key <= up && (D == 64 || key >= dn) ? s[sub][r] : -INFINITY;
           }
+      }
+      if (D == 64 && mask_lo) {
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            s[sub][r] = sub * 32 + 8 * (r >> 2) + (r & 3) >= dn ? s[sub][r] : -INFINITY;
       }
       float mt = -INFINITY;
 #pragma unroll
@@ -741,7 +750,8 @@ __device__ inline bool rows_of(const PArgs& p, int key, int& rlo, int& rhi) {
 // 1.7e-3), and not 2.5e-3 or, in short sequences, 3e-3.
 // Four sequences of up to 4096 (9 k tokens), 32 / 8 heads of 128: 435 us, four products (dS twice) at
 // 1.1 PFLOP/s, matrix cores 54 % and vector units 48 % busy; eleven of up to 2047, window 512, 12 heads of
-// 64: 52 us, 24 % and 47 %: ten key tiles behind each other in 1.5 rounds of blocks.
+// 64: 48 us, ten key tiles behind each other in 1.5 rounds of blocks (52 with 64 keys at a time, whether
+// seen or not, and both sides of the mask in one).
 template <int D>
 __global__ __launch_bounds__(256, 2) void packed_dq_kernel(GArgs ga) {
   const PArgs& p = ga.a;
@@ -824,9 +834,11 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(GArgs ga) {
     if (kb <= bd.whi && kb + BKV > bd.wlo) {
       const uint16_t* sk = lds + stage * STAGE;
       const uint16_t* sv = sk + TILE;
-      const bool mask = kb + BKV - 1 > bd.hi_min || kb < bd.lo_max;
 #pragma unroll 1
       for (int sub = 0; sub < 2; ++sub) {
+        const int k0 = kb + sub * 32;
+        if (k0 > bd.whi || k0 + 32 <= bd.wlo) continue;
+        const bool mask_hi = k0 + 31 > bd.hi_min, mask_lo = k0 < bd.lo_max;
         f32x16_t s, dp;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
@@ -845,7 +857,7 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(GArgs ga) {
         // A weight of zero does not silence a key that is not finite (as in packed_attn_kernel),
         // which shows in every row's score of it; where it is seen the result is NaN.
         bool odd = false;
-        if (mask) {
+        if (mask_hi || mask_lo) {
           float sum = 0.f;
 #pragma unroll
           for (int r = 0; r < 16; ++r) sum = fmaf(s[r], 0.f, sum);
@@ -854,12 +866,15 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(GArgs ga) {
         float e[16];
 #pragma unroll
         for (int r = 0; r < 16; ++r) e[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, mc)) * (dp[r] - delta);
-        if (mask) {
-          const int up = khi - kb - sub * 32 - 4 * lhalf, dn = klo - kb - sub * 32 - 4 * lhalf;
+        if (mask_hi || mask_lo) {
+          const int up = khi - k0 - 4 * lhalf, dn = klo - k0 - 4 * lhalf;
+          if (mask_hi) {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int key = 8 * (r >> 2) + (r & 3);
-            e[r] = key <= up && key >= dn ? e[r] : 0.f;
+            for (int r = 0; r < 16; ++r) e[r] = 8 * (r >> 2) + (r & 3) <= up ? e[r] : 0.f;
+          }
+          if (mask_lo) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) e[r] = 8 * (r >> 2) + (r & 3) >= dn ? e[r] : 0.f;
           }
           if (odd) {
 #pragma unroll
@@ -1035,7 +1050,7 @@ __global__ __launch_bounds__(64 * KW * RW, D == 64 ? 3 : 2) void packed_dkdv_ker
     odd = false;
     if (rb > bd.whi || rb + 32 <= bd.wlo) return false;
     const float* st = reinterpret_cast<const float*>(sg + TILE) + (r0 >> 6) * 128 + (r0 & 63);
-    const bool mask = rb + 31 > bd.hi_min || rb < bd.lo_max;
+    const bool mask_hi = rb + 31 > bd.hi_min, mask_lo = rb < bd.lo_max, mask = mask_hi || mask_lo;
     f32x16_t s, dp;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {  // (dP starts from -D)
@@ -1075,12 +1090,21 @@ __global__ __launch_bounds__(64 * KW * RW, D == 64 ? 3 : 2) void packed_dkdv_ker
     }
     if (mask) {
       const int up = rhi - rb - 4 * lhalf, dn = rlo - rb - 4 * lhalf;
+      if (mask_hi) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int at = 8 * (r >> 2) + (r & 3);
-        const bool sees = at <= up && at >= dn;
-        w[r] = sees ? w[r] : 0.f;
-        e[r] = sees ? e[r] : 0.f;
+        for (int r = 0; r < 16; ++r) {
+          const bool sees = 8 * (r >> 2) + (r & 3) <= up;
+          w[r] = sees ? w[r] : 0.f;
+          e[r] = sees ? e[r] : 0.f;
+        }
+      }
+      if (mask_lo) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const bool sees = 8 * (r >> 2) + (r & 3) >= dn;
+          w[r] = sees ? w[r] : 0.f;
+          e[r] = sees ? e[r] : 0.f;
+        }
       }
       if (odd) {
         for (int j = r0; j < r0 + 32; ++j) {
