@@ -700,11 +700,11 @@ __global__ __launch_bounds__(NT) void sample_block_kernel(SArgs g) {
 //   with top_k     all tokens down to the bin in which it ends: they decide everything
 //   with top_p     those of the bin in which it ends; what lies above is kept
 // Where that are more than a block ranks at once, the cut is found by passes over the row.
-// 64 rows of 131072 f32 logits with top_k and top_p, 33.5 MB, which the last-level cache holds after the first
+// 64 rows of 131072 f32 logits with top_p, 33.5 MB, which the last-level cache holds after the first
 // launch: 60 us, of which top 4.5 (7.4 TB/s), bins 17 (vector units 52 % busy with weights in 64 bits and
 // LDS atomics), find 7, lists and kept weights 11, pick 19 (64 blocks, chains of scans; a launch's
 // start is in each).  Three reads of the row and five launches take 34 us at those rates; one launch
-// a row (the form above, in passes) 123.
+// a row (the form above, in passes) 123.  With top_k 50 as well 56, its bins without weights (69 with).
 enum Way { ALL, TOP, BIN, CUT };  // (no rule but min_p; lists; a cut that is known)
 struct Found {
   int way, bin;
@@ -763,13 +763,14 @@ __global__ __launch_bounds__(NT) void sample_bins_kernel(SArgs g) {
   __syncthreads();
   x.each([&](float v, int i, int) {
     if (i >= 0)
-      add_to_bin(s, bin_of(v, top, r), r.p < 1. ? weight(v, top, r, g.scale, s.pw) : 0, r.k > 0);
+      add_to_bin(s, bin_of(v, top, r), r.k ? 0 : weight(v, top, r, g.scale, s.pw), r.k > 0);
   });
   __syncthreads();
   const int64_t at = (row * g.parts + part) * NB;
   for (int i = threadIdx.x; i < NB; i += NT) {
-    if (r.p < 1.) g.hm[at + i] = s.m[i];
+    // (where top_k ends goes by counts; the weights of its tokens are taken from the list)
     if (r.k) g.hc[at + i] = s.c[i];
+    else g.hm[at + i] = s.m[i];
   }
 }
 template <typename T>
@@ -786,13 +787,12 @@ __global__ __launch_bounds__(NT) void sample_find_kernel(SArgs g) {
     uint32_t c[2] = {0, 0};
     for (int part = 0; part < g.parts; ++part) {
       const int64_t at = (row * g.parts + part) * NB + 2 * threadIdx.x;
-      if (r.p < 1.) {
-        m[0] += g.hm[at];
-        m[1] += g.hm[at + 1];
-      }
       if (r.k) {
         c[0] += g.hc[at];
         c[1] += g.hc[at + 1];
+      } else {
+        m[0] += g.hm[at];
+        m[1] += g.hm[at + 1];
       }
     }
 #pragma unroll
@@ -817,6 +817,12 @@ __global__ __launch_bounds__(NT) void sample_find_kernel(SArgs g) {
       const InMemory<T> x((const char*)g.x + row * g.st * (int64_t)sizeof(T), g.V);
       fill(s.pw);
       __syncthreads();
+      if (r.p < 1.) {  // (the bins have no weights yet)
+        x.each([&](float v, int i, int) {
+          if (i >= 0) add_to_bin(s, bin_of(v, top, r), weight(v, top, r, g.scale, s.pw), false);
+        });
+        __syncthreads();
+      }
       const Cut cut = find_cut(x, s, r, top, g.scale);
       f.key = cut.key;
       f.index = cut.index;
