@@ -704,7 +704,8 @@ __global__ __launch_bounds__(NT) void sample_block_kernel(SArgs g) {
 // launch: 60 us, of which top 4.5 (7.4 TB/s), bins 17 (vector units 52 % busy with weights in 64 bits and
 // LDS atomics), find 7, lists and kept weights 11, pick 19 (64 blocks, chains of scans; a launch's
 // start is in each).  Three reads of the row and five launches take 34 us at those rates; one launch
-// a row (the form above, in passes) 123.  With top_k 50 as well 56, its bins without weights (69 with).
+// a row (the form above, in passes) 123.  With top_k 50 as well 47: bins by
+// counts alone (with weights 9 more), lists from registers (in passes over memory 9 more).
 enum Way { ALL, TOP, BIN, CUT };  // (no rule but min_p; lists; a cut that is known)
 struct Found {
   int way, bin;
@@ -859,8 +860,8 @@ __global__ __launch_bounds__(NT) void sample_part_kernel(SArgs g) {
     const int at = atomicAdd(&listed, 1);
     if (at < NT) list[at] = Entry{v, part * PART + i, weight(v, top, r, g.scale, pw)};
   };
-  if (sums) {
-    const float from = (float)f.bin, end = from + 1.f;
+  if (sums || f.way == TOP) {
+    const float end = (float)f.bin + 1.f, from = f.way == TOP ? -INFINITY : (float)f.bin;
     uint32_t hits = 0;
     x.each([&](float v, int i, int j) {
       const float t = place_of(v, top, r);
@@ -876,14 +877,14 @@ __global__ __launch_bounds__(NT) void sample_part_kernel(SArgs g) {
                             x.n);
     again.each([&](float v, int i, int) {
       if (i < 0) return;
-      const int bin = f.way == CUT || f.way == ALL ? 0 : bin_of(v, top, r);
+      const int bin = f.way == BIN ? bin_of(v, top, r) : 0;
       const bool keep = f.way == ALL || (f.way == CUT && kept(cut, key_of(v), i)) ||
                         (f.way == BIN && bin < f.bin);
       if (keep) {
         const uint64_t w = weight(v, top, r, g.scale, pw);
         m += w >= r.m ? w : 0;
       }
-      if (f.way == TOP ? bin <= f.bin : f.way == BIN && bin == f.bin) enter(v, i);
+      if (f.way == BIN && bin == f.bin) enter(v, i);
     });
   }
   m = sum_u64(m);
