@@ -1629,7 +1629,8 @@ int launch_packed_attention(const PackedAttnArgs& a, void* ws, hipStream_t s) {
 
 // Blocks that share a key tile's rows, each every so-many-th row tile: where the tiles are fewer than
 // keep the device even, at most 8 (`seen`: about how many rows a key has, 0 for unknown: a block
-// gets 256 of them or more).  Their parts cost a join of 4 to 10 us.  dk and dv, sliced with the join
+// gets 256 of them or more, f32 with d = 128, whose tiles take longest, 128: 54 sequences of up to 93, 8 / 1
+// heads, 72 us and 126, but 20 of 100, 12 / 4 heads of 64, 40 and 35).  Their parts cost a join of 4 to 10 us.  dk and dv, sliced with the join
 // and in one block:
 //   f32   12 / 4 heads of 64: 1000 + 77 + 439 tokens 110 and 191 us, 1000 + 780 + 439 139 and 195;
 //         8 / 1 heads of 128: 2 x 2000 827 and 1880; but with more blocks 12 / 12 of 64, 2 x 1000,
@@ -1642,7 +1643,7 @@ int key_slices(int64_t total, int Hkv, int d, bool f32, int64_t seen) {
   const int64_t blocks = (total + each - 1) / each * Hkv;
   const int64_t fill = f32 ? 1024 : d == 64 ? 768 : seen == 0 || seen >= 4096 ? 512 : 256;
   if (blocks < 1 || blocks >= fill) return 1;
-  const int64_t most = seen > 0 ? std::max<int64_t>(seen / 256, 1) : 8;
+  const int64_t most = seen > 0 ? std::max<int64_t>(seen / (f32 && d == 128 ? 128 : 256), 1) : 8;
   return (int)std::min<int64_t>(std::min<int64_t>(fill / blocks, 8), most);
 }
 // the stats of 64 rows each, the orders of row and key tiles, then the parts of dk and dv
