@@ -18,8 +18,8 @@
 // code: PREFIX takes the tokens of all sequences as the rows of one, over the keys of the
 // prefix, which they all see whole, in parts whose unnormalised outputs, maxima and sums it leaves
 // in memory.  Each sequence's keys from there on are either a launch behind it (TAILS), which joins its
-// rows' parts of the prefix to them, or (bf16, 33 rows or more in all, up to 32 of a sequence) blocks
-// beside it (OWN), with a launch that joins both.  (Joined by the block whose part ends
+// rows' parts of the prefix to them, or (bf16, 33 rows or more in all) blocks beside it (OWN), with a
+// launch that joins both.  (Joined by the block whose part ends
 // last, as others are, one block had all rows of a key head to join.)
 #include <algorithm>
 #include <type_traits>
@@ -620,7 +620,7 @@ __device__ inline bool shared_row(const KArgs& p, const Item& it, int token, int
         o[j >> 2][4 * (j & 3) + e] = a.o[e];
     }
   }
-  return MODE == PREFIX;
+  return MODE == PREFIX || MODE == OWN;
 }
 
 // ---- bf16, tiles of rows ---------------------------------------------------------
@@ -1293,24 +1293,28 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(KArgs p) {
   few_body<D, NR, NW, MODE>(p, blockIdx.x, lds, sm, sl, ptab);
 }
 
-// ---- bf16, a prefix and few rows of each sequence --------------------------------------
+// ---- bf16, a prefix and rows of their own beside it -------------------------------------
 // PREFIX and what the sequences have of their own in one launch, side by side, since neither fills
-// the chip for long; the first `first` blocks (a multiple of 8) are PREFIX's, of the others only two waves
-// stay.  With the join, against PREFIX and TAILS behind each other: 48 single tokens over 8192 shared
+// the chip for long; the first `first` blocks (a multiple of 8) are PREFIX's, the others in the form for
+// 16 NR rows, of which only two waves stay, or (NR = 0) in that for 128.  With the join, against PREFIX and TAILS behind each other: 48 single tokens over 8192 shared
 // and up to 200 own keys, 12 heads, 25.0 and 28.5 us (PREFIX alone 13.4, 25 MB of keys and values:
 // dependent steps); 16 drafts of up to 6 over 30001 and up to 900, 32 / 8 heads of 128, 73 and 81 (46 alone,
 // 123 MB: 2.6 TB/s, and 27 GFLOP), of up to 9 92 and 123; 64 single tokens over 4000 and
-// 300, 8 / 1 heads of 128, 20.6 and 32.4, where without a prefix they take 22.2.
+// 300, 8 / 1 heads of 128, 20.6 and 32.4, where without a prefix they take 22.2.  Chunks: 9 of up to 38 over
+// 3250 and 294, 8 / 1 heads of 128, 30 and 125 (29 without), 18 of up to 16 over 20679 43 and 142 (82); 4 of
+// up to 200 over 16000, 32 / 8 heads, 277 and 308 (258).
 template <int D, int NR>
 __global__ __launch_bounds__(256, 2) void paged_attn_both_kernel(KArgs pre, KArgs own,
                                                                  unsigned first) {
   static_assert(few_ring(D, 2) <= 2 * 2 * 64 * D && PTF >= PT, "one serves both");
   __shared__ __attribute__((aligned(1024))) uint16_t lds[2 * 2 * 64 * D];
-  __shared__ float sm[2][16 * NR], sl[2][16 * NR];
   __shared__ int ptab[PTF];
   if (blockIdx.x < first) {
     tiles_body<D, 2, PREFIX>(pre, blockIdx.x, lds, ptab);
+  } else if constexpr (NR == 0) {
+    tiles_body<D, 2, OWN>(own, blockIdx.x - first, lds, ptab);
   } else {
+    __shared__ float sm[2][16 * NR], sl[2][16 * NR];
     if (threadIdx.x >= 128) return;  // (a barrier waits for the waves that are left)
     few_body<D, NR, 2, OWN>(own, blockIdx.x - first, lds, sm, sl, ptab);
   }
@@ -1911,8 +1915,9 @@ template <int D, int MODE>
 int run_paged(const KArgs& p, const Shape& sh, unsigned nb, hipStream_t s) {
   const dim3 grid(nb), block(256);
   switch (sh.form) {
-    case FORM_TILES:
-      hipLaunchKernelGGL((paged_attn_kernel<D, 2, MODE>), grid, block, 0, s, p);
+    case FORM_TILES:  // (with a prefix: launch_both)
+      if constexpr (MODE == WHOLE)
+        hipLaunchKernelGGL((paged_attn_kernel<D, 2, MODE>), grid, block, 0, s, p);
       break;
     case FORM_FEW16:
       hipLaunchKernelGGL((paged_attn_few_kernel<D, 1, 2, MODE>), grid, dim3(128), 0, s, p);
@@ -2022,8 +2027,10 @@ static int launch_both(const Launch& pre, const Launch& own, int64_t total, hipS
   const dim3 grid(first + (unsigned)own.blocks);
   if (own.sh.form == FORM_FEW16)
     hipLaunchKernelGGL((paged_attn_both_kernel<D, 1>), grid, dim3(256), 0, s, pre.p, own.p, first);
-  else
+  else if (own.sh.form == FORM_FEW32)
     hipLaunchKernelGGL((paged_attn_both_kernel<D, 2>), grid, dim3(256), 0, s, pre.p, own.p, first);
+  else
+    hipLaunchKernelGGL((paged_attn_both_kernel<D, 0>), grid, dim3(256), 0, s, pre.p, own.p, first);
   constexpr int rows = 64 / (D / 4);
   hipLaunchKernelGGL((paged_attn_join_kernel<D>),
                      dim3((unsigned)((total * own.p.G + rows - 1) / rows), (unsigned)own.p.Hkv),
@@ -2041,7 +2048,7 @@ int launch_paged_attention(const blt_paged_cache& c, const PagedAttnArgs& a, voi
   }
   Launch pre = launch_of(c, a, PREFIX, ws);
   const Launch own = launch_of(c, a, TAILS, ws);
-  if (pre.sh.form == FORM_TILES && (own.sh.form == FORM_FEW16 || own.sh.form == FORM_FEW32))
+  if (pre.sh.form == FORM_TILES)  // (so bf16)
     return narrow ? launch_both<64>(pre, own, a.total, s) : launch_both<128>(pre, own, a.total, s);
   pre.p.taken = nullptr;
   if (int rc = narrow ? launch_one<64, PREFIX>(pre, s) : launch_one<128, PREFIX>(pre, s)) return rc;
