@@ -300,6 +300,17 @@ def test_many_rows_in_one_launch_with_their_prefix(d, H, Hkv, chunk, B):
     assert bool((o == 7).all())
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("d,H,Hkv", [(64, 4, 4), (64, 8, 2), (128, 8, 1), (128, 4, 2)])
+@pytest.mark.parametrize("ctx,tails,n", [(700, [200, 90, 64], [150, 60, 33]), (2000, [900, 40], [100, 40]),
+                                         (64, [300, 280, 5, 270], [290, 1, 0, 129])])
+def test_chunks_with_their_prefix(dtype, d, H, Hkv, ctx, tails, n):
+    """Chunks of more rows than a tile, over own keys in parts and in one."""
+    m = shared(ctx, tails, Hkv=Hkv, d=d, page=16, dtype=TYPES[dtype])
+    check(m, n, H)
+    check(m, n, H, causal=False, prefix=i32([ctx // 2]))
+
+
 @pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
 def test_not_finite_in_one_launch_with_their_prefix(value):
     m = shared(320, [8] * 50, Hkv=1, d=64, page=16)
