@@ -749,7 +749,7 @@ __device__ inline bool rows_of(const PArgs& p, int key, int& rlo, int& rhi) {
 // other kernel.  So both gradients are 2.3e-3 off or less (relative, rms; their own rounding is
 // 1.7e-3), and not 2.5e-3 or, in short sequences, 3e-3.
 // Four sequences of up to 4096 (9 k tokens), 32 / 8 heads of 128: 435 us, four products (dS twice) at
-// 1.1 PFLOP/s, matrix cores 54 % and vector units 48 % busy; eleven of up to 2047, window 512, 12 heads of
+// 1.1 PFLOP/s, matrix cores 55 % and vector units 47 % busy; eleven of up to 2047, window 512, 12 heads of
 // 64: 48 us, ten key tiles behind each other in 1.5 rounds of blocks (52 with 64 keys at a time, whether
 // seen or not, and both sides of the mask in one).
 template <int D>
@@ -954,9 +954,9 @@ __device__ inline int64_t part_at(const PArgs& p, int slice, int kvh, int what, 
 // The shares are added up at the end; with SLICED a block takes every gridDim.y-th row tile and leaves its sums
 // to packed_join_kernel (a kernel of its own: the few registers more would be spilled, beside DMA in
 // flight, by all calls).  For d = 128, K and the two sums fill the registers and V is read from LDS.
-// Same calls as dq's above: 515 us, four products at 0.94 PFLOP/s, matrix cores 43 % busy, the rest waits
+// Same calls as dq's above: 510 us, four products at 0.96 PFLOP/s, matrix cores 45 % busy, the rest waits
 // for LDS operands (16 reads of 16 bytes for 16 products of 32 cycles) and the exponentials between them;
-// and 53 us, 22 %.
+// and 51 us, 23 %.
 template <int D, int KW, int RW, int BR, bool SLICED>
 __global__ __launch_bounds__(64 * KW * RW, D == 64 ? 3 : 2) void packed_dkdv_kernel(GArgs ga) {
   const PArgs& p = ga.a;
@@ -1629,9 +1629,9 @@ int launch_packed_attention(const PackedAttnArgs& a, void* ws, hipStream_t s) {
 
 // Blocks that share a key tile's rows, each every so-many-th row tile: where the tiles are fewer than
 // keep the device even, at most 8 (`seen`: about how many rows a key has, 0 for unknown: a block
-// gets 256 of them or more, f32 with d = 128, whose tiles take longest, 128: 54 sequences of up to 93, 8 / 1
-// heads, 72 us and 126, but 20 of 100, 12 / 4 heads of 64, 40 and 35).  Their parts cost a join of 4 to 10 us.  dk and dv, sliced with the join
-// and in one block:
+// gets 256 of them or more; f32 with d = 128, whose tiles take longest, 128: 54 sequences of up to
+// 93, 8 / 1 heads, 72 us and 126, but 20 of 100, 12 / 4 heads of 64, 40 and 35).  Their parts cost a
+// join of 4 to 10 us.  dk and dv, sliced with the join and in one block:
 //   f32   12 / 4 heads of 64: 1000 + 77 + 439 tokens 110 and 191 us, 1000 + 780 + 439 139 and 195;
 //         8 / 1 heads of 128: 2 x 2000 827 and 1880; but with more blocks 12 / 12 of 64, 2 x 1000,
 //         133 and 124

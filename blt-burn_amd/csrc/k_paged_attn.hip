@@ -1296,8 +1296,8 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(KArgs p) {
 // ---- bf16, a prefix and rows of their own beside it -------------------------------------
 // PREFIX and what the sequences have of their own in one launch, side by side, since neither fills
 // the chip for long; the first `first` blocks (a multiple of 8) are PREFIX's, the others in the form for
-// 16 NR rows, of which only two waves stay, or (NR = 0) in that for 128.  With the join, against PREFIX and TAILS behind each other: 48 single tokens over 8192 shared
-// and up to 200 own keys, 12 heads, 25.0 and 28.5 us (PREFIX alone 13.4, 25 MB of keys and values:
+// 16 NR rows, of which only two waves stay, or (NR = 0) in that for 128.  With the join, against PREFIX
+// and TAILS behind each other: 48 single tokens over 8192 shared and up to 200 own keys, 12 heads, 25.0 and 28.5 us (PREFIX alone 13.4, 25 MB of keys and values:
 // dependent steps); 16 drafts of up to 6 over 30001 and up to 900, 32 / 8 heads of 128, 73 and 81 (46 alone,
 // 123 MB: 2.6 TB/s, and 27 GFLOP), of up to 9 92 and 123; 64 single tokens over 4000 and
 // 300, 8 / 1 heads of 128, 20.6 and 32.4, where without a prefix they take 22.2.  Chunks: 9 of up to 38 over
@@ -2046,6 +2046,7 @@ int launch_paged_attention(const blt_paged_cache& c, const PagedAttnArgs& a, voi
     const Launch x = launch_of(c, a, WHOLE, ws);
     return narrow ? launch_one<64, WHOLE>(x, s) : launch_one<128, WHOLE>(x, s);
   }
+  if (a.total * (a.H / c.n_kv_heads) > 0x7fff0000) return too_many();  // (rows are counted in 32 bits)
   Launch pre = launch_of(c, a, PREFIX, ws);
   const Launch own = launch_of(c, a, TAILS, ws);
   if (pre.sh.form == FORM_TILES)  // (so bf16)
