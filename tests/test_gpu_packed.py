@@ -352,6 +352,35 @@ def test_same_bits_in_every_run_and_in_a_graph(dtype):
         assert all(torch.equal(a, b) for a, b in zip(held, fresh))
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_autograd_in_a_graph(dtype):
+    """Forward and gradient through autograd, captured together, on leaves without another graph."""
+    t = TYPES[dtype]
+    q, k, v, do = (x.clone() for x in made([200, 90], 6, 8, 2, 64, t))
+    s = i32([0, 200, 290])
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(F.fused_packed_attention(*leaves, s, window=50), leaves, do)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o = F.fused_packed_attention(*leaves, s, window=50)
+        grads = torch.autograd.grad(o, leaves, do)
+        o = o.detach()
+    for n in range(3):
+        with torch.no_grad():
+            q.normal_()
+            do.normal_()
+            s.copy_(i32([[0, 200, 290], [0, 10, 280], [0, 0, 296]][n]))
+            want, lse = F.fused_packed_attention(q, k, v, s, window=50, return_lse=True)
+            fresh = F.fused_packed_attention_backward(do, q, k, v, want, lse, s, window=50)
+        torch.cuda.synchronize()
+        graph.replay()
+        assert torch.equal(o, want) and all(torch.equal(a, b) for a, b in zip(grads, fresh))
+
+
 def test_starts_that_do_not_ascend_stay_within_the_tensors():
     """Their outputs are not specified, but rows outside the pack are left alone."""
     for t in TYPES.values():
