@@ -489,10 +489,10 @@ __global__ __launch_bounds__(256, 2) void packed_attn_kernel(PArgs p) {
         w.y = pack_bf16x2(o[ds][4 * j + 2] * inv, o[ds][4 * j + 3] * inv);
         *reinterpret_cast<u32x2_t*>(orow + ds * 32 + 8 * j + 4 * lhalf) = w;
       }
-    if (LSE && lhalf == 0)
-      p.lse[(int64_t)tok * p.H + head] =
-          total == 0.f ? -INFINITY : fmaf(m, p.scale, logf(total));
   }
+  // (behind the last sequence too, whatever `tail` says of o)
+  if (LSE && rw + lrow < p.rows && lhalf == 0)
+    p.lse[(int64_t)tok * p.H + head] = total == 0.f ? -INFINITY : fmaf(m, p.scale, logf(total));
 }
 
 // ---- f32 -----------------------------------------------------------------------------
@@ -675,7 +675,7 @@ __global__ __launch_bounds__(256) void packed_attn_f32_kernel(PArgs p) {
   if (w == 0 && h == 0) {
     sl[0][l31] = lt;
     write[l31] = r0 + l31 < p.rows && (in || p.tail);
-    if (p.lse && write[l31])
+    if (p.lse && r0 + l31 < p.rows)  // (behind the last sequence too)
       p.lse[(int64_t)tok * p.H + head] = lt == 0.f ? -INFINITY : fmaf(mx, p.scale, logf(lt));
   }
   __syncthreads();

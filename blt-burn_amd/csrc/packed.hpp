@@ -20,7 +20,7 @@ struct PackedAttnArgs {
   int64_t B;
   int causal, window;
   float scale;
-  int tail;  // tokens behind the last sequence: 0 = left alone, 1 = zeros
+  int tail;  // o behind the last sequence: 0 = left alone, 1 = zeros (lse: -inf)
 };
 int64_t packed_attention_workspace_bytes(int64_t B, int64_t total, int H, int Hkv, int dtype);
 int launch_packed_attention(const PackedAttnArgs& a, void* ws, hipStream_t s);

@@ -320,7 +320,7 @@ def fused_packed_attention(q, k, v, starts, causal=True, window=0, scale=None, o
 
     Returns o [tokens, heads, head_dim]; with return_lse also the logarithms of the softmax's sums,
     f32 [tokens, heads] (-inf for none), which fused_packed_attention_backward takes.  Tokens at
-    starts[-1] and behind get 0 in a new tensor and are left alone in `out`.  Scores and sums
+    starts[-1] and behind get 0 in a new tensor and are left alone in `out` (lse -inf in both).  Scores and sums
     are f32 throughout; in bf16 the weights are rounded to bf16.  Autograd follows it for o
     (once; `out` takes no inputs that need a gradient)."""
     if torch.is_grad_enabled() and (getattr(q, "requires_grad", False)

@@ -162,7 +162,7 @@ int blt_fused_sample(const void* logits, int64_t row_stride, int32_t dtype, int6
  *   window: W > 0 (with causal) = only the last W of them
  *   scale:  of the scores, 1e-30 .. 1e30
  *   lse:    (may be NULL) f32 [total, Hq], log of the sum of e^score, -inf where it is 0
- *   tail:   tokens at starts[B] and behind: 0 = left alone, 1 = outputs 0, lse -inf
+ *   tail:   tokens at starts[B] and behind: 0 = o left alone, 1 = o 0; lse is -inf there in both
  * Scores, softmax and sums in f32; in bf16 the weights are rounded to bf16.  A key whose
  * score is -inf weighs nothing; infinite and NaN values come through where they are seen.
  * workspace: blt_packed_attention_workspace_bytes (0 for small calls and one sequence), 16-byte

@@ -428,3 +428,23 @@ def test_refusals():
               lambda: F.fused_packed_attention(q, k, v, [0, 10])):
         with pytest.raises(TypeError):
             f()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("d,H,K", [(64, 4, 4), (128, 6, 2)])
+@pytest.mark.parametrize("lens", [[40, 3], [130, 0], []])
+@pytest.mark.parametrize("causal,window", [(True, 0), (True, 9), (False, 0)])
+def test_lse_behind_the_last_sequence_with_out(dtype, d, H, K, lens, causal, window):
+    """`out` keeps its rows there; lse, a tensor of the call's own, has -inf in all of them."""
+    t, n, pad = TYPES[dtype], sum(lens), 200
+    q, k, v, _ = made(lens, pad, H, K, d, t)
+    st = starts_of(lens)
+    used = [torch.full((n + pad, H), 7.0, device=DEV) for _ in range(8)]
+    del used  # (memory that the call's tensors are likely to get)
+    out = torch.full((n + pad, H, d), 7.0, dtype=t, device=DEV)
+    kw = dict(causal=causal, window=window)
+    o, lse = F.fused_packed_attention(q, k, v, i32(st), out=out, return_lse=True, **kw)
+    assert o is out and bool((o[n:] == 7).all()) and bool((lse[n:] == -math.inf).all())
+    r = R.attention(q, k, v, st, u=U[t], **kw)
+    near(lse, r, "lse")
+    near(o[:n], {x: r[x][:n] for x in ("o", "tol_o")}, "o")
