@@ -272,8 +272,7 @@ class PagedCache:
         """Tokens that the listed sequences (None: all) have in common, as an int32 [1] tensor
         of the device (`out` if given): the leading whole pages that are the same pages, as fork
         leaves them.  Sequences without tokens are left out; 0 with fewer than two.  For attention's
-        `prefix`: it stays right for all layers and steps until one of these sequences is
-        cut, dropped or replaced, or pages are moved."""
+        `prefix`, in all layers and in later steps."""
         s, n = (None, self.max_seqs) if seqs is None else self._list(seqs, "seqs")
         if out is None:
             out = torch.empty(1, dtype=torch.int32, device=self.device)
@@ -300,9 +299,10 @@ class PagedCache:
         apart from many single tokens; and calls of more than some hundred rows are best cut
         into several (a call's cost has a part that grows with the square of its rows).
 
-        prefix: what common_prefix said of a list that holds these sequences.  The keys that they
-        share are then read once for all rows, which pays where several rows have a long
-        prefix and few tokens each (16 rows of up to 6 tokens over 30001 keys, 32 / 8 heads of 128,
+        prefix: what common_prefix said of a list that holds these sequences, now or in an earlier
+        step (where one of those with tokens does not have it, having been empty then, or cut or
+        replaced since, the call goes without).  The keys that they share are then read once for
+        all rows, which pays where several rows have a long prefix and few tokens each (16 rows of up to 6 tokens over 30001 keys, 32 / 8 heads of 128,
         73 us for 270; 4 of up to 200 over 16000 277 for 258); the outputs are those without it,
         up to their rounding.  (It is not used with a window, whose rows do not see all of it.)"""
         layer = self._layer(layer)

@@ -127,21 +127,41 @@ __device__ bool find_item(const KArgs& p, unsigned bid, Item& it) {
   float work = 0.f, tiles = 0.f, longest = 0.f;
   bool lost = false, crossed = false;
   if constexpr (MODE != WHOLE) {
-    // the shared keys, whole pages, as far as they lie before every row's tokens (so that all
-    // see all of them, whatever `prefix` says), and a sequence that has them
-    int room = 0x7fffffff, slot = -1;
-    for (int b0 = 0; b0 < p.B; b0 += 64) {
-      q = seq_at(p, b0 + lane, lost, crossed);
-      if (q.n) room = min(room, q.len - q.n);
-      const uint64_t any = __ballot(q.n > 0);
-      if (slot < 0 && any) slot = lane_of(q.slot, __ffsll((unsigned long long)any) - 1);
+    // The shared keys, whole pages, as far as they lie before every row's tokens (so that all
+    // see all of them, whatever `prefix` says), and a sequence that has them.  A sequence whose last
+    // shared page is another one does not have them (it was without tokens when the others were
+    // compared, or has been cut or replaced since): then nothing is taken as shared.  One page
+    // tells, for pages are shared by forks, with all before them; it is read beside the lengths, and
+    // again where these leave less than `prefix`.  (The comparison costs 0.9 us of a launch.)
+    const int number = p.prefix[0], a = p.starts[0], e = p.starts[B];
+    int slot = -1, last = max((min(number, p.cap) >> p.lps) - 1, 0), tries = 0;
+    for (; tries < 2; ++tries) {
+      int room = 0x7fffffff, page = 0;
+      bool other = false;
+      slot = -1;
+      for (int b0 = 0; b0 < B; b0 += 64) {
+        q = seq_at(p, b0 + lane, lost, crossed);
+        const int x = p.table[(int64_t)q.slot * p.max_pages + last];
+        if (q.n) room = min(room, q.len - q.n);
+        const uint64_t any = __ballot(q.n > 0);
+        if (slot < 0 && any) {
+          const int l = __ffsll((unsigned long long)any) - 1;
+          slot = lane_of(q.slot, l);
+          page = lane_of(x, l);
+        }
+        other = other || (q.n && x != page);
+      }
+      room = min(number, -wave_max_i32(-room));
+      from = __builtin_amdgcn_readfirstlane(room > 0 && slot >= 0 ? room >> p.lps << p.lps : 0);
+      const int col = (from >> p.lps) - 1;
+      if (from && col == last && __any(other)) from = 0;
+      if (from == 0 || col == last) break;
+      last = col;
     }
-    room = min(p.prefix[0], -wave_max_i32(-room));
-    from = __builtin_amdgcn_readfirstlane(room > 0 ? room >> p.lps << p.lps : 0);
+    if (tries == 2) from = 0;  // (lengths that change meanwhile)
     if constexpr (MODE == PREFIX) {
       if (p.taken && bid == 0 && threadIdx.x == 0) *p.taken = __any(crossed) ? 0 : from;
-      if (__any(crossed) || slot < 0 || from == 0) return false;  // (TAILS reports it)
-      const int a = p.starts[0], e = p.starts[p.B];
+      if (__any(crossed) || from == 0) return false;  // (TAILS or OWN reports it)
       it.q = Seq{a, e - a, from, slot};
       it.nrt = (int)(((uint32_t)(it.q.n * p.G) + BQ - 1) / BQ);
       it.ns = prefix_parts(p, from);
@@ -151,10 +171,10 @@ __device__ bool find_item(const KArgs& p, unsigned bid, Item& it) {
       const int all = p.Hkv * it.ns * it.nrt, per = (all + 7) >> 3;
       const int id = (int)(bid & 7) * per + (int)(bid >> 3);
       if ((int)(bid >> 3) >= per || id >= all) return false;
-      const int x = (int)((uint32_t)id / (uint32_t)it.nrt);
-      it.rt = id - x * it.nrt;
-      it.kvh = (int)((uint32_t)x / (uint32_t)it.ns);
-      it.split = x - it.kvh * it.ns;
+      const int at = (int)((uint32_t)id / (uint32_t)it.nrt);
+      it.rt = id - at * it.nrt;
+      it.kvh = (int)((uint32_t)at / (uint32_t)it.ns);
+      it.split = at - it.kvh * it.ns;
       return true;
     }
   }

@@ -365,8 +365,10 @@ int blt_cache_common_prefix(const blt_paged_cache* cache, const int32_t* seqs, i
 /* blt_paged_attention without a window for sequences that share their first prefix[0] tokens (int32
  * [1], device, from blt_cache_common_prefix of a list that holds these sequences): the shared
  * keys are read once for all rows (two launches).  What is no whole page, and what does not lie
- * before every row's new tokens, is not taken as shared, so any number is safe; but where the first
- * pages are not the same ones, rows see those of the first row that has tokens. */
+ * before every row's new tokens, is not taken as shared, and nothing is where the last page of
+ * that is not the same in all sequences with tokens.  So any number is safe for page tables in
+ * which a page that two sequences share has the same pages before it in both, as blt_cache_fork
+ * leaves them; in others it must be blt_cache_common_prefix's of the same tables. */
 int64_t blt_paged_attention_prefix_workspace_bytes(const blt_paged_cache* cache, int64_t B,
                                                    int64_t total, int64_t Hq);
 int blt_paged_attention_prefix(const blt_paged_cache* cache, int32_t layer, const void* q,

@@ -435,3 +435,38 @@ def test_prompts_continued_and_answered():
             assert bool(((out[i].double().cpu() - r["o"][-1]).abs() <= r["tol_o"][-1]).all()), step
     cache.check()
     assert len({tuple(r.tolist()) for r in rows}) > 1
+
+
+# ---- sequences that do not have the prefix ---------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("B,H,Hkv", [(3, 4, 2), (12, 4, 4), (40, 4, 2), (90, 8, 2)])
+@pytest.mark.parametrize("refilled", [False, True])
+def test_a_sequence_filled_after_the_prefix_was_taken(dtype, B, H, Hkv, refilled):
+    """One that was empty when common_prefix listed it (or dropped since), with tokens of its own now."""
+    ctx = 160
+    m = Made([ctx + 3 + b % 20 for b in range(B)], Hkv=Hkv, d=64, page=16, dtype=TYPES[dtype], seed=B)
+    other = B // 2
+    own = m.table[other].copy()
+    m.table[:B, :ctx // 16] = m.table[0, :ctx // 16]
+    if not refilled:
+        m.table[other] = own
+    m.cache.page_table.copy_(i32(m.table))
+    full = m.cache.lens.clone()
+    if not refilled:
+        m.cache.lens[other] = 0
+    prefix = m.cache.common_prefix()
+    assert prefix.tolist() == [ctx]
+    m.table[other] = own
+    m.cache.page_table.copy_(i32(m.table))
+    m.cache.lens.copy_(full)
+    check(m, [1] * B, H, prefix=prefix)
+    check(m, [1 + b % 3 for b in range(B)], H, prefix=prefix)
+    check(m, [1] * B, H, prefix=prefix, causal=False)
+    # without that sequence's tokens, or without the sequence, the prefix is taken as before
+    check(m, [1 if b != other else 0 for b in range(B)], H, prefix=prefix)
+    ids = [b for b in range(B) if b != other]
+    check(m, [1] * (B - 1), H, prefix=prefix, seqs=ids)
+    # the first row is the one that does not have it
+    ids = [other] + ids
+    check(m, [1] * B, H, prefix=prefix, seqs=ids)
