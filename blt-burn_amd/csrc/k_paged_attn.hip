@@ -643,6 +643,19 @@ __device__ inline bool shared_row(const KArgs& p, const Item& it, int token, int
   return MODE == PREFIX || MODE == OWN;
 }
 
+// p as two bf16 halves (p cut off, and what that left, rounded): off by 2^-15 at most, against
+// 2^-8 of the output's own rounding.  Cut off and not rounded, and the rest with 2^-22 p on
+// top, so that both halves are above zero: an infinite value times zero or a negative rest
+// would be NaN (below p = 2^-104, where the rest may vanish, it still is).  Of two weights in one word.
+constexpr float kAbove1 = 1.f + 0x1p-22f;
+__device__ inline uint32_t upper_halves(float p0, float p1) {
+  return __builtin_amdgcn_perm(__float_as_uint(p1), __float_as_uint(p0), 0x07060302);
+}
+__device__ inline uint32_t lower_halves(float p0, float p1) {
+  return pack_bf16x2(fmaf(p0, kAbove1, -__uint_as_float(__float_as_uint(p0) & 0xffff0000u)),
+                     fmaf(p1, kAbove1, -__uint_as_float(__float_as_uint(p1) & 0xffff0000u)));
+}
+
 // ---- bf16, tiles of rows ---------------------------------------------------------
 // One block = 4 waves of 32 rows each; key tiles of 64 keys go global -> LDS by DMA
 // through NST stages shared by the waves.  As in attn_fwd_kernel the scores are taken
@@ -658,7 +671,11 @@ __device__ inline bool shared_row(const KArgs& p, const Item& it, int token, int
 // 1.0 PFLOP/s of the visible pairs (an 8192^3 library product reaches 1.4); the matrix cores
 // are busy 46 % of the time and the vector units 43 %, hardly ever both.  With 64 rows a wave
 // (1.2 ms for 0.96 then), three stages, or 32-key tiles at three waves a SIMD it was slower.
-template <int D, int NST, int MODE>
+// HALVES: p as two halves, for a prefix of rows whose own keys go through the form for few rows (see
+// paged_attn_both_kernel), so that a prefix costs no accuracy: 16 drafts of 3 over 1500 and up to 35, 32 / 8
+// heads, 1.66e-3 off with and without it, 2.3e-3 where p is rounded (two layers of the drafts named
+// there 178 us and 155).
+template <int D, int NST, int MODE, bool HALVES>
 __device__ __forceinline__ void tiles_body(const KArgs& p, unsigned bid, uint16_t* lds, int* ptab) {
   constexpr int BKV = 64, QPW = 32, BQ = 4 * QPW;
   constexpr int TILE = BKV * D;        // elements of a K (or V) tile
@@ -907,20 +924,33 @@ __device__ __forceinline__ void tiles_body(const KArgs& p, unsigned bid, uint16_
       for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          uint32_t w[4];
+          uint32_t w[4], rest[4];
 #pragma unroll
           for (int e = 0; e < 8; e += 2) {
             const float p0 = __builtin_amdgcn_exp2f(fmaf(s[sub][8 * u + e], c, mc));
             const float p1 = __builtin_amdgcn_exp2f(fmaf(s[sub][8 * u + e + 1], c, mc));
-            w[e >> 1] = pack_bf16x2(p0, p1);
-            l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w[e >> 1]), ones2, l,
-                                                false);
+            if constexpr (HALVES) {
+              l += p0 + p1;
+              w[e >> 1] = upper_halves(p0, p1);
+              rest[e >> 1] = lower_halves(p0, p1);
+            } else {
+              w[e >> 1] = pack_bf16x2(p0, p1);
+              l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w[e >> 1]), ones2, l,
+                                                  false);
+            }
           }
           const bf16x8_t pb = __builtin_bit_cast(bf16x8_t, u32x4_t{w[0], w[1], w[2], w[3]});
 #pragma unroll
           for (int ds = 0; ds < DS; ++ds)  // (independent chains)
             o[ds] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
                 __builtin_bit_cast(bf16x8_t, vf[ds][sub][u]), pb, o[ds], 0, 0, 0);
+          if constexpr (HALVES) {
+            const bf16x8_t pr = __builtin_bit_cast(bf16x8_t, u32x4_t{rest[0], rest[1], rest[2], rest[3]});
+#pragma unroll
+            for (int ds = 0; ds < DS; ++ds)
+              o[ds] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                  __builtin_bit_cast(bf16x8_t, vf[ds][sub][u]), pr, o[ds], 0, 0, 0);
+          }
         }
     }
     stage = stage + 1 < NST ? stage + 1 : 0;
@@ -952,7 +982,7 @@ template <int D, int NST, int MODE>
 __global__ __launch_bounds__(256, 2) void paged_attn_kernel(KArgs p) {
   __shared__ __attribute__((aligned(1024))) uint16_t lds[NST * 2 * 64 * D];
   __shared__ int ptab[PT];
-  tiles_body<D, NST, MODE>(p, blockIdx.x, lds, ptab);
+  tiles_body<D, NST, MODE, false>(p, blockIdx.x, lds, ptab);
 }
 
 // ---- bf16, few rows ----------------------------------------------------------------
@@ -961,16 +991,12 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(KArgs p) {
 // every NW-th 32-key tile of the item through its own LDS ring of two tiles, filled by DMA
 // while the tiles before are consumed, and they meet once at the end.  16 x 16 x 32
 // MFMAs, scores transposed as above (a lane owns a row, the key blocks' registers are the
-// second product's operand).  p goes into that product as two bf16 halves (p cut off, and
-// what that left, rounded): the matrix cores have nothing else to do, and p is off by 2^-15 at
-// most, against 2^-8 of the output's own rounding.  Cut off and not rounded, and the rest with
-// 2^-22 p on top, so that both halves are above zero: an infinite value times zero or a
-// negative rest would be NaN (below p = 2^-104, where the rest may vanish, it still is).
+// second product's operand).  p goes into that product as two bf16 halves: the matrix cores have
+// nothing else to do.
 // 48 single tokens over up to 8192 keys, 12 heads of 64: 128 us, 5.0 TB/s; 16 over up to 32768
 // keys, 32 / 8 heads of 128: 169 us, 5.5 TB/s (a large copy: 6.15).  One token over 1000 keys,
 // 12 heads: 8.9 us of dependent steps: launch 1.7, find_item 0.5, pages 0.6, tiles 2.1, the
 // waves' merge 1.3, join 2.6; over 8192 keys 15.4 us, over 32768 26.8.
-constexpr float kAbove1 = 1.f + 0x1p-22f;
 template <int N>
 __device__ inline void wait_loads() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
@@ -1161,10 +1187,8 @@ __device__ __forceinline__ void few_body(const KArgs& p, unsigned bid, uint16_t*
         const float p0 = __builtin_amdgcn_exp2f(fmaf(s[n][e >> 2][e & 3], c, mc[n]));
         const float p1 = __builtin_amdgcn_exp2f(fmaf(s[n][e >> 2][(e & 3) + 1], c, mc[n]));
         l[n] += p0 + p1;
-        const uint32_t x0 = __float_as_uint(p0), x1 = __float_as_uint(p1);
-        wh[e >> 1] = __builtin_amdgcn_perm(x1, x0, 0x07060302);  // their upper halves
-        wl[e >> 1] = pack_bf16x2(fmaf(p0, kAbove1, -__uint_as_float(x0 & 0xffff0000u)),
-                                 fmaf(p1, kAbove1, -__uint_as_float(x1 & 0xffff0000u)));
+        wh[e >> 1] = upper_halves(p0, p1);
+        wl[e >> 1] = lower_halves(p0, p1);
       }
       ph[n] = __builtin_bit_cast(bf16x8_t, u32x4_t{wh[0], wh[1], wh[2], wh[3]});
       pl[n] = __builtin_bit_cast(bf16x8_t, u32x4_t{wl[0], wl[1], wl[2], wl[3]});
@@ -1330,9 +1354,9 @@ __global__ __launch_bounds__(256, 2) void paged_attn_both_kernel(KArgs pre, KArg
   __shared__ __attribute__((aligned(1024))) uint16_t lds[2 * 2 * 64 * D];
   __shared__ int ptab[PTF];
   if (blockIdx.x < first) {
-    tiles_body<D, 2, PREFIX>(pre, blockIdx.x, lds, ptab);
+    tiles_body<D, 2, PREFIX, NR != 0>(pre, blockIdx.x, lds, ptab);
   } else if constexpr (NR == 0) {
-    tiles_body<D, 2, OWN>(own, blockIdx.x - first, lds, ptab);
+    tiles_body<D, 2, OWN, false>(own, blockIdx.x - first, lds, ptab);
   } else {
     __shared__ float sm[2][16 * NR], sl[2][16 * NR];
     if (threadIdx.x >= 128) return;  // (a barrier waits for the waves that are left)

@@ -11,6 +11,7 @@ import packed_ref
 import paged_ref as R
 from blt_burn_amd import BltError, cache as C, fused_ops as F
 from test_gpu_paged import DEV, TYPES, Made, att_tol, f64, i32
+from test_gpu_paged_edges import few_tol
 from test_gpu_sample import reference as sample_reference
 
 pytestmark = pytest.mark.gpu
@@ -470,3 +471,24 @@ def test_a_sequence_filled_after_the_prefix_was_taken(dtype, B, H, Hkv, refilled
     # the first row is the one that does not have it
     ids = [other] + ids
     check(m, [1] * B, H, prefix=prefix, seqs=ids)
+
+
+# ---- accuracy ------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("d,H,Hkv,n,B", [(64, 4, 4, 1, 40), (64, 6, 2, 5, 30), (64, 8, 1, 4, 9), (128, 4, 4, 1, 48),
+                                         (128, 8, 2, 3, 12), (128, 8, 1, 4, 20), (64, 4, 2, 2, 3)])
+@pytest.mark.parametrize("causal,scale", [(True, None), (False, None), (True, 0.25)])
+def test_short_rows_are_rounded_once_with_their_prefix_too(d, H, Hkv, n, B, causal, scale):
+    """As without a prefix: the weights of rows of up to 32 tokens keep 2^-15."""
+    tails = [n + 7 * b % 50 for b in range(B)]
+    m = shared(720, tails, Hkv=Hkv, d=d, page=16, seed=d + B)
+    g = torch.Generator(device=DEV).manual_seed(B)
+    q = torch.randn(n * B, H, d, generator=g, device=DEV).bfloat16()
+    starts = i32(np.arange(B + 1) * n)
+    o = f64(m.cache.attention(0, q, starts, causal=causal, scale=scale, prefix=m.cache.common_prefix()))
+    x = f64(q)
+    for s in range(B):
+        keys, vals, rows = m.rows(0, s), m.rows(1, s), slice(s * n, s * n + n)
+        want, A = R.attention(x[rows], keys, vals, m.lens[s], causal, 0, scale)
+        err, tol = np.abs(o[rows] - want), few_tol(want, A, x[rows], keys, d, scale or d ** -0.5)
+        assert (err <= tol).all(), (s, (err / tol).max())
