@@ -46,8 +46,10 @@ class PagedCache:
     Beside them a cache keeps the workspace of its attention calls, as large as the calls
     so far have needed: at most 35 MB for single tokens, 104 MB (head_dim 64) or 136 MB (128)
     for any call, and up to a third more where it has grown; a call with a prefix takes
-    up to 26 or 52 MB more, or 8 (head_dim + 2) bytes for every token and head (rounded up to 128
-    a key head) where that is more.  The first call of a size may allocate."""
+    up to 26 (head_dim 64) or 52 MB (128) more, or 8 (head_dim + 2) bytes for every token and head
+    (those of a key head rounded up to 128) where that is more, and where calls with a prefix grow
+    past the sizes above, all that is kept may be four times what the largest of them takes.
+    The first call of a size may allocate."""
 
     def __init__(self, n_layers, n_kv_heads, head_dim, num_pages, max_seqs, max_len, page_size=16,
                  dtype=torch.bfloat16, device=None):
@@ -108,14 +110,15 @@ class PagedCache:
             self._ptr, 65536, 65536 * rows, self.n_kv_heads) for rows in (1, 32, 128))
 
     def _room(self, rows, total, heads, prefix):
-        """Workspace for attention calls of this size.  It grows by steps of four or more and, but
-        for calls with a prefix, never past the largest call's; what it was before stays, for the
-        graphs that use it."""
+        """Workspace for attention calls of this size.  It grows by steps of four or more up to the
+        largest call's without a prefix, from there (calls with one know no largest) by steps of
+        two or more; what it was before stays, for the graphs that use it."""
         f = (self._lib.blt_paged_attention_prefix_workspace_bytes if prefix
              else self._lib.blt_paged_attention_workspace_bytes)
         need = f(self._ptr, rows, total, heads)
         if need > self._ws_bytes:
-            size = max(need, min(4 * self._ws_bytes, self._ws_most))
+            size = max(need, min(4 * self._ws_bytes, self._ws_most) if need <= self._ws_most
+                       else 2 * self._ws_bytes)
             self._ws.append(self._workspace(size))
             self._wsp, self._ws_bytes = self._ws[-1].data_ptr(), size
         self._ws_for = (rows, total, heads, prefix)

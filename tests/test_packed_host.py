@@ -133,3 +133,29 @@ def test_host_tensors_are_refused():
         F.fused_packed_attention([1], q, q, s)
     with pytest.raises(TypeError):
         F.fused_sample(None, torch.zeros(2))
+
+
+@pytest.mark.parametrize("prefix", [False, True])
+@pytest.mark.parametrize("heads,kv_heads,dim,rows", [(32, 8, 128, 16), (12, 12, 64, 3), (8, 1, 128, 64)])
+def test_what_a_cache_keeps_for_its_calls_is_bounded(prefix, heads, kv_heads, dim, rows):
+    """Calls that grow token by token: few workspaces, at most four times the largest call's need in all
+    beside what calls without a prefix may take."""
+    d = desc(n_kv_heads=kv_heads, head_dim=dim, max_seqs=64, max_pages=4096, num_pages=1 << 16)
+    c = pkg.cache.PagedCache.__new__(pkg.cache.PagedCache)
+    sizes = []
+    c._lib, c._ptr, c.n_kv_heads = L, addr(d), kv_heads
+    c._workspace = lambda n: sizes.append(n) or torch.empty(n, dtype=torch.uint8, device="meta")
+    c._ws, c._wsp, c._ws_bytes, c._ws_for = [], None, 0, None
+    f = L.blt_paged_attention_workspace_bytes
+    c._ws_most = max(f(addr(d), 65536, 65536 * r, kv_heads) for r in (1, 32, 128))
+    need, most = L.blt_paged_attention_prefix_workspace_bytes if prefix else f, 0
+    for total in list(range(rows, 1500)) + list(range(1500, 8001, 7)):
+        c._room(rows, total, heads, prefix)
+        assert c._ws_bytes >= need(addr(d), rows, total, heads)
+        most = max(most, need(addr(d), rows, total, heads))
+        assert sum(sizes) <= 4 * most + 1.34 * c._ws_most, total
+    assert len(sizes) <= 10 and len(c._ws) == len(sizes)
+    # one large call alone takes what it needs
+    c._ws, c._ws_bytes, sizes[:] = [], 0, []
+    c._room(rows, 8000, heads, prefix)
+    assert sizes == [need(addr(d), rows, 8000, heads)]
