@@ -1052,13 +1052,15 @@ int run(const SArgs& g, hipStream_t s) {
 }  // namespace
 
 // Rows of one round of launches: where they are in parts, 8192 of these fill the chip four times, and
-// what they leave behind (41 KB each) stays below 340 MB.
-static int64_t rows_at_once(int64_t rows, int64_t parts) {
-  return parts ? std::min<int64_t>(rows, 8192 / parts) : rows;
+// what they leave behind (41 KB each) stays below 340 MB; else 2^31 work-items (a launch takes less than
+// 2^32), a wave a row or a block.
+static int64_t rows_at_once(int64_t rows, int vocab) {
+  const int64_t parts = parts_of(vocab);
+  return std::min<int64_t>(rows, parts ? 8192 / parts : vocab <= 1024 ? 1 << 25 : 1 << 21);
 }
 int64_t sample_workspace_bytes(int64_t rows, int vocab) {
   const int64_t parts = parts_of(vocab);
-  rows = rows_at_once(rows, parts);
+  rows = rows_at_once(rows, vocab);
   return parts ? rows * (parts * (12 * (int64_t)NB + sizeof(Entry) * NT + 16) + sizeof(Found)) : 0;
 }
 
@@ -1070,7 +1072,7 @@ int launch_sample(const SampleArgs& a, void* ws, hipStream_t s) {
   g.scale = 62 - l;
   g.parts = parts_of(a.vocab);
   if (a.rows > 0x7fffffff) return fail(BLT_ERR_SHAPE, "fused_sample: too many rows");
-  const int64_t each = rows_at_once(a.rows, g.parts), n = each * g.parts;
+  const int64_t each = rows_at_once(a.rows, a.vocab), n = each * g.parts;
   if (g.parts) {
     g.hm = (uint64_t*)ws;
     g.pmass = g.hm + n * NB;

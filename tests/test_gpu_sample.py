@@ -285,3 +285,17 @@ def test_refusals():
               lambda: F.fused_sample(x, u, out=[0])):
         with pytest.raises(TypeError):
             f()
+
+
+@pytest.mark.parametrize("V,R", [(2000, (1 << 22) + 5), (40, (1 << 26) + 9)])
+def test_more_rows_than_one_launch_holds(V, R):
+    """Many tokens from one distribution: a launch has at most 2^32 - 1 work-items."""
+    x, _ = logits_of(1, V, torch.float32, seed=7)
+    g = torch.Generator(device=DEV)
+    g.manual_seed(1)
+    u = torch.rand(R, generator=g, device=DEV)
+    got = F.fused_sample(x.expand(R, -1), u, top_k=30, top_p=0.9)
+    s = dict(k=30, p=0.9)
+    for rows in (slice(0, 50), slice(R // 2 - 25, R // 2 + 25), slice(R - 50, R)):
+        assert torch.equal(got[rows].cpu(), reference(x.expand(50, -1), u[rows], **s))
+    assert bool((got >= 0).all())
