@@ -69,7 +69,6 @@ __device__ inline bool kept(const Cut& c, uint32_t key, int i) {
 // ---- a row's rules ---------------------------------------------------------------------
 struct Rules {
   double a;     // log2(e) / temperature
-  float a32;
   double p;     // top_p; 1 or more: off
   uint64_t m;   // smallest weight kept
   int k;        // 0: off
@@ -87,7 +86,6 @@ __device__ inline Rules rules_of(const SArgs& g, int64_t row) {
   r.good = t >= 0. && t < (double)INFINITY && p > 0. && m >= 0. && m <= 1. && k >= 0 &&
            g.u[row] == g.u[row];
   r.a = t > 0. ? 1.4426950408889634074 / t : 1.;
-  r.a32 = (float)r.a;
   r.p = p;
   r.m = (uint64_t)ceil(ldexp(m, g.scale));
   r.k = t > 0. ? k : 1;  // (temperature 0: the first of the largest)
@@ -108,11 +106,13 @@ __device__ inline void fill(Powers& p) {  // (a barrier before their use)
 // The largest logit has 2^scale exactly, equal ones equal weights.
 __device__ inline uint64_t weight(float x, float top, const Rules& r, int scale, const Powers& pw) {
   if (x == top) return (uint64_t)1 << scale;
-  if (!((x - top) * r.a32 > -70.f)) return 0;  // (below 2^-70: scale <= 62)
+  // (in 64 bits here too: at temperatures near the ends of f32's range x - top or 1 / temperature passes
+  // it where the weight does not vanish)
+  const double y = ((double)x - (double)top) * r.a;
+  if (!(y > -70.)) return 0;  // (scale <= 62)
   constexpr double L = 0.693147180559945309417;
   constexpr double c2 = L * L / 2, c3 = c2 * L / 3, c4 = c3 * L / 4;
   constexpr double M = 1.5 * 70368744177664.;  // 2^46: the sum below is a multiple of 1 / 64
-  const double y = ((double)x - (double)top) * r.a;
   const double t = y + M, f = y - (t - M);
   const int k = (int)(uint32_t)__double_as_longlong(t);
   const double v = pw.of[k & 63] * fma(fma(fma(fma(c4, f, c3), f, c2), f, L), f, 1.);

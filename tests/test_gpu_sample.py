@@ -299,3 +299,32 @@ def test_more_rows_than_one_launch_holds(V, R):
     for rows in (slice(0, 50), slice(R // 2 - 25, R // 2 + 25), slice(R - 50, R)):
         assert torch.equal(got[rows].cpu(), reference(x.expand(50, -1), u[rows], **s))
     assert bool((got >= 0).all())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("V", [300, 2000, 20000])
+@pytest.mark.parametrize("t", [3e37, 1e38, 3e38, 1e39])
+def test_logits_further_apart_than_their_type_reaches(dtype, V, t):
+    """max - x passes the largest f32, the weight at that temperature does not vanish."""
+    g = torch.Generator(device=DEV)
+    g.manual_seed(V)
+    x = (6.6e38 * (torch.rand(6, V, generator=g, device=DEV, dtype=torch.float64) - 0.5)).to(TYPES[dtype])
+    assert bool((x.amax(1) - x.amin(1) == math.inf).all())
+    u = torch.rand(6, generator=g, device=DEV)
+    for s in (dict(t=t), dict(t=t, p=0.95), dict(t=t, k=V // 2), dict(t=t, k=V - 3, p=0.9, m=1e-3)):
+        assert torch.equal(F.fused_sample(x, u, **names(s)).cpu(), reference(x, u, **s)), s
+
+
+@pytest.mark.parametrize("dtype,step,temperatures", [("f32", 2.0 ** -149, (1e-44, 1e-43, 3e-42)),
+                                                     ("bf16", 2.0 ** -133, (1e-40, 1e-39, 2e-38))])
+@pytest.mark.parametrize("V", [300, 2000, 20000])
+def test_logits_closer_than_their_type_inverts(dtype, step, temperatures, V):
+    """Logits a few of the type's smallest steps apart, temperatures whose inverses pass the largest f32."""
+    g = torch.Generator(device=DEV)
+    g.manual_seed(V)
+    x = (step * torch.randint(-40, 40, (6, V), generator=g, device=DEV).double()).to(TYPES[dtype])
+    u = torch.rand(6, generator=g, device=DEV)
+    assert len(x.unique()) == 80
+    for t in temperatures:
+        for s in (dict(t=t), dict(t=t, p=0.95), dict(t=t, k=V // 2), dict(t=t, k=V - 3, p=0.9, m=1e-3)):
+            assert torch.equal(F.fused_sample(x, u, **names(s)).cpu(), reference(x, u, **s)), s
