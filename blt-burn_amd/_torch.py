@@ -1,6 +1,7 @@
 """Device-memory plumbing: torch CUDA tensors carry the buffers and streams
 handed to the C ABI (pointers, element counts, the current HIP stream)."""
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 from ._lib import BltError, check
 
@@ -41,6 +42,15 @@ def require_cuda(*tensors):
             raise TypeError("expected a torch.Tensor, got %r" % type(t))
         if not t.is_cuda:
             raise BltError("tensor must live on a GPU (got device %s)" % t.device)
+
+
+def no_tangents(what, *tensors):
+    """For the calls that autograd follows: forward-mode does not, and a tangent of an input would
+    be dropped without a word.  (One comparison where no dual_level is entered.)"""
+    if getattr(_forward_ad, "_current_level", 0) >= 0 and any(
+            isinstance(t, torch.Tensor) and _forward_ad.unpack_dual(t).tangent is not None
+            for t in tensors):
+        raise BltError("%s: forward-mode derivatives are not supported" % what)
 
 
 def contiguous(t):

@@ -12,7 +12,7 @@ import torch
 
 from . import _lib
 from ._lib import EPS_AFTER_SQRT, EPS_INSIDE_SQRT, BltError, check
-from ._torch import call_on, contiguous, require_cuda, stream_ptr
+from ._torch import call_on, contiguous, no_tangents, require_cuda, stream_ptr
 
 __all__ = ["fused_entropy", "fused_rms_norm", "fused_softmax", "fused_l2_norm",
            "fused_silu_gate", "fused_coherence", "fused_attention", "fused_sample",
@@ -322,7 +322,8 @@ def fused_packed_attention(q, k, v, starts, causal=True, window=0, scale=None, o
     f32 [tokens, heads] (-inf for none), which fused_packed_attention_backward takes.  Tokens at
     starts[-1] and behind get 0 in a new tensor and are left alone in `out` (lse -inf in both).  Scores and sums
     are f32 throughout; in bf16 the weights are rounded to bf16.  Autograd follows it for o
-    (once; `out` takes no inputs that need a gradient)."""
+    (once; `out` takes no inputs that need a gradient), forward-mode does not."""
+    no_tangents("fused_packed_attention", q, k, v)
     if torch.is_grad_enabled() and (getattr(q, "requires_grad", False)
                                     or getattr(k, "requires_grad", False)
                                     or getattr(v, "requires_grad", False)):
@@ -367,6 +368,7 @@ def fused_packed_attention_backward(grad_o, q, k, v, o, lse, starts, causal=True
     """(dq, dk, dv) of fused_packed_attention from its output's gradient, its o and lse, and its
     other arguments; tokens at starts[-1] and behind get 0.  Sums are f32, in bf16 the weights and
     (as two halves for dq) their gradients are rounded to bf16; the same bits in every run."""
+    no_tangents("fused_packed_attention_backward", grad_o, q, k, v, o, lse)
     q, qp, qs, qh = _packed_heads(q, "q")
     total, H, d = q.shape
     k, kp, ks, kh = _packed_heads(k, "k", q)
@@ -478,11 +480,12 @@ def fused_rotary(q, k, positions, plan, backward=False, out=None):
     dimension are read as they are, e.g. views into a packed QKV tensor.
     positions: int32 [seq] or [batch, seq].  backward=True applies the transposed
     rotation, which turns gradients of q', k' into those of q, k; autograd does so by
-    itself for inputs that need a gradient.  out: (q', k') to write, which may be q and k
+    itself for inputs that need a gradient (forward-mode does not).  out: (q', k') to write, which may be q and k
     themselves; other overlaps are not allowed, nor are inputs that need a gradient."""
     for t in (q, positions) if k is None else (q, k, positions):
         if not isinstance(t, torch.Tensor):
             raise TypeError("expected a torch.Tensor, got %r" % type(t))
+    no_tangents("fused_rotary", q, k)
     if not isinstance(plan, RotaryPlan):
         require_cuda(q, positions)
         raise TypeError("fused_rotary expects a RotaryPlan")

@@ -159,3 +159,22 @@ def test_what_a_cache_keeps_for_its_calls_is_bounded(prefix, heads, kv_heads, di
     c._ws, c._ws_bytes, sizes[:] = [], 0, []
     c._room(rows, 8000, heads, prefix)
     assert sizes == [need(addr(d), rows, 8000, heads)]
+
+
+def test_forward_mode_is_refused():
+    """A dual tensor needs no gradient, so its tangent would be dropped without a word."""
+    import torch.autograd.forward_ad as fw
+    q, s = torch.zeros(3, 2, 64), torch.tensor([0, 3], dtype=torch.int32)
+    pos = torch.zeros(3, dtype=torch.int32)
+    plan = F.RotaryPlan.__new__(F.RotaryPlan)
+    x, w = torch.zeros(1, 2, 3, 64), torch.ones(64)
+    with fw.dual_level():
+        d, dx = fw.make_dual(q, torch.ones_like(q)), fw.make_dual(x, torch.ones_like(x))
+        for f in (lambda: F.fused_packed_attention(d, q, q, s), lambda: F.fused_packed_attention(q, d, q, s),
+                  lambda: F.fused_packed_attention(q, q, d, s),
+                  lambda: F.fused_packed_attention_backward(d, q, q, q, q, q[..., 0], s),
+                  lambda: F.fused_rotary(dx, None, pos, plan), lambda: F.fused_rotary(x, dx, pos, plan)):
+            with pytest.raises(pkg.BltError, match="forward-mode"):
+                f()
+            with torch.no_grad(), pytest.raises(pkg.BltError, match="forward-mode"):
+                f()
