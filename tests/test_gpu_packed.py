@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 import torch
 
+import blt_burn_amd as pkg
 import packed_ref as R
 from blt_burn_amd import BltError, fused_ops as F
 
@@ -448,3 +449,46 @@ def test_lse_behind_the_last_sequence_with_out(dtype, d, H, K, lens, causal, win
     r = R.attention(q, k, v, st, u=U[t], **kw)
     near(lse, r, "lse")
     near(o[:n], {x: r[x][:n] for x in ("o", "tol_o")}, "o")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("T,H,K,d", [(100, 2, 2, 64), (70, 6, 2, 128), (9, 512, 512, 64)])
+@pytest.mark.parametrize("causal,window", [(True, 0), (True, 20), (False, 0)])
+def test_starts_that_do_not_ascend_write_nothing_beside_the_outputs(dtype, T, H, K, d, causal, window):
+    """Through the C entries, whose outputs and workspaces are slices of larger buffers here."""
+    L, t, edge = pkg.lib(), TYPES[dtype], 128
+    q, k, v, do = (x.contiguous() for x in made([T], 0, H, K, d, t))
+    code = 1 if t is torch.bfloat16 else 0
+
+    def inside(shape, kind=t, fill=7):
+        n = math.prod(shape)
+        whole = torch.full((n + 2 * edge,), fill, dtype=kind, device=DEV)
+        return whole, whole[edge:edge + n].view(shape)
+
+    def heads(x):
+        return x.data_ptr(), x.shape[1] * d, d
+
+    for st in ([0, 70, 30, T], [-5, 1000], [50, 20], [T, T, 0], [0, 2 ** 31 - 1], [0, -2 ** 31, 5, 2 ** 31 - 1],
+               [3] + [T - 1, 0] * 40):
+        s, B = i32(st), len(st) - 1
+        all_ = [inside((T, h, d)) for h in (H, H, K, K)] + [inside((T, H), torch.float32)]
+        o, dq, dk, dv, lse = (x[1] for x in all_)
+        stream = torch.cuda.current_stream().cuda_stream
+        for bytes_, call in (
+                (L.blt_packed_attention_workspace_bytes(B, T, H, K, code),
+                 lambda ws, n: L.blt_packed_attention(
+                     *heads(q), *heads(k), *heads(v), *heads(o), lse.data_ptr(), code, T, H, K, d, s.data_ptr(),
+                     B, causal, window, d ** -0.5, 1, ws, n, stream)),
+                (L.blt_packed_attention_backward_workspace_bytes(T, H, K, d, code),
+                 lambda ws, n: L.blt_packed_attention_backward(
+                     *heads(do), *heads(q), *heads(k), *heads(v), *heads(o), lse.data_ptr(), *heads(dq),
+                     *heads(dk), *heads(dv), code, T, H, K, d, s.data_ptr(), B, causal, window, d ** -0.5, ws, n,
+                     stream))):
+            room = inside((bytes_,), torch.uint8)
+            all_.append(room)
+            assert call(room[1].data_ptr(), bytes_) == 0
+        for whole, _ in all_:
+            assert bool((whole[:edge] == 7).all() and (whole[-edge:] == 7).all()), st
+        # (the tensors themselves are written whole)
+        for x in (dq, dk, dv):
+            assert not bool((x == 7).all())

@@ -492,3 +492,17 @@ def test_short_rows_are_rounded_once_with_their_prefix_too(d, H, Hkv, n, B, caus
         want, A = R.attention(x[rows], keys, vals, m.lens[s], causal, 0, scale)
         err, tol = np.abs(o[rows] - want), few_tol(want, A, x[rows], keys, d, scale or d ** -0.5)
         assert (err <= tol).all(), (s, (err / tol).max())
+
+
+# ---- f32 rows in tiles of 128 ------------------------------------------------------------------
+
+@pytest.mark.parametrize("ctx,tails,n", [
+    (160, [300, 250, 270, 260], [290, 250, 256, 260]),      # both launches in tiles of 128
+    (700, [1500, 40, 700], [500, 30, 600]),                 # own keys in several parts
+    (300, [16 + b % 40 for b in range(64)], [16] * 64),     # the prefix in tiles of 128, the tails of 32
+    (300, [16 + b % 9 for b in range(62)], [16] * 62)])     # and the prefix in two parts
+@pytest.mark.parametrize("causal", [True, False])
+def test_f32_in_tiles_of_128_rows(ctx, tails, n, causal):
+    m = shared(ctx, tails, Hkv=8, d=128, page=16, dtype=torch.float32, seed=len(n))
+    check(m, n, 32, causal=causal)
+    check(m, n, 32, causal=causal, prefix=i32([ctx // 2]), scale=0.2)
