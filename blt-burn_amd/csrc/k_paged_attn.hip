@@ -2066,7 +2066,10 @@ static int launch_one(const Launch& x, hipStream_t s) {
 }
 template <int D>
 static int launch_both(const Launch& pre, const Launch& own, int64_t total, hipStream_t s) {
-  if (pre.blocks + own.blocks > 0x7fffffff) return too_many();
+  constexpr int rows = 64 / (D / 4);
+  const int64_t joins = (total * own.p.G + rows - 1) / rows;
+  // (a launch takes less than 2^32 work-items; all are looked at before the first one)
+  if (std::max(pre.blocks + own.blocks, joins) > 0xffffff) return too_many();
   const unsigned first = (unsigned)pre.blocks;
   const dim3 grid(first + (unsigned)own.blocks);
   if (own.sh.form == FORM_FEW16)
@@ -2075,10 +2078,8 @@ static int launch_both(const Launch& pre, const Launch& own, int64_t total, hipS
     hipLaunchKernelGGL((paged_attn_both_kernel<D, 2>), grid, dim3(256), 0, s, pre.p, own.p, first);
   else
     hipLaunchKernelGGL((paged_attn_both_kernel<D, 0>), grid, dim3(256), 0, s, pre.p, own.p, first);
-  constexpr int rows = 64 / (D / 4);
-  hipLaunchKernelGGL((paged_attn_join_kernel<D>),
-                     dim3((unsigned)((total * own.p.G + rows - 1) / rows), (unsigned)own.p.Hkv),
-                     dim3(256), 0, s, own.p);
+  hipLaunchKernelGGL((paged_attn_join_kernel<D>), dim3((unsigned)joins, (unsigned)own.p.Hkv), dim3(256), 0, s,
+                     own.p);
   BLT_LAUNCH_CHECK("paged_attn_both_kernel");
   return 0;
 }

@@ -364,7 +364,8 @@ int blt_cache_common_prefix(const blt_paged_cache* cache, const int32_t* seqs, i
                             int32_t* tokens, blt_stream_t stream);
 /* blt_paged_attention without a window for sequences that share their first prefix[0] tokens (int32
  * [1], device, from blt_cache_common_prefix of a list that holds these sequences): the shared
- * keys are read once for all rows (two launches).  What is no whole page, and what does not lie
+ * keys are read once for all rows (two launches; tokens times the heads of a key head below 2^26, or 2^25
+ * with head_dim 128).  What is no whole page, and what does not lie
  * before every row's new tokens, is not taken as shared, and nothing is where the last page of
  * that is not the same in all sequences with tokens.  So any number is safe for page tables in
  * which a page that two sequences share has the same pages before it in both, as blt_cache_fork

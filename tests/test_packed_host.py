@@ -178,3 +178,13 @@ def test_forward_mode_is_refused():
                 f()
             with torch.no_grad(), pytest.raises(pkg.BltError, match="forward-mode"):
                 f()
+
+
+@pytest.mark.parametrize("dim,total", [(128, 1 << 25), (64, 1 << 26)])
+def test_a_prefix_call_that_no_launch_holds_is_refused_whole(dim, total):
+    """Its second launch would have 2^32 work-items: nothing of the first may run then."""
+    d = desc(n_kv_heads=1, head_dim=dim, max_seqs=65536, max_pages=4096, num_pages=1 << 20)
+    call = lambda n: L.blt_paged_attention_prefix(addr(d), 0, P, dim, dim, P, dim, dim, 1, P, None, 4, n, 1, 0.125,
+                                                  P, P, 1 << 60, None)
+    assert call(total) < 0 and "too many" in pkg.last_error(), pkg.last_error()
+    assert call(2 ** 31 - 1) < 0 and "too many" in pkg.last_error()
