@@ -320,8 +320,10 @@ def fused_packed_attention(q, k, v, starts, causal=True, window=0, scale=None, o
 
     Returns o [tokens, heads, head_dim]; with return_lse also the logarithms of the softmax's sums,
     f32 [tokens, heads] (-inf for none), which fused_packed_attention_backward takes.  Tokens at
-    starts[-1] and behind get 0 in a new tensor and are left alone in `out` (lse -inf in both).  Scores and sums
-    are f32 throughout; in bf16 the weights are rounded to bf16.  Autograd follows it for o
+    starts[-1] and behind get 0 in a new tensor and are left alone in `out` (lse -inf in both); `out` may be
+    q, but must not overlap k or v.  Scores and sums are f32 throughout; in bf16 the weights are rounded to
+    bf16, and the sums take the rounded ones, or with return_lse or a gradient those before it, by which the
+    gradient's weights go: o's last bits may differ between the two.  Autograd follows it for o
     (once; `out` takes no inputs that need a gradient), forward-mode does not."""
     no_tangents("fused_packed_attention", q, k, v)
     if torch.is_grad_enabled() and (getattr(q, "requires_grad", False)

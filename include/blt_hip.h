@@ -163,7 +163,9 @@ int blt_fused_sample(const void* logits, int64_t row_stride, int32_t dtype, int6
  *   scale:  of the scores, 1e-30 .. 1e30
  *   lse:    (may be NULL) f32 [total, Hq], log of the sum of e^score, -inf where it is 0
  *   tail:   tokens at starts[B] and behind: 0 = o left alone, 1 = o 0; lse is -inf there in both
- * Scores, softmax and sums in f32; in bf16 the weights are rounded to bf16.  A key whose
+ * Scores, softmax and sums in f32; in bf16 the weights are rounded to bf16, and the sums take the
+ * rounded ones, or with lse those before it (so o's last bits may differ).  o may be q, but must not
+ * overlap k or v.  A key whose
  * score is -inf weighs nothing; infinite and NaN values come through where they are seen.
  * workspace: blt_packed_attention_workspace_bytes (0 for small calls and one sequence), 16-byte
  * aligned, no initialisation; calls that share one must be stream-ordered. */

@@ -492,3 +492,14 @@ def test_starts_that_do_not_ascend_write_nothing_beside_the_outputs(dtype, T, H,
         # (the tensors themselves are written whole)
         for x in (dq, dk, dv):
             assert not bool((x == 7).all())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("d,H,K", [(64, 4, 2), (128, 8, 1)])
+def test_out_may_be_q(dtype, d, H, K):
+    lens = [300, 5, 0, 77]
+    q, k, v, _ = made(lens, 9, H, K, d, TYPES[dtype])
+    s, kept = i32(starts_of(lens)), q[sum(lens):].clone()
+    want = F.fused_packed_attention(q, k, v, s, window=100)
+    assert F.fused_packed_attention(q, k, v, s, window=100, out=q) is q
+    assert torch.equal(q[:sum(lens)], want[:sum(lens)]) and torch.equal(q[sum(lens):], kept)
