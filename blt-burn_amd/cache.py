@@ -305,8 +305,9 @@ class PagedCache:
         prefix: what common_prefix said of a list that holds these sequences, now or in an earlier
         step (where one of those with tokens does not have it, having been empty then, or cut or
         replaced since, the call goes without).  The keys that they share are then read once for
-        all rows, which pays where several rows have a long prefix and few tokens each (16 rows of up to 6 tokens over 30001 keys, 32 / 8 heads of 128,
-        73 us for 270; 4 of up to 200 over 16000 277 for 258); the outputs are those without it,
+        all rows, which pays where several rows have a long prefix and few tokens each (16 rows of
+        up to 6 tokens over 30001 keys, 32 / 8 heads of 128, 84 us for 262; 4 of up to 200 over
+        16000 243 for 226, in f32 4 of up to 400 over 700 342 for 238); the outputs are those without it,
         up to their rounding.  (It is not used with a window, whose rows do not see all of it.)"""
         layer = self._layer(layer)
         q, qp, total, H, qs, qh = self._tokens(q, "q")

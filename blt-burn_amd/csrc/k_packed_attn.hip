@@ -499,7 +499,9 @@ __global__ __launch_bounds__(256, 2) void packed_attn_kernel(PArgs p) {
 // Both products on the f32 matrix cores, one block = 32 rows, its four waves take every
 // fourth 32-key tile with operands straight from global memory, and meet once at the end.
 // Bound by the loads in front of the products, with two waves a SIMD to cover them: five sequences of up to
-// 1501, 12 heads of 64, 142 us, 79 TFLOP/s (an f32 library product: 136), matrix cores 53 % busy.
+// 1501, 12 heads of 64, 142 us, 79 TFLOP/s (an f32 library product: 136), matrix cores 53 % busy.  d = 128, one
+// wave a SIMD: sequences of 2000 and 1441, 8 / 1 heads, 175 us, 71 TFLOP/s; of 1000, 721, 1 and 303, 32 / 8 heads,
+// 209, 63.
 template <int ND>
 __global__ __launch_bounds__(256) void packed_attn_f32_kernel(PArgs p) {
   constexpr int D = 32 * ND, NW = 4, NC = 4 * ND, OP = D + 4, BKV = 32;
@@ -1242,7 +1244,8 @@ __global__ __launch_bounds__(64 * KW * RW, D == 64 ? 3 : 2) void packed_dkdv_ker
 // f32, as packed_attn_f32_kernel: a block has 32 rows (dq) or 32 keys (dk, dv) in registers, its four
 // waves take every fourth tile of 32 of the others from global memory and add up at the end.  Bound by
 // those loads: 12 heads of 64, five sequences of up to 1501, dq 223 us, 76 TFLOP/s, dk and dv 370, 61 (one
-// wave a SIMD 440, blocks of eight waves 422); 12 / 4 heads, 1000 + 780 + 439 tokens, 70 and 139.
+// wave a SIMD 440, blocks of eight waves 422); 12 / 4 heads, 1000 + 780 + 439 tokens, 70 and 139; heads of 128,
+// 2000 + 1441 tokens, 8 / 1 heads, 314 and 537 with the join, 1000 + 721 + 1 + 303, 32 / 8 heads, 370 and 452.
 // Sum of the waves' [D][32] results, scaled, into rows out(i).
 template <int ND, typename F>
 __device__ inline void add_waves(float* so, const f32x16_t (&acc)[ND], float scale, F out) {

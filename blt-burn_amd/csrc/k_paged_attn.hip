@@ -1340,13 +1340,14 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(KArgs p) {
 // ---- bf16, a prefix and rows of their own beside it -------------------------------------
 // PREFIX and what the sequences have of their own in one launch, side by side, since neither fills
 // the chip for long; the first `first` blocks (a multiple of 8) are PREFIX's, the others in the form for
-// 16 NR rows, of which only two waves stay, or (NR = 0) in that for 128.  With the join, against PREFIX
-// and TAILS behind each other: 48 single tokens over 8192 shared and up to 200 own keys, 12 heads, 25.0 and 28.5 us (PREFIX alone 13.4, 25 MB of keys and values:
-// dependent steps); 16 drafts of up to 6 over 30001 and up to 900, 32 / 8 heads of 128, 73 and 81 (46 alone,
-// 123 MB: 2.6 TB/s, and 27 GFLOP), of up to 9 92 and 123; 64 single tokens over 4000 and
-// 300, 8 / 1 heads of 128, 20.6 and 32.4, where without a prefix they take 22.2.  Chunks: 9 of up to 38 over
-// 3250 and 294, 8 / 1 heads of 128, 30 and 125 (29 without), 18 of up to 16 over 20679 43 and 142 (82); 4 of
-// up to 200 over 16000, 32 / 8 heads, 277 and 308 (258).
+// 16 NR rows, of which only two waves stay, or (NR = 0) in that for 128.  A layer with its join (without a
+// prefix in brackets): 48 single tokens over 8192 shared and up to 200 own keys, 12 heads, 26 us (114),
+// dependent steps over 25 MB of keys and values; 16 drafts of up to 6 over 30001 and up to 900, 32 / 8 heads of
+// 128, 84 (262), 123 MB and 41 GFLOP with the weights' second halves, of up to 9 103 (320); 64 single tokens
+// over 4000 and 300, 8 / 1 heads of 128, 22 (21).  Chunks: 9 of up to 38 over 3250 and 294, 8 / 1 heads of 128,
+// 29 (28), 18 of up to 16 over 20679 42 (78); 4 of up to 200 over 16000, 32 / 8 heads, 243 (226).
+// (PREFIX and TAILS behind each other, both with rounded weights, against this form: 28.5 and 25.0 us for the
+// first of these, 81 and 73, 123 and 92, 32 and 21; chunks 125 and 30, 142 and 43, 308 and 277.)
 template <int D, int NR>
 __global__ __launch_bounds__(256, 2) void paged_attn_both_kernel(KArgs pre, KArgs own,
                                                                  unsigned first) {
