@@ -473,6 +473,35 @@ def test_a_sequence_filled_after_the_prefix_was_taken(dtype, B, H, Hkv, refilled
     check(m, [1] * B, H, prefix=prefix, seqs=ids)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("B", [4, 40])
+def test_a_sequence_loses_and_regains_the_prefix_between_replays(dtype, B):
+    ctx = 320
+    m = Made([ctx + 5 + b % 30 for b in range(B)], Hkv=2, d=64, page=16, dtype=TYPES[dtype], seed=B)
+    own = m.table[1].copy()
+    m.table[:B, :ctx // 16] = m.table[0, :ctx // 16]
+    tables = [i32(m.table)]
+    m.table[1] = own
+    tables.append(i32(m.table))
+    c, s, prefix = m.cache, i32(range(B + 1)), i32([ctx])
+    q = torch.randn(B, 4, 64, device=DEV).to(TYPES[dtype])
+    c.page_table.copy_(tables[0])
+    run = lambda: c.attention(0, q, s, prefix=prefix)
+    run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = run()
+    for n in range(5):
+        q.normal_()
+        c.page_table.copy_(tables[n % 2])
+        fresh, plain = run(), c.attention(0, q, s)
+        torch.cuda.synchronize()
+        graph.replay()
+        assert torch.equal(held, fresh)
+        # (both are off by their outputs' rounding, 2^-8 at most, and less by their weights')
+        assert bool(((held.float() - plain.float()).abs() <= 2 ** -6 * plain.float().abs().amax()).all())
+
+
 # ---- accuracy ------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("d,H,Hkv,n,B", [(64, 4, 4, 1, 40), (64, 6, 2, 5, 30), (64, 8, 1, 4, 9), (128, 4, 4, 1, 48),
